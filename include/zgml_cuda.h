@@ -88,7 +88,13 @@ typedef enum ZgOpTag {
     ZG_OP_RG_LRU = 36,
     /* Stacks with several residual streams (csrc/streamops.cu): the step that closes a sublayer over all of them and opens the next. */
     ZG_OP_STREAM_STEP = 37,
-    ZG_OP_END = 38
+    /* A step of many requests at once (csrc/batchops.cu, csrc/shared_attention.cu): the rows' places in the caches, attention over a prefix that all
+     * share, low-rank adapters per request, and rules on logits per request. */
+    ZG_OP_BATCH_APPEND = 38,
+    ZG_OP_SHARED_ATTENTION = 39,
+    ZG_OP_ADAPTER_LINEAR = 40,
+    ZG_OP_LOGIT_RULES = 41,
+    ZG_OP_END = 42
 } ZgOpTag;
 
 /* Parameter pack of the sequence-model ops.  buf[] are program buffer indices (ZG_NO_BUF: absent), off[] element offsets,
@@ -304,7 +310,42 @@ typedef enum ZgOpTag {
  *                   buf 0 new streams [s, T, D] (without a close: buf 5 once more) 1 old streams 2 y 3 weights of the close 4 weights of the open 5 h [T, max(1, n6), D] 6 state 7 ctl
  *                   off 0 out 1 mix [s, s] (from, to) 2 ls 3 in 4 norm 5 mu [n6, D]
  *                   n 0 T 1 D 2 s 3 distance of the old streams (0: all equal, one [T, D]) 4 wdt 5 norm kind 6 shifts 7 ls given
- *                   f 0 multiplier 1 gain of h */
+ *                   f 0 multiplier 1 gain of h
+ *
+ * Steps of many requests.  `B` rows, each a token of some request; what tells them apart lies in a TABLE (int32 words inside an f32 buffer, rewritten by the
+ * host before every execution, as the control buffer is): [0] live rows (the rows behind them are left as they are), [1] length P of the prefix that all rows
+ * share, [2] its slot; from word ZG_BATCH_ROWS on four words a row: {slot, length, adapter, 0}.  `length` counts the positions of the row's own sequence
+ * behind the prefix that it sees, its own included: its position is P + length - 1 and its row in the slot's part of a cache length - 1 (no ring: a sequence ends
+ * at the cache's R rows).  A row with a negative slot is idle and left as it is.  A row with a word out of range (slot, length, adapter, prefix) gets NaN
+ * where it would have a result, and no cache row; nothing outside the buffers is touched.
+ *
+ * BATCH_APPEND      the rows join their caches (external [slots, R, width]): cache[slot, length - 1, off 1 + j] = src[row, off 0 + j], j < n1.  The first n5 heads
+ *                   of n6 values among them are turned by the row's rotary position on n8 values from n7 on (layout n9 and frequencies as ROTARY takes
+ *                   them; angles in 64 bits), the rest is copied.  n10 query heads of n6 values (column off 2 of the source) are turned the
+ *                   same way into buf 4.  A row of length 0 appends nothing; of rows that name the same place the last one stays.
+ *                   buf 0 cache 1 src 2 table 3 frequency table 4 turned query heads | off 0 src column 1 cache column 2 query column 3 column in buf 4 4 table offset
+ *                   n 0 B 1 columns 2 src row stride 3 width 4 R 5 key heads 6 head size 7 first turned value 8 turned values 9 layout 10 query heads
+ *                   11 row stride of buf 4 | f 0 base
+ * SHARED_ATTENTION  softmax attention of each row over the first P rows of the prefix and the first `length` rows of its slot, one softmax over both.  Query head h
+ *                   reads key head h / (H / G) and value head h / (H / G); value caches may be the key caches.  Prefix buffers (external [prefix slots, n11, width])
+ *                   may be absent (P is then 0).  Score cap f1 and sinks as CACHED_ATTENTION has them.  A row that sees no key gets zeros.
+ *                   buf 0 dst [B, H * dv] 1 q 2 key cache 3 value cache 4 prefix keys 5 prefix values 6 table 7 sinks
+ *                   off 0 q column 1 key column 2 value column 3 prefix key column 4 prefix value column 5 sinks 6 dst column
+ *                   n 0 B 1 H 2 G 3 dk 4 dv 5 q row stride 6 key row width 7 value row width 8 R 9 prefix key row width 10 prefix value row width
+ *                   11 prefix rows 12 dst row stride 13 wdt of the sinks | f 0 score scale 1 score cap
+ * ADAPTER_LINEAR    dst[r] = base[r] + s_a B_a (A_a src[r]), a the row's adapter (negative: none, dst[r] = base[r]): low-rank adapters of many requests beside the LINEAR
+ *                   that wrote `base` (which may be dst itself).  A [adapters, rank, K] and B [adapters, N, rank] are weights, s_a an f32 number per adapter (absent: 1).
+ *                   buf 0 dst 1 src 2 weights 3 scales 4 table 5 base | off 0 A 1 B 2 src 3 dst 4 scales 5 base
+ *                   n 0 B 1 N 2 K 3 rank 4 adapters 5 src row stride 6 dst row stride 7 wdt 8 base row stride
+ * LOGIT_RULES       what a request asks of its next token: a logit z of a token in the row's history becomes z / repetition (z > 0) or z * repetition; then
+ *                   z - presence - frequency * c where the history names the token c > 0 times from word `first` on; then the biases of the token are added;
+ *                   then tokens whose bit in the row's mask is clear get -inf.  May run in place.  The table of this op has ZG_RULE_WORDS words a row:
+ *                   {history slot, history length, first, mask row (negative: none), first bias entry, bias entries, repetition, presence, frequency (f32 bits), 0, 0, 0},
+ *                   [0] live rows as above.  Tokens outside the vocabulary are passed over; entries of one token add up in order.
+ *                   buf 0 dst 1 src 2 table 3 history (int32 [slots, n4]) 4 biases ({int32 token, f32 bias}) 5 masks (bit t % 32 of word t / 32, rows of ceil(V / 32) words)
+ *                   off 0 dst 1 src | n 0 B 1 V 2 src row stride 3 dst row stride 4 history rows */
+#define ZG_BATCH_ROWS 8
+#define ZG_RULE_WORDS 12
 #define ZG_NO_BUF 0xFFFFFFFFu
 #define ZG_W_F32 0
 #define ZG_W_BF16 1
@@ -651,6 +692,9 @@ size_t zg_cuda_trace_read(ZgCudaCtx* ctx, unsigned long long* host, size_t max_r
 /* f32 slots the scratch operand of a sequence-model op must have (MOE_FFN buf[4]: per-pair activations, or the sorted
  * rows, per-expert tiles and partial products of the grouped tensor-core form); 0 for ops without one. */
 size_t zg_cuda_seq_scratch_elems(const ZgOp* op);
+/* The static checks that zg_cuda_compile makes of a sequence-model op, without a device: 0 where a program with buffers of these sizes (f32 slots) may
+ * hold the op, -1 (and the error string) otherwise. */
+int zg_cuda_seq_check(const ZgOp* op, const size_t* buffer_sizes, size_t n_buffers);
 /* f32 slots per state slot of a sequence-model op that lays out its own state (SSM_SCAN, from H, N and P); 0 otherwise. */
 size_t zg_cuda_seq_state_elems(const ZgOp* op);
 

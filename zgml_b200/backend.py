@@ -207,6 +207,14 @@ class DeviceOp:
         return o
 
     @staticmethod
+    def _words(*values):
+        """Sizes and offsets as the 32-bit words of an op; what does not fit them is refused instead of cut."""
+        for v in values:
+            if not 0 <= int(v) < 1 << 32:
+                raise ValueError(f"a size or offset of {v} does not fit an op's 32-bit words")
+        return [int(v) for v in values]
+
+    @staticmethod
     def embed(dst, ctl, table, table_off, T, D, scale, wdt, positions_off=None, bigram=None, dyt_off=None):
         """Rows of the table times `scale`; with `positions_off` a learned position row of the same arena is added, unscaled.
         `bigram` = (offset, buckets, mul_prev, mul_cur): a row of that table (buckets + 1 rows in the same arena) is added, unscaled, at
@@ -432,6 +440,41 @@ class DeviceOp:
                                                   state if shifts else None, ctl if shifts else None], [out_off, mix_off, ls_off or 0, in_off, norm_off, mu_off],
                              [T, D, streams, src_stride, wdt, {"dyt": abi.NORM_DYNAMIC_TANH, "none": abi.NORM_NONE}[kind], shifts, int(ls_off is not None)], [mult, gain])
 
+    # ── steps of many requests: rows told apart by a table (host/batch.py) ──
+    @staticmethod
+    def batch_append(cache, src, table, src_col, cache_col, B, cols, src_rs, width, rows, key_heads=0, head_dim=0, turn_at=0, rot=0, rot_base=0.0, rot_layout="pairs",
+                     freqs=None, freqs_off=0, q_heads=0, q_col=0, turned=None, turned_col=0, turned_rs=0):
+        """`cols` columns of every row join the cache of the row's slot.  The first `key_heads` heads of `head_dim` values among them are turned by the row's rotary
+        position on `rot` values from `turn_at` on (frequencies from `rot_base`, or from the f32 table `freqs`); `q_heads` query heads at column `q_col`
+        are turned the same way into `turned`."""
+        return DeviceOp._seq(abi.OP_BATCH_APPEND, [cache, src, table, freqs if rot else None, turned if q_heads else None], DeviceOp._words(src_col, cache_col, q_col, turned_col, freqs_off),
+                             DeviceOp._words(B, cols, src_rs, width, rows, key_heads, head_dim, turn_at, rot) + [{"pairs": 0, "halves": 1}[rot_layout]] +
+                             DeviceOp._words(q_heads, turned_rs or turned_col + q_heads * head_dim), [rot_base])
+
+    @staticmethod
+    def shared_attention(dst, q, k_cache, v_cache, k_prefix, v_prefix, table, q_col, k_col, v_col, k_prefix_col, v_prefix_col, B, H, G, dk, dv, q_rs, k_width, v_width, rows,
+                         k_prefix_width, v_prefix_width, prefix_rows, scale, softcap=0.0, sink=None, sink_off=0, sink_wdt=0, dst_rs=0, dst_col=0):
+        """Attention of every row over a prefix that all rows share and over what its own slot holds, one softmax over both.  Without a prefix (both buffers None)
+        prefix_rows is 0.  `softcap` and `sink` as cached_attention has them."""
+        return DeviceOp._seq(abi.OP_SHARED_ATTENTION, [dst, q, k_cache, v_cache, k_prefix, v_prefix, table, sink],
+                             DeviceOp._words(q_col, k_col, v_col, k_prefix_col, v_prefix_col, sink_off, dst_col),
+                             DeviceOp._words(B, H, G, dk, dv, q_rs, k_width, v_width, rows, k_prefix_width, v_prefix_width, prefix_rows, dst_rs or dst_col + H * dv, sink_wdt), [scale, softcap])
+
+    @staticmethod
+    def adapter_linear(dst, src, w, a_off, b_off, table, B, N, K, rank, adapters, wdt, base=None, base_off=0, base_rs=0, scales=None, scales_off=0, src_off=0, src_rs=0, dst_off=0, dst_rs=0):
+        """dst = base + scale * B (A src) with the row's own adapter: A [adapters, rank, K] and B [adapters, N, rank] in arena `w`.  `base` None: dst itself, as the
+        LINEAR before left it."""
+        if base is None:
+            base, base_off, base_rs = dst, dst_off, dst_rs
+        return DeviceOp._seq(abi.OP_ADAPTER_LINEAR, [dst, src, w, scales, table, base], DeviceOp._words(a_off, b_off, src_off, dst_off, scales_off, base_off),
+                             DeviceOp._words(B, N, K, rank, adapters, src_rs or K, dst_rs or N, wdt, base_rs or N))
+
+    @staticmethod
+    def logit_rules(dst, src, table, B, V, history=None, history_rows=0, bias=None, masks=None, src_off=0, src_rs=0, dst_off=0, dst_rs=0):
+        """Penalties for tokens of the row's history, biases and a grammar's mask on rows of logits (dst may be src)."""
+        return DeviceOp._seq(abi.OP_LOGIT_RULES, [dst, src, table, history, bias, masks], DeviceOp._words(dst_off, src_off),
+                             DeviceOp._words(B, V, src_rs or V, dst_rs or V, history_rows if history is not None else 0))
+
 
 @dataclass
 class ProgramIO:  # reference src/backend.zig:252-257 (offset/size in bytes)
@@ -496,6 +539,12 @@ def seq_state_elems(op) -> int:
 def seq_scratch_elems(op) -> int:
     """f32 slots the scratch operand of a sequence-model op needs (zg_cuda_seq_scratch_elems)."""
     return int(load_library().zg_cuda_seq_scratch_elems(C.byref(op)))
+
+
+def seq_check(op, buffer_sizes: Sequence[int]) -> Optional[str]:
+    """Why no program with buffers of these sizes (f32 slots) may hold a sequence-model op; None where one may (zg_cuda_seq_check, needs no device)."""
+    sizes = (C.c_size_t * max(len(buffer_sizes), 1))(*[int(n) for n in buffer_sizes])
+    return None if load_library().zg_cuda_seq_check(C.byref(op), sizes, len(buffer_sizes)) == 0 else last_error()
 
 
 class DeviceBuffer:

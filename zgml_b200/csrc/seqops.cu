@@ -2372,6 +2372,7 @@ uint32_t zg_delta_row_slices(uint32_t dim) {
 
 // Static checks of a sequence op against the program's buffer sizes (f32 slots): shapes, strides and every extent.
 bool zg_seq_op_valid(const ZgOp& op, const size_t* elems, size_t n_bufs, char* why, size_t why_n) {
+    if (op.tag >= ZG_OP_BATCH_APPEND) return zg_batch_op_valid(op, elems, n_bufs, why, why_n);
     if (op.tag >= ZG_OP_STREAM_STEP) return zg_stream_op_valid(op, elems, n_bufs, why, why_n);
     if (op.tag >= ZG_OP_SSM_SCAN) return zg_rec_op_valid(op, elems, n_bufs, why, why_n);
     if (op.tag >= ZG_OP_TOKEN_SHIFT) return zg_mix_op_valid(op, elems, n_bufs, why, why_n);
@@ -2486,6 +2487,16 @@ bool zg_seq_op_valid(const ZgOp& op, const size_t* elems, size_t n_bufs, char* w
     }
 }
 
+extern "C" __attribute__((visibility("default"))) int zg_cuda_seq_check(const ZgOp* op, const size_t* buffer_sizes, size_t n_buffers) {
+    if (!op || (!buffer_sizes && n_buffers) || !zg_is_seq_op(op->tag)) { zg_set_error("seq_check: not a sequence op, or no buffers"); return -1; }
+    for (int i = 0; i < 8; i++)
+        if (i == 0 || op->u.seq.buf[i] != ZG_NO_BUF)
+            if (op->u.seq.buf[i] >= n_buffers) { zg_set_error("seq_check: operand %d names buffer %u of %zu", i, op->u.seq.buf[i], n_buffers); return -1; }
+    char why[96];
+    if (!zg_seq_op_valid(*op, buffer_sizes, n_buffers, why, sizeof(why))) { zg_set_error("%s", why); return -1; }
+    return 0;
+}
+
 // which of buf[0..8) an op writes (bit i); everything else it names is read
 uint32_t zg_seq_op_writes(uint32_t tag) {
     switch (tag) {
@@ -2495,7 +2506,7 @@ uint32_t zg_seq_op_writes(uint32_t tag) {
         case ZG_OP_DELTA_RULE: return 1u | (1u << 6);
         case ZG_OP_MOE_FFN: return 1u | (1u << 4);
         case ZG_OP_STREAM_STEP: return 1u | (1u << 5) | (1u << 6);   // streams, the next sublayer's input, a carried row
-        default: return tag >= ZG_OP_SSM_SCAN ? zg_rec_op_writes(tag) : (tag >= ZG_OP_TOKEN_SHIFT ? zg_mix_op_writes(tag) : 1u);
+        default: return tag >= ZG_OP_BATCH_APPEND ? zg_batch_op_writes(tag) : tag >= ZG_OP_SSM_SCAN ? zg_rec_op_writes(tag) : (tag >= ZG_OP_TOKEN_SHIFT ? zg_mix_op_writes(tag) : 1u);
     }
 }
 
@@ -2514,6 +2525,7 @@ static bool linear_split(const ZgSeqOp& s, float* const* bufs) {     // f32 weig
 }
 unsigned int zg_seq_timeouts() { return tc_timeouts(); }
 size_t zg_seq_op_scratch_elems(const ZgOp& op, float* const* bufs, bool least) {
+    if (op.tag >= ZG_OP_BATCH_APPEND) return zg_batch_op_scratch_elems(op);
     if (op.tag >= ZG_OP_STREAM_STEP) return 0;
     if (op.tag >= ZG_OP_SSM_SCAN) return zg_rec_op_scratch_elems(op);
     if (op.tag >= ZG_OP_TOKEN_SHIFT) return zg_mix_op_scratch_elems(op);
@@ -2557,7 +2569,7 @@ static bool launch_linear_ring(float* dst, const float* src, const WT* W, const 
 #undef ZG_RING
     return true;
 }
-bool zg_launch_seq_op(ZgCudaCtx* ctx, const ZgOp& op, float* const* bufs, float* scratch, size_t scratch_elems, cudaStream_t st, bool ahead) {
+bool zg_launch_seq_op(ZgCudaCtx* ctx, const ZgOp& op, float* const* bufs, const size_t* elems, float* scratch, size_t scratch_elems, cudaStream_t st, bool ahead) {
     (void)ctx;
     const ZgSeqOp& s = op.u.seq;
     switch (op.tag) {
@@ -2835,6 +2847,7 @@ bool zg_launch_seq_op(ZgCudaCtx* ctx, const ZgOp& op, float* const* bufs, float*
             return true;
         }
         default:
+            if (op.tag >= ZG_OP_BATCH_APPEND) return zg_launch_batch_op(op, bufs, elems, scratch, st);
             if (op.tag >= ZG_OP_STREAM_STEP) return zg_launch_stream_op(op, bufs, st, ahead);
             return op.tag >= ZG_OP_SSM_SCAN ? zg_launch_rec_op(op, bufs, scratch, st) : zg_launch_mix_op(op, bufs, scratch, st, ahead);
     }

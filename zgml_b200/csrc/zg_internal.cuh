@@ -461,7 +461,8 @@ unsigned int zg_seq_timeouts();       // waits that gave up (LINEAR of few rows,
 size_t zg_seq_op_scratch_elems(const ZgOp& op, float* const* bufs, bool least = false);
 // ahead: nothing writes the op's weights (CACHED_ATTENTION: the cache's rows of earlier positions) while the program runs, so that they may be read before the
 // launch's predecessor has completed
-bool zg_launch_seq_op(ZgCudaCtx* ctx, const ZgOp& op, float* const* bufs, float* scratch, size_t scratch_elems, cudaStream_t st, bool ahead);
+// elems: the buffers' sizes in f32 slots
+bool zg_launch_seq_op(ZgCudaCtx* ctx, const ZgOp& op, float* const* bufs, const size_t* elems, float* scratch, size_t scratch_elems, cudaStream_t st, bool ahead);
 // dense_gemm.cu : bf16 x bf16 -> f32 prefill matmul on tcgen05 (TMA-fed, TMEM accumulator)
 bool zg_dense_gemm_usable(const void* w_bf16, uint32_t M, uint32_t N, uint32_t K);
 size_t zg_dense_gemm_scratch_elems(uint32_t M, uint32_t K);
@@ -500,3 +501,11 @@ bool zg_dense_gemm_batched_launch(const void* w_bf16, const float* src, float* d
 // streamops.cu : ZG_OP_STREAM_STEP
 bool zg_stream_op_valid(const ZgOp& op, const size_t* elems, size_t n_bufs, char* why, size_t why_n);
 bool zg_launch_stream_op(const ZgOp& op, float* const* bufs, cudaStream_t st, bool const_weights);
+// batchops.cu : ZG_OP_BATCH_APPEND .. ZG_OP_LOGIT_RULES, reached through the functions above; shared_attention.cu : ZG_OP_SHARED_ATTENTION
+bool zg_batch_op_valid(const ZgOp& op, const size_t* elems, size_t n_bufs, char* why, size_t why_n);
+uint32_t zg_batch_op_writes(uint32_t tag);
+size_t zg_batch_op_scratch_elems(const ZgOp& op);
+bool zg_launch_batch_op(const ZgOp& op, float* const* bufs, const size_t* elems, float* scratch, cudaStream_t st);
+bool zg_shared_attention_valid(const ZgSeqOp& s, const size_t* elems, size_t n_bufs, char* why, size_t why_n);
+size_t zg_shared_attention_scratch_elems(const ZgSeqOp& s);
+bool zg_launch_shared_attention(const ZgOp& op, float* const* bufs, const size_t* elems, float* scratch, cudaStream_t st);

@@ -509,3 +509,4 @@ bool zg_launch_batch_op(const ZgOp& op, float* const* bufs, const size_t* elems,
 bool zg_shared_attention_valid(const ZgSeqOp& s, const size_t* elems, size_t n_bufs, char* why, size_t why_n);
 size_t zg_shared_attention_scratch_elems(const ZgSeqOp& s);
 bool zg_launch_shared_attention(const ZgOp& op, float* const* bufs, const size_t* elems, float* scratch, cudaStream_t st);
+unsigned int zg_shared_attention_timeouts();      // waits that gave up

@@ -13,7 +13,7 @@ namespace {
 struct SaArgs {
     float* dst; const float* q; const float* kc; const float* vc; const float* kp; const float* vp; const float* table;
     const void* sink;
-    float* part;                     // records [B, H, shares + splits, 4 + dv]: m, l, -, -, o; null: a row's keys are one share
+    float* part;                     // records [B, H, shares (0: splits), 4 + dv]: m, l, -, -, o
     uint32_t B, H, G, rep, dk, dv, q_rs, kw, vw, R, pkw, pvw, Rp, dst_rs, slots, pslots, sink_bf16;
     uint32_t shares, splits;         // shares of the prefix, which k_shared_prefix walks (0: k_shared_rows walks all keys), and of what is left to k_shared_rows
     float scale, cap;
@@ -39,7 +39,7 @@ __device__ __forceinline__ float sa_sink(const SaArgs& a, uint32_t h) {
     return a.sink_bf16 ? __bfloat162float(reinterpret_cast<const bf16*>(a.sink)[h]) : reinterpret_cast<const float*>(a.sink)[h];
 }
 // record of share i of a row's head
-__device__ __forceinline__ float* sa_record(const SaArgs& a, uint32_t r, uint32_t h, uint32_t i) { return a.part + ((size_t)(r * a.H + h) * (a.shares + a.splits) + i) * (4 + a.dv); }
+__device__ __forceinline__ float* sa_record(const SaArgs& a, uint32_t r, uint32_t h, uint32_t i) { return a.part + ((size_t)(r * a.H + h) * (a.shares ? a.shares : a.splits) + i) * (4 + a.dv); }
 // keys of a share when n keys fall into at most `shares` of them
 __device__ __forceinline__ uint32_t sa_share(uint32_t n, uint32_t shares, uint32_t least) { return max(least, ((n + shares - 1) / shares + 15) & ~15u); }
 constexpr uint32_t kSaShare = 64;    // the least
@@ -60,166 +60,326 @@ __device__ __forceinline__ float4 sa_load(const float* p, uint32_t d, uint32_t n
     return v;
 }
 
-// CTA (row, key head, chunk of RQ of its query heads; share of the keys).  LK lanes share a key: each holds NV float4 of it, of the queries and of the outputs; a warp
-// takes 32 / LK keys at a time, the warps' keys are interleaved.  Every lane group keeps its own running maximum and sum, merged once at the end.
-constexpr uint32_t kSaWarps = 4;
+// CTA (share of the keys; row, key head, chunk of RQ of its query heads).  LK lanes share a key: each holds NV float4 of it, of the queries and of the outputs; a warp
+// takes two keys per lane group at a time, the warps' keys are interleaved.  Keys and values come through a ring of kSaRing stages a warp, and a lane reads only what it
+// copied itself, so nothing but its own copies is waited for.  Every lane group keeps its own running maximum and sum and leaves a record in shared memory.
+// The shares of a row are a cluster (of at most 8) whose CTAs take a slice of the output columns each.  The records that k_shared_prefix has left join there, or in the
+// one CTA of a row.  Where eight shares are too few (a.part with a.shares = 0) CTAs leave records for k_shared_merge.
+// What bounds it is instruction latency beside the reads: 32 rows with 257 keys of their own on average took 53 us with one key per lane group and turn and the lane groups
+// merged by shuffles (600 instructions a turn of 4 keys).
+constexpr uint32_t kSaRing = 2, kSaMaxWarps = 8, kSaCluster = 8, kSaMost = 256 + 64;      // most records that meet: of 8 warps' lane groups and of the prefix
+__device__ __forceinline__ float sa_remote(const float* p, uint32_t rank) {
+    uint32_t at;
+    float v;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ void sa_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float sa_ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+template <bool VEC>
+__device__ __forceinline__ void sa_copy(uint32_t at, const float* p, uint32_t d, uint32_t n, bool on) {
+    if constexpr (VEC) {
+        const bool in = on && d < n;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(in ? p + d : p), "r"(in ? 16 : 0) : "memory");
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) {
+            const bool in = on && d + i < n;
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(at + 4 * i), "l"(in ? p + d + i : p), "r"(in ? 4 : 0) : "memory");
+        }
+    }
+}
+// weights of `count` records in the frame of the largest maximum, by one warp: at(e) is the maximum and sum of record e.  Returns the maximum; *sum: of all.
+template <class At>
+__device__ __forceinline__ float sa_weights(float* weight, uint32_t count, const At& at, float* sum) {
+    const uint32_t lane = threadIdx.x & 31;
+    float top = -INFINITY, total = 0.0f;
+    for (uint32_t e = lane; e < count; e += 32) top = fmaxf(top, at(e).x);
+    top = warp_max(top);
+    for (uint32_t e = lane; e < count; e += 32) {
+        const float2 y = at(e);
+        const float f = sa_weight(y.x, top);
+        weight[e] = f;
+        total = fmaf(y.y, f, total);
+    }
+    *sum = warp_sum(total);
+    return top;
+}
 template <int RQ, int NV, bool VEC>
-__global__ void __launch_bounds__(32 * kSaWarps) k_shared_rows(SaArgs a, uint32_t chunks, uint32_t LK) {
+__global__ void __launch_bounds__(32 * kSaMaxWarps) k_shared_rows(const SaArgs a, uint32_t chunks, uint32_t LK) {
     pdl_enter();
-    extern __shared__ float sh[];                                   // [warps][RQ][2 + dv]
-    const uint32_t c = blockIdx.x % chunks, g = blockIdx.x / chunks % a.G, r = blockIdx.x / chunks / a.G, split = blockIdx.y;
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane & (LK - 1), group = lane / LK, per_warp = 32 / LK;
+    extern __shared__ float4 ring[];                                // [warps][kSaRing][2][2 NV][32]; then the records [warps][lane groups][RQ][4 + padded dv], and the CTA's own
+    __shared__ float weight[RQ][kSaMost], sum_of[RQ], top_of[RQ];
+    float* const sh = reinterpret_cast<float*>(ring);
+    const uint32_t split = blockIdx.x % a.splits, item = blockIdx.x / a.splits, c = item % chunks, g = item / chunks % a.G, r = item / chunks / a.G, warps = blockDim.x >> 5;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane & (LK - 1), group = lane / LK, groups = 32 / LK;
     const uint32_t h0 = g * a.rep + c * RQ, nq = min((uint32_t)RQ, a.rep - c * RQ);
+    const bool records = a.part && !a.shares;                       // for k_shared_merge
     const SaKeys k = sa_keys(a, r, g);
-    if (!k.live) return;
-    const uint32_t first = a.shares ? k.prefix : 0u, n = k.prefix + k.own, share = sa_share(n - first, a.splits, kSaShare), k0 = first + split * share, k1 = min(n, k0 + share);
-    if (split && k0 >= n) return;                                   // (share 0 leaves a record however few the keys are)
-    float4 q[RQ][NV], o[RQ][NV];
+    if (!k.live) return;                                            // (the whole cluster)
+    const uint32_t first = a.shares ? k.prefix : 0u, n = k.prefix + k.own, share = sa_share(n - first, a.splits, kSaShare), k0 = min(n, first + split * share), k1 = min(n, k0 + share);
+    if (records && split && k0 >= n) return;                        // (share 0 leaves a record however few the keys are)
+    const uint32_t step = 2 * warps * groups, turns = (k1 - k0 + step - 1) / step;
+    float4* const mine = ring + (size_t)warp * kSaRing * 4 * NV * 32 + lane;
+    auto fetch = [&](uint32_t t) {
+        if (t < turns) {
+            const uint32_t to = smem_u32(mine + (t % kSaRing) * 4 * NV * 32);
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                const uint32_t u = k0 + t * step + (2 * warp + x) * groups + group;
+                const bool on = u < k1, own = u >= k.prefix;
+                const uint32_t at = own ? u - k.prefix : u;
+                const float* kr = on ? (own ? k.kc : k.kp) + (size_t)at * (own ? a.kw : a.pkw) : k.kc;
+                const float* vr = on ? (own ? k.vc : k.vp) + (size_t)at * (own ? a.vw : a.pvw) : k.vc;
+#pragma unroll
+                for (int j = 0; j < NV; j++) {
+                    sa_copy<VEC>(to + (x * 2 * NV + j) * 512, kr, 4 * (sub + LK * j), a.dk, on);
+                    sa_copy<VEC>(to + (x * 2 * NV + NV + j) * 512, vr, 4 * (sub + LK * j), a.dv, on);
+                }
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (uint32_t t = 0; t < kSaRing - 1; t++) fetch(t);
+    // Scores in units of log2: the scale and log2(e) are folded into the queries.
+    const float unit = a.cap > 0.0f ? a.scale : a.scale * kLog2e;
+    float2 q[RQ][2 * NV], o[RQ][2 * NV];
     float m[RQ], l[RQ];
 #pragma unroll
     for (int i = 0; i < RQ; i++) {
         m[i] = -INFINITY; l[i] = 0.0f;
 #pragma unroll
         for (int j = 0; j < NV; j++) {
-            q[i][j] = sa_load<VEC>(a.q + (size_t)r * a.q_rs + (size_t)(h0 + i) * a.dk, 4 * (sub + LK * j), a.dk, i < (int)nq);
-            o[i][j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            const float4 x = sa_load<VEC>(a.q + (size_t)r * a.q_rs + (size_t)(h0 + i) * a.dk, 4 * (sub + LK * j), a.dk, i < (int)nq);
+            q[i][2 * j] = make_float2(x.x * unit, x.y * unit); q[i][2 * j + 1] = make_float2(x.z * unit, x.w * unit);
+            o[i][2 * j] = o[i][2 * j + 1] = make_float2(0.0f, 0.0f);
         }
     }
-    for (uint32_t base = k0 + warp * per_warp; base < k1; base += kSaWarps * per_warp) {
-        const uint32_t u = base + group;
-        const bool on = u < k1, own = u >= k.prefix;
-        const float* kr = own ? k.kc + (size_t)(u - k.prefix) * a.kw : k.kp + (size_t)u * a.pkw;
-        const float* vr = own ? k.vc + (size_t)(u - k.prefix) * a.vw : k.vp + (size_t)u * a.pvw;
-        float4 x[NV], v[NV];
+#pragma unroll 1
+    for (uint32_t t = 0; t < turns; t++) {
+        fetch(t + kSaRing - 1);
+        asm volatile("cp.async.wait_group %0;" ::"n"(kSaRing - 1) : "memory");
+        const uint32_t u = k0 + t * step + 2 * warp * groups + group;
+        const float4* from = mine + (t % kSaRing) * 4 * NV * 32;
+        float s[2][RQ];
 #pragma unroll
-        for (int j = 0; j < NV; j++) {
-            x[j] = sa_load<VEC>(kr, 4 * (sub + LK * j), a.dk, on);
-            v[j] = sa_load<VEC>(vr, 4 * (sub + LK * j), a.dv, on);
-        }
-        float s[RQ];
+        for (int x = 0; x < 2; x++) {
+            float2 d[RQ];
 #pragma unroll
-        for (int i = 0; i < RQ; i++) {
-            s[i] = 0.0f;
+            for (int i = 0; i < RQ; i++) d[i] = make_float2(0.0f, 0.0f);
 #pragma unroll
-            for (int j = 0; j < NV; j++) s[i] = fmaf(q[i][j].x, x[j].x, fmaf(q[i][j].y, x[j].y, fmaf(q[i][j].z, x[j].z, fmaf(q[i][j].w, x[j].w, s[i]))));
+            for (int j = 0; j < NV; j++) {
+                const float4 y = from[32 * (x * 2 * NV + j)];
+#pragma unroll
+                for (int i = 0; i < RQ; i++) d[i] = __ffma2_rn(q[i][2 * j + 1], make_float2(y.z, y.w), __ffma2_rn(q[i][2 * j], make_float2(y.x, y.y), d[i]));
+            }
+#pragma unroll
+            for (int i = 0; i < RQ; i++) s[x][i] = d[i].x + d[i].y;
         }
         for (uint32_t w = LK >> 1; w > 0; w >>= 1)
 #pragma unroll
-            for (int i = 0; i < RQ; i++) s[i] += __shfl_xor_sync(0xffffffffu, s[i], w);
+            for (int x = 0; x < 2; x++)
+#pragma unroll
+                for (int i = 0; i < RQ; i++) s[x][i] += __shfl_xor_sync(0xffffffffu, s[x][i], w);
+        float up = -INFINITY;                                       // by how much any maximum grows
 #pragma unroll
         for (int i = 0; i < RQ; i++) {
-            s[i] *= a.scale;
-            if (a.cap > 0.0f) s[i] = a.cap * tanhf(s[i] / a.cap);
-            if (!on) s[i] = -INFINITY;
-            if (s[i] > m[i]) {
-                const float f = sa_weight(m[i], s[i]);
-                m[i] = s[i];
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                if (a.cap > 0.0f) s[x][i] = a.cap * kLog2e * tanhf(s[x][i] / a.cap);
+                if (u + x * groups >= k1) s[x][i] = -INFINITY;
+            }
+            up = fmaxf(up, fmaxf(s[0][i], s[1][i]) > m[i] ? 1.0f : -1.0f);
+        }
+        if (__any_sync(0xffffffffu, up > 0.0f)) {
+#pragma unroll
+            for (int i = 0; i < RQ; i++) {
+                const float top = fmaxf(m[i], fmaxf(s[0][i], s[1][i])), f = m[i] == -INFINITY ? 0.0f : sa_ex2(m[i] - top);
+                m[i] = top;
                 l[i] *= f;
 #pragma unroll
-                for (int j = 0; j < NV; j++) { o[i][j].x *= f; o[i][j].y *= f; o[i][j].z *= f; o[i][j].w *= f; }
+                for (int j = 0; j < 2 * NV; j++) o[i][j] = __fmul2_rn(o[i][j], make_float2(f, f));
             }
-            const float p = s[i] == -INFINITY ? 0.0f : expf(s[i] - m[i]);
-            l[i] += p;
-#pragma unroll
-            for (int j = 0; j < NV; j++) { o[i][j].x = fmaf(p, v[j].x, o[i][j].x); o[i][j].y = fmaf(p, v[j].y, o[i][j].y); o[i][j].z = fmaf(p, v[j].z, o[i][j].z); o[i][j].w = fmaf(p, v[j].w, o[i][j].w); }
         }
+#pragma unroll
+        for (int i = 0; i < RQ; i++) {
+#pragma unroll
+            for (int x = 0; x < 2; x++) s[x][i] = s[x][i] == -INFINITY ? 0.0f : sa_ex2(s[x][i] - m[i]);
+            l[i] += s[0][i] + s[1][i];
+        }
+#pragma unroll
+        for (int x = 0; x < 2; x++)
+#pragma unroll
+            for (int j = 0; j < NV; j++) {
+                const float4 v = from[32 * (x * 2 * NV + NV + j)];
+#pragma unroll
+                for (int i = 0; i < RQ; i++) {
+                    const float2 p = make_float2(s[x][i], s[x][i]);
+                    o[i][2 * j] = __ffma2_rn(p, make_float2(v.x, v.y), o[i][2 * j]);
+                    o[i][2 * j + 1] = __ffma2_rn(p, make_float2(v.z, v.w), o[i][2 * j + 1]);
+                }
+            }
     }
-    // the lane groups of a warp, then the warps
-    const uint32_t rec = 2 + a.dv;
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();                                                // the ring is idle
+    const uint32_t dvp = (a.dv + 3) & ~3u, rec = 4 + dvp, local = warps * groups;      // record e, head i: at (e RQ + i) rec
 #pragma unroll
     for (int i = 0; i < RQ; i++) {
-        float top = m[i];
-        for (uint32_t w = LK; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-        const float f = sa_weight(m[i], top);
-        l[i] *= f;
-        for (uint32_t w = LK; w < 32; w <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], w);
+        float* out = sh + ((size_t)(warp * groups + group) * RQ + i) * rec;
+        if (sub == 0) { out[0] = m[i] * kLn2; out[1] = l[i]; }      // (infinite where no key was seen)
 #pragma unroll
         for (int j = 0; j < NV; j++) {
-            float4 v = make_float4(o[i][j].x * f, o[i][j].y * f, o[i][j].z * f, o[i][j].w * f);
-            for (uint32_t w = LK; w < 32; w <<= 1) {
-                v.x += __shfl_xor_sync(0xffffffffu, v.x, w); v.y += __shfl_xor_sync(0xffffffffu, v.y, w);
-                v.z += __shfl_xor_sync(0xffffffffu, v.z, w); v.w += __shfl_xor_sync(0xffffffffu, v.w, w);
-            }
             const uint32_t d = 4 * (sub + LK * j);
-            float* out = sh + (warp * RQ + i) * rec + 2 + d;
-            if (group == 0) {
-                if (d < a.dv) out[0] = v.x;
-                if (d + 1 < a.dv) out[1] = v.y;
-                if (d + 2 < a.dv) out[2] = v.z;
-                if (d + 3 < a.dv) out[3] = v.w;
-            }
+            if (d < dvp) *reinterpret_cast<float4*>(out + 4 + d) = make_float4(o[i][2 * j].x, o[i][2 * j].y, o[i][2 * j + 1].x, o[i][2 * j + 1].y);
         }
-        if (lane == 0) { sh[(warp * RQ + i) * rec] = top; sh[(warp * RQ + i) * rec + 1] = l[i]; }
     }
     __syncthreads();
-    for (uint32_t i = 0; i < nq; i++) {
-        float top = -INFINITY, sum = 0.0f, f[kSaWarps];
-#pragma unroll
-        for (uint32_t w = 0; w < kSaWarps; w++) top = fmaxf(top, sh[(w * RQ + i) * rec]);
-#pragma unroll
-        for (uint32_t w = 0; w < kSaWarps; w++) { f[w] = sa_weight(sh[(w * RQ + i) * rec], top); sum = fmaf(sh[(w * RQ + i) * rec + 1], f[w], sum); }
-        const uint32_t h = h0 + i;
-        float* out;
-        float inv = 1.0f;
-        if (a.shares + a.splits > 1) {
-            float* mine = sa_record(a, r, h, a.shares + split);
-            if (threadIdx.x == 0) { mine[0] = top; mine[1] = sum; }
-            out = mine + 4;
+    const uint32_t per = sa_share(k.prefix, max(1u, a.shares), kSaShare), n_prefix = a.shares ? (k.prefix + per - 1) / per : 0u;
+    const bool alone = a.splits == 1;                               // the prefix's records join here; in a cluster later
+    for (uint32_t i = warp; i < nq; i += warps) {
+        const float* prefix = a.shares ? sa_record(a, r, h0 + i, 0) : nullptr;
+        const float* here = sh + i * rec;
+        float sum;
+        const float top = sa_weights(weight[i], local + (alone ? n_prefix : 0u), [&](uint32_t e) { return *reinterpret_cast<const float2*>(e < local ? here + (size_t)e * RQ * rec : prefix + (size_t)(e - local) * (4 + a.dv)); }, &sum);
+        if (lane == 0) { top_of[i] = top; sum_of[i] = sum; }
+    }
+    __syncthreads();
+    // what the CTA's sums and weights make of the row: the factor of its outputs
+    auto closing = [&](uint32_t i) {
+        float sum = sum_of[i];
+        if (a.sink && top_of[i] != -INFINITY) sum += expf(sa_sink(a, h0 + i) - top_of[i]);
+        return k.bad ? kBatchNaN : top_of[i] == -INFINITY ? 0.0f : 1.0f / sum;          // nothing seen: zeros
+    };
+    auto store = [&](uint32_t i, uint32_t d, float4 v) {
+        float* out = a.dst + (size_t)r * a.dst_rs + (size_t)(h0 + i) * a.dv + d;
+        if (d + 3 < a.dv && (reinterpret_cast<uintptr_t>(out) & 15) == 0) { *reinterpret_cast<float4*>(out) = v; return; }
+        out[0] = v.x;
+        if (d + 1 < a.dv) out[1] = v.y;
+        if (d + 2 < a.dv) out[2] = v.z;
+        if (d + 3 < a.dv) out[3] = v.w;
+    };
+    auto add = [](float4& v, const float4 x, float f) { v.x = fmaf(x.x, f, v.x); v.y = fmaf(x.y, f, v.y); v.z = fmaf(x.z, f, v.z); v.w = fmaf(x.w, f, v.w); };
+    auto add_prefix = [&](float4& v, uint32_t i, uint32_t d, uint32_t e0) {      // (dv is a multiple of four there)
+        const float* prefix = sa_record(a, r, h0 + i, 0) + 4 + d;
+#pragma unroll 6
+        for (uint32_t e = 0; e < n_prefix; e++) add(v, *reinterpret_cast<const float4*>(prefix + (size_t)e * (4 + a.dv)), weight[i][e0 + e]);
+    };
+    float* const sums = sh + (size_t)local * RQ * rec;              // in a cluster: the CTA's own record per head, behind the others
+    const uint32_t quads = dvp / 4;
+    for (uint32_t x = threadIdx.x; x < nq * quads; x += blockDim.x) {
+        const uint32_t i = x / quads, d = 4 * (x % quads);
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+        for (uint32_t e = 0; e < local; e++) add(v, *reinterpret_cast<const float4*>(sh + ((size_t)e * RQ + i) * rec + 4 + d), weight[i][e]);
+        if (records) {
+            float* out = sa_record(a, r, h0 + i, split);
+            if (d == 0) { out[0] = top_of[i]; out[1] = sum_of[i]; }
+            for (uint32_t e = 0; e < 4; e++) if (d + e < a.dv) out[4 + d + e] = (&v.x)[e];
+        } else if (alone) {
+            if (n_prefix) add_prefix(v, i, d, local);
+            const float f = closing(i);
+            store(i, d, make_float4(v.x * f, v.y * f, v.z * f, v.w * f));
         } else {
-            out = a.dst + (size_t)r * a.dst_rs + (size_t)h * a.dv;
-            if (a.sink && top != -INFINITY) sum += expf(sa_sink(a, h) - top);
-            inv = k.bad ? kBatchNaN : top == -INFINITY ? 0.0f : 1.0f / sum;          // nothing seen: zeros
-        }
-        for (uint32_t d = threadIdx.x; d < a.dv; d += 32 * kSaWarps) {
-            float v = 0.0f;
-#pragma unroll
-            for (uint32_t w = 0; w < kSaWarps; w++) v = fmaf(sh[(w * RQ + i) * rec + 2 + d], f[w], v);
-            out[d] = v * inv;
+            if (d == 0) { sums[i * rec] = top_of[i]; sums[i * rec + 1] = sum_of[i]; }
+            *reinterpret_cast<float4*>(sums + i * rec + 4 + d) = v;
         }
     }
+    if (records || alone) return;
+    sa_cluster_sync();
+    for (uint32_t i = warp; i < nq; i += warps) {
+        const float* prefix = a.shares ? sa_record(a, r, h0 + i, 0) : nullptr;
+        float sum;
+        const float top = sa_weights(weight[i], a.splits + n_prefix, [&](uint32_t e) {
+            return e < a.splits ? make_float2(sa_remote(sums + i * rec, e), sa_remote(sums + i * rec + 1, e)) : *reinterpret_cast<const float2*>(prefix + (size_t)(e - a.splits) * (4 + a.dv)); }, &sum);
+        if (lane == 0) { top_of[i] = top; sum_of[i] = sum; }
+    }
+    __syncthreads();
+    const uint32_t slice = (quads + a.splits - 1) / a.splits, q0 = min(quads, split * slice), width = min(quads, q0 + slice) - q0;
+    for (uint32_t x = threadIdx.x; x < nq * width; x += blockDim.x) {
+        const uint32_t i = x / width, d = 4 * (q0 + x % width);
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (uint32_t e = 0; e < a.splits; e++) {
+            const float* from = sums + i * rec + 4 + d;
+            add(v, make_float4(sa_remote(from, e), sa_remote(from + 1, e), sa_remote(from + 2, e), sa_remote(from + 3, e)), weight[i][e]);
+        }
+        if (n_prefix) add_prefix(v, i, d, a.splits);
+        const float f = closing(i);
+        store(i, d, make_float4(v.x * f, v.y * f, v.z * f, v.w * f));
+    }
+    sa_cluster_sync();                                              // no CTA leaves while its sums are read
 }
-// CTA (row, head): the records of its shares become the result
-__global__ void __launch_bounds__(128) k_shared_merge(SaArgs a) {
+// CTA (row, head): the records of its shares become the result.  Warp 0 finds the weights; then the warps take every fourth record each.
+__global__ void __launch_bounds__(256) k_shared_merge(const SaArgs a) {
     pdl_enter();
-    const uint32_t h = blockIdx.x % a.H, r = blockIdx.x / a.H;
+    __shared__ float weight[128], total, part[7][1024 / 4 * 4];
+    const uint32_t h = blockIdx.x % a.H, r = blockIdx.x / a.H, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const SaKeys k = sa_keys(a, r, 0);
     if (!k.live) return;
-    const uint32_t of_prefix = a.shares ? k.prefix : 0u, left = k.prefix + k.own - of_prefix, per = sa_share(of_prefix, max(1u, a.shares), kSaShare), per_left = sa_share(left, a.splits, kSaShare);
-    const uint32_t n0 = (of_prefix + per - 1) / per, n = n0 + max(1u, (left + per_left - 1) / per_left);
+    const uint32_t left = k.prefix + k.own, per = sa_share(left, a.splits, kSaShare), n = max(1u, (left + per - 1) / per);
     const float* rec = sa_record(a, r, h, 0);
-    auto at = [&](uint32_t s) { return rec + (size_t)(s < n0 ? s : a.shares + s - n0) * (4 + a.dv); };
-    float top = -INFINITY;
-    for (uint32_t s = 0; s < n; s++) top = fmaxf(top, at(s)[0]);
-    float sum = 0.0f;
-    for (uint32_t s = 0; s < n; s++) sum = fmaf(at(s)[1], sa_weight(at(s)[0], top), sum);
-    if (a.sink && top != -INFINITY) sum += expf(sa_sink(a, h) - top);
-    const float inv = k.bad ? kBatchNaN : top == -INFINITY ? 0.0f : 1.0f / sum;
+    if (warp == 0) {
+        float mm[4], ll[4], top = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+            const uint32_t e = lane + 32 * x;
+            mm[x] = -INFINITY; ll[x] = 0.0f;
+            if (e < n) { mm[x] = rec[(size_t)e * (4 + a.dv)]; ll[x] = rec[(size_t)e * (4 + a.dv) + 1]; }
+            top = fmaxf(top, mm[x]);
+        }
+        top = warp_max(top);
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+            const float f = sa_weight(mm[x], top);
+            sum = fmaf(ll[x], f, sum);
+            if (lane + 32 * x < n) weight[lane + 32 * x] = f;
+        }
+        sum = warp_sum(sum);
+        if (lane == 0) {
+            if (a.sink && top != -INFINITY) sum += expf(sa_sink(a, h) - top);
+            total = k.bad ? kBatchNaN : top == -INFINITY ? 0.0f : 1.0f / sum;
+        }
+    }
+    __syncthreads();
     float* out = a.dst + (size_t)r * a.dst_rs + (size_t)h * a.dv;
-    for (uint32_t d = threadIdx.x; d < a.dv; d += 128) {
+    for (uint32_t d = lane; d < a.dv; d += 32) {
         float v = 0.0f;
-        for (uint32_t s = 0; s < n; s++) v = fmaf(at(s)[4 + d], sa_weight(at(s)[0], top), v);
-        out[d] = v * inv;
+        for (uint32_t e = warp; e < n; e += 8) v = fmaf(rec[(size_t)e * (4 + a.dv) + 4 + d], weight[e], v);
+        if (warp) part[warp - 1][d] = v; else out[d] = v;
+    }
+    __syncthreads();
+    for (uint32_t d = threadIdx.x; d < a.dv; d += 256) {
+        float v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 7; w++) v += part[w][d];
+        out[d] = (out[d] + v) * total;
     }
 }
 
 // ── the prefix on the tensor cores ───────────────────────────────────────────────────────────────────────────────────
 // All query rows of a key head meet the same keys of the prefix, so its part of the attention is two matrix products.  CTA (key head, share of the prefix, tile of 128 query
-// rows): 64 keys and values at a time are read from the cache once, split into half-precision pairs on their way to shared memory (a scale per key, one per tile of
-// values; split_tc.cuh) and multiplied by tcgen05.mma, three MMAs a product.  Warps 0 - 15 do everything but issue: they load tile t + 2 while they split tile
-// t + 1 and take the softmax of tile t; four threads share a query row, each with a quarter of the keys and of the output columns.  Warp 16 issues.
+// rows): 64 keys and values at a time are read from the cache once, split into half-precision pairs on their way to shared memory (one scale per tile;
+// split_tc.cuh) and multiplied by tcgen05.mma, three MMAs a product.  The 16 warps load tile t + 2, split tile t + 1 and take the softmax of tile t; four threads share a
+// query row, each with a quarter of the keys and of the output columns.  Warp 0 issues the scores, warp 5 the products with the values.  (With a warp of its
+// own for the issue 17 warps had 96 registers each and spilled; 16 have 128.)
 //   TMEM: scores of two tiles, which become the probabilities in place (A operand), outputs of two tiles, the queries' pairs (A operand).
-//   What pairs cannot hold - something not finite, magnitudes too far apart for one scale - is found as it is split; the CTA then walks its share again in plain f32.
+//   Elements of a pair are off by at most 2^-25 where the largest of a row or tile is below 2^15 (split_tc.cuh), so a score by at most 2 dk 2^-10 times its scales'
+//   inverses; with those times log2(e) below kSpLoud = 2^-17 that is less than 2^-18 for 128 dims.  Louder scores (beyond 2^20), values that are small as a whole beside others of their tile
+//   and what is not finite are found on the way; the CTA then walks its share again in plain f32.
 // Every wait is bounded; a CTA whose wait ran out counts it and makes NaN of its rows.
-constexpr uint32_t kSpWorkers = 512, kSpThreads = kSpWorkers + 32, kSpStages = 3, kSpKeys = 64;
+constexpr uint32_t kSpThreads = 512, kSpStages = 3, kSpKeys = 64;
 template <int NC, int DV> struct SpLayout {
     static constexpr uint32_t k_part = NC * kSpKeys * 128, v_part = DV * 128, stage = 2 * (k_part + v_part);      // bytes; a part: hi or lo
-    static constexpr uint32_t share = kSpStages * stage, kf = share + 2 * 4 * 128 * 4, vf = kf + kSpStages * kSpKeys * 4, red = vf + 16, bars = red + 2 * 16 * 4, size = bars + 128 + 1024;
+    static constexpr uint32_t share = kSpStages * stage, factors = share + 2 * 4 * 128 * 4, red = factors + kSpStages * 16, rows = red + 2 * 32 * 4, bars = rows + 128 * 4, size = bars + 128 + 1024;
 };
-__device__ __forceinline__ float sp_ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-// Not zero, but below 2^-18 of the magnitude its scale is made for: a pair keeps fewer than 22 bits of it.  More than a few of them in a patch of 512 values (normally
-// distributed ones have 0.006) mean that something is small as a whole.
-__device__ __forceinline__ uint32_t sp_small(float x) { const float a = fabsf(x); return a < 0.0625f && a > 0.0f ? 1u : 0u; }
-constexpr uint32_t kSpSmall = 4;
+constexpr float kSpLoud = 1.0f / 131072.0f;
+// Eight values of one column, or two of one key, that are not zero but below these parts of the tile's largest: a pair keeps 22 bits of a value above 2^-18, 19 above 2^-21.
+constexpr float kSpColumn = 1.0f / 262144.0f, kSpKey = 1.0f / 2097152.0f;
 struct SpCta { uint32_t g, split, tile, k0, k1; const float* kp; const float* vp; };
 // query row i of the CTA's tile
 struct SpRow { bool on; uint32_t r, h; };
@@ -233,20 +393,19 @@ __device__ __forceinline__ SpRow sp_row(const SaArgs& a, const SpCta& c, const B
     return w;
 }
 // The CTA's share in plain f32: a warp takes four of its eight rows at a time, a lane four dims of a key and four columns of a value.
-__device__ __noinline__ void sp_plain(const SaArgs& a, const SpCta& c, const BatchHead& head) {
+__device__ __noinline__ void sp_plain(const SaArgs& a, const float* kp, const float* vp, uint32_t k0, uint32_t k1, uint32_t split, const uint32_t* rows) {
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     for (uint32_t i0 = warp * 8; i0 < warp * 8 + 8; i0 += 4) {
         float4 q[4], o[4];
         float m[4], l[4];
-        SpRow w[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            w[i] = sp_row(a, c, head, i0 + i);
-            q[i] = sa_load<true>(a.q + (size_t)w[i].r * a.q_rs + (size_t)w[i].h * a.dk, 4 * lane, a.dk, w[i].on);
+            const uint32_t w = rows[i0 + i];
+            q[i] = sa_load<true>(a.q + (size_t)(w >> 10) * a.q_rs + (size_t)(w & 1023) * a.dk, 4 * lane, a.dk, w != 0xffffffffu);
             o[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f); m[i] = -INFINITY; l[i] = 0.0f;
         }
-        for (uint32_t u = c.k0; u < c.k1; u++) {
-            const float4 x = sa_load<true>(c.kp + (size_t)u * a.pkw, 4 * lane, a.dk, true), v = sa_load<true>(c.vp + (size_t)u * a.pvw, 4 * lane, a.dv, true);
+        for (uint32_t u = k0; u < k1; u++) {
+            const float4 x = sa_load<true>(kp + (size_t)u * a.pkw, 4 * lane, a.dk, true), v = sa_load<true>(vp + (size_t)u * a.pvw, 4 * lane, a.dv, true);
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 float s = warp_sum(fmaf(q[i].x, x.x, fmaf(q[i].y, x.y, fmaf(q[i].z, x.z, q[i].w * x.w)))) * a.scale;
@@ -258,15 +417,16 @@ __device__ __noinline__ void sp_plain(const SaArgs& a, const SpCta& c, const Bat
         }
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            if (!w[i].on) continue;
-            float* rec = sa_record(a, w[i].r, w[i].h, c.split);
+            const uint32_t w = rows[i0 + i];
+            if (w == 0xffffffffu) continue;
+            float* rec = sa_record(a, w >> 10, w & 1023, split);
             if (lane == 0) { rec[0] = m[i]; rec[1] = l[i]; }
             if (4 * lane < a.dv) { rec[4 + 4 * lane] = o[i].x; rec[5 + 4 * lane] = o[i].y; rec[6 + 4 * lane] = o[i].z; rec[7 + 4 * lane] = o[i].w; }
         }
     }
 }
 template <int NC, int DV>
-__global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const SaArgs a, const uint32_t row_tiles) {
+__global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const __grid_constant__ SaArgs a, const uint32_t row_tiles) {
     typedef SpLayout<NC, DV> L;
     constexpr uint32_t kS = 0, kO = 2 * kSpKeys, kQ = kO + 2 * DV;         // TMEM columns
     static_assert(kQ + 64 * NC <= 512, "TMEM columns");
@@ -275,7 +435,7 @@ __global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const SaArgs a,
     uint8_t* const mem = dsm_raw + (base - smem_u32(dsm_raw));
     const uint32_t full = base + L::bars, empty = full + 8 * kSpStages, s_full = empty + 8 * kSpStages, o_full = s_full + 16, p_full = o_full + 16, q_full = p_full + 8, tmem_slot = q_full + 8;
     uint32_t* const trouble = reinterpret_cast<uint32_t*>(mem + (tmem_slot + 4 - base));          // 1: something that pairs cannot hold, 2: a wait that ran out
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;      // (in a form that the compiler knows to be the same in all lanes)
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < kSpStages; i++) { mbar_init(full + 8 * i, 16); mbar_init(empty + 8 * i, 1); }
         for (uint32_t i = 0; i < 2; i++) { mbar_init(s_full + 8 * i, 1); mbar_init(o_full + 8 * i, 1); }
@@ -283,7 +443,7 @@ __global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const SaArgs a,
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         *trouble = 0;
     }
-    if (warp == 16) {
+    if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(tmem_slot) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -296,66 +456,25 @@ __global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const SaArgs a,
     c.k0 = min(P, c.split * per); c.k1 = min(P, c.k0 + per);
     const size_t p0 = sound ? (size_t)head.prefix_slot * a.Rp : 0;
     c.kp = a.kp + p0 * a.pkw + c.g * a.dk; c.vp = a.vp + p0 * a.pvw + c.g * a.dv;
-    const uint32_t n_tiles = (c.k1 - c.k0 + kSpKeys - 1) / kSpKeys;
+    const uint32_t n_tiles = __shfl_sync(0xffffffffu, (c.k1 - c.k0 + kSpKeys - 1) / kSpKeys, 0);
+    uint32_t* const rows = reinterpret_cast<uint32_t*>(mem + L::rows);     // row << 10 | head of the tile's query rows, all bits set where there is none
+    if (threadIdx.x < 128) {
+        const SpRow w = sp_row(a, c, head, threadIdx.x);
+        rows[threadIdx.x] = w.on ? w.r << 10 | w.h : 0xffffffffu;
+    }
     fence_before();
     __syncthreads();
     fence_after();
 
-    if (n_tiles && warp == 16) {
-        constexpr uint32_t idesc_s = (1u << 4) | ((kSpKeys >> 3) << 17) | ((128u >> 4) << 24), idesc_o = (1u << 4) | ((DV >> 3) << 17) | ((128u >> 4) << 24);      // f16 x f16 -> f32
-        const bool leader = elect_one();
-        bool ok = mbar_wait(q_full, 0);
-        fence_after();
-        // three products, the small ones first: hi lo, lo hi, hi hi.  B parts of `part` bytes at b (hi, then lo), chunks of 64 along the summed dimension 8 KB apart
-        auto scores = [&](uint32_t t) {
-            if (ok) ok = mbar_wait(full + 8 * (t % kSpStages), (t / kSpStages) & 1);
-            fence_after();
-            if (!(leader && ok)) return;
-            const uint32_t d = kS + (t & 1) * kSpKeys, b = desc_low(base + (t % kSpStages) * L::stage);
-#pragma unroll
-            for (uint32_t x = 0; x < 3; x++) {
-                const uint32_t qa = kQ + (x == 1 ? 32 * NC : 0), kb = b + (x == 0 ? L::k_part >> 4 : 0);
-#pragma unroll
-                for (uint32_t k = 0; k < 4 * NC; k++) {
-                    if (x == 0 && k == 0) mma_ts<false>(d, qa, kb, idesc_s);
-                    else mma_ts<true>(d, qa + 8 * k, kb + (k / 4) * (kSpKeys * 128 >> 4) + 2 * (k % 4), idesc_s);
-                }
-            }
-            mma_commit(s_full + 8 * (t & 1));
-        };
-        // probabilities of 16 keys lie in 16 columns: 8 with their hi pairs, 8 with their lo pairs
-        auto values = [&](uint32_t t) {
-            if (ok) ok = mbar_wait(p_full, t & 1);
-            fence_after();
-            if (!(leader && ok)) return;
-            const uint32_t d = kO + (t & 1) * DV, pa = kS + (t & 1) * kSpKeys, b = desc_low(base + (t % kSpStages) * L::stage + 2 * L::k_part);
-#pragma unroll
-            for (uint32_t x = 0; x < 3; x++) {
-#pragma unroll
-                for (uint32_t k = 0; k < kSpKeys / 16; k++) {
-                    if (x == 0 && k == 0) mma_ts<false>(d, pa, b + (L::v_part >> 4), idesc_o);
-                    else mma_ts<true>(d, pa + 16 * k + (x == 1 ? 8 : 0), b + (x == 0 ? L::v_part >> 4 : 0) + 2 * k, idesc_o);
-                }
-            }
-            mma_commit(o_full + 8 * (t & 1));
-            mma_commit(empty + 8 * (t % kSpStages));
-        };
-        for (uint32_t t = 0; t < n_tiles && ok; t++) {
-            scores(t);
-            if (t) values(t - 1);
-        }
-        if (ok) values(n_tiles - 1);
-        if (!ok && lane == 0) { count_timeout(); atomicOr(trouble, 2u); }
-        __syncwarp();
-    } else if (n_tiles) {
+    if (n_tiles) {
         constexpr int OW = DV / 4, KT = DV == 128 ? 8 : 4;               // output columns and value rows of a thread
         const uint32_t part = warp >> 2, row = (warp & 3) * 32 + lane, lanes = ((warp & 3) * 32) << 16, half = lane >> 4, hl = lane & 15;
         const uint32_t v_key = DV == 128 ? 16 * (warp & 3) + 8 * half : 8 * (warp & 7) + 4 * half, v_col = 32 * (DV == 128 ? warp >> 2 : warp >> 3) + 2 * hl;
         float* const share = reinterpret_cast<float*>(mem + L::share);
-        float* const kf = reinterpret_cast<float*>(mem + L::kf);
-        float* const vf = reinterpret_cast<float*>(mem + L::vf);
+        float2* const factors = reinterpret_cast<float2*>(mem + L::factors);      // of a stage's keys and values
         uint32_t* const red = reinterpret_cast<uint32_t*>(mem + L::red);
         bool ok = true, slow = false;
+        float f = 0.0f;                                                  // a score in units of log2 is f times the keys' factor times the product
         float4 kr[2][NC];                                                // keys 2 warp + half and 32 more, 4 dims of every chunk of 64
         float2 vr[KT];                                                   // KT values, two columns
         auto load = [&](uint32_t t) {
@@ -372,51 +491,48 @@ __global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const SaArgs a,
                 vr[j] = u < c.k1 && v_col < a.dv ? *reinterpret_cast<const float2*>(c.vp + (size_t)u * a.pvw + v_col) : make_float2(0.0f, 0.0f);
             }
         };
+        uint32_t fill = 0, fill_phase = 1;                               // the stage that is filled next
         auto convert = [&](uint32_t t) {
-            const uint32_t s = t % kSpStages;
-            uint8_t* const stage = mem + s * L::stage;
-            float vm = 0.0f;
+            uint8_t* const stage = mem + fill * L::stage;
+            float km = 0.0f, c0 = 0.0f, c1 = 0.0f;
+            uint32_t least = 0xffffffffu;                                // the smallest of the keys' two values, zeros left out
 #pragma unroll
-            for (int j = 0; j < KT; j++) vm = abs_or_inf(abs_or_inf(vm, vr[j].x), vr[j].y);
-            const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(vm));           // magnitudes order as their bits do
-            if (lane == 0) red[(t & 1) * 16 + warp] = top;
-            bar_sync(5, kSpWorkers);
-            vm = __uint_as_float(__reduce_max_sync(0xffffffffu, red[(t & 1) * 16 + (lane & 15)]));
-            float vs, v_inv;
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int i = 0; i < NC; i++) km = fmaxf(fmaxf(fmaxf(km, fabsf(kr[j][i].x)), fmaxf(fabsf(kr[j][i].y), fabsf(kr[j][i].z))), fabsf(kr[j][i].w));
+#pragma unroll
+            for (int j = 0; j < KT; j++) {
+                c0 = fmaxf(c0, fabsf(vr[j].x)); c1 = fmaxf(c1, fabsf(vr[j].y));
+                least = min(least, __float_as_uint(fmaxf(fabsf(vr[j].x), fabsf(vr[j].y))) - 1u);
+            }
+            // magnitudes order as their bits do
+            const uint32_t k_top = __reduce_max_sync(0xffffffffu, __float_as_uint(km)), v_top = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(c0, c1)));
+            if (lane == 0) { red[(t & 1) * 32 + warp] = k_top; red[(t & 1) * 32 + 16 + warp] = v_top; }
+            bar_sync(5, kSpThreads);
+            km = __uint_as_float(__reduce_max_sync(0xffffffffu, red[(t & 1) * 32 + (lane & 15)]));
+            const float vm = __uint_as_float(__reduce_max_sync(0xffffffffu, red[(t & 1) * 32 + 16 + (lane & 15)]));
+            float ks, k_inv, vs, v_inv;
+            split_scale(km, ks, k_inv);
             split_scale(vm, vs, v_inv);
-            if (t >= kSpStages && ok) ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * s, (t / kSpStages - 1) & 1));
-            uint32_t small = 0, n_small = 0;
+            slow = slow || !(v_inv == v_inv) || !(fabsf(f * k_inv) <= kSpLoud) || least < __float_as_uint(vm * kSpKey) || (c0 > 0.0f && c0 < vm * kSpColumn) || (c1 > 0.0f && c1 < vm * kSpColumn);
+            if (threadIdx.x == 0) factors[fill] = make_float2(k_inv, v_inv);
+            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * fill, fill_phase));
+            uint8_t* const k_out = stage + (2 * warp + half) * 128 + (((hl >> 1) ^ ((2 * warp + half) & 7)) << 4) + 8 * (hl & 1);
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const uint32_t key = 32 * j + 2 * warp + half;
-                float km = 0.0f, ks, k_inv;
-#pragma unroll
-                for (int i = 0; i < NC; i++) km = abs_or_inf(abs_or_inf(abs_or_inf(abs_or_inf(km, kr[j][i].x), kr[j][i].y), kr[j][i].z), kr[j][i].w);
-#pragma unroll
-                for (int x = 8; x > 0; x >>= 1) km = fmaxf(km, __shfl_xor_sync(0xffffffffu, km, x));
-                split_scale(km, ks, k_inv);
-                slow = slow || !(k_inv == k_inv);
-                if (hl == 0) kf[s * kSpKeys + key] = k_inv;
+            for (int j = 0; j < 2; j++)
 #pragma unroll
                 for (int i = 0; i < NC; i++) {
-                    const float4 x = make_float4(kr[j][i].x * ks, kr[j][i].y * ks, kr[j][i].z * ks, kr[j][i].w * ks);
-                    small += sp_small(x.x) + sp_small(x.y) + sp_small(x.z) + sp_small(x.w);
                     uint2 hi, lo;
-                    split2(x.x, x.y, hi.x, lo.x); split2(x.z, x.w, hi.y, lo.y);
-                    uint8_t* const out = stage + i * kSpKeys * 128 + key * 128 + (((hl >> 1) ^ (key & 7)) << 4) + 8 * (hl & 1);
+                    split2(kr[j][i].x * ks, kr[j][i].y * ks, hi.x, lo.x); split2(kr[j][i].z * ks, kr[j][i].w * ks, hi.y, lo.y);
+                    uint8_t* const out = k_out + i * kSpKeys * 128 + j * 32 * 128;
                     *reinterpret_cast<uint2*>(out) = hi;
                     *reinterpret_cast<uint2*>(out + L::k_part) = lo;
                 }
-            }
 #pragma unroll
             for (int e = 0; e < 2; e++) {
                 uint32_t hi[KT / 2], lo[KT / 2];
 #pragma unroll
-                for (int j = 0; j < KT; j += 2) {
-                    const float x = (e ? vr[j].y : vr[j].x) * vs, y = (e ? vr[j + 1].y : vr[j + 1].x) * vs;
-                    n_small += sp_small(x) + sp_small(y);
-                    split2(x, y, hi[j / 2], lo[j / 2]);
-                }
+                for (int j = 0; j < KT; j += 2) split2((e ? vr[j].y : vr[j].x) * vs, (e ? vr[j + 1].y : vr[j + 1].x) * vs, hi[j / 2], lo[j / 2]);
                 const uint32_t col = v_col + e;
                 uint8_t* const out = stage + 2 * L::k_part + col * 128 + (((v_key >> 3) ^ (col & 7)) << 4) + 2 * (v_key & 7);
                 if constexpr (KT == 8) {
@@ -427,16 +543,13 @@ __global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const SaArgs a,
                     *reinterpret_cast<uint2*>(out + L::v_part) = make_uint2(lo[0], lo[1]);
                 }
             }
-            small = __reduce_add_sync(0xffffffffu, small); n_small = __reduce_add_sync(0xffffffffu, n_small);
-            slow = slow || !(v_inv == v_inv) || small >= kSpSmall || n_small >= kSpSmall;
-            if (threadIdx.x == 0) vf[s] = v_inv;
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            if (lane == 0) mbar_arrive(full + 8 * s);
+            if (lane == 0) mbar_arrive(full + 8 * fill);
+            if (++fill == kSpStages) { fill = 0; fill_phase ^= 1; }
         };
         load(0);
         // The queries come by whole rows into the later stages, and a thread takes its quarter row from there.
-        const SpRow w = sp_row(a, c, head, row);
         uint32_t n_share = 0;
         auto row_max = [&](float x) {                                    // over the row's four threads; two buffers in turns, so one barrier is enough
             float* s = share + (n_share++ & 1) * 512;
@@ -444,20 +557,19 @@ __global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const SaArgs a,
             bar_sync(1 + (warp & 3), 128);
             return fmaxf(fmaxf(s[row], s[128 + row]), fmaxf(s[256 + row], s[384 + row]));
         };
-        float f;                                                         // a score in units of log2 is f times the key's factor times the product
         {
             float* const stage = reinterpret_cast<float*>(mem + L::stage);
             constexpr uint32_t Q4 = 16 * NC;                             // float4s of a row; float4 j of row r lies at place j ^ (r & 7)
-            for (uint32_t i = threadIdx.x; i < 128 * Q4; i += kSpWorkers) {
+            for (uint32_t i = threadIdx.x; i < 128 * Q4; i += kSpThreads) {
                 const uint32_t r = i / Q4, j = i % Q4;
-                const SpRow x = sp_row(a, c, head, r);
-                const bool on = x.on && 4 * j < a.dk;
-                const float* from = a.q + (size_t)x.r * a.q_rs + (size_t)x.h * a.dk;
+                const uint32_t w = rows[r];
+                const bool on = w != 0xffffffffu && 4 * j < a.dk;
+                const float* from = on ? a.q + (size_t)(w >> 10) * a.q_rs + (size_t)(w & 1023) * a.dk : a.q;
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(stage + 4 * (r * Q4 + (j ^ (r & 7))))), "l"(on ? from + 4 * j : from), "r"(on ? 16 : 0) : "memory");
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
             asm volatile("cp.async.wait_group 0;" ::: "memory");
-            bar_sync(5, kSpWorkers);
+            bar_sync(5, kSpThreads);
             float4 x[4 * NC];                                            // 16 NC dims from 16 NC part on
             float mx = 0.0f, qs, q_inv;
 #pragma unroll
@@ -465,25 +577,23 @@ __global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const SaArgs a,
 #pragma unroll
             for (int i = 0; i < 4 * NC; i++) mx = abs_or_inf(abs_or_inf(abs_or_inf(abs_or_inf(mx, x[i].x), x[i].y), x[i].z), x[i].w);
             split_scale(row_max(mx), qs, q_inv);
-            uint32_t small = 0;
+            if (a.scale < 0.0f) qs = -qs;                                // f is not negative
 #pragma unroll
             for (int i = 0; i < NC; i++) {                               // 16 dims: 8 columns of pairs
                 uint32_t hi[8], lo[8];
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     const float4 y = make_float4(x[4 * i + j].x * qs, x[4 * i + j].y * qs, x[4 * i + j].z * qs, x[4 * i + j].w * qs);
-                    small += sp_small(y.x) + sp_small(y.y) + sp_small(y.z) + sp_small(y.w);
                     split2(y.x, y.y, hi[2 * j], lo[2 * j]);
                     split2(y.z, y.w, hi[2 * j + 1], lo[2 * j + 1]);
                 }
                 tmem_st(lanes + kQ + 8 * (NC * part + i), hi);
                 tmem_st(lanes + kQ + 32 * NC + 8 * (NC * part + i), lo);
             }
-            slow = small >= kSpSmall || !(q_inv == q_inv);
-            f = q_inv * a.scale * 1.4426950408889634f;
+            f = q_inv * fabsf(a.scale) * kLog2e;
             tmem_wait_st();
             fence_before();
-            bar_sync(5, kSpWorkers);                                     // the stages are free
+            bar_sync(5, kSpThreads);                                     // the stages are free
             if (lane == 0) mbar_arrive(q_full);
         }
         float o[OW];
@@ -503,31 +613,71 @@ __global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const SaArgs a,
                 o[j] = r.x; o[j + 1] = r.y;
             }
         };
+        // Issue.  Three products, the small ones first: hi lo, lo hi, hi hi.  B parts: hi, then lo; chunks of 64 along the summed dimension are 8 KB apart.  The whole warp does
+        // all but the issue itself, so that addresses stay warp-uniform.
+        constexpr uint32_t idesc_s = (1u << 4) | ((kSpKeys >> 3) << 17) | ((128u >> 4) << 24), idesc_o = (1u << 4) | ((DV >> 3) << 17) | ((128u >> 4) << 24);      // f16 x f16 -> f32
+        uint32_t issued = 0, issued_phase = 0;                           // stage of the next issue
+        auto scores = [&](uint32_t t) {
+            const uint32_t d = kS + (t & 1) * kSpKeys, b = desc_low(base) + issued * (L::stage >> 4);
+            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(full + 8 * issued, issued_phase));
+            fence_after();
+            if (elect_one() && ok) {
+#pragma unroll
+                for (uint32_t x = 0; x < 3; x++)
+#pragma unroll
+                    for (uint32_t k = 0; k < 4 * NC; k++) {
+                        const uint32_t qa = kQ + (x == 1 ? 32 * NC : 0) + 8 * k, kb = b + (x == 0 ? L::k_part >> 4 : 0) + (k / 4) * (kSpKeys * 128 >> 4) + 2 * (k % 4);
+                        if (x == 0 && k == 0) mma_ts<false>(d, qa, kb, idesc_s); else mma_ts<true>(d, qa, kb, idesc_s);
+                    }
+                mma_commit(s_full + 8 * (t & 1));
+            }
+            __syncwarp();
+            if (++issued == kSpStages) { issued = 0; issued_phase ^= 1; }
+        };
+        // probabilities of 16 keys lie in 16 columns: 8 with their hi pairs, 8 with their lo pairs
+        auto values = [&](uint32_t t) {
+            const uint32_t d = kO + (t & 1) * DV, pa = kS + (t & 1) * kSpKeys, b = desc_low(base) + issued * (L::stage >> 4) + (2 * L::k_part >> 4), freed = empty + 8 * issued;
+            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(p_full, t & 1));
+            fence_after();
+            if (elect_one() && ok) {
+#pragma unroll
+                for (uint32_t x = 0; x < 3; x++)
+#pragma unroll
+                    for (uint32_t k = 0; k < kSpKeys / 16; k++) {
+                        const uint32_t p = pa + 16 * k + (x == 1 ? 8 : 0), vb = b + (x == 0 ? L::v_part >> 4 : 0) + 2 * k;
+                        if (x == 0 && k == 0) mma_ts<false>(d, p, vb, idesc_o); else mma_ts<true>(d, p, vb, idesc_o);
+                    }
+                mma_commit(o_full + 8 * (t & 1));
+                mma_commit(freed);
+            }
+            __syncwarp();
+            if (++issued == kSpStages) { issued = 0; issued_phase ^= 1; }
+        };
+        uint32_t at = 0;                                                 // stage of tile t
         convert(0);
+        if (warp == 0) { if (ok) ok = __all_sync(0xffffffffu, mbar_wait(q_full, 0)); scores(0); }
         if (n_tiles > 1) load(1);
 #pragma unroll 1
         for (uint32_t t = 0; t < n_tiles; t++) {
             if (t + 1 < n_tiles) {
                 convert(t + 1);
                 if (t + 2 < n_tiles) load(t + 2);
-            } else bar_sync(5, kSpWorkers);                              // factors of tile t are there (inside the loop the barrier of the next tile says so)
+            } else bar_sync(5, kSpThreads);                              // factors of tile t are there (inside the loop the barrier of the next tile says so)
             const uint32_t s = lanes + kS + (t & 1) * kSpKeys + 16 * part, u0 = c.k0 + t * kSpKeys + 16 * part;
-            const float4* const key_f = reinterpret_cast<const float4*>(kf + (t % kSpStages) * kSpKeys + 16 * part);
-            const float v_inv = vf[t % kSpStages];
+            const float2 inv = factors[at];
+            if (++at == kSpStages) at = 0;
             if (ok) ok = __all_sync(0xffffffffu, mbar_wait(s_full + 8 * (t & 1), (t >> 1) & 1));
             fence_after();
             uint32_t v[16];
             tmem_ld(s, v);
             tmem_wait_ld(v);
-            float x[16];
+            float x[16], unit = fmaxf(f * inv.x, 1e-37f);
 #pragma unroll
-            for (int j = 0; j < 16; j += 4) {
-                const float4 y = key_f[j / 4];
-                x[j] = __uint_as_float(v[j]) * (y.x * f); x[j + 1] = __uint_as_float(v[j + 1]) * (y.y * f); x[j + 2] = __uint_as_float(v[j + 2]) * (y.z * f); x[j + 3] = __uint_as_float(v[j + 3]) * (y.w * f);
-            }
-            if (a.cap > 0.0f) {
+            for (int j = 0; j < 16; j++) x[j] = __uint_as_float(v[j]);
+            if (a.cap > 0.0f) {                                          // here in units of log2
 #pragma unroll
-                for (int j = 0; j < 16; j++) x[j] = a.cap * tanhf(x[j] * 0.6931471805599453f / a.cap) * 1.4426950408889634f;
+                for (int j = 0; j < 16; j++) x[j] = a.cap * tanhf(x[j] * unit * kLn2 / a.cap) * kLog2e;
+                unit = 1.0f;
             }
             if (u0 + 16 > c.k1) {
 #pragma unroll
@@ -536,16 +686,17 @@ __global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const SaArgs a,
             float m0 = x[0], m1 = x[1];
 #pragma unroll
             for (int j = 2; j < 16; j += 2) { m0 = fmaxf(m0, x[j]); m1 = fmaxf(m1, x[j + 1]); }
-            const float mx = row_max(fmaxf(m0, m1)), m_new = fmaxf(m, mx);
-            slow = slow || mx == INFINITY;
-            const float alpha = m == -INFINITY ? 0.0f : sp_ex2(m - m_new), shift = m_new == -INFINITY ? 14.0f : 14.0f - m_new;      // probabilities times 2^14
+            const float mx = fmaxf(m0, m1), m_new = fmaxf(m, row_max(mx * unit));
+            slow = slow || m_new == INFINITY;
+            const float alpha = m == -INFINITY ? 0.0f : sa_ex2(m - m_new), shift = m_new == -INFINITY ? 14.0f : 14.0f - m_new;      // probabilities times 2^14
             m = m_new;
             float l0 = 0.0f, l1 = 0.0f;
 #pragma unroll
             for (int j = 0; j < 16; j += 2) {
-                x[j] = sp_ex2(x[j] + shift); x[j + 1] = sp_ex2(x[j + 1] + shift);
-                l0 += x[j]; l1 += x[j + 1];
-                split2(x[j], x[j + 1], v[j / 2], v[8 + j / 2]);
+                const float2 y = __ffma2_rn(make_float2(x[j], x[j + 1]), make_float2(unit, unit), make_float2(shift, shift));
+                const float p0 = sa_ex2(y.x), p1 = sa_ex2(y.y);
+                l0 += p0; l1 += p1;
+                split2(p0, p1, v[j / 2], v[8 + j / 2]);
             }
             tmem_st(s, v);
             l = fmaf(l, alpha, l0 + l1);
@@ -554,7 +705,10 @@ __global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const SaArgs a,
             __syncwarp();
             if (lane == 0) mbar_arrive(p_full);
             if (t) add_output(t - 1);
-            alpha_prev = alpha; f_prev = v_inv;
+            alpha_prev = alpha; f_prev = inv.y;
+            // The products run beside the next tile's split.  Scores overwrite probabilities whose outputs have just been waited for.
+            if (warp == 0) { if (t + 1 < n_tiles) scores(t + 1); }
+            else if (warp == 5) values(t);
         }
         add_output(n_tiles - 1);
         {
@@ -563,24 +717,25 @@ __global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const SaArgs a,
             bar_sync(1 + (warp & 3), 128);
             l = (s[row] + s[128 + row]) + (s[256 + row] + s[384 + row]);
         }
-        constexpr float unit = 1.0f / 16384.0f;
+        constexpr float p_unit = 1.0f / 16384.0f;
         // Outputs leave by whole rows, through the idle stages.
         float4* const out = reinterpret_cast<float4*>(mem);
 #pragma unroll
-        for (int j = 0; j < OW; j += 4) out[row * (DV / 4) + (((OW * part + j) / 4) ^ (row & 7))] = make_float4(o[j] * unit, o[j + 1] * unit, o[j + 2] * unit, o[j + 3] * unit);
-        if (slow || (w.on && m < -1e36f)) atomicOr(trouble, 1u);
+        for (int j = 0; j < OW; j += 4) out[row * (DV / 4) + (((OW * part + j) / 4) ^ (row & 7))] = make_float4(o[j] * p_unit, o[j + 1] * p_unit, o[j + 2] * p_unit, o[j + 3] * p_unit);
+        const uint32_t mine = rows[row];
+        if (slow || (mine != 0xffffffffu && m < -1e36f)) atomicOr(trouble, 1u);
         if (!ok) { atomicOr(trouble, 2u); if (lane == 0) count_timeout(); }
-        bar_sync(5, kSpWorkers);
+        bar_sync(5, kSpThreads);
         const uint32_t what = *reinterpret_cast<volatile uint32_t*>(trouble);
-        if (what == 1) sp_plain(a, c, head);
+        if (what == 1) sp_plain(a, c.kp, c.vp, c.k0, c.k1, c.split, rows);
         else {
             const bool lost = what & 2u;
-            if (w.on && part == 0) { float* rec = sa_record(a, w.r, w.h, c.split); rec[0] = lost ? kBatchNaN : m * 0.6931471805599453f; rec[1] = lost ? kBatchNaN : l * unit; }
-            for (uint32_t i = threadIdx.x; i < 128 * (DV / 4); i += kSpWorkers) {
+            if (mine != 0xffffffffu && part == 0) { float* rec = sa_record(a, mine >> 10, mine & 1023, c.split); rec[0] = lost ? kBatchNaN : m * kLn2; rec[1] = lost ? kBatchNaN : l * p_unit; }
+            for (uint32_t i = threadIdx.x; i < 128 * (DV / 4); i += kSpThreads) {
                 const uint32_t r = i / (DV / 4), j = i % (DV / 4);
-                const SpRow x = sp_row(a, c, head, r);
-                if (!x.on || 4 * j >= a.dv) continue;
-                *reinterpret_cast<float4*>(sa_record(a, x.r, x.h, c.split) + 4 + 4 * j) = lost ? make_float4(kBatchNaN, kBatchNaN, kBatchNaN, kBatchNaN) : out[r * (DV / 4) + (j ^ (r & 7))];
+                const uint32_t w = rows[r];
+                if (w == 0xffffffffu || 4 * j >= a.dv) continue;
+                *reinterpret_cast<float4*>(sa_record(a, w >> 10, w & 1023, c.split) + 4 + 4 * j) = lost ? make_float4(kBatchNaN, kBatchNaN, kBatchNaN, kBatchNaN) : out[r * (DV / 4) + (j ^ (r & 7))];
             }
         }
     }
@@ -588,12 +743,12 @@ __global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const SaArgs a,
     __syncwarp();
     fence_before();
     __syncthreads();
-    if (warp == 16) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(0u) : "memory");
+    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(0u) : "memory");
 }
 
 // What decides a launch: queries a CTA of k_shared_rows holds (RQ), float4 a lane holds (NV), lanes that share a key (LK), shares of its keys; shares of the prefix
 // on the tensor cores (0: k_shared_rows walks the prefix too).
-struct SaShape { uint32_t RQ, NV, LK, chunks, splits, shares, row_tiles; };
+struct SaShape { uint32_t RQ, NV, LK, chunks, splits, warps, shares, row_tiles; bool records; };
 SaShape sa_shape(const ZgSeqOp& s, bool wide) {
     const uint32_t B = s.n[0], G = s.n[2], rep = s.n[1] / G, dk = s.n[3], dv = s.n[4], dim = std::max(dk, dv), R = s.n[8], Rp = s.n[11], sms = zg_sm_count();
     SaShape p = {};
@@ -612,8 +767,12 @@ SaShape sa_shape(const ZgSeqOp& s, bool wide) {
             if (cost < best) { best = cost; p.shares = n; }
         }
     }
-    const uint32_t ctas = B * G * p.chunks, keys = R + (p.shares ? 0 : Rp);
-    p.splits = std::max(1u, std::min({(8 * sms + ctas - 1) / ctas, (keys + kSaShare - 1) / kSaShare, 128u}));
+    // Shares of at least 64 keys while the SMs are not covered several times over.  Up to eight of a row merge inside a cluster; beyond that, which only few rows over many
+    // keys ask for, through records and a second launch.
+    const uint32_t ctas = B * G * p.chunks, keys = R + (p.shares ? 0 : Rp), most = (keys + kSaShare - 1) / kSaShare;
+    p.splits = std::max(1u, std::min({3 * sms / ctas, most, kSaCluster}));
+    p.warps = ctas * p.splits >= sms || p.NV > 4 ? 4 : kSaMaxWarps;      // (eight warps' rings of the widest rows do not fit)
+    if (!p.shares && 2 * ctas * kSaCluster < sms && most >= 4 * kSaCluster) { p.splits = std::min({(2 * sms + ctas - 1) / ctas, most / 2, 128u}); p.records = true; }
     return p;
 }
 // 16-byte loads of every operand, as far as sizes and offsets say so (buffers begin at 16 bytes at least)
@@ -628,18 +787,24 @@ bool sa_launch_prefix(const SaArgs& a, const SaShape& p, cudaStream_t st) {
     launch_pdl(k_shared_prefix<NC, DV>, dim3(p.row_tiles * a.shares * a.G), dim3(kSpThreads), L::size, st, a, p.row_tiles);
     return true;
 }
-template <int RQ, int NV>
-bool sa_launch_rows(const SaArgs& a, const SaShape& p, bool vec, cudaStream_t st) {
-    const dim3 grid(a.B * a.G * p.chunks, a.splits);
-    const size_t smem = sizeof(float) * kSaWarps * RQ * (2 + a.dv);
-    if (smem > 48 * 1024) {
-        if (!(vec ? zg_smem_limit<k_shared_rows<RQ, NV, true>>(sizeof(float) * kSaWarps * RQ * 1026) : zg_smem_limit<k_shared_rows<RQ, NV, false>>(sizeof(float) * kSaWarps * RQ * 1026))) return false;
-    }
-    if (vec) launch_pdl(k_shared_rows<RQ, NV, true>, grid, dim3(32 * kSaWarps), smem, st, a, p.chunks, p.LK);
-    else launch_pdl(k_shared_rows<RQ, NV, false>, grid, dim3(32 * kSaWarps), smem, st, a, p.chunks, p.LK);
+template <int RQ, int NV, bool VEC>
+bool sa_launch_rows(const SaArgs& a, const SaShape& p, cudaStream_t st) {
+    constexpr size_t limit = 200 * 1024;
+    const uint32_t dvp = (a.dv + 3) / 4 * 4;
+    const size_t smem = std::max<size_t>((size_t)p.warps * kSaRing * 4 * NV * 512, sizeof(float) * (p.warps * (32 / p.LK) + 1) * RQ * (4 + dvp));
+    if (smem > limit) { zg_set_error("shared_attention: %zu bytes of shared memory", smem); return false; }
+    if (!zg_smem_limit<k_shared_rows<RQ, NV, VEC>>(limit)) return false;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(p.splits * a.B * a.G * p.chunks); cfg.blockDim = dim3(32 * p.warps); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = g_zg_pdl ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = p.records ? 1 : p.splits; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr; cfg.numAttrs = 2;
+    cudaLaunchKernelEx(&cfg, k_shared_rows<RQ, NV, VEC>, a, p.chunks, p.LK);
     return true;
 }
-
 }  // namespace
 
 bool zg_shared_attention_valid(const ZgSeqOp& s, const size_t* elems, size_t n_bufs, char* why, size_t why_n) {
@@ -661,7 +826,7 @@ bool zg_shared_attention_valid(const ZgSeqOp& s, const size_t* elems, size_t n_b
 }
 size_t zg_shared_attention_scratch_elems(const ZgSeqOp& s) {
     const SaShape p = sa_shape(s, sa_vec(s));
-    return p.shares + p.splits > 1 ? (size_t)s.n[0] * s.n[1] * (p.shares + p.splits) * (4 + s.n[4]) : 0;
+    return (size_t)s.n[0] * s.n[1] * (p.shares + (p.records ? p.splits : 0)) * (4 + s.n[4]);
 }
 bool zg_launch_shared_attention(const ZgOp& op, float* const* bufs, const size_t* elems, float* scratch, cudaStream_t st) {
     const ZgSeqOp& s = op.u.seq;
@@ -680,9 +845,9 @@ bool zg_launch_shared_attention(const ZgOp& op, float* const* bufs, const size_t
     a.scale = s.f[0]; a.cap = s.f[1];
     const bool vec = sa_vec(s);
     SaShape p = sa_shape(s, vec && scratch);
-    if (!scratch) p.splits = 1;                       // no room for records: a row's keys are one share
+    if (p.records && !scratch) { p.records = false; p.splits = kSaCluster; }      // no room for records
     a.shares = p.shares; a.splits = p.splits;
-    a.part = scratch;
+    a.part = p.shares || p.records ? scratch : nullptr;
     if (a.shares) {
         const bool k1 = a.dk <= 64, v1 = a.dv <= 64;
         if (!(k1 ? v1 ? sa_launch_prefix<1, 64>(a, p, st) : sa_launch_prefix<1, 128>(a, p, st) : v1 ? sa_launch_prefix<2, 64>(a, p, st) : sa_launch_prefix<2, 128>(a, p, st))) return false;
@@ -691,20 +856,20 @@ bool zg_launch_shared_attention(const ZgOp& op, float* const* bufs, const size_t
     bool ok = false;
 #define ZG_SA(NV_)                                                                       \
     switch (p.RQ) {                                                                      \
-        case 1: ok = sa_launch_rows<1, NV_>(a, p, vec, st); break;                       \
-        case 2: ok = sa_launch_rows<2, NV_>(a, p, vec, st); break;                       \
-        case 3: ok = sa_launch_rows<3, NV_>(a, p, vec, st); break;                       \
-        default: ok = sa_launch_rows<4, NV_>(a, p, vec, st); break;                      \
+        case 1: ok = vec ? sa_launch_rows<1, NV_, true>(a, p, st) : sa_launch_rows<1, NV_, false>(a, p, st); break;                       \
+        case 2: ok = vec ? sa_launch_rows<2, NV_, true>(a, p, st) : sa_launch_rows<2, NV_, false>(a, p, st); break;                       \
+        case 3: ok = vec ? sa_launch_rows<3, NV_, true>(a, p, st) : sa_launch_rows<3, NV_, false>(a, p, st); break;                       \
+        default: ok = vec ? sa_launch_rows<4, NV_, true>(a, p, st) : sa_launch_rows<4, NV_, false>(a, p, st); break;                      \
     }
     if (p.NV == 4) { ZG_SA(4); }
     else if (p.NV == 5) { ZG_SA(5); }
-    else if (p.RQ == 1) ok = sa_launch_rows<1, 8>(a, p, vec, st);
-    else ok = sa_launch_rows<2, 8>(a, p, vec, st);
+    else if (p.RQ == 1) ok = vec ? sa_launch_rows<1, 8, true>(a, p, st) : sa_launch_rows<1, 8, false>(a, p, st);
+    else ok = vec ? sa_launch_rows<2, 8, true>(a, p, st) : sa_launch_rows<2, 8, false>(a, p, st);
 #undef ZG_SA
     if (!ok) return false;
     ZG_SEQ_CHECK();
-    if (a.shares + a.splits > 1) {
-        launch_pdl(k_shared_merge, dim3(a.B * a.H), dim3(128), 0, st, a);
+    if (p.records) {
+        launch_pdl(k_shared_merge, dim3(a.B * a.H), dim3(256), 0, st, a);
         ZG_SEQ_CHECK();
     }
     return true;

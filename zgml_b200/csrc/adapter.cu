@@ -1,0 +1,599 @@
+// ADAPTER_LINEAR (parameter pack in include/zgml_cuda.h): dst[r] = base[r] + s_a B_a (A_a src[r]), a the adapter of row r.  Two chained products through `rank` values a
+// row; a run of rows with one adapter shares its weights.
+//
+//   * k_adapter_few: a cluster of 8 CTAs per run of at most 8 rows.  Each CTA sums its eighth of the inputs, the eighths meet over distributed shared memory, and each CTA
+//     makes its eighth of the outputs: one launch, and the second product's weights are on their way while the first one is summed.
+//   * k_adapter_shrink, k_adapter_expand: blocks of 128 rows on tcgen05, for prompts.
+#include "batch_table.cuh"
+#include "split_tc.cuh"
+
+#include <algorithm>
+
+namespace {
+
+struct AdArgs {
+    float* dst; const float* src; const float* base; const float* scales; const float* table;
+    uint32_t B, N, K, rank, adapters, src_rs, dst_rs, base_rs;
+};
+// what a row asks for: an adapter, or ...
+constexpr int kAdNone = -1, kAdIdle = -2, kAdBad = -3;
+__device__ __forceinline__ int ad_of(const AdArgs& a, const BatchHead& head, uint32_t r) {
+    if (r >= head.rows) return kAdIdle;
+    const BatchRow w = batch_row(a.table, r);
+    return w.slot < 0 ? kAdIdle : w.adapter < 0 ? kAdNone : (uint32_t)w.adapter >= a.adapters ? kAdBad : w.adapter;
+}
+
+// ── few rows ─────────────────────────────────────────────────────────────────────────────────────────────────────────
+constexpr uint32_t kAfRows = 8, kAfCluster = 8, kAfThreads = 256, kAfStage = 96 * 1024;      // bytes of the second product's weights that are fetched ahead
+// R: rows of the run at most; J: rank values at a time.  x and the weights in vectors of WVec<WT>::n where VEC
+template <typename WT, int R, int J, bool VEC>
+__device__ __forceinline__ void af_shrink(const AdArgs& a, const WT* __restrict__ wa, const float* __restrict__ x, uint32_t rows, uint32_t k0, uint32_t k1, float* part) {
+    constexpr uint32_t V = VEC ? WVec<WT>::n : 1;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (uint32_t j0 = warp * J; j0 < a.rank; j0 += 8 * J) {
+        float acc[J][R];
+#pragma unroll
+        for (int j = 0; j < J; j++)
+#pragma unroll
+            for (int r = 0; r < R; r++) acc[j][r] = 0.0f;
+#pragma unroll 2
+        for (uint32_t k = k0 + V * lane; k < k1; k += 32 * V) {
+            float w[J][V];
+#pragma unroll
+            for (int j = 0; j < J; j++) {
+                const WT* from = wa + (size_t)min(j0 + j, a.rank - 1) * a.K + k;
+                if constexpr (VEC) wld_vec<WT>(from, w[j]); else w[j][0] = wld(from, 0);
+            }
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                if (R > 1 && r >= (int)rows) break;
+                float y[V];
+                if constexpr (VEC) {
+#pragma unroll
+                    for (int v = 0; v < (int)V; v += 4) wld_vec<float>(x + (size_t)r * a.src_rs + k + v, y + v);
+                } else y[0] = x[(size_t)r * a.src_rs + k];
+#pragma unroll
+                for (int j = 0; j < J; j++)
+#pragma unroll
+                    for (int v = 0; v < (int)V; v++) acc[j][r] = fmaf(w[j][v], y[v], acc[j][r]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < J; j++)
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                if (R > 1 && r >= (int)rows) break;
+                const float s = warp_sum(acc[j][r]);
+                if (lane == 0 && j0 + j < a.rank) part[r * a.rank + j0 + j] = s;
+            }
+    }
+}
+template <typename WT, int R, bool VEC>
+__device__ __forceinline__ void af_expand(const AdArgs& a, const WT* wb, const float* base, float* dst, uint32_t rows, uint32_t n0, uint32_t n1, const float* h) {
+    for (uint32_t n = n0 + threadIdx.x; n < n1; n += kAfThreads) {
+        const WT* row = wb + (size_t)(n - n0) * a.rank;
+        float acc[R];
+#pragma unroll
+        for (int r = 0; r < R; r++) acc[r] = 0.0f;
+        if constexpr (VEC) {
+            for (uint32_t j = 0; j < a.rank; j += 4) {
+                float w[4];
+                if constexpr (sizeof(WT) == 2) {
+                    const uint2 u = *reinterpret_cast<const uint2*>(row + j);
+                    w[0] = __uint_as_float(u.x << 16); w[1] = __uint_as_float(u.x & 0xFFFF0000u); w[2] = __uint_as_float(u.y << 16); w[3] = __uint_as_float(u.y & 0xFFFF0000u);
+                } else wld_vec<float>(row + j, w);
+#pragma unroll
+                for (int r = 0; r < R; r++) {
+                    const float4 y = *reinterpret_cast<const float4*>(h + r * a.rank + j);
+                    acc[r] = fmaf(w[0], y.x, fmaf(w[1], y.y, fmaf(w[2], y.z, fmaf(w[3], y.w, acc[r]))));
+                }
+            }
+        } else {
+            for (uint32_t j = 0; j < a.rank; j++) {
+                const float w = wld(row, j);
+#pragma unroll
+                for (int r = 0; r < R; r++) acc[r] = fmaf(w, h[r * a.rank + j], acc[r]);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < R; r++)
+            if (R == 1 || r < (int)rows) dst[(size_t)r * a.dst_rs + n] = base[(size_t)r * a.base_rs + n] + acc[r];
+    }
+}
+// vec_k: x and A in vectors; vec_j: rows of B in vectors of four; stage: bytes of B fetched ahead (0: not)
+template <typename WT>
+__global__ void __launch_bounds__(kAfThreads) __cluster_dims__(kAfCluster, 1, 1) k_adapter_few(AdArgs a, const WT* __restrict__ wa, const WT* __restrict__ wb, uint32_t k_slice, uint32_t n_slice,
+                                                                                             uint32_t vec_k, uint32_t vec_j, uint32_t stage) {
+    pdl_enter();
+    extern __shared__ float4 af_mem[];                               // [stage] weights of the CTA's outputs; [8][rank] the CTA's sums; [8][rank] all sums
+    const uint32_t rank_id = blockIdx.x % kAfCluster, r = blockIdx.x / kAfCluster;
+    const BatchHead head = batch_head(a.table, a.B);
+    const int mine = ad_of(a, head, r);
+    if (mine == kAdIdle) return;
+    const uint32_t n0 = min(a.N, rank_id * n_slice), n1 = min(a.N, n0 + n_slice);
+    const float* base = a.base + (size_t)r * a.base_rs;
+    float* dst = a.dst + (size_t)r * a.dst_rs;
+    if (mine < 0) {
+        if (mine == kAdBad || base != dst)
+            for (uint32_t n = n0 + threadIdx.x; n < n1; n += kAfThreads) dst[n] = mine == kAdNone ? base[n] : kBatchNaN;
+        return;
+    }
+    // the run of rows with this adapter, inside a block of eight rows: its first row's cluster takes all of it
+    if (r % kAfRows && ad_of(a, head, r - 1) == mine) return;
+    uint32_t rows = 1;
+    {
+        bool on = true;
+#pragma unroll
+        for (uint32_t i = 1; i < kAfRows; i++) {
+            on = on && r % kAfRows + i < kAfRows && ad_of(a, head, min(r + i, a.B - 1)) == mine && r + i < a.B;
+            rows += on ? 1u : 0u;
+        }
+    }
+    wa += (size_t)mine * a.rank * a.K;
+    wb += (size_t)mine * a.N * a.rank + (size_t)n0 * a.rank;
+    float* const part = reinterpret_cast<float*>(af_mem) + stage / 4;
+    float* const h = part + kAfRows * ((a.rank + 3) & ~3u);
+    if (stage && n1 > n0) {
+        const uint32_t bytes = (n1 - n0) * a.rank * (uint32_t)sizeof(WT), at = (uint32_t)__cvta_generic_to_shared(af_mem);
+        for (uint32_t i = 16 * threadIdx.x; i < bytes; i += 16 * kAfThreads)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at + i), "l"(reinterpret_cast<const char*>(wb) + i), "r"(min(16u, bytes - i)) : "memory");
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    const float scale = a.scales ? a.scales[mine] : 1.0f;
+    const float* x = a.src + (size_t)r * a.src_rs;
+    const uint32_t k0 = min(a.K, rank_id * k_slice), k1 = min(a.K, k0 + k_slice);
+    if (rows == 1) {
+        if (vec_k) af_shrink<WT, 1, 2, true>(a, wa, x, rows, k0, k1, part); else af_shrink<WT, 1, 2, false>(a, wa, x, rows, k0, k1, part);
+    } else {
+        if (vec_k) af_shrink<WT, kAfRows, 2, true>(a, wa, x, rows, k0, k1, part); else af_shrink<WT, kAfRows, 2, false>(a, wa, x, rows, k0, k1, part);
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    for (uint32_t i = threadIdx.x; i < kAfRows * a.rank; i += kAfThreads) {
+        float s = 0.0f;
+        if (i < rows * a.rank) {
+            const uint32_t at = (uint32_t)__cvta_generic_to_shared(part + i);
+#pragma unroll
+            for (uint32_t c = 0; c < kAfCluster; c++) {
+                uint32_t there;
+                float v;
+                asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(c));
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
+                s += v;
+            }
+        }
+        h[i] = s * scale;
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");      // its wait is at the end: no CTA leaves while its sums are read
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+    const WT* const from = stage ? reinterpret_cast<const WT*>(af_mem) : wb;
+    if (rows == 1) {
+        if (vec_j) af_expand<WT, 1, true>(a, from, base, dst, rows, n0, n1, h); else af_expand<WT, 1, false>(a, from, base, dst, rows, n0, n1, h);
+    } else {
+        if (vec_j) af_expand<WT, kAfRows, true>(a, from, base, dst, rows, n0, n1, h); else af_expand<WT, kAfRows, false>(a, from, base, dst, rows, n0, n1, h);
+    }
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// ── many rows ────────────────────────────────────────────────────────────────────────────────────────────────────────
+// Blocks of 128 rows on tcgen05.  Activations (and f32 weights) go in as three bfloat16 parts, all 24 bits of them: three products over bfloat16 weights, six over f32 ones.
+// Rows of a block that have another adapter than the product at hand are computed and left out.
+//   k_adapter_shrink: the 8 CTAs of a cluster share a block's inputs.  x is split on its way to shared memory; up to kAmRuns adapters accumulate side by side in TMEM; the
+//   partial sums meet over distributed shared memory and leave as the parts that the second product wants: x is read once.
+//   k_adapter_expand: a CTA keeps the block's rank values and walks tiles of 128 outputs: four warps bring weights and issue, sixteen add the base and write.  Base and dst
+//   are what bounds it.
+// (The same on mma.sync took 124 us for 2048 rows of 4096 inputs, 14336 outputs, rank 64, with its issue rate as the bound: 11.3 T operations of products at 130 T/s.)
+// Every wait is bounded; a CTA whose wait ran out counts it and makes NaN of its rows.
+constexpr uint32_t kAmRows = 128, kAmRank = 64, kAmPart = kAmRows * 128;      // rows of a block, rank values, bytes of a part of 128 rows of 64 values
+template <typename WT> struct AmParts { static constexpr uint32_t n = sizeof(WT) == 2 ? 1 : 3; };      // of the weights: bfloat16 ones are one part themselves
+template <typename WT> constexpr uint32_t kAmRuns = sizeof(WT) == 2 ? 4 : 2;
+// products, small ones first: {part of x, part of w}
+template <typename WT> struct AmProducts { static constexpr uint32_t n = sizeof(WT) == 2 ? 3 : 6; };
+template <typename WT> __device__ constexpr uint32_t am_x(uint32_t i) { return sizeof(WT) == 2 ? 2 - i : i == 0 ? 2 : i == 1 || i == 3 ? 1 : 0; }
+template <typename WT> __device__ constexpr uint32_t am_w(uint32_t i) { return sizeof(WT) == 2 ? 0 : i == 0 || i == 3 || i == 5 ? 0 : i == 1 || i == 4 ? 1 : 2; }
+// byte of piece c (16 bytes) of a row of 128 bytes in a K-major, 128-byte swizzled operand
+__device__ __forceinline__ uint32_t am_at(uint32_t row, uint32_t c) { return row * 128 + ((c ^ (row & 7)) << 4); }
+__device__ __forceinline__ uint32_t am_idesc(uint32_t n) { return (1u << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((128u >> 4) << 24); }      // bf16 x bf16 -> f32, 128 rows
+// eight f32 values as 16 bytes of each of three parts
+__device__ __forceinline__ void am_split(const float4 x, const float4 y, uint4 (&p)[3]) {
+    split3(x.x, x.y, p[0].x, p[1].x, p[2].x); split3(x.z, x.w, p[0].y, p[1].y, p[2].y);
+    split3(y.x, y.y, p[0].z, p[1].z, p[2].z); split3(y.z, y.w, p[0].w, p[1].w, p[2].w);
+}
+__device__ __forceinline__ void am_proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+template <typename WT> struct AsLayout {
+    static constexpr uint32_t weights = kAmRank * 128, w_run = AmParts<WT>::n * weights, stage = 3 * kAmPart + kAmRuns<WT> * w_run;
+    static constexpr uint32_t which = 2 * stage, bars = which + kAmRows * 4, size = bars + 64 + 1024;
+    static constexpr uint32_t width = kAmRank + 1;                   // of the partial sums, which take the first stage's place in the end
+    static_assert(kAmRows * width * 4 <= stage, "partial sums");
+};
+template <typename WT>
+__global__ void __launch_bounds__(256, 1) __cluster_dims__(kAfCluster, 1, 1) k_adapter_shrink(AdArgs a, const WT* __restrict__ wa, uint4* __restrict__ parts) {
+    typedef AsLayout<WT> L;
+    extern __shared__ uint8_t am_raw[];
+    const uint32_t base = (smem_u32(am_raw) + 1023u) & ~1023u;
+    uint8_t* const mem = am_raw + (base - smem_u32(am_raw));
+    const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, share = blockIdx.x % kAfCluster, r0 = blockIdx.x / kAfCluster * kAmRows;
+    int* const which = reinterpret_cast<int*>(mem + L::which);
+    const uint32_t done = base + L::bars, tmem_slot = done + 16;
+    if (threadIdx.x == 0) {
+        mbar_init(done, 1); mbar_init(done + 8, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" ::"r"(tmem_slot) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const BatchHead head = batch_head(a.table, a.B);
+    if (threadIdx.x < kAmRows) which[threadIdx.x] = r0 + threadIdx.x < a.B ? ad_of(a, head, r0 + threadIdx.x) : kAdIdle;
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(mem + (tmem_slot - base));
+    const uint32_t chunks = (a.K + 63) / 64, per = (chunks + kAfCluster - 1) / kAfCluster, c0 = min(chunks, share * per), n = min(chunks, c0 + per) - c0;
+    // thread: piece c (8 inputs) of rows p, p + 32, p + 64, p + 96 of x; of row p (and p + 32) of the weights
+    const uint32_t c = threadIdx.x & 7, p = threadIdx.x >> 3;
+    uint32_t uses = 0;                                               // chunks that have gone through the stages: use u takes stage u & 1
+    bool ok = true;
+    for (uint32_t at = 0; at < kAmRows;) {
+        // the next adapters of the block, a run of rows each
+        uint32_t run_at[kAmRuns<WT>], runs = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < kAmRuns<WT>; i++) {
+            while (at < kAmRows && which[at] < 0) at++;
+            run_at[i] = at;
+            if (at >= kAmRows) continue;
+            runs = i + 1;
+            const int mine = which[at];
+            while (at < kAmRows && which[at] == mine) at++;
+        }
+        if (!runs) break;
+        float4 x[4][2];
+        auto load = [&](uint32_t t) {
+            const uint32_t k = (c0 + t) * 64 + 8 * c;                // K is a multiple of eight here
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t row = p + 32 * i;
+                const bool on = t < n && k < a.K && which[row] >= 0;
+                const float* from = a.src + (size_t)(r0 + row) * a.src_rs + k;
+                x[i][0] = on ? *reinterpret_cast<const float4*>(from) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                x[i][1] = on ? *reinterpret_cast<const float4*>(from + 4) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+        };
+        load(0);
+#pragma unroll 1
+        for (uint32_t t = 0; t < n; t++, uses++) {
+            const uint32_t s = uses & 1, stage = base + s * L::stage, k = (c0 + t) * 64 + 8 * c;
+            uint8_t* const out = mem + s * L::stage;
+            if (uses >= 2 && ok) ok = __all_sync(0xffffffffu, mbar_wait(done + 8 * s, ((uses >> 1) - 1) & 1));
+#pragma unroll
+            for (uint32_t i = 0; i < kAmRuns<WT>; i++) {
+                if (i >= runs) break;
+                const WT* from = wa + (size_t)which[run_at[i]] * a.rank * a.K + k;
+#pragma unroll
+                for (uint32_t j = p; j < kAmRank; j += 32) {
+                    const bool on = j < a.rank && k < a.K;
+                    const uint32_t to = 3 * kAmPart + i * L::w_run + am_at(j, c);
+                    if constexpr (sizeof(WT) == 2) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(stage + to), "l"(on ? from + (size_t)j * a.K : wa), "r"(on ? 16 : 0) : "memory");
+                    else {
+                        uint4 w[3];
+                        const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        const float* row = reinterpret_cast<const float*>(from) + (size_t)j * a.K;
+                        am_split(on ? *reinterpret_cast<const float4*>(row) : zero, on ? *reinterpret_cast<const float4*>(row + 4) : zero, w);
+#pragma unroll
+                        for (int y = 0; y < 3; y++) *reinterpret_cast<uint4*>(out + to + y * L::weights) = w[y];
+                    }
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                uint4 w[3];
+                am_split(x[i][0], x[i][1], w);
+#pragma unroll
+                for (int y = 0; y < 3; y++) *reinterpret_cast<uint4*>(out + y * kAmPart + am_at(p + 32 * i, c)) = w[y];
+            }
+            load(t + 1);
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            am_proxy_fence();
+            __syncthreads();
+            if (warp == 0) {
+                const uint32_t d = tmem, xa = desc_low(stage), w0 = desc_low(stage + 3 * kAmPart), idesc = am_idesc(kAmRank);
+                fence_after();
+                if (elect_one() && ok) {
+                    for (uint32_t i = 0; i < runs; i++) {
+#pragma unroll
+                        for (uint32_t y = 0; y < AmProducts<WT>::n; y++)
+#pragma unroll
+                            for (uint32_t z = 0; z < 4; z++) {
+                                const uint32_t xs = xa + am_x<WT>(y) * (kAmPart >> 4) + 2 * z, ws = w0 + (i * L::w_run + am_w<WT>(y) * L::weights) / 16 + 2 * z;
+                                if (t == 0 && y == 0 && z == 0) mma_ss<false>(d + i * kAmRank, xs, ws, idesc); else mma_ss<true>(d + i * kAmRank, xs, ws, idesc);
+                            }
+                    }
+                    mma_commit(done + 8 * s);
+                }
+                __syncwarp();
+            }
+        }
+        // all products of these runs are there; their sums take the first stage's place
+        if (n && ok) ok = __all_sync(0xffffffffu, mbar_wait(done + 8 * ((uses - 1) & 1), ((uses - 1) >> 1) & 1));
+        fence_after();
+        __syncthreads();
+        float* const sums = reinterpret_cast<float*>(mem);           // [128][width]
+        const uint32_t row = (warp & 3) * 32 + lane, col = 32 * (warp >> 2), first = run_at[0], last = at;
+#pragma unroll 1
+        for (uint32_t i = 0; i < runs; i++) {
+            uint32_t v[32];
+            tmem_ld(tmem + (((warp & 3) * 32) << 16) + i * kAmRank + col, v);
+            tmem_wait_ld(v);
+            if (row >= run_at[i] && row < last && which[row] == which[run_at[i]] && (i + 1 >= runs || row < run_at[i + 1])) {
+#pragma unroll
+                for (int y = 0; y < 32; y++) sums[row * L::width + col + y] = !ok ? kBatchNaN : n ? __uint_as_float(v[y]) : 0.0f;
+            }
+        }
+        fence_before();
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        // this CTA's sixteen rows: four rank values a thread
+        {
+            const uint32_t mine = share * (kAmRows / kAfCluster) + (threadIdx.x >> 4), j = 4 * (threadIdx.x & 15);
+            if (mine >= first && mine < last && which[mine] >= 0) {
+                float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                const uint32_t from = smem_u32(sums + mine * L::width + j);
+                for (uint32_t e = 0; e < kAfCluster; e++) {
+                    uint32_t there;
+                    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(from), "r"(e));
+#pragma unroll
+                    for (int y = 0; y < 4; y++) {
+                        float w;
+                        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(w) : "r"(there + 4 * y) : "memory");
+                        v[y] += w;
+                    }
+                }
+                const float f = a.scales ? a.scales[which[mine]] : 1.0f;
+                uint2 w[3];
+                split3(v[0] * f, v[1] * f, w[0].x, w[1].x, w[2].x);
+                split3(v[2] * f, v[3] * f, w[0].y, w[1].y, w[2].y);
+#pragma unroll
+                for (int y = 0; y < 3; y++) reinterpret_cast<uint2*>(parts)[((size_t)y * a.B + r0 + mine) * (kAmRank / 4) + j / 4] = w[y];
+            }
+        }
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
+    if (!ok && threadIdx.x == 0) count_timeout();
+    __syncthreads();
+    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem) : "memory");
+}
+
+constexpr uint32_t kAxThreads = 640, kAxWriters = 512;
+template <typename WT> struct AxLayout {
+    static constexpr uint32_t stages = sizeof(WT) == 2 ? 3 : 2, stage = AmParts<WT>::n * kAmPart, ring = 3 * kAmPart, turn = ring + stages * stage;      // turn: 32 x 33 floats a writing warp
+    static constexpr uint32_t which = turn + 16 * 32 * 33 * 4, bars = which + kAmRows * 4, size = bars + 128 + 1024;
+};
+// CTA (share of the outputs, block of 128 rows)
+template <typename WT>
+__global__ void __launch_bounds__(kAxThreads, 1) k_adapter_expand(AdArgs a, const WT* __restrict__ wb, const uint4* __restrict__ parts, uint32_t quads) {
+    typedef AxLayout<WT> L;
+    extern __shared__ uint8_t am_raw[];
+    const uint32_t base = (smem_u32(am_raw) + 1023u) & ~1023u;
+    uint8_t* const mem = am_raw + (base - smem_u32(am_raw));
+    const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, r0 = blockIdx.y * kAmRows;
+    int* const which = reinterpret_cast<int*>(mem + L::which);
+    const uint32_t full = base + L::bars, empty = full + 8 * L::stages, sum_full = empty + 8 * L::stages, sum_empty = sum_full + 16, tmem_slot = sum_empty + 16;
+    if (threadIdx.x == 0) {
+        for (uint32_t i = 0; i < L::stages; i++) { mbar_init(full + 8 * i, 4); mbar_init(empty + 8 * i, 1); }
+        for (uint32_t i = 0; i < 2; i++) { mbar_init(sum_full + 8 * i, 1); mbar_init(sum_empty + 8 * i, 16); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 16) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" ::"r"(tmem_slot) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const BatchHead head = batch_head(a.table, a.B);
+    if (threadIdx.x < kAmRows) which[threadIdx.x] = r0 + threadIdx.x < a.B ? ad_of(a, head, r0 + threadIdx.x) : kAdIdle;
+    // the rows' rank values; those of rows without any are whatever was there: their outputs are left out
+    for (uint32_t i = threadIdx.x; i < 3 * kAmRows * 8; i += kAxThreads) {
+        const uint32_t y = i / (kAmRows * 8), row = i / 8 % kAmRows, c = i % 8;
+        const bool on = r0 + row < a.B;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(base + y * kAmPart + am_at(row, c)), "l"(on ? parts + ((size_t)y * a.B + r0 + row) * 8 + c : parts), "r"(on ? 16 : 0) : "memory");
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    am_proxy_fence();
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(mem + (tmem_slot - base));
+    const uint32_t tiles = (a.N + 127) / 128, per = (tiles + gridDim.x - 1) / gridDim.x, t0 = min(tiles, blockIdx.x * per), n = min(tiles, t0 + per) - t0;
+    bool ok = true;
+    if (warp >= 16) {
+        // bring weights, issue: the tiles of one run of rows after the other's
+        const uint32_t id = threadIdx.x - kAxWriters;                // piece id & 7 of rows id / 8 + 16 i
+        uint32_t slot = 0, phase = 1, at_slot = 0, at_phase = 0, item = 0;
+        auto fill = [&](int run, uint32_t t) {                       // the next stage
+            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * slot, phase));
+            const uint32_t c = id & 7;
+#pragma unroll
+            for (uint32_t i = 0; i < 8; i++) {
+                const uint32_t row = (id >> 3) + 16 * i, o = (t0 + t) * 128 + row;
+                const uint32_t to = L::ring + slot * L::stage + am_at(row, c);
+                const bool on = o < a.N && 8 * c < a.rank;           // the rank is a multiple of eight here
+                const WT* from = on ? wb + ((size_t)run * a.N + o) * a.rank + 8 * c : wb;
+                if constexpr (sizeof(WT) == 2) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(base + to), "l"(from), "r"(on ? 16 : 0) : "memory");
+                else {
+                    uint4 w[3];
+                    const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    am_split(on ? *reinterpret_cast<const float4*>(from) : zero, on ? *reinterpret_cast<const float4*>(from + 4) : zero, w);
+#pragma unroll
+                    for (int y = 0; y < 3; y++) *reinterpret_cast<uint4*>(mem + to + y * kAmPart) = w[y];
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            if (++slot == L::stages) { slot = 0; phase ^= 1; }
+        };
+        for (uint32_t i = 0; i < kAmRows;) {
+            const int run = which[i];
+            while (i < kAmRows && which[i] == run) i++;
+            if (run < 0 || !n) continue;
+            fill(run, 0);
+            for (uint32_t t = 0; t < n; t++, item++) {
+                if (t + 1 < n) { fill(run, t + 1); asm volatile("cp.async.wait_group 1;" ::: "memory"); }
+                else asm volatile("cp.async.wait_group 0;" ::: "memory");
+                am_proxy_fence();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(full + 8 * at_slot);
+                if (warp == 16) {
+                    const uint32_t d = tmem + (item & 1) * 128, xa = desc_low(base), w0 = desc_low(base + L::ring) + at_slot * (L::stage >> 4), freed = empty + 8 * at_slot, idesc = am_idesc(128);
+                    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(full + 8 * at_slot, at_phase));
+                    if (ok && item >= 2) ok = __all_sync(0xffffffffu, mbar_wait(sum_empty + 8 * (item & 1), ((item >> 1) - 1) & 1));
+                    fence_after();
+                    if (elect_one() && ok) {
+#pragma unroll
+                        for (uint32_t y = 0; y < AmProducts<WT>::n; y++)
+#pragma unroll
+                            for (uint32_t z = 0; z < 4; z++) {
+                                const uint32_t xs = xa + am_x<WT>(y) * (kAmPart >> 4) + 2 * z, ws = w0 + am_w<WT>(y) * (kAmPart >> 4) + 2 * z;
+                                if (y == 0 && z == 0) mma_ss<false>(d, xs, ws, idesc); else mma_ss<true>(d, xs, ws, idesc);
+                            }
+                        mma_commit(sum_full + 8 * (item & 1));
+                        mma_commit(freed);
+                    }
+                    __syncwarp();
+                }
+                if (++at_slot == L::stages) { at_slot = 0; at_phase ^= 1; }
+            }
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+    } else {
+        // add the base, write: a block of 32 rows and 32 outputs a warp; lanes hold a row each of the sums, and by way of shared memory an eighth of four rows each
+        const uint32_t row0 = (warp & 3) * 32, col0 = 32 * (warp >> 2), lr = lane >> 3, lc = 4 * (lane & 7);
+        float* const turn = reinterpret_cast<float*>(mem + L::turn) + warp * 32 * 33;
+        uint32_t item = 0;
+        for (uint32_t i = 0; i < kAmRows;) {
+            const int run = which[i];
+            const uint32_t first = i;
+            while (i < kAmRows && which[i] == run) i++;
+            if (run == kAdIdle || (run == kAdNone && a.base == a.dst) || !n) continue;
+            const bool here = first < row0 + 32 && i > row0;         // the run reaches this warp's rows
+            for (uint32_t t = 0; t < n; t++) {
+                const uint32_t o = (t0 + t) * 128 + col0 + lc;
+                float4 b[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const uint32_t row = row0 + 4 * e + lr;
+                    b[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (!here || row < first || row >= i) continue;
+                    const float* from = a.base + (size_t)(r0 + row) * a.base_rs + o;
+                    if (quads && o + 4 <= a.N) b[e] = *reinterpret_cast<const float4*>(from);
+                    else { if (o < a.N) b[e].x = from[0]; if (o + 1 < a.N) b[e].y = from[1]; if (o + 2 < a.N) b[e].z = from[2]; if (o + 3 < a.N) b[e].w = from[3]; }
+                }
+                if (run >= 0) {
+                    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(sum_full + 8 * (item & 1), (item >> 1) & 1));
+                    fence_after();
+                    if (here) {
+                        uint32_t v[32];
+                        tmem_ld(tmem + (row0 << 16) + (item & 1) * 128 + col0, v);
+                        tmem_wait_ld(v);
+#pragma unroll
+                        for (int e = 0; e < 32; e++) turn[lane * 33 + e] = ok ? __uint_as_float(v[e]) : kBatchNaN;
+                    }
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(sum_empty + 8 * (item & 1));
+                    item++;
+                }
+                if (here) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const uint32_t row = row0 + 4 * e + lr;
+                        if (row < first || row >= i) continue;
+                        float4 v = b[e];
+                        if (run >= 0) {
+                            const float* s = turn + (4 * e + lr) * 33 + lc;
+                            v.x += s[0]; v.y += s[1]; v.z += s[2]; v.w += s[3];
+                        } else if (run == kAdBad) v = make_float4(kBatchNaN, kBatchNaN, kBatchNaN, kBatchNaN);
+                        float* to = a.dst + (size_t)(r0 + row) * a.dst_rs + o;
+                        if (quads && o + 4 <= a.N) *reinterpret_cast<float4*>(to) = v;
+                        else { if (o < a.N) to[0] = v.x; if (o + 1 < a.N) to[1] = v.y; if (o + 2 < a.N) to[2] = v.z; if (o + 3 < a.N) to[3] = v.w; }
+                    }
+                }
+                __syncwarp();
+            }
+        }
+    }
+    if (!ok && lane == 0) count_timeout();
+    __syncwarp();
+    fence_before();
+    __syncthreads();
+    if (warp == 16) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem) : "memory");
+}
+
+// More rows than kAmLeast go in blocks, where rank and strides allow their 16-byte pieces.
+constexpr uint32_t kAmLeast = 256;
+bool many_rows(const ZgSeqOp& s) {
+    const uint32_t B = s.n[0], K = s.n[2], rank = s.n[3];
+    return B > kAmLeast && K % 8 == 0 && rank % 8 == 0 && rank <= kAmRank && s.n[5] % 4 == 0 && s.off[2] % 4 == 0 && s.off[0] % 8 == 0 && s.off[1] % 8 == 0;
+}
+template <typename WT>
+bool launch_few(const AdArgs& a, const WT* wa, const WT* wb, cudaStream_t st) {
+    auto aligned = [](const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; };
+    const uint32_t V = WVec<WT>::n, k_slice = ((a.K + kAfCluster - 1) / kAfCluster + V - 1) / V * V, n_slice = ((a.N + kAfCluster - 1) / kAfCluster + 7) / 8 * 8;
+    const uint32_t vec_k = a.K % V == 0 && a.src_rs % 4 == 0 && aligned(wa, 16) && aligned(a.src, 16);
+    const uint32_t vec_j = a.rank % 4 == 0 && aligned(wb, 4 * sizeof(WT));
+    // A slice begins at n_slice rank weights from the adapter's, which is N rank from the next one's
+    const size_t bytes = (size_t)n_slice * a.rank * sizeof(WT);
+    const uint32_t stage = bytes <= kAfStage && aligned(wb, 16) && (size_t)a.N * a.rank * sizeof(WT) % 16 == 0 ? (uint32_t)((bytes + 15) & ~(size_t)15) : 0;
+    const size_t smem = stage + 2 * kAfRows * sizeof(float) * ((a.rank + 3) / 4 * 4);
+    if (!zg_smem_limit<k_adapter_few<WT>>(kAfStage + 2 * kAfRows * sizeof(float) * 1024)) return false;
+    launch_pdl(k_adapter_few<WT>, dim3(a.B * kAfCluster), dim3(kAfThreads), smem, st, a, wa, wb, k_slice, n_slice, vec_k, vec_j, stage);
+    return true;
+}
+template <typename WT>
+bool launch_many(const AdArgs& a, const WT* wa, const WT* wb, float* parts, cudaStream_t st) {
+    if (!zg_smem_limit<k_adapter_shrink<WT>>(AsLayout<WT>::size) || !zg_smem_limit<k_adapter_expand<WT>>(AxLayout<WT>::size)) return false;
+    const uint32_t blocks = (a.B + kAmRows - 1) / kAmRows, tiles = (a.N + 127) / 128;
+    launch_pdl(k_adapter_shrink<WT>, dim3(blocks * kAfCluster), dim3(256), AsLayout<WT>::size, st, a, wa, reinterpret_cast<uint4*>(parts));
+    ZG_COUNT_LAUNCH();
+    const uint32_t quads = a.dst_rs % 4 == 0 && a.base_rs % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.dst) | reinterpret_cast<uintptr_t>(a.base)) & 15) == 0;
+    launch_pdl(k_adapter_expand<WT>, dim3(std::max(1u, std::min(tiles, zg_sm_count() / blocks)), blocks), dim3(kAxThreads), AxLayout<WT>::size, st, a, wb, reinterpret_cast<const uint4*>(parts), quads);
+    return true;
+}
+
+}  // namespace
+
+bool zg_adapter_linear_valid(const ZgSeqOp& s, const size_t* elems, size_t n_bufs, char* why, size_t why_n) {
+    auto fail = [&](const char* m) { snprintf(why, why_n, "%s", m); return false; };
+    auto have = [&](int i) { return s.buf[i] != ZG_NO_BUF && s.buf[i] < n_bufs; };
+    auto fits = [&](int i, size_t off, size_t n) { return have(i) && off + n <= elems[s.buf[i]]; };
+    auto wfits = [&](int i, uint32_t wdt, size_t off, size_t n) { return wdt <= ZG_W_BF16 && have(i) && (wdt == ZG_W_BF16 ? (off + n + 1) / 2 : off + n) <= elems[s.buf[i]]; };
+    const size_t B = s.n[0], N = s.n[1], K = s.n[2], rank = s.n[3], A = s.n[4], srs = s.n[5], drs = s.n[6], brs = s.n[8];
+    if (!B || !N || !K || !rank || !A || B > 65536 || rank > 1024) return fail("adapter_linear: shape");
+    if ((B > 1 && (srs < K || drs < N || brs < N)) || !fits(0, s.off[3], (B - 1) * drs + N) || !fits(1, s.off[2], (B - 1) * srs + K) || !fits(5, s.off[5], (B - 1) * brs + N)) return fail("adapter_linear: rows");
+    if (!wfits(2, s.n[7], s.off[0], A * rank * K) || !wfits(2, s.n[7], s.off[1], A * rank * N)) return fail("adapter_linear: weights");
+    if (s.buf[3] != ZG_NO_BUF && !fits(3, s.off[4], A)) return fail("adapter_linear: scales");
+    if (!fits(4, 0, ZG_BATCH_ROWS + 4 * B)) return fail("adapter_linear: table");
+    if (s.buf[0] == s.buf[1] || s.buf[0] == s.buf[2] || s.buf[0] == s.buf[3] || s.buf[0] == s.buf[4]) return fail("adapter_linear: in place");
+    if (s.buf[0] == s.buf[5] && (s.off[3] != s.off[5] || drs != brs)) return fail("adapter_linear: a base that overlaps the destination has to be the destination");
+    return true;
+}
+size_t zg_adapter_linear_scratch_elems(const ZgSeqOp& s) { return many_rows(s) ? (size_t)3 * s.n[0] * kAmRank / 2 : 0; }      // rank values in three bfloat16 parts
+bool zg_launch_adapter_linear(const ZgOp& op, float* const* bufs, float* scratch, cudaStream_t st) {
+    const ZgSeqOp& s = op.u.seq;
+    AdArgs a;
+    a.dst = bufs[s.buf[0]] + s.off[3]; a.src = bufs[s.buf[1]] + s.off[2]; a.base = bufs[s.buf[5]] + s.off[5]; a.scales = s.buf[3] != ZG_NO_BUF ? bufs[s.buf[3]] + s.off[4] : nullptr; a.table = bufs[s.buf[4]];
+    a.B = s.n[0]; a.N = s.n[1]; a.K = s.n[2]; a.rank = s.n[3]; a.adapters = s.n[4]; a.src_rs = s.n[5]; a.dst_rs = s.n[6]; a.base_rs = s.n[8];
+    bool ok = false;
+    const bool many = scratch && many_rows(s);
+    ZG_SEQ_WDT(s.n[7], ok = many ? launch_many<WT>(a, wptr<WT>(bufs, s.buf[2], s.off[0]), wptr<WT>(bufs, s.buf[2], s.off[1]), scratch, st)
+                                 : launch_few<WT>(a, wptr<WT>(bufs, s.buf[2], s.off[0]), wptr<WT>(bufs, s.buf[2], s.off[1]), st));
+    if (!ok) return false;
+    ZG_SEQ_CHECK();
+    return true;
+}
+unsigned int zg_adapter_timeouts() { return tc_timeouts(); }

@@ -1,5 +1,5 @@
-// Sequence-model DeviceOps of a step that advances many requests at once (parameter packs in include/zgml_cuda.h): BATCH_APPEND, ADAPTER_LINEAR and LOGIT_RULES;
-// SHARED_ATTENTION has a file of its own.  What distinguishes the rows - slot, length, adapter, rules - lies in a table that the host rewrites between
+// Sequence-model DeviceOps of a step that advances many requests at once (parameter packs in include/zgml_cuda.h): BATCH_APPEND and LOGIT_RULES;
+// SHARED_ATTENTION and ADAPTER_LINEAR have files of their own.  What distinguishes the rows - slot, length, adapter, rules - lies in a table that the host rewrites between
 // executions of one captured program.
 #include "batch_table.cuh"
 
@@ -57,45 +57,6 @@ __global__ void __launch_bounds__(256) k_batch_append(BaArgs a) {
         float* out = a.turned + (size_t)r * a.dst_rs + a.dst_col;
         const float* p = src + a.q_col;
         for (uint32_t c = threadIdx.x; c < a.q_heads * a.dim; c += blockDim.x) out[c] = ok ? value(p + c / a.dim * a.dim, c % a.dim) : kBatchNaN;
-    }
-}
-
-// ── ADAPTER_LINEAR ───────────────────────────────────────────────────────────────────────────────────────────────────
-struct AdArgs {
-    float* dst; const float* src; const float* base; const float* scales; const float* table;
-    uint32_t B, N, K, rank, adapters, src_rs, dst_rs, base_rs;
-};
-// CTA (row, share of the outputs): the row's rank values h = A x in shared memory, then its outputs
-template <typename WT>
-__global__ void __launch_bounds__(256) k_adapter_rows(AdArgs a, const WT* __restrict__ wa, const WT* __restrict__ wb, uint32_t share) {
-    pdl_enter();
-    extern __shared__ float h[];
-    const uint32_t r = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const BatchHead head = batch_head(a.table, a.B);
-    const BatchRow w = batch_row(a.table, r);
-    if (r >= head.rows || w.slot < 0) return;
-    const uint32_t n0 = blockIdx.y * share, n1 = min(a.N, n0 + share);
-    const float* base = a.base + (size_t)r * a.base_rs;
-    float* dst = a.dst + (size_t)r * a.dst_rs;
-    if (w.adapter < 0 || (uint32_t)w.adapter >= a.adapters) {
-        for (uint32_t n = n0 + threadIdx.x; n < n1; n += 256) dst[n] = w.adapter < 0 ? base[n] : kBatchNaN;
-        return;
-    }
-    const float* x = a.src + (size_t)r * a.src_rs;
-    const float scale = a.scales ? a.scales[w.adapter] : 1.0f;
-    for (uint32_t j = warp; j < a.rank; j += 8) {
-        const WT* row = wa + ((size_t)w.adapter * a.rank + j) * a.K;
-        float s = 0.0f;
-        for (uint32_t k = lane; k < a.K; k += 32) s = fmaf(wld(row, k), x[k], s);
-        s = warp_sum(s);
-        if (lane == 0) h[j] = s * scale;
-    }
-    __syncthreads();
-    for (uint32_t n = n0 + threadIdx.x; n < n1; n += 256) {
-        const WT* row = wb + ((size_t)w.adapter * a.N + n) * a.rank;
-        float s = 0.0f;
-        for (uint32_t j = 0; j < a.rank; j++) s = fmaf(wld(row, j), h[j], s);
-        dst[n] = base[n] + s;
     }
 }
 
@@ -176,7 +137,6 @@ bool zg_batch_op_valid(const ZgOp& op, const size_t* elems, size_t n_bufs, char*
     auto fail = [&](const char* m) { snprintf(why, why_n, "%s", m); return false; };
     auto have = [&](int i) { return s.buf[i] != ZG_NO_BUF && s.buf[i] < n_bufs; };
     auto fits = [&](int i, size_t off, size_t n) { return have(i) && off + n <= elems[s.buf[i]]; };
-    auto wfits = [&](int i, uint32_t wdt, size_t off, size_t n) { return wdt <= ZG_W_BF16 && have(i) && (wdt == ZG_W_BF16 ? (off + n + 1) / 2 : off + n) <= elems[s.buf[i]]; };
     switch (op.tag) {
         case ZG_OP_BATCH_APPEND: {
             const size_t B = s.n[0], cols = s.n[1], srs = s.n[2], width = s.n[3], R = s.n[4], heads = s.n[5], dim = s.n[6], rot = s.n[8], q_heads = s.n[10];
@@ -194,17 +154,7 @@ bool zg_batch_op_valid(const ZgOp& op, const size_t* elems, size_t n_bufs, char*
             return true;
         }
         case ZG_OP_SHARED_ATTENTION: return zg_shared_attention_valid(s, elems, n_bufs, why, why_n);
-        case ZG_OP_ADAPTER_LINEAR: {
-            const size_t B = s.n[0], N = s.n[1], K = s.n[2], rank = s.n[3], A = s.n[4], srs = s.n[5], drs = s.n[6], brs = s.n[8];
-            if (!B || !N || !K || !rank || !A || B > 65536 || rank > 1024) return fail("adapter_linear: shape");
-            if ((B > 1 && (srs < K || drs < N || brs < N)) || !fits(0, s.off[3], (B - 1) * drs + N) || !fits(1, s.off[2], (B - 1) * srs + K) || !fits(5, s.off[5], (B - 1) * brs + N)) return fail("adapter_linear: rows");
-            if (!wfits(2, s.n[7], s.off[0], A * rank * K) || !wfits(2, s.n[7], s.off[1], A * rank * N)) return fail("adapter_linear: weights");
-            if (s.buf[3] != ZG_NO_BUF && !fits(3, s.off[4], A)) return fail("adapter_linear: scales");
-            if (!fits(4, 0, ZG_BATCH_ROWS + 4 * B)) return fail("adapter_linear: table");
-            if (s.buf[0] == s.buf[1] || s.buf[0] == s.buf[2] || s.buf[0] == s.buf[3] || s.buf[0] == s.buf[4]) return fail("adapter_linear: in place");
-            if (s.buf[0] == s.buf[5] && (s.off[3] != s.off[5] || drs != brs)) return fail("adapter_linear: a base that overlaps the destination has to be the destination");
-            return true;
-        }
+        case ZG_OP_ADAPTER_LINEAR: return zg_adapter_linear_valid(s, elems, n_bufs, why, why_n);
         case ZG_OP_LOGIT_RULES: {
             const size_t B = s.n[0], V = s.n[1], srs = s.n[2], drs = s.n[3], Rh = s.n[4];
             if (!B || !V || B > 65535 || V >= (1u << 31) || Rh >= (1u << 31)) return fail("logit_rules: shape");
@@ -221,7 +171,9 @@ bool zg_batch_op_valid(const ZgOp& op, const size_t* elems, size_t n_bufs, char*
     }
 }
 uint32_t zg_batch_op_writes(uint32_t tag) { return tag == ZG_OP_BATCH_APPEND ? 1u | (1u << 4) : 1u; }      // the cache and the turned query heads
-size_t zg_batch_op_scratch_elems(const ZgOp& op) { return op.tag == ZG_OP_SHARED_ATTENTION ? zg_shared_attention_scratch_elems(op.u.seq) : 0; }
+size_t zg_batch_op_scratch_elems(const ZgOp& op) {
+    return op.tag == ZG_OP_SHARED_ATTENTION ? zg_shared_attention_scratch_elems(op.u.seq) : op.tag == ZG_OP_ADAPTER_LINEAR ? zg_adapter_linear_scratch_elems(op.u.seq) : 0;
+}
 
 bool zg_launch_batch_op(const ZgOp& op, float* const* bufs, const size_t* elems, float* scratch, cudaStream_t st) {
     const ZgSeqOp& s = op.u.seq;
@@ -241,16 +193,7 @@ bool zg_launch_batch_op(const ZgOp& op, float* const* bufs, const size_t* elems,
             return true;
         }
         case ZG_OP_SHARED_ATTENTION: return zg_launch_shared_attention(op, bufs, elems, scratch, st);
-        case ZG_OP_ADAPTER_LINEAR: {
-            AdArgs a;
-            a.dst = bufs[s.buf[0]] + s.off[3]; a.src = bufs[s.buf[1]] + s.off[2]; a.base = bufs[s.buf[5]] + s.off[5]; a.scales = s.buf[3] != ZG_NO_BUF ? bufs[s.buf[3]] + s.off[4] : nullptr; a.table = bufs[s.buf[4]];
-            a.B = s.n[0]; a.N = s.n[1]; a.K = s.n[2]; a.rank = s.n[3]; a.adapters = s.n[4]; a.src_rs = s.n[5]; a.dst_rs = s.n[6]; a.base_rs = s.n[8];
-            const uint32_t share = 1024;
-            ZG_SEQ_WDT(s.n[7], launch_pdl(k_adapter_rows<WT>, dim3(a.B, (a.N + share - 1) / share), dim3(256), a.rank * sizeof(float), st, a, wptr<WT>(bufs, s.buf[2], s.off[0]),
-                                          wptr<WT>(bufs, s.buf[2], s.off[1]), share));
-            ZG_SEQ_CHECK();
-            return true;
-        }
+        case ZG_OP_ADAPTER_LINEAR: return zg_launch_adapter_linear(op, bufs, scratch, st);
         case ZG_OP_LOGIT_RULES: {
             LrArgs a;
             a.dst = bufs[s.buf[0]] + s.off[0]; a.src = bufs[s.buf[1]] + s.off[1]; a.table = bufs[s.buf[2]];

@@ -501,7 +501,7 @@ bool zg_dense_gemm_batched_launch(const void* w_bf16, const float* src, float* d
 // streamops.cu : ZG_OP_STREAM_STEP
 bool zg_stream_op_valid(const ZgOp& op, const size_t* elems, size_t n_bufs, char* why, size_t why_n);
 bool zg_launch_stream_op(const ZgOp& op, float* const* bufs, cudaStream_t st, bool const_weights);
-// batchops.cu : ZG_OP_BATCH_APPEND .. ZG_OP_LOGIT_RULES, reached through the functions above; shared_attention.cu : ZG_OP_SHARED_ATTENTION
+// batchops.cu : ZG_OP_BATCH_APPEND .. ZG_OP_LOGIT_RULES, reached through the functions above; shared_attention.cu : ZG_OP_SHARED_ATTENTION; adapter.cu : ZG_OP_ADAPTER_LINEAR
 bool zg_batch_op_valid(const ZgOp& op, const size_t* elems, size_t n_bufs, char* why, size_t why_n);
 uint32_t zg_batch_op_writes(uint32_t tag);
 size_t zg_batch_op_scratch_elems(const ZgOp& op);
@@ -510,3 +510,7 @@ bool zg_shared_attention_valid(const ZgSeqOp& s, const size_t* elems, size_t n_b
 size_t zg_shared_attention_scratch_elems(const ZgSeqOp& s);
 bool zg_launch_shared_attention(const ZgOp& op, float* const* bufs, const size_t* elems, float* scratch, cudaStream_t st);
 unsigned int zg_shared_attention_timeouts();      // waits that gave up
+bool zg_adapter_linear_valid(const ZgSeqOp& s, const size_t* elems, size_t n_bufs, char* why, size_t why_n);
+size_t zg_adapter_linear_scratch_elems(const ZgSeqOp& s);
+bool zg_launch_adapter_linear(const ZgOp& op, float* const* bufs, float* scratch, cudaStream_t st);
+unsigned int zg_adapter_timeouts();

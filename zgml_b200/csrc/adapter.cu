@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(kAfThreads) __cluster_dims__(kAfCluster, 1, 1)
 // Rows of a block that have another adapter than the product at hand are computed and left out.
 //   k_adapter_shrink: the 8 CTAs of a cluster share a block's inputs.  x is split on its way to shared memory; up to kAmRuns adapters accumulate side by side in TMEM; the
 //   partial sums meet over distributed shared memory and leave as the parts that the second product wants: x is read once.
-//   k_adapter_expand: a CTA keeps the block's rank values and walks tiles of 128 outputs: four warps bring weights and issue, sixteen add the base and write.  Base and dst
+//   k_adapter_expand: a CTA keeps the block's rank values and walks tiles of 128 outputs: four warps bring weights and issue, eight add the base and write.  Base and dst
 //   are what bounds it.
 // (The same on mma.sync took 124 us for 2048 rows of 4096 inputs, 14336 outputs, rank 64, with its issue rate as the bound: 11.3 T operations of products at 130 T/s.)
 // Every wait is bounded; a CTA whose wait ran out counts it and makes NaN of its rows.
@@ -202,11 +202,35 @@ __device__ __forceinline__ void am_split(const float4 x, const float4 y, uint4 (
 }
 __device__ __forceinline__ void am_proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+// Runs of a block's rows: {first row, end, adapter or what else}.  Found by warp 0; `skip` of a run leaves it out.  Everybody waits for it.
+struct AmRun { int first, end, which; };
+template <class Skip>
+__device__ __forceinline__ void am_find_runs(const AdArgs& a, const BatchHead& head, uint32_t r0, int* which, AmRun* runs, uint32_t* count, const Skip& skip) {
+    if (threadIdx.x < kAmRows) which[threadIdx.x] = r0 + threadIdx.x < a.B ? ad_of(a, head, r0 + threadIdx.x) : kAdIdle;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        uint32_t n = 0;
+        int open = -1;                                               // where the run that is not closed yet starts
+        for (uint32_t w = 0; w < kAmRows; w += 32) {
+            const uint32_t i = w + threadIdx.x;
+            uint32_t starts = __ballot_sync(0xffffffffu, i == 0 || which[i] != which[i - 1]);
+            for (; starts; starts &= starts - 1) {
+                const int at = (int)w + __ffs(starts) - 1;
+                if (open >= 0 && !skip(which[open])) { if (threadIdx.x == 0) runs[n] = {open, at, which[open]}; n++; }
+                open = at;
+            }
+        }
+        if (!skip(which[open])) { if (threadIdx.x == 0) runs[n] = {open, (int)kAmRows, which[open]}; n++; }
+        if (threadIdx.x == 0) *count = n;
+    }
+    __syncthreads();
+}
 template <typename WT> struct AsLayout {
-    static constexpr uint32_t weights = kAmRank * 128, w_run = AmParts<WT>::n * weights, stage = 3 * kAmPart + kAmRuns<WT> * w_run;
-    static constexpr uint32_t which = 2 * stage, bars = which + kAmRows * 4, size = bars + 64 + 1024;
+    // weights of bfloat16 sessions come a chunk ahead, through three slots; f32 ones are split as they come, into two
+    static constexpr uint32_t weights = kAmRank * 128, w_run = AmParts<WT>::n * weights, w_slots = sizeof(WT) == 2 ? 3 : 2, w_slot = kAmRuns<WT> * w_run, x_stage = 3 * kAmPart;
+    static constexpr uint32_t w = 2 * x_stage, which = w + w_slots * w_slot, runs = which + kAmRows * 4, bars = runs + kAmRows * 12, size = bars + 64 + 1024;
     static constexpr uint32_t width = kAmRank + 1;                   // of the partial sums, which take the first stage's place in the end
-    static_assert(kAmRows * width * 4 <= stage, "partial sums");
+    static_assert(kAmRows * width * 4 <= x_stage, "partial sums");
 };
 template <typename WT>
 __global__ void __launch_bounds__(256, 1) __cluster_dims__(kAfCluster, 1, 1) k_adapter_shrink(AdArgs a, const WT* __restrict__ wa, uint4* __restrict__ parts) {
@@ -216,7 +240,9 @@ __global__ void __launch_bounds__(256, 1) __cluster_dims__(kAfCluster, 1, 1) k_a
     uint8_t* const mem = am_raw + (base - smem_u32(am_raw));
     const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, share = blockIdx.x % kAfCluster, r0 = blockIdx.x / kAfCluster * kAmRows;
     int* const which = reinterpret_cast<int*>(mem + L::which);
+    AmRun* const all = reinterpret_cast<AmRun*>(mem + L::runs);
     const uint32_t done = base + L::bars, tmem_slot = done + 16;
+    uint32_t* const count = reinterpret_cast<uint32_t*>(mem + L::bars + 24);
     if (threadIdx.x == 0) {
         mbar_init(done, 1); mbar_init(done + 8, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -228,67 +254,67 @@ __global__ void __launch_bounds__(256, 1) __cluster_dims__(kAfCluster, 1, 1) k_a
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const BatchHead head = batch_head(a.table, a.B);
-    if (threadIdx.x < kAmRows) which[threadIdx.x] = r0 + threadIdx.x < a.B ? ad_of(a, head, r0 + threadIdx.x) : kAdIdle;
     fence_before();
-    __syncthreads();
+    am_find_runs(a, head, r0, which, all, count, [](int w) { return w < 0; });
     fence_after();
-    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(mem + (tmem_slot - base));
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(mem + (tmem_slot - base)), n_runs = *count;
     const uint32_t chunks = (a.K + 63) / 64, per = (chunks + kAfCluster - 1) / kAfCluster, c0 = min(chunks, share * per), n = min(chunks, c0 + per) - c0;
     // thread: piece c (8 inputs) of rows p, p + 32, p + 64, p + 96 of x; of row p (and p + 32) of the weights
     const uint32_t c = threadIdx.x & 7, p = threadIdx.x >> 3;
     uint32_t uses = 0;                                               // chunks that have gone through the stages: use u takes stage u & 1
     bool ok = true;
-    for (uint32_t at = 0; at < kAmRows;) {
-        // the next adapters of the block, a run of rows each
-        uint32_t run_at[kAmRuns<WT>], runs = 0;
+    bool x_on[4];
 #pragma unroll
-        for (uint32_t i = 0; i < kAmRuns<WT>; i++) {
-            while (at < kAmRows && which[at] < 0) at++;
-            run_at[i] = at;
-            if (at >= kAmRows) continue;
-            runs = i + 1;
-            const int mine = which[at];
-            while (at < kAmRows && which[at] == mine) at++;
-        }
-        if (!runs) break;
-        float4 x[4][2];
-        auto load = [&](uint32_t t) {
+    for (int i = 0; i < 4; i++) x_on[i] = which[p + 32 * i] >= 0;
+    // as many adapters at a time as accumulate side by side
+    for (uint32_t e0 = 0; e0 < n_runs; e0 += kAmRuns<WT>) {
+        const uint32_t runs = min(kAmRuns<WT>, n_runs - e0);
+        const AmRun* const run = all + e0;
+        const WT* w_from[kAmRuns<WT>];
+#pragma unroll
+        for (uint32_t i = 0; i < kAmRuns<WT>; i++) w_from[i] = wa + (size_t)run[min(i, runs - 1)].which * a.rank * a.K;
+        float4 xa[4][2], xb[4][2];                                   // of the next even and odd chunk
+        auto load = [&](uint32_t t, float4 (&x)[4][2]) {
             const uint32_t k = (c0 + t) * 64 + 8 * c;                // K is a multiple of eight here
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const uint32_t row = p + 32 * i;
-                const bool on = t < n && k < a.K && which[row] >= 0;
-                const float* from = a.src + (size_t)(r0 + row) * a.src_rs + k;
+                const bool on = t < n && k < a.K && x_on[i];
+                const float* from = a.src + (size_t)(r0 + p + 32 * i) * a.src_rs + k;
                 x[i][0] = on ? *reinterpret_cast<const float4*>(from) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 x[i][1] = on ? *reinterpret_cast<const float4*>(from + 4) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             }
         };
-        load(0);
-#pragma unroll 1
-        for (uint32_t t = 0; t < n; t++, uses++) {
-            const uint32_t s = uses & 1, stage = base + s * L::stage, k = (c0 + t) * 64 + 8 * c;
-            uint8_t* const out = mem + s * L::stage;
-            if (uses >= 2 && ok) ok = __all_sync(0xffffffffu, mbar_wait(done + 8 * s, ((uses >> 1) - 1) & 1));
+        auto weights = [&](uint32_t t, uint32_t slot) {
+            const uint32_t k = (c0 + t) * 64 + 8 * c;
+            if (t < n) {
 #pragma unroll
-            for (uint32_t i = 0; i < kAmRuns<WT>; i++) {
-                if (i >= runs) break;
-                const WT* from = wa + (size_t)which[run_at[i]] * a.rank * a.K + k;
+                for (uint32_t i = 0; i < kAmRuns<WT>; i++) {
+                    if (i >= runs) break;
 #pragma unroll
-                for (uint32_t j = p; j < kAmRank; j += 32) {
-                    const bool on = j < a.rank && k < a.K;
-                    const uint32_t to = 3 * kAmPart + i * L::w_run + am_at(j, c);
-                    if constexpr (sizeof(WT) == 2) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(stage + to), "l"(on ? from + (size_t)j * a.K : wa), "r"(on ? 16 : 0) : "memory");
-                    else {
-                        uint4 w[3];
-                        const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                        const float* row = reinterpret_cast<const float*>(from) + (size_t)j * a.K;
-                        am_split(on ? *reinterpret_cast<const float4*>(row) : zero, on ? *reinterpret_cast<const float4*>(row + 4) : zero, w);
+                    for (uint32_t j = p; j < kAmRank; j += 32) {
+                        const bool on = j < a.rank && k < a.K;
+                        const uint32_t to = L::w + slot * L::w_slot + i * L::w_run + am_at(j, c);
+                        const WT* from = on ? w_from[i] + (size_t)j * a.K + k : wa;
+                        if constexpr (sizeof(WT) == 2) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(base + to), "l"(from), "r"(on ? 16 : 0) : "memory");
+                        else {
+                            uint4 w[3];
+                            const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                            am_split(on ? *reinterpret_cast<const float4*>(from) : zero, on ? *reinterpret_cast<const float4*>(from + 4) : zero, w);
 #pragma unroll
-                        for (int y = 0; y < 3; y++) *reinterpret_cast<uint4*>(out + to + y * L::weights) = w[y];
+                            for (int y = 0; y < 3; y++) *reinterpret_cast<uint4*>(mem + to + y * L::weights) = w[y];
+                        }
                     }
                 }
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        uint32_t slot = 0;                                           // of the weights of chunk t
+        auto chunk = [&](uint32_t t, float4 (&x)[4][2]) {
+            const uint32_t s = uses & 1;
+            uint8_t* const out = mem + s * L::x_stage;
+            if (uses >= 2 && ok) ok = __all_sync(0xffffffffu, mbar_wait(done + 8 * s, ((uses >> 1) - 1) & 1));
+            const uint32_t after = slot + 1 == L::w_slots ? 0 : slot + 1;
+            if constexpr (sizeof(WT) == 2) weights(t + 1, after); else weights(t, slot);
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 uint4 w[3];
@@ -296,40 +322,55 @@ __global__ void __launch_bounds__(256, 1) __cluster_dims__(kAfCluster, 1, 1) k_a
 #pragma unroll
                 for (int y = 0; y < 3; y++) *reinterpret_cast<uint4*>(out + y * kAmPart + am_at(p + 32 * i, c)) = w[y];
             }
-            load(t + 1);
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            load(t + 2, x);
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
             am_proxy_fence();
             __syncthreads();
             if (warp == 0) {
-                const uint32_t d = tmem, xa = desc_low(stage), w0 = desc_low(stage + 3 * kAmPart), idesc = am_idesc(kAmRank);
+                const uint32_t xs = desc_low(base) + s * (L::x_stage >> 4), w0 = desc_low(base + L::w) + slot * (L::w_slot >> 4), idesc = am_idesc(kAmRank), freed = done + 8 * s;
                 fence_after();
                 if (elect_one() && ok) {
-                    for (uint32_t i = 0; i < runs; i++) {
+#pragma unroll
+                    for (uint32_t i = 0; i < kAmRuns<WT>; i++) {
+                        if (i >= runs) break;
 #pragma unroll
                         for (uint32_t y = 0; y < AmProducts<WT>::n; y++)
 #pragma unroll
                             for (uint32_t z = 0; z < 4; z++) {
-                                const uint32_t xs = xa + am_x<WT>(y) * (kAmPart >> 4) + 2 * z, ws = w0 + (i * L::w_run + am_w<WT>(y) * L::weights) / 16 + 2 * z;
-                                if (t == 0 && y == 0 && z == 0) mma_ss<false>(d + i * kAmRank, xs, ws, idesc); else mma_ss<true>(d + i * kAmRank, xs, ws, idesc);
+                                const uint32_t xd = xs + am_x<WT>(y) * (kAmPart >> 4) + 2 * z, wd = w0 + (i * L::w_run + am_w<WT>(y) * L::weights) / 16 + 2 * z;
+                                if (y == 0 && z == 0) { if (t == 0) mma_ss<false>(tmem + i * kAmRank, xd, wd, idesc); else mma_ss<true>(tmem + i * kAmRank, xd, wd, idesc); }
+                                else mma_ss<true>(tmem + i * kAmRank, xd, wd, idesc);
                             }
                     }
-                    mma_commit(done + 8 * s);
+                    mma_commit(freed);
                 }
                 __syncwarp();
             }
+            slot = after;
+            uses++;
+        };
+        load(0, xa);
+        load(1, xb);
+        if constexpr (sizeof(WT) == 2) weights(0, 0);
+#pragma unroll 1
+        for (uint32_t t = 0; t < n; t += 2) {
+            chunk(t, xa);
+            if (t + 1 < n) chunk(t + 1, xb);
         }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
         // all products of these runs are there; their sums take the first stage's place
         if (n && ok) ok = __all_sync(0xffffffffu, mbar_wait(done + 8 * ((uses - 1) & 1), ((uses - 1) >> 1) & 1));
+        if (n > 1 && ok) ok = __all_sync(0xffffffffu, mbar_wait(done + 8 * (uses & 1), ((uses - 2) >> 1) & 1));
         fence_after();
         __syncthreads();
         float* const sums = reinterpret_cast<float*>(mem);           // [128][width]
-        const uint32_t row = (warp & 3) * 32 + lane, col = 32 * (warp >> 2), first = run_at[0], last = at;
+        const uint32_t row = (warp & 3) * 32 + lane, col = 32 * (warp >> 2);
 #pragma unroll 1
         for (uint32_t i = 0; i < runs; i++) {
             uint32_t v[32];
             tmem_ld(tmem + (((warp & 3) * 32) << 16) + i * kAmRank + col, v);
             tmem_wait_ld(v);
-            if (row >= run_at[i] && row < last && which[row] == which[run_at[i]] && (i + 1 >= runs || row < run_at[i + 1])) {
+            if (row >= (uint32_t)run[i].first && row < (uint32_t)run[i].end) {
 #pragma unroll
                 for (int y = 0; y < 32; y++) sums[row * L::width + col + y] = !ok ? kBatchNaN : n ? __uint_as_float(v[y]) : 0.0f;
             }
@@ -340,9 +381,10 @@ __global__ void __launch_bounds__(256, 1) __cluster_dims__(kAfCluster, 1, 1) k_a
         // this CTA's sixteen rows: four rank values a thread
         {
             const uint32_t mine = share * (kAmRows / kAfCluster) + (threadIdx.x >> 4), j = 4 * (threadIdx.x & 15);
-            if (mine >= first && mine < last && which[mine] >= 0) {
+            if (mine >= (uint32_t)run[0].first && mine < (uint32_t)run[runs - 1].end && which[mine] >= 0) {
                 float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                 const uint32_t from = smem_u32(sums + mine * L::width + j);
+#pragma unroll
                 for (uint32_t e = 0; e < kAfCluster; e++) {
                     uint32_t there;
                     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(from), "r"(e));
@@ -369,62 +411,73 @@ __global__ void __launch_bounds__(256, 1) __cluster_dims__(kAfCluster, 1, 1) k_a
     if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem) : "memory");
 }
 
-constexpr uint32_t kAxThreads = 640, kAxWriters = 512;
+constexpr uint32_t kAxWriters = 256, kAxThreads = kAxWriters + 128;
 template <typename WT> struct AxLayout {
-    static constexpr uint32_t stages = sizeof(WT) == 2 ? 3 : 2, stage = AmParts<WT>::n * kAmPart, ring = 3 * kAmPart, turn = ring + stages * stage;      // turn: 32 x 33 floats a writing warp
-    static constexpr uint32_t which = turn + 16 * 32 * 33 * 4, bars = which + kAmRows * 4, size = bars + 128 + 1024;
+    // turns: 32 rows of 64 outputs (68 floats a row: rows and columns of them meet different banks), two for each of 8 writing warps
+    static constexpr uint32_t stages = sizeof(WT) == 2 ? 3 : 1, stage = AmParts<WT>::n * kAmPart, width = 68, turn = 32 * width * 4, ring = stages * stage;
+    static constexpr uint32_t which = ring + 8 * 2 * turn, runs = which + kAmRows * 4, bars = runs + kAmRows * 12, size = bars + 128 + 1024;
 };
-// CTA (share of the outputs, block of 128 rows)
+// CTA (share of the outputs, block of 128 rows).  TMEM: sums of two tiles, the rows' rank values (A operand).
 template <typename WT>
 __global__ void __launch_bounds__(kAxThreads, 1) k_adapter_expand(AdArgs a, const WT* __restrict__ wb, const uint4* __restrict__ parts, uint32_t quads) {
     typedef AxLayout<WT> L;
+    constexpr uint32_t kH = 256;                                     // TMEM column of the rank values: 32 a part
     extern __shared__ uint8_t am_raw[];
     const uint32_t base = (smem_u32(am_raw) + 1023u) & ~1023u;
     uint8_t* const mem = am_raw + (base - smem_u32(am_raw));
     const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, r0 = blockIdx.y * kAmRows;
-    int* const which = reinterpret_cast<int*>(mem + L::which);
+    AmRun* const runs = reinterpret_cast<AmRun*>(mem + L::runs);
     const uint32_t full = base + L::bars, empty = full + 8 * L::stages, sum_full = empty + 8 * L::stages, sum_empty = sum_full + 16, tmem_slot = sum_empty + 16;
+    uint32_t* const count = reinterpret_cast<uint32_t*>(mem + (tmem_slot + 8 - base));
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < L::stages; i++) { mbar_init(full + 8 * i, 4); mbar_init(empty + 8 * i, 1); }
-        for (uint32_t i = 0; i < 2; i++) { mbar_init(sum_full + 8 * i, 1); mbar_init(sum_empty + 8 * i, 16); }
+        for (uint32_t i = 0; i < 2; i++) { mbar_init(sum_full + 8 * i, 1); mbar_init(sum_empty + 8 * i, 8); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 16) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" ::"r"(tmem_slot) : "memory");
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(tmem_slot) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const BatchHead head = batch_head(a.table, a.B);
-    if (threadIdx.x < kAmRows) which[threadIdx.x] = r0 + threadIdx.x < a.B ? ad_of(a, head, r0 + threadIdx.x) : kAdIdle;
-    // the rows' rank values; those of rows without any are whatever was there: their outputs are left out
-    for (uint32_t i = threadIdx.x; i < 3 * kAmRows * 8; i += kAxThreads) {
-        const uint32_t y = i / (kAmRows * 8), row = i / 8 % kAmRows, c = i % 8;
-        const bool on = r0 + row < a.B;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(base + y * kAmPart + am_at(row, c)), "l"(on ? parts + ((size_t)y * a.B + r0 + row) * 8 + c : parts), "r"(on ? 16 : 0) : "memory");
+    const bool in_place = a.base == a.dst;
+    int* const which = reinterpret_cast<int*>(mem + L::which);
+    fence_before();
+    am_find_runs(a, head, r0, which, runs, count, [](int w) { return w < 0; });
+    fence_after();
+    const uint32_t tiles = (a.N + 127) / 128, per = (tiles + gridDim.x - 1) / gridDim.x, t0 = min(tiles, blockIdx.x * per), n = min(tiles, t0 + per) - t0, n_runs = *count;
+    bool ok = true;
+    // The rows' rank values, a row a lane.  Those of rows without any are whatever was there: their outputs are left out.
+    if (warp < 4) {
+        const uint32_t row = r0 + 32 * warp + lane;
+#pragma unroll
+        for (uint32_t y = 0; y < 3; y++) {
+            uint32_t v[32];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const uint4 u = row < a.B ? parts[((size_t)y * a.B + row) * 8 + i] : make_uint4(0, 0, 0, 0);
+                v[4 * i] = u.x; v[4 * i + 1] = u.y; v[4 * i + 2] = u.z; v[4 * i + 3] = u.w;
+            }
+            tmem_st((32 * warp << 16) + kH + 32 * y, v);
+        }
+        tmem_wait_st();
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    am_proxy_fence();
     fence_before();
     __syncthreads();
     fence_after();
-    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(mem + (tmem_slot - base));
-    const uint32_t tiles = (a.N + 127) / 128, per = (tiles + gridDim.x - 1) / gridDim.x, t0 = min(tiles, blockIdx.x * per), n = min(tiles, t0 + per) - t0;
-    bool ok = true;
-    if (warp >= 16) {
-        // bring weights, issue: the tiles of one run of rows after the other's
-        const uint32_t id = threadIdx.x - kAxWriters;                // piece id & 7 of rows id / 8 + 16 i
-        uint32_t slot = 0, phase = 1, at_slot = 0, at_phase = 0, item = 0;
-        auto fill = [&](int run, uint32_t t) {                       // the next stage
+    if (warp >= 8) {
+        // bring weights, issue: of a tile one run of rows after the other
+        const uint32_t id = threadIdx.x - kAxWriters, c = id & 7, items = n * n_runs;      // piece c of rows id / 8 + 16 i
+        uint32_t slot = 0, phase = 1, at_slot = 0, at_phase = 0, f_tile = 0, f_run = 0;
+        auto fill = [&]() {                                          // the next stage
+            const int adapter = runs[f_run].which;
             if (ok) ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * slot, phase));
-            const uint32_t c = id & 7;
 #pragma unroll
             for (uint32_t i = 0; i < 8; i++) {
-                const uint32_t row = (id >> 3) + 16 * i, o = (t0 + t) * 128 + row;
-                const uint32_t to = L::ring + slot * L::stage + am_at(row, c);
+                const uint32_t row = (id >> 3) + 16 * i, o = (t0 + f_tile) * 128 + row, to = slot * L::stage + am_at(row, c);
                 const bool on = o < a.N && 8 * c < a.rank;           // the rank is a multiple of eight here
-                const WT* from = on ? wb + ((size_t)run * a.N + o) * a.rank + 8 * c : wb;
+                const WT* from = on ? wb + ((size_t)adapter * a.N + o) * a.rank + 8 * c : wb;
                 if constexpr (sizeof(WT) == 2) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(base + to), "l"(from), "r"(on ? 16 : 0) : "memory");
                 else {
                     uint4 w[3];
@@ -436,102 +489,119 @@ __global__ void __launch_bounds__(kAxThreads, 1) k_adapter_expand(AdArgs a, cons
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
             if (++slot == L::stages) { slot = 0; phase ^= 1; }
+            if (++f_run == n_runs) { f_run = 0; f_tile++; }
         };
-        for (uint32_t i = 0; i < kAmRows;) {
-            const int run = which[i];
-            while (i < kAmRows && which[i] == run) i++;
-            if (run < 0 || !n) continue;
-            fill(run, 0);
-            for (uint32_t t = 0; t < n; t++, item++) {
-                if (t + 1 < n) { fill(run, t + 1); asm volatile("cp.async.wait_group 1;" ::: "memory"); }
-                else asm volatile("cp.async.wait_group 0;" ::: "memory");
-                am_proxy_fence();
+        constexpr uint32_t kAhead = L::stages - 1;                   // stages that are on their way while one is used
+        for (uint32_t i = 0; i < min(kAhead, items); i++) fill();
+        for (uint32_t item = 0; item < items; item++) {
+            if (item + kAhead < items) fill(); else asm volatile("cp.async.commit_group;" ::: "memory");
+            asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
+            am_proxy_fence();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(full + 8 * at_slot);
+            if (warp == 8) {
+                const uint32_t d = (item & 1) * 128, w0 = desc_low(base) + at_slot * (L::stage >> 4), freed = empty + 8 * at_slot, idesc = am_idesc(128);
+                if (ok) ok = __all_sync(0xffffffffu, mbar_wait(full + 8 * at_slot, at_phase));
+                if (ok && item >= 2) ok = __all_sync(0xffffffffu, mbar_wait(sum_empty + 8 * (item & 1), ((item >> 1) - 1) & 1));
+                fence_after();
+                if (elect_one() && ok) {
+#pragma unroll
+                    for (uint32_t y = 0; y < AmProducts<WT>::n; y++)
+#pragma unroll
+                        for (uint32_t z = 0; z < 4; z++) {
+                            const uint32_t h = kH + 32 * am_x<WT>(y) + 8 * z, ws = w0 + am_w<WT>(y) * (kAmPart >> 4) + 2 * z;
+                            if (y == 0 && z == 0) mma_ts<false>(d, h, ws, idesc); else mma_ts<true>(d, h, ws, idesc);
+                        }
+                    mma_commit(sum_full + 8 * (item & 1));
+                    mma_commit(freed);
+                }
                 __syncwarp();
-                if (lane == 0) mbar_arrive(full + 8 * at_slot);
-                if (warp == 16) {
-                    const uint32_t d = tmem + (item & 1) * 128, xa = desc_low(base), w0 = desc_low(base + L::ring) + at_slot * (L::stage >> 4), freed = empty + 8 * at_slot, idesc = am_idesc(128);
-                    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(full + 8 * at_slot, at_phase));
-                    if (ok && item >= 2) ok = __all_sync(0xffffffffu, mbar_wait(sum_empty + 8 * (item & 1), ((item >> 1) - 1) & 1));
-                    fence_after();
-                    if (elect_one() && ok) {
-#pragma unroll
-                        for (uint32_t y = 0; y < AmProducts<WT>::n; y++)
-#pragma unroll
-                            for (uint32_t z = 0; z < 4; z++) {
-                                const uint32_t xs = xa + am_x<WT>(y) * (kAmPart >> 4) + 2 * z, ws = w0 + am_w<WT>(y) * (kAmPart >> 4) + 2 * z;
-                                if (y == 0 && z == 0) mma_ss<false>(d, xs, ws, idesc); else mma_ss<true>(d, xs, ws, idesc);
-                            }
-                        mma_commit(sum_full + 8 * (item & 1));
-                        mma_commit(freed);
-                    }
-                    __syncwarp();
-                }
-                if (++at_slot == L::stages) { at_slot = 0; at_phase ^= 1; }
             }
+            if (++at_slot == L::stages) { at_slot = 0; at_phase ^= 1; }
         }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
     } else {
-        // add the base, write: a block of 32 rows and 32 outputs a warp; lanes hold a row each of the sums, and by way of shared memory an eighth of four rows each
-        const uint32_t row0 = (warp & 3) * 32, col0 = 32 * (warp >> 2), lr = lane >> 3, lc = 4 * (lane & 7);
-        float* const turn = reinterpret_cast<float*>(mem + L::turn) + warp * 32 * 33;
+        // Add the base, write: 32 rows and 64 outputs of a tile a warp.  The base comes by whole rows, a tile ahead; a lane adds the sums of its row, and whole rows leave.
+        const uint32_t row0 = (warp & 3) * 32, col0 = 64 * (warp >> 2), lr = lane >> 4, lc = 4 * (lane & 15), lane_row = row0 + lane;
+        float* const ring = reinterpret_cast<float*>(mem + L::ring + warp * 2 * L::turn);
+        const uint32_t ring_at = smem_u32(ring);
+        uint32_t live = 0, bad = 0, none = 0;                        // rows of the warp: with a result, a result that is not a number, the base alone
+        {
+            const int w = which[lane_row];
+            live = __ballot_sync(0xffffffffu, w != kAdIdle && !(w == kAdNone && in_place)); bad = __ballot_sync(0xffffffffu, w == kAdBad); none = __ballot_sync(0xffffffffu, w < 0);
+        }
+        auto fetch = [&](uint32_t t) {
+            const uint32_t o = (t0 + t) * 128 + col0 + lc;
+            if (t < n && quads) {
+                const bool in = o + 4 <= a.N;                        // zeros otherwise
+#pragma unroll 4
+                for (uint32_t x = 0; x < 16; x++) {
+                    const uint32_t r = 2 * x + lr;
+                    if ((live & ~bad) >> r & 1)
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ring_at + (t & 1) * L::turn + r * (4 * L::width) + 4 * lc), "l"(in ? a.base + (size_t)(r0 + row0 + r) * a.base_rs + o : a.base), "r"(in ? 16 : 0) : "memory");
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        fetch(0);
         uint32_t item = 0;
-        for (uint32_t i = 0; i < kAmRows;) {
-            const int run = which[i];
-            const uint32_t first = i;
-            while (i < kAmRows && which[i] == run) i++;
-            if (run == kAdIdle || (run == kAdNone && a.base == a.dst) || !n) continue;
-            const bool here = first < row0 + 32 && i > row0;         // the run reaches this warp's rows
-            for (uint32_t t = 0; t < n; t++) {
-                const uint32_t o = (t0 + t) * 128 + col0 + lc;
-                float4 b[8];
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const uint32_t row = row0 + 4 * e + lr;
-                    b[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    if (!here || row < first || row >= i) continue;
-                    const float* from = a.base + (size_t)(r0 + row) * a.base_rs + o;
-                    if (quads && o + 4 <= a.N) b[e] = *reinterpret_cast<const float4*>(from);
-                    else { if (o < a.N) b[e].x = from[0]; if (o + 1 < a.N) b[e].y = from[1]; if (o + 2 < a.N) b[e].z = from[2]; if (o + 3 < a.N) b[e].w = from[3]; }
-                }
-                if (run >= 0) {
-                    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(sum_full + 8 * (item & 1), (item >> 1) & 1));
-                    fence_after();
-                    if (here) {
-                        uint32_t v[32];
-                        tmem_ld(tmem + (row0 << 16) + (item & 1) * 128 + col0, v);
-                        tmem_wait_ld(v);
-#pragma unroll
-                        for (int e = 0; e < 32; e++) turn[lane * 33 + e] = ok ? __uint_as_float(v[e]) : kBatchNaN;
-                    }
-                    fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(sum_empty + 8 * (item & 1));
-                    item++;
-                }
+        for (uint32_t t = 0; t < n; t++) {
+            fetch(t + 1);
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+            __syncwarp();
+            float* const turn = ring + (t & 1) * (L::turn / 4);
+            if (!quads) {
+                for (uint32_t x = 0; x < 64; x++) turn[lane * L::width + x] = 0.0f;
+            }
+            for (uint32_t e = 0; e < n_runs; e++, item++) {
+                const bool here = runs[e].first < (int)row0 + 32 && runs[e].end > (int)row0, mine = runs[e].first <= (int)lane_row && runs[e].end > (int)lane_row;
+                if (ok) ok = __all_sync(0xffffffffu, mbar_wait(sum_full + 8 * (item & 1), (item >> 1) & 1));
+                fence_after();
                 if (here) {
 #pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const uint32_t row = row0 + 4 * e + lr;
-                        if (row < first || row >= i) continue;
-                        float4 v = b[e];
-                        if (run >= 0) {
-                            const float* s = turn + (4 * e + lr) * 33 + lc;
-                            v.x += s[0]; v.y += s[1]; v.z += s[2]; v.w += s[3];
-                        } else if (run == kAdBad) v = make_float4(kBatchNaN, kBatchNaN, kBatchNaN, kBatchNaN);
-                        float* to = a.dst + (size_t)(r0 + row) * a.dst_rs + o;
-                        if (quads && o + 4 <= a.N) *reinterpret_cast<float4*>(to) = v;
-                        else { if (o < a.N) to[0] = v.x; if (o + 1 < a.N) to[1] = v.y; if (o + 2 < a.N) to[2] = v.z; if (o + 3 < a.N) to[3] = v.w; }
+                    for (uint32_t h = 0; h < 64; h += 32) {
+                        uint32_t v[32];
+                        tmem_ld((row0 << 16) + (item & 1) * 128 + col0 + h, v);
+                        tmem_wait_ld(v);
+                        if (mine) {
+#pragma unroll
+                            for (int x = 0; x < 32; x += 4) {
+                                float4* const to = reinterpret_cast<float4*>(turn + lane * L::width + h + x);
+                                float4 b = *to;
+                                b.x += __uint_as_float(v[x]); b.y += __uint_as_float(v[x + 1]); b.z += __uint_as_float(v[x + 2]); b.w += __uint_as_float(v[x + 3]);
+                                *to = ok ? b : make_float4(kBatchNaN, kBatchNaN, kBatchNaN, kBatchNaN);
+                            }
+                        }
                     }
                 }
+                fence_before();
                 __syncwarp();
+                if (lane == 0) mbar_arrive(sum_empty + 8 * (item & 1));
             }
+            const uint32_t o = (t0 + t) * 128 + col0 + lc;
+            const bool all = quads && o + 4 <= a.N;
+#pragma unroll 4
+            for (uint32_t x = 0; x < 16; x++) {
+                const uint32_t r = 2 * x + lr;
+                if (!(live >> r & 1)) continue;
+                float4 v = *reinterpret_cast<const float4*>(turn + r * L::width + lc);
+                if (bad >> r & 1) v = make_float4(kBatchNaN, kBatchNaN, kBatchNaN, kBatchNaN);
+                float* const to = a.dst + (size_t)(r0 + row0 + r) * a.dst_rs + o;
+                if (all) *reinterpret_cast<float4*>(to) = v;
+                else {
+                    const float* from = a.base + (size_t)(r0 + row0 + r) * a.base_rs + o;      // not copied: `v` is the sum alone
+#pragma unroll
+                    for (uint32_t z = 0; z < 4; z++) if (o + z < a.N) to[z] = bad >> r & 1 ? kBatchNaN : none >> r & 1 ? from[z] : from[z] + (&v.x)[z];
+                }
+            }
+            __syncwarp();
         }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
     if (!ok && lane == 0) count_timeout();
     __syncwarp();
     fence_before();
     __syncthreads();
-    if (warp == 16) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem) : "memory");
+    if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(0u) : "memory");
 }
 
 // More rows than kAmLeast go in blocks, where rank and strides allow their 16-byte pieces.

@@ -25,6 +25,20 @@ __device__ __forceinline__ int ad_of(const AdArgs& a, const BatchHead& head, uin
 
 // ── few rows ─────────────────────────────────────────────────────────────────────────────────────────────────────────
 constexpr uint32_t kAfRows = 8, kAfCluster = 8, kAfThreads = 256, kAfStage = 96 * 1024;      // bytes of the second product's weights that are fetched ahead
+__device__ __forceinline__ float af_remote(uint32_t at, uint32_t rank) {
+    uint32_t there;
+    float v;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 af_remote4(uint32_t at, uint32_t rank) {
+    uint32_t there;
+    float4 v;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(there) : "memory");
+    return v;
+}
 // R: rows of the run at most; J: rank values at a time.  x and the weights in vectors of WVec<WT>::n where VEC
 template <typename WT, int R, int J, bool VEC>
 __device__ __forceinline__ void af_shrink(const AdArgs& a, const WT* __restrict__ wa, const float* __restrict__ x, uint32_t rows, uint32_t k0, uint32_t k1, float* part) {
@@ -153,14 +167,11 @@ __global__ void __launch_bounds__(kAfThreads) __cluster_dims__(kAfCluster, 1, 1)
         float s = 0.0f;
         if (i < rows * a.rank) {
             const uint32_t at = (uint32_t)__cvta_generic_to_shared(part + i);
+            float v[kAfCluster];                                     // all on their way before the first is added
 #pragma unroll
-            for (uint32_t c = 0; c < kAfCluster; c++) {
-                uint32_t there;
-                float v;
-                asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(c));
-                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
-                s += v;
-            }
+            for (uint32_t c = 0; c < kAfCluster; c++) v[c] = af_remote(at, c);
+#pragma unroll
+            for (uint32_t c = 0; c < kAfCluster; c++) s += v[c];
         }
         h[i] = s * scale;
     }
@@ -229,7 +240,7 @@ template <typename WT> struct AsLayout {
     // weights of bfloat16 sessions come a chunk ahead, through three slots; f32 ones are split as they come, into two
     static constexpr uint32_t weights = kAmRank * 128, w_run = AmParts<WT>::n * weights, w_slots = sizeof(WT) == 2 ? 3 : 2, w_slot = kAmRuns<WT> * w_run, x_stage = 3 * kAmPart;
     static constexpr uint32_t w = 2 * x_stage, which = w + w_slots * w_slot, runs = which + kAmRows * 4, bars = runs + kAmRows * 12, size = bars + 64 + 1024;
-    static constexpr uint32_t width = kAmRank + 1;                   // of the partial sums, which take the first stage's place in the end
+    static constexpr uint32_t width = kAmRank + 4;                   // of the partial sums, which take the first stage's place in the end
     static_assert(kAmRows * width * 4 <= x_stage, "partial sums");
 };
 template <typename WT>
@@ -372,7 +383,9 @@ __global__ void __launch_bounds__(256, 1) __cluster_dims__(kAfCluster, 1, 1) k_a
             tmem_wait_ld(v);
             if (row >= (uint32_t)run[i].first && row < (uint32_t)run[i].end) {
 #pragma unroll
-                for (int y = 0; y < 32; y++) sums[row * L::width + col + y] = !ok ? kBatchNaN : n ? __uint_as_float(v[y]) : 0.0f;
+                for (int y = 0; y < 32; y += 4)
+                    *reinterpret_cast<float4*>(sums + row * L::width + col + y) = !ok ? make_float4(kBatchNaN, kBatchNaN, kBatchNaN, kBatchNaN) : !n ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
+                        : make_float4(__uint_as_float(v[y]), __uint_as_float(v[y + 1]), __uint_as_float(v[y + 2]), __uint_as_float(v[y + 3]));
             }
         }
         fence_before();
@@ -382,23 +395,15 @@ __global__ void __launch_bounds__(256, 1) __cluster_dims__(kAfCluster, 1, 1) k_a
         {
             const uint32_t mine = share * (kAmRows / kAfCluster) + (threadIdx.x >> 4), j = 4 * (threadIdx.x & 15);
             if (mine >= (uint32_t)run[0].first && mine < (uint32_t)run[runs - 1].end && which[mine] >= 0) {
-                float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                const uint32_t from = smem_u32(sums + mine * L::width + j);
+                float4 e[kAfCluster], v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);      // all on their way before the first is added
 #pragma unroll
-                for (uint32_t e = 0; e < kAfCluster; e++) {
-                    uint32_t there;
-                    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(from), "r"(e));
+                for (uint32_t x = 0; x < kAfCluster; x++) e[x] = af_remote4(smem_u32(sums + mine * L::width + j), x);
 #pragma unroll
-                    for (int y = 0; y < 4; y++) {
-                        float w;
-                        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(w) : "r"(there + 4 * y) : "memory");
-                        v[y] += w;
-                    }
-                }
+                for (uint32_t x = 0; x < kAfCluster; x++) { v.x += e[x].x; v.y += e[x].y; v.z += e[x].z; v.w += e[x].w; }
                 const float f = a.scales ? a.scales[which[mine]] : 1.0f;
                 uint2 w[3];
-                split3(v[0] * f, v[1] * f, w[0].x, w[1].x, w[2].x);
-                split3(v[2] * f, v[3] * f, w[0].y, w[1].y, w[2].y);
+                split3(v.x * f, v.y * f, w[0].x, w[1].x, w[2].x);
+                split3(v.z * f, v.w * f, w[0].y, w[1].y, w[2].y);
 #pragma unroll
                 for (int y = 0; y < 3; y++) reinterpret_cast<uint2*>(parts)[((size_t)y * a.B + r0 + mine) * (kAmRank / 4) + j / 4] = w[y];
             }

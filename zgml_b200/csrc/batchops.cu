@@ -4,6 +4,7 @@
 #include "batch_table.cuh"
 
 #include <algorithm>
+#include <cmath>
 
 namespace {
 
@@ -11,11 +12,14 @@ namespace {
 struct BaArgs {
     float* cache; const float* src; const float* table; const float* freqs; float* turned;
     uint32_t B, cols, src_rs, src_col, width, cache_col, R, slots, key_heads, dim, turn_at, rot, halves, q_heads, q_col, dst_rs, dst_col;
-    double base;
+    double ratio;                                                    // base^(-2 / rot)
 };
-// CTA: one row.  The angle of a far position needs more bits than f32 has (position 100000 times a frequency near 1 is off by 4e-3 there): it is formed
-// and reduced to a turn in 64 bits, once per pair for all heads, and only the remainder goes through f32 sine and cosine.
-__global__ void __launch_bounds__(256) k_batch_append(BaArgs a) {
+// CTA (row, share of its values).  The angle of a far position needs more bits than f32 has (position 100000 times a frequency near 1 is off by 4e-3 there): it is formed
+// and reduced to a turn in 64 bits, once per pair for all heads of the share, and only the remainder goes through f32 sine and cosine.  A frequency base^(-2i / rot) is
+// the i-th power of a number from the host, by squaring: off by some 10 roundings of 2^-53.
+// One row is bound by latency: with all of its 6144 values in one CTA and exp in 64 bits it took 4 us longer.
+constexpr uint32_t kBaThreads = 256, kBaValues = 4;                  // values a thread
+__global__ void __launch_bounds__(kBaThreads) k_batch_append(BaArgs a) {
     pdl_enter();
     extern __shared__ float2 turn[];                                 // [rot / 2]: cosine, sine
     const uint32_t r = blockIdx.x;
@@ -23,47 +27,65 @@ __global__ void __launch_bounds__(256) k_batch_append(BaArgs a) {
     const BatchRow w = batch_row(a.table, r);
     if (r >= head.rows || w.slot < 0) return;
     const bool ok = (uint32_t)w.slot < a.slots && (uint32_t)w.length <= a.R && head.prefix >= 0;
-    for (uint32_t i = threadIdx.x; i < a.rot / 2; i += blockDim.x) {
-        const double f = a.freqs ? (double)a.freqs[i] : exp(-2.0 * i / a.rot * log(a.base));
-        const double x = ((double)head.prefix + w.length - 1) * f, two_pi = 6.283185307179586476925;
+    const uint32_t keys = a.key_heads * a.dim, all = a.cols + a.q_heads * a.dim, first = blockIdx.y * (kBaThreads * kBaValues) + threadIdx.x;
+    const float* src = a.src + (size_t)r * a.src_rs;
+    // values: first the appended columns, then the query heads.  What a value of a turned head becomes: x cos - y sin or y cos + x sin, with its partner
+    float x[kBaValues], y[kBaValues];
+    uint32_t pair[kBaValues];                                        // bit 31: the second of its pair; all bits: copied
+#pragma unroll
+    for (uint32_t i = 0; i < kBaValues; i++) {
+        const uint32_t c = first + i * kBaThreads;
+        x[i] = y[i] = 0.0f; pair[i] = 0xffffffffu;
+        if (c >= all) continue;
+        const uint32_t at = c < a.cols ? c : c - a.cols, in = at % a.dim - a.turn_at, half = a.rot / 2;
+        const float* p = src + (c < a.cols ? a.src_col : a.q_col) + at;
+        x[i] = *p;
+        if ((c < a.cols && at >= keys) || in >= a.rot) continue;
+        const bool second = a.halves ? in >= half : in & 1;
+        const int partner = a.halves ? (second ? -(int)half : (int)half) : second ? -1 : 1;
+        y[i] = p[partner];
+        pair[i] = (a.halves ? (second ? in - half : in) : in >> 1) | (second ? 0x80000000u : 0u);
+    }
+    for (uint32_t i = threadIdx.x; i < a.rot / 2; i += kBaThreads) {
+        double f = 1.0;
+        if (a.freqs) f = (double)a.freqs[i];
+        else {
+            double power = a.ratio;
+            for (uint32_t e = i; e; e >>= 1) { if (e & 1) f *= power; power *= power; }
+        }
+        const double angle = ((double)head.prefix + w.length - 1) * f, two_pi = 6.283185307179586476925;
         float s, c;
-        sincosf((float)(x - two_pi * rint(x / two_pi)), &s, &c);
+        sincosf((float)(angle - two_pi * rint(angle / two_pi)), &s, &c);
         turn[i] = make_float2(c, s);
     }
     // Of rows that name the same place the last one stays, whatever order the CTAs run in.
     bool later = false;
-    for (uint32_t i = r + 1 + threadIdx.x; i < head.rows; i += blockDim.x) {
-        const BatchRow x = batch_row(a.table, i);
-        later = later || (x.slot == w.slot && x.length == w.length);
+    for (uint32_t i = r + 1 + threadIdx.x; i < head.rows; i += kBaThreads) {
+        const BatchRow z = batch_row(a.table, i);
+        later = later || (z.slot == w.slot && z.length == w.length);
     }
     later = __syncthreads_or(later);
-    const float* src = a.src + (size_t)r * a.src_rs;
-    // value j of a head that begins at p
-    auto value = [&](const float* p, uint32_t j) {
-        const uint32_t at = j - a.turn_at;
-        if (at >= a.rot) return p[j];
-        const uint32_t half = a.rot / 2, pair = a.halves ? (at < half ? at : at - half) : at >> 1, first = a.halves ? pair : 2 * pair, second = a.halves ? pair + half : 2 * pair + 1;
-        const float x = p[a.turn_at + first], y = p[a.turn_at + second];
-        const float2 t = turn[pair];
-        return at == first ? x * t.x - y * t.y : x * t.y + y * t.x;
-    };
-    const uint32_t heads = a.key_heads * a.dim;
-    if (ok && w.length > 0 && !later) {
-        float* out = a.cache + ((size_t)w.slot * a.R + (w.length - 1)) * a.width + a.cache_col;
-        const float* p = src + a.src_col;
-        for (uint32_t c = threadIdx.x; c < a.cols; c += blockDim.x) out[c] = c < heads ? value(p + c / a.dim * a.dim, c % a.dim) : p[c];
-    }
-    if (a.q_heads) {
-        float* out = a.turned + (size_t)r * a.dst_rs + a.dst_col;
-        const float* p = src + a.q_col;
-        for (uint32_t c = threadIdx.x; c < a.q_heads * a.dim; c += blockDim.x) out[c] = ok ? value(p + c / a.dim * a.dim, c % a.dim) : kBatchNaN;
+    const bool append = ok && w.length > 0 && !later;
+    float* const cache = a.cache + (append ? ((size_t)w.slot * a.R + (w.length - 1)) * a.width : 0) + a.cache_col;
+    float* const turned = a.turned + (size_t)r * a.dst_rs + a.dst_col;
+#pragma unroll
+    for (uint32_t i = 0; i < kBaValues; i++) {
+        const uint32_t c = first + i * kBaThreads;
+        if (c >= all) continue;
+        float v = x[i];
+        if (pair[i] != 0xffffffffu) {
+            const float2 t = turn[pair[i] & 0x7fffffffu];
+            v = pair[i] >> 31 ? v * t.x + y[i] * t.y : v * t.x - y[i] * t.y;
+        }
+        if (c >= a.cols) turned[c - a.cols] = ok ? v : kBatchNaN;
+        else if (append) cache[c] = v;
     }
 }
 
 // ── LOGIT_RULES ──────────────────────────────────────────────────────────────────────────────────────────────────────
 struct LrArgs {
     float* dst; const float* src; const float* table; const int32_t* history; const int2* bias; const uint32_t* masks;
-    uint32_t B, V, src_rs, dst_rs, history_rows, slots, entries, mask_rows, slice;
+    uint32_t B, V, src_rs, dst_rs, history_rows, slots, entries, mask_rows;
 };
 struct LrRow { int32_t slot, length, first, mask, bias_first, bias_count; float repetition, presence, frequency; };
 __device__ __forceinline__ LrRow lr_row(const float* table, uint32_t r) {
@@ -74,59 +96,114 @@ __device__ __forceinline__ LrRow lr_row(const float* table, uint32_t r) {
     w.repetition = __int_as_float(y.z); w.presence = __int_as_float(y.w); w.frequency = __int_as_float(z.x);
     return w;
 }
-constexpr uint32_t kLrSeen = 0x80000000u;
-// CTA (slice of the vocabulary, row): counts of the slice's tokens in the row's history (bit 31: the token occurs at all), biases of the slice, then one pass over the logits
-__global__ void __launch_bounds__(256) k_logit_rules(LrArgs a) {
+constexpr uint32_t kLrSeen = 0x80000000u, kLrThreads = 256;
+// CTA (row, slice of the vocabulary): counts of the slice's tokens in the row's history (bit 31: the token occurs at all) and biases of the slice in shared memory, then the
+// logits, which were asked for at the start: a thread holds NV times four neighbours.  A history is read once per slice (from L2), which costs less than counts of a whole
+// vocabulary in memory: 64 rows over 128256 tokens with 4096 words each read 33 MB for it beside the 66 MB of logits.
+template <int NV, bool VEC>
+__global__ void __launch_bounds__(kLrThreads) k_logit_rules(LrArgs a) {
     pdl_enter();
-    extern __shared__ uint32_t counts[];                             // [slice] counts, [slice] biases
-    float* const bias = reinterpret_cast<float*>(counts + a.slice);
-    const uint32_t r = blockIdx.y, v0 = blockIdx.x * a.slice, n = min(a.slice, a.V - v0);
+    extern __shared__ uint4 lr_mem[];                                // [slice] counts, [slice] biases
+    constexpr uint32_t slice = kLrThreads * 4 * NV;
+    uint32_t* const counts = reinterpret_cast<uint32_t*>(lr_mem);
+    float* const bias = reinterpret_cast<float*>(counts + slice);
+    const uint32_t r = blockIdx.y, v0 = blockIdx.x * slice, n = min(slice, a.V - v0);
     const BatchHead head = batch_head(a.table, a.B);
     const LrRow w = lr_row(a.table, r);
     if (r >= head.rows || w.slot < 0) return;
     const float* src = a.src + (size_t)r * a.src_rs + v0;
     float* dst = a.dst + (size_t)r * a.dst_rs + v0;
+    float4 z[NV];
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        const uint32_t t = 4 * (threadIdx.x + kLrThreads * i);
+        z[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (VEC && t + 4 <= n) z[i] = *reinterpret_cast<const float4*>(src + t);
+        else { if (t < n) z[i].x = src[t]; if (t + 1 < n) z[i].y = src[t + 1]; if (t + 2 < n) z[i].z = src[t + 2]; if (t + 3 < n) z[i].w = src[t + 3]; }
+    }
     const bool ok = (w.length == 0 || ((uint32_t)w.slot < a.slots && (uint32_t)w.length <= a.history_rows)) && w.first >= 0 && (w.mask < 0 || (uint32_t)w.mask < a.mask_rows) &&
                     (w.bias_count == 0 || (w.bias_count > 0 && w.bias_first >= 0 && (uint32_t)w.bias_first + (uint32_t)w.bias_count <= a.entries));
-    if (!ok) {
-        for (uint32_t i = threadIdx.x; i < n; i += 256) dst[i] = kBatchNaN;
-        return;
+    const bool counted = ok && w.length > 0, biased = ok && w.bias_count > 0;
+    // (a mask word serves 8 threads' tokens; a row of words begins anywhere)
+    const uint32_t* mask = ok && w.mask >= 0 ? a.masks + (size_t)w.mask * ((a.V + 31) / 32) + v0 / 32 : nullptr;
+    uint32_t allowed[NV];
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        const uint32_t t = 4 * (threadIdx.x + kLrThreads * i);
+        allowed[i] = mask && t < n ? mask[t / 32] >> (t & 31) : 0xfu;
     }
-    for (uint32_t i = threadIdx.x; i < n; i += 256) { counts[i] = 0; bias[i] = 0.0f; }
-    __syncthreads();
-    const int32_t* past = a.history + (size_t)(w.length ? w.slot : 0) * a.history_rows;
-    for (uint32_t i = threadIdx.x; i < (uint32_t)w.length; i += 256) {
-        const uint32_t t = (uint32_t)past[i] - v0;                   // tokens outside the vocabulary belong to no slice
-        if (t < n) { if (i >= (uint32_t)w.first) atomicAdd(counts + t, 1u); else atomicOr(counts + t, kLrSeen); }
-    }
-    // Entries in order, 32 at a time by one warp; those of one token are added by its first lane, so that a token named twice gets the same sum in every run.
-    if (threadIdx.x < 32) {
-        for (uint32_t i = 0; i < (uint32_t)w.bias_count; i += 32) {
-            const bool on = i + threadIdx.x < (uint32_t)w.bias_count;
-            const int2 e = on ? a.bias[(size_t)w.bias_first + i + threadIdx.x] : make_int2(-1, 0);
-            const uint32_t t = (uint32_t)e.x - v0, mine = on && t < n ? t : 0xffffffffu;
-            const uint32_t same = __match_any_sync(0xffffffffu, mine);
-            float sum = 0.0f;
-            for (uint32_t l = 0; l < 32; l++) {
-                const float x = __shfl_sync(0xffffffffu, __int_as_float(e.y), l);
-                if (same >> l & 1) sum += x;
+    if (counted || biased) {
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            lr_mem[threadIdx.x + kLrThreads * i] = make_uint4(0, 0, 0, 0);
+            if (biased) lr_mem[slice / 4 + threadIdx.x + kLrThreads * i] = make_uint4(0, 0, 0, 0);
+        }
+        __syncthreads();
+        if (counted) {
+            const int32_t* past = a.history + (size_t)w.slot * a.history_rows;
+            auto count = [&](int32_t token, uint32_t i) {
+                const uint32_t t = (uint32_t)token - v0;             // tokens outside the vocabulary belong to no slice
+                if (t < n) { if (i >= (uint32_t)w.first) atomicAdd(counts + t, 1u); else atomicOr(counts + t, kLrSeen); }
+            };
+            const uint32_t length = w.length, lead = min(length, (4u - ((uint32_t)(reinterpret_cast<uintptr_t>(past) >> 2) & 3u)) & 3u), body = (length - lead) / 4;
+            if (threadIdx.x < lead) count(past[threadIdx.x], threadIdx.x);
+#pragma unroll 4
+            for (uint32_t i = threadIdx.x; i < body; i += kLrThreads) {
+                const int4 x = *reinterpret_cast<const int4*>(past + lead + 4 * i);
+                const uint32_t at = lead + 4 * i;
+                count(x.x, at); count(x.y, at + 1); count(x.z, at + 2); count(x.w, at + 3);
             }
-            if (mine != 0xffffffffu && __ffs(same) - 1 == (int)threadIdx.x) bias[t] += sum;
-            __syncwarp();
+            if (lead + 4 * body + threadIdx.x < length) count(past[lead + 4 * body + threadIdx.x], lead + 4 * body + threadIdx.x);
         }
+        // Entries in order, 32 at a time by one warp; where a token is named twice among them its first lane adds them up, so that every run gives the same sum.
+        if (biased && threadIdx.x >= kLrThreads - 32) {
+            const uint32_t lane = threadIdx.x & 31;
+            for (uint32_t i = 0; i < (uint32_t)w.bias_count; i += 32) {
+                const bool on = i + lane < (uint32_t)w.bias_count;
+                const int2 e = on ? a.bias[(size_t)w.bias_first + i + lane] : make_int2(-1, 0);
+                const uint32_t t = (uint32_t)e.x - v0, mine = on && t < n ? t : 0xffffffffu;
+                if (!__any_sync(0xffffffffu, mine != 0xffffffffu)) continue;
+                const uint32_t same = __match_any_sync(0xffffffffu, mine);
+                float sum = __int_as_float(e.y);
+                if (__any_sync(0xffffffffu, mine != 0xffffffffu && (same & (same - 1)))) {
+                    sum = 0.0f;
+                    for (uint32_t l = 0; l < 32; l++) {
+                        const float x = __shfl_sync(0xffffffffu, __int_as_float(e.y), l);
+                        if (same >> l & 1) sum += x;
+                    }
+                }
+                if (mine != 0xffffffffu && __ffs(same) - 1 == (int)lane) bias[t] += sum;
+                __syncwarp();
+            }
+        }
+        __syncthreads();
     }
-    __syncthreads();
-    const uint32_t* mask = w.mask >= 0 ? a.masks + (size_t)w.mask * ((a.V + 31) / 32) : nullptr;
-    for (uint32_t i = threadIdx.x; i < n; i += 256) {
-        float z = src[i];
-        const uint32_t c = counts[i], made = c & ~kLrSeen;
-        if (c) {
-            z = z > 0.0f ? z / w.repetition : z * w.repetition;
-            if (made) z = z - w.presence - w.frequency * (float)made;
+    auto rule = [&](float v, uint32_t c) {
+        if (!c) return v;
+        const uint32_t made = c & ~kLrSeen;
+        v = v > 0.0f ? v / w.repetition : v * w.repetition;
+        return made ? v - w.presence - w.frequency * (float)made : v;
+    };
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        const uint32_t t = 4 * (threadIdx.x + kLrThreads * i);
+        if (t >= n) break;
+        float4 v = z[i];
+        if (counted) {
+            const uint4 c = lr_mem[threadIdx.x + kLrThreads * i];
+            v.x = rule(v.x, c.x); v.y = rule(v.y, c.y); v.z = rule(v.z, c.z); v.w = rule(v.w, c.w);
         }
-        z += bias[i];
-        if (mask && !(mask[(v0 + i) >> 5] >> ((v0 + i) & 31) & 1)) z = -INFINITY;
-        dst[i] = z;
+        if (biased) {
+            const float4 b = reinterpret_cast<const float4*>(lr_mem)[slice / 4 + threadIdx.x + kLrThreads * i];
+            v.x += b.x; v.y += b.y; v.z += b.z; v.w += b.w;
+        }
+        if (!(allowed[i] & 1)) v.x = -INFINITY;
+        if (!(allowed[i] & 2)) v.y = -INFINITY;
+        if (!(allowed[i] & 4)) v.z = -INFINITY;
+        if (!(allowed[i] & 8)) v.w = -INFINITY;
+        if (!ok) v = make_float4(kBatchNaN, kBatchNaN, kBatchNaN, kBatchNaN);
+        if (VEC && t + 4 <= n) *reinterpret_cast<float4*>(dst + t) = v;
+        else { dst[t] = v.x; if (t + 1 < n) dst[t + 1] = v.y; if (t + 2 < n) dst[t + 2] = v.z; if (t + 3 < n) dst[t + 3] = v.w; }
     }
 }
 
@@ -141,6 +218,7 @@ bool zg_batch_op_valid(const ZgOp& op, const size_t* elems, size_t n_bufs, char*
         case ZG_OP_BATCH_APPEND: {
             const size_t B = s.n[0], cols = s.n[1], srs = s.n[2], width = s.n[3], R = s.n[4], heads = s.n[5], dim = s.n[6], rot = s.n[8], q_heads = s.n[10];
             if (!B || !cols || B > 65536 || width < s.off[1] + cols || !R || R >= (1u << 31) || s.n[9] > 1) return fail("batch_append: shape");
+            if (cols > (1u << 24) || q_heads > 65536 || dim > 65536 || q_heads * dim > (1u << 24)) return fail("batch_append: width");
             if ((heads || q_heads) && !dim) return fail("batch_append: head size");
             if (heads * dim > cols || rot % 2 || rot > 2048 || (rot && (s.n[7] + rot > dim || (s.buf[3] == ZG_NO_BUF && !(s.f[0] > 0.0f && s.f[0] - s.f[0] == 0.0f))))) return fail("batch_append: turned heads");
             if (rot && s.buf[3] != ZG_NO_BUF && !fits(3, s.off[4], rot / 2)) return fail("batch_append: frequency table");
@@ -186,9 +264,10 @@ bool zg_launch_batch_op(const ZgOp& op, float* const* bufs, const size_t* elems,
             a.q_heads = s.n[10]; a.q_col = s.off[2]; a.dst_rs = s.n[11]; a.dst_col = s.off[3];
             a.freqs = a.rot && s.buf[3] != ZG_NO_BUF ? bufs[s.buf[3]] + s.off[4] : nullptr;
             a.turned = a.q_heads ? bufs[s.buf[4]] : nullptr;
-            a.base = s.f[0];
+            a.ratio = a.rot && !a.freqs ? std::pow((double)s.f[0], -2.0 / a.rot) : 1.0;
             a.slots = (uint32_t)std::min<size_t>(elems[s.buf[0]] / ((size_t)a.R * a.width), (size_t)1 << 31);
-            launch_pdl(k_batch_append, dim3(a.B), dim3(256), (a.rot / 2) * sizeof(float2), st, a);
+            const uint32_t share = kBaThreads * kBaValues;
+            launch_pdl(k_batch_append, dim3(a.B, (a.cols + a.q_heads * a.dim + share - 1) / share), dim3(kBaThreads), (a.rot / 2) * sizeof(float2), st, a);
             ZG_SEQ_CHECK();
             return true;
         }
@@ -205,8 +284,15 @@ bool zg_launch_batch_op(const ZgOp& op, float* const* bufs, const size_t* elems,
             a.slots = given(3) ? (uint32_t)std::min<size_t>(elems[s.buf[3]] / a.history_rows, (size_t)1 << 31) : 0;
             a.entries = given(4) ? (uint32_t)std::min<size_t>(elems[s.buf[4]] / 2, (size_t)1 << 31) : 0;
             a.mask_rows = given(5) ? (uint32_t)std::min<size_t>(elems[s.buf[5]] / ((a.V + 31) / 32), (size_t)1 << 31) : 0;
-            a.slice = 4096;
-            launch_pdl(k_logit_rules, dim3((a.V + a.slice - 1) / a.slice, a.B), dim3(256), a.slice * 8, st, a);
+            // Slices of 4096 tokens where they fill the GPU, of 1024 where they do not.
+            const bool vec = a.src_rs % 4 == 0 && a.dst_rs % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.src) | reinterpret_cast<uintptr_t>(a.dst)) & 15) == 0;
+            const bool large = (uint64_t)a.B * ((a.V + 4095) / 4096) >= 2 * zg_sm_count();
+            const uint32_t slice = large ? 4096 : 1024;
+            const dim3 grid((a.V + slice - 1) / slice, a.B);
+            const size_t smem = slice * (a.bias ? 8 : 4);
+            if (large) { if (vec) launch_pdl(k_logit_rules<4, true>, grid, dim3(kLrThreads), smem, st, a); else launch_pdl(k_logit_rules<4, false>, grid, dim3(kLrThreads), smem, st, a); }
+            else if (vec) launch_pdl(k_logit_rules<1, true>, grid, dim3(kLrThreads), smem, st, a);
+            else launch_pdl(k_logit_rules<1, false>, grid, dim3(kLrThreads), smem, st, a);
             ZG_SEQ_CHECK();
             return true;
         }

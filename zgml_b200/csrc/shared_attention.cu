@@ -68,11 +68,18 @@ __device__ __forceinline__ float4 sa_load(const float* p, uint32_t d, uint32_t n
 // What bounds it is instruction latency beside the reads: 32 rows with 257 keys of their own on average took 53 us with one key per lane group and turn and the lane groups
 // merged by shuffles (600 instructions a turn of 4 keys).
 constexpr uint32_t kSaRing = 2, kSaMaxWarps = 8, kSaCluster = 8, kSaMost = 256 + 64;      // most records that meet: of 8 warps' lane groups and of the prefix
-__device__ __forceinline__ float sa_remote(const float* p, uint32_t rank) {
+__device__ __forceinline__ float2 sa_remote2(const float* p, uint32_t rank) {
     uint32_t at;
-    float v;
+    float2 v;
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 sa_remote4(const float* p, uint32_t rank) {
+    uint32_t at;
+    float4 v;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
     return v;
 }
 __device__ __forceinline__ void sa_cluster_sync() {
@@ -296,7 +303,7 @@ __global__ void __launch_bounds__(32 * kSaMaxWarps) k_shared_rows(const SaArgs a
         const float* prefix = a.shares ? sa_record(a, r, h0 + i, 0) : nullptr;
         float sum;
         const float top = sa_weights(weight[i], a.splits + n_prefix, [&](uint32_t e) {
-            return e < a.splits ? make_float2(sa_remote(sums + i * rec, e), sa_remote(sums + i * rec + 1, e)) : *reinterpret_cast<const float2*>(prefix + (size_t)(e - a.splits) * (4 + a.dv)); }, &sum);
+            return e < a.splits ? sa_remote2(sums + i * rec, e) : *reinterpret_cast<const float2*>(prefix + (size_t)(e - a.splits) * (4 + a.dv)); }, &sum);
         if (lane == 0) { top_of[i] = top; sum_of[i] = sum; }
     }
     __syncthreads();
@@ -304,10 +311,11 @@ __global__ void __launch_bounds__(32 * kSaMaxWarps) k_shared_rows(const SaArgs a
     for (uint32_t x = threadIdx.x; x < nq * width; x += blockDim.x) {
         const uint32_t i = x / width, d = 4 * (q0 + x % width);
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (uint32_t e = 0; e < a.splits; e++) {
-            const float* from = sums + i * rec + 4 + d;
-            add(v, make_float4(sa_remote(from, e), sa_remote(from + 1, e), sa_remote(from + 2, e), sa_remote(from + 3, e)), weight[i][e]);
-        }
+        float4 y[kSaCluster];                                       // all on their way before the first is added
+#pragma unroll
+        for (uint32_t e = 0; e < kSaCluster; e++) if (e < a.splits) y[e] = sa_remote4(sums + i * rec + 4 + d, e);
+#pragma unroll
+        for (uint32_t e = 0; e < kSaCluster; e++) if (e < a.splits) add(v, y[e], weight[i][e]);
         if (n_prefix) add_prefix(v, i, d, a.splits);
         const float f = closing(i);
         store(i, d, make_float4(v.x * f, v.y * f, v.z * f, v.w * f));

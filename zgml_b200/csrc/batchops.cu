@@ -96,12 +96,13 @@ __device__ __forceinline__ LrRow lr_row(const float* table, uint32_t r) {
     w.repetition = __int_as_float(y.z); w.presence = __int_as_float(y.w); w.frequency = __int_as_float(z.x);
     return w;
 }
-constexpr uint32_t kLrSeen = 0x80000000u, kLrThreads = 256;
-// CTA (row, slice of the vocabulary): counts of the slice's tokens in the row's history (bit 31: the token occurs at all) and biases of the slice in shared memory, then the
+constexpr uint32_t kLrThreads = 256;
+// CTA (row, slice of the vocabulary): counts of the slice's tokens in the row's history (a half word for those before `first`, one for those from there on; LONG: bit 31 for
+// the former, where a history may hold more than 65535 words) and biases of the slice in shared memory, then the
 // logits, which were asked for at the start: a thread holds NV times four neighbours.  A history is read once per slice (from L2), which costs less than counts of a whole
 // vocabulary in memory: 64 rows over 128256 tokens with 4096 words each read 33 MB for it beside the 66 MB of logits.
-template <int NV, bool VEC>
-__global__ void __launch_bounds__(kLrThreads) k_logit_rules(LrArgs a) {
+template <int NV, bool VEC, bool LONG>
+__global__ void __launch_bounds__(kLrThreads, 6) k_logit_rules(LrArgs a) {
     pdl_enter();
     extern __shared__ uint4 lr_mem[];                                // [slice] counts, [slice] biases
     constexpr uint32_t slice = kLrThreads * 4 * NV;
@@ -143,7 +144,9 @@ __global__ void __launch_bounds__(kLrThreads) k_logit_rules(LrArgs a) {
             const int32_t* past = a.history + (size_t)w.slot * a.history_rows;
             auto count = [&](int32_t token, uint32_t i) {
                 const uint32_t t = (uint32_t)token - v0;             // tokens outside the vocabulary belong to no slice
-                if (t < n) { if (i >= (uint32_t)w.first) atomicAdd(counts + t, 1u); else atomicOr(counts + t, kLrSeen); }
+                if (t >= n) return;
+                if constexpr (LONG) { if (i >= (uint32_t)w.first) atomicAdd(counts + t, 1u); else atomicOr(counts + t, 0x80000000u); }
+                else atomicAdd(counts + t, i >= (uint32_t)w.first ? 1u : 0x10000u);
             };
             const uint32_t length = w.length, lead = min(length, (4u - ((uint32_t)(reinterpret_cast<uintptr_t>(past) >> 2) & 3u)) & 3u), body = (length - lead) / 4;
             if (threadIdx.x < lead) count(past[threadIdx.x], threadIdx.x);
@@ -180,7 +183,7 @@ __global__ void __launch_bounds__(kLrThreads) k_logit_rules(LrArgs a) {
     }
     auto rule = [&](float v, uint32_t c) {
         if (!c) return v;
-        const uint32_t made = c & ~kLrSeen;
+        const uint32_t made = c & (LONG ? 0x7fffffffu : 0xffffu);
         v = v > 0.0f ? v / w.repetition : v * w.repetition;
         return made ? v - w.presence - w.frequency * (float)made : v;
     };
@@ -209,6 +212,18 @@ __global__ void __launch_bounds__(kLrThreads) k_logit_rules(LrArgs a) {
 
 }  // namespace
 
+// As much shared memory as an SM has: six CTAs of 32 KB, once per kernel and device.
+template <auto KERNEL>
+static bool lr_carveout() {
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 64 && (done.load() >> dev & 1)) return true;
+    const cudaError_t e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
+    if (e != cudaSuccess) { zg_set_error("cudaFuncSetAttribute(shared memory carveout) failed: %s", cudaGetErrorString(e)); return false; }
+    if (dev < 64) done.fetch_or(1ull << dev);
+    return true;
+}
 bool zg_batch_op_valid(const ZgOp& op, const size_t* elems, size_t n_bufs, char* why, size_t why_n) {
     const ZgSeqOp& s = op.u.seq;
     auto fail = [&](const char* m) { snprintf(why, why_n, "%s", m); return false; };
@@ -286,13 +301,20 @@ bool zg_launch_batch_op(const ZgOp& op, float* const* bufs, const size_t* elems,
             a.mask_rows = given(5) ? (uint32_t)std::min<size_t>(elems[s.buf[5]] / ((a.V + 31) / 32), (size_t)1 << 31) : 0;
             // Slices of 4096 tokens where they fill the GPU, of 1024 where they do not.
             const bool vec = a.src_rs % 4 == 0 && a.dst_rs % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.src) | reinterpret_cast<uintptr_t>(a.dst)) & 15) == 0;
-            const bool large = (uint64_t)a.B * ((a.V + 4095) / 4096) >= 2 * zg_sm_count();
+            const bool large = a.history_rows >= 65536 || (uint64_t)a.B * ((a.V + 4095) / 4096) >= 2 * zg_sm_count();
             const uint32_t slice = large ? 4096 : 1024;
             const dim3 grid((a.V + slice - 1) / slice, a.B);
             const size_t smem = slice * (a.bias ? 8 : 4);
-            if (large) { if (vec) launch_pdl(k_logit_rules<4, true>, grid, dim3(kLrThreads), smem, st, a); else launch_pdl(k_logit_rules<4, false>, grid, dim3(kLrThreads), smem, st, a); }
-            else if (vec) launch_pdl(k_logit_rules<1, true>, grid, dim3(kLrThreads), smem, st, a);
-            else launch_pdl(k_logit_rules<1, false>, grid, dim3(kLrThreads), smem, st, a);
+#define ZG_RULES(NV_, VEC_, LONG_)                                                                                                     \
+    do {                                                                                                                               \
+        if (!lr_carveout<k_logit_rules<NV_, VEC_, LONG_>>()) return false;                                                             \
+        launch_pdl(k_logit_rules<NV_, VEC_, LONG_>, grid, dim3(kLrThreads), smem, st, a);                                              \
+    } while (0)
+            if (a.history_rows >= 65536) { if (vec) ZG_RULES(4, true, true); else ZG_RULES(4, false, true); }
+            else if (large) { if (vec) ZG_RULES(4, true, false); else ZG_RULES(4, false, false); }
+            else if (vec) ZG_RULES(1, true, false);
+            else ZG_RULES(1, false, false);
+#undef ZG_RULES
             ZG_SEQ_CHECK();
             return true;
         }

@@ -372,18 +372,17 @@ __global__ void __launch_bounds__(256) k_shared_merge(const SaArgs a) {
 // ── the prefix on the tensor cores ───────────────────────────────────────────────────────────────────────────────────
 // All query rows of a key head meet the same keys of the prefix, so its part of the attention is two matrix products.  CTA (key head, share of the prefix, tile of 128 query
 // rows): 64 keys and values at a time are read from the cache once, split into half-precision pairs on their way to shared memory (one scale per tile;
-// split_tc.cuh) and multiplied by tcgen05.mma, three MMAs a product.  The 16 warps load tile t + 2, split tile t + 1 and take the softmax of tile t; four threads share a
-// query row, each with a quarter of the keys and of the output columns.  Warp 0 issues the scores, warp 5 the products with the values.  (With a warp of its
-// own for the issue 17 warps had 96 registers each and spilled; 16 have 128.)
+// split_tc.cuh) and multiplied by tcgen05.mma, three MMAs a product.  Warps 16 - 23 load and split, warp 24 issues, warps 0 - 15 are the softmax: four threads share a query
+// row, each with a quarter of the keys and of the output columns.  (With all of it in the same 16 warps, one phase after the other, a tile took 7700 clocks.)
 //   TMEM: scores of two tiles, which become the probabilities in place (A operand), outputs of two tiles, the queries' pairs (A operand).
 //   Elements of a pair are off by at most 2^-25 where the largest of a row or tile is below 2^15 (split_tc.cuh), so a score by at most 2 dk 2^-10 times its scales'
 //   inverses; with those times log2(e) below kSpLoud = 2^-17 that is less than 2^-18 for 128 dims.  Louder scores (beyond 2^20), values that are small as a whole beside others of their tile
 //   and what is not finite are found on the way; the CTA then walks its share again in plain f32.
 // Every wait is bounded; a CTA whose wait ran out counts it and makes NaN of its rows.
-constexpr uint32_t kSpThreads = 512, kSpStages = 3, kSpKeys = 64;
+constexpr uint32_t kSpRows = 512, kSpSplit = 256, kSpThreads = kSpRows + kSpSplit + 128, kSpStages = 3, kSpKeys = 64;      // threads: softmax, splitting, issue (one warp of four)
 template <int NC, int DV> struct SpLayout {
     static constexpr uint32_t k_part = NC * kSpKeys * 128, v_part = DV * 128, stage = 2 * (k_part + v_part);      // bytes; a part: hi or lo
-    static constexpr uint32_t share = kSpStages * stage, factors = share + 2 * 4 * 128 * 4, red = factors + kSpStages * 16, rows = red + 2 * 32 * 4, bars = rows + 128 * 4, size = bars + 128 + 1024;
+    static constexpr uint32_t share = kSpStages * stage, factors = share + 2 * 4 * 128 * 4, red = factors + kSpStages * 16, rows = red + 4 * 8 * 4, bars = rows + 128 * 4, size = bars + 128 + 1024;
 };
 constexpr float kSpLoud = 1.0f / 131072.0f;
 // Eight values of one column, or two of one key, that are not zero but below these parts of the tile's largest: a pair keeps 22 bits of a value above 2^-18, 19 above 2^-21.
@@ -441,17 +440,17 @@ __global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const __grid_co
     extern __shared__ uint8_t dsm_raw[];
     const uint32_t base = (smem_u32(dsm_raw) + 1023u) & ~1023u;
     uint8_t* const mem = dsm_raw + (base - smem_u32(dsm_raw));
-    const uint32_t full = base + L::bars, empty = full + 8 * kSpStages, s_full = empty + 8 * kSpStages, o_full = s_full + 16, p_full = o_full + 16, q_full = p_full + 8, tmem_slot = q_full + 8;
+    const uint32_t full = base + L::bars, empty = full + 8 * kSpStages, s_full = empty + 8 * kSpStages, o_full = s_full + 16, p_full = o_full + 16, q_full = p_full + 16, tmem_slot = q_full + 8;
     uint32_t* const trouble = reinterpret_cast<uint32_t*>(mem + (tmem_slot + 4 - base));          // 1: something that pairs cannot hold, 2: a wait that ran out
     const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;      // (in a form that the compiler knows to be the same in all lanes)
     if (threadIdx.x == 0) {
-        for (uint32_t i = 0; i < kSpStages; i++) { mbar_init(full + 8 * i, 16); mbar_init(empty + 8 * i, 1); }
-        for (uint32_t i = 0; i < 2; i++) { mbar_init(s_full + 8 * i, 1); mbar_init(o_full + 8 * i, 1); }
-        mbar_init(p_full, 16); mbar_init(q_full, 16);
+        for (uint32_t i = 0; i < kSpStages; i++) { mbar_init(full + 8 * i, 8); mbar_init(empty + 8 * i, 1); }
+        for (uint32_t i = 0; i < 2; i++) { mbar_init(s_full + 8 * i, 1); mbar_init(o_full + 8 * i, 1); mbar_init(p_full + 8 * i, 16); }
+        mbar_init(q_full, 16);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         *trouble = 0;
     }
-    if (warp == 0) {
+    if (warp == 24) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(tmem_slot) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -474,90 +473,176 @@ __global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const __grid_co
     __syncthreads();
     fence_after();
 
-    if (n_tiles) {
-        constexpr int OW = DV / 4, KT = DV == 128 ? 8 : 4;               // output columns and value rows of a thread
-        const uint32_t part = warp >> 2, row = (warp & 3) * 32 + lane, lanes = ((warp & 3) * 32) << 16, half = lane >> 4, hl = lane & 15;
-        const uint32_t v_key = DV == 128 ? 16 * (warp & 3) + 8 * half : 8 * (warp & 7) + 4 * half, v_col = 32 * (DV == 128 ? warp >> 2 : warp >> 3) + 2 * hl;
-        float* const share = reinterpret_cast<float*>(mem + L::share);
-        float2* const factors = reinterpret_cast<float2*>(mem + L::factors);      // of a stage's keys and values
-        uint32_t* const red = reinterpret_cast<uint32_t*>(mem + L::red);
-        bool ok = true, slow = false;
-        float f = 0.0f;                                                  // a score in units of log2 is f times the keys' factor times the product
-        float4 kr[2][NC];                                                // keys 2 warp + half and 32 more, 4 dims of every chunk of 64
-        float2 vr[KT];                                                   // KT values, two columns
-        auto load = [&](uint32_t t) {
-            const uint32_t u0 = c.k0 + t * kSpKeys;
+    // Registers: 896 threads of 72 at launch, 64512 in all = 512 x 72 + 256 x 96 + 128 x 24.
+    if (warp >= 24) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 24;");
+        if (n_tiles && warp == 24) {
+            // Issue.  Three products, the small ones first: hi lo, lo hi, hi hi.  B parts: hi, then lo; chunks of 64 along the summed dimension are 8 KB apart.  The whole warp
+            // does all but the issue itself, so that addresses stay warp-uniform.
+            constexpr uint32_t idesc_s = (1u << 4) | ((kSpKeys >> 3) << 17) | ((128u >> 4) << 24), idesc_o = (1u << 4) | ((DV >> 3) << 17) | ((128u >> 4) << 24);      // f16 x f16 -> f32
+            uint32_t in = 0, in_phase = 0, out = 0;                      // stages of the next scores and values
+            bool ok = __all_sync(0xffffffffu, mbar_wait(q_full, 0));
+            auto scores = [&](uint32_t t) {
+                const uint32_t d = kS + (t & 1) * kSpKeys, b = desc_low(base) + in * (L::stage >> 4);
+                if (ok) ok = __all_sync(0xffffffffu, mbar_wait(full + 8 * in, in_phase));
+                fence_after();
+                if (elect_one() && ok) {
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const uint32_t u = u0 + 32 * j + 2 * warp + half;
+                    for (uint32_t x = 0; x < 3; x++)
 #pragma unroll
-                for (int i = 0; i < NC; i++) kr[j][i] = sa_load<true>(c.kp + (size_t)u * a.pkw, 64 * i + 4 * hl, a.dk, u < c.k1);
-            }
-#pragma unroll
-            for (int j = 0; j < KT; j++) {
-                const uint32_t u = u0 + v_key + j;
-                vr[j] = u < c.k1 && v_col < a.dv ? *reinterpret_cast<const float2*>(c.vp + (size_t)u * a.pvw + v_col) : make_float2(0.0f, 0.0f);
-            }
-        };
-        uint32_t fill = 0, fill_phase = 1;                               // the stage that is filled next
-        auto convert = [&](uint32_t t) {
-            uint8_t* const stage = mem + fill * L::stage;
-            float km = 0.0f, c0 = 0.0f, c1 = 0.0f;
-            uint32_t least = 0xffffffffu;                                // the smallest of the keys' two values, zeros left out
-#pragma unroll
-            for (int j = 0; j < 2; j++)
-#pragma unroll
-                for (int i = 0; i < NC; i++) km = fmaxf(fmaxf(fmaxf(km, fabsf(kr[j][i].x)), fmaxf(fabsf(kr[j][i].y), fabsf(kr[j][i].z))), fabsf(kr[j][i].w));
-#pragma unroll
-            for (int j = 0; j < KT; j++) {
-                c0 = fmaxf(c0, fabsf(vr[j].x)); c1 = fmaxf(c1, fabsf(vr[j].y));
-                least = min(least, __float_as_uint(fmaxf(fabsf(vr[j].x), fabsf(vr[j].y))) - 1u);
-            }
-            // magnitudes order as their bits do
-            const uint32_t k_top = __reduce_max_sync(0xffffffffu, __float_as_uint(km)), v_top = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(c0, c1)));
-            if (lane == 0) { red[(t & 1) * 32 + warp] = k_top; red[(t & 1) * 32 + 16 + warp] = v_top; }
-            bar_sync(5, kSpThreads);
-            km = __uint_as_float(__reduce_max_sync(0xffffffffu, red[(t & 1) * 32 + (lane & 15)]));
-            const float vm = __uint_as_float(__reduce_max_sync(0xffffffffu, red[(t & 1) * 32 + 16 + (lane & 15)]));
-            float ks, k_inv, vs, v_inv;
-            split_scale(km, ks, k_inv);
-            split_scale(vm, vs, v_inv);
-            slow = slow || !(v_inv == v_inv) || !(fabsf(f * k_inv) <= kSpLoud) || least < __float_as_uint(vm * kSpKey) || (c0 > 0.0f && c0 < vm * kSpColumn) || (c1 > 0.0f && c1 < vm * kSpColumn);
-            if (threadIdx.x == 0) factors[fill] = make_float2(k_inv, v_inv);
-            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * fill, fill_phase));
-            uint8_t* const k_out = stage + (2 * warp + half) * 128 + (((hl >> 1) ^ ((2 * warp + half) & 7)) << 4) + 8 * (hl & 1);
-#pragma unroll
-            for (int j = 0; j < 2; j++)
-#pragma unroll
-                for (int i = 0; i < NC; i++) {
-                    uint2 hi, lo;
-                    split2(kr[j][i].x * ks, kr[j][i].y * ks, hi.x, lo.x); split2(kr[j][i].z * ks, kr[j][i].w * ks, hi.y, lo.y);
-                    uint8_t* const out = k_out + i * kSpKeys * 128 + j * 32 * 128;
-                    *reinterpret_cast<uint2*>(out) = hi;
-                    *reinterpret_cast<uint2*>(out + L::k_part) = lo;
+                        for (uint32_t k = 0; k < 4 * NC; k++) {
+                            const uint32_t qa = kQ + (x == 1 ? 32 * NC : 0) + 8 * k, kb = b + (x == 0 ? L::k_part >> 4 : 0) + (k / 4) * (kSpKeys * 128 >> 4) + 2 * (k % 4);
+                            if (x == 0 && k == 0) mma_ts<false>(d, qa, kb, idesc_s); else mma_ts<true>(d, qa, kb, idesc_s);
+                        }
+                    mma_commit(s_full + 8 * (t & 1));
                 }
+                __syncwarp();
+                if (++in == kSpStages) { in = 0; in_phase ^= 1; }
+            };
+            // probabilities of 16 keys lie in 16 columns: 8 with their hi pairs, 8 with their lo pairs
+            auto values = [&](uint32_t t) {
+                const uint32_t d = kO + (t & 1) * DV, pa = kS + (t & 1) * kSpKeys, b = desc_low(base) + out * (L::stage >> 4) + (2 * L::k_part >> 4), freed = empty + 8 * out;
+                if (ok) ok = __all_sync(0xffffffffu, mbar_wait(p_full + 8 * (t & 1), (t >> 1) & 1));
+                fence_after();
+                if (elect_one() && ok) {
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                uint32_t hi[KT / 2], lo[KT / 2];
+                    for (uint32_t x = 0; x < 3; x++)
 #pragma unroll
-                for (int j = 0; j < KT; j += 2) split2((e ? vr[j].y : vr[j].x) * vs, (e ? vr[j + 1].y : vr[j + 1].x) * vs, hi[j / 2], lo[j / 2]);
-                const uint32_t col = v_col + e;
-                uint8_t* const out = stage + 2 * L::k_part + col * 128 + (((v_key >> 3) ^ (col & 7)) << 4) + 2 * (v_key & 7);
-                if constexpr (KT == 8) {
-                    *reinterpret_cast<uint4*>(out) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    *reinterpret_cast<uint4*>(out + L::v_part) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                } else {
-                    *reinterpret_cast<uint2*>(out) = make_uint2(hi[0], hi[1]);
-                    *reinterpret_cast<uint2*>(out + L::v_part) = make_uint2(lo[0], lo[1]);
+                        for (uint32_t k = 0; k < kSpKeys / 16; k++) {
+                            const uint32_t p = pa + 16 * k + (x == 1 ? 8 : 0), vb = b + (x == 0 ? L::v_part >> 4 : 0) + 2 * k;
+                            if (x == 0 && k == 0) mma_ts<false>(d, p, vb, idesc_o); else mma_ts<true>(d, p, vb, idesc_o);
+                        }
+                    mma_commit(o_full + 8 * (t & 1));
+                    mma_commit(freed);
                 }
+                __syncwarp();
+                if (++out == kSpStages) out = 0;
+            };
+            // (probabilities of tile t - 2, which scores of tile t overwrite, have been multiplied: products execute in order)
+            for (uint32_t t = 0; t < n_tiles; t++) {
+                scores(t);
+                if (t) values(t - 1);
             }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            values(n_tiles - 1);
+            if (!ok && lane == 0) { count_timeout(); atomicOr(trouble, 2u); }
             __syncwarp();
-            if (lane == 0) mbar_arrive(full + 8 * fill);
-            if (++fill == kSpStages) { fill = 0; fill_phase ^= 1; }
-        };
-        load(0);
-        // The queries come by whole rows into the later stages, and a thread takes its quarter row from there.
+        }
+    } else if (warp >= 16) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 96;");
+        if (n_tiles) {
+            // ── keys and values: global memory, registers, pairs in shared memory ──
+            constexpr int KT = DV == 128 ? 8 : 4;                        // value rows of a thread, of two blocks of 32 columns
+            const uint32_t sw = warp - 16, half = lane >> 4, hl = lane & 15;
+            const uint32_t v_key = DV == 128 ? 16 * (sw & 3) + 8 * half : 8 * sw + 4 * half, v_col = (DV == 128 ? 64 * (sw >> 2) : 0) + 2 * hl;
+            float2* const factors = reinterpret_cast<float2*>(mem + L::factors);
+            uint32_t* const red = reinterpret_cast<uint32_t*>(mem + L::red);
+            bool ok = true, slow = false;
+            float4 kr[4][NC];                                            // keys 16 j + 2 sw + half, 4 dims of every chunk of 64
+            float2 vr[2][KT];                                            // KT values, two columns of each block
+            const float* const k_from = c.kp + (size_t)(c.k0 + 2 * sw + half) * a.pkw;
+            const float* const v_from = c.vp + (size_t)(c.k0 + v_key) * a.pvw + v_col;
+            auto load_keys = [&](uint32_t t) {
+#pragma unroll
+                for (uint32_t j = 0; j < 4; j++) {
+                    const uint32_t u = t * kSpKeys + 16 * j;
+#pragma unroll
+                    for (int i = 0; i < NC; i++) kr[j][i] = sa_load<true>(k_from + (size_t)u * a.pkw, 64 * i + 4 * hl, a.dk, c.k0 + 2 * sw + half + u < c.k1);
+                }
+            };
+            auto load_values = [&](uint32_t t) {
+#pragma unroll
+                for (int b = 0; b < 2; b++)
+#pragma unroll
+                    for (uint32_t j = 0; j < KT; j++) {
+                        const uint32_t u = t * kSpKeys + j;
+                        vr[b][j] = c.k0 + v_key + u < c.k1 && v_col + 32 * b < a.dv ? *reinterpret_cast<const float2*>(v_from + (size_t)u * a.pvw + 32 * b) : make_float2(0.0f, 0.0f);
+                    }
+            };
+            // the largest magnitude over the warps, from a warp's; magnitudes order as their bits do
+            auto over_warps = [&](float x, uint32_t at) {
+                const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(x));
+                if (lane == 0) red[at * 8 + sw] = top;
+                bar_sync(5, kSpSplit);
+                return __uint_as_float(__reduce_max_sync(0xffffffffu, red[at * 8 + (lane & 7)]));
+            };
+            uint32_t fill = 0, fill_phase = 1;                           // the stage that is filled next
+            load_keys(0);
+            load_values(0);
+#pragma unroll 1
+            for (uint32_t t = 0; t < n_tiles; t++) {
+                uint8_t* const stage = mem + fill * L::stage;
+                float km = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+#pragma unroll
+                    for (int i = 0; i < NC; i++) km = fmaxf(fmaxf(fmaxf(km, fabsf(kr[j][i].x)), fmaxf(fabsf(kr[j][i].y), fabsf(kr[j][i].z))), fabsf(kr[j][i].w));
+                km = over_warps(km, t & 1);                              // (two places in turns: one barrier is enough)
+                float ks, k_inv, vs, v_inv;
+                split_scale(km, ks, k_inv);
+                if (ok) ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * fill, fill_phase));
+                if (t == 1 && ok) ok = __all_sync(0xffffffffu, mbar_wait(q_full, 0));      // the queries pass through the later stages
+                uint8_t* const k_out = stage + (2 * sw + half) * 128 + (((hl >> 1) ^ ((2 * sw + half) & 7)) << 4) + 8 * (hl & 1);
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+#pragma unroll
+                    for (int i = 0; i < NC; i++) {
+                        uint2 hi, lo;
+                        split2(kr[j][i].x * ks, kr[j][i].y * ks, hi.x, lo.x); split2(kr[j][i].z * ks, kr[j][i].w * ks, hi.y, lo.y);
+                        uint8_t* const out = k_out + i * kSpKeys * 128 + j * 16 * 128;
+                        *reinterpret_cast<uint2*>(out) = hi;
+                        *reinterpret_cast<uint2*>(out + L::k_part) = lo;
+                    }
+                if (t + 1 < n_tiles) load_keys(t + 1);
+                float vm = 0.0f, cm[2][2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
+                uint32_t least = 0xffffffffu;                            // the smallest of the keys' two values, zeros left out
+#pragma unroll
+                for (int b = 0; b < 2; b++) {
+#pragma unroll
+                    for (int j = 0; j < KT; j++) {
+                        cm[b][0] = fmaxf(cm[b][0], fabsf(vr[b][j].x)); cm[b][1] = fmaxf(cm[b][1], fabsf(vr[b][j].y));
+                        least = min(least, __float_as_uint(fmaxf(fabsf(vr[b][j].x), fabsf(vr[b][j].y))) - 1u);
+                    }
+                    vm = fmaxf(vm, fmaxf(cm[b][0], cm[b][1]));
+                }
+                vm = over_warps(vm, 2 + (t & 1));
+                split_scale(vm, vs, v_inv);
+                slow = slow || !(k_inv == k_inv) || !(v_inv == v_inv) || least < __float_as_uint(vm * kSpKey);
+#pragma unroll
+                for (int b = 0; b < 2; b++) slow = slow || (cm[b][0] > 0.0f && cm[b][0] < vm * kSpColumn) || (cm[b][1] > 0.0f && cm[b][1] < vm * kSpColumn);
+                if (sw == 0 && lane == 0) factors[fill] = make_float2(k_inv, v_inv);
+#pragma unroll
+                for (int b = 0; b < 2; b++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        uint32_t hi[KT / 2], lo[KT / 2];
+#pragma unroll
+                        for (int j = 0; j < KT; j += 2) split2((e ? vr[b][j].y : vr[b][j].x) * vs, (e ? vr[b][j + 1].y : vr[b][j + 1].x) * vs, hi[j / 2], lo[j / 2]);
+                        const uint32_t col = v_col + 32 * b + e;
+                        uint8_t* const out = stage + 2 * L::k_part + col * 128 + (((v_key >> 3) ^ (col & 7)) << 4) + 2 * (v_key & 7);
+                        if constexpr (KT == 8) {
+                            *reinterpret_cast<uint4*>(out) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                            *reinterpret_cast<uint4*>(out + L::v_part) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                        } else {
+                            *reinterpret_cast<uint2*>(out) = make_uint2(hi[0], hi[1]);
+                            *reinterpret_cast<uint2*>(out + L::v_part) = make_uint2(lo[0], lo[1]);
+                        }
+                    }
+                if (slow) atomicOr(trouble, 1u);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(full + 8 * fill);
+                if (t + 1 < n_tiles) load_values(t + 1);
+                if (++fill == kSpStages) { fill = 0; fill_phase ^= 1; }
+            }
+            if (!ok && lane == 0) { count_timeout(); atomicOr(trouble, 2u); }
+        }
+    } else if (n_tiles) {
+        // ── softmax: four threads per query row ──
+        constexpr int OW = DV / 4;                                       // output columns of a thread
+        const uint32_t part = warp >> 2, row = (warp & 3) * 32 + lane, lanes = ((warp & 3) * 32) << 16;
+        float* const share = reinterpret_cast<float*>(mem + L::share);
+        const float2* const factors = reinterpret_cast<const float2*>(mem + L::factors);      // of a stage's keys and values
+        bool ok = true, slow = false;
         uint32_t n_share = 0;
         auto row_max = [&](float x) {                                    // over the row's four threads; two buffers in turns, so one barrier is enough
             float* s = share + (n_share++ & 1) * 512;
@@ -565,10 +650,12 @@ __global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const __grid_co
             bar_sync(1 + (warp & 3), 128);
             return fmaxf(fmaxf(s[row], s[128 + row]), fmaxf(s[256 + row], s[384 + row]));
         };
+        float f;                                                         // a score in units of log2 is f times the keys' factor times the product
+        // The queries come by whole rows into the later stages, and a thread takes its quarter row from there.
         {
             float* const stage = reinterpret_cast<float*>(mem + L::stage);
             constexpr uint32_t Q4 = 16 * NC;                             // float4s of a row; float4 j of row r lies at place j ^ (r & 7)
-            for (uint32_t i = threadIdx.x; i < 128 * Q4; i += kSpThreads) {
+            for (uint32_t i = threadIdx.x; i < 128 * Q4; i += kSpRows) {
                 const uint32_t r = i / Q4, j = i % Q4;
                 const uint32_t w = rows[r];
                 const bool on = w != 0xffffffffu && 4 * j < a.dk;
@@ -577,7 +664,7 @@ __global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const __grid_co
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
             asm volatile("cp.async.wait_group 0;" ::: "memory");
-            bar_sync(5, kSpThreads);
+            bar_sync(6, kSpRows);
             float4 x[4 * NC];                                            // 16 NC dims from 16 NC part on
             float mx = 0.0f, qs, q_inv;
 #pragma unroll
@@ -601,8 +688,8 @@ __global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const __grid_co
             f = q_inv * fabsf(a.scale) * kLog2e;
             tmem_wait_st();
             fence_before();
-            bar_sync(5, kSpThreads);                                     // the stages are free
-            if (lane == 0) mbar_arrive(q_full);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full);                          // the queries are there, and the stages are free
         }
         float o[OW];
 #pragma unroll
@@ -611,75 +698,32 @@ __global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const __grid_co
         auto add_output = [&](uint32_t t) {                              // outputs of tile t join the running ones
             if (ok) ok = __all_sync(0xffffffffu, mbar_wait(o_full + 8 * (t & 1), (t >> 1) & 1));
             fence_after();
-            uint32_t v[OW];
-            tmem_ld(lanes + kO + (t & 1) * DV + OW * part, v);
-            tmem_wait_ld(v);
 #pragma unroll
-            for (int j = 0; j < OW; j += 2) {
-                const float2 r = __ffma2_rn(make_float2(o[j], o[j + 1]), make_float2(alpha_prev, alpha_prev),
-                                            __fmul2_rn(make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), make_float2(f_prev, f_prev)));
-                o[j] = r.x; o[j + 1] = r.y;
+            for (int h = 0; h < OW; h += 16) {                           // sixteen at a time: registers
+                uint32_t v[16];
+                tmem_ld(lanes + kO + (t & 1) * DV + OW * part + h, v);
+                tmem_wait_ld(v);
+#pragma unroll
+                for (int j = 0; j < 16; j += 2) {
+                    const float2 r = __ffma2_rn(make_float2(o[h + j], o[h + j + 1]), make_float2(alpha_prev, alpha_prev),
+                                                __fmul2_rn(make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), make_float2(f_prev, f_prev)));
+                    o[h + j] = r.x; o[h + j + 1] = r.y;
+                }
             }
         };
-        // Issue.  Three products, the small ones first: hi lo, lo hi, hi hi.  B parts: hi, then lo; chunks of 64 along the summed dimension are 8 KB apart.  The whole warp does
-        // all but the issue itself, so that addresses stay warp-uniform.
-        constexpr uint32_t idesc_s = (1u << 4) | ((kSpKeys >> 3) << 17) | ((128u >> 4) << 24), idesc_o = (1u << 4) | ((DV >> 3) << 17) | ((128u >> 4) << 24);      // f16 x f16 -> f32
-        uint32_t issued = 0, issued_phase = 0;                           // stage of the next issue
-        auto scores = [&](uint32_t t) {
-            const uint32_t d = kS + (t & 1) * kSpKeys, b = desc_low(base) + issued * (L::stage >> 4);
-            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(full + 8 * issued, issued_phase));
-            fence_after();
-            if (elect_one() && ok) {
-#pragma unroll
-                for (uint32_t x = 0; x < 3; x++)
-#pragma unroll
-                    for (uint32_t k = 0; k < 4 * NC; k++) {
-                        const uint32_t qa = kQ + (x == 1 ? 32 * NC : 0) + 8 * k, kb = b + (x == 0 ? L::k_part >> 4 : 0) + (k / 4) * (kSpKeys * 128 >> 4) + 2 * (k % 4);
-                        if (x == 0 && k == 0) mma_ts<false>(d, qa, kb, idesc_s); else mma_ts<true>(d, qa, kb, idesc_s);
-                    }
-                mma_commit(s_full + 8 * (t & 1));
-            }
-            __syncwarp();
-            if (++issued == kSpStages) { issued = 0; issued_phase ^= 1; }
-        };
-        // probabilities of 16 keys lie in 16 columns: 8 with their hi pairs, 8 with their lo pairs
-        auto values = [&](uint32_t t) {
-            const uint32_t d = kO + (t & 1) * DV, pa = kS + (t & 1) * kSpKeys, b = desc_low(base) + issued * (L::stage >> 4) + (2 * L::k_part >> 4), freed = empty + 8 * issued;
-            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(p_full, t & 1));
-            fence_after();
-            if (elect_one() && ok) {
-#pragma unroll
-                for (uint32_t x = 0; x < 3; x++)
-#pragma unroll
-                    for (uint32_t k = 0; k < kSpKeys / 16; k++) {
-                        const uint32_t p = pa + 16 * k + (x == 1 ? 8 : 0), vb = b + (x == 0 ? L::v_part >> 4 : 0) + 2 * k;
-                        if (x == 0 && k == 0) mma_ts<false>(d, p, vb, idesc_o); else mma_ts<true>(d, p, vb, idesc_o);
-                    }
-                mma_commit(o_full + 8 * (t & 1));
-                mma_commit(freed);
-            }
-            __syncwarp();
-            if (++issued == kSpStages) { issued = 0; issued_phase ^= 1; }
-        };
-        uint32_t at = 0;                                                 // stage of tile t
-        convert(0);
-        if (warp == 0) { if (ok) ok = __all_sync(0xffffffffu, mbar_wait(q_full, 0)); scores(0); }
-        if (n_tiles > 1) load(1);
+        uint32_t at = 0, at_phase = 0;                                   // stage of tile t
 #pragma unroll 1
         for (uint32_t t = 0; t < n_tiles; t++) {
-            if (t + 1 < n_tiles) {
-                convert(t + 1);
-                if (t + 2 < n_tiles) load(t + 2);
-            } else bar_sync(5, kSpThreads);                              // factors of tile t are there (inside the loop the barrier of the next tile says so)
             const uint32_t s = lanes + kS + (t & 1) * kSpKeys + 16 * part, u0 = c.k0 + t * kSpKeys + 16 * part;
-            const float2 inv = factors[at];
-            if (++at == kSpStages) at = 0;
-            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(s_full + 8 * (t & 1), (t >> 1) & 1));
+            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(full + 8 * at, at_phase) && mbar_wait(s_full + 8 * (t & 1), (t >> 1) & 1));      // (the former for the factors)
             fence_after();
+            const float2 inv = factors[at];
+            if (++at == kSpStages) { at = 0; at_phase ^= 1; }
             uint32_t v[16];
             tmem_ld(s, v);
             tmem_wait_ld(v);
             float x[16], unit = fmaxf(f * inv.x, 1e-37f);
+            slow = slow || !(fabsf(f * inv.x) <= kSpLoud);
 #pragma unroll
             for (int j = 0; j < 16; j++) x[j] = __uint_as_float(v[j]);
             if (a.cap > 0.0f) {                                          // here in units of log2
@@ -711,12 +755,10 @@ __global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const __grid_co
             tmem_wait_st();
             fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(p_full);
+            // (a barrier for even and one for odd tiles: warps may be a tile apart)
+            if (lane == 0) mbar_arrive(p_full + 8 * (t & 1));
             if (t) add_output(t - 1);
             alpha_prev = alpha; f_prev = inv.y;
-            // The products run beside the next tile's split.  Scores overwrite probabilities whose outputs have just been waited for.
-            if (warp == 0) { if (t + 1 < n_tiles) scores(t + 1); }
-            else if (warp == 5) values(t);
         }
         add_output(n_tiles - 1);
         {
@@ -733,13 +775,13 @@ __global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const __grid_co
         const uint32_t mine = rows[row];
         if (slow || (mine != 0xffffffffu && m < -1e36f)) atomicOr(trouble, 1u);
         if (!ok) { atomicOr(trouble, 2u); if (lane == 0) count_timeout(); }
-        bar_sync(5, kSpThreads);
+        bar_sync(6, kSpRows);
         const uint32_t what = *reinterpret_cast<volatile uint32_t*>(trouble);
         if (what == 1) sp_plain(a, c.kp, c.vp, c.k0, c.k1, c.split, rows);
         else {
             const bool lost = what & 2u;
             if (mine != 0xffffffffu && part == 0) { float* rec = sa_record(a, mine >> 10, mine & 1023, c.split); rec[0] = lost ? kBatchNaN : m * kLn2; rec[1] = lost ? kBatchNaN : l * p_unit; }
-            for (uint32_t i = threadIdx.x; i < 128 * (DV / 4); i += kSpThreads) {
+            for (uint32_t i = threadIdx.x; i < 128 * (DV / 4); i += kSpRows) {
                 const uint32_t r = i / (DV / 4), j = i % (DV / 4);
                 const uint32_t w = rows[r];
                 if (w == 0xffffffffu || 4 * j >= a.dv) continue;
@@ -751,7 +793,7 @@ __global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const __grid_co
     __syncwarp();
     fence_before();
     __syncthreads();
-    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(0u) : "memory");
+    if (warp == 24) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(0u) : "memory");
 }
 
 // What decides a launch: queries a CTA of k_shared_rows holds (RQ), float4 a lane holds (NV), lanes that share a key (LK), shares of its keys; shares of the prefix

@@ -17,6 +17,7 @@ struct SaArgs {
     uint32_t B, H, G, rep, dk, dv, q_rs, kw, vw, R, pkw, pvw, Rp, dst_rs, slots, pslots, sink_bf16;
     uint32_t shares, splits;         // shares of the prefix, which k_shared_prefix walks (0: k_shared_rows walks all keys), and of what is left to k_shared_rows
     float scale, cap;
+    uint32_t k_x, v_x;               // first columns of the prefix's key and value heads, for copies by tensor maps over whole rows
 };
 // What a row sees: `prefix` keys of the shared prefix, then `own` of its slot.
 struct SaKeys { const float* kp; const float* vp; const float* kc; const float* vc; uint32_t prefix, own; bool live, bad; };
@@ -372,17 +373,19 @@ __global__ void __launch_bounds__(256) k_shared_merge(const SaArgs a) {
 // ── the prefix on the tensor cores ───────────────────────────────────────────────────────────────────────────────────
 // All query rows of a key head meet the same keys of the prefix, so its part of the attention is two matrix products.  CTA (key head, share of the prefix, tile of 128 query
 // rows): 64 keys and values at a time are read from the cache once, split into half-precision pairs on their way to shared memory (one scale per tile;
-// split_tc.cuh) and multiplied by tcgen05.mma, three MMAs a product.  Warps 16 - 23 load and split, warp 24 issues, warps 0 - 15 are the softmax: four threads share a query
+// split_tc.cuh) and multiplied by tcgen05.mma, three MMAs a product.  Warp 25 copies (TMA), warps 16 - 23 split, warp 24 issues, warps 0 - 15 are the softmax: four threads share a query
 // row, each with a quarter of the keys and of the output columns.  (With all of it in the same 16 warps, one phase after the other, a tile took 7700 clocks.)
 //   TMEM: scores of two tiles, which become the probabilities in place (A operand), outputs of two tiles, the queries' pairs (A operand).
 //   Elements of a pair are off by at most 2^-25 where the largest of a row or tile is below 2^15 (split_tc.cuh), so a score by at most 2 dk 2^-10 times its scales'
 //   inverses; with those times log2(e) below kSpLoud = 2^-17 that is less than 2^-18 for 128 dims.  Louder scores (beyond 2^20), values that are small as a whole beside others of their tile
 //   and what is not finite are found on the way; the CTA then walks its share again in plain f32.
 // Every wait is bounded; a CTA whose wait ran out counts it and makes NaN of its rows.
-constexpr uint32_t kSpRows = 512, kSpSplit = 256, kSpThreads = kSpRows + kSpSplit + 128, kSpStages = 3, kSpKeys = 64;      // threads: softmax, splitting, issue (one warp of four)
+constexpr uint32_t kSpRows = 512, kSpSplit = 256, kSpThreads = kSpRows + kSpSplit + 128, kSpStages = 2, kSpKeys = 64;      // threads: softmax, splitting, issue and copies (two warps of four)
 template <int NC, int DV> struct SpLayout {
     static constexpr uint32_t k_part = NC * kSpKeys * 128, v_part = DV * 128, stage = 2 * (k_part + v_part);      // bytes; a part: hi or lo
-    static constexpr uint32_t share = kSpStages * stage, factors = share + 2 * 4 * 128 * 4, red = factors + kSpStages * 16, rows = red + 4 * 8 * 4, bars = rows + 128 * 4, size = bars + 128 + 1024;
+    // the queries pass through the second stage on their way to TMEM; keys and values as they come lie behind
+    static constexpr uint32_t k_raw = kSpStages * stage > stage + NC * 32768 ? kSpStages * stage : stage + NC * 32768, v_raw = k_raw + kSpKeys * 64 * NC * 4, share = v_raw + kSpKeys * DV * 4;
+    static constexpr uint32_t factors = share + 2 * 4 * 128 * 4, red = factors + kSpStages * 16, rows = red + 4 * 8 * 4, bars = rows + 128 * 4, size = bars + 192 + 1024;
 };
 constexpr float kSpLoud = 1.0f / 131072.0f;
 // Eight values of one column, or two of one key, that are not zero but below these parts of the tile's largest: a pair keeps 22 bits of a value above 2^-18, 19 above 2^-21.
@@ -433,19 +436,19 @@ __device__ __noinline__ void sp_plain(const SaArgs& a, const float* kp, const fl
     }
 }
 template <int NC, int DV>
-__global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const __grid_constant__ SaArgs a, const uint32_t row_tiles) {
+__global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const __grid_constant__ SaArgs a, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const uint32_t row_tiles) {
     typedef SpLayout<NC, DV> L;
     constexpr uint32_t kS = 0, kO = 2 * kSpKeys, kQ = kO + 2 * DV;         // TMEM columns
     static_assert(kQ + 64 * NC <= 512, "TMEM columns");
     extern __shared__ uint8_t dsm_raw[];
     const uint32_t base = (smem_u32(dsm_raw) + 1023u) & ~1023u;
     uint8_t* const mem = dsm_raw + (base - smem_u32(dsm_raw));
-    const uint32_t full = base + L::bars, empty = full + 8 * kSpStages, s_full = empty + 8 * kSpStages, o_full = s_full + 16, p_full = o_full + 16, q_full = p_full + 16, tmem_slot = q_full + 8;
+    const uint32_t full = base + L::bars, empty = full + 8 * kSpStages, s_full = empty + 8 * kSpStages, o_full = s_full + 16, p_full = o_full + 16, q_full = p_full + 16, tmem_slot = q_full + 8, raw_full = tmem_slot + 8, raw_empty = raw_full + 16;      // (the latter: keys, values)
     uint32_t* const trouble = reinterpret_cast<uint32_t*>(mem + (tmem_slot + 4 - base));          // 1: something that pairs cannot hold, 2: a wait that ran out
     const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;      // (in a form that the compiler knows to be the same in all lanes)
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < kSpStages; i++) { mbar_init(full + 8 * i, 8); mbar_init(empty + 8 * i, 1); }
-        for (uint32_t i = 0; i < 2; i++) { mbar_init(s_full + 8 * i, 1); mbar_init(o_full + 8 * i, 1); mbar_init(p_full + 8 * i, 16); }
+        for (uint32_t i = 0; i < 2; i++) { mbar_init(s_full + 8 * i, 1); mbar_init(o_full + 8 * i, 1); mbar_init(p_full + 8 * i, 16); mbar_init(raw_full + 8 * i, 1); mbar_init(raw_empty + 8 * i, 8); }
         mbar_init(q_full, 16);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         *trouble = 0;
@@ -526,6 +529,19 @@ __global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const __grid_co
             values(n_tiles - 1);
             if (!ok && lane == 0) { count_timeout(); atomicOr(trouble, 2u); }
             __syncwarp();
+        } else if (n_tiles && warp == 25) {
+            // copies: 64 rows of the prefix at a time, what lies behind the share among them
+            if (elect_one()) {
+                const uint32_t y0 = (uint32_t)head.prefix_slot * a.Rp + c.k0;
+                bool ok = true;
+                for (uint32_t t = 0; t < n_tiles && ok; t++) {
+                    ok = mbar_wait(raw_empty, (t & 1) ^ 1);
+                    if (ok) { mbar_expect_tx(raw_full, kSpKeys * a.dk * 4); tma_2d(base + L::k_raw, &map_k, a.k_x + c.g * a.dk, y0 + t * kSpKeys, raw_full); ok = mbar_wait(raw_empty + 8, (t & 1) ^ 1); }
+                    if (ok) { mbar_expect_tx(raw_full + 8, kSpKeys * a.dv * 4); tma_2d(base + L::v_raw, &map_v, a.v_x + c.g * a.dv, y0 + t * kSpKeys, raw_full + 8); }
+                }
+                if (!ok) { count_timeout(); atomicOr(trouble, 2u); }
+            }
+            __syncwarp();
         }
     } else if (warp >= 16) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 96;");
@@ -539,24 +555,31 @@ __global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const __grid_co
             bool ok = true, slow = false;
             float4 kr[4][NC];                                            // keys 16 j + 2 sw + half, 4 dims of every chunk of 64
             float2 vr[2][KT];                                            // KT values, two columns of each block
-            const float* const k_from = c.kp + (size_t)(c.k0 + 2 * sw + half) * a.pkw;
-            const float* const v_from = c.vp + (size_t)(c.k0 + v_key) * a.pvw + v_col;
+            // what TMA has brought -> registers; the place is free for the next tile then.  Keys behind the share count as zeros: what lies there is not looked at
+            const float* const k_raw = reinterpret_cast<const float*>(mem + L::k_raw);
+            const float* const v_raw = reinterpret_cast<const float*>(mem + L::v_raw);
             auto load_keys = [&](uint32_t t) {
+                if (ok) ok = __all_sync(0xffffffffu, mbar_wait(raw_full, t & 1));
 #pragma unroll
                 for (uint32_t j = 0; j < 4; j++) {
-                    const uint32_t u = t * kSpKeys + 16 * j;
+                    const uint32_t key = 16 * j + 2 * sw + half;
 #pragma unroll
-                    for (int i = 0; i < NC; i++) kr[j][i] = sa_load<true>(k_from + (size_t)u * a.pkw, 64 * i + 4 * hl, a.dk, c.k0 + 2 * sw + half + u < c.k1);
+                    for (int i = 0; i < NC; i++) kr[j][i] = sa_load<true>(k_raw + key * a.dk, 64 * i + 4 * hl, a.dk, c.k0 + t * kSpKeys + key < c.k1);
                 }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(raw_empty);
             };
             auto load_values = [&](uint32_t t) {
+                if (ok) ok = __all_sync(0xffffffffu, mbar_wait(raw_full + 8, t & 1));
 #pragma unroll
                 for (int b = 0; b < 2; b++)
 #pragma unroll
                     for (uint32_t j = 0; j < KT; j++) {
-                        const uint32_t u = t * kSpKeys + j;
-                        vr[b][j] = c.k0 + v_key + u < c.k1 && v_col + 32 * b < a.dv ? *reinterpret_cast<const float2*>(v_from + (size_t)u * a.pvw + 32 * b) : make_float2(0.0f, 0.0f);
+                        const uint32_t key = v_key + j;
+                        vr[b][j] = c.k0 + t * kSpKeys + key < c.k1 && v_col + 32 * b < a.dv ? *reinterpret_cast<const float2*>(v_raw + key * a.dv + v_col + 32 * b) : make_float2(0.0f, 0.0f);
                     }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(raw_empty + 8);
             };
             // the largest magnitude over the warps, from a warp's; magnitudes order as their bits do
             auto over_warps = [&](float x, uint32_t at) {
@@ -566,12 +589,11 @@ __global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const __grid_co
                 return __uint_as_float(__reduce_max_sync(0xffffffffu, red[at * 8 + (lane & 7)]));
             };
             uint32_t fill = 0, fill_phase = 1;                           // the stage that is filled next
-            load_keys(0);
-            load_values(0);
 #pragma unroll 1
             for (uint32_t t = 0; t < n_tiles; t++) {
                 uint8_t* const stage = mem + fill * L::stage;
                 float km = 0.0f;
+                load_keys(t);
 #pragma unroll
                 for (int j = 0; j < 4; j++)
 #pragma unroll
@@ -592,7 +614,7 @@ __global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const __grid_co
                         *reinterpret_cast<uint2*>(out) = hi;
                         *reinterpret_cast<uint2*>(out + L::k_part) = lo;
                     }
-                if (t + 1 < n_tiles) load_keys(t + 1);
+                load_values(t);
                 float vm = 0.0f, cm[2][2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
                 uint32_t least = 0xffffffffu;                            // the smallest of the keys' two values, zeros left out
 #pragma unroll
@@ -631,7 +653,6 @@ __global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const __grid_co
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(full + 8 * fill);
-                if (t + 1 < n_tiles) load_values(t + 1);
                 if (++fill == kSpStages) { fill = 0; fill_phase ^= 1; }
             }
             if (!ok && lane == 0) { count_timeout(); atomicOr(trouble, 2u); }
@@ -830,11 +851,25 @@ bool sa_vec(const ZgSeqOp& s) {
     for (uint32_t x : {s.n[3], s.n[4], s.n[5], s.n[6], s.n[7], s.off[0], s.off[1], s.off[2]}) if (x % 4) return false;
     return s.buf[4] == ZG_NO_BUF || !(s.n[9] % 4 || s.n[10] % 4 || s.off[3] % 4 || s.off[4] % 4);
 }
+// rows of a prefix cache, boxes of 64 rows of one head
+bool sa_encode(CUtensorMap* map, const float* base, uint64_t width, uint64_t rows, uint32_t dim) {
+    const cuuint64_t dims[2] = {width, rows}, stride[1] = {width * 4};
+    const cuuint32_t box[2] = {dim, kSpKeys}, one[2] = {1, 1};
+    EncodeTiledFn fn = encode_tiled();
+    if (!fn) { zg_set_error("cuTensorMapEncodeTiled entry point not available"); return false; }
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<float*>(base), dims, stride, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) { zg_set_error("cuTensorMapEncodeTiled(prefix) failed (%d)", (int)r); return false; }
+    return true;
+}
 template <int NC, int DV>
 bool sa_launch_prefix(const SaArgs& a, const SaShape& p, cudaStream_t st) {
     typedef SpLayout<NC, DV> L;
+    CUtensorMap mk, mv;
+    const uint64_t rows = (uint64_t)a.pslots * a.Rp;
+    if (!sa_encode(&mk, a.kp - a.k_x, a.pkw, rows, a.dk) || !sa_encode(&mv, a.vp - a.v_x, a.pvw, rows, a.dv)) return false;
     if (!zg_smem_limit<k_shared_prefix<NC, DV>>(L::size)) return false;
-    launch_pdl(k_shared_prefix<NC, DV>, dim3(p.row_tiles * a.shares * a.G), dim3(kSpThreads), L::size, st, a, p.row_tiles);
+    launch_pdl(k_shared_prefix<NC, DV>, dim3(p.row_tiles * a.shares * a.G), dim3(kSpThreads), L::size, st, a, mk, mv, p.row_tiles);
     return true;
 }
 template <int RQ, int NV, bool VEC>
@@ -889,7 +924,8 @@ bool zg_launch_shared_attention(const ZgOp& op, float* const* bufs, const size_t
     if (!prefix) { a.pkw = a.kw; a.pvw = a.vw; }
     auto slots = [&](int k, int v, size_t kn, size_t vn) { return (uint32_t)std::min<size_t>({elems[s.buf[k]] / kn, elems[s.buf[v]] / vn, (size_t)1 << 31}); };
     a.slots = slots(2, 3, (size_t)a.R * a.kw, (size_t)a.R * a.vw);
-    a.pslots = prefix ? slots(4, 5, (size_t)a.Rp * a.pkw, (size_t)a.Rp * a.pvw) : 0;
+    a.pslots = prefix ? std::min(slots(4, 5, (size_t)a.Rp * a.pkw, (size_t)a.Rp * a.pvw), 0x7fffffffu / a.Rp) : 0;      // (rows are counted in 31 bits)
+    a.k_x = s.off[3]; a.v_x = s.off[4];
     a.table = bufs[s.buf[6]];
     a.sink = s.buf[7] == ZG_NO_BUF ? nullptr : a.sink_bf16 ? (const void*)wptr<bf16>(bufs, s.buf[7], s.off[5]) : (const void*)wptr<float>(bufs, s.buf[7], s.off[5]);
     a.scale = s.f[0]; a.cap = s.f[1];

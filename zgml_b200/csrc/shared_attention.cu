@@ -89,6 +89,19 @@ __device__ __forceinline__ void sa_cluster_sync() {
 }
 __device__ __forceinline__ float sa_ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+// cap * tanh(s / cap), from the definition 1 - 2 / (e^2x + 1) and, where that cancels, the series to x^9 (the next term is below 2^-26 of the value there).  Sixteen
+// tanhf of a thread took 3700 clocks a tile.
+__device__ __forceinline__ float sa_capped(float s, float cap, float inv_cap) {
+    const float x = fabsf(s * inv_cap), x2 = x * x;
+    const float series = fmaf(x * x2, fmaf(x2, fmaf(x2, fmaf(x2, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), x);
+    const float far = 1.0f - __fdividef(2.0f, sa_ex2(x * (2.0f * kLog2e)) + 1.0f);
+    return copysignf(cap * (x < 0.25f ? series : x > 10.0f ? 1.0f : far), s);
+}
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
 template <bool VEC>
 __device__ __forceinline__ void sa_copy(uint32_t at, const float* p, uint32_t d, uint32_t n, bool on) {
     if constexpr (VEC) {
@@ -157,6 +170,7 @@ __global__ void __launch_bounds__(32 * kSaMaxWarps) k_shared_rows(const SaArgs a
     for (uint32_t t = 0; t < kSaRing - 1; t++) fetch(t);
     // Scores in units of log2: the scale and log2(e) are folded into the queries.
     const float unit = a.cap > 0.0f ? a.scale : a.scale * kLog2e;
+    const float inv_cap = a.cap > 0.0f ? 1.0f / a.cap : 0.0f;
     float2 q[RQ][2 * NV], o[RQ][2 * NV];
     float m[RQ], l[RQ];
 #pragma unroll
@@ -200,7 +214,7 @@ __global__ void __launch_bounds__(32 * kSaMaxWarps) k_shared_rows(const SaArgs a
         for (int i = 0; i < RQ; i++) {
 #pragma unroll
             for (int x = 0; x < 2; x++) {
-                if (a.cap > 0.0f) s[x][i] = a.cap * kLog2e * tanhf(s[x][i] / a.cap);
+                if (a.cap > 0.0f) s[x][i] = kLog2e * sa_capped(s[x][i], a.cap, inv_cap);
                 if (u + x * groups >= k1) s[x][i] = -INFINITY;
             }
             up = fmaxf(up, fmaxf(s[0][i], s[1][i]) > m[i] ? 1.0f : -1.0f);
@@ -487,9 +501,8 @@ __global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const __grid_co
             bool ok = __all_sync(0xffffffffu, mbar_wait(q_full, 0));
             auto scores = [&](uint32_t t) {
                 const uint32_t d = kS + (t & 1) * kSpKeys, b = desc_low(base) + in * (L::stage >> 4);
-                if (ok) ok = __all_sync(0xffffffffu, mbar_wait(full + 8 * in, in_phase));
                 fence_after();
-                if (elect_one() && ok) {
+                if (elect_one()) {
 #pragma unroll
                     for (uint32_t x = 0; x < 3; x++)
 #pragma unroll
@@ -505,9 +518,8 @@ __global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const __grid_co
             // probabilities of 16 keys lie in 16 columns: 8 with their hi pairs, 8 with their lo pairs
             auto values = [&](uint32_t t) {
                 const uint32_t d = kO + (t & 1) * DV, pa = kS + (t & 1) * kSpKeys, b = desc_low(base) + out * (L::stage >> 4) + (2 * L::k_part >> 4), freed = empty + 8 * out;
-                if (ok) ok = __all_sync(0xffffffffu, mbar_wait(p_full + 8 * (t & 1), (t >> 1) & 1));
                 fence_after();
-                if (elect_one() && ok) {
+                if (elect_one()) {
 #pragma unroll
                     for (uint32_t x = 0; x < 3; x++)
 #pragma unroll
@@ -521,12 +533,14 @@ __global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const __grid_co
                 __syncwarp();
                 if (++out == kSpStages) out = 0;
             };
-            // (probabilities of tile t - 2, which scores of tile t overwrite, have been multiplied: products execute in order)
-            for (uint32_t t = 0; t < n_tiles; t++) {
-                scores(t);
-                if (t) values(t - 1);
+            // Whichever is ready comes next.  (Scores before values in turns cost 1500 clocks a tile: the values waited for keys that waited for their stage.)  Scores of tile t
+            // overwrite the probabilities of tile t - 2, whose values have been issued: products execute in order.
+            uint32_t next_s = 0, next_v = 0, spins = 0;
+            while (ok && next_v < n_tiles) {
+                if (next_v < next_s && __all_sync(0xffffffffu, mbar_test(p_full + 8 * (next_v & 1), (next_v >> 1) & 1))) { values(next_v++); spins = 0; }
+                else if (next_s < n_tiles && next_s <= next_v + 1 && __all_sync(0xffffffffu, mbar_test(full + 8 * in, in_phase))) { scores(next_s++); spins = 0; }
+                else ok = ++spins < kTcSpin;
             }
-            values(n_tiles - 1);
             if (!ok && lane == 0) { count_timeout(); atomicOr(trouble, 2u); }
             __syncwarp();
         } else if (n_tiles && warp == 25) {
@@ -748,8 +762,9 @@ __global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const __grid_co
 #pragma unroll
             for (int j = 0; j < 16; j++) x[j] = __uint_as_float(v[j]);
             if (a.cap > 0.0f) {                                          // here in units of log2
+                const float inv_cap = 1.0f / a.cap;
 #pragma unroll
-                for (int j = 0; j < 16; j++) x[j] = a.cap * tanhf(x[j] * unit * kLn2 / a.cap) * kLog2e;
+                for (int j = 0; j < 16; j++) x[j] = sa_capped(x[j] * (unit * kLn2), a.cap, inv_cap) * kLog2e;
                 unit = 1.0f;
             }
             if (u0 + 16 > c.k1) {

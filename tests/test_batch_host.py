@@ -114,3 +114,14 @@ def test_logit_rules_in_place_and_without_operands():
 
 def test_check_of_other_things():
     assert seq_check(DeviceOp.softmax(0, 0, 1, 4), [4]) and seq_check(DeviceOp.activation(0, 1, 4, "relu"), [4]) and seq_check(DeviceOp.activation(0, 1, 4, "relu"), [4, 4]) is None
+
+
+def test_rules_of_the_command_line():
+    from argparse import Namespace
+    from zgml_b200.cli import _rules
+    a = dict(repetition_penalty=1.0, presence_penalty=0.0, frequency_penalty=0.0, bias="", allow="")
+    assert _rules(Namespace(**a)) is None
+    r = _rules(Namespace(**dict(a, repetition_penalty=1.2, bias="3:1.5,7:-2", allow="1,2")))
+    assert r.repetition == 1.2 and r.bias == {3: 1.5, 7: -2.0} and list(r.allowed) == [1, 2]
+    with pytest.raises(ValueError):
+        _rules(Namespace(**dict(a, repetition_penalty=0.0)))

@@ -1,6 +1,7 @@
 """Command line of the framework: `python -m zgml_b200 <command>`.
 
   generate   --model PATH --prompt 1,2,3 --max-new-tokens N [--temperature T --top-k K --top-p P --seed S]
+             [--repetition-penalty R --presence-penalty A --frequency-penalty B --bias ID:VALUE,… --allow ID,…]   (sequence models)
   trace-run  --model DIR --dtype bfloat16|float32 --out DIR --max-tokens N     (steps as JSON lines on standard input)
 
 `trace-run` replays a serving trace through the model's own session: one JSON object per line,
@@ -22,13 +23,27 @@ def _backend():
     return CudaBackend(0)
 
 
+def _rules(a):
+    """LogitRules of the command's options; None where it has none of them."""
+    if a.repetition_penalty == 1.0 and a.presence_penalty == 0.0 and a.frequency_penalty == 0.0 and not a.bias and not a.allow:
+        return None
+    from .host.batch import LogitRules
+    bias = {int(k): float(v) for k, v in (e.split(":") for e in a.bias.split(",") if e.strip())}
+    allowed = np.array([int(t) for t in a.allow.split(",") if t.strip()], np.int64) if a.allow else None
+    return LogitRules(a.repetition_penalty, a.presence_penalty, a.frequency_penalty, bias, allowed)
+
+
 def cmd_generate(a) -> int:
     from .host.registry import open_session
     from .host.sampling import Sampler
     be = _backend()
     prompt = [int(t) for t in a.prompt.split(",") if t.strip()]
     s = open_session(be, a.model, a.dtype, max_chunk=a.max_chunk, max_tokens=len(prompt) + a.max_new_tokens)
-    out = s.generate(prompt, a.max_new_tokens, Sampler(a.temperature, a.top_k, a.top_p, a.seed))
+    rules = _rules(a)
+    if rules is not None and not hasattr(s, "max_history"):
+        raise SystemExit("penalties, biases and masks need a sequence model (a folder with config.json)")
+    sampler = Sampler(a.temperature, a.top_k, a.top_p, a.seed)
+    out = s.generate(prompt, a.max_new_tokens, sampler) if rules is None else s.generate(prompt, a.max_new_tokens, sampler, rules=rules)
     print(",".join(str(t) for t in out))
     s.close()
     return 0
@@ -70,6 +85,11 @@ def main(argv=None) -> int:
     g.add_argument("--top-p", type=float, default=1.0)
     g.add_argument("--seed", type=int, default=None)
     g.add_argument("--max-chunk", type=int, default=256)
+    g.add_argument("--repetition-penalty", type=float, default=1.0, help="divides (negative logits: multiplies) the logits of tokens seen before")
+    g.add_argument("--presence-penalty", type=float, default=0.0, help="taken off the logits of tokens generated before")
+    g.add_argument("--frequency-penalty", type=float, default=0.0, help="taken off once for every time a token was generated")
+    g.add_argument("--bias", default="", help="comma-separated ID:VALUE, added to logits")
+    g.add_argument("--allow", default="", help="comma-separated token ids: no other token is chosen")
     g.set_defaults(fn=cmd_generate)
     t = sub.add_parser("trace-run", help="replay a serving trace and write the wanted logits")
     t.add_argument("--model", required=True)

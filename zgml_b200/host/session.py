@@ -12,6 +12,8 @@ A model object provides
 sizes (powers of two up to `max_chunk`, compiled on first use and kept), writes the control buffer (position, state slot,
 previous token, token ids) and executes; the CUDA graph of a program is replayed unchanged from step to step.  How a prompt is cut
 changes nothing but rounding: state is carried exactly, and every chunk attends through the same key ring.
+`feed(..., rules=LogitRules(...))` asks for the last place's logits as the request's penalties, biases and grammar mask leave them: LOGIT_RULES joins the program that
+makes them, over the tokens that the session has fed for the request.
 `step(entries, end)` is the batch form (requests are advanced one after the other, each alone in its program, so a
 request's logits cannot depend on its neighbours); `generate` is greedy / sampled decoding on top of `feed`.
 """
@@ -21,7 +23,8 @@ from typing import Dict, Iterable, List, Optional, Sequence, Tuple
 import numpy as np
 
 from .. import abi
-from ..backend import CudaBackend, DeviceProgram, ProgramIO
+from ..backend import CudaBackend, DeviceOp, DeviceProgram, ProgramIO
+from .batch import LogitRules, rule_table, rule_words
 from .sampling import Sampler
 from .state import SequenceStatePool
 
@@ -33,6 +36,7 @@ class LoweredProgram:
     buf_logits: Optional[int]      # None for head == "none"
     logits_rows: int
     layer_bufs: Optional[List[int]] = None   # residual stream after every layer (debug lowering only)
+    rule_bufs: Optional[Tuple[int, int, int, int]] = None    # table, history, biases and mask of LOGIT_RULES, which made the logits
 
 
 def chunk_menu(max_chunk: int) -> List[int]:
@@ -56,7 +60,11 @@ def cut(n: int, menu: Sequence[int]) -> List[int]:
 
 class SequenceSession:
     def __init__(self, be: CudaBackend, model, n_slots: int = 1, max_chunk: int = 256, keep_layers: bool = False,
-                 max_context: Optional[int] = None):
+                 max_context: Optional[int] = None, max_history: int = 32768, max_bias: int = 1024):
+        """`max_history` tokens of a request, `max_bias` biases: what steps with rules have room for."""
+        self.max_history, self.max_bias = max_history, max_bias
+        self._history: Dict[object, List[int]] = {}
+        self._prompt: Dict[object, int] = {}
         self.be, self.model, self.keep_layers = be, model, keep_layers
         self.menu = chunk_menu(max_chunk)
         self.max_chunk = self.menu[0]
@@ -66,10 +74,22 @@ class SequenceSession:
         self.executions = 0
 
     # ── programs ──
-    def program(self, T: int, head: str):
-        key = (T, head)
+    def _with_rules(self, lp: LoweredProgram) -> LoweredProgram:
+        """The program whose one row of logits passes LOGIT_RULES on its way out."""
+        V, p = self.model.vocab, lp.program
+        n = p.n_buffers
+        table, history, bias, mask, out = range(n, n + 5)
+        sizes = list(p.buffer_sizes) + [rule_words(1), self.max_history, 2 * self.max_bias, (V + 31) // 32, V]
+        op = DeviceOp.logit_rules(out, lp.buf_logits, table, 1, V, history=history, history_rows=self.max_history, bias=bias, masks=mask)
+        return LoweredProgram(DeviceProgram(list(p.ops) + [op], sizes, p.initial_uploads, p.qweights, p.externs), lp.buf_ctl, out, lp.logits_rows, lp.layer_bufs,
+                              (table, history, bias, mask))
+
+    def program(self, T: int, head: str, ruled: bool = False):
+        key = (T, head, True) if ruled else (T, head)
         if key not in self._programs:
             lp = self.model.lower(T, head, self.pool, keep_layers=self.keep_layers)
+            if ruled:
+                lp = self._with_rules(lp)
             handle = self.be.compile_program(lp.program)
             if handle is None:
                 from ..backend import last_error
@@ -79,34 +99,50 @@ class SequenceSession:
             self._programs[key] = (lp, handle, ctl, logits)
         return self._programs[key]
 
-    def _run(self, T, head, slot, pos, prev, tokens):
-        lp, handle, ctl, logits = self.program(T, head)
+    def _run(self, T, head, slot, pos, prev, tokens, request_id=None, rules: Optional[LogitRules] = None):
+        lp, handle, ctl, logits = self.program(T, head, rules is not None)
         ctl[abi.CTL_POS], ctl[abi.CTL_SLOT], ctl[abi.CTL_PREV] = pos, slot, prev
         ctl[abi.CTL_IDS:] = tokens
         outs = [ProgramIO(lp.buf_logits, logits)] if logits is not None else []
-        self.be.execute_program(handle, [ProgramIO(lp.buf_ctl, ctl)], outs)
+        ins = [ProgramIO(lp.buf_ctl, ctl)]
+        if rules is not None:
+            past = np.asarray(self._history[request_id], np.int32)
+            table, bias, masks = rule_table([rules], [0], [past.size], [self._prompt[request_id]], self.model.vocab, 1)
+            ins += [ProgramIO(b, a) for b, a in zip(lp.rule_bufs, (table, past, bias.ravel(), masks.ravel())) if a.size]
+        self.be.execute_program(handle, ins, outs)
         self.executions += 1
         return logits
 
     # ── the step function ──
-    def feed(self, request_id, tokens: Sequence[int], want: Iterable[int] = ()) -> np.ndarray:
-        """Advance `request_id` by `tokens`; returns the logits at the places `want` (indices into `tokens`), in order."""
+    def feed(self, request_id, tokens: Sequence[int], want: Iterable[int] = (), rules: Optional[LogitRules] = None, generated: bool = False) -> np.ndarray:
+        """Advance `request_id` by `tokens`; returns the logits at the places `want` (indices into `tokens`), in order.  With `rules` (the last place alone may be wanted)
+        they are what the rules make of them, over all tokens fed for the request; those fed with `generated` count as generated."""
         tokens = [int(t) for t in tokens]
         if any(t < 0 or t >= self.model.vocab for t in tokens):
             raise ValueError("token id outside the vocabulary")
         want = [int(w) for w in want]
         if any(w < 0 or w >= len(tokens) for w in want):
             raise ValueError("wanted place outside the step's tokens")
+        past = self._history.get(request_id, [])
+        if rules is not None:
+            if any(w != len(tokens) - 1 for w in want):
+                raise ValueError("rules apply to the logits of a step's last place")
+            if len(past) + len(tokens) > self.max_history or len(rules.bias) > self.max_bias:
+                raise ValueError(f"rules over {len(past) + len(tokens)} tokens with {len(rules.bias)} biases: the session has room for {self.max_history} and {self.max_bias}")
+            rule_table([rules], [0], [0], [0], self.model.vocab, 1)      # its tokens are in the vocabulary
         slot = self.pool.acquire(request_id)
         if self.context_limit is not None and self.pool.position(request_id) + len(tokens) > self.context_limit:
             raise ValueError(f"request {request_id!r} would reach position {self.pool.position(request_id) + len(tokens)}: the session's caches hold "
                              f"{self.context_limit} positions per sequence")
+        self._history.setdefault(request_id, []).extend(tokens)
+        if not generated:
+            self._prompt[request_id] = len(self._history[request_id])
         rows: Dict[int, np.ndarray] = {}
         at = 0
         for T in cut(len(tokens), self.menu):
             local = sorted({w - at for w in want if at <= w < at + T})
             head = "none" if not local else ("last" if local == [T - 1] else "all")
-            logits = self._run(T, head, slot, self.pool.position(request_id), self.pool.last_token(request_id), tokens[at:at + T])
+            logits = self._run(T, head, slot, self.pool.position(request_id), self.pool.last_token(request_id), tokens[at:at + T], request_id, rules if local else None)
             for w in local:
                 rows[at + w] = logits[0 if head == "last" else w].copy()
             self.pool.advance(request_id, T, tokens[at + T - 1])
@@ -115,6 +151,8 @@ class SequenceSession:
 
     def release(self, request_id):
         self.pool.release(request_id)
+        self._history.pop(request_id, None)
+        self._prompt.pop(request_id, None)
 
     def step(self, entries: Sequence[dict], end: Iterable = ()) -> List[np.ndarray]:
         """entries: [{"id", "tokens", "want"}]; `end`: requests whose state is given back after the step."""
@@ -134,10 +172,10 @@ class SequenceSession:
         return out
 
     def generate(self, prompt: Sequence[int], max_new_tokens: int, sampler: Optional[Sampler] = None, request_id="generate",
-                 stop: Optional[int] = None) -> List[int]:
-        """Prefill `prompt`, then decode token by token through the same step function."""
+                 stop: Optional[int] = None, rules: Optional[LogitRules] = None) -> List[int]:
+        """Prefill `prompt`, then decode token by token through the same step function; with `rules` the sampler sees logits that have passed them."""
         sampler = sampler or Sampler()
-        logits = self.feed(request_id, prompt, [len(prompt) - 1])[0]
+        logits = self.feed(request_id, prompt, [len(prompt) - 1], rules)[0]
         out: List[int] = []
         try:
             for _ in range(max_new_tokens):
@@ -146,7 +184,7 @@ class SequenceSession:
                 if stop is not None and tok == stop:
                     break
                 if len(out) < max_new_tokens:
-                    logits = self.feed(request_id, [tok], [0])[0]
+                    logits = self.feed(request_id, [tok], [0], rules, generated=True)[0]
         finally:
             self.release(request_id)
         return out

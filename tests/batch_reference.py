@@ -62,7 +62,7 @@ def attend(dst, q, kc, vc, kp, vp, table_rows, live, prefix, prefix_slot, scale,
             z = q[r, h].astype(np.float64)
             s = scale * (k @ z)
             # A product of dk f32 terms, each factor held to 2^-22 of the largest magnitude of its row, is off by at most this; a cap has slope one at most.
-            off = scale * ((np.abs(k) @ np.abs(z)).max() * dk * 2.0 ** -24 + 3 * 2.0 ** -22 * np.abs(k).max() * np.abs(z).sum())
+            off = abs(scale) * ((np.abs(k) @ np.abs(z)).max() * dk * 2.0 ** -24 + 3 * 2.0 ** -22 * np.abs(k).max() * np.abs(z).sum())
             if cap:
                 s = cap * np.tanh(s / cap)
             off += 4 * 2.0 ** -24 * np.abs(s).max()

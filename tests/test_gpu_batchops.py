@@ -115,12 +115,12 @@ def test_batch_append_twice_into_one_row(cuda_backend):
 
 
 # ── SHARED_ATTENTION ─────────────────────────────────────────────────────────────────────────────────────────────────
-def attend_case(be, B, H, G, dk, dv, prefix, R, entries, *, cap=0.0, sink=None, pad=0, latent=False, prefix_slots=2, prefix_slot=1, live=None, seed=0, spare=3, scale=None, loud=1.0, graph=True):
+def attend_case(be, B, H, G, dk, dv, prefix, R, entries, *, cap=0.0, sink=None, pad=0, latent=False, prefix_slots=2, prefix_slot=1, live=None, seed=0, spare=3, scale=None, loud=1.0, graph=True, v_shift=0):
     from zgml_b200 import DeviceOp, abi
     r = np.random.default_rng(seed)
     slots = max([e[0] for e in entries if e[0] < 100] + [0]) + 1
     width = pad + G * dk + (0 if latent else G * dv) + pad
-    v_col = pad if latent else pad + G * dk
+    v_col = pad + v_shift if latent else pad + G * dk
     Rp = prefix + spare
     def cache(n, rows):
         c = r.standard_normal((n, rows, width)).astype(np.float32)
@@ -429,3 +429,81 @@ def test_rule_rows_left_alone_and_out_of_range(cuda_backend):
         got = p.run(["dst"])
         assert np.isfinite(got[0]).all() and np.isnan(got[1]).all() and (got[2] == 7.0).all(), w
         p.close()
+
+
+# ── wide heads with many query rows over a long prefix: tensor cores ─────────────────────────────────────────────────
+def wide_entries(B, R):
+    return [(i, (5 + 7 * i) % (R + 1), 0) for i in range(B)]
+
+
+@pytest.mark.parametrize("B,H,G,dk,dv,prefix,R", [(12, 16, 1, 576, 512, 700, 20), (64, 16, 1, 576, 512, 2500, 5), (40, 8, 2, 192, 136, 1000, 9), (33, 4, 2, 132, 128, 1100, 3), (34, 4, 2, 64, 260, 1000, 3),
+                                                  (40, 6, 1, 1024, 640, 900, 7), (9, 16, 1, 320, 1024, 1025, 4)])
+def test_wide_heads(cuda_backend, B, H, G, dk, dv, prefix, R):
+    attend_case(cuda_backend, B, H, G, dk, dv, prefix, R, wide_entries(B, R), latent=G == 1 and dv <= dk, seed=B)
+
+
+@pytest.mark.parametrize("shift", [0, 8, 64, 4])
+def test_wide_values_inside_keys(cuda_backend, shift):
+    """Values that are columns of the keys' rows, from the first or a later one on (4: no multiple of 16 bytes of half-precision pairs)."""
+    attend_case(cuda_backend, 12, 16, 1, 576, 512, 800, 11, wide_entries(12, 11), latent=True, v_shift=shift, pad=4)
+
+
+@pytest.mark.parametrize("cap,sink,scale", [(0.0, "f32", None), (5.0, None, None), (2.0, "bf16", None), (0.0, None, -0.05), (3.0, None, -0.1)])
+def test_wide_caps_and_sinks(cuda_backend, cap, sink, scale):
+    attend_case(cuda_backend, 40, 8, 2, 160, 160, 500, 33, wide_entries(40, 33), cap=cap, sink=sink, scale=scale)
+
+
+def test_wide_idle_rows(cuda_backend):
+    """Rows without a sequence, bad slots and lengths, rows behind the last, a prefix shorter than its cache, and none."""
+    e = wide_entries(40, 9)
+    e[3], e[7], e[11] = (-1, 0, 0), (200, 1, 0), (2, 10, 0)
+    attend_case(cuda_backend, 40, 8, 2, 160, 160, 500, 9, e, live=37)
+    attend_case(cuda_backend, 40, 8, 2, 160, 160, 100, 9, e, spare=900)
+    attend_case(cuda_backend, 40, 8, 2, 160, 160, 0, 9, wide_entries(40, 9), spare=900)
+    attend_case(cuda_backend, 40, 8, 2, 160, 160, 1, 9, wide_entries(40, 9), spare=900)
+
+
+@pytest.mark.parametrize("loud", [1e-12, 300.0, 3e4])
+def test_wide_magnitudes(cuda_backend, loud):
+    attend_case(cuda_backend, 40, 8, 2, 160, 160, 500, 9, wide_entries(40, 9), loud=loud)
+
+
+@pytest.mark.parametrize("what", ["column", "keys", "query nan", "key inf", "value inf", "value nan"])
+def test_wide_what_pairs_cannot_hold(cuda_backend, what):
+    """Columns of values and values of keys that are small beside the others; what is not finite."""
+    from zgml_b200 import DeviceOp
+    B, H, G, d, P, R = 40, 8, 2, 160, 500, 4
+    r = np.random.default_rng(5)
+    q, own, pre = r.standard_normal((B, H * d)).astype(np.float32), r.standard_normal((B, R, 2 * G * d)).astype(np.float32), r.standard_normal((1, P, 2 * G * d)).astype(np.float32)
+    v = G * d
+    if what == "column":
+        pre[:, :, v + 7] *= 1e-9
+        own[:, :, v + 7] *= 1e-9
+    elif what == "keys":                                # the ones that count have small values, others that do not have large ones
+        pre[:, ::2, v:] *= 1e-8
+        own[:, :, v:] *= 1e-8
+        pre[:, ::2, :v], pre[:, 1::2, :v] = 2 * q[0, :1], -30 * np.sign(q[0, :1])
+        q[:] = q[0, 0]
+    elif what == "query nan":
+        q[17, 5] = NAN
+    elif what == "key inf":
+        pre[0, 333, 11] = np.inf
+    else:
+        pre[0, 333, v + 11] = np.inf if what == "value inf" else NAN
+    entries = wide_entries(B, R)
+    t = table(entries, B, P)
+    op = DeviceOp.shared_attention(0, 1, 2, 2, 3, 3, 4, 0, 0, v, 0, v, B, H, G, d, d, H * d, 2 * v, 2 * v, R, 2 * v, 2 * v, P, 0.05)
+    heads = lambda c, col: c[:, :, col:col + v].reshape(c.shape[0], c.shape[1], G, d)
+    with np.errstate(all="ignore"):
+        want, tol = ref.attend(np.zeros((B, H, d), np.float32), q.reshape(B, H, d), heads(own, 0), heads(own, v), heads(pre, 0), heads(pre, v), entries, B, P, 0, 0.05)
+    p = Prog(cuda_backend, lambda at: [op], dict(dst=np.zeros((B, H * d), np.float32), q=q, own=own, pre=pre, table=t))
+    got = p.run(["dst"]).reshape(B, H, d)
+    p.close()
+    if what in ("column", "keys"):
+        relative = want[:, :, 7] if what == "column" else want      # small beside the rest, and as exact as if it were alone
+        mine = got[:, :, 7] if what == "column" else got
+        assert np.abs(mine - relative).max() <= 1e-4 * np.abs(relative).max()
+        return
+    fine = np.isfinite(want)
+    assert np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(got[~fine & ~np.isnan(want)], want[~fine & ~np.isnan(want)])
+    assert (np.abs(got[fine] - want[fine]) <= np.where(np.isfinite(tol), tol, 1e-4)[fine]).all()

@@ -832,9 +832,379 @@ __global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const __grid_co
     if (warp == 24) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(0u) : "memory");
 }
 
+// ── the prefix on the tensor cores, heads wider than 128 ─────────────────────────────────────────────────────────────
+// A head of 576 dims has no room for 128 queries beside its keys, and 512 columns of outputs none beside the scores.  So everything streams: a first kernel leaves the
+// queries, keys and values as half-precision pairs in the workspace (a scale per row; values inside the key rows of a latent are the same pairs), and CTA (key head, share
+// of the prefix, up to 256 output columns, tile of 128 query rows) multiplies tiles of 128 keys from there, 64 dims at a time, through three stages that TMA fills:
+//   scores[128 rows x 128 keys] += queries[64 dims] keys[64 dims]^T, three MMAs a product;  outputs[128 x 64 columns] += probabilities[128 keys] values[128 keys x 64 columns].
+// Values come as the keys do, by rows, and are read as a transposed operand.  TMEM: scores of two tiles (which become the probabilities in place), outputs.
+// Outputs stay in TMEM from tile to tile; where a row's maximum grows they are scaled there.  Warps 0 - 3 are the softmax (a thread a query row), warp 4 issues, warp 5 copies.
+// What bounds it: 64 KB of operands for every 64 dims of a tile, which an SM takes 1000 clocks to read and 770 to multiply.
+// What pairs cannot hold is known before the first product (the first kernel's scales and flags): the CTA then walks its share in plain f32.
+constexpr uint32_t kSwKeys = 128, kSwCols = 256, kSwStages = 3, kSwPart = 128 * 128, kSwStage = 4 * kSwPart, kSwThreads = 192;
+constexpr uint32_t kSwFactors = kSwStages * kSwStage, kSwRows = kSwFactors + 2 * 128 * 8, kSwRed = kSwRows + 512, kSwBars = kSwRed + 128, kSwSmem = kSwBars + 128 + 1024;
+struct SwArgs {
+    __half* q; __half* k; __half* v;             // pairs: [hi, lo][G][rows][dims, padded to 64]
+    float* qf; float* kf; float* vf;             // what a row's pairs were divided by: [G][rows]; of a row of zeros 0, of a query that is not finite NaN
+    uint32_t* flags;                             // [keys, values][G][blocks of eight rows]: something that pairs cannot hold
+    uint32_t KR, QR, dkp, dvp, v0, latent, halves, row_tiles;      // rows of keys and queries; first column of the values in their plane; values are the keys' pairs
+};
+// Block of eight rows -> pairs.  Blocks: keys, values (unless they are the keys'), queries.  A thread holds four dims of the eight rows.
+__global__ void __launch_bounds__(256) k_shared_pairs(const SaArgs a, const SwArgs w) {
+    pdl_enter();
+    __shared__ uint32_t red[8][8], bad_rows;
+    const uint32_t kb = w.KR / 8, kinds = w.latent ? 1 : 2, keys = kinds * kb * a.G;
+    const uint32_t kind = blockIdx.x >= keys ? 2 : blockIdx.x / (kb * a.G), in = kind == 2 ? blockIdx.x - keys : blockIdx.x % (kb * a.G), per = kind == 2 ? w.QR / 8 : kb, g = in / per, b = in % per;
+    const BatchHead head = batch_head(a.table, a.B);
+    const bool sound = head.prefix > 0 && (uint32_t)head.prefix <= a.Rp && (uint32_t)head.prefix_slot < a.pslots;
+    const uint32_t P = sound ? (uint32_t)head.prefix : 0u, r0 = 8 * b, dim = kind == 1 ? a.dv : a.dk, dimp = kind == 1 ? w.dvp : w.dkp, t4 = 4 * threadIdx.x;
+    if (!sound || (kind == 2 ? r0 >= head.rows * a.rep : r0 >= P + kSwKeys)) return;      // (a tile may reach so far behind the prefix: zeros there)
+    float4 x[8];
+    float mx[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const float* from = nullptr;
+        if (kind == 2) {
+            SpCta c; c.g = g; c.tile = 0;
+            const SpRow q = sp_row(a, c, head, r0 + i);
+            if (q.on) from = a.q + (size_t)q.r * a.q_rs + (size_t)q.h * a.dk;
+        } else if (r0 + i < P) {
+            const size_t row = (size_t)head.prefix_slot * a.Rp + r0 + i;
+            from = kind ? a.vp + row * a.pvw + g * a.dv : a.kp + row * a.pkw + g * a.dk;
+        }
+        x[i] = sa_load<true>(from, t4, dim, from != nullptr);
+        mx[i] = abs_or_inf(abs_or_inf(abs_or_inf(abs_or_inf(0.0f, x[i].x), x[i].y), x[i].z), x[i].w);
+    }
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) bad_rows = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(mx[i]));
+        if (lane == 0) red[i][warp] = top;
+    }
+    __syncthreads();
+    bool bad = false;
+    float4 cm = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const uint32_t rows = kind == 2 ? w.QR : w.KR;
+    __half* const plane = kind == 2 ? w.q : kind ? w.v : w.k;
+    float* const factor = kind == 2 ? w.qf : kind ? w.vf : w.kf;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, red[i][lane & 7]));
+        float s, inv;
+        split_scale(top, s, inv);
+        const bool wrong = !(inv == inv);
+        if (wrong) { x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f); bad = true; }
+        if (threadIdx.x == 0) factor[(size_t)g * rows + r0 + i] = wrong && kind == 2 ? kBatchNaN : wrong || top == 0.0f ? 0.0f : kind == 2 ? inv * fabsf(a.scale) * kLog2e : inv;
+        if (kind == 2 && a.scale < 0.0f) s = -s;
+        x[i] = make_float4(x[i].x * s, x[i].y * s, x[i].z * s, x[i].w * s);
+        cm = make_float4(fmaxf(cm.x, fabsf(x[i].x)), fmaxf(cm.y, fabsf(x[i].y)), fmaxf(cm.z, fabsf(x[i].z)), fmaxf(cm.w, fabsf(x[i].w)));
+        if (t4 < dimp) {
+            uint2 hi, lo;
+            split2(x[i].x, x[i].y, hi.x, lo.x); split2(x[i].z, x[i].w, hi.y, lo.y);
+            *reinterpret_cast<uint2*>(plane + ((size_t)g * rows + r0 + i) * dimp + t4) = hi;
+            *reinterpret_cast<uint2*>(plane + ((size_t)(a.G + g) * rows + r0 + i) * dimp + t4) = lo;
+        }
+    }
+    if (kind == 2) return;
+    // a column of values that is small as a whole beside its rows: pairs keep 22 bits above 2^-18 of a row's largest, which is scaled to 2^14 at least
+    if (kind == 1 || (w.latent && t4 >= w.v0 && t4 < w.v0 + a.dv)) {
+        constexpr float least = 32768.0f * kSpColumn;
+        bad = bad || (cm.x > 0.0f && cm.x < least) || (cm.y > 0.0f && cm.y < least) || (cm.z > 0.0f && cm.z < least) || (cm.w > 0.0f && cm.w < least);
+    }
+    if (__syncthreads_or(bad) && threadIdx.x == 0) bad_rows = 1;
+    if (threadIdx.x == 0) w.flags[((size_t)kind * a.G + g) * kb + b] = bad_rows;
+}
+// The CTA's share in plain f32, a warp a row at a time
+__device__ __noinline__ void sw_plain(const SaArgs& a, const float* kp, const float* vp, uint32_t k0, uint32_t k1, uint32_t split, uint32_t c0, const uint32_t* rows) {
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (uint32_t i = warp; i < 128; i += kSwThreads / 32) {
+        const uint32_t w = rows[i];
+        if (w == 0xffffffffu) continue;
+        float4 q[8], o[2] = {};
+        float m = -INFINITY, l = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) q[j] = sa_load<true>(a.q + (size_t)(w >> 10) * a.q_rs + (size_t)(w & 1023) * a.dk, 4 * lane + 128 * j, a.dk, true);
+        for (uint32_t u = k0; u < k1; u++) {
+            float s = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float4 x = sa_load<true>(kp + (size_t)u * a.pkw, 4 * lane + 128 * j, a.dk, true);
+                s = fmaf(q[j].x, x.x, fmaf(q[j].y, x.y, fmaf(q[j].z, x.z, fmaf(q[j].w, x.w, s))));
+            }
+            s = warp_sum(s) * a.scale;
+            if (a.cap > 0.0f) s = a.cap * tanhf(s / a.cap);
+            const float top = fmaxf(m, s), f = sa_weight(m, top), p = s == -INFINITY ? 0.0f : expf(s - top);
+            m = top; l = fmaf(l, f, p);
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const float4 v = sa_load<true>(vp + (size_t)u * a.pvw, c0 + 4 * lane + 128 * j, a.dv, true);
+                o[j].x = fmaf(o[j].x, f, p * v.x); o[j].y = fmaf(o[j].y, f, p * v.y); o[j].z = fmaf(o[j].z, f, p * v.z); o[j].w = fmaf(o[j].w, f, p * v.w);
+            }
+        }
+        float* rec = sa_record(a, w >> 10, w & 1023, split);
+        if (lane == 0 && c0 == 0) { rec[0] = m; rec[1] = l; }
+#pragma unroll
+        for (int j = 0; j < 2; j++) if (c0 + 4 * lane + 128 * j < a.dv) *reinterpret_cast<float4*>(rec + 4 + c0 + 4 * lane + 128 * j) = o[j];
+    }
+}
+__global__ void __launch_bounds__(kSwThreads, 1) k_shared_wide(const __grid_constant__ SaArgs a, const __grid_constant__ SwArgs w, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                                                              const __grid_constant__ CUtensorMap map_v) {
+    constexpr uint32_t kS = 0, kO = 2 * kSwKeys;                            // TMEM columns
+    extern __shared__ uint8_t dsm_raw[];
+    const uint32_t base = (smem_u32(dsm_raw) + 1023u) & ~1023u;
+    uint8_t* const mem = dsm_raw + (base - smem_u32(dsm_raw));
+    const uint32_t full = base + kSwBars, empty = full + 8 * kSwStages, s_full = empty + 8 * kSwStages, p_full = s_full + 16, o_full = p_full + 16, tmem_slot = o_full + 8;
+    uint32_t* const lost = reinterpret_cast<uint32_t*>(mem + (tmem_slot + 4 - base));      // a wait ran out
+    uint32_t* const red = reinterpret_cast<uint32_t*>(mem + kSwRed);        // largest and smallest factor of the values, largest of the keys
+    uint32_t* const rows = reinterpret_cast<uint32_t*>(mem + kSwRows);
+    const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (uint32_t i = 0; i < kSwStages; i++) { mbar_init(full + 8 * i, 1); mbar_init(empty + 8 * i, 1); }
+        for (uint32_t i = 0; i < 2; i++) { mbar_init(s_full + 8 * i, 1); mbar_init(p_full + 8 * i, 4); }
+        mbar_init(o_full, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        *lost = 0;
+        red[0] = 0; red[1] = 0x7f800000u; red[2] = 0;
+    }
+    if (warp == 4) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(tmem_slot) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const BatchHead head = batch_head(a.table, a.B);
+    SpCta c;
+    const uint32_t half = blockIdx.x / w.row_tiles % w.halves, c0 = half * kSwCols, cols = min(kSwCols, a.dv - c0);
+    c.tile = blockIdx.x % w.row_tiles; c.split = blockIdx.x / w.row_tiles / w.halves % a.shares; c.g = blockIdx.x / w.row_tiles / w.halves / a.shares;      // CTAs of the same keys are neighbours
+    const bool sound = head.prefix > 0 && (uint32_t)head.prefix <= a.Rp && (uint32_t)head.prefix_slot < a.pslots && c.tile * 128 < head.rows * a.rep;
+    const uint32_t P = sound ? (uint32_t)head.prefix : 0u, per = sa_share(P, a.shares, kSaShare);
+    c.k0 = min(P, c.split * per); c.k1 = min(P, c.k0 + per);
+    const size_t p0 = sound ? (size_t)head.prefix_slot * a.Rp : 0;
+    c.kp = a.kp + p0 * a.pkw + c.g * a.dk; c.vp = a.vp + p0 * a.pvw + c.g * a.dv;
+    const uint32_t n_tiles = __shfl_sync(0xffffffffu, (c.k1 - c.k0 + kSwKeys - 1) / kSwKeys, 0), nc = w.dkp / 64, nv = (cols + 63) / 64;
+    const float* const kf = w.kf + (size_t)c.g * w.KR;
+    const float* const vf = (w.latent ? w.kf : w.vf) + (size_t)c.g * w.KR;
+    __syncthreads();
+    // The largest and smallest factors of the share, and flags of all rows that its tiles touch
+    bool slow = false;
+    float f = 0.0f;                                                         // of the thread's query row
+    if (n_tiles) {
+        uint32_t v_top = 0, v_low = 0x7f800000u, k_top = 0;                 // (factors order as their bits do)
+        for (uint32_t u = c.k0 + threadIdx.x; u < c.k1; u += kSwThreads) {
+            const uint32_t y = __float_as_uint(vf[u]);
+            v_top = max(v_top, y);
+            if (y) v_low = min(v_low, y);
+            k_top = max(k_top, __float_as_uint(kf[u]));
+        }
+        const uint32_t kb = w.KR / 8, b1 = (c.k0 + n_tiles * kSwKeys) / 8;
+        for (uint32_t b = c.k0 / 8 + threadIdx.x; b < b1; b += kSwThreads) {
+            slow = slow || w.flags[(size_t)c.g * kb + b] != 0;
+            if (!w.latent) slow = slow || w.flags[(size_t)(a.G + c.g) * kb + b] != 0;
+        }
+        v_top = __reduce_max_sync(0xffffffffu, v_top); v_low = __reduce_min_sync(0xffffffffu, v_low); k_top = __reduce_max_sync(0xffffffffu, k_top);
+        if (lane == 0) { atomicMax(red, v_top); atomicMin(red + 1, v_low); atomicMax(red + 2, k_top); }
+        if (threadIdx.x < 128) {
+            const SpRow q = sp_row(a, c, head, threadIdx.x);
+            rows[threadIdx.x] = q.on ? q.r << 10 | q.h : 0xffffffffu;
+            const uint32_t at = c.tile * 128 + threadIdx.x;
+            if (at < head.rows * a.rep) f = w.qf[(size_t)c.g * w.QR + at];
+        }
+    }
+    __syncthreads();
+    const float v_ref = __uint_as_float(red[0]), k_ref = __uint_as_float(red[2]);
+    slow = slow || !(f * k_ref <= kSpLoud * 128.0f / (float)max(128u, a.dk)) || (red[0] && __uint_as_float(red[1]) < v_ref * (1.0f / 32768.0f));
+    fence_before();
+    const bool plain = __syncthreads_or(slow);
+    fence_after();
+    if (plain) {
+        sw_plain(a, c.kp, c.vp, c.k0, c.k1, c.split, c0, rows);
+    } else if (!n_tiles) {
+    } else if (warp == 5) {
+        if (elect_one()) {
+            const uint32_t yq = c.g * w.QR + c.tile * 128, yk = c.g * w.KR + c.k0, q_lo = a.G * w.QR, k_lo = a.G * w.KR;
+            uint32_t s = 0, phase = 1;
+            bool ok = true;
+            auto place = [&](uint32_t bytes) {
+                ok = ok && mbar_wait(empty + 8 * s, phase);
+                if (ok) mbar_expect_tx(full + 8 * s, bytes);
+                return ok;
+            };
+            auto next = [&] { if (++s == kSwStages) { s = 0; phase ^= 1; } };
+            for (uint32_t t = 0; t <= n_tiles && ok; t++) {
+                if (t < n_tiles)
+                    for (uint32_t i = 0; i < nc && place(kSwStage); i++) {
+                        const uint32_t to = base + s * kSwStage, bar = full + 8 * s;
+                        tma_2d(to, &map_q, 64 * i, yq, bar); tma_2d(to + kSwPart, &map_q, 64 * i, yq + q_lo, bar);
+                        tma_2d(to + 2 * kSwPart, &map_k, 64 * i, yk + t * kSwKeys, bar); tma_2d(to + 3 * kSwPart, &map_k, 64 * i, yk + t * kSwKeys + k_lo, bar);
+                        next();
+                    }
+                if (t)
+                    for (uint32_t i = 0; i < nv && place(min(2u, nv - i) * 2 * kSwPart); i += 2) {
+                        for (uint32_t e = 0; e < min(2u, nv - i); e++) {
+                            const uint32_t to = base + s * kSwStage + 2 * e * kSwPart, bar = full + 8 * s, x = w.v0 + c0 + 64 * (i + e);
+                            tma_2d(to, &map_v, x, yk + (t - 1) * kSwKeys, bar); tma_2d(to + kSwPart, &map_v, x, yk + (t - 1) * kSwKeys + k_lo, bar);
+                        }
+                        next();
+                    }
+            }
+            if (!ok) { count_timeout(); atomicOr(lost, 1u); }
+        }
+        __syncwarp();
+    } else if (warp == 4) {
+        // Issue.  Three products, the small ones first: hi lo, lo hi, hi hi.
+        constexpr uint32_t idesc_s = (1u << 4) | ((kSwKeys >> 3) << 17) | ((128u >> 4) << 24), idesc_o = (1u << 4) | (1u << 16) | ((64u >> 3) << 17) | ((128u >> 4) << 24);      // f16 x f16 -> f32; B transposed
+        uint32_t s = 0, phase = 0;
+        bool ok = true;
+        auto take = [&] { ok = ok && __all_sync(0xffffffffu, mbar_wait(full + 8 * s, phase)); fence_after(); return ok; };
+        auto next = [&] { if (++s == kSwStages) { s = 0; phase ^= 1; } };
+        for (uint32_t t = 0; t <= n_tiles && ok; t++) {
+            if (t < n_tiles) {
+                const uint32_t d = kS + (t & 1) * kSwKeys;
+                for (uint32_t i = 0; i < nc && take(); i++) {
+                    const uint32_t q = desc_low(base + s * kSwStage), k = q + (2 * kSwPart >> 4);
+                    if (elect_one()) {
+#pragma unroll
+                        for (uint32_t x = 0; x < 3; x++)
+#pragma unroll
+                            for (uint32_t j = 0; j < 4; j++) {
+                                const uint32_t qa = q + (x == 1 ? kSwPart >> 4 : 0) + 2 * j, ka = k + (x == 0 ? kSwPart >> 4 : 0) + 2 * j;
+                                if (x == 0 && j == 0 && i == 0) mma_ss<false>(d, qa, ka, idesc_s); else mma_ss<true>(d, qa, ka, idesc_s);
+                            }
+                        mma_commit(empty + 8 * s);
+                        if (i + 1 == nc) mma_commit(s_full + 8 * (t & 1));
+                    }
+                    __syncwarp();
+                    next();
+                }
+            }
+            if (t && ok) {
+                const uint32_t u = t - 1, p = kS + (u & 1) * kSwKeys;
+                ok = __all_sync(0xffffffffu, mbar_wait(p_full + 8 * (u & 1), (u >> 1) & 1));
+                fence_after();
+                for (uint32_t i = 0; i < nv && take(); i += 2) {
+                    if (elect_one()) {
+                        for (uint32_t e = 0; e < min(2u, nv - i); e++) {
+                            const uint32_t d = kO + 64 * (i + e), v = (((base + s * kSwStage + 2 * e * kSwPart) & 0x3FFFF) >> 4) | (64u << 16);      // groups of eight keys are 1024 B apart
+#pragma unroll
+                            for (uint32_t x = 0; x < 3; x++)
+#pragma unroll
+                                for (uint32_t j = 0; j < kSwKeys / 16; j++) {
+                                    const uint32_t pa = p + 16 * j + (x == 1 ? 8 : 0), va = v + (x == 0 ? kSwPart >> 4 : 0) + 128 * j;
+                                    if (x == 0 && j == 0 && u == 0) mma_ts<false>(d, pa, va, idesc_o); else mma_ts<true>(d, pa, va, idesc_o);
+                                }
+                        }
+                        mma_commit(empty + 8 * s);
+                        if (i + 2 >= nv) mma_commit(o_full);
+                    }
+                    __syncwarp();
+                    next();
+                }
+            }
+        }
+        if (!ok && lane == 0) { count_timeout(); atomicOr(lost, 1u); }
+        __syncwarp();
+    } else {
+        const uint32_t row = threadIdx.x, lanes = (warp * 32) << 16;
+        float2* const factors = reinterpret_cast<float2*>(mem + kSwFactors);
+        const float v_inv = v_ref > 0.0f ? 1.0f / v_ref : 0.0f, inv_cap = a.cap > 0.0f ? 1.0f / a.cap : 0.0f;      // (a power of two)
+        float m = -INFINITY, l = 0.0f;
+        bool ok = true;
+#pragma unroll 1
+        for (uint32_t t = 0; t < n_tiles; t++) {
+            float2* const fs = factors + (t & 1) * 128;
+            {
+                const uint32_t u = c.k0 + t * kSwKeys + row;
+                fs[row] = u < c.k1 ? make_float2(kf[u], vf[u] * v_inv * 16384.0f) : make_float2(0.0f, 0.0f);      // probabilities times 2^14, in the frame of the share's largest values
+            }
+            bar_sync(1, 128);
+            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(s_full + 8 * (t & 1), (t >> 1) & 1));
+            fence_after();
+            const uint32_t s = lanes + kS + (t & 1) * kSwKeys, left = c.k1 - c.k0 - t * kSwKeys;
+            float x[128], top = -INFINITY;
+#pragma unroll
+            for (int h = 0; h < 4; h++) {
+                uint32_t v[32];
+                tmem_ld(s + 32 * h, v);
+                tmem_wait_ld(v);
+#pragma unroll
+                for (int j = 0; j < 32; j++) {
+                    float y = __uint_as_float(v[j]) * (f * fs[32 * h + j].x);
+                    if (a.cap > 0.0f) y = sa_capped(y * kLn2, a.cap, inv_cap) * kLog2e;
+                    x[32 * h + j] = 32 * h + j < left ? y : -INFINITY;
+                }
+#pragma unroll
+                for (int j = 0; j < 32; j++) top = fmaxf(top, x[32 * h + j]);
+            }
+            const float m_new = fmaxf(m, top), alpha = m == -INFINITY ? 0.0f : sa_ex2(m - m_new);
+            if (t) {
+                if (ok) ok = __all_sync(0xffffffffu, mbar_wait(o_full, (t - 1) & 1));
+                fence_after();
+                if (__any_sync(0xffffffffu, m_new > m)) {
+#pragma unroll 1
+                    for (uint32_t h = 0; h < 2 * nv; h++) {
+                        uint32_t v[32];
+                        tmem_ld(lanes + kO + 32 * h, v);
+                        tmem_wait_ld(v);
+#pragma unroll
+                        for (int j = 0; j < 32; j++) v[j] = __float_as_uint(__uint_as_float(v[j]) * alpha);
+                        tmem_st(lanes + kO + 32 * h, v);
+                    }
+                }
+            }
+            m = m_new;
+            float l0 = 0.0f, l1 = 0.0f;
+#pragma unroll
+            for (int h = 0; h < 8; h++) {
+                uint32_t v[16];
+#pragma unroll
+                for (int j = 0; j < 16; j += 2) {
+                    const float p0 = sa_ex2(x[16 * h + j] - m), p1 = sa_ex2(x[16 * h + j + 1] - m);
+                    l0 += p0; l1 += p1;
+                    split2(p0 * fs[16 * h + j].y, p1 * fs[16 * h + j + 1].y, v[j / 2], v[8 + j / 2]);
+                }
+                tmem_st(s + 16 * h, v);
+            }
+            l = fmaf(l, alpha, l0 + l1);
+            tmem_wait_st();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_full + 8 * (t & 1));
+        }
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(o_full, (n_tiles - 1) & 1));
+        fence_after();
+        if (!ok && lane == 0) { count_timeout(); atomicOr(lost, 1u); }
+        // Outputs leave by whole rows, through the idle stages.
+        const float unit = v_ref * (1.0f / 16384.0f);
+        float4* const out = reinterpret_cast<float4*>(mem);
+        for (uint32_t h = 0; h < 2 * nv; h++) {
+            uint32_t v[32];
+            tmem_ld(lanes + kO + 32 * h, v);
+            tmem_wait_ld(v);
+#pragma unroll
+            for (int j = 0; j < 32; j += 4)
+                out[row * (kSwCols / 4) + ((8 * h + j / 4) ^ (row & 7))] = make_float4(__uint_as_float(v[j]) * unit, __uint_as_float(v[j + 1]) * unit, __uint_as_float(v[j + 2]) * unit, __uint_as_float(v[j + 3]) * unit);
+        }
+        bar_sync(1, 128);
+        const bool gone = *reinterpret_cast<volatile uint32_t*>(lost);
+        const uint32_t mine = rows[row];
+        if (mine != 0xffffffffu && half == 0) { float* rec = sa_record(a, mine >> 10, mine & 1023, c.split); rec[0] = gone ? kBatchNaN : m * kLn2; rec[1] = gone ? kBatchNaN : l; }
+        for (uint32_t i = threadIdx.x; i < 128 * (cols / 4); i += 128) {
+            const uint32_t r = i / (cols / 4), j = i % (cols / 4), to = rows[r];
+            if (to == 0xffffffffu) continue;
+            *reinterpret_cast<float4*>(sa_record(a, to >> 10, to & 1023, c.split) + 4 + c0 + 4 * j) = gone ? make_float4(kBatchNaN, kBatchNaN, kBatchNaN, kBatchNaN) : out[r * (kSwCols / 4) + (j ^ (r & 7))];
+        }
+    }
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    __syncwarp();
+    fence_before();
+    __syncthreads();
+    if (warp == 4) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(0u) : "memory");
+}
+
 // What decides a launch: queries a CTA of k_shared_rows holds (RQ), float4 a lane holds (NV), lanes that share a key (LK), shares of its keys; shares of the prefix
 // on the tensor cores (0: k_shared_rows walks the prefix too).
-struct SaShape { uint32_t RQ, NV, LK, chunks, splits, warps, shares, row_tiles; bool records; };
+constexpr uint64_t kSwLeast = 1u << 17;
+struct SaShape { uint32_t RQ, NV, LK, chunks, splits, warps, shares, row_tiles, halves; bool records; };      // halves: of the output columns, of a head wider than 128 (0: k_shared_prefix)
 SaShape sa_shape(const ZgSeqOp& s, bool wide) {
     const uint32_t B = s.n[0], G = s.n[2], rep = s.n[1] / G, dk = s.n[3], dv = s.n[4], dim = std::max(dk, dv), R = s.n[8], Rp = s.n[11], sms = zg_sm_count();
     SaShape p = {};
@@ -843,13 +1213,16 @@ SaShape sa_shape(const ZgSeqOp& s, bool wide) {
     while (p.LK * 4 * p.NV < dim) p.LK <<= 1;
     p.RQ = std::min(rep, p.NV == 8 ? 2u : 4u);
     p.chunks = (rep + p.RQ - 1) / p.RQ;
-    if (wide && Rp && dk <= 128 && dv <= 128 && B * rep >= 32) {
-        // The number of shares that keeps the GPU busy with the fewest tiles of 64 keys one after the other, and six tiles' time for each start and end.
+    const bool narrow = dim <= 128;
+    if (wide && Rp && B * rep >= 32 && (narrow || (uint64_t)B * s.n[1] * Rp >= kSwLeast)) {
+        // The number of shares that keeps the GPU busy with the fewest tiles of 64 (128) keys one after the other, and six tiles' (one tile's) time for each start and end.
         p.row_tiles = (B * rep + 127) / 128;
-        const uint32_t items = p.row_tiles * G, tiles = (Rp + 63) / 64;
+        p.halves = narrow ? 0 : (dv + kSwCols - 1) / kSwCols;
+        const uint32_t items = p.row_tiles * G * std::max(1u, p.halves), tile = narrow ? 64 : kSwKeys, tiles = (Rp + tile - 1) / tile;
         uint64_t best = ~0ull;
         for (uint32_t n = 1; n <= std::min(tiles, 64u); n++) {
-            const uint64_t cost = (uint64_t)((items * n + sms - 1) / sms) * (((Rp + n - 1) / n + 15) / 16 + 24);
+            const uint32_t keys = ((Rp + n - 1) / n + 15) / 16;
+            const uint64_t cost = (uint64_t)((items * n + sms - 1) / sms) * (narrow ? keys + 24 : (keys + 7) / 8 + 1);
             if (cost < best) { best = cost; p.shares = n; }
         }
     }
@@ -885,6 +1258,44 @@ bool sa_launch_prefix(const SaArgs& a, const SaShape& p, cudaStream_t st) {
     if (!sa_encode(&mk, a.kp - a.k_x, a.pkw, rows, a.dk) || !sa_encode(&mv, a.vp - a.v_x, a.pvw, rows, a.dv)) return false;
     if (!zg_smem_limit<k_shared_prefix<NC, DV>>(L::size)) return false;
     launch_pdl(k_shared_prefix<NC, DV>, dim3(p.row_tiles * a.shares * a.G), dim3(kSpThreads), L::size, st, a, mk, mv, p.row_tiles);
+    return true;
+}
+// Where the pairs of k_shared_wide lie in the workspace, behind the records; `base` null: how many floats all of it takes
+size_t sw_layout(const ZgSeqOp& s, const SaShape& p, float* base, uint32_t k_x, uint32_t v_x, SwArgs* w) {
+    const uint32_t G = s.n[2], dk = s.n[3], dv = s.n[4];
+    w->KR = (s.n[11] + 7) / 8 * 8 + kSwKeys; w->QR = p.row_tiles * 128;
+    w->dkp = (dk + 63) / 64 * 64; w->dvp = (dv + 63) / 64 * 64;
+    // the values of a latent: columns of the same rows, from a multiple of 16 bytes of pairs on
+    w->latent = s.buf[4] == s.buf[5] && s.n[9] == s.n[10] && G == 1 && v_x >= k_x && v_x - k_x + dv <= dk && (v_x - k_x) % 8 == 0;
+    w->v0 = w->latent ? v_x - k_x : 0;
+    w->halves = p.halves; w->row_tiles = p.row_tiles;
+    size_t at = ((size_t)s.n[0] * s.n[1] * p.shares * (4 + dv) + 255) & ~(size_t)255;
+    auto place = [&](auto*& ptr, size_t floats) { ptr = base ? reinterpret_cast<std::remove_reference_t<decltype(ptr)>>(base + at) : nullptr; at = (at + floats + 255) & ~(size_t)255; };
+    place(w->q, (size_t)G * w->QR * w->dkp);                        // (two halves of 16 bits a value)
+    place(w->k, (size_t)G * w->KR * w->dkp);
+    place(w->v, w->latent ? 0 : (size_t)G * w->KR * w->dvp);
+    place(w->qf, (size_t)G * w->QR); place(w->kf, (size_t)G * w->KR); place(w->vf, w->latent ? 0 : (size_t)G * w->KR);
+    place(w->flags, (size_t)2 * G * w->KR / 8);
+    return at;
+}
+bool sw_encode(CUtensorMap* map, const __half* base, uint64_t dims_, uint64_t rows) {
+    const cuuint64_t dims[2] = {dims_, rows}, stride[1] = {dims_ * 2};
+    const cuuint32_t box[2] = {64, 128}, one[2] = {1, 1};
+    EncodeTiledFn fn = encode_tiled();
+    if (!fn) { zg_set_error("cuTensorMapEncodeTiled entry point not available"); return false; }
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<__half*>(base), dims, stride, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) { zg_set_error("cuTensorMapEncodeTiled(pairs) failed (%d)", (int)r); return false; }
+    return true;
+}
+bool sa_launch_wide(const ZgOp& op, const SaArgs& a, const SwArgs& w, cudaStream_t st) {
+    CUtensorMap mq, mk, mv;
+    if (!sw_encode(&mq, w.q, w.dkp, 2ull * a.G * w.QR) || !sw_encode(&mk, w.k, w.dkp, 2ull * a.G * w.KR)) return false;
+    if (!sw_encode(&mv, w.latent ? w.k : w.v, w.latent ? w.dkp : w.dvp, 2ull * a.G * w.KR)) return false;
+    if (!zg_smem_limit<k_shared_wide>(kSwSmem)) return false;
+    launch_pdl(k_shared_pairs, dim3(a.G * ((w.latent ? 1 : 2) * (w.KR / 8) + w.QR / 8)), dim3(256), 0, st, a, w);
+    ZG_SEQ_CHECK();
+    launch_pdl(k_shared_wide, dim3(w.row_tiles * w.halves * a.shares * a.G), dim3(kSwThreads), kSwSmem, st, a, w, mq, mk, mv);
     return true;
 }
 template <int RQ, int NV, bool VEC>
@@ -926,6 +1337,8 @@ bool zg_shared_attention_valid(const ZgSeqOp& s, const size_t* elems, size_t n_b
 }
 size_t zg_shared_attention_scratch_elems(const ZgSeqOp& s) {
     const SaShape p = sa_shape(s, sa_vec(s));
+    SwArgs w;
+    if (p.halves) return sw_layout(s, p, nullptr, s.off[3], s.off[4], &w);
     return (size_t)s.n[0] * s.n[1] * (p.shares + (p.records ? p.splits : 0)) * (4 + s.n[4]);
 }
 bool zg_launch_shared_attention(const ZgOp& op, float* const* bufs, const size_t* elems, float* scratch, cudaStream_t st) {
@@ -949,7 +1362,12 @@ bool zg_launch_shared_attention(const ZgOp& op, float* const* bufs, const size_t
     if (p.records && !scratch) { p.records = false; p.splits = kSaCluster; }      // no room for records
     a.shares = p.shares; a.splits = p.splits;
     a.part = p.shares || p.records ? scratch : nullptr;
-    if (a.shares) {
+    if (a.shares && p.halves) {
+        SwArgs w;
+        sw_layout(s, p, scratch, a.k_x, a.v_x, &w);
+        if (!sa_launch_wide(op, a, w, st)) return false;
+        ZG_SEQ_CHECK();
+    } else if (a.shares) {
         const bool k1 = a.dk <= 64, v1 = a.dv <= 64;
         if (!(k1 ? v1 ? sa_launch_prefix<1, 64>(a, p, st) : sa_launch_prefix<1, 128>(a, p, st) : v1 ? sa_launch_prefix<2, 64>(a, p, st) : sa_launch_prefix<2, 128>(a, p, st))) return false;
         ZG_SEQ_CHECK();

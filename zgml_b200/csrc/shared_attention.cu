@@ -1120,21 +1120,29 @@ __global__ void __launch_bounds__(kSwThreads, 1) k_shared_wide(const __grid_cons
             if (ok) ok = __all_sync(0xffffffffu, mbar_wait(s_full + 8 * (t & 1), (t >> 1) & 1));
             fence_after();
             const uint32_t s = lanes + kS + (t & 1) * kSwKeys, left = c.k1 - c.k0 - t * kSwKeys;
-            float x[128], top = -INFINITY;
-#pragma unroll
-            for (int h = 0; h < 4; h++) {
-                uint32_t v[32];
-                tmem_ld(s + 32 * h, v);
+            // Loops of 16 keys, whose scores go back to TMEM in between: a tile is often the only one, and code that runs once costs its fetching (all 128 unrolled took
+            // 18000 clocks).
+            float top = -INFINITY;
+#pragma unroll 1
+            for (uint32_t h = 0; h < 128; h += 16) {
+                uint32_t v[16];
+                tmem_ld(s + h, v);
                 tmem_wait_ld(v);
 #pragma unroll
-                for (int j = 0; j < 32; j++) {
-                    float y = __uint_as_float(v[j]) * (f * fs[32 * h + j].x);
-                    if (a.cap > 0.0f) y = sa_capped(y * kLn2, a.cap, inv_cap) * kLog2e;
-                    x[32 * h + j] = 32 * h + j < left ? y : -INFINITY;
+                for (int j = 0; j < 16; j++) v[j] = __float_as_uint(__uint_as_float(v[j]) * (f * fs[h + j].x));
+                if (a.cap > 0.0f) {
+#pragma unroll
+                    for (int j = 0; j < 16; j++) v[j] = __float_as_uint(sa_capped(__uint_as_float(v[j]) * kLn2, a.cap, inv_cap) * kLog2e);
+                }
+                if (h + 16 > left) {
+#pragma unroll
+                    for (int j = 0; j < 16; j++) if (h + j >= left) v[j] = 0xff800000u;
                 }
 #pragma unroll
-                for (int j = 0; j < 32; j++) top = fmaxf(top, x[32 * h + j]);
+                for (int j = 0; j < 16; j++) top = fmaxf(top, __uint_as_float(v[j]));
+                tmem_st(s + h, v);
             }
+            tmem_wait_st();
             const float m_new = fmaxf(m, top), alpha = m == -INFINITY ? 0.0f : sa_ex2(m - m_new);
             if (t) {
                 if (ok) ok = __all_sync(0xffffffffu, mbar_wait(o_full, (t - 1) & 1));
@@ -1153,16 +1161,18 @@ __global__ void __launch_bounds__(kSwThreads, 1) k_shared_wide(const __grid_cons
             }
             m = m_new;
             float l0 = 0.0f, l1 = 0.0f;
-#pragma unroll
-            for (int h = 0; h < 8; h++) {
-                uint32_t v[16];
+#pragma unroll 1
+            for (uint32_t h = 0; h < 128; h += 16) {
+                uint32_t x[16], v[16];
+                tmem_ld(s + h, x);
+                tmem_wait_ld(x);
 #pragma unroll
                 for (int j = 0; j < 16; j += 2) {
-                    const float p0 = sa_ex2(x[16 * h + j] - m), p1 = sa_ex2(x[16 * h + j + 1] - m);
+                    const float p0 = sa_ex2(__uint_as_float(x[j]) - m), p1 = sa_ex2(__uint_as_float(x[j + 1]) - m);
                     l0 += p0; l1 += p1;
-                    split2(p0 * fs[16 * h + j].y, p1 * fs[16 * h + j + 1].y, v[j / 2], v[8 + j / 2]);
+                    split2(p0 * fs[h + j].y, p1 * fs[h + j + 1].y, v[j / 2], v[8 + j / 2]);
                 }
-                tmem_st(s + 16 * h, v);
+                tmem_st(s + h, v);
             }
             l = fmaf(l, alpha, l0 + l1);
             tmem_wait_st();
@@ -1176,6 +1186,7 @@ __global__ void __launch_bounds__(kSwThreads, 1) k_shared_wide(const __grid_cons
         // Outputs leave by whole rows, through the idle stages.
         const float unit = v_ref * (1.0f / 16384.0f);
         float4* const out = reinterpret_cast<float4*>(mem);
+#pragma unroll 1
         for (uint32_t h = 0; h < 2 * nv; h++) {
             uint32_t v[32];
             tmem_ld(lanes + kO + 32 * h, v);
@@ -1188,10 +1199,17 @@ __global__ void __launch_bounds__(kSwThreads, 1) k_shared_wide(const __grid_cons
         const bool gone = *reinterpret_cast<volatile uint32_t*>(lost);
         const uint32_t mine = rows[row];
         if (mine != 0xffffffffu && half == 0) { float* rec = sa_record(a, mine >> 10, mine & 1023, c.split); rec[0] = gone ? kBatchNaN : m * kLn2; rec[1] = gone ? kBatchNaN : l; }
-        for (uint32_t i = threadIdx.x; i < 128 * (cols / 4); i += 128) {
-            const uint32_t r = i / (cols / 4), j = i % (cols / 4), to = rows[r];
-            if (to == 0xffffffffu) continue;
-            *reinterpret_cast<float4*>(sa_record(a, to >> 10, to & 1023, c.split) + 4 + c0 + 4 * j) = gone ? make_float4(kBatchNaN, kBatchNaN, kBatchNaN, kBatchNaN) : out[r * (kSwCols / 4) + (j ^ (r & 7))];
+        const uint32_t e = threadIdx.x % (kSwCols / 4);
+#pragma unroll 1
+        for (uint32_t r0 = threadIdx.x / (kSwCols / 4); r0 < 128; r0 += 16) {
+            uint32_t to[8];
+            float4 y[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) { to[i] = rows[r0 + 2 * i]; y[i] = out[(r0 + 2 * i) * (kSwCols / 4) + (e ^ ((r0 + 2 * i) & 7))]; }
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (to[i] != 0xffffffffu && 4 * e < cols)
+                    *reinterpret_cast<float4*>(sa_record(a, to[i] >> 10, to[i] & 1023, c.split) + 4 + c0 + 4 * e) = gone ? make_float4(kBatchNaN, kBatchNaN, kBatchNaN, kBatchNaN) : y[i];
         }
     }
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");

@@ -97,6 +97,13 @@ def test_adapter_linear_refuses(kw):
     assert change(DeviceOp.adapter_linear, ADAPTER, ADAPTER_SIZES, **kw)
 
 
+@pytest.mark.parametrize("kw", [dict(adapters=1 << 31, K=1 << 31, N=1 << 31), dict(adapters=1 << 30, K=1 << 24, N=1 << 24)])
+def test_adapter_linear_refuses_products_that_pass_64_bits(kw):
+    """Buffers as large as the rows ask for, and weights whose size is a multiple of 2^64."""
+    sizes = [1 << 33, 1 << 33, 2 * 4 * 14, table_words(1), 1 << 33, 2]
+    assert change(DeviceOp.adapter_linear, ADAPTER, sizes, **dict(kw, B=1, rank=1024, scales=None, a_off=0, b_off=0))
+
+
 def test_adapter_linear_in_place():
     assert change(DeviceOp.adapter_linear, ADAPTER, ADAPTER_SIZES, base=None) is None
 

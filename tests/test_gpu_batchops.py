@@ -507,3 +507,24 @@ def test_wide_what_pairs_cannot_hold(cuda_backend, what):
     fine = np.isfinite(want)
     assert np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(got[~fine & ~np.isnan(want)], want[~fine & ~np.isnan(want)])
     assert (np.abs(got[fine] - want[fine]) <= np.where(np.isfinite(tol), tol, 1e-4)[fine]).all()
+
+
+@pytest.mark.parametrize("prefix,slot", [(501, 0), (500, 2), (500, -1), (-1, 0), (2 ** 31 - 1, 0)])
+def test_wide_prefix_out_of_range(cuda_backend, prefix, slot):
+    from zgml_b200 import DeviceOp
+    B, d = 40, 160
+    one = np.ones((B, 8 * d), np.float32)
+    make = lambda at: [DeviceOp.shared_attention(at["dst"], at["q"], at["own"], at["own"], at["pre"], at["pre"], at["table"], 0, 0, 0, 0, 0, B, 8, 1, d, d, 8 * d, d, d, 4, d, d, 500, 0.1)]
+    p = Prog(cuda_backend, make, dict(dst=one, q=one, own=np.ones((B, 4, d), np.float32), pre=np.ones((2, 500, d), np.float32), table=np.zeros(8 + 4 * B, np.int32)))
+    assert np.isnan(p.run(["dst"], table=table([(i, 1, 0) for i in range(B)], B, prefix, slot))).all()
+    assert np.abs(p.run(["dst"], table=table([(i, 1, 0) for i in range(B)], B, 500, 1)) - 1.0).max() <= 2.0 ** -20          # the same program, another table: a mean of ones
+    assert (p.run(["dst"], table=table([(i, 0, 0) for i in range(B)], B, 0, -5)) == 0.0).all()
+    p.close()
+
+
+def test_no_wait_ran_out(cuda_backend):
+    """The kernels that wait on barriers count waits that gave up."""
+    from zgml_b200 import DeviceOp, DeviceProgram
+    h = cuda_backend.compile_program(DeviceProgram([DeviceOp.logit_rules(0, 0, 1, 1, 4)], [4, 20]))
+    assert cuda_backend.lib.zg_cuda_program_stats(h.ptr, 5) == 0
+    cuda_backend.free_program(h)

@@ -648,7 +648,7 @@ bool zg_adapter_linear_valid(const ZgSeqOp& s, const size_t* elems, size_t n_buf
     auto fits = [&](int i, size_t off, size_t n) { return have(i) && off + n <= elems[s.buf[i]]; };
     auto wfits = [&](int i, uint32_t wdt, size_t off, size_t n) { return wdt <= ZG_W_BF16 && have(i) && (wdt == ZG_W_BF16 ? (off + n + 1) / 2 : off + n) <= elems[s.buf[i]]; };
     const size_t B = s.n[0], N = s.n[1], K = s.n[2], rank = s.n[3], A = s.n[4], srs = s.n[5], drs = s.n[6], brs = s.n[8];
-    if (!B || !N || !K || !rank || !A || B > 65536 || rank > 1024) return fail("adapter_linear: shape");
+    if (!B || !N || !K || !rank || !A || B > 65536 || rank > 1024 || A > ((size_t)1 << 48) / (rank * std::max(N, K))) return fail("adapter_linear: shape");      // (no product below passes 64 bits)
     if ((B > 1 && (srs < K || drs < N || brs < N)) || !fits(0, s.off[3], (B - 1) * drs + N) || !fits(1, s.off[2], (B - 1) * srs + K) || !fits(5, s.off[5], (B - 1) * brs + N)) return fail("adapter_linear: rows");
     if (!wfits(2, s.n[7], s.off[0], A * rank * K) || !wfits(2, s.n[7], s.off[1], A * rank * N)) return fail("adapter_linear: weights");
     if (s.buf[3] != ZG_NO_BUF && !fits(3, s.off[4], A)) return fail("adapter_linear: scales");

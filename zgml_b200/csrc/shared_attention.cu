@@ -839,7 +839,8 @@ __global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const __grid_co
 //   scores[128 rows x 128 keys] += queries[64 dims] keys[64 dims]^T, three MMAs a product;  outputs[128 x 64 columns] += probabilities[128 keys] values[128 keys x 64 columns].
 // Values come as the keys do, by rows, and are read as a transposed operand.  TMEM: scores of two tiles (which become the probabilities in place), outputs.
 // Outputs stay in TMEM from tile to tile; where a row's maximum grows they are scaled there.  Warps 0 - 3 are the softmax (a thread a query row), warp 4 issues, warp 5 copies.
-// What bounds it: 64 KB of operands for every 64 dims of a tile, which an SM takes 1000 clocks to read and 770 to multiply.
+// What bounds it: 64 KB of operands for every 64 dims of a tile, which an SM takes 1030 clocks to read and 770 to multiply.  256 query rows, 4096 keys of 576 dims, 512 columns:
+// pairs 10 us, this kernel 22 us (a tile a CTA: 7500 clocks until the first copy, 11500 scores, 4700 softmax, 4000 outputs, 8000 until they are stored), k_shared_rows 27 us.
 // What pairs cannot hold is known before the first product (the first kernel's scales and flags): the CTA then walks its share in plain f32.
 constexpr uint32_t kSwKeys = 128, kSwCols = 256, kSwStages = 3, kSwPart = 128 * 128, kSwStage = 4 * kSwPart, kSwThreads = 192;
 constexpr uint32_t kSwFactors = kSwStages * kSwStage, kSwRows = kSwFactors + 2 * 128 * 8, kSwRed = kSwRows + 512, kSwBars = kSwRed + 128, kSwSmem = kSwBars + 128 + 1024;
@@ -1221,6 +1222,8 @@ __global__ void __launch_bounds__(kSwThreads, 1) k_shared_wide(const __grid_cons
 
 // What decides a launch: queries a CTA of k_shared_rows holds (RQ), float4 a lane holds (NV), lanes that share a key (LK), shares of its keys; shares of the prefix
 // on the tensor cores (0: k_shared_rows walks the prefix too).
+// Rows x heads x prefix from which the two launches of k_shared_wide pay (16 heads of 576 and 512 dims, up to 256 keys of their own; us, on the tensor cores and in
+// k_shared_rows alone): 16 rows, 256 keys 45.1 / 43.1, 512 keys 45.2 / 55.5, 4096 keys 53 / 230; 6 rows, 1024 keys 41.1 / 36.9; 2 rows, 8192 keys 57.4 / 69.7; 64 rows, 256 keys 74.0 / 88.1.
 constexpr uint64_t kSwLeast = 1u << 17;
 struct SaShape { uint32_t RQ, NV, LK, chunks, splits, warps, shares, row_tiles, halves; bool records; };      // halves: of the output columns, of a head wider than 128 (0: k_shared_prefix)
 SaShape sa_shape(const ZgSeqOp& s, bool wide) {
@@ -1232,7 +1235,7 @@ SaShape sa_shape(const ZgSeqOp& s, bool wide) {
     p.RQ = std::min(rep, p.NV == 8 ? 2u : 4u);
     p.chunks = (rep + p.RQ - 1) / p.RQ;
     const bool narrow = dim <= 128;
-    if (wide && Rp && B * rep >= 32 && (narrow || (uint64_t)B * s.n[1] * Rp >= kSwLeast)) {
+    if (wide && Rp && B * rep >= 32 && (narrow || ((uint64_t)B * s.n[1] * Rp >= kSwLeast && 2ull * G * (Rp + 2 * kSwKeys) < 1u << 31))) {      // (rows of pairs are counted in 31 bits)
         // The number of shares that keeps the GPU busy with the fewest tiles of 64 (128) keys one after the other, and six tiles' (one tile's) time for each start and end.
         p.row_tiles = (B * rep + 127) / 128;
         p.halves = narrow ? 0 : (dv + kSwCols - 1) / kSwCols;

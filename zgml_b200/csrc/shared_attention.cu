@@ -840,7 +840,7 @@ __global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const __grid_co
 // Values come as the keys do, by rows, and are read as a transposed operand.  TMEM: scores of two tiles (which become the probabilities in place), outputs.
 // Outputs stay in TMEM from tile to tile; where a row's maximum grows they are scaled there.  Warps 0 - 3 are the softmax (a thread a query row), warp 4 issues, warp 5 copies.
 // What bounds it: 64 KB of operands for every 64 dims of a tile, which an SM takes 1030 clocks to read and 770 to multiply.  256 query rows, 4096 keys of 576 dims, 512 columns:
-// pairs 10 us, this kernel 22 us (a tile a CTA: 7500 clocks until the first copy, 11500 scores, 4700 softmax, 4000 outputs, 8000 until they are stored), k_shared_rows 27 us.
+// pairs 8.6 us, this kernel 22 us (a tile a CTA: 7500 clocks until the first copy, 11500 scores, 4700 softmax, 4000 outputs, 8000 until they are stored), k_shared_rows 27 us.
 // What pairs cannot hold is known before the first product (the first kernel's scales and flags): the CTA then walks its share in plain f32.
 constexpr uint32_t kSwKeys = 128, kSwCols = 256, kSwStages = 3, kSwPart = 128 * 128, kSwStage = 4 * kSwPart, kSwThreads = 192;
 constexpr uint32_t kSwFactors = kSwStages * kSwStage, kSwRows = kSwFactors + 2 * 128 * 8, kSwRed = kSwRows + 512, kSwBars = kSwRed + 128, kSwSmem = kSwBars + 128 + 1024;
@@ -850,7 +850,7 @@ struct SwArgs {
     uint32_t* flags;                             // [keys, values][G][blocks of eight rows]: something that pairs cannot hold
     uint32_t KR, QR, dkp, dvp, v0, latent, halves, row_tiles;      // rows of keys and queries; first column of the values in their plane; values are the keys' pairs
 };
-// Block of eight rows -> pairs.  Blocks: keys, values (unless they are the keys'), queries.  A thread holds four dims of the eight rows.
+// Block of eight rows -> pairs.  Blocks: keys, values (unless they are the keys'), queries.  A thread holds four dims of the eight rows, and there are no more threads than that takes.
 __global__ void __launch_bounds__(256) k_shared_pairs(const SaArgs a, const SwArgs w) {
     pdl_enter();
     __shared__ uint32_t red[8][8], bad_rows;
@@ -891,7 +891,7 @@ __global__ void __launch_bounds__(256) k_shared_pairs(const SaArgs a, const SwAr
     float* const factor = kind == 2 ? w.qf : kind ? w.vf : w.kf;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, red[i][lane & 7]));
+        const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, lane < blockDim.x / 32 ? red[i][lane] : 0u));
         float s, inv;
         split_scale(top, s, inv);
         const bool wrong = !(inv == inv);
@@ -1314,7 +1314,7 @@ bool sa_launch_wide(const ZgOp& op, const SaArgs& a, const SwArgs& w, cudaStream
     if (!sw_encode(&mq, w.q, w.dkp, 2ull * a.G * w.QR) || !sw_encode(&mk, w.k, w.dkp, 2ull * a.G * w.KR)) return false;
     if (!sw_encode(&mv, w.latent ? w.k : w.v, w.latent ? w.dkp : w.dvp, 2ull * a.G * w.KR)) return false;
     if (!zg_smem_limit<k_shared_wide>(kSwSmem)) return false;
-    launch_pdl(k_shared_pairs, dim3(a.G * ((w.latent ? 1 : 2) * (w.KR / 8) + w.QR / 8)), dim3(256), 0, st, a, w);
+    launch_pdl(k_shared_pairs, dim3(a.G * ((w.latent ? 1 : 2) * (w.KR / 8) + w.QR / 8)), dim3((std::max(w.dkp, w.dvp) / 4 + 31) / 32 * 32), 0, st, a, w);
     ZG_SEQ_CHECK();
     launch_pdl(k_shared_wide, dim3(w.row_tiles * w.halves * a.shares * a.G), dim3(kSwThreads), kSwSmem, st, a, w, mq, mk, mv);
     return true;

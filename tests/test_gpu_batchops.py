@@ -431,6 +431,16 @@ def test_rule_rows_left_alone_and_out_of_range(cuda_backend):
         p.close()
 
 
+@pytest.mark.parametrize("wdt", ["bf16", "f32"])
+@pytest.mark.parametrize("rank", [8, 24, 64])
+@pytest.mark.parametrize("B,N,runs", [(300, 976, 1), (584, 640, 1), (700, 128, 1), (300, 976, 2), (1400, 300, 3)])
+def test_adapters_of_one_tile(cuda_backend, wdt, rank, B, N, runs):
+    """As many CTAs as tiles: a CTA has one product to do, or as many as its block has runs.  Other programs run between, so that nothing right lies in shared memory yet."""
+    for seed in range(3):
+        adapter_case(cuda_backend, wdt, B, N, 440, rank, 4, [(0, 0, (i * runs // B + seed) % 4) for i in range(B)], seed=seed)
+        attend_case(cuda_backend, 3, 8, 2, 64, 64, 90, 33, [(i, 5, 0) for i in range(3)], loud=1e4)
+
+
 # ── wide heads with many query rows over a long prefix: tensor cores ─────────────────────────────────────────────────
 def wide_entries(B, R):
     return [(i, (5 + 7 * i) % (R + 1), 0) for i in range(B)]

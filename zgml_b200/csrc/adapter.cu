@@ -497,7 +497,8 @@ __global__ void __launch_bounds__(kAxThreads, 1) k_adapter_expand(AdArgs a, cons
             if (++f_run == n_runs) { f_run = 0; f_tile++; }
         };
         constexpr uint32_t kAhead = L::stages - 1;                   // stages that are on their way while one is used
-        for (uint32_t i = 0; i < min(kAhead, items); i++) fill();
+        // (a group for every stage ahead, empty where there are fewer items: the waits below count groups)
+        for (uint32_t i = 0; i + 1 < L::stages; i++) { if (i < items) fill(); else asm volatile("cp.async.commit_group;" ::: "memory"); }
         for (uint32_t item = 0; item < items; item++) {
             if (item + kAhead < items) fill(); else asm volatile("cp.async.commit_group;" ::: "memory");
             asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");

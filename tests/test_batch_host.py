@@ -104,6 +104,16 @@ def test_adapter_linear_refuses_products_that_pass_64_bits(kw):
     assert change(DeviceOp.adapter_linear, ADAPTER, sizes, **dict(kw, B=1, rank=1024, scales=None, a_off=0, b_off=0))
 
 
+def test_adapter_linear_forms():
+    for form in ("auto", "runs", "blocks"):
+        assert change(DeviceOp.adapter_linear, ADAPTER, ADAPTER_SIZES, form=form) is None
+    with pytest.raises(ValueError):
+        DeviceOp.adapter_linear(**ADAPTER, form="rows")
+    op = DeviceOp.adapter_linear(**ADAPTER)
+    op.u.seq.n[9] = 3
+    assert seq_check(op, ADAPTER_SIZES)
+
+
 def test_adapter_linear_in_place():
     assert change(DeviceOp.adapter_linear, ADAPTER, ADAPTER_SIZES, base=None) is None
 

@@ -269,7 +269,7 @@ def exact16(r, *shape, scale=1.0):
     return (v.view(np.uint32) & np.uint32(0xFFFF0000)).view(np.float32)
 
 
-def adapter_case(be, fmt, B, N, K, rank, A, entries, *, pad=0, offset=0, scaled=True, in_place=False, live=None, seed=0):
+def adapter_case(be, fmt, B, N, K, rank, A, entries, *, pad=0, offset=0, scaled=True, in_place=False, live=None, seed=0, form="auto"):
     from zgml_b200 import DeviceOp, abi
     r = np.random.default_rng(seed)
     a, b = exact16(r, A, rank, K, scale=K ** -0.5), exact16(r, A, N, rank, scale=rank ** -0.5)
@@ -279,7 +279,7 @@ def adapter_case(be, fmt, B, N, K, rank, A, entries, *, pad=0, offset=0, scaled=
     arrays = dict(dst=base if in_place else dst, x=x, w=bf16_bits(flat) if fmt == "bf16" else flat, scales=scales, table=table(entries, B, live=live))
     if not in_place:
         arrays["base"] = base
-    make = lambda at: [DeviceOp.adapter_linear(at["dst"], at["x"], at["w"], offset, offset + A * rank * K, at["table"], B, N, K, rank, A, abi.W_BF16 if fmt == "bf16" else abi.W_F32, base=at.get("base"),
+    make = lambda at: [DeviceOp.adapter_linear(at["dst"], at["x"], at["w"], offset, offset + A * rank * K, at["table"], B, N, K, rank, A, abi.W_BF16 if fmt == "bf16" else abi.W_F32, form=form, base=at.get("base"),
                                                base_off=0 if in_place else pad, base_rs=N + pad, scales=at["scales"] if scaled else None, src_off=pad, src_rs=K + pad, dst_off=0 if in_place else pad, dst_rs=N + pad)]
     p = Prog(be, make, arrays)
     c = 0 if in_place else pad
@@ -439,6 +439,26 @@ def test_adapters_of_one_tile(cuda_backend, wdt, rank, B, N, runs):
     for seed in range(3):
         adapter_case(cuda_backend, wdt, B, N, 440, rank, 4, [(0, 0, (i * runs // B + seed) % 4) for i in range(B)], seed=seed)
         attend_case(cuda_backend, 3, 8, 2, 64, 64, 90, 33, [(i, 5, 0) for i in range(3)], loud=1e4)
+
+
+@pytest.mark.parametrize("wdt", ["bf16", "f32"])
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("form", ["runs", "blocks"])
+def test_adapters_in_blocks_and_by_runs(cuda_backend, wdt, in_place, form):
+    """Blocks of 128 rows with long runs, with runs of one to nine rows, without any adapter, with a bad one, and the last one cut short."""
+    which = [i // 64 for i in range(128)] + [i % 5 - 1 for i in range(128)] + [-1] * 128 + [i // 9 % 4 for i in range(100)] + [7] * 28 + [2] * 33 + [i // 31 % 3 for i in range(110)]
+    entries = [(-1 if i % 50 == 49 else 0, 0, w) for i, w in enumerate(which)]
+    adapter_case(cuda_backend, wdt, len(entries), 328, 200, 24, 4, entries, in_place=in_place, form=form)
+    adapter_case(cuda_backend, wdt, len(entries), 328, 200, 24, 4, entries, in_place=in_place, live=500, form=form)
+
+
+@pytest.mark.parametrize("wdt", ["bf16", "f32"])
+@pytest.mark.parametrize("rank", [8, 16, 24, 40, 64, 128, 136])
+def test_adapters_of_many_outputs(cuda_backend, wdt, rank):
+    """Runs of one row and of more, weights beyond what is fetched ahead, outputs that end inside a warp's."""
+    for N in (9003, 333):
+        for form in ("runs", "blocks"):
+            adapter_case(cuda_backend, wdt, 13, N, 72, rank, 3, [(0, 0, w) for w in (0, 1, 1, 2, 2, 2, 2, 0, 0, 0, 0, 0, 1)], form=form)
 
 
 # ── wide heads with many query rows over a long prefix: tensor cores ─────────────────────────────────────────────────

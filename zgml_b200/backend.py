@@ -461,13 +461,14 @@ class DeviceOp:
                              DeviceOp._words(B, H, G, dk, dv, q_rs, k_width, v_width, rows, k_prefix_width, v_prefix_width, prefix_rows, dst_rs or dst_col + H * dv, sink_wdt), [scale, softcap])
 
     @staticmethod
-    def adapter_linear(dst, src, w, a_off, b_off, table, B, N, K, rank, adapters, wdt, base=None, base_off=0, base_rs=0, scales=None, scales_off=0, src_off=0, src_rs=0, dst_off=0, dst_rs=0):
+    def adapter_linear(dst, src, w, a_off, b_off, table, B, N, K, rank, adapters, wdt, base=None, base_off=0, base_rs=0, scales=None, scales_off=0, src_off=0, src_rs=0, dst_off=0, dst_rs=0, form="auto"):
         """dst = base + scale * B (A src) with the row's own adapter: A [adapters, rank, K] and B [adapters, N, rank] in arena `w`.  `base` None: dst itself, as the
-        LINEAR before left it."""
+        LINEAR before left it.  `form`: "runs" (rows of decoding, whose adapters change from row to row), "blocks" (prompts: long runs of rows with one adapter), or by
+        the number of rows."""
         if base is None:
             base, base_off, base_rs = dst, dst_off, dst_rs
         return DeviceOp._seq(abi.OP_ADAPTER_LINEAR, [dst, src, w, scales, table, base], DeviceOp._words(a_off, b_off, src_off, dst_off, scales_off, base_off),
-                             DeviceOp._words(B, N, K, rank, adapters, src_rs or K, dst_rs or N, wdt, base_rs or N))
+                             DeviceOp._words(B, N, K, rank, adapters, src_rs or K, dst_rs or N, wdt, base_rs or N, ["auto", "runs", "blocks"].index(form)))
 
     @staticmethod
     def logit_rules(dst, src, table, B, V, history=None, history_rows=0, bias=None, masks=None, src_off=0, src_rs=0, dst_off=0, dst_rs=0):

@@ -114,10 +114,103 @@ __device__ __forceinline__ void af_expand(const AdArgs& a, const WT* wb, const f
             if (R == 1 || r < (int)rows) dst[(size_t)r * a.dst_rs + n] = base[(size_t)r * a.base_rs + n] + acc[r];
     }
 }
-// vec_k: x and A in vectors; vec_j: rows of B in vectors of four; stage: bytes of B fetched ahead (0: not)
-template <typename WT>
-__global__ void __launch_bounds__(kAfThreads) __cluster_dims__(kAfCluster, 1, 1) k_adapter_few(AdArgs a, const WT* __restrict__ wa, const WT* __restrict__ wb, uint32_t k_slice, uint32_t n_slice,
-                                                                                             uint32_t vec_k, uint32_t vec_j, uint32_t stage) {
+// The same with LJ lanes to an output, 16 bytes of its weights each, so that a warp reads whole rows side by side: of rank 64 a lane per output met one bank, or
+// 32 lines a load (14336 outputs, 8 rows: 51 us).  U outputs (of one row) or R rows (of one output) at a time make C sums a lane, which meet by halves: a lane ends with
+// C / LJ of them, or one.  Loads of the next outputs, and the base, are under way meanwhile.
+template <typename WT, int R, int LJ>
+__device__ __forceinline__ void af_expand_wide(const AdArgs& a, const WT* wb, const float* base, float* dst, uint32_t rows, uint32_t n0, uint32_t n1, const float* h) {
+    constexpr uint32_t E = 16 / sizeof(WT), G = 32 / LJ, U = R == 1 ? 8 : 1, C = R * U, kept = C > LJ ? C / LJ : 1, step = kAfThreads / 32 * G * U;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane & (LJ - 1);
+    const bool on = sub * E < a.rank;
+    uint32_t c0 = 0;                                                 // the first sum that the lane ends with
+    bool mine = true;                                                // it stores
+    {
+        uint32_t count = C;
+#pragma unroll
+        for (int d = LJ / 2; d > 0; d >>= 1) {
+            if (count > 1) { count /= 2; c0 += lane & d ? count : 0; }
+            else mine = mine && !(lane & d);
+        }
+    }
+    float2 y[R][E / 2];
+#pragma unroll
+    for (int r = 0; r < R; r++)
+#pragma unroll
+        for (int e = 0; e < (int)E / 2; e++) y[r][e] = on ? make_float2(h[r * a.rank + sub * E + 2 * e], h[r * a.rank + sub * E + 2 * e + 1]) : make_float2(0.0f, 0.0f);
+    uint4 next[U];
+    auto load = [&](uint32_t first) {
+#pragma unroll
+        for (uint32_t u = 0; u < U; u++) {
+            const uint32_t n = first + u * G + lane / LJ;
+            next[u] = on && n < n1 ? *reinterpret_cast<const uint4*>(wb + (size_t)(n - n0) * a.rank + sub * E) : make_uint4(0, 0, 0, 0);
+        }
+    };
+    uint32_t first = n0 + warp * G * U;
+    load(first);
+    for (; first < n1; first += step) {
+        uint4 now[U];
+        float b[kept], v[C];
+        bool to[kept];
+#pragma unroll
+        for (uint32_t u = 0; u < U; u++) now[u] = next[u];
+        load(first + step);
+#pragma unroll
+        for (uint32_t i = 0; i < kept; i++) {
+            const uint32_t c = c0 + i, r = R == 1 ? 0 : c, n = first + (R == 1 ? c * G : 0) + lane / LJ;
+            to[i] = mine && n < n1 && r < rows;
+            b[i] = to[i] ? base[(size_t)r * a.base_rs + n] : 0.0f;
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < U; u++) {
+            const uint32_t x[4] = {now[u].x, now[u].y, now[u].z, now[u].w};
+            float2 w[E / 2];
+#pragma unroll
+            for (int e = 0; e < (int)E / 2; e++)
+                w[e] = sizeof(WT) == 2 ? make_float2(__uint_as_float(x[e] << 16), __uint_as_float(x[e] & 0xFFFF0000u)) : make_float2(__uint_as_float(x[2 * e & 3]), __uint_as_float(x[(2 * e + 1) & 3]));
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                float2 z = __fmul2_rn(w[0], y[r][0]);
+#pragma unroll
+                for (int e = 1; e < (int)E / 2; e++) z = __ffma2_rn(w[e], y[r][e], z);
+                v[R == 1 ? u : r] = z.x + z.y;
+            }
+        }
+        int count = C;
+#pragma unroll
+        for (int d = LJ / 2; d > 0; d >>= 1) {
+            const bool up = lane & d;
+            if (count > 1) {
+                count /= 2;
+#pragma unroll
+                for (int i = 0; i < count; i++) {
+                    const float there = __shfl_xor_sync(0xffffffffu, up ? v[i] : v[i + count], d);
+                    v[i] = (up ? v[i + count] : v[i]) + there;
+                }
+            } else v[0] += __shfl_xor_sync(0xffffffffu, v[0], d);
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kept; i++) {
+            const uint32_t c = c0 + i, r = R == 1 ? 0 : c, n = first + (R == 1 ? c * G : 0) + lane / LJ;
+            if (to[i]) dst[(size_t)r * a.dst_rs + n] = b[i] + v[i];
+        }
+    }
+}
+template <typename WT, int R>
+__device__ __forceinline__ void af_expand_by(uint32_t lanes, const AdArgs& a, const WT* wb, const float* base, float* dst, uint32_t rows, uint32_t n0, uint32_t n1, const float* h) {
+    switch (lanes) {
+        case 1: af_expand_wide<WT, R, 1>(a, wb, base, dst, rows, n0, n1, h); break;
+        case 2: af_expand_wide<WT, R, 2>(a, wb, base, dst, rows, n0, n1, h); break;
+        case 4: af_expand_wide<WT, R, 4>(a, wb, base, dst, rows, n0, n1, h); break;
+        case 8: af_expand_wide<WT, R, 8>(a, wb, base, dst, rows, n0, n1, h); break;
+        default: af_expand_wide<WT, R, 16>(a, wb, base, dst, rows, n0, n1, h);
+    }
+}
+// vec_k: x and A in vectors; vec_j: rows of B in vectors of four; WIDE: `lanes` lanes share an output; stage: bytes of B fetched
+// ahead (0: not)
+// (64 registers: 64 rows are 512 CTAs, four an SM; at 80 they took 12.4 us instead of 8.3)
+template <typename WT, bool WIDE>
+__global__ void __launch_bounds__(kAfThreads, WIDE ? 2 : 4) __cluster_dims__(kAfCluster, 1, 1) k_adapter_few(AdArgs a, const WT* __restrict__ wa, const WT* __restrict__ wb, uint32_t k_slice, uint32_t n_slice,
+                                                                                             uint32_t vec_k, uint32_t vec_j, uint32_t lanes, uint32_t stage) {
     pdl_enter();
     extern __shared__ float4 af_mem[];                               // [stage] weights of the CTA's outputs; [8][rank] the CTA's sums; [8][rank] all sums
     const uint32_t rank_id = blockIdx.x % kAfCluster, r = blockIdx.x / kAfCluster;
@@ -179,7 +272,9 @@ __global__ void __launch_bounds__(kAfThreads) __cluster_dims__(kAfCluster, 1, 1)
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
     const WT* const from = stage ? reinterpret_cast<const WT*>(af_mem) : wb;
-    if (rows == 1) {
+    if constexpr (WIDE) {
+        if (rows == 1) af_expand_by<WT, 1>(lanes, a, from, base, dst, rows, n0, n1, h); else af_expand_by<WT, kAfRows>(lanes, a, from, base, dst, rows, n0, n1, h);
+    } else if (rows == 1) {
         if (vec_j) af_expand<WT, 1, true>(a, from, base, dst, rows, n0, n1, h); else af_expand<WT, 1, false>(a, from, base, dst, rows, n0, n1, h);
     } else {
         if (vec_j) af_expand<WT, kAfRows, true>(a, from, base, dst, rows, n0, n1, h); else af_expand<WT, kAfRows, false>(a, from, base, dst, rows, n0, n1, h);
@@ -610,11 +705,13 @@ __global__ void __launch_bounds__(kAxThreads, 1) k_adapter_expand(AdArgs a, cons
     if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(0u) : "memory");
 }
 
-// More rows than kAmLeast go in blocks, where rank and strides allow their 16-byte pieces.
+// More rows than kAmLeast go in blocks, where rank and strides allow their 16-byte pieces, unless the op says which way to take: a block walks its runs one after the other, and only the
+// host knows how long they are.  us in blocks and by runs of eight: 4096 inputs and outputs, rank 16: 256 rows in runs of 64 26.7 / 20.4, 512 in runs of 128 24.6 / 30.4, of 8 102 / 27, of one 712 / 45;
+// 14336 outputs, rank 64: 64 rows of one run 27 / 42, 256 in runs of 128 26.5 / 57.7.
 constexpr uint32_t kAmLeast = 256;
 bool many_rows(const ZgSeqOp& s) {
-    const uint32_t B = s.n[0], K = s.n[2], rank = s.n[3];
-    return B > kAmLeast && K % 8 == 0 && rank % 8 == 0 && rank <= kAmRank && s.n[5] % 4 == 0 && s.off[2] % 4 == 0 && s.off[0] % 8 == 0 && s.off[1] % 8 == 0;
+    const uint32_t B = s.n[0], K = s.n[2], rank = s.n[3], form = s.n[9];
+    return (form == 2 || (form == 0 && B > kAmLeast)) && K % 8 == 0 && rank % 8 == 0 && rank <= kAmRank && s.n[5] % 4 == 0 && s.off[2] % 4 == 0 && s.off[0] % 8 == 0 && s.off[1] % 8 == 0;
 }
 template <typename WT>
 bool launch_few(const AdArgs& a, const WT* wa, const WT* wb, cudaStream_t st) {
@@ -622,12 +719,24 @@ bool launch_few(const AdArgs& a, const WT* wa, const WT* wb, cudaStream_t st) {
     const uint32_t V = WVec<WT>::n, k_slice = ((a.K + kAfCluster - 1) / kAfCluster + V - 1) / V * V, n_slice = ((a.N + kAfCluster - 1) / kAfCluster + 7) / 8 * 8;
     const uint32_t vec_k = a.K % V == 0 && a.src_rs % 4 == 0 && aligned(wa, 16) && aligned(a.src, 16);
     const uint32_t vec_j = a.rank % 4 == 0 && aligned(wb, 4 * sizeof(WT));
+    // Several lanes an output for long weights or many outputs; a lane an output, in a kernel of half the registers, otherwise.  64 rows of 4096 inputs, a run each, us by several
+    // lanes and by one: rank 8, 2048 outputs 10.3 / 6.3; rank 16, 4096 outputs 10.3 / 8.4, 8192 12.4 / 10.3, 14336 14.4 / 19.7; rank 32, 4096 12.4 / 14.4; rank 64, 4096 18.5 / 42.8
+    constexpr uint32_t E = 16 / sizeof(WT);
+    uint32_t lanes = 1;
+    while (lanes * E < a.rank) lanes *= 2;
+    const bool wide = a.rank % E == 0 && lanes <= 16 && aligned(wb, 16) && (a.rank * sizeof(WT) >= 64 || n_slice > 1024);
     // A slice begins at n_slice rank weights from the adapter's, which is N rank from the next one's
     const size_t bytes = (size_t)n_slice * a.rank * sizeof(WT);
     const uint32_t stage = bytes <= kAfStage && aligned(wb, 16) && (size_t)a.N * a.rank * sizeof(WT) % 16 == 0 ? (uint32_t)((bytes + 15) & ~(size_t)15) : 0;
     const size_t smem = stage + 2 * kAfRows * sizeof(float) * ((a.rank + 3) / 4 * 4);
-    if (!zg_smem_limit<k_adapter_few<WT>>(kAfStage + 2 * kAfRows * sizeof(float) * 1024)) return false;
-    launch_pdl(k_adapter_few<WT>, dim3(a.B * kAfCluster), dim3(kAfThreads), smem, st, a, wa, wb, k_slice, n_slice, vec_k, vec_j, stage);
+    constexpr size_t limit = kAfStage + 2 * kAfRows * sizeof(float) * 1024;
+    if (wide) {
+        if (!zg_smem_limit<k_adapter_few<WT, true>>(limit)) return false;
+        launch_pdl(k_adapter_few<WT, true>, dim3(a.B * kAfCluster), dim3(kAfThreads), smem, st, a, wa, wb, k_slice, n_slice, vec_k, vec_j, lanes, stage);
+    } else {
+        if (!zg_smem_limit<k_adapter_few<WT, false>>(limit)) return false;
+        launch_pdl(k_adapter_few<WT, false>, dim3(a.B * kAfCluster), dim3(kAfThreads), smem, st, a, wa, wb, k_slice, n_slice, vec_k, vec_j, lanes, stage);
+    }
     return true;
 }
 template <typename WT>
@@ -648,6 +757,7 @@ bool zg_adapter_linear_valid(const ZgSeqOp& s, const size_t* elems, size_t n_buf
     auto have = [&](int i) { return s.buf[i] != ZG_NO_BUF && s.buf[i] < n_bufs; };
     auto fits = [&](int i, size_t off, size_t n) { return have(i) && off + n <= elems[s.buf[i]]; };
     auto wfits = [&](int i, uint32_t wdt, size_t off, size_t n) { return wdt <= ZG_W_BF16 && have(i) && (wdt == ZG_W_BF16 ? (off + n + 1) / 2 : off + n) <= elems[s.buf[i]]; };
+    if (s.n[9] > 2) return fail("adapter_linear: form");
     const size_t B = s.n[0], N = s.n[1], K = s.n[2], rank = s.n[3], A = s.n[4], srs = s.n[5], drs = s.n[6], brs = s.n[8];
     if (!B || !N || !K || !rank || !A || B > 65536 || rank > 1024 || A > ((size_t)1 << 48) / (rank * std::max(N, K))) return fail("adapter_linear: shape");      // (no product below passes 64 bits)
     if ((B > 1 && (srs < K || drs < N || brs < N)) || !fits(0, s.off[3], (B - 1) * drs + N) || !fits(1, s.off[2], (B - 1) * srs + K) || !fits(5, s.off[5], (B - 1) * brs + N)) return fail("adapter_linear: rows");

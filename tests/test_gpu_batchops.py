@@ -115,12 +115,14 @@ def test_batch_append_twice_into_one_row(cuda_backend):
 
 
 # ── SHARED_ATTENTION ─────────────────────────────────────────────────────────────────────────────────────────────────
-def attend_case(be, B, H, G, dk, dv, prefix, R, entries, *, cap=0.0, sink=None, pad=0, latent=False, prefix_slots=2, prefix_slot=1, live=None, seed=0, spare=3, scale=None, loud=1.0, graph=True, v_shift=0):
+def attend_case(be, B, H, G, dk, dv, prefix, R, entries, *, cap=0.0, sink=None, pad=0, latent=False, prefix_slots=2, prefix_slot=1, live=None, seed=0, spare=None, scale=None, loud=1.0, graph=True, v_shift=0):
     from zgml_b200 import DeviceOp, abi
     r = np.random.default_rng(seed)
     slots = max([e[0] for e in entries if e[0] < 100] + [0]) + 1
     width = pad + G * dk + (0 if latent else G * dv) + pad
     v_col = pad + v_shift if latent else pad + G * dk
+    if spare is None:                                   # many query rows: a capacity that asks for the tensor cores
+        spare = max(3, (3 << 17) // (B * H) + 1 - prefix) if prefix and B * H // G >= 32 and max(dk, dv) <= 128 else 3
     Rp = prefix + spare
     def cache(n, rows):
         c = r.standard_normal((n, rows, width)).astype(np.float32)
@@ -217,13 +219,14 @@ def test_idle_rows_and_rows_out_of_range(cuda_backend, big):
             assert np.isnan(got[2]).all() and np.isnan(got[3]).all() and np.isnan(got[4]).all() and np.isfinite(got[[0, 1, 5, 6]]).all()
 
 
-@pytest.mark.parametrize("prefix,slot", [(11, 0), (5, 2), (5, -1), (-1, 0), (2 ** 31 - 1, 0)])
+@pytest.mark.parametrize("R", [10, 1300])
+@pytest.mark.parametrize("prefix,slot", [(1301, 0), (5, 2), (5, -1), (-1, 0), (2 ** 31 - 1, 0)])
 @pytest.mark.parametrize("B", [2, 40])
-def test_prefix_out_of_range(cuda_backend, prefix, slot, B):
+def test_prefix_out_of_range(cuda_backend, prefix, slot, B, R):
     from zgml_b200 import DeviceOp
     one = np.ones((B, 8 * 64), np.float32)
-    make = lambda at: [DeviceOp.shared_attention(at["dst"], at["q"], at["own"], at["own"], at["pre"], at["pre"], at["table"], 0, 0, 0, 0, 0, B, 8, 1, 64, 64, 512, 64, 64, 4, 64, 64, 10, 0.1)]
-    p = Prog(cuda_backend, make, dict(dst=one, q=one, own=np.ones((B, 4, 64), np.float32), pre=np.ones((2, 10, 64), np.float32), table=np.zeros(8 + 4 * B, np.int32)))
+    make = lambda at: [DeviceOp.shared_attention(at["dst"], at["q"], at["own"], at["own"], at["pre"], at["pre"], at["table"], 0, 0, 0, 0, 0, B, 8, 1, 64, 64, 512, 64, 64, 4, 64, 64, R, 0.1)]
+    p = Prog(cuda_backend, make, dict(dst=one, q=one, own=np.ones((B, 4, 64), np.float32), pre=np.ones((2, R, 64), np.float32), table=np.zeros(8 + 4 * B, np.int32)))
     assert np.isnan(p.run(["dst"], table=table([(i, 1, 0) for i in range(B)], B, prefix, slot))).all()
     assert (p.run(["dst"], table=table([(i, 1, 0) for i in range(B)], B, 10, 1)) == 1.0).all()          # the same program, another table
     assert (p.run(["dst"], table=table([(i, 0, 0) for i in range(B)], B, 0, -5)) == 0.0).all()          # no prefix: its slot is not looked at; nothing seen: zeros

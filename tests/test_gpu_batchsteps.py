@@ -159,9 +159,9 @@ def test_two_programs_at_once(cuda_backend):
     r = np.random.default_rng(0)
     handles = []
     for seed in range(2):
-        q, own, pre = r.standard_normal((48, 8 * 64)).astype(np.float32), r.standard_normal((48, 5, 256)).astype(np.float32), r.standard_normal((1, 700, 256)).astype(np.float32)
-        t = table([(i, 1 + i % 5, 0) for i in range(48)], 48, 700)
-        op = DeviceOp.shared_attention(0, 1, 2, 2, 3, 3, 4, 0, 0, 128, 0, 128, 48, 8, 2, 64, 64, 512, 256, 256, 5, 256, 256, 700, 0.125)
+        q, own, pre = r.standard_normal((48, 8 * 64)).astype(np.float32), r.standard_normal((48, 5, 256)).astype(np.float32), r.standard_normal((1, 1100, 256)).astype(np.float32)
+        t = table([(i, 1 + i % 5, 0) for i in range(48)], 48, 1100)
+        op = DeviceOp.shared_attention(0, 1, 2, 2, 3, 3, 4, 0, 0, 128, 0, 128, 48, 8, 2, 64, 64, 512, 256, 256, 5, 256, 256, 1100, 0.125)
         h = cuda_backend.compile_program(DeviceProgram([op], [48 * 512, q.size, own.size, pre.size, t.size]))
         first = np.zeros((48, 512), np.float32)
         cuda_backend.execute_program(h, [ProgramIO(1, q.ravel()), ProgramIO(2, own.ravel()), ProgramIO(3, pre.ravel()), ProgramIO(4, t)], [ProgramIO(0, first)])

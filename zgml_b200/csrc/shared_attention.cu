@@ -1225,6 +1225,10 @@ __global__ void __launch_bounds__(kSwThreads, 1) k_shared_wide(const __grid_cons
 // Rows x heads x prefix from which the two launches of k_shared_wide pay (16 heads of 576 and 512 dims, up to 256 keys of their own; us, on the tensor cores and in
 // k_shared_rows alone): 16 rows, 256 keys 45.1 / 43.1, 512 keys 45.2 / 55.5, 4096 keys 53 / 230; 6 rows, 1024 keys 41.1 / 36.9; 2 rows, 8192 keys 57.4 / 69.7; 64 rows, 256 keys 74.0 / 88.1.
 constexpr uint64_t kSwLeast = 1u << 17;
+// The same for k_shared_prefix (32 heads over 8 key heads of 128, up to 512 keys of their own; us, with it and without): 8 rows, 512 keys 33 / 26, 1024 34.6 / 32, 2048 37 / 43,
+// 8192 49 / 108; 32 rows, 64 keys 35 / 25, 256 36.8 / 32.8, 512 36 / 41, 1024 39 / 59; 128 rows, 64 keys 77 / 69, 256 84 / 94.  And from 32 query rows a key head on, since a quarter of
+// a tile is still full then: 4 rows (16 query rows), 4096 keys 37 / 29, 8192 45 / 47; 2 rows, 4096 keys 36.6 / 36.9, 8192 45 / 57; 1 row, 8192 keys 37 / 29.
+constexpr uint64_t kSpLeast = 3u << 17;
 struct SaShape { uint32_t RQ, NV, LK, chunks, splits, warps, shares, row_tiles, halves; bool records; };      // halves: of the output columns, of a head wider than 128 (0: k_shared_prefix)
 SaShape sa_shape(const ZgSeqOp& s, bool wide) {
     const uint32_t B = s.n[0], G = s.n[2], rep = s.n[1] / G, dk = s.n[3], dv = s.n[4], dim = std::max(dk, dv), R = s.n[8], Rp = s.n[11], sms = zg_sm_count();
@@ -1235,7 +1239,7 @@ SaShape sa_shape(const ZgSeqOp& s, bool wide) {
     p.RQ = std::min(rep, p.NV == 8 ? 2u : 4u);
     p.chunks = (rep + p.RQ - 1) / p.RQ;
     const bool narrow = dim <= 128;
-    if (wide && Rp && B * rep >= 32 && (narrow || ((uint64_t)B * s.n[1] * Rp >= kSwLeast && 2ull * G * (Rp + 2 * kSwKeys) < 1u << 31))) {      // (rows of pairs are counted in 31 bits)
+    if (wide && Rp && B * rep >= 32 && (uint64_t)B * s.n[1] * Rp >= (narrow ? kSpLeast : kSwLeast) && (narrow || (2ull * G * (Rp + 2 * kSwKeys) < 1u << 31))) {      // (rows of pairs are counted in 31 bits)
         // The number of shares that keeps the GPU busy with the fewest tiles of 64 (128) keys one after the other, and six tiles' (one tile's) time for each start and end.
         p.row_tiles = (B * rep + 127) / 128;
         p.halves = narrow ? 0 : (dv + kSwCols - 1) / kSwCols;

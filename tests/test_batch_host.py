@@ -32,7 +32,8 @@ def test_rule_table():
     assert masks.tolist() == [[1, 2], [0x55555555, 0x55]]
 
 
-@pytest.mark.parametrize("kw", [dict(repetition=0.0), dict(repetition=-1.0), dict(repetition=float("nan")), dict(repetition=float("inf")), dict(presence=float("inf")), dict(frequency=float("nan"))])
+@pytest.mark.parametrize("kw", [dict(repetition=0.0), dict(repetition=-1.0), dict(repetition=float("nan")), dict(repetition=float("inf")), dict(presence=float("inf")), dict(frequency=float("nan")),
+                                dict(repetition=1e-60), dict(repetition=1e60), dict(presence=1e60), dict(bias={3: float("nan")})])
 def test_rules_refuse(kw):
     with pytest.raises(ValueError):
         LogitRules(**kw)

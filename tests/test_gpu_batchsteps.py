@@ -227,6 +227,8 @@ def test_session_rules(cuda_backend):
     with pytest.raises(ValueError):
         ruled.feed("b", [1], [0], LogitRules(bias={97: 1.0}))
     assert ruled.pool.position("b") == raw.pool.position("b")                              # refused before anything ran
+    a, b = (s.step([{"id": "a", "tokens": [9], "want": [0], **x}], ["b"])[0] for s, x in ((ruled, {"rules": LogitRules(bias={5: 2.0}), "generated": True}), (raw, {})))
+    assert a[0, 5] == b[0, 5] + np.float32(2.0) and np.array_equal(np.delete(a, 5), np.delete(b, 5)) and not ruled.pool.has("b")
     ruled.release("a")
     assert np.array_equal(ruled.feed("a", [7, 8], [1], LogitRules(repetition=1.0)), sessions(cuda_backend, 1)[0].feed("a", [7, 8], [1]))      # a new request, nothing kept of the old one
     for s in (ruled, raw):

@@ -57,10 +57,15 @@ class LogitRules:
     allowed: Optional[np.ndarray] = None
 
     def __post_init__(self):
-        if not (np.isfinite(self.repetition) and self.repetition > 0.0):
+        with np.errstate(over="ignore", under="ignore"):            # (what they are to the kernel)
+            repetition, *others = (np.float32(x) for x in (self.repetition, self.presence, self.frequency))
+            biases = [np.float32(x) for x in self.bias.values()]
+        if not (np.isfinite(repetition) and repetition > 0.0):
             raise ValueError("repetition is a factor above zero")
-        if not (np.isfinite(self.presence) and np.isfinite(self.frequency)):
+        if not np.isfinite(others).all():
             raise ValueError("presence and frequency are finite")
+        if np.isnan(biases).any():
+            raise ValueError("a bias is not a number")
 
     def mask(self, vocab: int) -> Optional[np.ndarray]:
         """int32 words, bit t % 32 of word t / 32 set where token t is allowed."""

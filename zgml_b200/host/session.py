@@ -116,7 +116,7 @@ class SequenceSession:
     # ── the step function ──
     def feed(self, request_id, tokens: Sequence[int], want: Iterable[int] = (), rules: Optional[LogitRules] = None, generated: bool = False) -> np.ndarray:
         """Advance `request_id` by `tokens`; returns the logits at the places `want` (indices into `tokens`), in order.  With `rules` (the last place alone may be wanted)
-        they are what the rules make of them, over all tokens fed for the request; those fed with `generated` count as generated."""
+        they are what the rules make of them, over all tokens fed for the request; those fed with `generated` since the last ones without it count as generated."""
         tokens = [int(t) for t in tokens]
         if any(t < 0 or t >= self.model.vocab for t in tokens):
             raise ValueError("token id outside the vocabulary")
@@ -155,8 +155,8 @@ class SequenceSession:
         self._prompt.pop(request_id, None)
 
     def step(self, entries: Sequence[dict], end: Iterable = ()) -> List[np.ndarray]:
-        """entries: [{"id", "tokens", "want"}]; `end`: requests whose state is given back after the step."""
-        out = [self.feed(e["id"], e["tokens"], e.get("want", ())) for e in entries]
+        """entries: [{"id", "tokens", "want", "rules", "generated"}] (the last three may be absent); `end`: requests whose state is given back after the step."""
+        out = [self.feed(e["id"], e["tokens"], e.get("want", ()), e.get("rules"), e.get("generated", False)) for e in entries]
         for r in end:
             self.release(r)
         return out

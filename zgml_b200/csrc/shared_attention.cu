@@ -729,6 +729,8 @@ __global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const __grid_co
         float o[OW];
 #pragma unroll
         for (int i = 0; i < OW; i++) o[i] = 0.0f;
+        // Probabilities are held times 2^14.  The outputs lose that factor as they join the running ones: what was kept with it would overflow 2^14 times too early.
+        constexpr float p_unit = 1.0f / 16384.0f;
         float m = -INFINITY, l = 0.0f, alpha_prev = 1.0f, f_prev = 0.0f;
         auto add_output = [&](uint32_t t) {                              // outputs of tile t join the running ones
             if (ok) ok = __all_sync(0xffffffffu, mbar_wait(o_full + 8 * (t & 1), (t >> 1) & 1));
@@ -794,7 +796,7 @@ __global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const __grid_co
             // (a barrier for even and one for odd tiles: warps may be a tile apart)
             if (lane == 0) mbar_arrive(p_full + 8 * (t & 1));
             if (t) add_output(t - 1);
-            alpha_prev = alpha; f_prev = inv.y;
+            alpha_prev = alpha; f_prev = inv.y * p_unit;
         }
         add_output(n_tiles - 1);
         {
@@ -803,11 +805,10 @@ __global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const __grid_co
             bar_sync(1 + (warp & 3), 128);
             l = (s[row] + s[128 + row]) + (s[256 + row] + s[384 + row]);
         }
-        constexpr float p_unit = 1.0f / 16384.0f;
         // Outputs leave by whole rows, through the idle stages.
         float4* const out = reinterpret_cast<float4*>(mem);
 #pragma unroll
-        for (int j = 0; j < OW; j += 4) out[row * (DV / 4) + (((OW * part + j) / 4) ^ (row & 7))] = make_float4(o[j] * p_unit, o[j + 1] * p_unit, o[j + 2] * p_unit, o[j + 3] * p_unit);
+        for (int j = 0; j < OW; j += 4) out[row * (DV / 4) + (((OW * part + j) / 4) ^ (row & 7))] = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
         const uint32_t mine = rows[row];
         if (slow || (mine != 0xffffffffu && m < -1e36f)) atomicOr(trouble, 1u);
         if (!ok) { atomicOr(trouble, 2u); if (lane == 0) count_timeout(); }

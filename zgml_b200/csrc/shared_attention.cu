@@ -664,12 +664,13 @@ __global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const __grid_co
                         }
                     }
                 if (slow) atomicOr(trouble, 1u);
+                if (!ok && lane == 0) atomicOr(trouble, 2u);             // before the pairs are handed over: whoever takes them reads it afterwards
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(full + 8 * fill);
                 if (++fill == kSpStages) { fill = 0; fill_phase ^= 1; }
             }
-            if (!ok && lane == 0) { count_timeout(); atomicOr(trouble, 2u); }
+            if (!ok && lane == 0) count_timeout();
         }
     } else if (n_tiles) {
         // ── softmax: four threads per query row ──

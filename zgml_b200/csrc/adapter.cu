@@ -349,7 +349,9 @@ __global__ void __launch_bounds__(256, 1) __cluster_dims__(kAfCluster, 1, 1) k_a
     AmRun* const all = reinterpret_cast<AmRun*>(mem + L::runs);
     const uint32_t done = base + L::bars, tmem_slot = done + 16;
     uint32_t* const count = reinterpret_cast<uint32_t*>(mem + L::bars + 24);
+    volatile uint32_t* const lost = count + 1;
     if (threadIdx.x == 0) {
+        *lost = 0;
         mbar_init(done, 1); mbar_init(done + 8, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -468,7 +470,9 @@ __global__ void __launch_bounds__(256, 1) __cluster_dims__(kAfCluster, 1, 1) k_a
         if (n && ok) ok = __all_sync(0xffffffffu, mbar_wait(done + 8 * ((uses - 1) & 1), ((uses - 1) >> 1) & 1));
         if (n > 1 && ok) ok = __all_sync(0xffffffffu, mbar_wait(done + 8 * (uses & 1), ((uses - 2) >> 1) & 1));
         fence_after();
+        if (!ok) *lost = 1;                                          // a warp whose wait ran out has written over operands that others read
         __syncthreads();
+        ok = !*lost;
         float* const sums = reinterpret_cast<float*>(mem);           // [128][width]
         const uint32_t row = (warp & 3) * 32 + lane, col = 32 * (warp >> 2);
 #pragma unroll 1
@@ -573,18 +577,20 @@ __global__ void __launch_bounds__(kAxThreads, 1) k_adapter_expand(AdArgs a, cons
         auto fill = [&]() {                                          // the next stage
             const int adapter = runs[f_run].which;
             if (ok) ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * slot, phase));
+            if (ok) {                                                // otherwise the stage may still be read
 #pragma unroll
-            for (uint32_t i = 0; i < 8; i++) {
-                const uint32_t row = (id >> 3) + 16 * i, o = (t0 + f_tile) * 128 + row, to = slot * L::stage + am_at(row, c);
-                const bool on = o < a.N && 8 * c < a.rank;           // the rank is a multiple of eight here
-                const WT* from = on ? wb + ((size_t)adapter * a.N + o) * a.rank + 8 * c : wb;
-                if constexpr (sizeof(WT) == 2) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(base + to), "l"(from), "r"(on ? 16 : 0) : "memory");
-                else {
-                    uint4 w[3];
-                    const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    am_split(on ? *reinterpret_cast<const float4*>(from) : zero, on ? *reinterpret_cast<const float4*>(from + 4) : zero, w);
+                for (uint32_t i = 0; i < 8; i++) {
+                    const uint32_t row = (id >> 3) + 16 * i, o = (t0 + f_tile) * 128 + row, to = slot * L::stage + am_at(row, c);
+                    const bool on = o < a.N && 8 * c < a.rank;       // the rank is a multiple of eight here
+                    const WT* from = on ? wb + ((size_t)adapter * a.N + o) * a.rank + 8 * c : wb;
+                    if constexpr (sizeof(WT) == 2) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(base + to), "l"(from), "r"(on ? 16 : 0) : "memory");
+                    else {
+                        uint4 w[3];
+                        const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        am_split(on ? *reinterpret_cast<const float4*>(from) : zero, on ? *reinterpret_cast<const float4*>(from + 4) : zero, w);
 #pragma unroll
-                    for (int y = 0; y < 3; y++) *reinterpret_cast<uint4*>(mem + to + y * kAmPart) = w[y];
+                        for (int y = 0; y < 3; y++) *reinterpret_cast<uint4*>(mem + to + y * kAmPart) = w[y];
+                    }
                 }
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
@@ -599,7 +605,7 @@ __global__ void __launch_bounds__(kAxThreads, 1) k_adapter_expand(AdArgs a, cons
             asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
             am_proxy_fence();
             __syncwarp();
-            if (lane == 0) mbar_arrive(full + 8 * at_slot);
+            if (lane == 0 && ok) mbar_arrive(full + 8 * at_slot);     // (otherwise the waits for this stage run out too, and its sums are never there)
             if (warp == 8) {
                 const uint32_t d = (item & 1) * 128, w0 = desc_low(base) + at_slot * (L::stage >> 4), freed = empty + 8 * at_slot, idesc = am_idesc(128);
                 if (ok) ok = __all_sync(0xffffffffu, mbar_wait(full + 8 * at_slot, at_phase));

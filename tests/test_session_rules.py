@@ -1,0 +1,92 @@
+"""A session's rules on logits without a device: a backend that keeps what it is given and computes LOGIT_RULES from its definition, under a model whose logits are a table."""
+import numpy as np
+import pytest
+
+import batch_reference as ref
+from zgml_b200 import DeviceProgram, abi
+from zgml_b200.host.batch import LogitRules
+from zgml_b200.host.session import LoweredProgram, SequenceSession
+
+V = 40
+LOGITS = np.random.default_rng(0).standard_normal((V, V)).astype(np.float32)      # after a token
+
+
+class Backend:
+    """Programs are dicts of buffers that stay from one execution to the next."""
+
+    def __init__(self):
+        self.compiled, self.freed, self.executed, self.refuse, self.uploaded = 0, 0, [], lambda program: False, []
+
+    def compile_program(self, program):
+        if self.refuse(program):
+            return None
+        self.compiled += 1
+        return {"program": program, "buffers": [np.zeros(max(1, int(n)), np.int32) for n in program.buffer_sizes]}
+
+    def free_program(self, handle):
+        self.freed += 1
+
+    def execute_program(self, handle, inputs, outputs):
+        buffers = handle["buffers"]
+        for io in inputs:
+            words = np.ascontiguousarray(io.host).view(np.int32).ravel()
+            assert io.offset % 4 == 0 and io.offset // 4 + words.size <= buffers[io.buf_idx].size
+            buffers[io.buf_idx][io.offset // 4:io.offset // 4 + words.size] = words
+            self.uploaded.append((io.buf_idx, words.size))
+        self.executed.append((buffers[0][abi.CTL_POS], buffers[0][abi.CTL_IDS:].tolist()))
+        for op in handle["program"].ops:
+            if op.tag == abi.OP_LOGIT_RULES:
+                b = op.u.seq.buf
+                t = buffers[b[2]][abi.BATCH_ROWS:abi.BATCH_ROWS + abi.RULE_WORDS]
+                row = (*t[:6].tolist(), *t[6:9].copy().view(np.float32).tolist())
+                bias = buffers[b[4]].reshape(-1, 2)
+                bias = list(zip(bias[:, 0].tolist(), bias[:, 1].copy().view(np.float32).tolist()))
+                z, _ = ref.rules(np.zeros((1, V)), buffers[b[1]].view(np.float32).reshape(1, V), [row], 1, buffers[b[3]].reshape(1, -1)[:, :op.u.seq.n[4]], bias, buffers[b[5]].reshape(1, -1))
+                buffers[b[0]][:] = z.astype(np.float32).view(np.int32).ravel()
+            else:
+                buffers[1][:] = LOGITS[buffers[0][abi.CTL_IDS:][-1]].view(np.int32)
+        for io in outputs:
+            io.host[...] = buffers[io.buf_idx].view(np.float32).reshape(io.host.shape)
+
+
+class Model:
+    vocab = V
+
+    def state_specs(self, max_chunk, max_context):
+        return []
+
+    def lower(self, T, head, pool, keep_layers=False):
+        ops = [] if head == "none" else [abi.ZgOp()]
+        return LoweredProgram(DeviceProgram(ops, [abi.CTL_IDS + T, V]), 0, None if head == "none" else 1, 1)
+
+
+def session(max_chunk=4, **kw):
+    be = Backend()
+    return SequenceSession(be, Model(), n_slots=2, max_chunk=max_chunk, **kw), be
+
+
+def want(fed, prompt, rules):
+    """The rules' result after the tokens `fed`, of which `prompt` were not generated."""
+    masks = None if rules.allowed is None else rules.mask(V)[None]
+    line = (0, len(fed), prompt, -1 if masks is None else 0, 0, len(rules.bias), rules.repetition, rules.presence, rules.frequency)
+    z, _ = ref.rules(np.zeros((1, V)), LOGITS[fed[-1]][None], [line], 1, np.array([fed]), list(rules.bias.items()), masks)
+    return z.astype(np.float32)
+
+
+RULES = LogitRules(1.5, 0.25, 0.5, {3: 1.0})
+
+
+def test_rules_over_a_request():
+    s, _ = session()
+    fed = [1, 2, 3, 4, 5, 6, 7]
+    assert np.array_equal(s.feed("a", fed, [6], RULES), want(fed, 7, RULES))
+    for t in (9, 9, 3):
+        fed.append(t)
+        assert np.array_equal(s.feed("a", [t], [0], RULES, generated=True), want(fed, 7, RULES))
+    fed += [11, 12]                                     # another turn of the user's
+    assert np.array_equal(s.feed("a", [11, 12], [1], RULES), want(fed, len(fed), RULES))
+
+
+def test_a_request_that_begins_with_generated_tokens():
+    s, _ = session()
+    assert np.array_equal(s.feed("a", [5, 6, 5], [2], RULES, generated=True), want([5, 6, 5], 0, RULES))

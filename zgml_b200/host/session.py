@@ -107,7 +107,7 @@ class SequenceSession:
         ins = [ProgramIO(lp.buf_ctl, ctl)]
         if rules is not None:
             past = np.asarray(self._history[request_id], np.int32)
-            table, bias, masks = rule_table([rules], [0], [past.size], [self._prompt[request_id]], self.model.vocab, 1)
+            table, bias, masks = rule_table([rules], [0], [past.size], [self._prompt.get(request_id, 0)], self.model.vocab, 1)
             ins += [ProgramIO(b, a) for b, a in zip(lp.rule_bufs, (table, past, bias.ravel(), masks.ravel())) if a.size]
         self.be.execute_program(handle, ins, outs)
         self.executions += 1

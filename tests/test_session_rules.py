@@ -90,3 +90,37 @@ def test_rules_over_a_request():
 def test_a_request_that_begins_with_generated_tokens():
     s, _ = session()
     assert np.array_equal(s.feed("a", [5, 6, 5], [2], RULES, generated=True), want([5, 6, 5], 0, RULES))
+
+
+@pytest.mark.parametrize("ruled_only", [True, False])
+def test_a_step_that_cannot_be_compiled_leaves_nothing(ruled_only):
+    """The request stays where it was, and the same tokens again count once."""
+    s, be = session()
+    s.feed("a", [1, 2, 2], [2])
+    is_ruled = lambda program: any(op.tag == abi.OP_LOGIT_RULES for op in program.ops)
+    be.refuse = is_ruled if ruled_only else lambda program: True
+    for new in ([2, 7, 7, 7, 8, 7], [9]):
+        with pytest.raises(RuntimeError):
+            s.feed("a", new, [len(new) - 1], RULES)
+        assert s.pool.position("a") == 3 and len(be.executed) == 2
+    be.refuse = lambda program: False
+    assert np.array_equal(s.feed("a", [2, 7], [1], RULES, generated=True), want([1, 2, 2, 2, 7], 3, RULES))
+
+
+def test_a_step_that_fails_on_its_way():
+    """What had run counts, what had not does not."""
+    s, be = session()
+    s.feed("a", [1], [0], RULES)
+    run, left = be.execute_program, [1]
+
+    def fails(*args):
+        if not left:
+            raise RuntimeError("no")
+        left.pop()
+        run(*args)
+    be.execute_program = fails
+    with pytest.raises(RuntimeError):
+        s.feed("a", [2, 3, 4, 5, 6, 7], [5], RULES, generated=True)
+    be.execute_program = run
+    assert s.pool.position("a") == 5
+    assert np.array_equal(s.feed("a", [6, 7], [1], RULES, generated=True), want([1, 2, 3, 4, 5, 6, 7], 1, RULES))

@@ -58,13 +58,31 @@ def cut(n: int, menu: Sequence[int]) -> List[int]:
     return out
 
 
+class History:
+    """The tokens fed for a request, int32 words that grow in place: `n` of them count, those from `prompt` on as generated."""
+
+    def __init__(self):
+        self.words, self.n, self.prompt = np.zeros(64, np.int32), 0, 0
+
+    def put(self, tokens: Sequence[int]):
+        """Writes the tokens of a step behind those that count; they do once `advance` is told."""
+        need = self.n + len(tokens)
+        if need > self.words.size:
+            self.words = np.concatenate([self.words[:self.n], np.zeros(max(need, 2 * self.words.size) - self.n, np.int32)])
+        self.words[self.n:need] = tokens
+
+    def advance(self, T: int, generated: bool):
+        self.n += T
+        if not generated:
+            self.prompt = self.n
+
+
 class SequenceSession:
     def __init__(self, be: CudaBackend, model, n_slots: int = 1, max_chunk: int = 256, keep_layers: bool = False,
                  max_context: Optional[int] = None, max_history: int = 32768, max_bias: int = 1024):
         """`max_history` tokens of a request, `max_bias` biases: what steps with rules have room for."""
         self.max_history, self.max_bias = max_history, max_bias
-        self._history: Dict[object, List[int]] = {}
-        self._prompt: Dict[object, int] = {}
+        self._history: Dict[object, History] = {}
         self.be, self.model, self.keep_layers = be, model, keep_layers
         self.menu = chunk_menu(max_chunk)
         self.max_chunk = self.menu[0]
@@ -99,15 +117,15 @@ class SequenceSession:
             self._programs[key] = (lp, handle, ctl, logits)
         return self._programs[key]
 
-    def _run(self, T, head, slot, pos, prev, tokens, request_id=None, rules: Optional[LogitRules] = None):
+    def _run(self, T, head, slot, pos, prev, tokens, past: Optional[np.ndarray] = None, generated_from: int = 0, rules: Optional[LogitRules] = None):
+        """`past`: the request's tokens, this step's among them (with rules)."""
         lp, handle, ctl, logits = self.program(T, head, rules is not None)
         ctl[abi.CTL_POS], ctl[abi.CTL_SLOT], ctl[abi.CTL_PREV] = pos, slot, prev
         ctl[abi.CTL_IDS:] = tokens
         outs = [ProgramIO(lp.buf_logits, logits)] if logits is not None else []
         ins = [ProgramIO(lp.buf_ctl, ctl)]
         if rules is not None:
-            past = np.asarray(self._history[request_id], np.int32)
-            table, bias, masks = rule_table([rules], [0], [past.size], [self._prompt.get(request_id, 0)], self.model.vocab, 1)
+            table, bias, masks = rule_table([rules], [0], [past.size], [generated_from], self.model.vocab, 1)
             ins += [ProgramIO(b, a) for b, a in zip(lp.rule_bufs, (table, past, bias.ravel(), masks.ravel())) if a.size]
         self.be.execute_program(handle, ins, outs)
         self.executions += 1
@@ -123,36 +141,40 @@ class SequenceSession:
         want = [int(w) for w in want]
         if any(w < 0 or w >= len(tokens) for w in want):
             raise ValueError("wanted place outside the step's tokens")
-        past = self._history.get(request_id, [])
+        past = self._history.get(request_id) or History()
         if rules is not None:
             if any(w != len(tokens) - 1 for w in want):
                 raise ValueError("rules apply to the logits of a step's last place")
-            if len(past) + len(tokens) > self.max_history or len(rules.bias) > self.max_bias:
-                raise ValueError(f"rules over {len(past) + len(tokens)} tokens with {len(rules.bias)} biases: the session has room for {self.max_history} and {self.max_bias}")
+            if past.n + len(tokens) > self.max_history or len(rules.bias) > self.max_bias:
+                raise ValueError(f"rules over {past.n + len(tokens)} tokens with {len(rules.bias)} biases: the session has room for {self.max_history} and {self.max_bias}")
             rule_table([rules], [0], [0], [0], self.model.vocab, 1)      # its tokens are in the vocabulary
         slot = self.pool.acquire(request_id)
         if self.context_limit is not None and self.pool.position(request_id) + len(tokens) > self.context_limit:
             raise ValueError(f"request {request_id!r} would reach position {self.pool.position(request_id) + len(tokens)}: the session's caches hold "
                              f"{self.context_limit} positions per sequence")
-        self._history.setdefault(request_id, []).extend(tokens)
-        if not generated:
-            self._prompt[request_id] = len(self._history[request_id])
-        rows: Dict[int, np.ndarray] = {}
-        at = 0
+        self._history[request_id] = past
+        plan, at = [], 0
         for T in cut(len(tokens), self.menu):
             local = sorted({w - at for w in want if at <= w < at + T})
             head = "none" if not local else ("last" if local == [T - 1] else "all")
-            logits = self._run(T, head, slot, self.pool.position(request_id), self.pool.last_token(request_id), tokens[at:at + T], request_id, rules if local else None)
+            self.program(T, head, rules is not None and bool(local))     # what cannot be compiled is known before anything runs
+            plan.append((at, T, head, local))
+            at += T
+        rows: Dict[int, np.ndarray] = {}
+        for at, T, head, local in plan:
+            step = tokens[at:at + T]
+            past.put(step)
+            ruled = (past.words[:past.n + T], past.prompt if generated else past.n + T, rules) if rules is not None and local else ()
+            logits = self._run(T, head, slot, self.pool.position(request_id), self.pool.last_token(request_id), step, *ruled)
             for w in local:
                 rows[at + w] = logits[0 if head == "last" else w].copy()
-            self.pool.advance(request_id, T, tokens[at + T - 1])
-            at += T
+            self.pool.advance(request_id, T, step[-1])
+            past.advance(T, generated)
         return np.stack([rows[w] for w in want]) if want else np.zeros((0, self.model.vocab), np.float32)
 
     def release(self, request_id):
         self.pool.release(request_id)
         self._history.pop(request_id, None)
-        self._prompt.pop(request_id, None)
 
     def step(self, entries: Sequence[dict], end: Iterable = ()) -> List[np.ndarray]:
         """entries: [{"id", "tokens", "want", "rules", "generated"}] (the last three may be absent); `end`: requests whose state is given back after the step."""

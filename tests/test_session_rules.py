@@ -124,3 +124,57 @@ def test_a_step_that_fails_on_its_way():
     be.execute_program = run
     assert s.pool.position("a") == 5
     assert np.array_equal(s.feed("a", [6, 7], [1], RULES, generated=True), want([1, 2, 3, 4, 5, 6, 7], 1, RULES))
+
+
+def test_a_history_longer_than_the_first_room():
+    """Without a limit of the user's the room grows: programs with rules are made again."""
+    s, be = session(max_chunk=32768)
+    past = (np.arange(40000) % V).tolist()
+    assert np.array_equal(s.feed("a", past, [39999], RULES), want(past, 40000, RULES))
+    assert np.array_equal(s.feed("b", [1, 2], [1], RULES), want([1, 2], 2, RULES))
+    compiled = be.compiled
+    assert np.array_equal(s.feed("a", [7], [0], RULES, generated=True), want(past + [7], 40000, RULES))
+    assert be.compiled <= compiled + 1                   # (the step of one token)
+    s.close()
+    assert be.freed == be.compiled
+
+
+def test_generate_past_the_first_room():
+    """The room is there before the first token: nothing is made again between two tokens."""
+    s, be = session(max_chunk=32768)
+    prompt = (np.arange(32766) % V).tolist()
+    one = LogitRules(presence=100.0, repetition=1.0)
+    out = s.generate(prompt, 12, rules=one)
+    assert len(set(out)) == 12 and be.freed == 0
+    fed = prompt + out[:-1]
+    assert out[-1] == int(np.argmax(want(fed, len(prompt), one)))
+
+
+def test_generate_refuses_at_the_start():
+    s, be = session(max_history=10)
+    with pytest.raises(ValueError):
+        s.generate([1, 2, 3], 9, rules=LogitRules(presence=1.0))
+    assert be.executed == [] and not s.pool.has("generate")
+    assert len(s.generate([1, 2, 3], 8, rules=LogitRules(presence=1.0))) == 8
+    assert s.generate([1, 2, 3], 0, rules=LogitRules(presence=1.0)) == []
+
+
+@pytest.mark.parametrize("rules", [LogitRules(bias={3: 9.0}), LogitRules(allowed=np.array([5, 6]))])
+def test_rules_that_read_no_history_have_no_limit(rules):
+    s, be = session(max_history=4)
+    fed = [1, 2, 3, 4, 5, 6]
+    be.uploaded.clear()
+    assert np.array_equal(s.feed("a", fed, [5], rules), want(fed, 6, rules))
+    assert s.generate(fed, 20, rules=rules) and all(b != 3 for b, _ in be.uploaded)      # (the history's buffer)
+    with pytest.raises(ValueError):
+        s.feed("a", [1], [0], LogitRules(frequency=0.5))
+    assert s.pool.position("a") == 6
+
+
+def test_generate_until_a_stop():
+    """A number of tokens that is never reached asks for no memory."""
+    s, be = session()
+    rules = LogitRules(presence=100.0)
+    few = s.generate([1, 2], 6, rules=rules)
+    assert s.generate([1, 2], 10 ** 12, stop=few[-1], rules=rules) == few
+    assert s._room <= 1 << 19

@@ -67,6 +67,12 @@ class LogitRules:
         if np.isnan(biases).any():
             raise ValueError("a bias is not a number")
 
+    @property
+    def reads_history(self) -> bool:
+        """Whether any history can change a logit, with these numbers as the kernel's f32."""
+        with np.errstate(over="ignore", under="ignore"):
+            return bool(np.float32(self.repetition) != 1.0 or np.float32(self.presence) != 0.0 or np.float32(self.frequency) != 0.0)
+
     def mask(self, vocab: int) -> Optional[np.ndarray]:
         """int32 words, bit t % 32 of word t / 32 set where token t is allowed."""
         if self.allowed is None:

@@ -79,9 +79,11 @@ class History:
 
 class SequenceSession:
     def __init__(self, be: CudaBackend, model, n_slots: int = 1, max_chunk: int = 256, keep_layers: bool = False,
-                 max_context: Optional[int] = None, max_history: int = 32768, max_bias: int = 1024):
-        """`max_history` tokens of a request, `max_bias` biases: what steps with rules have room for."""
+                 max_context: Optional[int] = None, max_history: Optional[int] = None, max_bias: int = 1024):
+        """`max_history` tokens of a request, `max_bias` biases: the most that steps with rules take.  Without a `max_history` the programs with rules have room for
+        32768 tokens and are compiled again, for twice as many or more, when a request has more of them."""
         self.max_history, self.max_bias = max_history, max_bias
+        self._room = 32768 if max_history is None else max(1, max_history)      # words of a history in the programs with rules
         self._history: Dict[object, History] = {}
         self.be, self.model, self.keep_layers = be, model, keep_layers
         self.menu = chunk_menu(max_chunk)
@@ -97,10 +99,21 @@ class SequenceSession:
         V, p = self.model.vocab, lp.program
         n = p.n_buffers
         table, history, bias, mask, out = range(n, n + 5)
-        sizes = list(p.buffer_sizes) + [rule_words(1), self.max_history, 2 * self.max_bias, (V + 31) // 32, V]
-        op = DeviceOp.logit_rules(out, lp.buf_logits, table, 1, V, history=history, history_rows=self.max_history, bias=bias, masks=mask)
+        sizes = list(p.buffer_sizes) + [rule_words(1), self._room, 2 * self.max_bias, (V + 31) // 32, V]
+        op = DeviceOp.logit_rules(out, lp.buf_logits, table, 1, V, history=history, history_rows=self._room, bias=bias, masks=mask)
         return LoweredProgram(DeviceProgram(list(p.ops) + [op], sizes, p.initial_uploads, p.qweights, p.externs), lp.buf_ctl, out, lp.logits_rows, lp.layer_bufs,
                               (table, history, bias, mask))
+
+    def _check_history(self, rules: LogitRules, tokens: int):
+        if self.max_history is not None and rules.reads_history and tokens > self.max_history:
+            raise ValueError(f"rules over {tokens} tokens: the session takes {self.max_history}")
+
+    def _make_room(self, rules: LogitRules, tokens: int):
+        if not rules.reads_history or tokens <= self._room:
+            return
+        self._room = max(tokens, 2 * self._room)
+        for key in [k for k in self._programs if len(k) == 3]:
+            self.be.free_program(self._programs.pop(key)[1])
 
     def program(self, T: int, head: str, ruled: bool = False):
         key = (T, head, True) if ruled else (T, head)
@@ -118,13 +131,15 @@ class SequenceSession:
         return self._programs[key]
 
     def _run(self, T, head, slot, pos, prev, tokens, past: Optional[np.ndarray] = None, generated_from: int = 0, rules: Optional[LogitRules] = None):
-        """`past`: the request's tokens, this step's among them (with rules)."""
+        """With rules: `past` is the request's tokens, this step's among them."""
         lp, handle, ctl, logits = self.program(T, head, rules is not None)
         ctl[abi.CTL_POS], ctl[abi.CTL_SLOT], ctl[abi.CTL_PREV] = pos, slot, prev
         ctl[abi.CTL_IDS:] = tokens
         outs = [ProgramIO(lp.buf_logits, logits)] if logits is not None else []
         ins = [ProgramIO(lp.buf_ctl, ctl)]
         if rules is not None:
+            if not rules.reads_history:
+                past, generated_from = past[:0], 0
             table, bias, masks = rule_table([rules], [0], [past.size], [generated_from], self.model.vocab, 1)
             ins += [ProgramIO(b, a) for b, a in zip(lp.rule_bufs, (table, past, bias.ravel(), masks.ravel())) if a.size]
         self.be.execute_program(handle, ins, outs)
@@ -145,14 +160,17 @@ class SequenceSession:
         if rules is not None:
             if any(w != len(tokens) - 1 for w in want):
                 raise ValueError("rules apply to the logits of a step's last place")
-            if past.n + len(tokens) > self.max_history or len(rules.bias) > self.max_bias:
-                raise ValueError(f"rules over {past.n + len(tokens)} tokens with {len(rules.bias)} biases: the session has room for {self.max_history} and {self.max_bias}")
+            self._check_history(rules, past.n + len(tokens))
+            if len(rules.bias) > self.max_bias:
+                raise ValueError(f"{len(rules.bias)} biases: the session takes {self.max_bias}")
             rule_table([rules], [0], [0], [0], self.model.vocab, 1)      # its tokens are in the vocabulary
         slot = self.pool.acquire(request_id)
         if self.context_limit is not None and self.pool.position(request_id) + len(tokens) > self.context_limit:
             raise ValueError(f"request {request_id!r} would reach position {self.pool.position(request_id) + len(tokens)}: the session's caches hold "
                              f"{self.context_limit} positions per sequence")
         self._history[request_id] = past
+        if rules is not None:
+            self._make_room(rules, past.n + len(tokens))
         plan, at = [], 0
         for T in cut(len(tokens), self.menu):
             local = sorted({w - at for w in want if at <= w < at + T})
@@ -197,6 +215,11 @@ class SequenceSession:
                  stop: Optional[int] = None, rules: Optional[LogitRules] = None) -> List[int]:
         """Prefill `prompt`, then decode token by token through the same step function; with `rules` the sampler sees logits that have passed them."""
         sampler = sampler or Sampler()
+        if rules is not None:                            # what it will look back at has room, or is refused, before the first token
+            past = self._history.get(request_id) or History()
+            tokens = past.n + len(prompt) + max(0, max_new_tokens - 1)
+            self._check_history(rules, tokens)
+            self._make_room(rules, min(tokens, past.n + len(prompt) + (1 << 18)))      # (the most that it makes for tokens that may never come)
         logits = self.feed(request_id, prompt, [len(prompt) - 1], rules)[0]
         out: List[int] = []
         try:

@@ -178,3 +178,51 @@ def test_generate_until_a_stop():
     few = s.generate([1, 2], 6, rules=rules)
     assert s.generate([1, 2], 10 ** 12, stop=few[-1], rules=rules) == few
     assert s._room <= 1 << 19
+
+
+def test_a_history_goes_to_a_program_once():
+    """Between two tokens of one request only what is new is uploaded; another request's tokens take its place."""
+    s, be = session()
+    fed = {"a": [1, 2, 3, 4, 5], "b": [6, 7]}
+    for k, t in fed.items():
+        s.feed(k, t, [len(t) - 1], RULES)
+    words = []
+    for step, k in enumerate(["a", "a", "a", "b", "a", "b", "b"]):
+        fed[k].append(10 + step)
+        be.uploaded.clear()
+        prompt = 5 if k == "a" else 2
+        assert np.array_equal(s.feed(k, fed[k][-1:], [0], RULES, generated=True), want(fed[k], prompt, RULES))
+        words.append(sum(n for b, n in be.uploaded if b == 3))
+    assert words == [1, 1, 1, 3, 9, 4, 1]                # (the first steps of one token found the last chunk of the prompt's program, which is theirs too)
+
+
+def test_rules_that_change_between_tokens():
+    """What a request asks is read anew in each step."""
+    s, _ = session()
+    rules = LogitRules(1.25, bias={1: 1.0})
+    fed = [3, 4]
+    s.feed("a", fed, [1], rules)
+    for t in (5, 6):
+        rules.bias = {t: 2.0}
+        rules.presence = 0.5
+        fed.append(t)
+        assert np.array_equal(s.feed("a", [t], [0], rules, generated=True), want(fed, 2, rules))
+
+
+def test_an_execution_that_fails_behind_its_uploads():
+    """What it left in the history's buffer belongs to nobody."""
+    s, be = session()
+    s.feed("a", [1, 2, 3, 4, 5], [4], RULES)
+    run = be.execute_program
+
+    def fails(*args):
+        run(*args)
+        raise RuntimeError("no")
+    be.execute_program = fails
+    with pytest.raises(RuntimeError):
+        s.feed("b", [9], [0], RULES)
+    be.execute_program = run
+    assert np.array_equal(s.feed("a", [6], [0], RULES, generated=True), want([1, 2, 3, 4, 5, 6], 5, RULES))
+    assert np.array_equal(s.feed("b", [8], [0], RULES, generated=True), want([8], 0, RULES))
+    s.release("a")
+    assert np.array_equal(s.feed("a", [7], [0], RULES), want([7], 1, RULES))

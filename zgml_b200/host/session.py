@@ -85,6 +85,7 @@ class SequenceSession:
         self.max_history, self.max_bias = max_history, max_bias
         self._room = 32768 if max_history is None else max(1, max_history)      # words of a history in the programs with rules
         self._history: Dict[object, History] = {}
+        self._uploaded: Dict[tuple, Tuple[History, int]] = {}      # program with rules -> whose tokens its history buffer begins with, and how many
         self.be, self.model, self.keep_layers = be, model, keep_layers
         self.menu = chunk_menu(max_chunk)
         self.max_chunk = self.menu[0]
@@ -114,6 +115,7 @@ class SequenceSession:
         self._room = max(tokens, 2 * self._room)
         for key in [k for k in self._programs if len(k) == 3]:
             self.be.free_program(self._programs.pop(key)[1])
+        self._uploaded = {}
 
     def program(self, T: int, head: str, ruled: bool = False):
         key = (T, head, True) if ruled else (T, head)
@@ -130,19 +132,25 @@ class SequenceSession:
             self._programs[key] = (lp, handle, ctl, logits)
         return self._programs[key]
 
-    def _run(self, T, head, slot, pos, prev, tokens, past: Optional[np.ndarray] = None, generated_from: int = 0, rules: Optional[LogitRules] = None):
-        """With rules: `past` is the request's tokens, this step's among them."""
-        lp, handle, ctl, logits = self.program(T, head, rules is not None)
+    def _run(self, T, head, slot, pos, prev, tokens, past: Optional[History] = None, rule_words=None):
+        """With rules: the request's history, this step's tokens behind those that count, and the words of rule_table."""
+        lp, handle, ctl, logits = self.program(T, head, rule_words is not None)
         ctl[abi.CTL_POS], ctl[abi.CTL_SLOT], ctl[abi.CTL_PREV] = pos, slot, prev
         ctl[abi.CTL_IDS:] = tokens
         outs = [ProgramIO(lp.buf_logits, logits)] if logits is not None else []
         ins = [ProgramIO(lp.buf_ctl, ctl)]
-        if rules is not None:
-            if not rules.reads_history:
-                past, generated_from = past[:0], 0
-            table, bias, masks = rule_table([rules], [0], [past.size], [generated_from], self.model.vocab, 1)
-            ins += [ProgramIO(b, a) for b, a in zip(lp.rule_bufs, (table, past, bias.ravel(), masks.ravel())) if a.size]
+        if rule_words is not None:
+            table, bias, masks = rule_words
+            at, history, biases, mask = lp.rule_bufs
+            ins += [ProgramIO(b, a) for b, a in ((at, table), (biases, bias.ravel()), (mask, masks.ravel())) if a.size]
+            n = int(table[abi.BATCH_ROWS + 1])                      # tokens that the rules read
+            if n:                                                   # a history only grows: what the buffer holds of it stays
+                owner, there = self._uploaded.pop((T, head), (None, 0))      # (back when this execution is through)
+                there = there if owner is past else 0
+                ins.append(ProgramIO(history, past.words[there:n], 4 * there))
         self.be.execute_program(handle, ins, outs)
+        if rule_words is not None and n:
+            self._uploaded[(T, head)] = (past, n)
         self.executions += 1
         return logits
 
@@ -163,7 +171,8 @@ class SequenceSession:
             self._check_history(rules, past.n + len(tokens))
             if len(rules.bias) > self.max_bias:
                 raise ValueError(f"{len(rules.bias)} biases: the session takes {self.max_bias}")
-            rule_table([rules], [0], [0], [0], self.model.vocab, 1)      # its tokens are in the vocabulary
+            n = past.n + len(tokens) if rules.reads_history else 0
+            words = rule_table([rules], [0], [n], [past.prompt if generated and n else n], self.model.vocab, 1)
         slot = self.pool.acquire(request_id)
         if self.context_limit is not None and self.pool.position(request_id) + len(tokens) > self.context_limit:
             raise ValueError(f"request {request_id!r} would reach position {self.pool.position(request_id) + len(tokens)}: the session's caches hold "
@@ -182,8 +191,7 @@ class SequenceSession:
         for at, T, head, local in plan:
             step = tokens[at:at + T]
             past.put(step)
-            ruled = (past.words[:past.n + T], past.prompt if generated else past.n + T, rules) if rules is not None and local else ()
-            logits = self._run(T, head, slot, self.pool.position(request_id), self.pool.last_token(request_id), step, *ruled)
+            logits = self._run(T, head, slot, self.pool.position(request_id), self.pool.last_token(request_id), step, *((past, words) if rules is not None and local else ()))
             for w in local:
                 rows[at + w] = logits[0 if head == "last" else w].copy()
             self.pool.advance(request_id, T, step[-1])

@@ -226,3 +226,15 @@ def test_an_execution_that_fails_behind_its_uploads():
     assert np.array_equal(s.feed("b", [8], [0], RULES, generated=True), want([8], 0, RULES))
     s.release("a")
     assert np.array_equal(s.feed("a", [7], [0], RULES), want([7], 1, RULES))
+
+
+@pytest.mark.parametrize("make", [lambda: LogitRules(bias={1.5: 2.0}), lambda: LogitRules(bias={"3": 2.0}), lambda: LogitRules(allowed=np.array([1.0, 2.5])).mask(V), lambda: LogitRules(allowed=["1"]).mask(V)])
+def test_token_ids_are_whole_numbers(make):
+    """2.5 is no token, and not token 2 either."""
+    with pytest.raises(ValueError):
+        make()
+
+
+def test_token_ids_of_any_integer_type():
+    r = LogitRules(bias={np.int64(3): 2.0, np.uint8(4): 1.0}, allowed=np.array([3, 4], np.uint16))
+    assert r.mask(V).tolist() == [24, 0] and LogitRules(allowed=[]).mask(V).tolist() == [0, 0] and LogitRules(allowed=[True] * V).mask(V).tolist() == [-1, 255]

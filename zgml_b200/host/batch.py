@@ -66,6 +66,11 @@ class LogitRules:
             raise ValueError("presence and frequency are finite")
         if np.isnan(biases).any():
             raise ValueError("a bias is not a number")
+        self._check_ids()
+
+    def _check_ids(self):
+        if not all(isinstance(k, (int, np.integer)) for k in self.bias):
+            raise ValueError("a bias names its token by a whole number")
 
     @property
     def reads_history(self) -> bool:
@@ -83,6 +88,8 @@ class LogitRules:
                 raise ValueError(f"truth values for {a.shape} tokens over a vocabulary of {vocab}")
             bits = a
         else:
+            if a.size and a.dtype.kind not in "iu":
+                raise ValueError("allowed tokens are whole numbers, or truth values over the vocabulary")
             ids = a.astype(np.int64).ravel()
             if ids.size and (ids.min() < 0 or ids.max() >= vocab):
                 raise ValueError("an allowed token is outside the vocabulary")
@@ -105,6 +112,7 @@ def rule_table(rules: Sequence[LogitRules], slots: Sequence[int], lengths: Seque
     for i, r in enumerate(rules):
         if lengths[i] < 0 or firsts[i] < 0:
             raise ValueError(f"row {i}: a history of {lengths[i]} words generated from word {firsts[i]} on")
+        r._check_ids()
         if any(not 0 <= k < vocab for k in r.bias):
             raise ValueError("a bias names a token outside the vocabulary")
         m = r.mask(vocab)

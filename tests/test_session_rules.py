@@ -238,3 +238,10 @@ def test_token_ids_are_whole_numbers(make):
 def test_token_ids_of_any_integer_type():
     r = LogitRules(bias={np.int64(3): 2.0, np.uint8(4): 1.0}, allowed=np.array([3, 4], np.uint16))
     assert r.mask(V).tolist() == [24, 0] and LogitRules(allowed=[]).mask(V).tolist() == [0, 0] and LogitRules(allowed=[True] * V).mask(V).tolist() == [-1, 255]
+
+
+def test_generate_stops_where_no_token_is_left():
+    s, be = session()
+    with pytest.raises(ValueError):
+        s.generate([1, 2], 4, rules=LogitRules(allowed=np.array([], np.int64)))
+    assert not s.pool.has("generate") and (s.feed("a", [1], [0], LogitRules(allowed=[])) == -np.inf).all()      # (a row of logits says it by itself)

@@ -232,6 +232,8 @@ class SequenceSession:
         out: List[int] = []
         try:
             for _ in range(max_new_tokens):
+                if rules is not None and logits.max() == -np.inf:
+                    raise ValueError(f"the rules leave no token to choose after {len(out)} of them")
                 tok = sampler(logits)
                 out.append(tok)
                 if stop is not None and tok == stop:

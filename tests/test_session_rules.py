@@ -245,3 +245,14 @@ def test_generate_stops_where_no_token_is_left():
     with pytest.raises(ValueError):
         s.generate([1, 2], 4, rules=LogitRules(allowed=np.array([], np.int64)))
     assert not s.pool.has("generate") and (s.feed("a", [1], [0], LogitRules(allowed=[])) == -np.inf).all()      # (a row of logits says it by itself)
+
+
+@pytest.mark.parametrize("option", [["--repetition-penalty", "0"], ["--presence-penalty", "inf"], ["--bias", "3:nan"], ["--bias", "3"], ["--allow", "x"]])
+def test_the_command_line_refuses_before_it_loads_a_model(monkeypatch, option):
+    from zgml_b200 import cli
+
+    def no_device():
+        raise AssertionError("a model would be loaded")
+    monkeypatch.setattr(cli, "_backend", no_device)
+    with pytest.raises(ValueError):
+        cli.main(["generate", "--model", "none", "--prompt", "1,2", "--max-new-tokens", "1", *option])

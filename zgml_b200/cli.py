@@ -36,10 +36,9 @@ def _rules(a):
 def cmd_generate(a) -> int:
     from .host.registry import open_session
     from .host.sampling import Sampler
+    prompt, rules = [int(t) for t in a.prompt.split(",") if t.strip()], _rules(a)      # (what cannot be is refused before a model is loaded)
     be = _backend()
-    prompt = [int(t) for t in a.prompt.split(",") if t.strip()]
     s = open_session(be, a.model, a.dtype, max_chunk=a.max_chunk, max_tokens=len(prompt) + a.max_new_tokens)
-    rules = _rules(a)
     if rules is not None and not hasattr(s, "max_history"):
         raise SystemExit("penalties, biases and masks need a sequence model (a folder with config.json)")
     sampler = Sampler(a.temperature, a.top_k, a.top_p, a.seed)

@@ -133,3 +133,27 @@ def test_loud_scores(cuda_backend, d, bits, cap):
     plain = 2 ** bits // d >= 2 ** 14
     off = (4.0 * 1.01 if cap else 0.0 if plain else 1.0) * 2.0 ** (bits - 3 - 24)
     assert (np.abs(got - want) <= (2 * off + (64 + 32) * 2.0 ** -24 + 4 * 2.0 ** -22) * (mean + np.abs(pre[:, :P, 1]).max() * 2.0 ** -14)).all()
+
+
+@pytest.mark.parametrize("H,dk,dv", [(16, 160, 160), (16, 160, 300), (16, 128, 128)])
+def test_sums_over_many_tiles_do_not_drift(cuda_backend, H, dk, dv):
+    """Sums on the tensor cores are cut at 24 bits, always towards zero.  Positive values over some twenty tiles a CTA: eight products of full size make a tile's sum, each cut by less
+    than 2^-23 of it (the others' sums are 2^-11 as large, and come first); tiles, shares and the sum of weights are rounded, which has no direction.  So the mean error over all
+    results is below 8 * 2^-23 of them, however many tiles there are, and 2^-23 for what roundings leave of a mean."""
+    from zgml_b200 import DeviceOp
+    r = np.random.default_rng(3)
+    B, G, P = 128, 2, 20000
+    q = r.standard_normal((B, H, dk)).astype(np.float32)
+    k, v = r.standard_normal((P, G, dk)).astype(np.float32), r.uniform(1.0, 2.0, (P, G, dv)).astype(np.float32)
+    pre = np.concatenate([k.reshape(P, -1), v.reshape(P, -1)], 1)
+    w, scale = pre.shape[1], 0.3 * dk ** -0.5
+    op = DeviceOp.shared_attention(0, 1, 2, 2, 3, 3, 4, 0, 0, G * dk, 0, G * dk, B, H, G, dk, dv, H * dk, w, w, 1, w, w, P, scale)
+    p = Prog(cuda_backend, lambda at: [op], dict(dst=np.zeros((B, H * dv), np.float32), q=q, own=np.zeros((1, 1, w), np.float32), pre=pre, table=table([(0, 0, 0)] * B, B, P)))
+    got = p.run(["dst"]).reshape(B, H, dv)
+    p.close()
+    for g in range(G):
+        z = q[:, g * (H // G):(g + 1) * (H // G)].reshape(-1, dk).astype(np.float64)
+        s = np.exp(scale * (z @ k[:, g].astype(np.float64).T))
+        want = s @ v[:, g].astype(np.float64) / s.sum(1, keepdims=True)
+        off = got[:, g * (H // G):(g + 1) * (H // G)].reshape(-1, dv) / want - 1.0
+        assert abs(off.mean()) <= 9 * 2.0 ** -23 and np.abs(off).max() <= 2.0 ** -16, (off.mean(), np.abs(off).max())

@@ -839,13 +839,18 @@ __global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const __grid_co
 // queries, keys and values as half-precision pairs in the workspace (a scale per row; values inside the key rows of a latent are the same pairs), and CTA (key head, share
 // of the prefix, up to 256 output columns, tile of 128 query rows) multiplies tiles of 128 keys from there, 64 dims at a time, through three stages that TMA fills:
 //   scores[128 rows x 128 keys] += queries[64 dims] keys[64 dims]^T, three MMAs a product;  outputs[128 x 64 columns] += probabilities[128 keys] values[128 keys x 64 columns].
-// Values come as the keys do, by rows, and are read as a transposed operand.  TMEM: scores of two tiles (which become the probabilities in place), outputs.
-// Outputs stay in TMEM from tile to tile; where a row's maximum grows they are scaled there.  Warps 0 - 3 are the softmax (a thread a query row), warp 4 issues, warp 5 copies.
+// Values come as the keys do, by rows, and are read as a transposed operand.  Warps 0 - 7 are the softmax (two threads a query row, each with half of the keys and of the output
+// columns), warp 8 issues, warp 9 copies.
+// A tensor core's f32 sum is cut, not rounded, at every product that joins it, always towards zero.  So the small products (hi lo, lo hi) of the scores have sums of their own, which
+// are added as the scores are read, and a tile's outputs join running ones in registers.  (With all three in one sum, and outputs that stayed in TMEM from tile to tile: 16 rows, 16
+// heads of 576 / 512 were off by 1.9e-6 behind 4096 keys and 4.3e-6 behind 32768, instead of 7.7e-7 and 8.7e-7; twenty tiles of positive values came out 1.8e-5 too small.)
+// TMEM: large sums of two tiles (which become scores and then probabilities in place), outputs of one.  Small sums borrow half of the outputs' columns.  The products go scores of
+// tile t + 1, values of tile t, scores of t + 2; values of t fill the half first that has no small sums of t + 1 in it, and the other one when those have been read, so nothing waits.
 // What bounds it: 64 KB of operands for every 64 dims of a tile, which an SM takes 1030 clocks to read and 770 to multiply.  256 query rows, 4096 keys of 576 dims, 512 columns:
 // pairs 8.6 us, this kernel 22 us (a tile a CTA: 7500 clocks until the first copy, 11500 scores, 4700 softmax, 4000 outputs, 8000 until they are stored), k_shared_rows 27 us.
 // What pairs cannot hold is known before the first product (the first kernel's scales and flags): the CTA then walks its share in plain f32.
-constexpr uint32_t kSwKeys = 128, kSwCols = 256, kSwStages = 3, kSwPart = 128 * 128, kSwStage = 4 * kSwPart, kSwThreads = 192;
-constexpr uint32_t kSwFactors = kSwStages * kSwStage, kSwRows = kSwFactors + 2 * 128 * 8, kSwRed = kSwRows + 512, kSwBars = kSwRed + 128, kSwSmem = kSwBars + 128 + 1024;
+constexpr uint32_t kSwKeys = 128, kSwCols = 256, kSwStages = 3, kSwPart = 128 * 128, kSwStage = 4 * kSwPart, kSwSoft = 256, kSwThreads = kSwSoft + 128;
+constexpr uint32_t kSwFactors = kSwStages * kSwStage, kSwRows = kSwFactors + 2 * 128 * 8, kSwShare = kSwRows + 512, kSwRed = kSwShare + 2 * 256 * 4, kSwBars = kSwRed + 128, kSwSmem = kSwBars + 128 + 1024;
 struct SwArgs {
     __half* q; __half* k; __half* v;             // pairs: [hi, lo][G][rows][dims, padded to 64]
     float* qf; float* kf; float* vf;             // what a row's pairs were divided by: [G][rows]; of a row of zeros 0, of a query that is not finite NaN
@@ -953,24 +958,25 @@ __device__ __noinline__ void sw_plain(const SaArgs& a, const float* kp, const fl
 }
 __global__ void __launch_bounds__(kSwThreads, 1) k_shared_wide(const __grid_constant__ SaArgs a, const __grid_constant__ SwArgs w, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                                                               const __grid_constant__ CUtensorMap map_v) {
-    constexpr uint32_t kS = 0, kO = 2 * kSwKeys;                            // TMEM columns
+    constexpr uint32_t kS = 0, kO = 2 * kSwKeys, kHalf = kSwCols / 2;       // TMEM columns; a half of the outputs
+    static_assert(kHalf >= kSwKeys, "small sums in a half of the outputs");
     extern __shared__ uint8_t dsm_raw[];
     const uint32_t base = (smem_u32(dsm_raw) + 1023u) & ~1023u;
     uint8_t* const mem = dsm_raw + (base - smem_u32(dsm_raw));
-    const uint32_t full = base + kSwBars, empty = full + 8 * kSwStages, s_full = empty + 8 * kSwStages, p_full = s_full + 16, o_full = p_full + 16, tmem_slot = o_full + 8;
+    const uint32_t full = base + kSwBars, empty = full + 8 * kSwStages, s_full = empty + 8 * kSwStages, p_full = s_full + 16, o_full = p_full + 16, o_read = o_full + 16, small_read = o_read + 16, tmem_slot = small_read + 8;
     uint32_t* const lost = reinterpret_cast<uint32_t*>(mem + (tmem_slot + 4 - base));      // a wait ran out
     uint32_t* const red = reinterpret_cast<uint32_t*>(mem + kSwRed);        // largest and smallest factor of the values, largest of the keys
     uint32_t* const rows = reinterpret_cast<uint32_t*>(mem + kSwRows);
     const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < kSwStages; i++) { mbar_init(full + 8 * i, 1); mbar_init(empty + 8 * i, 1); }
-        for (uint32_t i = 0; i < 2; i++) { mbar_init(s_full + 8 * i, 1); mbar_init(p_full + 8 * i, 4); }
-        mbar_init(o_full, 1);
+        for (uint32_t i = 0; i < 2; i++) { mbar_init(s_full + 8 * i, 1); mbar_init(p_full + 8 * i, kSwSoft / 32); mbar_init(o_full + 8 * i, 1); mbar_init(o_read + 8 * i, kSwSoft / 64); }
+        mbar_init(small_read, kSwSoft / 32);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         *lost = 0;
         red[0] = 0; red[1] = 0x7f800000u; red[2] = 0;
     }
-    if (warp == 4) {
+    if (warp == kSwSoft / 32) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(tmem_slot) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -1006,10 +1012,10 @@ __global__ void __launch_bounds__(kSwThreads, 1) k_shared_wide(const __grid_cons
         }
         v_top = __reduce_max_sync(0xffffffffu, v_top); v_low = __reduce_min_sync(0xffffffffu, v_low); k_top = __reduce_max_sync(0xffffffffu, k_top);
         if (lane == 0) { atomicMax(red, v_top); atomicMin(red + 1, v_low); atomicMax(red + 2, k_top); }
-        if (threadIdx.x < 128) {
-            const SpRow q = sp_row(a, c, head, threadIdx.x);
-            rows[threadIdx.x] = q.on ? q.r << 10 | q.h : 0xffffffffu;
-            const uint32_t at = c.tile * 128 + threadIdx.x;
+        if (threadIdx.x < kSwSoft) {
+            const uint32_t row = threadIdx.x & 127, at = c.tile * 128 + row;
+            const SpRow q = sp_row(a, c, head, row);
+            rows[row] = q.on ? q.r << 10 | q.h : 0xffffffffu;
             if (at < head.rows * a.rep) f = w.qf[(size_t)c.g * w.QR + at];
         }
     }
@@ -1019,120 +1025,165 @@ __global__ void __launch_bounds__(kSwThreads, 1) k_shared_wide(const __grid_cons
     fence_before();
     const bool plain = __syncthreads_or(slow);
     fence_after();
+    // Registers: 384 threads of 168 at launch, 64512 in all = 256 x 232 + 128 x 40.
     if (plain) {
         sw_plain(a, c.kp, c.vp, c.k0, c.k1, c.split, c0, rows);
     } else if (!n_tiles) {
-    } else if (warp == 5) {
-        if (elect_one()) {
-            const uint32_t yq = c.g * w.QR + c.tile * 128, yk = c.g * w.KR + c.k0, q_lo = a.G * w.QR, k_lo = a.G * w.KR;
-            uint32_t s = 0, phase = 1;
+    } else if (warp >= kSwSoft / 32) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        if (warp == kSwSoft / 32 + 1) {
+            if (elect_one()) {
+                const uint32_t yq = c.g * w.QR + c.tile * 128, yk = c.g * w.KR + c.k0, q_lo = a.G * w.QR, k_lo = a.G * w.KR;
+                uint32_t s = 0, phase = 1;
+                bool ok = true;
+                auto place = [&](uint32_t bytes) {
+                    ok = ok && mbar_wait(empty + 8 * s, phase);
+                    if (ok) mbar_expect_tx(full + 8 * s, bytes);
+                    return ok;
+                };
+                auto next = [&] { if (++s == kSwStages) { s = 0; phase ^= 1; } };
+                for (uint32_t t = 0; t <= n_tiles && ok; t++) {
+                    if (t < n_tiles)
+                        for (uint32_t i = 0; i < nc && place(kSwStage); i++) {
+                            const uint32_t to = base + s * kSwStage, bar = full + 8 * s;
+                            tma_2d(to, &map_q, 64 * i, yq, bar); tma_2d(to + kSwPart, &map_q, 64 * i, yq + q_lo, bar);
+                            tma_2d(to + 2 * kSwPart, &map_k, 64 * i, yk + t * kSwKeys, bar); tma_2d(to + 3 * kSwPart, &map_k, 64 * i, yk + t * kSwKeys + k_lo, bar);
+                            next();
+                        }
+                    if (t)
+                        for (uint32_t z = 0; z < 2; z++) {
+                            const uint32_t i = 2 * ((t & 1) ^ 1 ^ z), n = i < nv ? min(2u, nv - i) : 0u;
+                            if (!n || !place(n * 2 * kSwPart)) continue;
+                            for (uint32_t e = 0; e < n; e++) {
+                                const uint32_t to = base + s * kSwStage + 2 * e * kSwPart, bar = full + 8 * s, x = w.v0 + c0 + 64 * (i + e);
+                                tma_2d(to, &map_v, x, yk + (t - 1) * kSwKeys, bar); tma_2d(to + kSwPart, &map_v, x, yk + (t - 1) * kSwKeys + k_lo, bar);
+                            }
+                            next();
+                        }
+                }
+                if (!ok) { count_timeout(); atomicOr(lost, 1u); }
+            }
+            __syncwarp();
+        } else if (warp == kSwSoft / 32) {
+            // Issue.  Three products: hi lo and lo hi into the small sums, hi hi into the large ones; of a tile's values the small ones first.
+            constexpr uint32_t idesc_s = (1u << 4) | ((kSwKeys >> 3) << 17) | ((128u >> 4) << 24), idesc_o = (1u << 4) | (1u << 16) | ((64u >> 3) << 17) | ((128u >> 4) << 24);      // f16 x f16 -> f32; B transposed
+            uint32_t s = 0, phase = 0;
             bool ok = true;
-            auto place = [&](uint32_t bytes) {
-                ok = ok && mbar_wait(empty + 8 * s, phase);
-                if (ok) mbar_expect_tx(full + 8 * s, bytes);
-                return ok;
-            };
+            auto take = [&] { ok = ok && __all_sync(0xffffffffu, mbar_wait(full + 8 * s, phase)); fence_after(); return ok; };
             auto next = [&] { if (++s == kSwStages) { s = 0; phase ^= 1; } };
             for (uint32_t t = 0; t <= n_tiles && ok; t++) {
-                if (t < n_tiles)
-                    for (uint32_t i = 0; i < nc && place(kSwStage); i++) {
-                        const uint32_t to = base + s * kSwStage, bar = full + 8 * s;
-                        tma_2d(to, &map_q, 64 * i, yq, bar); tma_2d(to + kSwPart, &map_q, 64 * i, yq + q_lo, bar);
-                        tma_2d(to + 2 * kSwPart, &map_k, 64 * i, yk + t * kSwKeys, bar); tma_2d(to + 3 * kSwPart, &map_k, 64 * i, yk + t * kSwKeys + k_lo, bar);
-                        next();
-                    }
-                if (t)
-                    for (uint32_t i = 0; i < nv && place(min(2u, nv - i) * 2 * kSwPart); i += 2) {
-                        for (uint32_t e = 0; e < min(2u, nv - i); e++) {
-                            const uint32_t to = base + s * kSwStage + 2 * e * kSwPart, bar = full + 8 * s, x = w.v0 + c0 + 64 * (i + e);
-                            tma_2d(to, &map_v, x, yk + (t - 1) * kSwKeys, bar); tma_2d(to + kSwPart, &map_v, x, yk + (t - 1) * kSwKeys + k_lo, bar);
-                        }
-                        next();
-                    }
-            }
-            if (!ok) { count_timeout(); atomicOr(lost, 1u); }
-        }
-        __syncwarp();
-    } else if (warp == 4) {
-        // Issue.  Three products, the small ones first: hi lo, lo hi, hi hi.
-        constexpr uint32_t idesc_s = (1u << 4) | ((kSwKeys >> 3) << 17) | ((128u >> 4) << 24), idesc_o = (1u << 4) | (1u << 16) | ((64u >> 3) << 17) | ((128u >> 4) << 24);      // f16 x f16 -> f32; B transposed
-        uint32_t s = 0, phase = 0;
-        bool ok = true;
-        auto take = [&] { ok = ok && __all_sync(0xffffffffu, mbar_wait(full + 8 * s, phase)); fence_after(); return ok; };
-        auto next = [&] { if (++s == kSwStages) { s = 0; phase ^= 1; } };
-        for (uint32_t t = 0; t <= n_tiles && ok; t++) {
-            if (t < n_tiles) {
-                const uint32_t d = kS + (t & 1) * kSwKeys;
-                for (uint32_t i = 0; i < nc && take(); i++) {
-                    const uint32_t q = desc_low(base + s * kSwStage), k = q + (2 * kSwPart >> 4);
-                    if (elect_one()) {
-#pragma unroll
-                        for (uint32_t x = 0; x < 3; x++)
-#pragma unroll
-                            for (uint32_t j = 0; j < 4; j++) {
-                                const uint32_t qa = q + (x == 1 ? kSwPart >> 4 : 0) + 2 * j, ka = k + (x == 0 ? kSwPart >> 4 : 0) + 2 * j;
-                                if (x == 0 && j == 0 && i == 0) mma_ss<false>(d, qa, ka, idesc_s); else mma_ss<true>(d, qa, ka, idesc_s);
-                            }
-                        mma_commit(empty + 8 * s);
-                        if (i + 1 == nc) mma_commit(s_full + 8 * (t & 1));
-                    }
-                    __syncwarp();
-                    next();
-                }
-            }
-            if (t && ok) {
-                const uint32_t u = t - 1, p = kS + (u & 1) * kSwKeys;
-                ok = __all_sync(0xffffffffu, mbar_wait(p_full + 8 * (u & 1), (u >> 1) & 1));
-                fence_after();
-                for (uint32_t i = 0; i < nv && take(); i += 2) {
-                    if (elect_one()) {
-                        for (uint32_t e = 0; e < min(2u, nv - i); e++) {
-                            const uint32_t d = kO + 64 * (i + e), v = (((base + s * kSwStage + 2 * e * kSwPart) & 0x3FFFF) >> 4) | (64u << 16);      // groups of eight keys are 1024 B apart
+                const uint32_t small = kO + (t & 1) * kHalf;                // the half where this tile's small sums go
+                if (t < n_tiles) {
+                    // (the large ones overwrite the probabilities of tile t - 2, whose values have been issued: products execute in order)
+                    if (t >= 2) ok = __all_sync(0xffffffffu, mbar_wait(o_read + 8 * (t & 1), t & 1));
+                    const uint32_t d = kS + (t & 1) * kSwKeys;
+                    for (uint32_t i = 0; i < nc && take(); i++) {
+                        const uint32_t q = desc_low(base + s * kSwStage), k = q + (2 * kSwPart >> 4);
+                        if (elect_one()) {
 #pragma unroll
                             for (uint32_t x = 0; x < 3; x++)
 #pragma unroll
-                                for (uint32_t j = 0; j < kSwKeys / 16; j++) {
-                                    const uint32_t pa = p + 16 * j + (x == 1 ? 8 : 0), va = v + (x == 0 ? kSwPart >> 4 : 0) + 128 * j;
-                                    if (x == 0 && j == 0 && u == 0) mma_ts<false>(d, pa, va, idesc_o); else mma_ts<true>(d, pa, va, idesc_o);
+                                for (uint32_t j = 0; j < 4; j++) {
+                                    const uint32_t qa = q + (x == 1 ? kSwPart >> 4 : 0) + 2 * j, ka = k + (x == 0 ? kSwPart >> 4 : 0) + 2 * j;
+                                    if (x != 1 && j == 0 && i == 0) mma_ss<false>(x < 2 ? small : d, qa, ka, idesc_s); else mma_ss<true>(x < 2 ? small : d, qa, ka, idesc_s);
                                 }
+                            mma_commit(empty + 8 * s);
+                            if (i + 1 == nc) mma_commit(s_full + 8 * (t & 1));
                         }
-                        mma_commit(empty + 8 * s);
-                        if (i + 2 >= nv) mma_commit(o_full);
+                        __syncwarp();
+                        next();
                     }
-                    __syncwarp();
-                    next();
+                }
+                if (t && ok) {
+                    const uint32_t u = t - 1, p = kS + (u & 1) * kSwKeys;
+                    ok = __all_sync(0xffffffffu, mbar_wait(p_full + 8 * (u & 1), (u >> 1) & 1));
+                    for (uint32_t z = 0; z < 2 && ok; z++) {                // the half with the small sums of tile t comes last
+                        const uint32_t h = (t & 1) ^ 1 ^ z, i = 2 * h, n = i < nv ? min(2u, nv - i) : 0u;
+                        if (u) ok = __all_sync(0xffffffffu, mbar_wait(o_read + 8 * h, (u - 1) & 1));
+                        if (ok && z && t < n_tiles) ok = __all_sync(0xffffffffu, mbar_wait(small_read, t & 1));
+                        fence_after();
+                        if (!ok || (n && !take())) break;
+                        if (elect_one()) {
+                            for (uint32_t e = 0; e < n; e++) {
+                                const uint32_t d = kO + 64 * (i + e), v = (((base + s * kSwStage + 2 * e * kSwPart) & 0x3FFFF) >> 4) | (64u << 16);      // groups of eight keys are 1024 B apart
+#pragma unroll
+                                for (uint32_t x = 0; x < 3; x++)
+#pragma unroll
+                                    for (uint32_t j = 0; j < kSwKeys / 16; j++) {
+                                        const uint32_t pa = p + 16 * j + (x == 1 ? 8 : 0), va = v + (x == 0 ? kSwPart >> 4 : 0) + 128 * j;
+                                        if (x == 0 && j == 0) mma_ts<false>(d, pa, va, idesc_o); else mma_ts<true>(d, pa, va, idesc_o);
+                                    }
+                            }
+                            if (n) mma_commit(empty + 8 * s);
+                            mma_commit(o_full + 8 * h);
+                        }
+                        __syncwarp();
+                        if (n) next();
+                    }
                 }
             }
+            if (!ok && lane == 0) { count_timeout(); atomicOr(lost, 1u); }
+            __syncwarp();
         }
-        if (!ok && lane == 0) { count_timeout(); atomicOr(lost, 1u); }
-        __syncwarp();
     } else {
-        const uint32_t row = threadIdx.x, lanes = (warp * 32) << 16;
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+        // softmax: two threads a query row, each with half of the keys and of the output columns
+        constexpr int OW = kHalf;
+        const uint32_t part = warp >> 2, row = threadIdx.x & 127, lanes = ((warp & 3) * 32) << 16;
         float2* const factors = reinterpret_cast<float2*>(mem + kSwFactors);
+        float* const share = reinterpret_cast<float*>(mem + kSwShare);
         const float v_inv = v_ref > 0.0f ? 1.0f / v_ref : 0.0f, inv_cap = a.cap > 0.0f ? 1.0f / a.cap : 0.0f;      // (a power of two)
-        float m = -INFINITY, l = 0.0f;
+        uint32_t n_share = 0;
+        auto other = [&](float x) {                                         // what the row's other thread has; two buffers in turns, so one barrier is enough
+            float* s = share + (n_share++ & 1) * 256;
+            s[part * 128 + row] = x;
+            bar_sync(2 + (warp & 3), 64);
+            return s[(part ^ 1) * 128 + row];
+        };
+        float m = -INFINITY, l = 0.0f, alpha_prev = 0.0f;
+        float2 o[OW / 2];
+#pragma unroll
+        for (int i = 0; i < OW / 2; i++) o[i] = make_float2(0.0f, 0.0f);
         bool ok = true;
+        auto add_output = [&](uint32_t t) {                                 // outputs of tile t, the thread's half of them, join the running ones
+            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(o_full + 8 * part, t & 1));
+            fence_after();
+#pragma unroll
+            for (int h = 0; h < OW; h += 16) {
+                if (OW * part + h >= 64 * nv) break;
+                uint32_t v[16];
+                tmem_ld(lanes + kO + OW * part + h, v);
+                tmem_wait_ld(v);
+#pragma unroll
+                for (int j = 0; j < 16; j += 2) o[(h + j) / 2] = __ffma2_rn(o[(h + j) / 2], make_float2(alpha_prev, alpha_prev), make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])));
+            }
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(o_read + 8 * part);
+        };
 #pragma unroll 1
         for (uint32_t t = 0; t < n_tiles; t++) {
             float2* const fs = factors + (t & 1) * 128;
-            {
+            if (part == 0) {
                 const uint32_t u = c.k0 + t * kSwKeys + row;
                 fs[row] = u < c.k1 ? make_float2(kf[u], vf[u] * v_inv * 16384.0f) : make_float2(0.0f, 0.0f);      // probabilities times 2^14, in the frame of the share's largest values
             }
-            bar_sync(1, 128);
+            bar_sync(1, kSwSoft);
             if (ok) ok = __all_sync(0xffffffffu, mbar_wait(s_full + 8 * (t & 1), (t >> 1) & 1));
             fence_after();
-            const uint32_t s = lanes + kS + (t & 1) * kSwKeys, left = c.k1 - c.k0 - t * kSwKeys;
+            const uint32_t s = lanes + kS + (t & 1) * kSwKeys, small = lanes + kO + (t & 1) * kHalf, h0 = 64 * part, left = c.k1 - c.k0 - t * kSwKeys;
             // Loops of 16 keys, whose scores go back to TMEM in between: a tile is often the only one, and code that runs once costs its fetching (all 128 unrolled took
             // 18000 clocks).
             float top = -INFINITY;
 #pragma unroll 1
-            for (uint32_t h = 0; h < 128; h += 16) {
-                uint32_t v[16];
+            for (uint32_t h = h0; h < h0 + 64; h += 16) {
+                uint32_t v[16], u[16];
                 tmem_ld(s + h, v);
+                tmem_ld(small + h, u);
                 tmem_wait_ld(v);
+                tmem_wait_ld(u);
 #pragma unroll
-                for (int j = 0; j < 16; j++) v[j] = __float_as_uint(__uint_as_float(v[j]) * (f * fs[h + j].x));
+                for (int j = 0; j < 16; j++) v[j] = __float_as_uint((__uint_as_float(v[j]) + __uint_as_float(u[j])) * (f * fs[h + j].x));
                 if (a.cap > 0.0f) {
 #pragma unroll
                     for (int j = 0; j < 16; j++) v[j] = __float_as_uint(sa_capped(__uint_as_float(v[j]) * kLn2, a.cap, inv_cap) * kLog2e);
@@ -1146,26 +1197,15 @@ __global__ void __launch_bounds__(kSwThreads, 1) k_shared_wide(const __grid_cons
                 tmem_st(s + h, v);
             }
             tmem_wait_st();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(small_read);
+            top = fmaxf(top, other(top));
             const float m_new = fmaxf(m, top), alpha = m == -INFINITY ? 0.0f : sa_ex2(m - m_new);
-            if (t) {
-                if (ok) ok = __all_sync(0xffffffffu, mbar_wait(o_full, (t - 1) & 1));
-                fence_after();
-                if (__any_sync(0xffffffffu, m_new > m)) {
-#pragma unroll 1
-                    for (uint32_t h = 0; h < 2 * nv; h++) {
-                        uint32_t v[32];
-                        tmem_ld(lanes + kO + 32 * h, v);
-                        tmem_wait_ld(v);
-#pragma unroll
-                        for (int j = 0; j < 32; j++) v[j] = __float_as_uint(__uint_as_float(v[j]) * alpha);
-                        tmem_st(lanes + kO + 32 * h, v);
-                    }
-                }
-            }
             m = m_new;
             float l0 = 0.0f, l1 = 0.0f;
 #pragma unroll 1
-            for (uint32_t h = 0; h < 128; h += 16) {
+            for (uint32_t h = h0; h < h0 + 64; h += 16) {
                 uint32_t x[16], v[16];
                 tmem_ld(s + h, x);
                 tmem_wait_ld(x);
@@ -1182,33 +1222,30 @@ __global__ void __launch_bounds__(kSwThreads, 1) k_shared_wide(const __grid_cons
             fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(p_full + 8 * (t & 1));
+            if (t) add_output(t - 1);
+            alpha_prev = alpha;
         }
-        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(o_full, (n_tiles - 1) & 1));
-        fence_after();
+        add_output(n_tiles - 1);
+        l += other(l);
         if (!ok && lane == 0) { count_timeout(); atomicOr(lost, 1u); }
         // Outputs leave by whole rows, through the idle stages.
         const float unit = v_ref * (1.0f / 16384.0f);
         float4* const out = reinterpret_cast<float4*>(mem);
-#pragma unroll 1
-        for (uint32_t h = 0; h < 2 * nv; h++) {
-            uint32_t v[32];
-            tmem_ld(lanes + kO + 32 * h, v);
-            tmem_wait_ld(v);
 #pragma unroll
-            for (int j = 0; j < 32; j += 4)
-                out[row * (kSwCols / 4) + ((8 * h + j / 4) ^ (row & 7))] = make_float4(__uint_as_float(v[j]) * unit, __uint_as_float(v[j + 1]) * unit, __uint_as_float(v[j + 2]) * unit, __uint_as_float(v[j + 3]) * unit);
-        }
-        bar_sync(1, 128);
+        for (int j = 0; j < OW; j += 4)
+            out[row * (kSwCols / 4) + (((OW * part + j) / 4) ^ (row & 7))] = make_float4(o[j / 2].x * unit, o[j / 2].y * unit, o[j / 2 + 1].x * unit, o[j / 2 + 1].y * unit);
+        bar_sync(1, kSwSoft);
         const bool gone = *reinterpret_cast<volatile uint32_t*>(lost);
         const uint32_t mine = rows[row];
-        if (mine != 0xffffffffu && half == 0) { float* rec = sa_record(a, mine >> 10, mine & 1023, c.split); rec[0] = gone ? kBatchNaN : m * kLn2; rec[1] = gone ? kBatchNaN : l; }
+        if (mine != 0xffffffffu && half == 0 && part == 0) { float* rec = sa_record(a, mine >> 10, mine & 1023, c.split); rec[0] = gone ? kBatchNaN : m * kLn2; rec[1] = gone ? kBatchNaN : l; }
         const uint32_t e = threadIdx.x % (kSwCols / 4);
+        constexpr uint32_t kStep = kSwSoft / (kSwCols / 4);                 // rows at a time
 #pragma unroll 1
-        for (uint32_t r0 = threadIdx.x / (kSwCols / 4); r0 < 128; r0 += 16) {
+        for (uint32_t r0 = threadIdx.x / (kSwCols / 4); r0 < 128; r0 += 8 * kStep) {
             uint32_t to[8];
             float4 y[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) { to[i] = rows[r0 + 2 * i]; y[i] = out[(r0 + 2 * i) * (kSwCols / 4) + (e ^ ((r0 + 2 * i) & 7))]; }
+            for (int i = 0; i < 8; i++) { to[i] = rows[r0 + kStep * i]; y[i] = out[(r0 + kStep * i) * (kSwCols / 4) + (e ^ ((r0 + kStep * i) & 7))]; }
 #pragma unroll
             for (int i = 0; i < 8; i++)
                 if (to[i] != 0xffffffffu && 4 * e < cols)
@@ -1219,7 +1256,7 @@ __global__ void __launch_bounds__(kSwThreads, 1) k_shared_wide(const __grid_cons
     __syncwarp();
     fence_before();
     __syncthreads();
-    if (warp == 4) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(0u) : "memory");
+    if (warp == kSwSoft / 32) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(0u) : "memory");
 }
 
 // What decides a launch: queries a CTA of k_shared_rows holds (RQ), float4 a lane holds (NV), lanes that share a key (LK), shares of its keys; shares of the prefix

@@ -292,6 +292,10 @@ __global__ void __launch_bounds__(kAfThreads, WIDE ? 2 : 4) __cluster_dims__(kAf
 // (The same on mma.sync took 124 us for 2048 rows of 4096 inputs, 14336 outputs, rank 64, with its issue rate as the bound: 11.3 T operations of products at 130 T/s.)
 // Every wait is bounded; a CTA whose wait ran out counts it and makes NaN of its rows.
 constexpr uint32_t kAmRows = 128, kAmRank = 64, kAmPart = kAmRows * 128;      // rows of a block, rank values, bytes of a part of 128 rows of 64 values
+// Chunks of 64 inputs that a sum on the tensor cores holds before it joins those before it, rounded: the cores cut their sums, always towards zero.  2048 rows, rank 64, error
+// against 64 bits and us with all of a CTA's inputs in one sum and in sums of four chunks: 4096 inputs 8.2e-7, 84.2 / 4.0e-7, 85.2; 14336 inputs 3.0e-6, 109 / 4.0e-7, 113; 32768
+// inputs 9.2e-6, 196 / 5.2e-7, 204; 512 rows of f32 weights, 14336 inputs 8.1e-6, 65.7 / 1.0e-6, 67.7.  (Plain f32: 5.9e-7, 1.1e-6, 2.2e-6, 6.0e-7.)
+constexpr uint32_t kAmJoin = 4;
 template <typename WT> struct AmParts { static constexpr uint32_t n = sizeof(WT) == 2 ? 1 : 3; };      // of the weights: bfloat16 ones are one part themselves
 template <typename WT> constexpr uint32_t kAmRuns = sizeof(WT) == 2 ? 4 : 2;
 // products, small ones first: {part of x, part of w}
@@ -341,6 +345,8 @@ template <typename WT> struct AsLayout {
 template <typename WT>
 __global__ void __launch_bounds__(256, 1) __cluster_dims__(kAfCluster, 1, 1) k_adapter_shrink(AdArgs a, const WT* __restrict__ wa, uint4* __restrict__ parts) {
     typedef AsLayout<WT> L;
+    constexpr uint32_t kJoined = 256;                                // TMEM column of the joined sums, behind those under way
+    static_assert(kAmJoin % 2 == 0 && kAmJoin >= 4 && kJoined >= kAmRuns<WT> * kAmRank, "pairs of chunks, TMEM columns");
     extern __shared__ uint8_t am_raw[];
     const uint32_t base = (smem_u32(am_raw) + 1023u) & ~1023u;
     uint8_t* const mem = am_raw + (base - smem_u32(am_raw));
@@ -356,7 +362,7 @@ __global__ void __launch_bounds__(256, 1) __cluster_dims__(kAfCluster, 1, 1) k_a
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" ::"r"(tmem_slot) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(tmem_slot) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -416,6 +422,10 @@ __global__ void __launch_bounds__(256, 1) __cluster_dims__(kAfCluster, 1, 1) k_a
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
+        // Where the sums of kAmJoin chunks are under way, number g of them.  Up to two runs have room for two of them, so that one is joined to those before while the next one is
+        // made; more runs wait for it.
+        const bool twice = runs <= 2;
+        auto at = [&](uint32_t g) { return tmem + (twice && (g & 1) ? 2 * kAmRank : 0u); };
         uint32_t slot = 0;                                           // of the weights of chunk t
         auto chunk = [&](uint32_t t, float4 (&x)[4][2]) {
             const uint32_t s = uses & 1;
@@ -435,7 +445,7 @@ __global__ void __launch_bounds__(256, 1) __cluster_dims__(kAfCluster, 1, 1) k_a
             am_proxy_fence();
             __syncthreads();
             if (warp == 0) {
-                const uint32_t xs = desc_low(base) + s * (L::x_stage >> 4), w0 = desc_low(base + L::w) + slot * (L::w_slot >> 4), idesc = am_idesc(kAmRank), freed = done + 8 * s;
+                const uint32_t xs = desc_low(base) + s * (L::x_stage >> 4), w0 = desc_low(base + L::w) + slot * (L::w_slot >> 4), idesc = am_idesc(kAmRank), freed = done + 8 * s, to = at(t / kAmJoin);
                 fence_after();
                 if (elect_one() && ok) {
 #pragma unroll
@@ -446,8 +456,8 @@ __global__ void __launch_bounds__(256, 1) __cluster_dims__(kAfCluster, 1, 1) k_a
 #pragma unroll
                             for (uint32_t z = 0; z < 4; z++) {
                                 const uint32_t xd = xs + am_x<WT>(y) * (kAmPart >> 4) + 2 * z, wd = w0 + (i * L::w_run + am_w<WT>(y) * L::weights) / 16 + 2 * z;
-                                if (y == 0 && z == 0) { if (t == 0) mma_ss<false>(tmem + i * kAmRank, xd, wd, idesc); else mma_ss<true>(tmem + i * kAmRank, xd, wd, idesc); }
-                                else mma_ss<true>(tmem + i * kAmRank, xd, wd, idesc);
+                                if (y == 0 && z == 0) { if (t % kAmJoin == 0) mma_ss<false>(to + i * kAmRank, xd, wd, idesc); else mma_ss<true>(to + i * kAmRank, xd, wd, idesc); }
+                                else mma_ss<true>(to + i * kAmRank, xd, wd, idesc);
                             }
                     }
                     mma_commit(freed);
@@ -457,6 +467,28 @@ __global__ void __launch_bounds__(256, 1) __cluster_dims__(kAfCluster, 1, 1) k_a
             slot = after;
             uses++;
         };
+        const uint32_t row = (warp & 3) * 32 + lane, col = 32 * (warp >> 2), lanes = ((warp & 3) * 32) << 16;
+        // Sums of kAmJoin chunks (number g of them) join those of the chunks before
+        auto join = [&](uint32_t g) {
+            fence_after();
+#pragma unroll 1
+            for (uint32_t i = 0; i < runs; i++) {
+                uint32_t v[32], w[32];
+                tmem_ld(at(g) + lanes + i * kAmRank + col, v);
+                if (g) tmem_ld(tmem + lanes + kJoined + i * kAmRank + col, w);
+                tmem_wait_ld(v);
+                if (g) {
+                    tmem_wait_ld(w);
+#pragma unroll
+                    for (int y = 0; y < 32; y++) v[y] = __float_as_uint(__uint_as_float(v[y]) + __uint_as_float(w[y]));
+                }
+                tmem_st(tmem + lanes + kJoined + i * kAmRank + col, v);
+            }
+            tmem_wait_st();
+            fence_before();
+        };
+        // products of the last chunk (1) or the one before (2)
+        auto wait_for = [&](uint32_t back) { if (ok) ok = __all_sync(0xffffffffu, mbar_wait(done + 8 * ((uses - back) & 1), ((uses - back) >> 1) & 1)); };
         load(0, xa);
         load(1, xb);
         if constexpr (sizeof(WT) == 2) weights(0, 0);
@@ -464,22 +496,33 @@ __global__ void __launch_bounds__(256, 1) __cluster_dims__(kAfCluster, 1, 1) k_a
         for (uint32_t t = 0; t < n; t += 2) {
             chunk(t, xa);
             if (t + 1 < n) chunk(t + 1, xb);
+            if (!twice && (t + 2) % kAmJoin == 0 && t + 2 < n) { wait_for(1); join(t / kAmJoin); }
+            if (twice && t && t % kAmJoin == 0) {                    // (chunk t + 1 has waited for the last of the sums before)
+                if (t + 1 == n) wait_for(2);
+                join(t / kAmJoin - 1);
+            }
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
         // all products of these runs are there; their sums take the first stage's place
-        if (n && ok) ok = __all_sync(0xffffffffu, mbar_wait(done + 8 * ((uses - 1) & 1), ((uses - 1) >> 1) & 1));
-        if (n > 1 && ok) ok = __all_sync(0xffffffffu, mbar_wait(done + 8 * (uses & 1), ((uses - 2) >> 1) & 1));
+        if (n) wait_for(1);
+        if (n > 1) wait_for(2);
         fence_after();
         if (!ok) *lost = 1;                                          // a warp whose wait ran out has written over operands that others read
         __syncthreads();
         ok = !*lost;
         float* const sums = reinterpret_cast<float*>(mem);           // [128][width]
-        const uint32_t row = (warp & 3) * 32 + lane, col = 32 * (warp >> 2);
 #pragma unroll 1
         for (uint32_t i = 0; i < runs; i++) {
             uint32_t v[32];
-            tmem_ld(tmem + (((warp & 3) * 32) << 16) + i * kAmRank + col, v);
+            tmem_ld(at((n - 1) / kAmJoin) + lanes + i * kAmRank + col, v);
             tmem_wait_ld(v);
+            if (n > kAmJoin) {
+                uint32_t w[32];
+                tmem_ld(tmem + lanes + kJoined + i * kAmRank + col, w);
+                tmem_wait_ld(w);
+#pragma unroll
+                for (int y = 0; y < 32; y++) v[y] = __float_as_uint(__uint_as_float(v[y]) + __uint_as_float(w[y]));
+            }
             if (row >= (uint32_t)run[i].first && row < (uint32_t)run[i].end) {
 #pragma unroll
                 for (int y = 0; y < 32; y += 4)
@@ -512,7 +555,7 @@ __global__ void __launch_bounds__(256, 1) __cluster_dims__(kAfCluster, 1, 1) k_a
     }
     if (!ok && threadIdx.x == 0) count_timeout();
     __syncthreads();
-    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem) : "memory");
+    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
 constexpr uint32_t kAxWriters = 256, kAxThreads = kAxWriters + 128;

@@ -330,7 +330,8 @@ typedef enum ZgOpTag {
  *                   reads key head h / (H / G) and value head h / (H / G); value caches may be the key caches.  Prefix buffers (external [prefix slots, n11, width])
  *                   may be absent (P is then 0).  Score cap f1 and sinks as CACHED_ATTENTION has them.  A row that sees no key gets zeros.
  *                   Many query rows over a long prefix run on the tensor cores: queries, keys and values as half-precision pairs (22 to 24 bits of what lies
- *                   within 2^-18 of the largest of a query's row and of 64 keys, or of a key's row), a share that these cannot hold in plain f32.
+ *                   within 2^-18 of the largest of a query's row and of 64 keys, or of a key's row), a share that these cannot hold in plain f32.  Weights are the hardware's
+ *                   exponentials of base 2 (off by 2^-22 of a weight), score caps are made of them too (a series near 0); sums of weights times values are f32.
  *                   buf 0 dst [B, H * dv] 1 q 2 key cache 3 value cache 4 prefix keys 5 prefix values 6 table 7 sinks
  *                   off 0 q column 1 key column 2 value column 3 prefix key column 4 prefix value column 5 sinks 6 dst column
  *                   n 0 B 1 H 2 G 3 dk 4 dv 5 q row stride 6 key row width 7 value row width 8 R 9 prefix key row width 10 prefix value row width
@@ -338,7 +339,7 @@ typedef enum ZgOpTag {
  * ADAPTER_LINEAR    dst[r] = base[r] + s_a B_a (A_a src[r]), a the row's adapter (negative: none, dst[r] = base[r]): low-rank adapters of many requests beside the LINEAR
  *                   that wrote `base` (which may be dst itself).  A [adapters, rank, K] and B [adapters, N, rank] are weights, s_a an f32 number per adapter (absent: 1).
  *                   Form 2, and form 0 with more than 256 rows: blocks of 128 rows on the tensor cores, one run of rows with one adapter after the other, over three bfloat16 parts
- *                   of each f32 operand (there what is not finite comes out as NaN), where ranks of 8 to 64 and sizes in multiples of 16 bytes allow it.  Otherwise, and form 1: runs of at
+ *                   of each f32 operand (six of the nine products of two such; there what is not finite comes out as NaN), where ranks of 8 to 64, multiples of 8, and sizes in multiples of 16 bytes allow it.  Otherwise, and form 1: runs of at
  *                   most eight rows side by side.
  *                   buf 0 dst 1 src 2 weights 3 scales 4 table 5 base | off 0 A 1 B 2 src 3 dst 4 scales 5 base
  *                   n 0 B 1 N 2 K 3 rank 4 adapters 5 src row stride 6 dst row stride 7 wdt 8 base row stride 9 form

@@ -756,7 +756,8 @@ __global__ void __launch_bounds__(kAxThreads, 1) k_adapter_expand(AdArgs a, cons
 
 // More rows than kAmLeast go in blocks, where rank and strides allow their 16-byte pieces, unless the op says which way to take: a block walks its runs one after the other, and only the
 // host knows how long they are.  us in blocks and by runs of eight: 4096 inputs and outputs, rank 16: 256 rows in runs of 64 26.7 / 20.4, 512 in runs of 128 24.6 / 30.4, of 8 102 / 27, of one 712 / 45;
-// 14336 outputs, rank 64: 64 rows of one run 27 / 42, 256 in runs of 128 26.5 / 57.7.
+// 14336 outputs, rank 64: 64 rows of one run 27 / 42, 256 in runs of 128 26.5 / 57.7.  (The length of runs decides, which no size says: the number of rows is right where many rows are
+// prompts and few rows are decoded, and `form` is for the rest.)
 constexpr uint32_t kAmLeast = 256;
 bool many_rows(const ZgSeqOp& s) {
     const uint32_t B = s.n[0], K = s.n[2], rank = s.n[3], form = s.n[9];

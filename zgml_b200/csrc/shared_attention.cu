@@ -847,7 +847,7 @@ __global__ void __launch_bounds__(kSpThreads, 1) k_shared_prefix(const __grid_co
 // TMEM: large sums of two tiles (which become scores and then probabilities in place), outputs of one.  Small sums borrow half of the outputs' columns.  The products go scores of
 // tile t + 1, values of tile t, scores of t + 2; values of t fill the half first that has no small sums of t + 1 in it, and the other one when those have been read, so nothing waits.
 // What bounds it: 64 KB of operands for every 64 dims of a tile, which an SM takes 1030 clocks to read and 770 to multiply.  256 query rows, 4096 keys of 576 dims, 512 columns:
-// pairs 8.6 us, this kernel 22 us (a tile a CTA: 7500 clocks until the first copy, 11500 scores, 4700 softmax, 4000 outputs, 8000 until they are stored), k_shared_rows 27 us.
+// pairs 8.5 us, this kernel 21.4 us (a tile a CTA: about 7500 clocks until the first copy, 11500 scores, 4000 outputs), k_shared_rows 27 us.
 // What pairs cannot hold is known before the first product (the first kernel's scales and flags): the CTA then walks its share in plain f32.
 constexpr uint32_t kSwKeys = 128, kSwCols = 256, kSwStages = 3, kSwPart = 128 * 128, kSwStage = 4 * kSwPart, kSwSoft = 256, kSwThreads = kSwSoft + 128;
 constexpr uint32_t kSwFactors = kSwStages * kSwStage, kSwRows = kSwFactors + 2 * 128 * 8, kSwShare = kSwRows + 512, kSwRed = kSwShare + 2 * 256 * 4, kSwBars = kSwRed + 128, kSwSmem = kSwBars + 128 + 1024;
@@ -1266,7 +1266,8 @@ __global__ void __launch_bounds__(kSwThreads, 1) k_shared_wide(const __grid_cons
 constexpr uint64_t kSwLeast = 1u << 17;
 // The same for k_shared_prefix (32 heads over 8 key heads of 128, up to 512 keys of their own; us, with it and without): 8 rows, 512 keys 33 / 26, 1024 34.6 / 32, 2048 37 / 43,
 // 8192 49 / 108; 32 rows, 64 keys 35 / 25, 256 36.8 / 32.8, 512 36 / 41, 1024 39 / 59; 128 rows, 64 keys 77 / 69, 256 84 / 94.  And from 32 query rows a key head on, since a quarter of
-// a tile is still full then: 4 rows (16 query rows), 4096 keys 37 / 29, 8192 45 / 47; 2 rows, 4096 keys 36.6 / 36.9, 8192 45 / 57; 1 row, 8192 keys 37 / 29.
+// a tile is still full then: 4 rows (16 query rows), 4096 keys 37 / 29, 8192 45 / 47; 2 rows, 4096 keys 36.6 / 36.9, 8192 45 / 57; 1 row, 8192 keys 37 / 29.  (So few rows over
+// more keys would gain: the plain walk grows with rows and keys, this form with keys alone, and the rule does not weigh them against each other.)
 constexpr uint64_t kSpLeast = 3u << 17;
 struct SaShape { uint32_t RQ, NV, LK, chunks, splits, warps, shares, row_tiles, halves; bool records; };      // halves: of the output columns, of a head wider than 128 (0: k_shared_prefix)
 SaShape sa_shape(const ZgSeqOp& s, bool wide) {

@@ -94,7 +94,13 @@ typedef enum ZgOpTag {
     ZG_OP_SHARED_ATTENTION = 39,
     ZG_OP_ADAPTER_LINEAR = 40,
     ZG_OP_LOGIT_RULES = 41,
-    ZG_OP_END = 42
+    /* The same over paged caches in 8 bits (csrc/pageops.cu, csrc/paged_attention.cu), and the choice of the next tokens (csrc/sample.cu). */
+    ZG_OP_PAGE_APPEND = 42,
+    ZG_OP_PAGED_ATTENTION = 43,
+    ZG_OP_PAGE_READ = 44,
+    ZG_OP_PAGE_COPY = 45,
+    ZG_OP_SAMPLE = 46,
+    ZG_OP_END = 47
 } ZgOpTag;
 
 /* Parameter pack of the sequence-model ops.  buf[] are program buffer indices (ZG_NO_BUF: absent), off[] element offsets,
@@ -349,9 +355,44 @@ typedef enum ZgOpTag {
  *                   {history slot, history length, first, mask row (negative: none), first bias entry, bias entries, repetition, presence, frequency (f32 bits), 0, 0, 0},
  *                   [0] live rows as above.  Tokens outside the vocabulary are passed over; entries of one token add up in order.
  *                   buf 0 dst 1 src 2 table 3 history (int32 [slots, n4]) 4 biases ({int32 token, f32 bias}) 5 masks (bit t % 32 of word t / 32, rows of ceil(V / 32) words)
- *                   off 0 dst 1 src | n 0 B 1 V 2 src row stride 3 dst row stride 4 history rows */
+ *                   off 0 dst 1 src | n 0 B 1 V 2 src row stride 3 dst row stride 4 history rows
+ *
+ * Paged caches.  A POOL (external) holds pages of n5 or n7 tokens (16, 32 or 64) for all G key heads; a PAGE TABLE (int32 [slots, most]) names the pages of a slot's
+ * positions in order, and may name one page for several slots.  The rows' words are those of the batch table; position length - 1 of a slot is token (length - 1) mod page of
+ * its page (length - 1) / page.  dk and dv are at most 256.  A page is G parts of 16 + page * (kp + vp) bytes, kp = dk rounded up to 32 and vp = dv rounded up to 16: the f32
+ * scale of its keys, that of its values, 8 bytes that are not used; keys, then values, a byte each: a code of -127 to 127 plus 128, worth code * scale; scales are powers of two.
+ * The key of (token t, dim d) is byte ((t / 8) * (kp / 32) + d / 32) * 256 + (t % 8) * 32 + d % 32 of the keys, the value byte ((t / 16) * (vp / 16) + d / 16) * 256 +
+ * (4 * (d % 8) + t % 8 / 2) * 8 + 4 * (d / 8 % 2) + 2 * (t / 8 % 2) + t % 2 of the values.  A pool starts as zeros.  A page that does not exist makes a row NaN, like a word out of range.
+ *
+ * PAGE_APPEND       the rows join their pages, their keys and query heads turned as BATCH_APPEND turns them, in 64 bits, rounded once.  Per page, head, and keys or values: the
+ *                   scale becomes the larger of its own (none yet, if token 0 is among those that join) and the smallest power of two (2^-126 at least) of which 127 times
+ *                   reach the largest magnitude that joins; codes that the page has become the nearest multiples of a larger scale, new ones the nearest to value / scale, halves to even
+ *                   codes.  So a code is off by less than one scale whatever joined since, by half of one where the scale did not grow.  Values that are not finite make a scale NaN, and with it
+ *                   the page's part of that head, until its token 0 is written anew.  A row of length 0 appends nothing; of rows that name the same place the last one
+ *                   stays; two slots that append to one page in a step race for its bytes.
+ *                   buf 0 pool 1 src 2 page table 3 table 4 frequency table 5 turned query heads | off 0 key column 1 value column 2 query column 3 column in buf 5 4 frequency offset
+ *                   n 0 B 1 G 2 dk 3 dv 4 src row stride 5 page 6 most 7 first turned value 8 turned values 9 layout 10 query heads 11 row stride of buf 5 | f 0 base
+ * PAGED_ATTENTION   softmax attention of each row over the first `length` positions of its slot, with a window n9 > 0 over the last n9 of them.  Query head h reads key head
+ *                   h / (H / G).  Score cap f1 and sinks as CACHED_ATTENTION has them.  A row that sees no key gets zeros.
+ *                   buf 0 dst [B, H * dv] 1 q 2 pool 3 page table 4 table 5 sinks | off 0 q column 1 dst column 2 sinks
+ *                   n 0 B 1 H 2 G 3 dk 4 dv 5 q row stride 6 dst row stride 7 page 8 most 9 window 10 wdt of the sinks | f 0 score scale 1 score cap
+ * PAGE_READ         dst[row] = the cache row at each row's position (keys at column off 0, values at off 1), code * scale; a row of length 0 gets zeros.
+ *                   buf 0 dst 1 pool 2 page table 3 table | off 0 key column 1 value column | n 0 B 1 G 2 dk 3 dv 4 dst row stride 5 page 6 most
+ * PAGE_COPY         pages of n1 words are copied inside the pool (a fork's last page, a compaction).  Table: [0] live moves, from word ZG_BATCH_ROWS on four words a move:
+ *                   {source, destination, 0, 0}.  A move that names no page, or one page twice, is not made.  Moves run at once: a page that two of them write, or that one
+ *                   reads and another writes, holds undefined bytes (page_moves refuses them).
+ *                   buf 0 pool 1 table | n 0 B 1 words of a page
+ * SAMPLE            the next token of each row of logits z.  Of e^((z - largest z) / temperature) the top_k largest stay (0: all), of those the fewest of the largest whose sum reaches
+ *                   top_p of theirs (1: all), of those the ones that are at least min_p; the token is the first, in the vocabulary's order, up to which what stays sums to more
+ *                   than u of all that stays.  Among equal logits the lower token counts as the larger.  Temperature 0: the largest logit.  Exponentials in 64 bits, sums exact over
+ *                   multiples of 2^-43.  Table: [0] live rows, from word ZG_BATCH_ROWS on ZG_SAMPLE_WORDS words a row: {temperature, top_k (int), top_p, min_p, u, 0, 0, 0}; a row
+ *                   whose top_k is below zero is idle and left as it is.  A row with a NaN among its logits, with none above -inf, with temperature negative or not finite, or with top_p, min_p outside [0, 1], u outside
+ *                   [0, 1), gets token -1 and probability NaN.
+ *                   buf 0 dst (int32 [B]) 1 logits 2 table 3 probability of the token among those that stay (f32 [B], may be absent)
+ *                   off 0 dst 1 logits 2 probability | n 0 B 1 V 2 logits row stride */
 #define ZG_BATCH_ROWS 8
 #define ZG_RULE_WORDS 12
+#define ZG_SAMPLE_WORDS 8
 #define ZG_NO_BUF 0xFFFFFFFFu
 #define ZG_W_F32 0
 #define ZG_W_BF16 1

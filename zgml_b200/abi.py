@@ -25,7 +25,8 @@ OP_ALLREDUCE, OP_ALLGATHER = 12, 13   # multi-GPU extensions (need comm_init)
 (OP_SSM_SCAN, OP_MIN_GRU, OP_GATED_NORM, OP_HEAD_NORM, OP_ACTIVATION, OP_RG_LRU) = range(31, 37)
 OP_STREAM_STEP = 37
 (OP_BATCH_APPEND, OP_SHARED_ATTENTION, OP_ADAPTER_LINEAR, OP_LOGIT_RULES) = range(38, 42)
-OP_END = 42
+(OP_PAGE_APPEND, OP_PAGED_ATTENTION, OP_PAGE_READ, OP_PAGE_COPY, OP_SAMPLE) = range(42, 47)
+OP_END = 47
 MASK_CAUSAL, MASK_WINDOW, MASK_BLOCK, MASK_POOLED = 0, 1, 2, 3      # pooled: a window, and one mean key and value per block before it
 NORM_LAYER, NORM_RMS, NORM_UNIT_OFFSET, NORM_GAIN = 0, 1, 2, 4
 NORM_DYNAMIC_TANH, NORM_NONE = 8, 16       # tanh(alpha x) w + b (bias and alpha follow w); the row itself: no statistics either way
@@ -37,7 +38,7 @@ ACTIVATIONS = {"relu2": 0, "silu": 1, "gelu_tanh": 2, "relu": 3, "softcap": 4, "
 NO_BUF = 0xFFFFFFFF
 W_F32, W_BF16 = 0, 1
 CTL_POS, CTL_SLOT, CTL_PREV, CTL_IDS = 0, 1, 2, 8
-BATCH_ROWS, BATCH_WORDS, RULE_WORDS = 8, 4, 12      # tables of a batch: words before the rows, per row, per row of LOGIT_RULES
+BATCH_ROWS, BATCH_WORDS, RULE_WORDS, SAMPLE_WORDS = 8, 4, 12, 8      # tables of a batch: words before the rows, per row, per row of LOGIT_RULES, of SAMPLE
 GATE_AFTER, GATE_SIGMOID = 1, 2            # forms of GATED_NORM (n7)
 ROTATE_THEN_NORM, NORM_THEN_ROTATE, ROTATE_ONLY = 0, 1, 2     # CACHE_APPEND (n13)
 QWEIGHT_RESIDENT = (1 << 64) - 1

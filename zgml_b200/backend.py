@@ -476,6 +476,39 @@ class DeviceOp:
         return DeviceOp._seq(abi.OP_LOGIT_RULES, [dst, src, table, history, bias, masks], DeviceOp._words(dst_off, src_off),
                              DeviceOp._words(B, V, src_rs or V, dst_rs or V, history_rows if history is not None else 0))
 
+    # ── the same over paged caches in 8 bits (host/pages.py) ──
+    @staticmethod
+    def page_append(pages, src, page_table, table, k_col, v_col, B, G, dk, dv, src_rs, page_tokens, most, turn_at=0, rot=0, rot_base=0.0, rot_layout="pairs", freqs=None, freqs_off=0,
+                    q_heads=0, q_col=0, turned=None, turned_col=0, turned_rs=0):
+        """Keys (column `k_col`) and values of every row join the pages of the row's slot, of which `page_table` has `most` a slot, as 8-bit codes with a scale per page and
+        head.  Keys and `q_heads` query heads are turned as batch_append turns them."""
+        return DeviceOp._seq(abi.OP_PAGE_APPEND, [pages, src, page_table, table, freqs if rot else None, turned if q_heads else None], DeviceOp._words(k_col, v_col, q_col, turned_col, freqs_off),
+                             DeviceOp._words(B, G, dk, dv, src_rs, page_tokens, most, turn_at, rot) + [{"pairs": 0, "halves": 1}[rot_layout]] +
+                             DeviceOp._words(q_heads, turned_rs or turned_col + q_heads * dk), [rot_base])
+
+    @staticmethod
+    def paged_attention(dst, q, pages, page_table, table, B, H, G, dk, dv, q_rs, page_tokens, most, scale, q_col=0, window=0, softcap=0.0, sink=None, sink_off=0, sink_wdt=0, dst_rs=0, dst_col=0):
+        """Attention of every row over what its slot's pages hold, with `window` over the last positions only.  `softcap` and `sink` as cached_attention has them."""
+        return DeviceOp._seq(abi.OP_PAGED_ATTENTION, [dst, q, pages, page_table, table, sink], DeviceOp._words(q_col, dst_col, sink_off),
+                             DeviceOp._words(B, H, G, dk, dv, q_rs, dst_rs or dst_col + H * dv, page_tokens, most, window, sink_wdt), [scale, softcap])
+
+    @staticmethod
+    def page_read(dst, pages, page_table, table, B, G, dk, dv, page_tokens, most, k_col=0, v_col=None, dst_rs=0):
+        """The cache rows at the rows' positions, as numbers: keys from column `k_col`, values from `v_col` (behind the keys) of each row of dst."""
+        v_col = k_col + G * dk if v_col is None else v_col
+        return DeviceOp._seq(abi.OP_PAGE_READ, [dst, pages, page_table, table], DeviceOp._words(k_col, v_col), DeviceOp._words(B, G, dk, dv, dst_rs or max(k_col + G * dk, v_col + G * dv), page_tokens, most))
+
+    @staticmethod
+    def page_copy(pages, moves, B, page_words):
+        """Copies of whole pages inside their pool, at most `B` of them: the moves of host/pages.py's `page_moves`."""
+        return DeviceOp._seq(abi.OP_PAGE_COPY, [pages, moves], [], DeviceOp._words(B, page_words))
+
+    @staticmethod
+    def sample(dst, logits, table, B, V, probability=None, dst_off=0, logits_off=0, logits_rs=0, probability_off=0):
+        """The next token (int32) of every row of logits by the row's temperature, top_k, top_p, min_p and random number (host/batch.py `sample_table`), and the probability
+        that it had among the tokens that stayed."""
+        return DeviceOp._seq(abi.OP_SAMPLE, [dst, logits, table, probability], DeviceOp._words(dst_off, logits_off, probability_off), DeviceOp._words(B, V, logits_rs or V))
+
 
 @dataclass
 class ProgramIO:  # reference src/backend.zig:252-257 (offset/size in bytes)

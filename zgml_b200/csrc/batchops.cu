@@ -1,5 +1,5 @@
 // Sequence-model DeviceOps of a step that advances many requests at once (parameter packs in include/zgml_cuda.h): BATCH_APPEND and LOGIT_RULES;
-// SHARED_ATTENTION and ADAPTER_LINEAR have files of their own.  What distinguishes the rows - slot, length, adapter, rules - lies in a table that the host rewrites between
+// SHARED_ATTENTION, ADAPTER_LINEAR, SAMPLE and the ops over pages have files of their own.  What distinguishes the rows - slot, length, adapter, rules - lies in a table that the host rewrites between
 // executions of one captured program.
 #include "batch_table.cuh"
 
@@ -261,12 +261,21 @@ bool zg_batch_op_valid(const ZgOp& op, const size_t* elems, size_t n_bufs, char*
             if (s.buf[0] == s.buf[1] && (s.off[0] != s.off[1] || srs != drs)) return fail("logit_rules: logits that overlap the destination have to be the destination");
             return true;
         }
-        default: return fail("not a sequence op");
+        case ZG_OP_PAGED_ATTENTION: return zg_paged_attention_valid(s, elems, n_bufs, why, why_n);
+        case ZG_OP_SAMPLE: return zg_sample_valid(s, elems, n_bufs, why, why_n);
+        default: return zg_page_op_valid(op, elems, n_bufs, why, why_n);
     }
 }
-uint32_t zg_batch_op_writes(uint32_t tag) { return tag == ZG_OP_BATCH_APPEND ? 1u | (1u << 4) : 1u; }      // the cache and the turned query heads
+uint32_t zg_batch_op_writes(uint32_t tag) {
+    return tag == ZG_OP_BATCH_APPEND ? 1u | (1u << 4) : tag == ZG_OP_PAGE_APPEND ? 1u | (1u << 5) : tag == ZG_OP_SAMPLE ? 1u | (1u << 3) : 1u;      // (the turned query heads, the probabilities)
+}
 size_t zg_batch_op_scratch_elems(const ZgOp& op) {
-    return op.tag == ZG_OP_SHARED_ATTENTION ? zg_shared_attention_scratch_elems(op.u.seq) : op.tag == ZG_OP_ADAPTER_LINEAR ? zg_adapter_linear_scratch_elems(op.u.seq) : 0;
+    switch (op.tag) {
+        case ZG_OP_SHARED_ATTENTION: return zg_shared_attention_scratch_elems(op.u.seq);
+        case ZG_OP_ADAPTER_LINEAR: return zg_adapter_linear_scratch_elems(op.u.seq);
+        case ZG_OP_PAGED_ATTENTION: return zg_paged_attention_scratch_elems(op.u.seq);
+        default: return 0;
+    }
 }
 
 bool zg_launch_batch_op(const ZgOp& op, float* const* bufs, const size_t* elems, float* scratch, cudaStream_t st) {
@@ -320,6 +329,8 @@ bool zg_launch_batch_op(const ZgOp& op, float* const* bufs, const size_t* elems,
             ZG_SEQ_CHECK();
             return true;
         }
-        default: zg_set_error("not a sequence op"); return false;
+        case ZG_OP_PAGED_ATTENTION: return zg_launch_paged_attention(op, bufs, elems, scratch, st);
+        case ZG_OP_SAMPLE: return zg_launch_sample(op, bufs, st);
+        default: return zg_launch_page_op(op, bufs, elems, st);
     }
 }

@@ -501,7 +501,7 @@ bool zg_dense_gemm_batched_launch(const void* w_bf16, const float* src, float* d
 // streamops.cu : ZG_OP_STREAM_STEP
 bool zg_stream_op_valid(const ZgOp& op, const size_t* elems, size_t n_bufs, char* why, size_t why_n);
 bool zg_launch_stream_op(const ZgOp& op, float* const* bufs, cudaStream_t st, bool const_weights);
-// batchops.cu : ZG_OP_BATCH_APPEND .. ZG_OP_LOGIT_RULES, reached through the functions above; shared_attention.cu : ZG_OP_SHARED_ATTENTION; adapter.cu : ZG_OP_ADAPTER_LINEAR
+// batchops.cu : ZG_OP_BATCH_APPEND .. ZG_OP_SAMPLE, reached through the functions above; shared_attention.cu : ZG_OP_SHARED_ATTENTION; adapter.cu : ZG_OP_ADAPTER_LINEAR
 bool zg_batch_op_valid(const ZgOp& op, const size_t* elems, size_t n_bufs, char* why, size_t why_n);
 uint32_t zg_batch_op_writes(uint32_t tag);
 size_t zg_batch_op_scratch_elems(const ZgOp& op);
@@ -514,3 +514,11 @@ bool zg_adapter_linear_valid(const ZgSeqOp& s, const size_t* elems, size_t n_buf
 size_t zg_adapter_linear_scratch_elems(const ZgSeqOp& s);
 bool zg_launch_adapter_linear(const ZgOp& op, float* const* bufs, float* scratch, cudaStream_t st);
 unsigned int zg_adapter_timeouts();
+// pageops.cu : ZG_OP_PAGE_APPEND, ZG_OP_PAGE_READ, ZG_OP_PAGE_COPY; paged_attention.cu : ZG_OP_PAGED_ATTENTION; sample.cu : ZG_OP_SAMPLE (reached through zg_batch_op_*)
+bool zg_page_op_valid(const ZgOp& op, const size_t* elems, size_t n_bufs, char* why, size_t why_n);
+bool zg_launch_page_op(const ZgOp& op, float* const* bufs, const size_t* elems, cudaStream_t st);
+bool zg_paged_attention_valid(const ZgSeqOp& s, const size_t* elems, size_t n_bufs, char* why, size_t why_n);
+size_t zg_paged_attention_scratch_elems(const ZgSeqOp& s);
+bool zg_launch_paged_attention(const ZgOp& op, float* const* bufs, const size_t* elems, float* scratch, cudaStream_t st);
+bool zg_sample_valid(const ZgSeqOp& s, const size_t* elems, size_t n_bufs, char* why, size_t why_n);
+bool zg_launch_sample(const ZgOp& op, float* const* bufs, cudaStream_t st);

@@ -1,4 +1,4 @@
-"""Tables of the ops that advance many requests in one step (BATCH_APPEND, SHARED_ATTENTION, ADAPTER_LINEAR, LOGIT_RULES): what tells the rows apart, as the
+"""Tables of the ops that advance many requests in one step (BATCH_APPEND, SHARED_ATTENTION, ADAPTER_LINEAR, LOGIT_RULES, SAMPLE and the ops over pages): what tells the rows apart, as the
 words that a program's table buffer is given before every execution.  The kernels check every word once more before it becomes an address; what is
 refused here would come back as rows of NaN."""
 from dataclasses import dataclass, field
@@ -126,3 +126,46 @@ def rule_table(rules: Sequence[LogitRules], slots: Sequence[int], lengths: Seque
         bias[:, 0] = [k for k, _ in entries]
         bias[:, 1] = np.array([v for _, v in entries], np.float32).view(np.int32)
     return t, bias, np.stack(masks) if masks else np.zeros((0, (vocab + 31) // 32), np.int32)
+
+
+@dataclass(frozen=True)
+class TokenChoice:
+    """How a request's next token is drawn: of the softmax of logits / temperature the `top_k` likeliest tokens stay (0: all), of those the fewest whose probability reaches
+    `top_p` of theirs, of those the ones with at least `min_p` times the likeliest one's.  Temperature 0: the likeliest token."""
+    temperature: float = 1.0
+    top_k: int = 0
+    top_p: float = 1.0
+    min_p: float = 0.0
+
+    def __post_init__(self):
+        with np.errstate(over="ignore", under="ignore"):            # (what they are to the kernel)
+            temperature, top_p, min_p = (np.float32(x) for x in (self.temperature, self.top_p, self.min_p))
+        if not (np.isfinite(temperature) and temperature >= 0.0):
+            raise ValueError("a temperature is a finite number, zero or more")
+        if not (0.0 <= top_p <= 1.0 and 0.0 <= min_p <= 1.0):
+            raise ValueError("top_p and min_p are probabilities")
+        if not isinstance(self.top_k, (int, np.integer)) or not 0 <= self.top_k < 1 << 31:
+            raise ValueError("top_k is a whole number, zero or more")
+
+
+def sample_words(rows: int) -> int:
+    return abi.BATCH_ROWS + abi.SAMPLE_WORDS * rows
+
+
+def sample_table(choices: Sequence[Optional[TokenChoice]], draws: Sequence[float], rows: int) -> np.ndarray:
+    """The table of a SAMPLE of `rows` rows of logits: a choice (None: the row is idle) and a random number of [0, 1) for each of the first ones, rounded to f32 below 1."""
+    if len(choices) != len(draws) or len(choices) > rows:
+        raise ValueError(f"{len(choices)} choices and {len(draws)} random numbers for a step of {rows}")
+    t = np.zeros(sample_words(rows), np.int32)
+    t[0] = len(choices)
+    body = t[abi.BATCH_ROWS:].reshape(rows, abi.SAMPLE_WORDS)
+    for i, (c, u) in enumerate(zip(choices, draws)):
+        if not 0.0 <= u < 1.0:
+            raise ValueError(f"row {i}: {u} as a random number of [0, 1)")
+        if c is None:
+            body[i, 1] = -1
+            continue
+        u = min(np.float32(u), np.nextafter(np.float32(1.0), np.float32(0.0)))
+        body[i, [0, 2, 3, 4]] = np.array([c.temperature, c.top_p, c.min_p, u], np.float32).view(np.int32)
+        body[i, 1] = c.top_k
+    return t

@@ -288,9 +288,8 @@ def prepare(case, seed):
     if own:                                      # compiled once, executed every step; caches are kept as pages
         given = {k: t for k, t in tensors.items() if k not in ("keys", "values", "scales", "written")}
         if kind in ("append", "attend"):
-            given["pages"] = _packed(case, tensors)
-            for k in ("keys", "values", "scales"):
-                tensors[k] = None
+            tensors = {**{k: t for k, t in tensors.items() if k not in ("keys", "values", "scales")}, "pages": _packed(case, tensors)}
+            given["pages"] = tensors["pages"]
         sizes = dict(case, read=(given["read"].numel() - HEAD) // ROW) if kind == "append" else case
         torch.cuda.synchronize()
         program = _Program(lambda at: globals()["_ops_" + kind](sizes, at), given)

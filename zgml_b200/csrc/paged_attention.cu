@@ -1,5 +1,14 @@
 // PAGED_ATTENTION (parameter pack in include/zgml_cuda.h): softmax attention of the rows of a step over the 8-bit pages of their sequences.
+//
+// Both products run on the tensor cores with operands that hold what f32 would: codes are whole numbers of 8 bits and exact in half precision, a query (scaled so that its
+// largest element is in [2^14, 2^15)) and a weight (of [0, 2^14]) are the sum of two halves, 22 to 24 bits of what lies within 2^-18 of the largest.  The two halves of eight
+// queries are the sixteen rows of one matrix instruction, so a step of few queries fills it.  Scales are powers of two: a key's joins its scores, a value's its weights, exactly.
+// A weight is 2^(s + e - n), with the score s in powers of two, e the exponent of its value's scale and n a whole number not below any s + e so far, so that the largest
+// contributions keep their bits whatever the pages' scales are; the sum of the softmax has a frame m of its own, and the quotient is put right by 2^(n - m).
 #include "pages.cuh"
+#include "exp2.cuh"
+
+#include <cuda_fp16.h>
 
 #include <algorithm>
 
@@ -8,55 +17,328 @@ namespace {
 struct PgArgs {
     PagePool pool; PageShape s;
     float* dst; const float* q; const float* table; const void* sink;
-    uint32_t B, H, rep, q_rs, dst_rs, window, sink_bf16;
+    uint32_t B, H, rep, q_rs, dst_rs, window, sink_bf16, tokens, chunks;      // tokens of a sequence a CTA takes together, chunks of a key head's query heads
     float scale, cap;
 };
-constexpr uint32_t kPgWarps = 8;
+constexpr uint32_t kPgWarps = 4, kPgStages = 3, kPgTile = 32, kPgShift = 14;
 __device__ __forceinline__ float pg_sink(const PgArgs& a, uint32_t h) { return a.sink_bf16 ? __bfloat162float(reinterpret_cast<const bf16*>(a.sink)[h]) : reinterpret_cast<const float*>(a.sink)[h]; }
+__device__ __forceinline__ uint32_t pg_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+// 2^d of a whole number d, 0 below 2^-126
+__device__ __forceinline__ float pg_pow2(float d) { return d < -126.0f ? 0.0f : __int_as_float(((int)fminf(d, 127.0f) + 127) << 23); }
+// two of a word's four codes, as halves: 1024 + x by its bits, minus 1024 + 128
+__device__ __forceinline__ uint32_t pg_codes(uint32_t w, uint32_t which) {
+    const uint32_t x = __byte_perm(w, 0x64646464u, which);
+    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&x), __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void pg_split(float x, float y, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h); lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+__device__ __forceinline__ void pg_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void pg_copy16(uint32_t to, const uint8_t* from, bool on) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(on ? 16 : 0) : "memory"); }
+__device__ __forceinline__ float pg_remote(const float* p, uint32_t rank) {
+    uint32_t at;
+    float v;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(pg_smem(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ void pg_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 
-// CTA (query head, row): a warp per token, the warps' tokens interleaved, one running maximum and sum a warp.
-__global__ void __launch_bounds__(32 * kPgWarps) k_paged_rows(const PgArgs a) {
+// CTA (share of the positions; key head and chunk of its query heads; row that begins a group of rows of one sequence).  A warp takes every kPgWarps-th tile of 32 positions of
+// the share through a ring of its own of kPgStages copied tiles, so that warps wait for nothing but their own copies.  8 MT queries a CTA.
+template <int KC, int VC, int MT>
+__global__ void __launch_bounds__(32 * kPgWarps) k_paged(const __grid_constant__ PgArgs a) {
     pdl_enter();
-    __shared__ float q[256], acc[kPgWarps][256], m_[kPgWarps], l_[kPgWarps];
-    const uint32_t h = blockIdx.x, r = blockIdx.y, warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = h / a.rep;
+    extern __shared__ float4 pg_mem[];
+    __shared__ float stats[kPgWarps][8 * MT][3], joined[8 * MT][3], factor[8 * MT][2];      // m, n, sum
     const PageShape& s = a.s;
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, row8 = lane / 4, j = lane % 4;
+    const uint32_t r = blockIdx.z, g = blockIdx.y / a.chunks, chunk = blockIdx.y % a.chunks, splits = gridDim.x, split = blockIdx.x;
     const BatchHead head = batch_head(a.table, a.B);
     const BatchRow w = batch_row(a.table, r);
     if (r >= head.rows || w.slot < 0) return;
-    const bool ok = page_row_ok(a.pool, s, w);
-    for (uint32_t d = threadIdx.x; d < s.dk; d += blockDim.x) q[d] = a.q[(size_t)r * a.q_rs + h * s.dk + d] * a.scale;
+    uint32_t group = 1;                                              // rows from r on that this CTA takes
+    if (a.tokens > 1) {
+        uint32_t back = 0;                                           // rows of the same slot directly before r
+        for (bool more = true; more;) {
+            const uint32_t i = back + lane;
+            const bool same = i < r && batch_row(a.table, r - 1 - i).slot == w.slot;
+            const uint32_t other = ~__ballot_sync(0xffffffffu, same);
+            back += other ? __ffs(other) - 1 : 32;
+            more = !other;
+        }
+        if (back % a.tokens) return;
+        const bool same = lane > 0 && lane < a.tokens && r + lane < head.rows && batch_row(a.table, r + lane).slot == w.slot;
+        group = min(a.tokens, (uint32_t)__ffs(~(__ballot_sync(0xffffffffu, same) | 1u)) - 1);
+    }
+    const uint32_t heads = min(a.rep, 8u * MT);                      // of a chunk
+    // the lane's queries: what they see, and their halves
+    uint32_t len[MT], low[MT], all_lo = 0xffffffffu, all_hi = 0;
+    uint32_t qf[MT][2 * KC][4];
+    float q_scale[MT];
+#pragma unroll
+    for (int t = 0; t < MT; t++) {
+        const uint32_t i = 8 * t + row8, token = i / heads, h = chunk * heads + i % heads;
+        const bool on = token < group && h < a.rep;
+        len[t] = low[t] = 0;
+        if (on) {
+            const BatchRow x = batch_row(a.table, r + token);
+            if (page_row_ok(a.pool, s, x)) { len[t] = x.length; low[t] = a.window && len[t] > a.window ? len[t] - a.window : 0; }
+        }
+        if (len[t]) { all_lo = min(all_lo, low[t]); all_hi = max(all_hi, len[t]); }
+        const float* q = a.q + (size_t)(r + (on ? token : 0)) * a.q_rs + (g * a.rep + (on ? h : 0)) * s.dk;
+        float x[KC][8];
+        uint32_t top = 0;
+#pragma unroll
+        for (int c = 0; c < KC; c++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const uint32_t d = 32 * c + 8 * j + e;
+                x[c][e] = on && d < s.dk ? q[d] : 0.0f;
+                top = max(top, __float_as_uint(fabsf(x[c][e])));
+            }
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const uint32_t e = top ? max(top >> 23, 15u) : 141u;         // its exponent
+        const float f = __uint_as_float((268u - e) << 23);           // 2^14 / 2^(e - 127)
+        q_scale[t] = __uint_as_float((e - 14u) << 23) * a.scale * (a.cap > 0.0f ? 1.0f : kLog2e);
+#pragma unroll
+        for (int c = 0; c < KC; c++)
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                pg_split(x[c][4 * k] * f, x[c][4 * k + 1] * f, qf[t][2 * c + k][0], qf[t][2 * c + k][1]);
+                pg_split(x[c][4 * k + 2] * f, x[c][4 * k + 3] * f, qf[t][2 * c + k][2], qf[t][2 * c + k][3]);
+            }
+    }
+    all_lo = __reduce_min_sync(0xffffffffu, all_lo);
+    all_hi = __reduce_max_sync(0xffffffffu, all_hi);
+    // this CTA's tiles
+    const uint32_t first = all_hi ? all_lo / kPgTile : 0, tiles = all_hi ? (all_hi + kPgTile - 1) / kPgTile - first : 0;
+    const uint32_t t0 = first + (uint32_t)((uint64_t)tiles * split / splits), t1 = first + (uint32_t)((uint64_t)tiles * (split + 1) / splits);
+    const uint32_t k_bytes = kPgTile * s.kp, stage_bytes = k_bytes + kPgTile * s.vp + 32, kc = s.kp / 32, vc = s.vp / 16;
+    uint8_t* const ring = reinterpret_cast<uint8_t*>(pg_mem) + (size_t)warp * kPgStages * stage_bytes;
+    const uint32_t pages = (all_hi + s.page - 1) >> s.shift;
+    // the page of half `lane & 1` of a tile: its id, -1 for one that does not exist, -2 behind the last one that a row sees
+    auto find = [&](uint32_t tile) {
+        if (tile >= t1) return -2;
+        const uint32_t n = (tile * kPgTile + 16 * (lane & 1)) >> s.shift;
+        return n < pages ? page_id(a.pool, w.slot, n) : -2;
+    };
+    auto fetch = [&](uint32_t tile, int32_t id, uint32_t stage) {
+        uint8_t* const at = ring + (size_t)stage * stage_bytes;
+        const uint32_t to = pg_smem(at);
+#pragma unroll
+        for (uint32_t u = 0; u < 2; u++) {
+            const int32_t page = __shfl_sync(0xffffffffu, id, u);
+            const uint32_t in = (tile * kPgTile + 16 * u) & (s.page - 1);
+            const uint8_t* part = a.pool.pages + (size_t)max(page, 0) * page_bytes(s) + (size_t)g * s.head;
+            const uint8_t* k = part + kPageHead + in * s.kp;
+            const uint8_t* v = part + kPageHead + s.page * s.kp + in * s.vp;
+            for (uint32_t i = lane; i < s.kp; i += 32) pg_copy16(to + 16 * (u * s.kp + i), k + 16 * i, page >= 0);
+            for (uint32_t i = lane; i < s.vp; i += 32) pg_copy16(to + k_bytes + 16 * (u * s.vp + i), v + 16 * i, page >= 0);
+            if (lane == 0) {
+                const uint32_t scales = to + k_bytes + kPgTile * s.vp + 8 * u;
+                if (page >= 0) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(scales), "l"(part) : "memory");
+                else *reinterpret_cast<float2*>(at + k_bytes + kPgTile * s.vp + 8 * u) = page == -1 ? make_float2(kBatchNaN, kBatchNaN) : make_float2(1.0f, 1.0f);
+            }
+        }
+    };
+    float m[MT], n[MT], sum[MT], o[MT][VC][4];
+#pragma unroll
+    for (int t = 0; t < MT; t++) {
+        m[t] = n[t] = -INFINITY; sum[t] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < VC; c++) { o[t][c][0] = o[t][c][1] = o[t][c][2] = o[t][c][3] = 0.0f; }
+    }
+    const float inv_cap = a.cap > 0.0f ? 1.0f / a.cap : 0.0f;
+    int32_t id = find(t0 + warp);
+#pragma unroll
+    for (uint32_t i = 0; i < kPgStages - 1; i++) {
+        if (t0 + warp + i * kPgWarps < t1) fetch(t0 + warp + i * kPgWarps, id, i);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        id = find(t0 + warp + (i + 1) * kPgWarps);
+    }
+    uint32_t stage = 0;
+    for (uint32_t tile = t0 + warp; tile < t1; tile += kPgWarps) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kPgStages - 2) : "memory");
+        __syncwarp();
+        {
+            const uint32_t next = tile + (kPgStages - 1) * kPgWarps;
+            if (next < t1) fetch(next, id, stage == 0 ? kPgStages - 1 : stage - 1);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            id = find(next + kPgWarps);
+        }
+        const uint8_t* const at = ring + (size_t)stage * stage_bytes;
+        stage = stage + 1 == kPgStages ? 0 : stage + 1;
+        const float4 scales = *reinterpret_cast<const float4*>(at + k_bytes + kPgTile * s.vp);      // of keys and values of each half
+        // scores: eight positions a step, of which a lane holds two of each query
+        float sc[MT][4][2];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            float acc[MT][4];
+#pragma unroll
+            for (int t = 0; t < MT; t++) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < KC; c++) {
+                if (c >= kc) break;
+                const uint2 x = *reinterpret_cast<const uint2*>(at + (i * kc + c) * 256 + 8 * lane);
+                const uint32_t b0 = pg_codes(x.x, 0x4140), b1 = pg_codes(x.x, 0x4342), b2 = pg_codes(x.y, 0x4140), b3 = pg_codes(x.y, 0x4342);
+#pragma unroll
+                for (int t = 0; t < MT; t++) { pg_mma(acc[t], qf[t][2 * c], b0, b1); pg_mma(acc[t], qf[t][2 * c + 1], b2, b3); }
+            }
+#pragma unroll
+            for (int t = 0; t < MT; t++) {
+                sc[t][i][0] = (acc[t][0] + acc[t][2]) * q_scale[t] * (i < 2 ? scales.x : scales.z);
+                sc[t][i][1] = (acc[t][1] + acc[t][3]) * q_scale[t] * (i < 2 ? scales.x : scales.z);
+            }
+        }
+        // weights
+        const float e0 = scales.y == scales.y ? (float)((int)(__float_as_uint(scales.y) >> 23) - 127) : kBatchNaN, e1 = scales.w == scales.w ? (float)((int)(__float_as_uint(scales.w) >> 23) - 127) : kBatchNaN;
+        uint32_t pf[MT][2][4];
+        float alpha[MT];
+#pragma unroll
+        for (int t = 0; t < MT; t++) {
+            float top0 = -INFINITY, top1 = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    const uint32_t p = tile * kPgTile + 8 * i + 2 * j + k;
+                    float x = sc[t][i][k];
+                    if (a.cap > 0.0f) x = sa_capped(x, a.cap, inv_cap) * kLog2e;
+                    x = p < len[t] && p >= low[t] ? x : -INFINITY;
+                    sc[t][i][k] = x;
+                    if (i < 2) top0 = fmaxf(top0, x); else top1 = fmaxf(top1, x);
+                }
+            top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, 1)); top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, 1));
+            top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, 2)); top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, 2));
+            const float new_m = fmaxf(m[t], ceilf(fmaxf(top0, top1))), new_n = fmaxf(n[t], ceilf(fmaxf(top0 + e0, top1 + e1)));
+            sum[t] *= new_m == m[t] ? 1.0f : pg_pow2(m[t] - new_m);
+            alpha[t] = new_n == n[t] ? 1.0f : pg_pow2(n[t] - new_n);
+            m[t] = new_m; n[t] = new_n;
+            const float fm = new_m == -INFINITY ? 0.0f : new_m, fn = (float)kPgShift - (new_n == -INFINITY ? 0.0f : new_n);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float e = fn + (i < 2 ? e0 : e1), x = sc[t][i][0], y = sc[t][i][1];
+                sum[t] += sa_ex2(x - fm) + sa_ex2(y - fm);
+                pg_split(x == -INFINITY ? 0.0f : sa_ex2(x + e), y == -INFINITY ? 0.0f : sa_ex2(y + e), pf[t][i / 2][2 * (i % 2)], pf[t][i / 2][2 * (i % 2) + 1]);
+            }
+        }
+        // outputs: sums over the tile join the running ones rounded (the tensor cores cut theirs)
+#pragma unroll
+        for (int c = 0; c < VC; c++) {
+            if (c >= vc) break;
+            float acc[MT][2][4];
+#pragma unroll
+            for (int t = 0; t < MT; t++)
+#pragma unroll
+                for (int k = 0; k < 8; k++) acc[t][k / 4][k % 4] = 0.0f;
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const uint2 x = *reinterpret_cast<const uint2*>(at + k_bytes + (u * vc + c) * 256 + 8 * lane);
+                const uint32_t b0 = pg_codes(x.x, 0x4140), b1 = pg_codes(x.x, 0x4342), b2 = pg_codes(x.y, 0x4140), b3 = pg_codes(x.y, 0x4342);
+#pragma unroll
+                for (int t = 0; t < MT; t++) { pg_mma(acc[t][0], pf[t][u], b0, b1); pg_mma(acc[t][1], pf[t][u], b2, b3); }
+            }
+#pragma unroll
+            for (int t = 0; t < MT; t++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) o[t][c][k] = fmaf(o[t][c][k], alpha[t], acc[t][k / 2][k % 2] + acc[t][k / 2][k % 2 + 2]);
+        }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
-    float m = -INFINITY, l = 0.0f, o[8] = {};
-    bool bad = !ok;
-    const uint32_t length = ok ? w.length : 0, lo = a.window && length > a.window ? length - a.window : 0;
-    for (uint32_t j = lo + warp; j < length; j += kPgWarps) {
-        const uint32_t t = j & (s.page - 1);
-        const int32_t id = page_id(a.pool, w.slot, j >> s.shift);
-        if (id < 0) { bad = true; break; }
-        const uint8_t* part = a.pool.pages + (size_t)id * page_bytes(s) + (size_t)g * s.head;
-        const float2 scale = *reinterpret_cast<const float2*>(part);
-        float dot = 0.0f;
-        for (uint32_t d = lane; d < s.dk; d += 32) dot = fmaf(q[d], ((float)part[key_byte(s, t, d)] - 128.0f) * scale.x, dot);
-        dot = warp_sum(dot);
-        if (a.cap > 0.0f) dot = a.cap * tanhf(dot / a.cap);
-        const float top = fmaxf(m, dot), f = m == -INFINITY ? 0.0f : expf(m - top), p = expf(dot - top);
-        m = top; l = l * f + p;
-        for (uint32_t i = 0, d = lane; d < s.dv; i++, d += 32) o[i] = o[i] * f + p * ((float)part[value_byte(s, t, d)] - 128.0f) * scale.y;
+    // the warps' records join in shared memory, then those of the cluster's CTAs
+    const uint32_t pitch = s.vp + 4;
+    float* const rec = reinterpret_cast<float*>(pg_mem);              // [warps + 1][8 MT][pitch]
+#pragma unroll
+    for (int t = 0; t < MT; t++) {
+        sum[t] += __shfl_xor_sync(0xffffffffu, sum[t], 1);
+        sum[t] += __shfl_xor_sync(0xffffffffu, sum[t], 2);
+        float* const to = rec + (size_t)(warp * 8 * MT + 8 * t + row8) * pitch;
+#pragma unroll
+        for (int c = 0; c < VC; c++) {
+            if (c >= vc) break;
+            *reinterpret_cast<float2*>(to + 16 * c + 2 * j) = make_float2(o[t][c][0], o[t][c][1]);
+            *reinterpret_cast<float2*>(to + 16 * c + 8 + 2 * j) = make_float2(o[t][c][2], o[t][c][3]);
+        }
+        if (j == 0) { stats[warp][8 * t + row8][0] = m[t]; stats[warp][8 * t + row8][1] = n[t]; stats[warp][8 * t + row8][2] = sum[t]; }
     }
-    for (uint32_t i = 0, d = lane; d < s.dv; i++, d += 32) acc[warp][d] = o[i];
-    if (lane == 0) { m_[warp] = m; l_[warp] = l; }
-    bad = __syncthreads_or(bad);
-    float top = -INFINITY, sum = 0.0f;
-    for (uint32_t i = 0; i < kPgWarps; i++) top = fmaxf(top, m_[i]);
-    const bool none = top == -INFINITY && length <= lo;
-    if (a.sink) top = fmaxf(top, pg_sink(a, h));
-    for (uint32_t i = 0; i < kPgWarps; i++) sum += m_[i] == -INFINITY ? l_[i] : l_[i] * expf(m_[i] - top);
-    if (a.sink) sum += expf(pg_sink(a, h) - top);
-    for (uint32_t d = threadIdx.x; d < s.dv; d += blockDim.x) {
-        float v = 0.0f;
-        for (uint32_t i = 0; i < kPgWarps; i++) v += m_[i] == -INFINITY ? acc[i][d] : acc[i][d] * expf(m_[i] - top);
-        a.dst[(size_t)r * a.dst_rs + h * s.dv + d] = bad ? kBatchNaN : none ? 0.0f : v / sum;
+    __syncthreads();
+    auto frame = [](float from, float to) { return from == to ? 1.0f : pg_pow2(from - to); };      // (also where both are infinite)
+    float* const mine = rec + (size_t)kPgWarps * 8 * MT * pitch;
+    const uint32_t queries = group * heads;
+    for (uint32_t x = threadIdx.x; x < queries * s.vp; x += 32 * kPgWarps) {
+        const uint32_t i = x / s.vp, d = x - i * s.vp;
+        float top_m = -INFINITY, top_n = -INFINITY, l = 0.0f, v = 0.0f;
+#pragma unroll
+        for (uint32_t k = 0; k < kPgWarps; k++) { top_m = fmaxf(top_m, stats[k][i][0]); top_n = fmaxf(top_n, stats[k][i][1]); }
+#pragma unroll
+        for (uint32_t k = 0; k < kPgWarps; k++) {
+            l = fmaf(stats[k][i][2], frame(stats[k][i][0], top_m), l);
+            v = fmaf(rec[(k * 8 * MT + i) * pitch + d], frame(stats[k][i][1], top_n), v);
+        }
+        mine[i * pitch + d] = v;
+        if (d == 0) { joined[i][0] = top_m; joined[i][1] = top_n; joined[i][2] = l; }
     }
+    if (splits > 1) pg_cluster_sync(); else __syncthreads();
+    if (threadIdx.x < queries) {                                     // a query's frame over all CTAs, and what its outputs are multiplied by
+        const uint32_t i = threadIdx.x, h = chunk * heads + i % heads;
+        float top_m = -INFINITY, top_n = -INFINITY, l = 0.0f;
+        for (uint32_t k = 0; k < splits; k++) { top_m = fmaxf(top_m, pg_remote(&joined[i][0], k)); top_n = fmaxf(top_n, pg_remote(&joined[i][1], k)); }
+        for (uint32_t k = 0; k < splits; k++) l = fmaf(pg_remote(&joined[i][2], k), frame(pg_remote(&joined[i][0], k), top_m), l);
+        float back = top_n - top_m - (float)kPgShift;
+        if (a.sink && h < a.rep) {
+            const float sink = pg_sink(a, g * a.rep + h) * kLog2e;
+            const float to = fmaxf(top_m, ceilf(sink));              // (a sink far above the scores takes the frame with it)
+            l = l * frame(top_m, to) + (to == -INFINITY ? 0.0f : sa_ex2(sink - to));
+            back += top_m - to;
+        }
+        factor[i][0] = back; factor[i][1] = l;
+    }
+    __syncthreads();
+    const uint32_t share = (s.dv + splits - 1) / splits, d0 = split * share, d1 = min(d0 + share, s.dv);
+    for (uint32_t x = threadIdx.x; d0 < d1 && x < queries * (d1 - d0); x += 32 * kPgWarps) {
+        const uint32_t i = x / (d1 - d0), d = d0 + x - i * (d1 - d0), h = chunk * heads + i % heads, row = r + i / heads;
+        if (h >= a.rep) continue;
+        float top_n = -INFINITY, v = 0.0f;
+        for (uint32_t k = 0; k < splits; k++) top_n = fmaxf(top_n, pg_remote(&joined[i][1], k));
+        for (uint32_t k = 0; k < splits; k++) v = fmaf(pg_remote(mine + i * pitch + d, k), frame(pg_remote(&joined[i][1], k), top_n), v);
+        const BatchRow z = batch_row(a.table, row);
+        const float back = factor[i][0], half = truncf(back * 0.5f);      // (in two steps: the scales of the values may lie anywhere)
+        float out = v / factor[i][1] * exp2f(half) * exp2f(back - half);
+        if (z.length == 0) out = 0.0f;
+        if (!page_row_ok(a.pool, s, z)) out = kBatchNaN;
+        a.dst[(size_t)row * a.dst_rs + (g * a.rep + h) * s.dv + d] = out;
+    }
+    if (splits > 1) pg_cluster_sync();                               // no CTA leaves while its record is read
+}
+
+template <int KC, int VC, int MT>
+bool pg_launch(const PgArgs& a, uint32_t splits, cudaStream_t st) {
+    const size_t ring = (size_t)kPgWarps * kPgStages * (kPgTile * (a.s.kp + a.s.vp) + 32), records = sizeof(float) * (kPgWarps + 1) * 8 * MT * (a.s.vp + 4);
+    constexpr size_t most = std::max<size_t>((size_t)kPgWarps * kPgStages * (kPgTile * (32 * KC + 16 * VC) + 32), sizeof(float) * (kPgWarps + 1) * 8 * MT * (16 * VC + 4));
+    if (!zg_smem_limit<k_paged<KC, VC, MT>>(most)) return false;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(splits, a.s.G * a.chunks, a.B); cfg.blockDim = dim3(32 * kPgWarps); cfg.dynamicSmemBytes = std::max(ring, records); cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = g_zg_pdl ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = splits; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr; cfg.numAttrs = 2;
+    cudaLaunchKernelEx(&cfg, k_paged<KC, VC, MT>, a);
+    return true;
 }
 
 }  // namespace
@@ -84,7 +366,19 @@ bool zg_launch_paged_attention(const ZgOp& op, float* const* bufs, const size_t*
     a.dst = bufs[s.buf[0]] + s.off[1]; a.q = bufs[s.buf[1]] + s.off[0]; a.table = bufs[s.buf[4]];
     a.sink = s.buf[5] == ZG_NO_BUF ? nullptr : a.sink_bf16 ? (const void*)wptr<bf16>(bufs, s.buf[5], s.off[2]) : (const void*)wptr<float>(bufs, s.buf[5], s.off[2]);
     a.scale = s.f[0]; a.cap = s.f[1];
-    launch_pdl(k_paged_rows, dim3(a.H, a.B), dim3(32 * kPgWarps), 0, st, a);
+    const bool narrow = a.s.kp <= 64 && a.s.vp <= 64, wide = a.s.kp > 128 || a.s.vp > 128, two = a.rep > 8 && !wide;
+    const uint32_t queries = two ? 16 : 8;
+    a.chunks = (a.rep + queries - 1) / queries;
+    a.tokens = std::max(1u, queries / a.rep);
+    const uint32_t ctas = a.B * a.s.G * a.chunks, most = std::max<uint32_t>(1, (uint32_t)std::min<uint64_t>(8, ((uint64_t)s.n[8] << a.s.shift) / 256));
+    uint32_t splits = 1;
+    while (splits < most && ctas * splits < 4 * zg_sm_count()) splits *= 2;
+    if (splits > most) splits = most;
+    bool ok;
+    if (narrow) ok = two ? pg_launch<2, 4, 2>(a, splits, st) : pg_launch<2, 4, 1>(a, splits, st);
+    else if (!wide) ok = two ? pg_launch<4, 8, 2>(a, splits, st) : pg_launch<4, 8, 1>(a, splits, st);
+    else ok = pg_launch<8, 16, 1>(a, splits, st);
+    if (!ok) return false;
     ZG_SEQ_CHECK();
     return true;
 }

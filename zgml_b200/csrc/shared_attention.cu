@@ -4,6 +4,7 @@
 // Softmax attention over a set of keys that falls into shares needs a record (m, l, o) per share: the largest score, the sum of exp(s - m) and the sum of
 // exp(s - m) v.  Records of any shares merge into the whole: m = max m_i, l = sum l_i e^(m_i - m), o = sum o_i e^(m_i - m) / l.
 #include "batch_table.cuh"
+#include "exp2.cuh"
 #include "split_tc.cuh"
 
 #include <algorithm>
@@ -86,16 +87,6 @@ __device__ __forceinline__ float4 sa_remote4(const float* p, uint32_t rank) {
 __device__ __forceinline__ void sa_cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ float sa_ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-// cap * tanh(s / cap), from the definition 1 - 2 / (e^2x + 1) and, where that cancels, the series to x^9 (the next term is below 2^-26 of the value there).  Sixteen
-// tanhf of a thread took 3700 clocks a tile.
-__device__ __forceinline__ float sa_capped(float s, float cap, float inv_cap) {
-    const float x = fabsf(s * inv_cap), x2 = x * x;
-    const float series = fmaf(x * x2, fmaf(x2, fmaf(x2, fmaf(x2, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), x);
-    const float far = 1.0f - __fdividef(2.0f, sa_ex2(x * (2.0f * kLog2e)) + 1.0f);
-    return copysignf(cap * (x < 0.25f ? series : x > 10.0f ? 1.0f : far), s);
 }
 __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
     uint32_t ok;

@@ -1,8 +1,8 @@
 // PAGED_ATTENTION (parameter pack in include/zgml_cuda.h): softmax attention of the rows of a step over the 8-bit pages of their sequences.
 //
 // Both products run on the tensor cores with operands that hold what f32 would: codes are whole numbers of 8 bits and exact in half precision, a query (scaled so that its
-// largest element is in [2^14, 2^15)) and a weight (of [0, 2^14]) are the sum of two halves, 22 to 24 bits of what lies within 2^-18 of the largest.  The two halves of eight
-// queries are the sixteen rows of one matrix instruction, so a step of few queries fills it.  Scales are powers of two: a key's joins its scores, a value's its weights, exactly.
+// largest element is in [2^14, 2^15)) and a weight (of [0, 2^14]) are the sum of two halves, 22 to 24 bits of what lies within 2^-18 of the largest.  Codes are the instructions' rows
+// (16 positions, 16 values of a head), the two halves of four queries their eight columns, side by side, so that four queries fill an instruction and a lane adds up what belongs together.  Scales are powers of two: a key's joins its scores, a value's its weights, exactly.
 // A weight is 2^(s + e - n), with the score s in powers of two, e the exponent of its value's scale and n a whole number not below any s + e so far, so that the largest
 // contributions keep their bits whatever the pages' scales are; the sum of the softmax has a frame m of its own, and the quotient is put right by 2^(n - m).
 #include "pages.cuh"
@@ -20,7 +20,7 @@ struct PgArgs {
     uint32_t B, H, rep, q_rs, dst_rs, window, sink_bf16, tokens, chunks;      // tokens of a sequence a CTA takes together, chunks of a key head's query heads
     float scale, cap;
 };
-constexpr uint32_t kPgWarps = 4, kPgStages = 3, kPgTile = 32, kPgShift = 14;
+constexpr uint32_t kPgWarps = 4, kPgStages = 2, kPgTile = 32, kPgShift = 14;
 __device__ __forceinline__ float pg_sink(const PgArgs& a, uint32_t h) { return a.sink_bf16 ? __bfloat162float(reinterpret_cast<const bf16*>(a.sink)[h]) : reinterpret_cast<const float*>(a.sink)[h]; }
 __device__ __forceinline__ uint32_t pg_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 // 2^d of a whole number d, 0 below 2^-126
@@ -55,12 +55,12 @@ __device__ __forceinline__ void pg_cluster_sync() {
 }
 
 // CTA (share of the positions; key head and chunk of its query heads; row that begins a group of rows of one sequence).  A warp takes every kPgWarps-th tile of 32 positions of
-// the share through a ring of its own of kPgStages copied tiles, so that warps wait for nothing but their own copies.  8 MT queries a CTA.
-template <int KC, int VC, int MT>
+// the share through a ring of its own of kPgStages copied tiles, so that warps wait for nothing but their own copies.  4 NT queries a CTA, query 4 t + lane % 4 a lane.
+template <int KC, int VC, int NT>
 __global__ void __launch_bounds__(32 * kPgWarps) k_paged(const __grid_constant__ PgArgs a) {
     pdl_enter();
     extern __shared__ float4 pg_mem[];
-    __shared__ float stats[kPgWarps][8 * MT][3], joined[8 * MT][3], factor[8 * MT][2];      // m, n, sum
+    __shared__ float stats[kPgWarps][4 * NT][3], joined[4 * NT][3], factor[4 * NT][2];      // m, n, sum
     const PageShape& s = a.s;
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, row8 = lane / 4, j = lane % 4;
     const uint32_t r = blockIdx.z, g = blockIdx.y / a.chunks, chunk = blockIdx.y % a.chunks, splits = gridDim.x, split = blockIdx.x;
@@ -81,21 +81,22 @@ __global__ void __launch_bounds__(32 * kPgWarps) k_paged(const __grid_constant__
         const bool same = lane > 0 && lane < a.tokens && r + lane < head.rows && batch_row(a.table, r + lane).slot == w.slot;
         group = min(a.tokens, (uint32_t)__ffs(~(__ballot_sync(0xffffffffu, same) | 1u)) - 1);
     }
-    const uint32_t heads = min(a.rep, 8u * MT);                      // of a chunk
-    // the lane's queries: what they see, and their halves
-    uint32_t len[MT], low[MT], all_lo = 0xffffffffu, all_hi = 0;
-    uint32_t qf[MT][2 * KC][4];
-    float q_scale[MT];
+    const uint32_t heads = min(a.rep, 4u * NT);                      // of a chunk
+    // what the lane's queries see, and the halves of the query that its column of the products is (its upper or its lower one)
+    uint32_t len[NT], low[NT], all_lo = 0xffffffffu, all_hi = 0;
+    uint32_t qf[NT][2 * KC][2];
+    float q_scale[NT];
 #pragma unroll
-    for (int t = 0; t < MT; t++) {
-        const uint32_t i = 8 * t + row8, token = i / heads, h = chunk * heads + i % heads;
-        const bool on = token < group && h < a.rep;
+    for (int t = 0; t < NT; t++) {
         len[t] = low[t] = 0;
-        if (on) {
-            const BatchRow x = batch_row(a.table, r + token);
+        const uint32_t mine = 4 * t + j;
+        if (mine / heads < group && chunk * heads + mine % heads < a.rep) {
+            const BatchRow x = batch_row(a.table, r + mine / heads);
             if (page_row_ok(a.pool, s, x)) { len[t] = x.length; low[t] = a.window && len[t] > a.window ? len[t] - a.window : 0; }
         }
         if (len[t]) { all_lo = min(all_lo, low[t]); all_hi = max(all_hi, len[t]); }
+        const uint32_t i = 4 * t + row8 / 2, token = i / heads, h = chunk * heads + i % heads;
+        const bool on = token < group && h < a.rep;
         const float* q = a.q + (size_t)(r + (on ? token : 0)) * a.q_rs + (g * a.rep + (on ? h : 0)) * s.dk;
         float x[KC][8];
         uint32_t top = 0;
@@ -111,13 +112,14 @@ __global__ void __launch_bounds__(32 * kPgWarps) k_paged(const __grid_constant__
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const uint32_t e = top ? max(top >> 23, 15u) : 141u;         // its exponent
         const float f = __uint_as_float((268u - e) << 23);           // 2^14 / 2^(e - 127)
-        q_scale[t] = __uint_as_float((e - 14u) << 23) * a.scale * (a.cap > 0.0f ? 1.0f : kLog2e);
+        q_scale[t] = __shfl_sync(0xffffffffu, __uint_as_float((e - 14u) << 23), 8 * j) * a.scale * (a.cap > 0.0f ? 1.0f : kLog2e);      // (of the lane's scores)
 #pragma unroll
         for (int c = 0; c < KC; c++)
 #pragma unroll
-            for (int k = 0; k < 2; k++) {
-                pg_split(x[c][4 * k] * f, x[c][4 * k + 1] * f, qf[t][2 * c + k][0], qf[t][2 * c + k][1]);
-                pg_split(x[c][4 * k + 2] * f, x[c][4 * k + 3] * f, qf[t][2 * c + k][2], qf[t][2 * c + k][3]);
+            for (int k = 0; k < 4; k++) {
+                uint32_t hi, lo;
+                pg_split(x[c][2 * k] * f, x[c][2 * k + 1] * f, hi, lo);
+                qf[t][2 * c + k / 2][k % 2] = row8 & 1 ? lo : hi;
             }
     }
     all_lo = __reduce_min_sync(0xffffffffu, all_lo);
@@ -136,29 +138,30 @@ __global__ void __launch_bounds__(32 * kPgWarps) k_paged(const __grid_constant__
     };
     auto fetch = [&](uint32_t tile, int32_t id, uint32_t stage) {
         uint8_t* const at = ring + (size_t)stage * stage_bytes;
-        const uint32_t to = pg_smem(at);
 #pragma unroll
         for (uint32_t u = 0; u < 2; u++) {
             const int32_t page = __shfl_sync(0xffffffffu, id, u);
-            const uint32_t in = (tile * kPgTile + 16 * u) & (s.page - 1);
+            const uint32_t in = (tile * kPgTile + 16 * u) & (s.page - 1), to = pg_smem(at) + u * 16 * s.kp + 16 * lane, to_v = pg_smem(at) + k_bytes + u * 16 * s.vp + 16 * lane;
             const uint8_t* part = a.pool.pages + (size_t)max(page, 0) * page_bytes(s) + (size_t)g * s.head;
-            const uint8_t* k = part + kPageHead + in * s.kp;
-            const uint8_t* v = part + kPageHead + s.page * s.kp + in * s.vp;
-            for (uint32_t i = lane; i < s.kp; i += 32) pg_copy16(to + 16 * (u * s.kp + i), k + 16 * i, page >= 0);
-            for (uint32_t i = lane; i < s.vp; i += 32) pg_copy16(to + k_bytes + 16 * (u * s.vp + i), v + 16 * i, page >= 0);
+            const uint8_t* k = part + kPageHead + in * s.kp + 16 * lane;
+            const uint8_t* v = part + kPageHead + s.page * s.kp + in * s.vp + 16 * lane;
+#pragma unroll
+            for (uint32_t i = 0; i < KC; i++) if (i < kc) pg_copy16(to + 512 * i, k + 512 * i, page >= 0);
+#pragma unroll
+            for (uint32_t i = 0; i < VC / 2; i++) if (32 * i + lane < s.vp) pg_copy16(to_v + 512 * i, v + 512 * i, page >= 0);
             if (lane == 0) {
-                const uint32_t scales = to + k_bytes + kPgTile * s.vp + 8 * u;
+                const uint32_t scales = pg_smem(at) + k_bytes + kPgTile * s.vp + 8 * u;
                 if (page >= 0) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(scales), "l"(part) : "memory");
                 else *reinterpret_cast<float2*>(at + k_bytes + kPgTile * s.vp + 8 * u) = page == -1 ? make_float2(kBatchNaN, kBatchNaN) : make_float2(1.0f, 1.0f);
             }
         }
     };
-    float m[MT], n[MT], sum[MT], o[MT][VC][4];
+    float m[NT], n[NT], sum[NT], o[NT][VC][2];
 #pragma unroll
-    for (int t = 0; t < MT; t++) {
+    for (int t = 0; t < NT; t++) {
         m[t] = n[t] = -INFINITY; sum[t] = 0.0f;
 #pragma unroll
-        for (int c = 0; c < VC; c++) { o[t][c][0] = o[t][c][1] = o[t][c][2] = o[t][c][3] = 0.0f; }
+        for (int c = 0; c < VC; c++) o[t][c][0] = o[t][c][1] = 0.0f;
     }
     const float inv_cap = a.cap > 0.0f ? 1.0f / a.cap : 0.0f;
     int32_t id = find(t0 + warp);
@@ -181,102 +184,108 @@ __global__ void __launch_bounds__(32 * kPgWarps) k_paged(const __grid_constant__
         const uint8_t* const at = ring + (size_t)stage * stage_bytes;
         stage = stage + 1 == kPgStages ? 0 : stage + 1;
         const float4 scales = *reinterpret_cast<const float4*>(at + k_bytes + kPgTile * s.vp);      // of keys and values of each half
-        // scores: eight positions a step, of which a lane holds two of each query
-        float sc[MT][4][2];
+        // scores: sixteen positions a step, of which a lane gets two (row8 and row8 + 8) of its query
+        float sc[NT][2][2];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            float acc[MT][4];
+        for (int u = 0; u < 2; u++) {
+            float acc[NT][4];
 #pragma unroll
-            for (int t = 0; t < MT; t++) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.0f;
+            for (int t = 0; t < NT; t++) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.0f;
 #pragma unroll
             for (int c = 0; c < KC; c++) {
                 if (c >= kc) break;
-                const uint2 x = *reinterpret_cast<const uint2*>(at + (i * kc + c) * 256 + 8 * lane);
-                const uint32_t b0 = pg_codes(x.x, 0x4140), b1 = pg_codes(x.x, 0x4342), b2 = pg_codes(x.y, 0x4140), b3 = pg_codes(x.y, 0x4342);
+                const uint2 x = *reinterpret_cast<const uint2*>(at + (2 * u * kc + c) * 256 + 8 * lane), y = *reinterpret_cast<const uint2*>(at + ((2 * u + 1) * kc + c) * 256 + 8 * lane);
+                const uint32_t f0[4] = {pg_codes(x.x, 0x4140), pg_codes(y.x, 0x4140), pg_codes(x.x, 0x4342), pg_codes(y.x, 0x4342)};
+                const uint32_t f1[4] = {pg_codes(x.y, 0x4140), pg_codes(y.y, 0x4140), pg_codes(x.y, 0x4342), pg_codes(y.y, 0x4342)};
 #pragma unroll
-                for (int t = 0; t < MT; t++) { pg_mma(acc[t], qf[t][2 * c], b0, b1); pg_mma(acc[t], qf[t][2 * c + 1], b2, b3); }
+                for (int t = 0; t < NT; t++) { pg_mma(acc[t], f0, qf[t][2 * c][0], qf[t][2 * c][1]); pg_mma(acc[t], f1, qf[t][2 * c + 1][0], qf[t][2 * c + 1][1]); }
             }
+            const float scale = u ? scales.z : scales.x;
 #pragma unroll
-            for (int t = 0; t < MT; t++) {
-                sc[t][i][0] = (acc[t][0] + acc[t][2]) * q_scale[t] * (i < 2 ? scales.x : scales.z);
-                sc[t][i][1] = (acc[t][1] + acc[t][3]) * q_scale[t] * (i < 2 ? scales.x : scales.z);
+            for (int t = 0; t < NT; t++) {
+                sc[t][u][0] = (acc[t][0] + acc[t][1]) * q_scale[t] * scale;
+                sc[t][u][1] = (acc[t][2] + acc[t][3]) * q_scale[t] * scale;
             }
         }
         // weights
-        const float e0 = scales.y == scales.y ? (float)((int)(__float_as_uint(scales.y) >> 23) - 127) : kBatchNaN, e1 = scales.w == scales.w ? (float)((int)(__float_as_uint(scales.w) >> 23) - 127) : kBatchNaN;
-        uint32_t pf[MT][2][4];
-        float alpha[MT];
+        const float e[2] = {scales.y == scales.y ? (float)((int)(__float_as_uint(scales.y) >> 23) - 127) : kBatchNaN, scales.w == scales.w ? (float)((int)(__float_as_uint(scales.w) >> 23) - 127) : kBatchNaN};
+        uint32_t pf[NT][2][2];
+        float alpha[NT];
 #pragma unroll
-        for (int t = 0; t < MT; t++) {
-            float top0 = -INFINITY, top1 = -INFINITY;
+        for (int t = 0; t < NT; t++) {
+            float top[2];
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+            for (int u = 0; u < 2; u++) {
 #pragma unroll
                 for (int k = 0; k < 2; k++) {
-                    const uint32_t p = tile * kPgTile + 8 * i + 2 * j + k;
-                    float x = sc[t][i][k];
+                    const uint32_t p = tile * kPgTile + 16 * u + 8 * k + row8;
+                    float x = sc[t][u][k];
                     if (a.cap > 0.0f) x = sa_capped(x, a.cap, inv_cap) * kLog2e;
-                    x = p < len[t] && p >= low[t] ? x : -INFINITY;
-                    sc[t][i][k] = x;
-                    if (i < 2) top0 = fmaxf(top0, x); else top1 = fmaxf(top1, x);
+                    sc[t][u][k] = p < len[t] && p >= low[t] ? x : -INFINITY;
                 }
-            top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, 1)); top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, 1));
-            top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, 2)); top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, 2));
-            const float new_m = fmaxf(m[t], ceilf(fmaxf(top0, top1))), new_n = fmaxf(n[t], ceilf(fmaxf(top0 + e0, top1 + e1)));
+                top[u] = fmaxf(sc[t][u][0], sc[t][u][1]);
+#pragma unroll
+                for (int k = 4; k < 32; k *= 2) top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], k));
+            }
+            const float new_m = fmaxf(m[t], ceilf(fmaxf(top[0], top[1]))), new_n = fmaxf(n[t], ceilf(fmaxf(top[0] + e[0], top[1] + e[1])));
             sum[t] *= new_m == m[t] ? 1.0f : pg_pow2(m[t] - new_m);
             alpha[t] = new_n == n[t] ? 1.0f : pg_pow2(n[t] - new_n);
             m[t] = new_m; n[t] = new_n;
             const float fm = new_m == -INFINITY ? 0.0f : new_m, fn = (float)kPgShift - (new_n == -INFINITY ? 0.0f : new_n);
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float e = fn + (i < 2 ? e0 : e1), x = sc[t][i][0], y = sc[t][i][1];
-                sum[t] += sa_ex2(x - fm) + sa_ex2(y - fm);
-                pg_split(x == -INFINITY ? 0.0f : sa_ex2(x + e), y == -INFINITY ? 0.0f : sa_ex2(y + e), pf[t][i / 2][2 * (i % 2)], pf[t][i / 2][2 * (i % 2) + 1]);
-            }
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    const float x = sc[t][u][k], y = x == -INFINITY ? 0.0f : sa_ex2(x + (fn + e[u]));
+                    sum[t] += sa_ex2(x - fm);
+                    // the halves side by side, position by position; turned around they are the second product's columns
+                    const __half hi = __float2half_rn(y);
+                    const __half2 both = __halves2half2(hi, __float2half_rn(y - __half2float(hi)));
+                    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(pf[t][u][k]) : "r"(*reinterpret_cast<const uint32_t*>(&both)));
+                }
         }
         // outputs: sums over the tile join the running ones rounded (the tensor cores cut theirs)
 #pragma unroll
         for (int c = 0; c < VC; c++) {
             if (c >= vc) break;
-            float acc[MT][2][4];
+            float acc[NT][4];
 #pragma unroll
-            for (int t = 0; t < MT; t++)
-#pragma unroll
-                for (int k = 0; k < 8; k++) acc[t][k / 4][k % 4] = 0.0f;
+            for (int t = 0; t < NT; t++) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.0f;
 #pragma unroll
             for (int u = 0; u < 2; u++) {
                 const uint2 x = *reinterpret_cast<const uint2*>(at + k_bytes + (u * vc + c) * 256 + 8 * lane);
-                const uint32_t b0 = pg_codes(x.x, 0x4140), b1 = pg_codes(x.x, 0x4342), b2 = pg_codes(x.y, 0x4140), b3 = pg_codes(x.y, 0x4342);
+                const uint32_t f[4] = {pg_codes(x.x, 0x4140), pg_codes(x.y, 0x4140), pg_codes(x.x, 0x4342), pg_codes(x.y, 0x4342)};
 #pragma unroll
-                for (int t = 0; t < MT; t++) { pg_mma(acc[t][0], pf[t][u], b0, b1); pg_mma(acc[t][1], pf[t][u], b2, b3); }
+                for (int t = 0; t < NT; t++) pg_mma(acc[t], f, pf[t][u][0], pf[t][u][1]);
             }
 #pragma unroll
-            for (int t = 0; t < MT; t++)
-#pragma unroll
-                for (int k = 0; k < 4; k++) o[t][c][k] = fmaf(o[t][c][k], alpha[t], acc[t][k / 2][k % 2] + acc[t][k / 2][k % 2 + 2]);
+            for (int t = 0; t < NT; t++) {
+                o[t][c][0] = fmaf(o[t][c][0], alpha[t], acc[t][0] + acc[t][1]);
+                o[t][c][1] = fmaf(o[t][c][1], alpha[t], acc[t][2] + acc[t][3]);
+            }
         }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
     // the warps' records join in shared memory, then those of the cluster's CTAs
     const uint32_t pitch = s.vp + 4;
-    float* const rec = reinterpret_cast<float*>(pg_mem);              // [warps + 1][8 MT][pitch]
+    float* const rec = reinterpret_cast<float*>(pg_mem);              // [warps + 1][4 NT][pitch]
 #pragma unroll
-    for (int t = 0; t < MT; t++) {
-        sum[t] += __shfl_xor_sync(0xffffffffu, sum[t], 1);
-        sum[t] += __shfl_xor_sync(0xffffffffu, sum[t], 2);
-        float* const to = rec + (size_t)(warp * 8 * MT + 8 * t + row8) * pitch;
+    for (int t = 0; t < NT; t++) {
+#pragma unroll
+        for (int k = 4; k < 32; k *= 2) sum[t] += __shfl_xor_sync(0xffffffffu, sum[t], k);
+        float* const to = rec + (size_t)(warp * 4 * NT + 4 * t + j) * pitch;
 #pragma unroll
         for (int c = 0; c < VC; c++) {
             if (c >= vc) break;
-            *reinterpret_cast<float2*>(to + 16 * c + 2 * j) = make_float2(o[t][c][0], o[t][c][1]);
-            *reinterpret_cast<float2*>(to + 16 * c + 8 + 2 * j) = make_float2(o[t][c][2], o[t][c][3]);
+            to[16 * c + row8] = o[t][c][0];
+            to[16 * c + 8 + row8] = o[t][c][1];
         }
-        if (j == 0) { stats[warp][8 * t + row8][0] = m[t]; stats[warp][8 * t + row8][1] = n[t]; stats[warp][8 * t + row8][2] = sum[t]; }
+        if (row8 == 0) { stats[warp][4 * t + j][0] = m[t]; stats[warp][4 * t + j][1] = n[t]; stats[warp][4 * t + j][2] = sum[t]; }
     }
     __syncthreads();
     auto frame = [](float from, float to) { return from == to ? 1.0f : pg_pow2(from - to); };      // (also where both are infinite)
-    float* const mine = rec + (size_t)kPgWarps * 8 * MT * pitch;
+    float* const mine = rec + (size_t)kPgWarps * 4 * NT * pitch;
     const uint32_t queries = group * heads;
     for (uint32_t x = threadIdx.x; x < queries * s.vp; x += 32 * kPgWarps) {
         const uint32_t i = x / s.vp, d = x - i * s.vp;
@@ -286,7 +295,7 @@ __global__ void __launch_bounds__(32 * kPgWarps) k_paged(const __grid_constant__
 #pragma unroll
         for (uint32_t k = 0; k < kPgWarps; k++) {
             l = fmaf(stats[k][i][2], frame(stats[k][i][0], top_m), l);
-            v = fmaf(rec[(k * 8 * MT + i) * pitch + d], frame(stats[k][i][1], top_n), v);
+            v = fmaf(rec[(k * 4 * NT + i) * pitch + d], frame(stats[k][i][1], top_n), v);
         }
         mine[i * pitch + d] = v;
         if (d == 0) { joined[i][0] = top_m; joined[i][1] = top_n; joined[i][2] = l; }
@@ -324,11 +333,11 @@ __global__ void __launch_bounds__(32 * kPgWarps) k_paged(const __grid_constant__
     if (splits > 1) pg_cluster_sync();                               // no CTA leaves while its record is read
 }
 
-template <int KC, int VC, int MT>
+template <int KC, int VC, int NT>
 bool pg_launch(const PgArgs& a, uint32_t splits, cudaStream_t st) {
-    const size_t ring = (size_t)kPgWarps * kPgStages * (kPgTile * (a.s.kp + a.s.vp) + 32), records = sizeof(float) * (kPgWarps + 1) * 8 * MT * (a.s.vp + 4);
-    constexpr size_t most = std::max<size_t>((size_t)kPgWarps * kPgStages * (kPgTile * (32 * KC + 16 * VC) + 32), sizeof(float) * (kPgWarps + 1) * 8 * MT * (16 * VC + 4));
-    if (!zg_smem_limit<k_paged<KC, VC, MT>>(most)) return false;
+    const size_t ring = (size_t)kPgWarps * kPgStages * (kPgTile * (a.s.kp + a.s.vp) + 32), records = sizeof(float) * (kPgWarps + 1) * 4 * NT * (a.s.vp + 4);
+    constexpr size_t most = std::max<size_t>((size_t)kPgWarps * kPgStages * (kPgTile * (32 * KC + 16 * VC) + 32), sizeof(float) * (kPgWarps + 1) * 4 * NT * (16 * VC + 4));
+    if (!zg_smem_limit<k_paged<KC, VC, NT>>(most)) return false;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(splits, a.s.G * a.chunks, a.B); cfg.blockDim = dim3(32 * kPgWarps); cfg.dynamicSmemBytes = std::max(ring, records); cfg.stream = st;
     cudaLaunchAttribute attr[2];
@@ -337,7 +346,7 @@ bool pg_launch(const PgArgs& a, uint32_t splits, cudaStream_t st) {
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = splits; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr; cfg.numAttrs = 2;
-    cudaLaunchKernelEx(&cfg, k_paged<KC, VC, MT>, a);
+    cudaLaunchKernelEx(&cfg, k_paged<KC, VC, NT>, a);
     return true;
 }
 
@@ -366,8 +375,10 @@ bool zg_launch_paged_attention(const ZgOp& op, float* const* bufs, const size_t*
     a.dst = bufs[s.buf[0]] + s.off[1]; a.q = bufs[s.buf[1]] + s.off[0]; a.table = bufs[s.buf[4]];
     a.sink = s.buf[5] == ZG_NO_BUF ? nullptr : a.sink_bf16 ? (const void*)wptr<bf16>(bufs, s.buf[5], s.off[2]) : (const void*)wptr<float>(bufs, s.buf[5], s.off[2]);
     a.scale = s.f[0]; a.cap = s.f[1];
-    const bool narrow = a.s.kp <= 64 && a.s.vp <= 64, wide = a.s.kp > 128 || a.s.vp > 128, two = a.rep > 8 && !wide;
-    const uint32_t queries = two ? 16 : 8;
+    // Queries that a CTA takes together: of one row, or, where the step has more rows than the page table slots, of the rows that a slot has then.
+    const bool narrow = a.s.kp <= 64 && a.s.vp <= 64, wide = a.s.kp > 128 || a.s.vp > 128;
+    const uint64_t together = (uint64_t)a.rep * std::max<uint32_t>(1, a.B / std::max(1u, a.pool.slots));
+    const uint32_t queries = together <= 4 ? 4 : together <= 8 || wide ? 8 : 16;
     a.chunks = (a.rep + queries - 1) / queries;
     a.tokens = std::max(1u, queries / a.rep);
     const uint32_t ctas = a.B * a.s.G * a.chunks, most = std::max<uint32_t>(1, (uint32_t)std::min<uint64_t>(8, ((uint64_t)s.n[8] << a.s.shift) / 256));
@@ -375,9 +386,9 @@ bool zg_launch_paged_attention(const ZgOp& op, float* const* bufs, const size_t*
     while (splits < most && ctas * splits < 4 * zg_sm_count()) splits *= 2;
     if (splits > most) splits = most;
     bool ok;
-    if (narrow) ok = two ? pg_launch<2, 4, 2>(a, splits, st) : pg_launch<2, 4, 1>(a, splits, st);
-    else if (!wide) ok = two ? pg_launch<4, 8, 2>(a, splits, st) : pg_launch<4, 8, 1>(a, splits, st);
-    else ok = pg_launch<8, 16, 1>(a, splits, st);
+    if (narrow) ok = queries == 4 ? pg_launch<2, 4, 1>(a, splits, st) : queries == 8 ? pg_launch<2, 4, 2>(a, splits, st) : pg_launch<2, 4, 4>(a, splits, st);
+    else if (!wide) ok = queries == 4 ? pg_launch<4, 8, 1>(a, splits, st) : queries == 8 ? pg_launch<4, 8, 2>(a, splits, st) : pg_launch<4, 8, 4>(a, splits, st);
+    else ok = queries == 4 ? pg_launch<8, 16, 1>(a, splits, st) : pg_launch<8, 16, 2>(a, splits, st);
     if (!ok) return false;
     ZG_SEQ_CHECK();
     return true;

@@ -1,10 +1,10 @@
 // PAGED_ATTENTION (parameter pack in include/zgml_cuda.h): softmax attention of the rows of a step over the 8-bit pages of their sequences.
 //
 // Both products run on the tensor cores with operands that hold what f32 would: codes are whole numbers of 8 bits and exact in half precision, a query (scaled so that its
-// largest element is in [2^14, 2^15)) and a weight (of [0, 2^14]) are the sum of two halves, 22 to 24 bits of what lies within 2^-18 of the largest.  Codes are the instructions' rows
+// largest element is in [2^14, 2^15)) and a weight (of [0, 2^15]) are the sum of two halves, 22 to 24 bits of what lies within 2^-18 of the largest.  Codes are the instructions' rows
 // (16 positions, 16 values of a head), the two halves of four queries their eight columns, side by side, so that four queries fill an instruction and a lane adds up what belongs together.  Scales are powers of two: a key's joins its scores, a value's its weights, exactly.
-// A weight is 2^(s + e - n), with the score s in powers of two, e the exponent of its value's scale and n a whole number not below any s + e so far, so that the largest
-// contributions keep their bits whatever the pages' scales are; the sum of the softmax has a frame m of its own, and the quotient is put right by 2^(n - m).
+// A weight is 2^(s + e - n), with the score s in powers of two, e the exponent of its value's scale and n a whole number that no s + e so far passes by more than 4, so that the
+// largest contributions keep their bits whatever the pages' scales are; the sum of the softmax has a frame m of its own, and the quotient is put right by 2^(n - m).
 #include "pages.cuh"
 #include "exp2.cuh"
 
@@ -20,7 +20,8 @@ struct PgArgs {
     uint32_t B, H, rep, q_rs, dst_rs, window, sink_bf16, tokens, chunks;      // tokens of a sequence a CTA takes together, chunks of a key head's query heads
     float scale, cap;
 };
-constexpr uint32_t kPgWarps = 4, kPgStages = 2, kPgTile = 32, kPgShift = 14;
+constexpr uint32_t kPgWarps = 4, kPgStages = 2, kPgTile = 32, kPgShift = 11;
+constexpr float kPgSlack = 4.0f;                                     // weights reach 2^(11 + 4)
 __device__ __forceinline__ float pg_sink(const PgArgs& a, uint32_t h) { return a.sink_bf16 ? __bfloat162float(reinterpret_cast<const bf16*>(a.sink)[h]) : reinterpret_cast<const float*>(a.sink)[h]; }
 __device__ __forceinline__ uint32_t pg_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 // 2^d of a whole number d, 0 below 2^-126
@@ -41,7 +42,7 @@ __device__ __forceinline__ void pg_mma(float (&d)[4], const uint32_t (&a)[4], ui
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void pg_copy16(uint32_t to, const uint8_t* from, bool on) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(on ? 16 : 0) : "memory"); }
+__device__ __forceinline__ void pg_copy16(uint32_t to, const uint8_t* from, uint32_t size) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(size) : "memory"); }
 __device__ __forceinline__ float pg_remote(const float* p, uint32_t rank) {
     uint32_t at;
     float v;
@@ -56,7 +57,7 @@ __device__ __forceinline__ void pg_cluster_sync() {
 
 // CTA (share of the positions; key head and chunk of its query heads; row that begins a group of rows of one sequence).  A warp takes every kPgWarps-th tile of 32 positions of
 // the share through a ring of its own of kPgStages copied tiles, so that warps wait for nothing but their own copies.  4 NT queries a CTA, query 4 t + lane % 4 a lane.
-template <int KC, int VC, int NT>
+template <int KC, int VC, int NT, bool FULL>
 __global__ void __launch_bounds__(32 * kPgWarps) k_paged(const __grid_constant__ PgArgs a) {
     pdl_enter();
     extern __shared__ float4 pg_mem[];
@@ -127,7 +128,7 @@ __global__ void __launch_bounds__(32 * kPgWarps) k_paged(const __grid_constant__
     // this CTA's tiles
     const uint32_t first = all_hi ? all_lo / kPgTile : 0, tiles = all_hi ? (all_hi + kPgTile - 1) / kPgTile - first : 0;
     const uint32_t t0 = first + (uint32_t)((uint64_t)tiles * split / splits), t1 = first + (uint32_t)((uint64_t)tiles * (split + 1) / splits);
-    const uint32_t k_bytes = kPgTile * s.kp, stage_bytes = k_bytes + kPgTile * s.vp + 32, kc = s.kp / 32, vc = s.vp / 16;
+    const uint32_t kp = FULL ? 32 * KC : s.kp, vp = FULL ? 16 * VC : s.vp, kc = kp / 32, vc = vp / 16, k_bytes = kPgTile * kp, stage_bytes = k_bytes + kPgTile * vp + 32;
     uint8_t* const ring = reinterpret_cast<uint8_t*>(pg_mem) + (size_t)warp * kPgStages * stage_bytes;
     const uint32_t pages = (all_hi + s.page - 1) >> s.shift;
     // the page of half `lane & 1` of a tile: its id, -1 for one that does not exist, -2 behind the last one that a row sees
@@ -136,33 +137,42 @@ __global__ void __launch_bounds__(32 * kPgWarps) k_paged(const __grid_constant__
         const uint32_t n = (tile * kPgTile + 16 * (lane & 1)) >> s.shift;
         return n < pages ? page_id(a.pool, w.slot, n) : -2;
     };
+    const size_t page_size = page_bytes(s);
+    const uint8_t* const parts = a.pool.pages + (size_t)g * s.head;
     auto fetch = [&](uint32_t tile, int32_t id, uint32_t stage) {
-        uint8_t* const at = ring + (size_t)stage * stage_bytes;
+        uint8_t* const at = ring + stage * stage_bytes;
+        const uint32_t to = pg_smem(at) + 16 * lane;
 #pragma unroll
         for (uint32_t u = 0; u < 2; u++) {
             const int32_t page = __shfl_sync(0xffffffffu, id, u);
-            const uint32_t in = (tile * kPgTile + 16 * u) & (s.page - 1), to = pg_smem(at) + u * 16 * s.kp + 16 * lane, to_v = pg_smem(at) + k_bytes + u * 16 * s.vp + 16 * lane;
-            const uint8_t* part = a.pool.pages + (size_t)max(page, 0) * page_bytes(s) + (size_t)g * s.head;
-            const uint8_t* k = part + kPageHead + in * s.kp + 16 * lane;
-            const uint8_t* v = part + kPageHead + s.page * s.kp + in * s.vp + 16 * lane;
+            const uint32_t in = (tile * kPgTile + 16 * u) & (s.page - 1);
+            const uint8_t* part = parts + (size_t)max(page, 0) * page_size;
+            const uint8_t* k = part + kPageHead + in * kp + 16 * lane;
+            const uint8_t* v = part + kPageHead + s.page * kp + in * vp + 16 * lane;
+            const uint32_t size = page >= 0 ? 16 : 0;
 #pragma unroll
-            for (uint32_t i = 0; i < KC; i++) if (i < kc) pg_copy16(to + 512 * i, k + 512 * i, page >= 0);
+            for (uint32_t i = 0; i < KC; i++) if (FULL || i < kc) pg_copy16(to + u * 16 * kp + 512 * i, k + 512 * i, size);
 #pragma unroll
-            for (uint32_t i = 0; i < VC / 2; i++) if (32 * i + lane < s.vp) pg_copy16(to_v + 512 * i, v + 512 * i, page >= 0);
+            for (uint32_t i = 0; i < VC / 2; i++) if (FULL || 32 * i + lane < vp) pg_copy16(to + k_bytes + u * 16 * vp + 512 * i, v + 512 * i, size);
             if (lane == 0) {
-                const uint32_t scales = pg_smem(at) + k_bytes + kPgTile * s.vp + 8 * u;
+                const uint32_t scales = pg_smem(at) + k_bytes + kPgTile * vp + 8 * u;
                 if (page >= 0) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(scales), "l"(part) : "memory");
-                else *reinterpret_cast<float2*>(at + k_bytes + kPgTile * s.vp + 8 * u) = page == -1 ? make_float2(kBatchNaN, kBatchNaN) : make_float2(1.0f, 1.0f);
+                else *reinterpret_cast<float2*>(at + k_bytes + kPgTile * vp + 8 * u) = page == -1 ? make_float2(kBatchNaN, kBatchNaN) : make_float2(1.0f, 1.0f);
             }
         }
     };
+    // Frames: m of the lane's sum of weights, n of the products' weights.  They stay while no score passes them by much, which one vote of the warp tells.
     float m[NT], n[NT], sum[NT], o[NT][VC][2];
+    uint32_t all_in = 0xffffffffu, least = 0;                        // positions that every query sees
 #pragma unroll
     for (int t = 0; t < NT; t++) {
         m[t] = n[t] = -INFINITY; sum[t] = 0.0f;
+        if (len[t]) { all_in = min(all_in, len[t]); least = max(least, low[t]); }
 #pragma unroll
         for (int c = 0; c < VC; c++) o[t][c][0] = o[t][c][1] = 0.0f;
     }
+    all_in = __reduce_min_sync(0xffffffffu, all_in);
+    least = __reduce_max_sync(0xffffffffu, least);
     const float inv_cap = a.cap > 0.0f ? 1.0f / a.cap : 0.0f;
     int32_t id = find(t0 + warp);
 #pragma unroll
@@ -181,9 +191,10 @@ __global__ void __launch_bounds__(32 * kPgWarps) k_paged(const __grid_constant__
             asm volatile("cp.async.commit_group;" ::: "memory");
             id = find(next + kPgWarps);
         }
-        const uint8_t* const at = ring + (size_t)stage * stage_bytes;
+        const uint8_t* const at = ring + stage * stage_bytes;
+        const uint8_t* const mine = at + 8 * lane;
         stage = stage + 1 == kPgStages ? 0 : stage + 1;
-        const float4 scales = *reinterpret_cast<const float4*>(at + k_bytes + kPgTile * s.vp);      // of keys and values of each half
+        const float4 scales = *reinterpret_cast<const float4*>(at + k_bytes + kPgTile * vp);      // of keys and values of each half
         // scores: sixteen positions a step, of which a lane gets two (row8 and row8 + 8) of its query
         float sc[NT][2][2];
 #pragma unroll
@@ -193,45 +204,61 @@ __global__ void __launch_bounds__(32 * kPgWarps) k_paged(const __grid_constant__
             for (int t = 0; t < NT; t++) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.0f;
 #pragma unroll
             for (int c = 0; c < KC; c++) {
-                if (c >= kc) break;
-                const uint2 x = *reinterpret_cast<const uint2*>(at + (2 * u * kc + c) * 256 + 8 * lane), y = *reinterpret_cast<const uint2*>(at + ((2 * u + 1) * kc + c) * 256 + 8 * lane);
+                if (!FULL && c >= kc) break;
+                const uint2 x = *reinterpret_cast<const uint2*>(mine + (2 * u * kc + c) * 256), y = *reinterpret_cast<const uint2*>(mine + ((2 * u + 1) * kc + c) * 256);
                 const uint32_t f0[4] = {pg_codes(x.x, 0x4140), pg_codes(y.x, 0x4140), pg_codes(x.x, 0x4342), pg_codes(y.x, 0x4342)};
                 const uint32_t f1[4] = {pg_codes(x.y, 0x4140), pg_codes(y.y, 0x4140), pg_codes(x.y, 0x4342), pg_codes(y.y, 0x4342)};
 #pragma unroll
                 for (int t = 0; t < NT; t++) { pg_mma(acc[t], f0, qf[t][2 * c][0], qf[t][2 * c][1]); pg_mma(acc[t], f1, qf[t][2 * c + 1][0], qf[t][2 * c + 1][1]); }
             }
-            const float scale = u ? scales.z : scales.x;
 #pragma unroll
             for (int t = 0; t < NT; t++) {
-                sc[t][u][0] = (acc[t][0] + acc[t][1]) * q_scale[t] * scale;
-                sc[t][u][1] = (acc[t][2] + acc[t][3]) * q_scale[t] * scale;
+                const float scale = q_scale[t] * (u ? scales.z : scales.x);
+                sc[t][u][0] = (acc[t][0] + acc[t][1]) * scale;
+                sc[t][u][1] = (acc[t][2] + acc[t][3]) * scale;
             }
+        }
+        if (a.cap > 0.0f) {
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) sc[t][k / 2][k % 2] = sa_capped(sc[t][k / 2][k % 2], a.cap, inv_cap) * kLog2e;
+        }
+        if (tile * kPgTile < least || tile * kPgTile + kPgTile > all_in) {
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const uint32_t p = tile * kPgTile + 8 * k + row8;
+                    if (p >= len[t] || p < low[t]) sc[t][k / 2][k % 2] = -INFINITY;
+                }
         }
         // weights
         const float e[2] = {scales.y == scales.y ? (float)((int)(__float_as_uint(scales.y) >> 23) - 127) : kBatchNaN, scales.w == scales.w ? (float)((int)(__float_as_uint(scales.w) >> 23) - 127) : kBatchNaN};
-        uint32_t pf[NT][2][2];
-        float alpha[NT];
+        bool over = false;
 #pragma unroll
         for (int t = 0; t < NT; t++) {
-            float top[2];
+            const float top0 = fmaxf(sc[t][0][0], sc[t][0][1]), top1 = fmaxf(sc[t][1][0], sc[t][1][1]);
+            over = over || fmaxf(top0 + e[0], top1 + e[1]) > n[t] + kPgSlack || fmaxf(top0, top1) > m[t] + 64.0f;
+        }
+        if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
+            for (int t = 0; t < NT; t++) {
+                const float top0 = fmaxf(sc[t][0][0], sc[t][0][1]), top1 = fmaxf(sc[t][1][0], sc[t][1][1]), new_m = fmaxf(m[t], ceilf(fmaxf(top0, top1)));
+                float new_n = fmaxf(n[t], ceilf(fmaxf(top0 + e[0], top1 + e[1])));
 #pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    const uint32_t p = tile * kPgTile + 16 * u + 8 * k + row8;
-                    float x = sc[t][u][k];
-                    if (a.cap > 0.0f) x = sa_capped(x, a.cap, inv_cap) * kLog2e;
-                    sc[t][u][k] = p < len[t] && p >= low[t] ? x : -INFINITY;
-                }
-                top[u] = fmaxf(sc[t][u][0], sc[t][u][1]);
+                for (int k = 4; k < 32; k *= 2) new_n = fmaxf(new_n, __shfl_xor_sync(0xffffffffu, new_n, k));
+                const float alpha = new_n == n[t] ? 1.0f : pg_pow2(n[t] - new_n);
+                sum[t] *= new_m == m[t] ? 1.0f : pg_pow2(m[t] - new_m);
+                m[t] = new_m; n[t] = new_n;
 #pragma unroll
-                for (int k = 4; k < 32; k *= 2) top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], k));
+                for (int c = 0; c < VC; c++) { o[t][c][0] *= alpha; o[t][c][1] *= alpha; }
             }
-            const float new_m = fmaxf(m[t], ceilf(fmaxf(top[0], top[1]))), new_n = fmaxf(n[t], ceilf(fmaxf(top[0] + e[0], top[1] + e[1])));
-            sum[t] *= new_m == m[t] ? 1.0f : pg_pow2(m[t] - new_m);
-            alpha[t] = new_n == n[t] ? 1.0f : pg_pow2(n[t] - new_n);
-            m[t] = new_m; n[t] = new_n;
-            const float fm = new_m == -INFINITY ? 0.0f : new_m, fn = (float)kPgShift - (new_n == -INFINITY ? 0.0f : new_n);
+        }
+        uint32_t pf[NT][2][2];
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            const float fm = m[t] == -INFINITY ? 0.0f : m[t], fn = (float)kPgShift - (n[t] == -INFINITY ? 0.0f : n[t]);
 #pragma unroll
             for (int u = 0; u < 2; u++)
 #pragma unroll
@@ -247,21 +274,21 @@ __global__ void __launch_bounds__(32 * kPgWarps) k_paged(const __grid_constant__
         // outputs: sums over the tile join the running ones rounded (the tensor cores cut theirs)
 #pragma unroll
         for (int c = 0; c < VC; c++) {
-            if (c >= vc) break;
+            if (!FULL && c >= vc) break;
             float acc[NT][4];
 #pragma unroll
             for (int t = 0; t < NT; t++) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.0f;
 #pragma unroll
             for (int u = 0; u < 2; u++) {
-                const uint2 x = *reinterpret_cast<const uint2*>(at + k_bytes + (u * vc + c) * 256 + 8 * lane);
+                const uint2 x = *reinterpret_cast<const uint2*>(mine + k_bytes + (u * vc + c) * 256);
                 const uint32_t f[4] = {pg_codes(x.x, 0x4140), pg_codes(x.y, 0x4140), pg_codes(x.x, 0x4342), pg_codes(x.y, 0x4342)};
 #pragma unroll
                 for (int t = 0; t < NT; t++) pg_mma(acc[t], f, pf[t][u][0], pf[t][u][1]);
             }
 #pragma unroll
             for (int t = 0; t < NT; t++) {
-                o[t][c][0] = fmaf(o[t][c][0], alpha[t], acc[t][0] + acc[t][1]);
-                o[t][c][1] = fmaf(o[t][c][1], alpha[t], acc[t][2] + acc[t][3]);
+                o[t][c][0] += acc[t][0] + acc[t][1];
+                o[t][c][1] += acc[t][2] + acc[t][3];
             }
         }
     }
@@ -272,6 +299,11 @@ __global__ void __launch_bounds__(32 * kPgWarps) k_paged(const __grid_constant__
     float* const rec = reinterpret_cast<float*>(pg_mem);              // [warps + 1][4 NT][pitch]
 #pragma unroll
     for (int t = 0; t < NT; t++) {
+        float top = m[t];
+#pragma unroll
+        for (int k = 4; k < 32; k *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+        sum[t] *= m[t] == top ? 1.0f : pg_pow2(m[t] - top);
+        m[t] = top;
 #pragma unroll
         for (int k = 4; k < 32; k *= 2) sum[t] += __shfl_xor_sync(0xffffffffu, sum[t], k);
         float* const to = rec + (size_t)(warp * 4 * NT + 4 * t + j) * pitch;
@@ -333,11 +365,11 @@ __global__ void __launch_bounds__(32 * kPgWarps) k_paged(const __grid_constant__
     if (splits > 1) pg_cluster_sync();                               // no CTA leaves while its record is read
 }
 
-template <int KC, int VC, int NT>
-bool pg_launch(const PgArgs& a, uint32_t splits, cudaStream_t st) {
+template <int KC, int VC, int NT, bool FULL>
+bool pg_launch_as(const PgArgs& a, uint32_t splits, cudaStream_t st) {
     const size_t ring = (size_t)kPgWarps * kPgStages * (kPgTile * (a.s.kp + a.s.vp) + 32), records = sizeof(float) * (kPgWarps + 1) * 4 * NT * (a.s.vp + 4);
     constexpr size_t most = std::max<size_t>((size_t)kPgWarps * kPgStages * (kPgTile * (32 * KC + 16 * VC) + 32), sizeof(float) * (kPgWarps + 1) * 4 * NT * (16 * VC + 4));
-    if (!zg_smem_limit<k_paged<KC, VC, NT>>(most)) return false;
+    if (!zg_smem_limit<k_paged<KC, VC, NT, FULL>>(most)) return false;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(splits, a.s.G * a.chunks, a.B); cfg.blockDim = dim3(32 * kPgWarps); cfg.dynamicSmemBytes = std::max(ring, records); cfg.stream = st;
     cudaLaunchAttribute attr[2];
@@ -346,8 +378,13 @@ bool pg_launch(const PgArgs& a, uint32_t splits, cudaStream_t st) {
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = splits; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr; cfg.numAttrs = 2;
-    cudaLaunchKernelEx(&cfg, k_paged<KC, VC, NT>, a);
+    cudaLaunchKernelEx(&cfg, k_paged<KC, VC, NT, FULL>, a);
     return true;
+}
+// FULL: sizes that fill the kernel's, whose loops and addresses are then known when it is compiled
+template <int KC, int VC, int NT>
+bool pg_launch(const PgArgs& a, uint32_t splits, cudaStream_t st) {
+    return a.s.kp == 32 * KC && a.s.vp == 16 * VC ? pg_launch_as<KC, VC, NT, true>(a, splits, st) : pg_launch_as<KC, VC, NT, false>(a, splits, st);
 }
 
 }  // namespace

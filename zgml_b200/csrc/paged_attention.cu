@@ -20,7 +20,7 @@ struct PgArgs {
     uint32_t B, H, rep, q_rs, dst_rs, window, sink_bf16, tokens, chunks;      // tokens of a sequence a CTA takes together, chunks of a key head's query heads
     float scale, cap;
 };
-constexpr uint32_t kPgWarps = 4, kPgStages = 2, kPgTile = 32, kPgShift = 11;
+constexpr uint32_t kPgWarps = 4, kPgTile = 32, kPgShift = 11;
 constexpr float kPgSlack = 4.0f;                                     // weights reach 2^(11 + 4)
 __device__ __forceinline__ float pg_sink(const PgArgs& a, uint32_t h) { return a.sink_bf16 ? __bfloat162float(reinterpret_cast<const bf16*>(a.sink)[h]) : reinterpret_cast<const float*>(a.sink)[h]; }
 __device__ __forceinline__ uint32_t pg_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -56,9 +56,10 @@ __device__ __forceinline__ void pg_cluster_sync() {
 }
 
 // CTA (share of the positions; key head and chunk of its query heads; row that begins a group of rows of one sequence).  A warp takes every kPgWarps-th tile of 32 positions of
-// the share through a ring of its own of kPgStages copied tiles, so that warps wait for nothing but their own copies.  4 NT queries a CTA, query 4 t + lane % 4 a lane.
+// the share through a buffer of its own, so that warps wait for nothing but their own copies: the next tile's keys come while this one's weights and outputs are computed, its
+// values while the scores are.  4 NT queries a CTA, query 4 t + lane % 4 a lane.
 template <int KC, int VC, int NT, bool FULL>
-__global__ void __launch_bounds__(32 * kPgWarps) k_paged(const __grid_constant__ PgArgs a) {
+__global__ void __launch_bounds__(32 * kPgWarps, NT == 1 && KC <= 4 ? 6 : 1) k_paged(const __grid_constant__ PgArgs a) {
     pdl_enter();
     extern __shared__ float4 pg_mem[];
     __shared__ float stats[kPgWarps][4 * NT][3], joined[4 * NT][3], factor[4 * NT][2];      // m, n, sum
@@ -128,8 +129,8 @@ __global__ void __launch_bounds__(32 * kPgWarps) k_paged(const __grid_constant__
     // this CTA's tiles
     const uint32_t first = all_hi ? all_lo / kPgTile : 0, tiles = all_hi ? (all_hi + kPgTile - 1) / kPgTile - first : 0;
     const uint32_t t0 = first + (uint32_t)((uint64_t)tiles * split / splits), t1 = first + (uint32_t)((uint64_t)tiles * (split + 1) / splits);
-    const uint32_t kp = FULL ? 32 * KC : s.kp, vp = FULL ? 16 * VC : s.vp, kc = kp / 32, vc = vp / 16, k_bytes = kPgTile * kp, stage_bytes = k_bytes + kPgTile * vp + 32;
-    uint8_t* const ring = reinterpret_cast<uint8_t*>(pg_mem) + (size_t)warp * kPgStages * stage_bytes;
+    const uint32_t kp = FULL ? 32 * KC : s.kp, vp = FULL ? 16 * VC : s.vp, kc = kp / 32, vc = vp / 16, k_bytes = kPgTile * kp;
+    uint8_t* const buffer = reinterpret_cast<uint8_t*>(pg_mem) + warp * (k_bytes + kPgTile * vp + 32);
     const uint32_t pages = (all_hi + s.page - 1) >> s.shift;
     // the page of half `lane & 1` of a tile: its id, -1 for one that does not exist, -2 behind the last one that a row sees
     auto find = [&](uint32_t tile) {
@@ -139,27 +140,24 @@ __global__ void __launch_bounds__(32 * kPgWarps) k_paged(const __grid_constant__
     };
     const size_t page_size = page_bytes(s);
     const uint8_t* const parts = a.pool.pages + (size_t)g * s.head;
-    auto fetch = [&](uint32_t tile, int32_t id, uint32_t stage) {
-        uint8_t* const at = ring + stage * stage_bytes;
-        const uint32_t to = pg_smem(at) + 16 * lane;
+    // keys, with the scales, or values of a tile
+    auto fetch = [&](uint32_t tile, int32_t id, bool values) {
+        const uint32_t size_row = values ? vp : kp, to = pg_smem(buffer) + (values ? k_bytes : 0) + 16 * lane;
 #pragma unroll
         for (uint32_t u = 0; u < 2; u++) {
             const int32_t page = __shfl_sync(0xffffffffu, id, u);
-            const uint32_t in = (tile * kPgTile + 16 * u) & (s.page - 1);
             const uint8_t* part = parts + (size_t)max(page, 0) * page_size;
-            const uint8_t* k = part + kPageHead + in * kp + 16 * lane;
-            const uint8_t* v = part + kPageHead + s.page * kp + in * vp + 16 * lane;
+            const uint8_t* from = part + kPageHead + (values ? s.page * kp : 0) + ((tile * kPgTile + 16 * u) & (s.page - 1)) * size_row + 16 * lane;
             const uint32_t size = page >= 0 ? 16 : 0;
 #pragma unroll
-            for (uint32_t i = 0; i < KC; i++) if (FULL || i < kc) pg_copy16(to + u * 16 * kp + 512 * i, k + 512 * i, size);
-#pragma unroll
-            for (uint32_t i = 0; i < VC / 2; i++) if (FULL || 32 * i + lane < vp) pg_copy16(to + k_bytes + u * 16 * vp + 512 * i, v + 512 * i, size);
-            if (lane == 0) {
-                const uint32_t scales = pg_smem(at) + k_bytes + kPgTile * vp + 8 * u;
-                if (page >= 0) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(scales), "l"(part) : "memory");
-                else *reinterpret_cast<float2*>(at + k_bytes + kPgTile * vp + 8 * u) = page == -1 ? make_float2(kBatchNaN, kBatchNaN) : make_float2(1.0f, 1.0f);
+            for (uint32_t i = 0; i < (values ? VC / 2 : KC); i++) if (FULL || 32 * i + lane < size_row) pg_copy16(to + u * 16 * size_row + 512 * i, from + 512 * i, size);
+            if (!values && lane == 0) {
+                uint8_t* const at = buffer + k_bytes + kPgTile * vp + 8 * u;
+                if (page >= 0) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(pg_smem(at)), "l"(part) : "memory");
+                else *reinterpret_cast<float2*>(at) = page == -1 ? make_float2(kBatchNaN, kBatchNaN) : make_float2(1.0f, 1.0f);
             }
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
     // Frames: m of the lane's sum of weights, n of the products' weights.  They stay while no score passes them by much, which one vote of the warp tells.
     float m[NT], n[NT], sum[NT], o[NT][VC][2];
@@ -174,27 +172,17 @@ __global__ void __launch_bounds__(32 * kPgWarps) k_paged(const __grid_constant__
     all_in = __reduce_min_sync(0xffffffffu, all_in);
     least = __reduce_max_sync(0xffffffffu, least);
     const float inv_cap = a.cap > 0.0f ? 1.0f / a.cap : 0.0f;
-    int32_t id = find(t0 + warp);
-#pragma unroll
-    for (uint32_t i = 0; i < kPgStages - 1; i++) {
-        if (t0 + warp + i * kPgWarps < t1) fetch(t0 + warp + i * kPgWarps, id, i);
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        id = find(t0 + warp + (i + 1) * kPgWarps);
+    {
+        const int32_t id = find(t0 + warp);
+        if (t0 + warp < t1) { fetch(t0 + warp, id, false); fetch(t0 + warp, id, true); }
     }
-    uint32_t stage = 0;
+    int32_t id = find(t0 + warp + kPgWarps);
     for (uint32_t tile = t0 + warp; tile < t1; tile += kPgWarps) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(kPgStages - 2) : "memory");
+        const bool more = tile + kPgWarps < t1;
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
         __syncwarp();
-        {
-            const uint32_t next = tile + (kPgStages - 1) * kPgWarps;
-            if (next < t1) fetch(next, id, stage == 0 ? kPgStages - 1 : stage - 1);
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            id = find(next + kPgWarps);
-        }
-        const uint8_t* const at = ring + stage * stage_bytes;
-        const uint8_t* const mine = at + 8 * lane;
-        stage = stage + 1 == kPgStages ? 0 : stage + 1;
-        const float4 scales = *reinterpret_cast<const float4*>(at + k_bytes + kPgTile * vp);      // of keys and values of each half
+        const uint8_t* const mine = buffer + 8 * lane;
+        const float4 scales = *reinterpret_cast<const float4*>(buffer + k_bytes + kPgTile * vp);      // of keys and values of each half
         // scores: sixteen positions a step, of which a lane gets two (row8 and row8 + 8) of its query
         float sc[NT][2][2];
 #pragma unroll
@@ -218,6 +206,9 @@ __global__ void __launch_bounds__(32 * kPgWarps) k_paged(const __grid_constant__
                 sc[t][u][1] = (acc[t][2] + acc[t][3]) * scale;
             }
         }
+        __syncwarp();
+        if (more) fetch(tile + kPgWarps, id, false);
+        else asm volatile("cp.async.commit_group;" ::: "memory");
         if (a.cap > 0.0f) {
 #pragma unroll
             for (int t = 0; t < NT; t++)
@@ -271,6 +262,8 @@ __global__ void __launch_bounds__(32 * kPgWarps) k_paged(const __grid_constant__
                     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(pf[t][u][k]) : "r"(*reinterpret_cast<const uint32_t*>(&both)));
                 }
         }
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        __syncwarp();
         // outputs: sums over the tile join the running ones rounded (the tensor cores cut theirs)
 #pragma unroll
         for (int c = 0; c < VC; c++) {
@@ -291,6 +284,8 @@ __global__ void __launch_bounds__(32 * kPgWarps) k_paged(const __grid_constant__
                 o[t][c][1] += acc[t][2] + acc[t][3];
             }
         }
+        __syncwarp();
+        if (more) { fetch(tile + kPgWarps, id, true); id = find(tile + 2 * kPgWarps); }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
@@ -367,11 +362,11 @@ __global__ void __launch_bounds__(32 * kPgWarps) k_paged(const __grid_constant__
 
 template <int KC, int VC, int NT, bool FULL>
 bool pg_launch_as(const PgArgs& a, uint32_t splits, cudaStream_t st) {
-    const size_t ring = (size_t)kPgWarps * kPgStages * (kPgTile * (a.s.kp + a.s.vp) + 32), records = sizeof(float) * (kPgWarps + 1) * 4 * NT * (a.s.vp + 4);
-    constexpr size_t most = std::max<size_t>((size_t)kPgWarps * kPgStages * (kPgTile * (32 * KC + 16 * VC) + 32), sizeof(float) * (kPgWarps + 1) * 4 * NT * (16 * VC + 4));
+    const size_t buffers = (size_t)kPgWarps * (kPgTile * (a.s.kp + a.s.vp) + 32), records = sizeof(float) * (kPgWarps + 1) * 4 * NT * (a.s.vp + 4);
+    constexpr size_t most = std::max<size_t>((size_t)kPgWarps * (kPgTile * (32 * KC + 16 * VC) + 32), sizeof(float) * (kPgWarps + 1) * 4 * NT * (16 * VC + 4));
     if (!zg_smem_limit<k_paged<KC, VC, NT, FULL>>(most)) return false;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(splits, a.s.G * a.chunks, a.B); cfg.blockDim = dim3(32 * kPgWarps); cfg.dynamicSmemBytes = std::max(ring, records); cfg.stream = st;
+    cfg.gridDim = dim3(splits, a.s.G * a.chunks, a.B); cfg.blockDim = dim3(32 * kPgWarps); cfg.dynamicSmemBytes = std::max(buffers, records); cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = g_zg_pdl ? 1 : 0;

@@ -7,8 +7,7 @@
 // largest contributions keep their bits whatever the pages' scales are; the sum of the softmax has a frame m of its own, and the quotient is put right by 2^(n - m).
 #include "pages.cuh"
 #include "exp2.cuh"
-
-#include <cuda_fp16.h>
+#include "split_tc.cuh"
 
 #include <algorithm>
 
@@ -23,7 +22,6 @@ struct PgArgs {
 constexpr uint32_t kPgWarps = 4, kPgTile = 32, kPgShift = 11;
 constexpr float kPgSlack = 4.0f;                                     // weights reach 2^(11 + 4)
 __device__ __forceinline__ float pg_sink(const PgArgs& a, uint32_t h) { return a.sink_bf16 ? __bfloat162float(reinterpret_cast<const bf16*>(a.sink)[h]) : reinterpret_cast<const float*>(a.sink)[h]; }
-__device__ __forceinline__ uint32_t pg_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 // 2^d of a whole number d, 0 below 2^-126
 __device__ __forceinline__ float pg_pow2(float d) { return d < -126.0f ? 0.0f : __int_as_float(((int)fminf(d, 127.0f) + 127) << 23); }
 // two of a word's four codes, as halves: 1024 + x by its bits, minus 1024 + 128
@@ -32,21 +30,17 @@ __device__ __forceinline__ uint32_t pg_codes(uint32_t w, uint32_t which) {
     const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&x), __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
     return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ void pg_split(float x, float y, uint32_t& hi, uint32_t& lo) {
-    const __half2 h = __floats2half2_rn(x, y);
-    const float2 f = __half22float2(h);
-    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
-    hi = *reinterpret_cast<const uint32_t*>(&h); lo = *reinterpret_cast<const uint32_t*>(&l);
-}
 __device__ __forceinline__ void pg_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void pg_copy16(uint32_t to, const uint8_t* from, uint32_t size) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(size) : "memory"); }
+__device__ __forceinline__ void pg_copy(uint32_t to, const uint8_t* from, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to), "l"(from), "r"(bytes), "r"(bar) : "memory");
+}
 __device__ __forceinline__ float pg_remote(const float* p, uint32_t rank) {
     uint32_t at;
     float v;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(pg_smem(p)), "r"(rank));
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
     return v;
 }
@@ -62,6 +56,7 @@ template <int KC, int VC, int NT, bool FULL>
 __global__ void __launch_bounds__(32 * kPgWarps, NT == 1 && KC <= 4 ? 6 : 1) k_paged(const __grid_constant__ PgArgs a) {
     pdl_enter();
     extern __shared__ float4 pg_mem[];
+    __shared__ uint64_t bars[kPgWarps][2];                           // of a warp's keys and values
     __shared__ float stats[kPgWarps][4 * NT][3], joined[4 * NT][3], factor[4 * NT][2];      // m, n, sum
     const PageShape& s = a.s;
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, row8 = lane / 4, j = lane % 4;
@@ -120,7 +115,7 @@ __global__ void __launch_bounds__(32 * kPgWarps, NT == 1 && KC <= 4 ? 6 : 1) k_p
 #pragma unroll
             for (int k = 0; k < 4; k++) {
                 uint32_t hi, lo;
-                pg_split(x[c][2 * k] * f, x[c][2 * k + 1] * f, hi, lo);
+                split2(x[c][2 * k] * f, x[c][2 * k + 1] * f, hi, lo);
                 qf[t][2 * c + k / 2][k % 2] = row8 & 1 ? lo : hi;
             }
     }
@@ -140,24 +135,29 @@ __global__ void __launch_bounds__(32 * kPgWarps, NT == 1 && KC <= 4 ? 6 : 1) k_p
     };
     const size_t page_size = page_bytes(s);
     const uint8_t* const parts = a.pool.pages + (size_t)g * s.head;
-    // keys, with the scales, or values of a tile
+    // Keys, with the scales, or values of a tile: a bulk copy for each half, by lanes 0 and 1.  What no page holds is left as it is, and gets scales alone.
+    const uint32_t k_bar = smem_u32(&bars[warp][0]), v_bar = k_bar + 8, at = smem_u32(buffer), heads_at = at + k_bytes + kPgTile * vp;
+    if (lane == 0) {
+        mbar_init(k_bar, 2);
+        mbar_init(v_bar, 2);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncwarp();
     auto fetch = [&](uint32_t tile, int32_t id, bool values) {
-        const uint32_t size_row = values ? vp : kp, to = pg_smem(buffer) + (values ? k_bytes : 0) + 16 * lane;
-#pragma unroll
-        for (uint32_t u = 0; u < 2; u++) {
-            const int32_t page = __shfl_sync(0xffffffffu, id, u);
-            const uint8_t* part = parts + (size_t)max(page, 0) * page_size;
-            const uint8_t* from = part + kPageHead + (values ? s.page * kp : 0) + ((tile * kPgTile + 16 * u) & (s.page - 1)) * size_row + 16 * lane;
-            const uint32_t size = page >= 0 ? 16 : 0;
-#pragma unroll
-            for (uint32_t i = 0; i < (values ? VC / 2 : KC); i++) if (FULL || 32 * i + lane < size_row) pg_copy16(to + u * 16 * size_row + 512 * i, from + 512 * i, size);
-            if (!values && lane == 0) {
-                uint8_t* const at = buffer + k_bytes + kPgTile * vp + 8 * u;
-                if (page >= 0) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(pg_smem(at)), "l"(part) : "memory");
-                else *reinterpret_cast<float2*>(at) = page == -1 ? make_float2(kBatchNaN, kBatchNaN) : make_float2(1.0f, 1.0f);
+        if (lane >= 2) return;
+        const uint8_t* part = parts + (size_t)max(id, 0) * page_size;
+        const uint32_t in = (tile * kPgTile + 16 * lane) & (s.page - 1), bar = values ? v_bar : k_bar;
+        mbar_expect_tx(bar, id < 0 ? 0 : values ? 16 * vp : 16 * kp + kPageHead);
+        if (id < 0) {
+            if (!values) {
+                *reinterpret_cast<float2*>(buffer + k_bytes + kPgTile * vp + kPageHead * lane) = id == -1 ? make_float2(kBatchNaN, kBatchNaN) : make_float2(1.0f, 1.0f);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             }
+        } else if (values) pg_copy(at + k_bytes + 16 * vp * lane, part + kPageHead + s.page * kp + in * vp, 16 * vp, bar);
+        else {
+            pg_copy(at + 16 * kp * lane, part + kPageHead + in * kp, 16 * kp, bar);
+            pg_copy(heads_at + kPageHead * lane, part, kPageHead, bar);
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
     };
     // Frames: m of the lane's sum of weights, n of the products' weights.  They stay while no score passes them by much, which one vote of the warp tells.
     float m[NT], n[NT], sum[NT], o[NT][VC][2];
@@ -175,14 +175,17 @@ __global__ void __launch_bounds__(32 * kPgWarps, NT == 1 && KC <= 4 ? 6 : 1) k_p
     {
         const int32_t id = find(t0 + warp);
         if (t0 + warp < t1) { fetch(t0 + warp, id, false); fetch(t0 + warp, id, true); }
+        __syncwarp();
     }
     int32_t id = find(t0 + warp + kPgWarps);
+    bool gave_up = false;
+    uint32_t k_phase = 0, v_phase = 0;
     for (uint32_t tile = t0 + warp; tile < t1; tile += kPgWarps) {
         const bool more = tile + kPgWarps < t1;
-        asm volatile("cp.async.wait_group 1;" ::: "memory");
-        __syncwarp();
+        if (!__all_sync(0xffffffffu, mbar_wait(k_bar, k_phase))) { gave_up = true; break; }
         const uint8_t* const mine = buffer + 8 * lane;
-        const float4 scales = *reinterpret_cast<const float4*>(buffer + k_bytes + kPgTile * vp);      // of keys and values of each half
+        const float2 s0 = *reinterpret_cast<const float2*>(buffer + k_bytes + kPgTile * vp), s1 = *reinterpret_cast<const float2*>(buffer + k_bytes + kPgTile * vp + kPageHead);
+        const float4 scales = make_float4(s0.x, s0.y, s1.x, s1.y);      // of keys and values of each half
         // scores: sixteen positions a step, of which a lane gets two (row8 and row8 + 8) of its query
         float sc[NT][2][2];
 #pragma unroll
@@ -207,8 +210,7 @@ __global__ void __launch_bounds__(32 * kPgWarps, NT == 1 && KC <= 4 ? 6 : 1) k_p
             }
         }
         __syncwarp();
-        if (more) fetch(tile + kPgWarps, id, false);
-        else asm volatile("cp.async.commit_group;" ::: "memory");
+        if (more) { fetch(tile + kPgWarps, id, false); k_phase ^= 1; }
         if (a.cap > 0.0f) {
 #pragma unroll
             for (int t = 0; t < NT; t++)
@@ -262,8 +264,8 @@ __global__ void __launch_bounds__(32 * kPgWarps, NT == 1 && KC <= 4 ? 6 : 1) k_p
                     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(pf[t][u][k]) : "r"(*reinterpret_cast<const uint32_t*>(&both)));
                 }
         }
-        asm volatile("cp.async.wait_group 1;" ::: "memory");
         __syncwarp();
+        if (!__all_sync(0xffffffffu, mbar_wait(v_bar, v_phase))) { gave_up = true; break; }
         // outputs: sums over the tile join the running ones rounded (the tensor cores cut theirs)
 #pragma unroll
         for (int c = 0; c < VC; c++) {
@@ -285,9 +287,16 @@ __global__ void __launch_bounds__(32 * kPgWarps, NT == 1 && KC <= 4 ? 6 : 1) k_p
             }
         }
         __syncwarp();
-        if (more) { fetch(tile + kPgWarps, id, true); id = find(tile + 2 * kPgWarps); }
+        if (more) { fetch(tile + kPgWarps, id, true); v_phase ^= 1; id = find(tile + 2 * kPgWarps); }
+        __syncwarp();
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (gave_up) {                                                   // what is under way lands before the memory is used for other things; outputs are not numbers
+        mbar_wait(k_bar, k_phase);
+        mbar_wait(v_bar, v_phase);
+        if (lane == 0) count_timeout();
+#pragma unroll
+        for (int t = 0; t < NT; t++) sum[t] = kBatchNaN;
+    }
     __syncthreads();
     // the warps' records join in shared memory, then those of the cluster's CTAs
     const uint32_t pitch = s.vp + 4;
@@ -398,6 +407,7 @@ bool zg_paged_attention_valid(const ZgSeqOp& s, const size_t* elems, size_t n_bu
     return true;
 }
 size_t zg_paged_attention_scratch_elems(const ZgSeqOp&) { return 0; }
+unsigned int zg_paged_attention_timeouts() { return tc_timeouts(); }
 bool zg_launch_paged_attention(const ZgOp& op, float* const* bufs, const size_t* elems, float*, cudaStream_t st) {
     const ZgSeqOp& s = op.u.seq;
     PgArgs a;

@@ -520,5 +520,6 @@ bool zg_launch_page_op(const ZgOp& op, float* const* bufs, const size_t* elems, 
 bool zg_paged_attention_valid(const ZgSeqOp& s, const size_t* elems, size_t n_bufs, char* why, size_t why_n);
 size_t zg_paged_attention_scratch_elems(const ZgSeqOp& s);
 bool zg_launch_paged_attention(const ZgOp& op, float* const* bufs, const size_t* elems, float* scratch, cudaStream_t st);
+unsigned int zg_paged_attention_timeouts();      // waits that gave up
 bool zg_sample_valid(const ZgSeqOp& s, const size_t* elems, size_t n_bufs, char* why, size_t why_n);
 bool zg_launch_sample(const ZgOp& op, float* const* bufs, cudaStream_t st);

@@ -1,10 +1,10 @@
 // PAGED_ATTENTION (parameter pack in include/zgml_cuda.h): softmax attention of the rows of a step over the 8-bit pages of their sequences.
 //
-// Both products run on the tensor cores with operands that hold what f32 would: codes are whole numbers of 8 bits and exact in half precision, a query (scaled so that its
-// largest element is in [2^14, 2^15)) and a weight (of [0, 2^15]) are the sum of two halves, 22 to 24 bits of what lies within 2^-18 of the largest.  Codes are the instructions' rows
-// (16 positions, 16 values of a head), the two halves of four queries their eight columns, side by side, so that four queries fill an instruction and a lane adds up what belongs together.  Scales are powers of two: a key's joins its scores, a value's its weights, exactly.
-// A weight is 2^(s + e - n), with the score s in powers of two, e the exponent of its value's scale and n a whole number that no s + e so far passes by more than 4, so that the
-// largest contributions keep their bits whatever the pages' scales are; the sum of the softmax has a frame m of its own, and the quotient is put right by 2^(n - m).
+// Both products run on the tensor cores in whole numbers, whose sums are exact: codes of 8 bits, which need no conversion, times digits of 8 bits.  A query is six digits of base 256 (45 bits
+// of its largest element), a weight four (32 bits of the largest contribution); the digits of four queries are 24 and 16 columns of the instructions, codes their rows.  Stored codes are offset
+// by 128: sum (c + 128) d - 128 sum d is exact too, and a bit of each code of a value is turned over.  Scales are powers of two: a key's joins its scores, a value's its weights.  A weight is 2^(s + e - n), with the score s in powers of
+// two, e the exponent of its value's scale and n a whole number that no s + e so far passes by more than 3, so that the largest contributions keep their bits whatever the pages' scales
+// are; the sum of the softmax has a frame m of its own, and the quotient is put right by 2^(n - m).
 #include "pages.cuh"
 #include "exp2.cuh"
 #include "split_tc.cuh"
@@ -19,20 +19,23 @@ struct PgArgs {
     uint32_t B, H, rep, q_rs, dst_rs, window, sink_bf16, tokens, chunks;      // tokens of a sequence a CTA takes together, chunks of a key head's query heads
     float scale, cap;
 };
-constexpr uint32_t kPgWarps = 4, kPgTile = 32, kPgShift = 11;
-constexpr float kPgSlack = 4.0f;                                     // weights reach 2^(11 + 4)
+constexpr uint32_t kPgWarps = 4, kPgTile = 32, kPgShift = 29, kPgFlush = 512;      // (512 tiles of 32 products of two bytes: below 2^31)
+constexpr float kPgSlack = 3.0f;                                     // weights reach 2^(29 + 3)
 __device__ __forceinline__ float pg_sink(const PgArgs& a, uint32_t h) { return a.sink_bf16 ? __bfloat162float(reinterpret_cast<const bf16*>(a.sink)[h]) : reinterpret_cast<const float*>(a.sink)[h]; }
 // 2^d of a whole number d, 0 below 2^-126
 __device__ __forceinline__ float pg_pow2(float d) { return d < -126.0f ? 0.0f : __int_as_float(((int)fminf(d, 127.0f) + 127) << 23); }
-// two of a word's four codes, as halves: 1024 + x by its bits, minus 1024 + 128
-__device__ __forceinline__ uint32_t pg_codes(uint32_t w, uint32_t which) {
-    const uint32_t x = __byte_perm(w, 0x64646464u, which);
-    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&x), __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
-    return *reinterpret_cast<const uint32_t*>(&h);
+// D = A B (+ D): 16 rows of 32 codes as they are stored and signed digits of a query; codes that have their sign and unsigned digits of weights
+__device__ __forceinline__ void pg_scores(int (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2], bool first) {
+    if (first)
+        asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "r"(0));
+    else
+        asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
-__device__ __forceinline__ void pg_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+__device__ __forceinline__ void pg_outputs(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void pg_copy(uint32_t to, const uint8_t* from, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to), "l"(from), "r"(bytes), "r"(bar) : "memory");
@@ -53,7 +56,7 @@ __device__ __forceinline__ void pg_cluster_sync() {
 // the share through a buffer of its own, so that warps wait for nothing but their own copies: the next tile's keys come while this one's weights and outputs are computed, its
 // values while the scores are.  4 NT queries a CTA, query 4 t + lane % 4 a lane.
 template <int KC, int VC, int NT, bool FULL>
-__global__ void __launch_bounds__(32 * kPgWarps, NT == 1 && KC <= 4 ? 6 : 1) k_paged(const __grid_constant__ PgArgs a) {
+__global__ void __launch_bounds__(32 * kPgWarps, NT == 1 && KC <= 4 ? 3 : 1) k_paged(const __grid_constant__ PgArgs a) {
     pdl_enter();
     extern __shared__ float4 pg_mem[];
     __shared__ uint64_t bars[kPgWarps][2];                           // of a warp's keys and values
@@ -79,9 +82,10 @@ __global__ void __launch_bounds__(32 * kPgWarps, NT == 1 && KC <= 4 ? 6 : 1) k_p
         group = min(a.tokens, (uint32_t)__ffs(~(__ballot_sync(0xffffffffu, same) | 1u)) - 1);
     }
     const uint32_t heads = min(a.rep, 4u * NT);                      // of a chunk
-    // what the lane's queries see, and the halves of the query that its column of the products is (its upper or its lower one)
+    // what the lane's queries see, and its column of the first product: two of the six digits of a query, and 128 times their sums
     uint32_t len[NT], low[NT], all_lo = 0xffffffffu, all_hi = 0;
-    uint32_t qf[NT][2 * KC][2];
+    uint32_t qd[NT][KC][3][2];
+    int offset[NT][3];
     float q_scale[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) {
@@ -107,17 +111,42 @@ __global__ void __launch_bounds__(32 * kPgWarps, NT == 1 && KC <= 4 ? 6 : 1) k_p
             }
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const uint32_t e = top ? max(top >> 23, 15u) : 141u;         // its exponent
-        const float f = __uint_as_float((268u - e) << 23);           // 2^14 / 2^(e - 127)
-        q_scale[t] = __shfl_sync(0xffffffffu, __uint_as_float((e - 14u) << 23), 8 * j) * a.scale * (a.cap > 0.0f ? 1.0f : kLog2e);      // (of the lane's scores)
+        const uint32_t e = max(top >> 23, 46u);                      // its exponent
+        const float f = __uint_as_float((275u - e) << 23);           // 2^21 / 2^(e - 127): elements are below 2^22, so that their first digits are at most 64
+        q_scale[t] = top >= 0x7f800000u ? kBatchNaN : __uint_as_float((e - 44u) << 23) * a.scale * (a.cap > 0.0f ? 1.0f : kLog2e);      // (1 / (f 2^23))
+        q_scale[t] = __shfl_sync(0xffffffffu, q_scale[t], 8 * j);    // (of the lane's scores)
+        // element = (hi + lo 2^-23) / f, hi and lo three digits each, of which an even row8's column takes 5, 3, 1 and an odd one's 4, 2, 0
+        const bool odd = row8 & 1;
+        int sums[3] = {0, 0, 0};
 #pragma unroll
         for (int c = 0; c < KC; c++)
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                uint32_t hi, lo;
-                split2(x[c][2 * k] * f, x[c][2 * k + 1] * f, hi, lo);
-                qf[t][2 * c + k / 2][k % 2] = row8 & 1 ? lo : hi;
+            for (int k = 0; k < 2; k++) {
+                uint32_t hi[4], lo[4], word[3];
+#pragma unroll
+                for (int i4 = 0; i4 < 4; i4++) {
+                    const float y = x[c][4 * k + i4] * f, whole = rintf(y);
+                    hi[i4] = (uint32_t)((int)whole + 0x8080);
+                    lo[i4] = (uint32_t)((int)((y - whole) * 8388608.0f) + 0x8080);
+                }
+#pragma unroll
+                for (int n3 = 0; n3 < 3; n3++) {
+                    const bool high = n3 == 0 || (n3 == 1 && !odd);
+                    const uint32_t at = n3 == 0 ? (odd ? 1 : 2) : n3 == 1 ? (odd ? 2 : 0) : (odd ? 0 : 1), pick = at | (at + 4) << 4;
+                    uint32_t v[4];
+#pragma unroll
+                    for (int i4 = 0; i4 < 4; i4++) v[i4] = high ? hi[i4] : lo[i4];
+                    word[n3] = __byte_perm(__byte_perm(v[0], v[1], pick), __byte_perm(v[2], v[3], pick), 0x5410) ^ (at == 2 ? 0u : 0x80808080u);
+                    sums[n3] = __dp4a((int)word[n3], 0x01010101, sums[n3]);
+                    qd[t][c][n3][k] = word[n3];
+                }
             }
+#pragma unroll
+        for (int n3 = 0; n3 < 3; n3++) {
+            sums[n3] += __shfl_xor_sync(0xffffffffu, sums[n3], 1);
+            sums[n3] += __shfl_xor_sync(0xffffffffu, sums[n3], 2);
+            offset[t][n3] = -128 * ((n3 == 1 ? 128 : 256) * __shfl_sync(0xffffffffu, sums[n3], 8 * j) + __shfl_sync(0xffffffffu, sums[n3], 8 * j + 4));
+        }
     }
     all_lo = __reduce_min_sync(0xffffffffu, all_lo);
     all_hi = __reduce_max_sync(0xffffffffu, all_hi);
@@ -125,7 +154,9 @@ __global__ void __launch_bounds__(32 * kPgWarps, NT == 1 && KC <= 4 ? 6 : 1) k_p
     const uint32_t first = all_hi ? all_lo / kPgTile : 0, tiles = all_hi ? (all_hi + kPgTile - 1) / kPgTile - first : 0;
     const uint32_t t0 = first + (uint32_t)((uint64_t)tiles * split / splits), t1 = first + (uint32_t)((uint64_t)tiles * (split + 1) / splits);
     const uint32_t kp = FULL ? 32 * KC : s.kp, vp = FULL ? 16 * VC : s.vp, kc = kp / 32, vc = vp / 16, k_bytes = kPgTile * kp;
-    uint8_t* const buffer = reinterpret_cast<uint8_t*>(pg_mem) + warp * (k_bytes + kPgTile * vp + 32);
+    const uint32_t buffer_bytes = k_bytes + kPgTile * vp + 32, pitch = vp + 4;
+    uint8_t* const buffer = reinterpret_cast<uint8_t*>(pg_mem) + warp * buffer_bytes;
+    float* const rec = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(pg_mem) + kPgWarps * buffer_bytes);      // [warps][4 NT][pitch]
     const uint32_t pages = (all_hi + s.page - 1) >> s.shift;
     // the page of half `lane & 1` of a tile: its id, -1 for one that does not exist, -2 behind the last one that a row sees
     auto find = [&](uint32_t tile) {
@@ -160,15 +191,41 @@ __global__ void __launch_bounds__(32 * kPgWarps, NT == 1 && KC <= 4 ? 6 : 1) k_p
         }
     };
     // Frames: m of the lane's sum of weights, n of the products' weights.  They stay while no score passes them by much, which one vote of the warp tells.
-    float m[NT], n[NT], sum[NT], o[NT][VC][2];
-    uint32_t all_in = 0xffffffffu, least = 0;                        // positions that every query sees
+    float m[NT], n[NT], sum[NT];
+    int o[NT][VC][2][4];                                             // even and odd digits: two of each
+    uint32_t all_in = 0xffffffffu, least = 0, since = 0;             // positions that every query sees; tiles since the sums were put away
+    bool stored = false;
 #pragma unroll
     for (int t = 0; t < NT; t++) {
         m[t] = n[t] = -INFINITY; sum[t] = 0.0f;
         if (len[t]) { all_in = min(all_in, len[t]); least = max(least, low[t]); }
 #pragma unroll
-        for (int c = 0; c < VC; c++) o[t][c][0] = o[t][c][1] = 0.0f;
+        for (int c = 0; c < VC; c++)
+#pragma unroll
+            for (int k = 0; k < 8; k++) o[t][c][k / 4][k % 4] = 0;
     }
+    // The sums so far, times alpha, go to the warp's record, where a lane has places of its own.
+    auto flush = [&](const float (&alpha)[NT]) {
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            float* const to = rec + (size_t)(warp * 4 * NT + 4 * t + j) * pitch;
+#pragma unroll
+            for (int c = 0; c < VC; c++) {
+                if (!FULL && c >= vc) break;
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    const int (&x)[2][4] = o[t][c];
+                    const float v = fmaf(fmaf(fmaf((float)x[1][2 * k + 1], 256.0f, (float)x[0][2 * k + 1]), 256.0f, (float)x[1][2 * k]), 256.0f, (float)x[0][2 * k]);
+                    float* const at = to + 16 * c + 8 * k + row8;
+                    *at = ((stored ? *at : 0.0f) + v) * alpha[t];
+                }
+#pragma unroll
+                for (int k = 0; k < 8; k++) o[t][c][k / 4][k % 4] = 0;
+            }
+        }
+        stored = true;
+        since = 0;
+    };
     all_in = __reduce_min_sync(0xffffffffu, all_in);
     least = __reduce_max_sync(0xffffffffu, least);
     const float inv_cap = a.cap > 0.0f ? 1.0f / a.cap : 0.0f;
@@ -190,23 +247,27 @@ __global__ void __launch_bounds__(32 * kPgWarps, NT == 1 && KC <= 4 ? 6 : 1) k_p
         float sc[NT][2][2];
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            float acc[NT][4];
-#pragma unroll
-            for (int t = 0; t < NT; t++) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.0f;
+            int acc[NT][3][4];
 #pragma unroll
             for (int c = 0; c < KC; c++) {
                 if (!FULL && c >= kc) break;
                 const uint2 x = *reinterpret_cast<const uint2*>(mine + (2 * u * kc + c) * 256), y = *reinterpret_cast<const uint2*>(mine + ((2 * u + 1) * kc + c) * 256);
-                const uint32_t f0[4] = {pg_codes(x.x, 0x4140), pg_codes(y.x, 0x4140), pg_codes(x.x, 0x4342), pg_codes(y.x, 0x4342)};
-                const uint32_t f1[4] = {pg_codes(x.y, 0x4140), pg_codes(y.y, 0x4140), pg_codes(x.y, 0x4342), pg_codes(y.y, 0x4342)};
+                const uint32_t f[4] = {x.x, y.x, x.y, y.y};
 #pragma unroll
-                for (int t = 0; t < NT; t++) { pg_mma(acc[t], f0, qf[t][2 * c][0], qf[t][2 * c][1]); pg_mma(acc[t], f1, qf[t][2 * c + 1][0], qf[t][2 * c + 1][1]); }
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int n3 = 0; n3 < 3; n3++) pg_scores(acc[t][n3], f, qd[t][c][n3], c == 0);
             }
 #pragma unroll
             for (int t = 0; t < NT; t++) {
                 const float scale = q_scale[t] * (u ? scales.z : scales.x);
-                sc[t][u][0] = (acc[t][0] + acc[t][1]) * scale;
-                sc[t][u][1] = (acc[t][2] + acc[t][3]) * scale;
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    float part[3];
+#pragma unroll
+                    for (int n3 = 0; n3 < 3; n3++) part[n3] = (float)(acc[t][n3][2 * k] * (n3 == 1 ? 128 : 256) + acc[t][n3][2 * k + 1] + offset[t][n3]);
+                    sc[t][u][k] = fmaf(fmaf(part[0], 32768.0f, part[1]), 65536.0f, part[2]) * scale;
+                }
             }
         }
         __syncwarp();
@@ -234,57 +295,49 @@ __global__ void __launch_bounds__(32 * kPgWarps, NT == 1 && KC <= 4 ? 6 : 1) k_p
             const float top0 = fmaxf(sc[t][0][0], sc[t][0][1]), top1 = fmaxf(sc[t][1][0], sc[t][1][1]);
             over = over || fmaxf(top0 + e[0], top1 + e[1]) > n[t] + kPgSlack || fmaxf(top0, top1) > m[t] + 64.0f;
         }
-        if (__any_sync(0xffffffffu, over)) {
+        if (__any_sync(0xffffffffu, over) || since == kPgFlush) {
+            float alpha[NT];
 #pragma unroll
             for (int t = 0; t < NT; t++) {
                 const float top0 = fmaxf(sc[t][0][0], sc[t][0][1]), top1 = fmaxf(sc[t][1][0], sc[t][1][1]), new_m = fmaxf(m[t], ceilf(fmaxf(top0, top1)));
                 float new_n = fmaxf(n[t], ceilf(fmaxf(top0 + e[0], top1 + e[1])));
 #pragma unroll
                 for (int k = 4; k < 32; k *= 2) new_n = fmaxf(new_n, __shfl_xor_sync(0xffffffffu, new_n, k));
-                const float alpha = new_n == n[t] ? 1.0f : pg_pow2(n[t] - new_n);
+                alpha[t] = new_n == n[t] ? 1.0f : pg_pow2(n[t] - new_n);
                 sum[t] *= new_m == m[t] ? 1.0f : pg_pow2(m[t] - new_m);
                 m[t] = new_m; n[t] = new_n;
-#pragma unroll
-                for (int c = 0; c < VC; c++) { o[t][c][0] *= alpha; o[t][c][1] *= alpha; }
             }
+            if (stored || since) flush(alpha);
         }
-        uint32_t pf[NT][2][2];
+        since++;
+        uint32_t low_digits[NT][2], high_digits[NT][2];              // of each half's weights: digits 0 and 2, and 1 and 3, of four positions
 #pragma unroll
         for (int t = 0; t < NT; t++) {
             const float fm = m[t] == -INFINITY ? 0.0f : m[t], fn = (float)kPgShift - (n[t] == -INFINITY ? 0.0f : n[t]);
 #pragma unroll
-            for (int u = 0; u < 2; u++)
+            for (int u = 0; u < 2; u++) {
+                uint32_t turned[2];
 #pragma unroll
                 for (int k = 0; k < 2; k++) {
                     const float x = sc[t][u][k], y = x == -INFINITY ? 0.0f : sa_ex2(x + (fn + e[u]));
-                    sum[t] += sa_ex2(x - fm);
-                    // the halves side by side, position by position; turned around they are the second product's columns
-                    const __half hi = __float2half_rn(y);
-                    const __half2 both = __halves2half2(hi, __float2half_rn(y - __half2float(hi)));
-                    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(pf[t][u][k]) : "r"(*reinterpret_cast<const uint32_t*>(&both)));
+                    sum[t] += sa_ex2(x - fm) + (y - y);              // (a scale that is not a number is one of the sum's too)
+                    const uint32_t w = __float2uint_rn(y);
+                    // a lane's weight is two columns of 16 bits, a position a row; turned around they are rows of positions
+                    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(turned[k]) : "r"(w));
                 }
+                low_digits[t][u] = __byte_perm(turned[0], turned[1], 0x6420);
+                high_digits[t][u] = __byte_perm(turned[0], turned[1], 0x7531);
+            }
         }
         __syncwarp();
         if (!__all_sync(0xffffffffu, mbar_wait(v_bar, v_phase))) { gave_up = true; break; }
-        // outputs: sums over the tile join the running ones rounded (the tensor cores cut theirs)
 #pragma unroll
         for (int c = 0; c < VC; c++) {
             if (!FULL && c >= vc) break;
-            float acc[NT][4];
+            const uint2 x = *reinterpret_cast<const uint2*>(mine + k_bytes + c * 256), y = *reinterpret_cast<const uint2*>(mine + k_bytes + (vc + c) * 256);
+            const uint32_t f[4] = {x.x ^ 0x80808080u, x.y ^ 0x80808080u, y.x ^ 0x80808080u, y.y ^ 0x80808080u};
 #pragma unroll
-            for (int t = 0; t < NT; t++) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.0f;
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const uint2 x = *reinterpret_cast<const uint2*>(mine + k_bytes + (u * vc + c) * 256);
-                const uint32_t f[4] = {pg_codes(x.x, 0x4140), pg_codes(x.y, 0x4140), pg_codes(x.x, 0x4342), pg_codes(x.y, 0x4342)};
-#pragma unroll
-                for (int t = 0; t < NT; t++) pg_mma(acc[t], f, pf[t][u][0], pf[t][u][1]);
-            }
-#pragma unroll
-            for (int t = 0; t < NT; t++) {
-                o[t][c][0] += acc[t][0] + acc[t][1];
-                o[t][c][1] += acc[t][2] + acc[t][3];
-            }
+            for (int t = 0; t < NT; t++) { pg_outputs(o[t][c][0], f, low_digits[t][0], low_digits[t][1]); pg_outputs(o[t][c][1], f, high_digits[t][0], high_digits[t][1]); }
         }
         __syncwarp();
         if (more) { fetch(tile + kPgWarps, id, true); v_phase ^= 1; id = find(tile + 2 * kPgWarps); }
@@ -297,34 +350,29 @@ __global__ void __launch_bounds__(32 * kPgWarps, NT == 1 && KC <= 4 ? 6 : 1) k_p
 #pragma unroll
         for (int t = 0; t < NT; t++) sum[t] = kBatchNaN;
     }
-    __syncthreads();
     // the warps' records join in shared memory, then those of the cluster's CTAs
-    const uint32_t pitch = s.vp + 4;
-    float* const rec = reinterpret_cast<float*>(pg_mem);              // [warps + 1][4 NT][pitch]
+    {
+        float one[NT];
+#pragma unroll
+        for (int t = 0; t < NT; t++) one[t] = 1.0f;
+        flush(one);
+    }
 #pragma unroll
     for (int t = 0; t < NT; t++) {
         float top = m[t];
 #pragma unroll
         for (int k = 4; k < 32; k *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
         sum[t] *= m[t] == top ? 1.0f : pg_pow2(m[t] - top);
-        m[t] = top;
 #pragma unroll
         for (int k = 4; k < 32; k *= 2) sum[t] += __shfl_xor_sync(0xffffffffu, sum[t], k);
-        float* const to = rec + (size_t)(warp * 4 * NT + 4 * t + j) * pitch;
-#pragma unroll
-        for (int c = 0; c < VC; c++) {
-            if (c >= vc) break;
-            to[16 * c + row8] = o[t][c][0];
-            to[16 * c + 8 + row8] = o[t][c][1];
-        }
-        if (row8 == 0) { stats[warp][4 * t + j][0] = m[t]; stats[warp][4 * t + j][1] = n[t]; stats[warp][4 * t + j][2] = sum[t]; }
+        if (row8 == 0) { stats[warp][4 * t + j][0] = top; stats[warp][4 * t + j][1] = n[t]; stats[warp][4 * t + j][2] = sum[t]; }
     }
     __syncthreads();
     auto frame = [](float from, float to) { return from == to ? 1.0f : pg_pow2(from - to); };      // (also where both are infinite)
-    float* const mine = rec + (size_t)kPgWarps * 4 * NT * pitch;
+    float* const mine = reinterpret_cast<float*>(pg_mem);             // [4 NT][pitch], where tiles were
     const uint32_t queries = group * heads;
-    for (uint32_t x = threadIdx.x; x < queries * s.vp; x += 32 * kPgWarps) {
-        const uint32_t i = x / s.vp, d = x - i * s.vp;
+    for (uint32_t x = threadIdx.x; x < queries * vp; x += 32 * kPgWarps) {
+        const uint32_t i = x / vp, d = x - i * vp;
         float top_m = -INFINITY, top_n = -INFINITY, l = 0.0f, v = 0.0f;
 #pragma unroll
         for (uint32_t k = 0; k < kPgWarps; k++) { top_m = fmaxf(top_m, stats[k][i][0]); top_n = fmaxf(top_n, stats[k][i][1]); }
@@ -371,11 +419,11 @@ __global__ void __launch_bounds__(32 * kPgWarps, NT == 1 && KC <= 4 ? 6 : 1) k_p
 
 template <int KC, int VC, int NT, bool FULL>
 bool pg_launch_as(const PgArgs& a, uint32_t splits, cudaStream_t st) {
-    const size_t buffers = (size_t)kPgWarps * (kPgTile * (a.s.kp + a.s.vp) + 32), records = sizeof(float) * (kPgWarps + 1) * 4 * NT * (a.s.vp + 4);
-    constexpr size_t most = std::max<size_t>((size_t)kPgWarps * (kPgTile * (32 * KC + 16 * VC) + 32), sizeof(float) * (kPgWarps + 1) * 4 * NT * (16 * VC + 4));
+    const size_t buffers = (size_t)kPgWarps * (kPgTile * (a.s.kp + a.s.vp) + 32), records = sizeof(float) * kPgWarps * 4 * NT * (a.s.vp + 4);
+    constexpr size_t most = (size_t)kPgWarps * (kPgTile * (32 * KC + 16 * VC) + 32) + sizeof(float) * kPgWarps * 4 * NT * (16 * VC + 4);
     if (!zg_smem_limit<k_paged<KC, VC, NT, FULL>>(most)) return false;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(splits, a.s.G * a.chunks, a.B); cfg.blockDim = dim3(32 * kPgWarps); cfg.dynamicSmemBytes = std::max(buffers, records); cfg.stream = st;
+    cfg.gridDim = dim3(splits, a.s.G * a.chunks, a.B); cfg.blockDim = dim3(32 * kPgWarps); cfg.dynamicSmemBytes = buffers + records; cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = g_zg_pdl ? 1 : 0;
@@ -420,7 +468,7 @@ bool zg_launch_paged_attention(const ZgOp& op, float* const* bufs, const size_t*
     // Queries that a CTA takes together: of one row, or, where the step has more rows than the page table slots, of the rows that a slot has then.
     const bool narrow = a.s.kp <= 64 && a.s.vp <= 64, wide = a.s.kp > 128 || a.s.vp > 128;
     const uint64_t together = (uint64_t)a.rep * std::max<uint32_t>(1, a.B / std::max(1u, a.pool.slots));
-    const uint32_t queries = together <= 4 ? 4 : together <= 8 || wide ? 8 : 16;
+    const uint32_t queries = together <= 4 || wide ? 4 : 8;
     a.chunks = (a.rep + queries - 1) / queries;
     a.tokens = std::max(1u, queries / a.rep);
     const uint32_t ctas = a.B * a.s.G * a.chunks, most = std::max<uint32_t>(1, (uint32_t)std::min<uint64_t>(8, ((uint64_t)s.n[8] << a.s.shift) / 256));
@@ -428,9 +476,9 @@ bool zg_launch_paged_attention(const ZgOp& op, float* const* bufs, const size_t*
     while (splits < most && ctas * splits < 4 * zg_sm_count()) splits *= 2;
     if (splits > most) splits = most;
     bool ok;
-    if (narrow) ok = queries == 4 ? pg_launch<2, 4, 1>(a, splits, st) : queries == 8 ? pg_launch<2, 4, 2>(a, splits, st) : pg_launch<2, 4, 4>(a, splits, st);
-    else if (!wide) ok = queries == 4 ? pg_launch<4, 8, 1>(a, splits, st) : queries == 8 ? pg_launch<4, 8, 2>(a, splits, st) : pg_launch<4, 8, 4>(a, splits, st);
-    else ok = queries == 4 ? pg_launch<8, 16, 1>(a, splits, st) : pg_launch<8, 16, 2>(a, splits, st);
+    if (narrow) ok = queries == 4 ? pg_launch<2, 4, 1>(a, splits, st) : pg_launch<2, 4, 2>(a, splits, st);
+    else if (!wide) ok = queries == 4 ? pg_launch<4, 8, 1>(a, splits, st) : pg_launch<4, 8, 2>(a, splits, st);
+    else ok = pg_launch<8, 16, 1>(a, splits, st);
     if (!ok) return false;
     ZG_SEQ_CHECK();
     return true;

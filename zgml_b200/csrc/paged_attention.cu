@@ -21,7 +21,7 @@ struct PgArgs {
     float scale, cap;
 };
 constexpr uint32_t kPgTile = 32, kPgShift = 29, kPgFlush = 512;      // (512 tiles of 32 products of two bytes: below 2^31)
-constexpr uint32_t kPgLeast = 2;                                     // tiles a warp at least, where there are few
+constexpr uint32_t kPgRows = 8, kPgLeast = 2;                                     // tiles a warp at least, where there are few
 constexpr float kPgSlack = 3.0f;                                     // weights reach 2^(29 + 3)
 // Warps (CTAs) of an SM, by their registers: 168, 128 or 255 a thread.
 constexpr uint32_t pg_warps(int KC, int VC, int NT) { return NT == 1 && KC <= 2 && VC <= 4 ? 16 : NT == 1 && KC <= 4 && VC <= 8 ? 12 : 8; }
@@ -114,39 +114,67 @@ __global__ void __launch_bounds__(32, pg_warps(KC, VC, NT)) k_paged(const __grid
     uint64_t left;                                                   // tiles that the warp takes
     PgGroup group;
     if (a.part) {
-        uint64_t* const before = reinterpret_cast<uint64_t*>(a.plan + 4);      // tiles before each row
+        // Tiles before each row, of all, and the row in which the warp's share begins.  The rows of a step of at most 32 * kPgRows are read at once and kept.
+        uint64_t* const before = reinterpret_cast<uint64_t*>(a.plan + 4);
+        auto upto = [&](uint32_t mine) {
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) { const uint32_t t = __shfl_up_sync(0xffffffffu, mine, o); if (lane >= (uint32_t)o) mine += t; }
+            return mine;
+        };
+        const bool few = a.tokens == 1 && a.B <= 32 * kPgRows;
+        uint32_t kept[kPgRows];
         uint64_t all = 0;
-        uint32_t run = 0;
-        for (uint32_t row = 0; row < live; row += 32) {
-            uint32_t upto = pg_tiles(a, live, row, run);
-            const uint32_t mine = upto;
-            for (int o = 1; o < 32; o <<= 1) { const uint32_t t = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= (uint32_t)o) upto += t; }
-            if (blockIdx.x == 0 && row + lane < live) before[row + lane] = all + upto - mine;
-            all += __shfl_sync(0xffffffffu, upto, 31);
+        if (few) {
+            int2 z[kPgRows];                                         // slot, length
+#pragma unroll
+            for (uint32_t b = 0; b < kPgRows; b++)
+                z[b] = 32 * b + lane < a.B ? *reinterpret_cast<const int2*>(a.table + ZG_BATCH_ROWS + (size_t)4 * (32 * b + lane)) : make_int2(-1, 0);
+#pragma unroll
+            for (uint32_t b = 0; b < kPgRows; b++) {
+                if (32 * b >= live) break;
+                BatchRow x;
+                x.slot = 32 * b + lane < live ? z[b].x : -1; x.length = z[b].y; x.adapter = 0;
+                const uint32_t hi = x.slot >= 0 && page_row_ok(a.pool, s, x) ? x.length : 0, lo = a.window && hi > a.window ? hi - a.window : 0;
+                kept[b] = hi ? (hi + kPgTile - 1) / kPgTile - lo / kPgTile : 0;
+                const uint32_t sum = upto(kept[b]);
+                if (blockIdx.x == 0 && 32 * b + lane < live) before[32 * b + lane] = all + sum - kept[b];
+                all += __shfl_sync(0xffffffffu, sum, 31);
+            }
+        } else {
+            uint32_t run = 0;
+            for (uint32_t row = 0; row < live; row += 32) {
+                const uint32_t mine = pg_tiles(a, live, row, run), sum = upto(mine);
+                if (blockIdx.x == 0 && row + lane < live) before[row + lane] = all + sum - mine;
+                all += __shfl_sync(0xffffffffu, sum, 31);
+            }
         }
-        for (uint32_t row = blockIdx.x; row < live; row += gridDim.x) settle(row);
         const uint64_t total = all * per_row;
         const uint32_t warps = (uint32_t)min((uint64_t)gridDim.x, max((uint64_t)1, total / kPgLeast));
         if (blockIdx.x == 0 && lane == 0) { before[live] = all; a.plan[0] = (uint32_t)total; a.plan[1] = (uint32_t)(total >> 32); a.plan[2] = warps; }
-        if (blockIdx.x >= warps || !total) return;
+        const bool idle = blockIdx.x >= warps || !total;
+        for (uint32_t row = gridDim.x - 1 - blockIdx.x; row < live; row += gridDim.x) settle(row);      // (from the last warp on, which may have nothing else to do)
+        if (idle) return;
         const uint64_t begin = pg_share(total, blockIdx.x, warps), x = begin / per_row;
         left = pg_share(total, blockIdx.x + 1, warps) - begin;
-        uint64_t sum = 0;
-        run = 0;
-        for (uint32_t row = 0;; row += 32) {
-            const uint32_t mine = pg_tiles(a, live, row, run);
-            uint32_t upto = mine;
-            for (int o = 1; o < 32; o <<= 1) { const uint32_t t = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= (uint32_t)o) upto += t; }
-            const uint32_t here = __ballot_sync(0xffffffffu, sum + upto > x);
+        uint64_t seen = 0;
+        uint32_t run = 0;
+        r = item = off = 0;
+        auto look = [&](uint32_t row, uint32_t mine) {
+            const uint32_t sum = upto(mine), here = __ballot_sync(0xffffffffu, seen + sum > x);
             if (here) {
                 const int l = __ffs(here) - 1;
                 const uint32_t tiles = __shfl_sync(0xffffffffu, mine, l);
-                const uint64_t in = begin - (sum + __shfl_sync(0xffffffffu, upto, l) - tiles) * per_row;
+                const uint64_t in = begin - (seen + __shfl_sync(0xffffffffu, sum, l) - tiles) * per_row;
                 r = row + l; item = (uint32_t)(in / tiles); off = (uint32_t)(in % tiles);
-                break;
+                return true;
             }
-            sum += __shfl_sync(0xffffffffu, upto, 31);
-        }
+            seen += __shfl_sync(0xffffffffu, sum, 31);
+            return false;
+        };
+        if (few) {
+#pragma unroll
+            for (uint32_t b = 0; b < kPgRows; b++) if (look(32 * b, kept[b])) break;
+        } else for (uint32_t row = 0; row < live && !look(row, pg_tiles(a, live, row, run)); row += 32) {}
         group = pg_group(a, live, r, batch_row(a.table, r).slot);
     } else {
         r = blockIdx.x / per_row; item = blockIdx.x % per_row; off = 0;
@@ -480,16 +508,17 @@ __global__ void __launch_bounds__(128) k_paged_join(const __grid_constant__ PgAr
     const PageShape& s = a.s;
     const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, r = blockIdx.y, item = blockIdx.x / queries, i = blockIdx.x % queries, per_row = s.G * a.chunks;
     const uint32_t live = batch_head(a.table, a.B).rows;
-    if (r >= live) return;
     const uint64_t* const before = reinterpret_cast<const uint64_t*>(a.plan + 4);
-    const uint64_t all = a.plan[0] | (uint64_t)a.plan[1] << 32, tiles = before[r + 1] - before[r];
-    const uint32_t warps = a.plan[2];
-    if (!tiles) return;
-    const uint64_t first = before[r] * per_row + item * tiles;
+    const uint4 plan = *reinterpret_cast<const uint4*>(a.plan);      // (asked for at once: what belongs to rows that are not live is not looked at)
+    const uint64_t b0 = before[r], b1 = before[r + 1];
+    const BatchRow begins = batch_row(a.table, r);
+    if (r >= live || b1 == b0) return;
+    const uint64_t all = plan.x | (uint64_t)plan.y << 32, tiles = b1 - b0, first = b0 * per_row + item * tiles;
+    const uint32_t warps = plan.z;
     const uint32_t w0 = (uint32_t)(((first + 1) * warps - 1) / all), w1 = (uint32_t)(((first + tiles) * warps - 1) / all), count = w1 - w0 + 1;
     const uint32_t heads = min(a.rep, queries), token = i / heads, g = item / a.chunks, h = item % a.chunks * heads + i % heads;
-    if (w0 == w1 || h >= a.rep || token >= pg_group(a, live, r, batch_row(a.table, r).slot).rows) return;
-    const BatchRow z = batch_row(a.table, r + token);
+    if (w0 == w1 || h >= a.rep || (token && token >= pg_group(a, live, r, begins.slot).rows)) return;
+    const BatchRow z = token ? batch_row(a.table, r + token) : begins;
     if (!page_row_ok(a.pool, s, z) || z.length == 0) return;
     const uint32_t pitch = s.vp + 4;
     auto record = [&](uint32_t k) { return a.part + ((size_t)(2 * (w0 + k) + (k ? 0 : 1)) * queries + i) * pitch; };

@@ -7,17 +7,18 @@ namespace {
 
 struct SmArgs {
     int32_t* dst; const float* logits; const float* table; float* probability;
-    uint32_t B, V, rs, slice;
+    uint32_t B, V, rs, slice, vec;
 };
-constexpr uint32_t kSmThreads = 512, kSmWarps = kSmThreads / 32, kSmBins = 1024, kSmList = 512, kSmCluster = 8, kSmSlice = 40960;
-constexpr uint32_t kSmIndexBits = 20;
+constexpr uint32_t kSmBins = 1024, kSmList = 512, kSmCluster = 8, kSmSlice = 40960;
+constexpr uint32_t kSmIndexBits = 20, kSmIndexMask = (1u << kSmIndexBits) - 1;
+constexpr double kSmOne = 8796093022208.0;                           // 2^43: the largest weight
 typedef unsigned long long u64;
 
 struct SmShared {
     u64 mass[kSmBins]; uint32_t count[kSmBins];
     ulonglong2 list[kSmList], all_list[kSmList];                     // {order, weight} of candidates, own and of the cluster
-    u64 best, total, warp_mass[kSmWarps], found_mass, threshold;
-    uint32_t nan, n_list, found_count, found_bin, warp_count[kSmWarps];
+    u64 best, total, warp_mass[32], found_mass, threshold, found_target;
+    uint32_t nan, n_list[2], n_all, found_count, found_bin, warp_count[32];
 };
 __device__ __forceinline__ uint32_t sm_at(const void* p, uint32_t rank) {
     uint32_t at;
@@ -31,30 +32,32 @@ __device__ __forceinline__ ulonglong2 sm_peer(const ulonglong2* p, uint32_t rank
     asm volatile("ld.shared::cluster.v2.u64 {%0, %1}, [%2];" : "=l"(v.x), "=l"(v.y) : "r"(sm_at(p, rank)) : "memory");
     return v;
 }
-__device__ __forceinline__ void sm_cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
+__device__ __forceinline__ void sm_cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void sm_cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // numbers that are ordered as the floats are (no NaN; -0 has become 0)
 __device__ __forceinline__ uint32_t sm_key(float z) { const uint32_t b = __float_as_uint(z); return b & 0x80000000u ? ~b : b | 0x80000000u; }
 __device__ __forceinline__ float sm_value(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
 // what decides who comes first: the logit, then the lower index
-__device__ __forceinline__ u64 sm_order(float z, uint32_t index) { return ((u64)sm_key(z) << kSmIndexBits) | ((1u << kSmIndexBits) - 1 - index); }
+__device__ __forceinline__ u64 sm_order(float z, uint32_t index) { return ((u64)sm_key(z) << kSmIndexBits) | (kSmIndexMask - index); }
 __device__ __forceinline__ u64 warp_sum64(u64 v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
 
-// A cluster per row, its CTAs each a slice of the vocabulary in shared memory.  What top_k and top_p cut at is found by counts (sums of weights) of the tokens by bins of
-// logits, the bin where the target is passed looked at more closely until at most kSmList candidates are left, which are ranked one against the other.  Weights are whole
-// multiples of 2^-43 of the largest, their sums exact in 64 bits, so that no order of additions changes a choice.
-__global__ void __launch_bounds__(kSmThreads) k_sample(const SmArgs a) {
+// A cluster per row, its CTAs each a slice of the vocabulary: kept in shared memory (KEEP), or read again, from L2, where the rows fill the GPU more than once (with 64 rows of 128256 tokens
+// all logits would take all of its shared memory).  Tokens are counted by bins of logits below the largest, 1 / 32 of an exponent wide; what top_k or top_p cuts off begins in the bin in which
+// the counts (sums of weights) reach their target.  Where at most kSmList tokens lie in the bins up to there, one CTA gets them all and ranks them one against the other; otherwise
+// the bin is looked at more closely until at most so many candidates are left in it.  Weights are whole multiples of 2^-43 of the largest, their sums exact in 64 bits, so that
+// no order of additions changes a choice.
+template <int C, bool KEEP>
+__global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 1 : 4) k_sample(const SmArgs a) {
     pdl_enter();
+    constexpr uint32_t T_ = KEEP ? 512 : 256, kWarps = T_ / 32, kBinsEach = kSmBins / T_;
     extern __shared__ float4 sm_mem[];
     __shared__ SmShared sh;
     float* const z = reinterpret_cast<float*>(sm_mem);
-    const uint32_t r = blockIdx.y, rank = blockIdx.x, C = gridDim.x, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+    const uint32_t r = blockIdx.y, rank = blockIdx.x, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     const BatchHead head = batch_head(a.table, a.B);
     const int4 w0 = *reinterpret_cast<const int4*>(a.table + ZG_BATCH_ROWS + (size_t)ZG_SAMPLE_WORDS * r);
     const float u = a.table[ZG_BATCH_ROWS + (size_t)ZG_SAMPLE_WORDS * r + 4], T = __int_as_float(w0.x), top_p = __int_as_float(w0.z), min_p = __int_as_float(w0.w);
@@ -63,176 +66,304 @@ __global__ void __launch_bounds__(kSmThreads) k_sample(const SmArgs a) {
     const bool ok = T >= 0.0f && T < INFINITY && top_p >= 0.0f && top_p <= 1.0f && min_p >= 0.0f && min_p <= 1.0f && u >= 0.0f && u < 1.0f;
     const uint32_t v0 = min(rank * a.slice, a.V), n = min(a.slice, a.V - v0);
     const float* src = a.logits + (size_t)r * a.rs + v0;
-    if (tid == 0) { sh.best = 0; sh.nan = 0; }
+    // f(logit, place in the slice) for every token of places [from, to), `from` a multiple of 4, four at a time; `again`: they have been read before
+    auto each = [&](uint32_t from, uint32_t to, uint32_t first, uint32_t step, bool again, auto&& f) {
+#pragma unroll 4
+        for (uint32_t i = from + 4 * first; i < to; i += 4 * step) {
+            float4 x;
+            if (KEEP && again) x = *reinterpret_cast<const float4*>(z + i);
+            else if (a.vec && i + 4 <= n) x = *reinterpret_cast<const float4*>(src + i);
+            else { x.x = src[i]; x.y = i + 1 < n ? src[i + 1] : 0.0f; x.z = i + 2 < n ? src[i + 2] : 0.0f; x.w = i + 3 < n ? src[i + 3] : 0.0f; }
+            if (!again || !KEEP) { x.x += 0.0f; x.y += 0.0f; x.z += 0.0f; x.w += 0.0f; }      // (-0 becomes 0)
+            if (KEEP && !again) *reinterpret_cast<float4*>(z + i) = x;
+            f(x.x, i);
+            if (i + 1 < to) f(x.y, i + 1);
+            if (i + 2 < to) f(x.z, i + 2);
+            if (i + 3 < to) f(x.w, i + 3);
+        }
+    };
+    auto cluster_sync = [&] { if (C > 1) { sm_cluster_arrive(); sm_cluster_wait(); } else __syncthreads(); };
+    if (tid == 0) { sh.best = 0; sh.nan = 0; sh.n_all = 0; sh.n_list[0] = sh.n_list[1] = 0; }
+    for (uint32_t i = tid; i < kSmBins; i += T_) { sh.count[i] = 0; sh.mass[i] = 0; }
     __syncthreads();
     {
-        u64 best = 0;
+        float top = -INFINITY;
+        uint32_t where = 0;
         bool nan = false;
-        for (uint32_t i = tid; i < n; i += kSmThreads) {
-            const float x = src[i] + 0.0f;
-            z[i] = x;
-            nan = nan || x != x;
-            best = max(best, sm_order(x, v0 + i));
-        }
+        each(0, n, tid, T_, false, [&](float x, uint32_t i) { nan = nan || x != x; if (x > top) { top = x; where = i; } });
+        u64 best = n ? sm_order(top, v0 + where) : 0;                // (a thread's places ascend: its first largest one)
+        if (top == -INFINITY) best = 0;
         for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
         nan = __any_sync(0xffffffffu, nan);
         if (lane == 0) { atomicMax(&sh.best, best); if (nan) sh.nan = 1; }
     }
     __syncthreads();
-    if (C > 1) sm_cluster_sync();
+    cluster_sync();
     u64 best = 0;
     bool bad = !ok;
+#pragma unroll
     for (uint32_t c = 0; c < C; c++) { best = max(best, sm_peer(&sh.best, c)); bad = bad || sm_peer(&sh.nan, c); }
     const float M = sm_value((uint32_t)(best >> kSmIndexBits));
-    bad = bad || M == -INFINITY;
-    const bool greedy = T == 0.0f;
-    if (bad || greedy) {
+    bad = bad || best == 0;
+    if (bad || T == 0.0f) {
         if (rank == 0 && tid == 0) {
-            a.dst[r] = bad ? -1 : (int32_t)((1u << kSmIndexBits) - 1 - (uint32_t)(best & ((1u << kSmIndexBits) - 1)));
+            a.dst[r] = bad ? -1 : (int32_t)(kSmIndexMask - (uint32_t)(best & kSmIndexMask));
             if (a.probability) a.probability[r] = bad ? kBatchNaN : 1.0f;
         }
-        if (C > 1) sm_cluster_sync();                                // no CTA leaves while it is read
+        cluster_sync();                                              // no CTA leaves while it is read
         return;
     }
-    const double inv_t = 1.0 / (double)T;
-    const float bins_at = 32.0f / T;                                 // bins of 1 / 32 of an exponent; what is below e^-32 has no weight
-    const double least = log((double)min_p);                         // (compared as exponents: those of tokens just below the largest logit round to 1)
+    const double inv_t = 1.0 / (double)T, least = log((double)min_p);      // (min_p is compared as an exponent: those of tokens just below the largest logit round to 1)
+    const float bins_at = 32.0f / T;                                 // what is below e^-32 has no weight
     auto exponent = [&](float x) { return x == M ? 0.0 : ((double)x - (double)M) * inv_t; };
     auto share = [&](float x) { return exp(exponent(x)); };
-    auto weight = [&](float x) { return __double2ull_rn(share(x) * 8796093022208.0); };      // 2^43
+    auto weight = [&](float x) { return (u64)__double2ull_rn(share(x) * kSmOne); };
     auto bin_of = [&](float x) { const float d = (M - x) * bins_at; return d < (float)kSmBins ? (uint32_t)d : x == M ? 0u : kSmBins - 1; };
+    auto draw = [&](float x, uint32_t index, u64 all) {
+        a.dst[r] = (int32_t)index;
+        if (a.probability) a.probability[r] = (float)(share(x) * kSmOne / (double)all);
+    };
+    const bool by_k = top_k != 0 && (uint32_t)top_k < a.V, by_p = top_p < 1.0f;
     u64 threshold = 0;
-    for (int by_mass = 0; by_mass < 2; by_mass++) {
-        if (by_mass ? top_p >= 1.0f : top_k == 0 || (uint32_t)top_k >= a.V) continue;
-        u64 lo = threshold, hi = best, above = 0, target = top_k;
-        uint32_t shift = 0;
-        bool linear = true;
-        for (;;) {
-            for (uint32_t i = tid; i < kSmBins; i += kSmThreads) { sh.count[i] = 0; sh.mass[i] = 0; }
-            if (tid == 0) sh.n_list = 0;
+    // counts (and sums of weights) of the tokens in [lo, hi] by their bins: of equal width below the largest logit, or of the order's numbers
+    auto count_bins = [&](u64 lo, u64 hi, bool linear, uint32_t shift, bool masses) {
+        each(0, n, tid, T_, true, [&](float x, uint32_t i) {
+            const u64 o = sm_order(x, v0 + i);
+            if (o < lo || o > hi) return;
+            const uint32_t b = linear ? bin_of(x) : (uint32_t)((hi - o) >> shift);
+            atomicAdd(&sh.count[b], 1u);
+            if (masses) { const u64 w = weight(x); if (w) atomicAdd(&sh.mass[b], w); }
+        });
+        __syncthreads();
+        cluster_sync();
+    };
+    // Of the cluster's bins: the one in which `target` is reached (with `share_of` >= 0: target = share_of of the sum), how many tokens it has, what comes before it and the tokens up to its end.
+    auto find_bin = [&](bool masses, u64 target, double share_of, u64 above, uint32_t* upto) {
+        u64 mine[kBinsEach];
+        uint32_t here[kBinsEach], tokens = 0;
+        u64 sum = 0;
+#pragma unroll
+        for (uint32_t k = 0; k < kBinsEach; k++) {
+            const uint32_t b = kBinsEach * tid + k;
+            u64 m = 0;
+            uint32_t q = 0;
+#pragma unroll
+            for (uint32_t c = 0; c < C; c++) q += sm_peer(&sh.count[b], c);
+            if (masses) {
+#pragma unroll
+                for (uint32_t c = 0; c < C; c++) m += sm_peer(&sh.mass[b], c);
+            }
+            here[k] = q; mine[k] = masses ? m : q;
+            tokens += q; sum += mine[k];
+        }
+        u64 before = sum;
+        uint32_t tokens_before = tokens;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const u64 t = __shfl_up_sync(0xffffffffu, before, o);
+            const uint32_t q = __shfl_up_sync(0xffffffffu, tokens_before, o);
+            if (lane >= (uint32_t)o) { before += t; tokens_before += q; }
+        }
+        if (lane == 31) { sh.warp_mass[warp] = before; sh.warp_count[warp] = tokens_before; }
+        __syncthreads();
+        u64 all = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < kWarps; i++) {
+            if (i < warp) { before += sh.warp_mass[i]; tokens_before += sh.warp_count[i]; }
+            all += sh.warp_mass[i];
+        }
+        if (share_of >= 0.0) target = max((u64)1, (u64)ceil(share_of * (double)all));
+        before += above - sum;
+        tokens_before -= tokens;
+#pragma unroll
+        for (uint32_t k = 0; k < kBinsEach; k++) {
+            tokens_before += here[k];
+            if (before < target && before + mine[k] >= target) { sh.found_bin = kBinsEach * tid + k; sh.found_count = here[k]; sh.found_mass = before; sh.n_list[0] = tokens_before; sh.found_target = target; }
+            before += mine[k];
+        }
+        __syncthreads();
+        *upto = sh.n_list[0];
+        return sh.found_target;
+    };
+    if (by_k || by_p) {
+        uint32_t upto;
+        count_bins(0, best, true, 0, !by_k);
+        u64 target = find_bin(!by_k, top_k, by_k ? -1.0 : (double)top_p, 0, &upto);
+        const uint32_t first_bin = sh.found_bin;
+        if (upto <= kSmList) {
+            // few: they go to the first CTA
+            each(0, n, tid, T_, true, [&](float x, uint32_t i) {
+                if (bin_of(x) > first_bin) return;
+                uint32_t at;
+                asm volatile("atom.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(sm_at(&sh.n_all, 0)) : "memory");
+                asm volatile("st.shared::cluster.v2.u64 [%0], {%1, %2};" ::"r"(sm_at(&sh.all_list[at], 0)), "l"(sm_order(x, v0 + i)), "l"(weight(x)) : "memory");
+            });
             __syncthreads();
-            for (uint32_t i = tid; i < n; i += kSmThreads) {
-                const float x = z[i];
-                const u64 o = sm_order(x, v0 + i);
-                if (o < lo || o > hi) continue;
-                const uint32_t b = linear ? bin_of(x) : (uint32_t)((hi - o) >> shift);
-                atomicAdd(&sh.count[b], 1u);
-                if (by_mass) { const u64 w = weight(x); if (w) atomicAdd(&sh.mass[b], w); }
+            cluster_sync();                                          // (before that no CTA leaves: its bins are read)
+            if (rank != 0) return;
+            const uint32_t count = sh.n_all;
+            constexpr uint32_t kEach = kSmList / T_;
+            u64 ahead[kEach];
+            bool stays[kEach];
+            ulonglong2 me[kEach];
+            u64 sum = 0;
+            for (uint32_t k = 0; k < kEach; k++) {
+                const uint32_t t = tid + k * T_;
+                stays[k] = false; ahead[k] = 0; me[k] = make_ulonglong2(0, 0);
+                if (t >= count) continue;
+                me[k] = sh.all_list[t];
+                uint32_t before = 0;
+                for (uint32_t i = 0; i < count; i++) { const ulonglong2 x = sh.all_list[i]; if (x.x > me[k].x) { before++; ahead[k] += x.y; } }
+                stays[k] = !by_k || before < (uint32_t)top_k;
+                if (stays[k]) sum += me[k].y;
             }
-            __syncthreads();
-            if (C > 1) sm_cluster_sync();
-            // a thread adds up two neighbours of the cluster's bins, and the block finds the one in which the target is reached
-            u64 mine[2];
-            uint32_t here[2];
-            for (int j = 0; j < 2; j++) {
-                const uint32_t b = 2 * tid + j;
-                u64 m = 0;
-                uint32_t k = 0;
-                for (uint32_t c = 0; c < C; c++) { k += sm_peer(&sh.count[b], c); if (by_mass) m += sm_peer(&sh.mass[b], c); }
-                here[j] = k;
-                mine[j] = by_mass ? m : k;
+            auto block_sum = [&](u64 v) {
+                v = warp_sum64(v);
+                __syncthreads();
+                if (lane == 0) sh.warp_mass[warp] = v;
+                __syncthreads();
+                u64 t = 0;
+                for (uint32_t i = 0; i < kWarps; i++) t += sh.warp_mass[i];
+                return t;
+            };
+            if (by_p) {
+                if (by_k) target = max((u64)1, (u64)ceil((double)top_p * (double)block_sum(sum)));
+                for (uint32_t k = 0; k < kEach; k++) stays[k] = stays[k] && ahead[k] < target;
             }
-            u64 before = mine[0] + mine[1];
-            for (int o = 1; o < 32; o <<= 1) { const u64 t = __shfl_up_sync(0xffffffffu, before, o); if (lane >= (uint32_t)o) before += t; }
-            if (lane == 31) sh.warp_mass[warp] = before;
-            __syncthreads();
-            u64 all = 0;
-            for (uint32_t i = 0; i < kSmWarps; i++) { if (i < warp) before += sh.warp_mass[i]; all += sh.warp_mass[i]; }
-            if (by_mass && linear) target = max((u64)1, (u64)ceil((double)top_p * (double)all));
-            before += above - mine[0] - mine[1];
-            for (int j = 0; j < 2; j++) {
-                if (before < target && before + mine[j] >= target) { sh.found_bin = 2 * tid + j; sh.found_count = here[j]; sh.found_mass = before; }
-                before += mine[j];
+            sum = 0;
+            for (uint32_t k = 0; k < kEach; k++) {
+                const uint32_t t = tid + k * T_;
+                stays[k] = stays[k] && exponent(sm_value((uint32_t)(me[k].x >> kSmIndexBits))) >= least;
+                if (t < count) sh.list[t] = make_ulonglong2(me[k].x & kSmIndexMask, stays[k] ? me[k].y : 0);      // (numbers that fall as indices rise)
+                if (stays[k]) sum += me[k].y;
             }
-            __syncthreads();
-            const uint32_t bin = sh.found_bin, count = sh.found_count;
-            above = sh.found_mass;
-            // where the bin lies in the order
-            if (linear) {
-                auto bound = [&](bool upper) {                       // largest key whose bin is >= bin (upper), or smallest one whose bin is <= bin
-                    uint32_t l = 0x007fffffu, h = (uint32_t)(best >> kSmIndexBits);      // keys from -inf to the largest logit's
-                    while (l < h) {
-                        const uint32_t m = l + (h - l + (upper ? 1 : 0)) / 2, b = bin_of(sm_value(m));
-                        if (upper) { if (b >= bin) l = m; else h = m - 1; }
-                        else { if (b <= bin) h = m; else l = m + 1; }
-                    }
-                    return l;
-                };
-                hi = min(hi, ((u64)bound(true) << kSmIndexBits) | ((1u << kSmIndexBits) - 1));
-                lo = max(lo, (u64)bound(false) << kSmIndexBits);
-                linear = false;
-            } else {
-                hi -= (u64)bin << shift;
-                lo = max(lo, hi >= (1ull << shift) - 1 ? hi - ((1ull << shift) - 1) : 0);
+            const u64 all = block_sum(sum);                          // (its barriers stand between the list's writes and reads)
+            const double drawn = (double)u * (double)all;
+            for (uint32_t k = 0; k < kEach; k++) {
+                if (!stays[k] || !me[k].y) continue;
+                const u64 place = me[k].x & kSmIndexMask;
+                u64 before = 0;
+                for (uint32_t i = 0; i < count; i++) { const ulonglong2 x = sh.list[i]; if (x.x > place) before += x.y; }
+                if (!((double)before > drawn) && (double)(before + me[k].y) > drawn) draw(sm_value((uint32_t)(me[k].x >> kSmIndexBits)), kSmIndexMask - (uint32_t)place, all);
             }
-            if (C > 1) sm_cluster_sync();                            // (peers have read the bins)
-            if (count > kSmList) {
-                shift = 0;
-                while ((hi - lo) >> shift >= kSmBins) shift++;
-                continue;
+            return;
+        }
+        for (int by_mass = by_k ? 0 : 1; by_mass <= (by_p ? 1 : 0); by_mass++) {
+            u64 lo = threshold, hi = best, above = 0;
+            uint32_t shift = 0;
+            bool linear = true, counted = by_mass == !by_k;          // (the bins above are this one's first)
+            for (;;) {
+                if (!counted) {
+                    __syncthreads();
+                    for (uint32_t i = tid; i < kSmBins; i += T_) { sh.count[i] = 0; sh.mass[i] = 0; }
+                    __syncthreads();
+                    count_bins(lo, hi, linear, shift, by_mass);
+                    target = find_bin(by_mass, by_mass ? target : (u64)top_k, by_mass && linear ? (double)top_p : -1.0, above, &upto);
+                }
+                counted = false;
+                const uint32_t bin = sh.found_bin, count = sh.found_count;
+                above = sh.found_mass;
+                // where the bin lies in the order
+                if (linear) {
+                    auto bound = [&](bool upper) {                   // largest key whose bin is >= bin (upper), or smallest one whose bin is <= bin
+                        uint32_t l = 0x007fffffu, h = (uint32_t)(best >> kSmIndexBits);      // keys from -inf to the largest logit's
+                        while (l < h) {
+                            const uint32_t m = l + (h - l + (upper ? 1 : 0)) / 2, b = bin_of(sm_value(m));
+                            if (upper) { if (b >= bin) l = m; else h = m - 1; }
+                            else { if (b <= bin) h = m; else l = m + 1; }
+                        }
+                        return l;
+                    };
+                    hi = min(hi, ((u64)bound(true) << kSmIndexBits) | kSmIndexMask);
+                    lo = max(lo, (u64)bound(false) << kSmIndexBits);
+                    linear = false;
+                } else {
+                    hi -= (u64)bin << shift;
+                    lo = max(lo, hi >= (1ull << shift) - 1 ? hi - ((1ull << shift) - 1) : 0);
+                }
+                if (count > kSmList) {
+                    shift = 0;
+                    while ((hi - lo) >> shift >= kSmBins) shift++;
+                    cluster_sync();                                  // (peers have read the bins)
+                    continue;
+                }
+                uint32_t* const n_list = &sh.n_list[1];
+                each(0, n, tid, T_, true, [&](float x, uint32_t i) {
+                    const u64 o = sm_order(x, v0 + i);
+                    if (o < lo || o > hi) return;
+                    sh.list[atomicAdd(n_list, 1u)] = make_ulonglong2(o, by_mass ? weight(x) : 1);
+                });
+                __syncthreads();
+                cluster_sync();
+                uint32_t at = 0;
+                for (uint32_t c = 0; c < C; c++) {
+                    const uint32_t k = sm_peer(n_list, c);
+                    for (uint32_t i = tid; i < k; i += T_) sh.all_list[at + i] = sm_peer(&sh.list[i], c);
+                    at += k;
+                }
+                __syncthreads();
+                for (uint32_t t = tid; t < count; t += T_) {
+                    const ulonglong2 me = sh.all_list[t];
+                    u64 ahead = above;
+                    for (uint32_t i = 0; i < count; i++) { const ulonglong2 x = sh.all_list[i]; if (x.x > me.x) ahead += x.y; }
+                    if (ahead < target && ahead + me.y >= target) sh.threshold = me.x;
+                }
+                __syncthreads();
+                threshold = sh.threshold;
+                cluster_sync();                                      // (peers have read the list)
+                if (tid == 0) *n_list = 0;
+                break;
             }
-            for (uint32_t i = tid; i < n; i += kSmThreads) {
-                const float x = z[i];
-                const u64 o = sm_order(x, v0 + i);
-                if (o < lo || o > hi) continue;
-                sh.list[atomicAdd(&sh.n_list, 1u)] = make_ulonglong2(o, by_mass ? weight(x) : 1);
-            }
-            __syncthreads();
-            if (C > 1) sm_cluster_sync();
-            for (uint32_t c = 0, at = 0; c < C; c++) {
-                const uint32_t k = sm_peer(&sh.n_list, c);
-                for (uint32_t i = tid; i < k; i += kSmThreads) sh.all_list[at + i] = sm_peer(&sh.list[i], c);
-                at += k;
-            }
-            __syncthreads();
-            if (tid < count) {
-                const ulonglong2 me = sh.all_list[tid];
-                u64 ahead = above;
-                for (uint32_t i = 0; i < count; i++) { const ulonglong2 x = sh.all_list[i]; if (x.x > me.x) ahead += x.y; }
-                if (ahead < target && ahead + me.y >= target) sh.threshold = me.x;
-            }
-            __syncthreads();
-            threshold = sh.threshold;
-            if (C > 1) sm_cluster_sync();                            // (peers have read the list)
-            break;
         }
     }
     // the draw: sums of what stays by warps' parts, then the part in which u of all is passed
-    const uint32_t part = ((n + kSmWarps - 1) / kSmWarps + 31) / 32 * 32, from = min(warp * part, n), to = min(from + part, n);
-    auto stays = [&](uint32_t i) {
-        const float x = z[i];
-        if (sm_order(x, v0 + i) < threshold) return (u64)0;
-        return exponent(x) >= least ? (u64)weight(x) : (u64)0;
-    };
+    const uint32_t part = ((n + kWarps - 1) / kWarps + 127) / 128 * 128, from = min(warp * part, n), to = min(from + part, n);
+    auto stays = [&](float x, uint32_t i) { return sm_order(x, v0 + i) >= threshold && exponent(x) >= least ? weight(x) : (u64)0; };
     u64 sum = 0;
-    for (uint32_t i = from + lane; i < to; i += 32) sum += stays(i);
+    each(from, to, lane, 32, true, [&](float x, uint32_t i) { sum += stays(x, i); });
     sum = warp_sum64(sum);
+    __syncthreads();
     if (lane == 0) sh.warp_mass[warp] = sum;
     __syncthreads();
-    if (tid == 0) { u64 t = 0; for (uint32_t i = 0; i < kSmWarps; i++) t += sh.warp_mass[i]; sh.total = t; }
+    if (tid == 0) { u64 t = 0; for (uint32_t i = 0; i < kWarps; i++) t += sh.warp_mass[i]; sh.total = t; }
     __syncthreads();
-    if (C > 1) sm_cluster_sync();
+    cluster_sync();
     u64 all = 0, base = 0;
+#pragma unroll
     for (uint32_t c = 0; c < C; c++) { const u64 t = sm_peer(&sh.total, c); all += t; if (c < rank) base += t; }
     const double drawn = (double)u * (double)all;
     for (uint32_t i = 0; i < warp; i++) base += sh.warp_mass[i];
     if (!((double)base > drawn) && (double)(base + sum) > drawn) {
         for (uint32_t i = from; i < to; i += 32) {
-            const u64 w = i + lane < to ? stays(i + lane) : 0;
-            u64 upto = w;
+            const bool in = i + lane < to;
+            const float x = in ? (KEEP ? z[i + lane] : src[i + lane] + 0.0f) : 0.0f;
+            u64 upto = in ? stays(x, i + lane) : 0;
+#pragma unroll
             for (int o = 1; o < 32; o <<= 1) { const u64 t = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= (uint32_t)o) upto += t; }
             const uint32_t passed = __ballot_sync(0xffffffffu, (double)(base + upto) > drawn);
             if (passed) {
-                if ((int)lane == __ffs(passed) - 1) {
-                    a.dst[r] = (int32_t)(v0 + i + lane);
-                    if (a.probability) a.probability[r] = (float)(share(z[i + lane]) * 8796093022208.0 / (double)all);
-                }
+                if ((int)lane == __ffs(passed) - 1) draw(x, v0 + i + lane, all);
                 break;
             }
             base += __shfl_sync(0xffffffffu, upto, 31);
         }
     }
-    if (C > 1) sm_cluster_sync();                                    // no CTA leaves while its sums are read
+    cluster_sync();                                                  // no CTA leaves while its sums are read
+}
+
+template <int C, bool KEEP>
+bool sm_launch(const SmArgs& a, cudaStream_t st) {
+    if (KEEP && !zg_smem_limit<k_sample<C, KEEP>>(sizeof(float) * kSmSlice)) return false;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(C, a.B); cfg.blockDim = dim3(KEEP ? 512 : 256); cfg.dynamicSmemBytes = KEEP ? sizeof(float) * a.slice : 0; cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = g_zg_pdl ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = C; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr; cfg.numAttrs = 2;
+    cudaLaunchKernelEx(&cfg, k_sample<C, KEEP>, a);
+    return true;
 }
 
 }  // namespace
@@ -253,18 +384,11 @@ bool zg_launch_sample(const ZgOp& op, float* const* bufs, cudaStream_t st) {
     a.dst = reinterpret_cast<int32_t*>(bufs[s.buf[0]]) + s.off[0]; a.logits = bufs[s.buf[1]] + s.off[1]; a.table = bufs[s.buf[2]];
     a.probability = s.buf[3] == ZG_NO_BUF ? nullptr : bufs[s.buf[3]] + s.off[2];
     a.B = s.n[0]; a.V = s.n[1]; a.rs = s.n[2];
+    a.vec = a.rs % 4 == 0 && (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0;
     const uint32_t C = a.V <= 1024 ? 1 : kSmCluster;
     a.slice = ((a.V + C - 1) / C + 3) / 4 * 4;
-    if (!zg_smem_limit<k_sample>(sizeof(float) * kSmSlice)) return false;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(C, a.B); cfg.blockDim = dim3(kSmThreads); cfg.dynamicSmemBytes = sizeof(float) * a.slice; cfg.stream = st;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = g_zg_pdl ? 1 : 0;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = C; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr; cfg.numAttrs = 2;
-    cudaLaunchKernelEx(&cfg, k_sample, a);
+    const bool keep = C == 1 || a.B * C <= 2 * zg_sm_count();
+    if (!(C == 1 ? sm_launch<1, true>(a, st) : keep ? sm_launch<kSmCluster, true>(a, st) : sm_launch<kSmCluster, false>(a, st))) return false;
     ZG_SEQ_CHECK();
     return true;
 }

@@ -9,14 +9,15 @@ struct SmArgs {
     int32_t* dst; const float* logits; const float* table; float* probability;
     uint32_t B, V, rs, slice, vec;
 };
-constexpr uint32_t kSmBins = 1024, kSmList = 512, kSmCluster = 8, kSmSlice = 40960;
+constexpr uint32_t kSmBins = 1024, kSmList = 1024, kSmFew = 512, kSmCluster = 8, kSmSlice = 40960;
 constexpr uint32_t kSmIndexBits = 20, kSmIndexMask = (1u << kSmIndexBits) - 1;
 constexpr double kSmOne = 8796093022208.0;                           // 2^43: the largest weight
 typedef unsigned long long u64;
 
 struct SmShared {
-    u64 mass[kSmBins]; uint32_t count[kSmBins];
+    uint32_t mass_low[kSmBins], mass_high[kSmBins], count[kSmBins];      // (sums of 64 bits by words: additions of 64 bits to shared memory are loops)
     ulonglong2 list[kSmList], all_list[kSmList];                     // {order, weight} of candidates, own and of the cluster
+    double table[32];                                                // 2^(i / 32)
     u64 best, total, warp_mass[32], found_mass, threshold, found_target;
     uint32_t nan, n_list[2], n_all, found_count, found_bin, warp_count[32];
 };
@@ -45,13 +46,24 @@ __device__ __forceinline__ u64 warp_sum64(u64 v) {
     return v;
 }
 
+// round(2^43 e^x), x <= 0: 2^(k / 32) of a table times the exponential's series up to f^5, |f| <= ln 2 / 64, whose next term is below 2^-48 (reduction by a table: P. Tang,
+// ACM Transactions on Mathematical Software 15, 1989).
+__device__ __forceinline__ u64 sm_weight(double x, const double* table) {
+    if (!(x > -32.0)) return 0;
+    const double k = rint(x * 46.166241308446828384);               // 32 / ln 2
+    const double f = fma(k, -0.021660849392498290, x);               // ln 2 / 32
+    const int n = (int)k;
+    const double p = fma(f, fma(f, fma(f, fma(f, 1.0 / 120.0, 1.0 / 24.0), 1.0 / 6.0), 0.5), 1.0);
+    return __double2ull_rn(fma(p * f, table[n & 31], table[n & 31]) * __hiloint2double((1023 + 43 + (n >> 5)) << 20, 0));
+}
+
 // A cluster per row, its CTAs each a slice of the vocabulary: kept in shared memory (KEEP), or read again, from L2, where the rows fill the GPU more than once (with 64 rows of 128256 tokens
-// all logits would take all of its shared memory).  Tokens are counted by bins of logits below the largest, 1 / 32 of an exponent wide; what top_k or top_p cuts off begins in the bin in which
-// the counts (sums of weights) reach their target.  Where at most kSmList tokens lie in the bins up to there, one CTA gets them all and ranks them one against the other; otherwise
-// the bin is looked at more closely until at most so many candidates are left in it.  Weights are whole multiples of 2^-43 of the largest, their sums exact in 64 bits, so that
+// all logits would take all of its shared memory).  Tokens are counted by bins of logits below the largest, 1 / 64 of an exponent wide; what top_k or top_p cuts off begins in the bin in which
+// the counts (sums of weights) reach their target.  Where at most kSmFew tokens lie in the bins up to there, one CTA gets them all and ranks them one against the other; otherwise
+// the bin is looked at more closely until at most kSmList candidates are left in it, of which each CTA ranks its own.  Weights are whole multiples of 2^-43 of the largest, their sums exact in 64 bits, so that
 // no order of additions changes a choice.
 template <int C, bool KEEP>
-__global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 1 : 4) k_sample(const SmArgs a) {
+__global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 2 : 4) k_sample(const SmArgs a) {
     pdl_enter();
     constexpr uint32_t T_ = KEEP ? 512 : 256, kWarps = T_ / 32, kBinsEach = kSmBins / T_;
     extern __shared__ float4 sm_mem[];
@@ -68,7 +80,7 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 1 : 4) k_sample(const
     const float* src = a.logits + (size_t)r * a.rs + v0;
     // f(logit, place in the slice) for every token of places [from, to), `from` a multiple of 4, four at a time; `again`: they have been read before
     auto each = [&](uint32_t from, uint32_t to, uint32_t first, uint32_t step, bool again, auto&& f) {
-#pragma unroll 4
+#pragma unroll 1
         for (uint32_t i = from + 4 * first; i < to; i += 4 * step) {
             float4 x;
             if (KEEP && again) x = *reinterpret_cast<const float4*>(z + i);
@@ -83,8 +95,9 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 1 : 4) k_sample(const
         }
     };
     auto cluster_sync = [&] { if (C > 1) { sm_cluster_arrive(); sm_cluster_wait(); } else __syncthreads(); };
+    if (tid < 32) sh.table[tid] = exp2(tid / 32.0);
     if (tid == 0) { sh.best = 0; sh.nan = 0; sh.n_all = 0; sh.n_list[0] = sh.n_list[1] = 0; }
-    for (uint32_t i = tid; i < kSmBins; i += T_) { sh.count[i] = 0; sh.mass[i] = 0; }
+    for (uint32_t i = tid; i < kSmBins; i += T_) sh.count[i] = sh.mass_low[i] = sh.mass_high[i] = 0;
     __syncthreads();
     {
         float top = -INFINITY;
@@ -114,10 +127,10 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 1 : 4) k_sample(const
         return;
     }
     const double inv_t = 1.0 / (double)T, least = log((double)min_p);      // (min_p is compared as an exponent: those of tokens just below the largest logit round to 1)
-    const float bins_at = 32.0f / T;                                 // what is below e^-32 has no weight
+    const float bins_at = 64.0f / T;                                 // (the last bin: all below e^-16 of the largest)
     auto exponent = [&](float x) { return x == M ? 0.0 : ((double)x - (double)M) * inv_t; };
     auto share = [&](float x) { return exp(exponent(x)); };
-    auto weight = [&](float x) { return (u64)__double2ull_rn(share(x) * kSmOne); };
+    auto weight = [&](float x) { return sm_weight(exponent(x), sh.table); };
     auto bin_of = [&](float x) { const float d = (M - x) * bins_at; return d < (float)kSmBins ? (uint32_t)d : x == M ? 0u : kSmBins - 1; };
     auto draw = [&](float x, uint32_t index, u64 all) {
         a.dst[r] = (int32_t)index;
@@ -128,11 +141,19 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 1 : 4) k_sample(const
     // counts (and sums of weights) of the tokens in [lo, hi] by their bins: of equal width below the largest logit, or of the order's numbers
     auto count_bins = [&](u64 lo, u64 hi, bool linear, uint32_t shift, bool masses) {
         each(0, n, tid, T_, true, [&](float x, uint32_t i) {
-            const u64 o = sm_order(x, v0 + i);
-            if (o < lo || o > hi) return;
-            const uint32_t b = linear ? bin_of(x) : (uint32_t)((hi - o) >> shift);
+            uint32_t b;
+            if (lo == 0 && linear) b = bin_of(x);                    // (all of them)
+            else {
+                const u64 o = sm_order(x, v0 + i);
+                if (o < lo || o > hi) return;
+                b = linear ? bin_of(x) : (uint32_t)((hi - o) >> shift);
+            }
             atomicAdd(&sh.count[b], 1u);
-            if (masses) { const u64 w = weight(x); if (w) atomicAdd(&sh.mass[b], w); }
+            if (masses) {
+                const u64 w = weight(x);
+                const uint32_t low = (uint32_t)w, old = atomicAdd(&sh.mass_low[b], low), high = (uint32_t)(w >> 32) + (old + low < old);
+                if (high) atomicAdd(&sh.mass_high[b], high);
+            }
         });
         __syncthreads();
         cluster_sync();
@@ -151,7 +172,7 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 1 : 4) k_sample(const
             for (uint32_t c = 0; c < C; c++) q += sm_peer(&sh.count[b], c);
             if (masses) {
 #pragma unroll
-                for (uint32_t c = 0; c < C; c++) m += sm_peer(&sh.mass[b], c);
+                for (uint32_t c = 0; c < C; c++) m += sm_peer(&sh.mass_low[b], c) + ((u64)sm_peer(&sh.mass_high[b], c) << 32);
             }
             here[k] = q; mine[k] = masses ? m : q;
             tokens += q; sum += mine[k];
@@ -190,7 +211,7 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 1 : 4) k_sample(const
         count_bins(0, best, true, 0, !by_k);
         u64 target = find_bin(!by_k, top_k, by_k ? -1.0 : (double)top_p, 0, &upto);
         const uint32_t first_bin = sh.found_bin;
-        if (upto <= kSmList) {
+        if (upto <= kSmFew) {
             // few: they go to the first CTA
             each(0, n, tid, T_, true, [&](float x, uint32_t i) {
                 if (bin_of(x) > first_bin) return;
@@ -202,7 +223,7 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 1 : 4) k_sample(const
             cluster_sync();                                          // (before that no CTA leaves: its bins are read)
             if (rank != 0) return;
             const uint32_t count = sh.n_all;
-            constexpr uint32_t kEach = kSmList / T_;
+            constexpr uint32_t kEach = kSmFew / T_;
             u64 ahead[kEach];
             bool stays[kEach];
             ulonglong2 me[kEach];
@@ -255,7 +276,7 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 1 : 4) k_sample(const
             for (;;) {
                 if (!counted) {
                     __syncthreads();
-                    for (uint32_t i = tid; i < kSmBins; i += T_) { sh.count[i] = 0; sh.mass[i] = 0; }
+                    for (uint32_t i = tid; i < kSmBins; i += T_) sh.count[i] = sh.mass_low[i] = sh.mass_high[i] = 0;
                     __syncthreads();
                     count_bins(lo, hi, linear, shift, by_mass);
                     target = find_bin(by_mass, by_mass ? target : (u64)top_k, by_mass && linear ? (double)top_p : -1.0, above, &upto);
@@ -263,25 +284,25 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 1 : 4) k_sample(const
                 counted = false;
                 const uint32_t bin = sh.found_bin, count = sh.found_count;
                 above = sh.found_mass;
-                // where the bin lies in the order
-                if (linear) {
-                    auto bound = [&](bool upper) {                   // largest key whose bin is >= bin (upper), or smallest one whose bin is <= bin
-                        uint32_t l = 0x007fffffu, h = (uint32_t)(best >> kSmIndexBits);      // keys from -inf to the largest logit's
-                        while (l < h) {
-                            const uint32_t m = l + (h - l + (upper ? 1 : 0)) / 2, b = bin_of(sm_value(m));
-                            if (upper) { if (b >= bin) l = m; else h = m - 1; }
-                            else { if (b <= bin) h = m; else l = m + 1; }
-                        }
-                        return l;
-                    };
-                    hi = min(hi, ((u64)bound(true) << kSmIndexBits) | kSmIndexMask);
-                    lo = max(lo, (u64)bound(false) << kSmIndexBits);
-                    linear = false;
-                } else {
-                    hi -= (u64)bin << shift;
-                    lo = max(lo, hi >= (1ull << shift) - 1 ? hi - ((1ull << shift) - 1) : 0);
-                }
                 if (count > kSmList) {
+                    // where the bin lies in the order, and bins of that
+                    if (linear) {
+                        auto bound = [&](bool upper) {               // largest key whose bin is >= bin (upper), or smallest one whose bin is <= bin
+                            uint32_t l = 0x007fffffu, h = (uint32_t)(best >> kSmIndexBits);      // keys from -inf to the largest logit's
+                            while (l < h) {
+                                const uint32_t m = l + (h - l + (upper ? 1 : 0)) / 2, b = bin_of(sm_value(m));
+                                if (upper) { if (b >= bin) l = m; else h = m - 1; }
+                                else { if (b <= bin) h = m; else l = m + 1; }
+                            }
+                            return l;
+                        };
+                        hi = min(hi, ((u64)bound(true) << kSmIndexBits) | kSmIndexMask);
+                        lo = max(lo, (u64)bound(false) << kSmIndexBits);
+                        linear = false;
+                    } else {
+                        hi -= (u64)bin << shift;
+                        lo = max(lo, hi >= (1ull << shift) - 1 ? hi - ((1ull << shift) - 1) : 0);
+                    }
                     shift = 0;
                     while ((hi - lo) >> shift >= kSmBins) shift++;
                     cluster_sync();                                  // (peers have read the bins)
@@ -290,7 +311,7 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 1 : 4) k_sample(const
                 uint32_t* const n_list = &sh.n_list[1];
                 each(0, n, tid, T_, true, [&](float x, uint32_t i) {
                     const u64 o = sm_order(x, v0 + i);
-                    if (o < lo || o > hi) return;
+                    if (o < lo || o > hi || (linear ? bin_of(x) : (uint32_t)((hi - o) >> shift)) != bin) return;
                     sh.list[atomicAdd(n_list, 1u)] = make_ulonglong2(o, by_mass ? weight(x) : 1);
                 });
                 __syncthreads();
@@ -302,15 +323,16 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 1 : 4) k_sample(const
                     at += k;
                 }
                 __syncthreads();
-                for (uint32_t t = tid; t < count; t += T_) {
-                    const ulonglong2 me = sh.all_list[t];
-                    u64 ahead = above;
-                    for (uint32_t i = 0; i < count; i++) { const ulonglong2 x = sh.all_list[i]; if (x.x > me.x) ahead += x.y; }
-                    if (ahead < target && ahead + me.y >= target) sh.threshold = me.x;
+                for (uint32_t t = warp; t < *n_list; t += kWarps) {
+                    const ulonglong2 me = sh.list[t];
+                    u64 ahead = 0;
+                    for (uint32_t i = lane; i < count; i += 32) { const ulonglong2 x = sh.all_list[i]; if (x.x > me.x) ahead += x.y; }
+                    ahead = above + warp_sum64(ahead);
+                    if (ahead < target && ahead + me.y >= target && lane < C) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(sm_at(&sh.threshold, lane)), "l"(me.x) : "memory");
                 }
                 __syncthreads();
+                cluster_sync();                                      // (and peers have read the list)
                 threshold = sh.threshold;
-                cluster_sync();                                      // (peers have read the list)
                 if (tid == 0) *n_list = 0;
                 break;
             }
@@ -318,7 +340,13 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 1 : 4) k_sample(const
     }
     // the draw: sums of what stays by warps' parts, then the part in which u of all is passed
     const uint32_t part = ((n + kWarps - 1) / kWarps + 127) / 128 * 128, from = min(warp * part, n), to = min(from + part, n);
-    auto stays = [&](float x, uint32_t i) { return sm_order(x, v0 + i) >= threshold && exponent(x) >= least ? weight(x) : (u64)0; };
+    const float last = threshold ? sm_value((uint32_t)(threshold >> kSmIndexBits)) : -INFINITY;      // what stays: larger logits, and this one up to an index
+    const uint32_t last_index = threshold ? kSmIndexMask - (uint32_t)(threshold & kSmIndexMask) : 0xffffffffu;
+    auto stays = [&](float x, uint32_t i) {
+        if (x < last || (x == last && v0 + i > last_index)) return (u64)0;
+        const double e = exponent(x);
+        return e >= least ? sm_weight(e, sh.table) : (u64)0;
+    };
     u64 sum = 0;
     each(from, to, lane, 32, true, [&](float x, uint32_t i) { sum += stays(x, i); });
     sum = warp_sum64(sum);
@@ -334,15 +362,30 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 1 : 4) k_sample(const
     const double drawn = (double)u * (double)all;
     for (uint32_t i = 0; i < warp; i++) base += sh.warp_mass[i];
     if (!((double)base > drawn) && (double)(base + sum) > drawn) {
-        for (uint32_t i = from; i < to; i += 32) {
-            const bool in = i + lane < to;
-            const float x = in ? (KEEP ? z[i + lane] : src[i + lane] + 0.0f) : 0.0f;
-            u64 upto = in ? stays(x, i + lane) : 0;
+        for (uint32_t i = from; i < to; i += 128) {                  // a lane's four neighbours at a time
+            float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            u64 w[4] = {0, 0, 0, 0}, mine = 0;
+            each(i, min(i + 128, to), lane, 32, true, [&](float v, uint32_t at) {
+                const uint32_t k = at & 3;
+                const u64 y = stays(v, at);
+#pragma unroll
+                for (uint32_t q = 0; q < 4; q++) if (q == k) { x[q] = v; w[q] = y; }
+                mine += y;
+            });
+            u64 upto = mine;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) { const u64 t = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= (uint32_t)o) upto += t; }
             const uint32_t passed = __ballot_sync(0xffffffffu, (double)(base + upto) > drawn);
             if (passed) {
-                if ((int)lane == __ffs(passed) - 1) draw(x, v0 + i + lane, all);
+                if ((int)lane == __ffs(passed) - 1) {
+                    u64 at = base + upto - mine;
+                    bool found = false;
+#pragma unroll
+                    for (uint32_t q = 0; q < 4; q++) {
+                        at += w[q];
+                        if (!found && (double)at > drawn) { found = true; draw(x[q], v0 + i + 4 * lane + q, all); }
+                    }
+                }
                 break;
             }
             base += __shfl_sync(0xffffffffu, upto, 31);

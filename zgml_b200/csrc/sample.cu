@@ -2,6 +2,7 @@
 #include "batch_table.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
@@ -9,29 +10,29 @@ struct SmArgs {
     int32_t* dst; const float* logits; const float* table; float* probability;
     uint32_t B, V, rs, slice, vec;
 };
-constexpr uint32_t kSmBins = 1024, kSmList = 1024, kSmFew = 512, kSmCluster = 8, kSmSlice = 40960;
+constexpr uint32_t kSmBins = 1024, kSmList = 1024, kSmCluster = 8, kSmSlice = 40960;
 constexpr uint32_t kSmIndexBits = 20, kSmIndexMask = (1u << kSmIndexBits) - 1;
 constexpr double kSmOne = 8796093022208.0;                           // 2^43: the largest weight
 typedef unsigned long long u64;
 
 struct SmShared {
-    uint32_t mass_low[kSmBins], mass_high[kSmBins], count[kSmBins];      // (sums of 64 bits by words: additions of 64 bits to shared memory are loops)
+    alignas(16) uint32_t mass_low[kSmBins], mass_high[kSmBins], count[kSmBins];      // (sums of 64 bits by words: additions of 64 bits to shared memory are loops)
     ulonglong2 list[kSmList], all_list[kSmList];                     // {order, weight} of candidates, own and of the cluster
     double table[32];                                                // 2^(i / 32)
     u64 best, total, warp_mass[32], found_mass, threshold, found_target;
-    uint32_t nan, n_list[2], n_all, found_count, found_bin, warp_count[32];
+    uint32_t n_list[2], n_all, found_count, found_bin, warp_count[32];
 };
 __device__ __forceinline__ uint32_t sm_at(const void* p, uint32_t rank) {
     uint32_t at;
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
     return at;
 }
-__device__ __forceinline__ uint32_t sm_peer(const uint32_t* p, uint32_t rank) { uint32_t v; asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(sm_at(p, rank)) : "memory"); return v; }
-__device__ __forceinline__ u64 sm_peer(const u64* p, uint32_t rank) { u64 v; asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(sm_at(p, rank)) : "memory"); return v; }
-__device__ __forceinline__ ulonglong2 sm_peer(const ulonglong2* p, uint32_t rank) {
-    ulonglong2 v;
-    asm volatile("ld.shared::cluster.v2.u64 {%0, %1}, [%2];" : "=l"(v.x), "=l"(v.y) : "r"(sm_at(p, rank)) : "memory");
-    return v;
+// the same place of another CTA of the cluster, as an address of ordinary loads, of which many are under way at once
+template <class X>
+__device__ __forceinline__ const X* sm_peer(const X* p, uint32_t rank) {
+    const X* at;
+    asm("mapa.u64 %0, %1, %2;" : "=l"(at) : "l"(p), "r"(rank));
+    return at;
 }
 __device__ __forceinline__ void sm_cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void sm_cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
@@ -48,18 +49,20 @@ __device__ __forceinline__ u64 warp_sum64(u64 v) {
 
 // round(2^43 e^x), x <= 0: 2^(k / 32) of a table times the exponential's series up to f^5, |f| <= ln 2 / 64, whose next term is below 2^-48 (reduction by a table: P. Tang,
 // ACM Transactions on Mathematical Software 15, 1989).
+// Whole numbers are taken from the mantissa of sums with 2^52: conversions of 64 bits are slow (a draw from 64 rows of 128256 tokens took 58 us with them).
 __device__ __forceinline__ u64 sm_weight(double x, const double* table) {
     if (!(x > -32.0)) return 0;
-    const double k = rint(x * 46.166241308446828384);               // 32 / ln 2
+    const double shifted = fma(x, 46.166241308446828384, 6755399441055744.0), k = shifted - 6755399441055744.0;      // 32 / ln 2; 1.5 * 2^52
     const double f = fma(k, -0.021660849392498290, x);               // ln 2 / 32
-    const int n = (int)k;
-    const double p = fma(f, fma(f, fma(f, fma(f, 1.0 / 120.0, 1.0 / 24.0), 1.0 / 6.0), 0.5), 1.0);
-    return __double2ull_rn(fma(p * f, table[n & 31], table[n & 31]) * __hiloint2double((1023 + 43 + (n >> 5)) << 20, 0));
+    const int n = __double2loint(shifted);
+    const double p = fma(f, fma(f, fma(f, fma(f, 1.0 / 120.0, 1.0 / 24.0), 1.0 / 6.0), 0.5), 1.0), t = table[n & 31];
+    const double w = fma(fma(p * f, t, t), __hiloint2double((1023 + 43 + (n >> 5)) << 20, 0), 4503599627370496.0);
+    return (u64)__double_as_longlong(w) & 0xfffffffffffffull;
 }
 
 // A cluster per row, its CTAs each a slice of the vocabulary: kept in shared memory (KEEP), or read again, from L2, where the rows fill the GPU more than once (with 64 rows of 128256 tokens
 // all logits would take all of its shared memory).  Tokens are counted by bins of logits below the largest, 1 / 64 of an exponent wide; what top_k or top_p cuts off begins in the bin in which
-// the counts (sums of weights) reach their target.  Where at most kSmFew tokens lie in the bins up to there, one CTA gets them all and ranks them one against the other; otherwise
+// the counts (sums of weights) reach their target.  Where at most kSmList tokens lie in the bins up to there, one CTA gets them all and ranks them one against the other; otherwise
 // the bin is looked at more closely until at most kSmList candidates are left in it, of which each CTA ranks its own.  Weights are whole multiples of 2^-43 of the largest, their sums exact in 64 bits, so that
 // no order of additions changes a choice.
 template <int C, bool KEEP>
@@ -78,46 +81,60 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 2 : 4) k_sample(const
     const bool ok = T >= 0.0f && T < INFINITY && top_p >= 0.0f && top_p <= 1.0f && min_p >= 0.0f && min_p <= 1.0f && u >= 0.0f && u < 1.0f;
     const uint32_t v0 = min(rank * a.slice, a.V), n = min(a.slice, a.V - v0);
     const float* src = a.logits + (size_t)r * a.rs + v0;
-    // f(logit, place in the slice) for every token of places [from, to), `from` a multiple of 4, four at a time; `again`: they have been read before
-    auto each = [&](uint32_t from, uint32_t to, uint32_t first, uint32_t step, bool again, auto&& f) {
+    auto four = [&](uint32_t i, bool again) {                        // tokens i .. i + 3 of the slice, i a multiple of 4; what is behind its end counts nothing
+        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (i >= n) return x;
+        if (KEEP && again) return *reinterpret_cast<const float4*>(z + i);
+        if (a.vec && i + 4 <= n) x = *reinterpret_cast<const float4*>(src + i);
+        else { x.x = src[i]; if (i + 1 < n) x.y = src[i + 1]; if (i + 2 < n) x.z = src[i + 2]; if (i + 3 < n) x.w = src[i + 3]; }
+        x.x += 0.0f; x.y += 0.0f; x.z += 0.0f; x.w += 0.0f;          // (-0 becomes 0)
+        return x;
+    };
+    // f(logit, place in the slice) for every token of places [from, to), four at a time, the next ones asked for before.  (What f does is long: loops that are not unrolled stay in the
+    // instruction cache.)
+    auto each = [&](uint32_t from, uint32_t to, uint32_t first, uint32_t step, auto&& f) {
+        uint32_t i = from + 4 * first;
+        float4 x = four(i, true), y = four(i + 4 * step, true);
 #pragma unroll 1
-        for (uint32_t i = from + 4 * first; i < to; i += 4 * step) {
-            float4 x;
-            if (KEEP && again) x = *reinterpret_cast<const float4*>(z + i);
-            else if (a.vec && i + 4 <= n) x = *reinterpret_cast<const float4*>(src + i);
-            else { x.x = src[i]; x.y = i + 1 < n ? src[i + 1] : 0.0f; x.z = i + 2 < n ? src[i + 2] : 0.0f; x.w = i + 3 < n ? src[i + 3] : 0.0f; }
-            if (!again || !KEEP) { x.x += 0.0f; x.y += 0.0f; x.z += 0.0f; x.w += 0.0f; }      // (-0 becomes 0)
-            if (KEEP && !again) *reinterpret_cast<float4*>(z + i) = x;
+        for (; i < to; i += 4 * step) {
+            const float4 next = four(i + 8 * step, true);
             f(x.x, i);
             if (i + 1 < to) f(x.y, i + 1);
             if (i + 2 < to) f(x.z, i + 2);
             if (i + 3 < to) f(x.w, i + 3);
+            x = y; y = next;
         }
     };
     auto cluster_sync = [&] { if (C > 1) { sm_cluster_arrive(); sm_cluster_wait(); } else __syncthreads(); };
     if (tid < 32) sh.table[tid] = exp2(tid / 32.0);
-    if (tid == 0) { sh.best = 0; sh.nan = 0; sh.n_all = 0; sh.n_list[0] = sh.n_list[1] = 0; }
+    if (tid == 0) { sh.best = 0; sh.n_all = 0; sh.n_list[0] = sh.n_list[1] = 0; }
     for (uint32_t i = tid; i < kSmBins; i += T_) sh.count[i] = sh.mass_low[i] = sh.mass_high[i] = 0;
     __syncthreads();
     {
         float top = -INFINITY;
         uint32_t where = 0;
         bool nan = false;
-        each(0, n, tid, T_, false, [&](float x, uint32_t i) { nan = nan || x != x; if (x > top) { top = x; where = i; } });
+#pragma unroll 4
+        for (uint32_t i = 4 * tid; i < n; i += 4 * T_) {
+            const float4 x = four(i, false);
+            if (KEEP) *reinterpret_cast<float4*>(z + i) = x;
+            const float v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (uint32_t k = 0; k < 4; k++) if (i + k < n) { nan = nan || v[k] != v[k]; if (v[k] > top) { top = v[k]; where = i + k; } }
+        }
         u64 best = n ? sm_order(top, v0 + where) : 0;                // (a thread's places ascend: its first largest one)
         if (top == -INFINITY) best = 0;
         for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-        nan = __any_sync(0xffffffffu, nan);
-        if (lane == 0) { atomicMax(&sh.best, best); if (nan) sh.nan = 1; }
+        if (__any_sync(0xffffffffu, nan)) best = ~0ull;
+        if (lane == 0) atomicMax(&sh.best, best);
     }
     __syncthreads();
     cluster_sync();
     u64 best = 0;
-    bool bad = !ok;
 #pragma unroll
-    for (uint32_t c = 0; c < C; c++) { best = max(best, sm_peer(&sh.best, c)); bad = bad || sm_peer(&sh.nan, c); }
+    for (uint32_t c = 0; c < C; c++) best = max(best, *sm_peer(&sh.best, c));
     const float M = sm_value((uint32_t)(best >> kSmIndexBits));
-    bad = bad || best == 0;
+    const bool bad = !ok || best == 0 || best == ~0ull;              // (nothing above -inf; something that is no number)
     if (bad || T == 0.0f) {
         if (rank == 0 && tid == 0) {
             a.dst[r] = bad ? -1 : (int32_t)(kSmIndexMask - (uint32_t)(best & kSmIndexMask));
@@ -140,7 +157,7 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 2 : 4) k_sample(const
     u64 threshold = 0;
     // counts (and sums of weights) of the tokens in [lo, hi] by their bins: of equal width below the largest logit, or of the order's numbers
     auto count_bins = [&](u64 lo, u64 hi, bool linear, uint32_t shift, bool masses) {
-        each(0, n, tid, T_, true, [&](float x, uint32_t i) {
+        each(0, n, tid, T_, [&](float x, uint32_t i) {
             uint32_t b;
             if (lo == 0 && linear) b = bin_of(x);                    // (all of them)
             else {
@@ -160,22 +177,28 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 2 : 4) k_sample(const
     };
     // Of the cluster's bins: the one in which `target` is reached (with `share_of` >= 0: target = share_of of the sum), how many tokens it has, what comes before it and the tokens up to its end.
     auto find_bin = [&](bool masses, u64 target, double share_of, u64 above, uint32_t* upto) {
-        u64 mine[kBinsEach];
-        uint32_t here[kBinsEach], tokens = 0;
+        typedef typename std::conditional<kBinsEach == 4, uint4, uint2>::type Bins;
+        u64 mine[kBinsEach] = {};
+        uint32_t here[kBinsEach] = {}, tokens = 0;
         u64 sum = 0;
+        auto add = [&](const uint32_t* bins, auto&& take) {
+            Bins x[C];
+#pragma unroll
+            for (uint32_t c = 0; c < C; c++) x[c] = *reinterpret_cast<const Bins*>(sm_peer(bins, c) + kBinsEach * tid);
+#pragma unroll
+            for (uint32_t c = 0; c < C; c++)
+#pragma unroll
+                for (uint32_t k = 0; k < kBinsEach; k++) take(k, reinterpret_cast<const uint32_t*>(&x[c])[k]);
+        };
+        add(sh.count, [&](uint32_t k, uint32_t v) { here[k] += v; });
+        if (masses) {
+            add(sh.mass_low, [&](uint32_t k, uint32_t v) { mine[k] += v; });
+            add(sh.mass_high, [&](uint32_t k, uint32_t v) { mine[k] += (u64)v << 32; });
+        }
 #pragma unroll
         for (uint32_t k = 0; k < kBinsEach; k++) {
-            const uint32_t b = kBinsEach * tid + k;
-            u64 m = 0;
-            uint32_t q = 0;
-#pragma unroll
-            for (uint32_t c = 0; c < C; c++) q += sm_peer(&sh.count[b], c);
-            if (masses) {
-#pragma unroll
-                for (uint32_t c = 0; c < C; c++) m += sm_peer(&sh.mass_low[b], c) + ((u64)sm_peer(&sh.mass_high[b], c) << 32);
-            }
-            here[k] = q; mine[k] = masses ? m : q;
-            tokens += q; sum += mine[k];
+            if (!masses) mine[k] = here[k];
+            tokens += here[k]; sum += mine[k];
         }
         u64 before = sum;
         uint32_t tokens_before = tokens;
@@ -211,9 +234,9 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 2 : 4) k_sample(const
         count_bins(0, best, true, 0, !by_k);
         u64 target = find_bin(!by_k, top_k, by_k ? -1.0 : (double)top_p, 0, &upto);
         const uint32_t first_bin = sh.found_bin;
-        if (upto <= kSmFew) {
+        if (upto <= kSmList) {
             // few: they go to the first CTA
-            each(0, n, tid, T_, true, [&](float x, uint32_t i) {
+            each(0, n, tid, T_, [&](float x, uint32_t i) {
                 if (bin_of(x) > first_bin) return;
                 uint32_t at;
                 asm volatile("atom.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(sm_at(&sh.n_all, 0)) : "memory");
@@ -223,49 +246,74 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 2 : 4) k_sample(const
             cluster_sync();                                          // (before that no CTA leaves: its bins are read)
             if (rank != 0) return;
             const uint32_t count = sh.n_all;
-            constexpr uint32_t kEach = kSmFew / T_;
-            u64 ahead[kEach];
-            bool stays[kEach];
-            ulonglong2 me[kEach];
-            u64 sum = 0;
-            for (uint32_t k = 0; k < kEach; k++) {
-                const uint32_t t = tid + k * T_;
-                stays[k] = false; ahead[k] = 0; me[k] = make_ulonglong2(0, 0);
-                if (t >= count) continue;
-                me[k] = sh.all_list[t];
-                uint32_t before = 0;
-                for (uint32_t i = 0; i < count; i++) { const ulonglong2 x = sh.all_list[i]; if (x.x > me[k].x) { before++; ahead[k] += x.y; } }
-                stays[k] = !by_k || before < (uint32_t)top_k;
-                if (stays[k]) sum += me[k].y;
-            }
-            auto block_sum = [&](u64 v) {
-                v = warp_sum64(v);
+            uint32_t size = 32;
+            while (size < count) size *= 2;
+            // in falling order of x (the order of the logits; then that of falling numbers, in which indices rise), what is behind the last one 0
+            // (by one warp where they are few, which waits for itself alone)
+            const uint32_t sorters = size <= 256 ? 32 : T_;
+            auto sort = [&] {
                 __syncthreads();
-                if (lane == 0) sh.warp_mass[warp] = v;
+                for (uint32_t k = 2; k <= size; k *= 2)
+                    for (uint32_t d = k / 2; d > 0; d /= 2) {
+                        if (tid < sorters)
+                            for (uint32_t t = tid; t < size / 2; t += sorters) {
+                                const uint32_t i = 2 * t - (t & (d - 1)), j = i + d;
+                                const ulonglong2 x = sh.all_list[i], y = sh.all_list[j];
+                                if (x.x < y.x == !(i & k)) { sh.all_list[i] = y; sh.all_list[j] = x; }
+                            }
+                        if (sorters == 32) __syncwarp(); else __syncthreads();
+                    }
                 __syncthreads();
-                u64 t = 0;
-                for (uint32_t i = 0; i < kWarps; i++) t += sh.warp_mass[i];
-                return t;
             };
+            // sums of y up to each place; the sum of all
+            constexpr uint32_t kEach = kSmList / T_;
+            u64 upto_[kEach];
+            auto scan = [&] {
+                u64 sum = 0;
+#pragma unroll
+                for (uint32_t k = 0; k < kEach; k++) { const uint32_t t = kEach * tid + k; sum += t < size ? sh.all_list[t].y : 0; upto_[k] = sum; }
+                u64 before = sum;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) { const u64 t = __shfl_up_sync(0xffffffffu, before, o); if (lane >= (uint32_t)o) before += t; }
+                __syncthreads();
+                if (lane == 31) sh.warp_mass[warp] = before;
+                __syncthreads();
+                u64 all = 0;
+#pragma unroll
+                for (uint32_t i = 0; i < kWarps; i++) { if (i < warp) before += sh.warp_mass[i]; all += sh.warp_mass[i]; }
+#pragma unroll
+                for (uint32_t k = 0; k < kEach; k++) upto_[k] += before - sum;
+                return all;
+            };
+            for (uint32_t t = count + tid; t < size; t += T_) sh.all_list[t] = make_ulonglong2(0, 0);
+            sort();
+            if (by_k) {
+                for (uint32_t t = top_k + tid; t < size; t += T_) sh.all_list[t].y = 0;
+                __syncthreads();
+            }
             if (by_p) {
-                if (by_k) target = max((u64)1, (u64)ceil((double)top_p * (double)block_sum(sum)));
-                for (uint32_t k = 0; k < kEach; k++) stays[k] = stays[k] && ahead[k] < target;
+                const u64 sum = scan();
+                if (by_k) target = max((u64)1, (u64)ceil((double)top_p * (double)sum));
+#pragma unroll
+                for (uint32_t k = 0; k < kEach; k++) { const uint32_t t = kEach * tid + k; if (t < size && upto_[k] - sh.all_list[t].y >= target) sh.all_list[t].y = 0; }
             }
-            sum = 0;
-            for (uint32_t k = 0; k < kEach; k++) {
-                const uint32_t t = tid + k * T_;
-                stays[k] = stays[k] && exponent(sm_value((uint32_t)(me[k].x >> kSmIndexBits))) >= least;
-                if (t < count) sh.list[t] = make_ulonglong2(me[k].x & kSmIndexMask, stays[k] ? me[k].y : 0);      // (numbers that fall as indices rise)
-                if (stays[k]) sum += me[k].y;
+            __syncthreads();
+            // in order of their indices
+            for (uint32_t t = tid; t < size; t += T_) {
+                const ulonglong2 x = sh.all_list[t];
+                const float v = sm_value((uint32_t)(x.x >> kSmIndexBits));
+                const bool on = t < count && x.y && exponent(v) >= least;
+                sh.all_list[t] = make_ulonglong2(t < count ? (x.x & kSmIndexMask) << 32 | __float_as_uint(v) : 0, on ? x.y : 0);
             }
-            const u64 all = block_sum(sum);                          // (its barriers stand between the list's writes and reads)
+            sort();
+            const u64 all = scan();
             const double drawn = (double)u * (double)all;
+#pragma unroll
             for (uint32_t k = 0; k < kEach; k++) {
-                if (!stays[k] || !me[k].y) continue;
-                const u64 place = me[k].x & kSmIndexMask;
-                u64 before = 0;
-                for (uint32_t i = 0; i < count; i++) { const ulonglong2 x = sh.list[i]; if (x.x > place) before += x.y; }
-                if (!((double)before > drawn) && (double)(before + me[k].y) > drawn) draw(sm_value((uint32_t)(me[k].x >> kSmIndexBits)), kSmIndexMask - (uint32_t)place, all);
+                const uint32_t t = kEach * tid + k;
+                if (t >= size) break;
+                const ulonglong2 x = sh.all_list[t];
+                if (x.y && !((double)(upto_[k] - x.y) > drawn) && (double)upto_[k] > drawn) draw(__uint_as_float((uint32_t)x.x), kSmIndexMask - (uint32_t)(x.x >> 32), all);
             }
             return;
         }
@@ -309,18 +357,23 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 2 : 4) k_sample(const
                     continue;
                 }
                 uint32_t* const n_list = &sh.n_list[1];
-                each(0, n, tid, T_, true, [&](float x, uint32_t i) {
+                each(0, n, tid, T_, [&](float x, uint32_t i) {
                     const u64 o = sm_order(x, v0 + i);
                     if (o < lo || o > hi || (linear ? bin_of(x) : (uint32_t)((hi - o) >> shift)) != bin) return;
                     sh.list[atomicAdd(n_list, 1u)] = make_ulonglong2(o, by_mass ? weight(x) : 1);
                 });
                 __syncthreads();
                 cluster_sync();
-                uint32_t at = 0;
-                for (uint32_t c = 0; c < C; c++) {
-                    const uint32_t k = sm_peer(n_list, c);
-                    for (uint32_t i = tid; i < k; i += T_) sh.all_list[at + i] = sm_peer(&sh.list[i], c);
-                    at += k;
+                uint32_t ends[C];
+#pragma unroll
+                for (uint32_t c = 0; c < C; c++) ends[c] = *sm_peer(n_list, c);
+#pragma unroll
+                for (uint32_t c = 1; c < C; c++) ends[c] += ends[c - 1];
+                for (uint32_t t = tid; t < count; t += T_) {
+                    uint32_t c = 0, begin = 0;
+#pragma unroll
+                    for (uint32_t k = 0; k + 1 < C; k++) if (t >= ends[k]) { c = k + 1; begin = ends[k]; }
+                    sh.all_list[t] = *sm_peer(&sh.list[t - begin], c);
                 }
                 __syncthreads();
                 for (uint32_t t = warp; t < *n_list; t += kWarps) {
@@ -348,7 +401,7 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 2 : 4) k_sample(const
         return e >= least ? sm_weight(e, sh.table) : (u64)0;
     };
     u64 sum = 0;
-    each(from, to, lane, 32, true, [&](float x, uint32_t i) { sum += stays(x, i); });
+    each(from, to, lane, 32, [&](float x, uint32_t i) { sum += stays(x, i); });
     sum = warp_sum64(sum);
     __syncthreads();
     if (lane == 0) sh.warp_mass[warp] = sum;
@@ -358,14 +411,14 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 2 : 4) k_sample(const
     cluster_sync();
     u64 all = 0, base = 0;
 #pragma unroll
-    for (uint32_t c = 0; c < C; c++) { const u64 t = sm_peer(&sh.total, c); all += t; if (c < rank) base += t; }
+    for (uint32_t c = 0; c < C; c++) { const u64 t = *sm_peer(&sh.total, c); all += t; if (c < rank) base += t; }
     const double drawn = (double)u * (double)all;
     for (uint32_t i = 0; i < warp; i++) base += sh.warp_mass[i];
     if (!((double)base > drawn) && (double)(base + sum) > drawn) {
         for (uint32_t i = from; i < to; i += 128) {                  // a lane's four neighbours at a time
             float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             u64 w[4] = {0, 0, 0, 0}, mine = 0;
-            each(i, min(i + 128, to), lane, 32, true, [&](float v, uint32_t at) {
+            each(i, min(i + 128, to), lane, 32, [&](float v, uint32_t at) {
                 const uint32_t k = at & 3;
                 const u64 y = stays(v, at);
 #pragma unroll

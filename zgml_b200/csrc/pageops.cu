@@ -7,19 +7,24 @@
 namespace {
 
 // ── PAGE_APPEND ──────────────────────────────────────────────────────────────────────────────────────────────────────
-constexpr uint32_t kPaThreads = 256, kPaQueries = 1024, kPaPairs = 128;      // query values a CTA; pairs of a head
+constexpr uint32_t kPaThreads = 256, kPaPairs = 128, kPaRows = 16;   // pairs of a head; rows a CTA at most
 struct PaArgs {
     PagePool pool; PageShape s;
     uint8_t* pages; const float* src; const float* table; float* turned; const float* freqs;
-    uint32_t B, src_rs, k_col, v_col, q_col, q_heads, dst_rs, turn_at, rot, halves;
+    uint32_t B, src_rs, k_col, v_col, q_col, q_heads, dst_rs, turn_at, rot, halves, rows, part, vec;      // rows a CTA, query values of one
     double freq[kPaPairs];                                           // base^(-2i / rot), where no table of frequencies is given
 };
 // Cosine and sine of a position's turn.  Everything up to the turned value is in 64 bits, and that is rounded once: a code is a turned value over its scale, rounded, and an
-// error of f32's size would now and then make it its neighbour, an error of a hundredth of a head's largest value.
-__device__ __forceinline__ void pa_turn(const PaArgs& a, double position, uint32_t i, double* sin_, double* cos_) {
-    const double angle = position * (a.freqs ? (double)a.freqs[i] : a.freq[i]), turns = rint(angle * 0.15915494309189533577);
-    sincos(fma(-turns, 2.449293598294706e-16, fma(-turns, 6.283185307179586232, angle)), sin_, cos_);      // (two parts of 2 pi: 106 bits)
+// error of f32's size would now and then make it its neighbour, an error of a hundredth of a head's largest value.  The angle over pi, less an even whole number, comes from a product
+// with both parts of 1 / pi.
+__device__ __forceinline__ double2 pa_turn(const PaArgs& a, double position, uint32_t i) {
+    constexpr double inv_pi = 0.31830988618379069122, inv_pi_low = -1.9678676675182485832e-17;
+    const double angle = position * (a.freqs ? (double)a.freqs[i] : a.freq[i]), even = 2.0 * rint(angle * (0.5 * inv_pi));
+    double2 t;
+    sincospi(fma(angle, inv_pi_low, fma(angle, inv_pi, -even)), &t.y, &t.x);
+    return t;
 }
+__device__ __forceinline__ float2 pa_turned(float x, float y, double2 t) { return make_float2((float)((double)x * t.x - (double)y * t.y), (float)((double)x * t.y + (double)y * t.x)); }
 // what a scale has to be at least: the smallest power of two (2^-126 at least) of which 127 times reach the value whose bits are given; NaN where that is not finite
 __device__ __forceinline__ float pa_scale(uint32_t bits) {
     if (bits >= 0x7f800000u) return kBatchNaN;
@@ -29,50 +34,80 @@ __device__ __forceinline__ float pa_scale(uint32_t bits) {
 }
 __device__ __forceinline__ uint32_t pa_code(float x, float inv) { return (uint32_t)(int)(rintf(x * inv) + 128.0f); }
 
-// CTA (row, key head | share of the query heads).  The first of a step's rows that join a page owns it: it finds the others in the table (the last of several at one place
-// counts), and no other CTA touches the page's part of its head, so no order of CTAs changes anything.
-__global__ void __launch_bounds__(kPaThreads) k_page_append(const __grid_constant__ PaArgs a) {
-    pdl_enter();
-    extern __shared__ float4 pa_mem[];
-    __shared__ int32_t joined[64];                                   // row that brings token t of the page, or -1
-    __shared__ uint32_t list[64];                                    // tokens that come, in order
-    __shared__ uint32_t most[2];
-    __shared__ double2 turn[kPaPairs];
-    const uint32_t r = blockIdx.x, tid = threadIdx.x;
+// Query heads of the CTA's rows: a part of their values.  Bound by reading and writing them.
+__device__ void pa_queries(const PaArgs& a, const BatchHead& head, uint32_t r0, uint32_t first, double2* turn) {
     const PageShape& s = a.s;
-    const BatchHead head = batch_head(a.table, a.B);
-    const BatchRow w = batch_row(a.table, r);
-    if (r >= head.rows || w.slot < 0) return;
-    bool ok = page_row_ok(a.pool, s, w) && head.prefix >= 0;
-    const uint32_t place = ok && w.length > 0 ? (uint32_t)w.length - 1 : 0;
-    const int32_t id = ok && w.length > 0 ? page_id(a.pool, w.slot, place >> s.shift) : 0;
-    ok = ok && id >= 0;
-    if (blockIdx.y >= s.G) {                                         // query heads
-        const uint32_t first = (blockIdx.y - s.G) * kPaQueries, n = a.q_heads * s.dk, half = a.rot / 2;
-        const float* src = a.src + (size_t)r * a.src_rs + a.q_col;
-        float* dst = a.turned + (size_t)r * a.dst_rs;
-        if (ok)
-            for (uint32_t i = tid; i < half; i += kPaThreads) pa_turn(a, (double)head.prefix + w.length - 1, i, &turn[i].y, &turn[i].x);
-        __syncthreads();
-        for (uint32_t c = first + tid; c < min(first + kPaQueries, n); c += kPaThreads) {
+    const uint32_t rows = min(a.rows, head.rows - r0), n = min(a.part, a.q_heads * s.dk - first), half = a.rot / 2;
+    for (uint32_t x = threadIdx.x; x < rows * half; x += kPaThreads) {
+        const uint32_t m = x / half;
+        const BatchRow w = batch_row(a.table, r0 + m);
+        if (w.slot >= 0 && w.length >= 0 && head.prefix >= 0) turn[x] = pa_turn(a, (double)head.prefix + w.length - 1, x - m * half);
+    }
+    __syncthreads();
+    for (uint32_t m = 0; m < rows; m++) {
+        const BatchRow w = batch_row(a.table, r0 + m);
+        if (w.slot < 0) continue;
+        bool ok = page_row_ok(a.pool, s, w) && head.prefix >= 0;
+        ok = ok && (w.length == 0 || page_id(a.pool, w.slot, (w.length - 1) >> s.shift) >= 0);
+        const float* src = a.src + (size_t)(r0 + m) * a.src_rs + a.q_col + first;
+        float* dst = a.turned + (size_t)(r0 + m) * a.dst_rs + first;
+        const double2* t = turn + m * half;
+        if (a.vec) {                                                 // four pairs, or four values that stay
+            const uint32_t quads = a.rot / 8, each = quads + (s.dk - a.rot) / 4;
+            for (uint32_t x = threadIdx.x; x < n / s.dk * each; x += kPaThreads) {
+                const uint32_t h = x / each, k = x - h * each;
+                uint32_t p = h * s.dk, q = p;
+                if (k < quads) { p += a.turn_at + (a.halves ? 4 * k : 8 * k); q = p + (a.halves ? half : 4); }
+                else { const uint32_t d = 4 * (k - quads); p += d < a.turn_at ? d : d + a.rot; }
+                float4 u = *reinterpret_cast<const float4*>(src + p);
+                if (k < quads) {
+                    float4 v = *reinterpret_cast<const float4*>(src + q);
+                    const double2* y = t + 4 * k;
+                    float2 z[4];
+                    if (a.halves) { z[0] = pa_turned(u.x, v.x, y[0]); z[1] = pa_turned(u.y, v.y, y[1]); z[2] = pa_turned(u.z, v.z, y[2]); z[3] = pa_turned(u.w, v.w, y[3]); }
+                    else { z[0] = pa_turned(u.x, u.y, y[0]); z[1] = pa_turned(u.z, u.w, y[1]); z[2] = pa_turned(v.x, v.y, y[2]); z[3] = pa_turned(v.z, v.w, y[3]); }
+                    if (a.halves) { u = make_float4(z[0].x, z[1].x, z[2].x, z[3].x); v = make_float4(z[0].y, z[1].y, z[2].y, z[3].y); }
+                    else { u = make_float4(z[0].x, z[0].y, z[1].x, z[1].y); v = make_float4(z[2].x, z[2].y, z[3].x, z[3].y); }
+                    *reinterpret_cast<float4*>(dst + q) = ok ? v : make_float4(kBatchNaN, kBatchNaN, kBatchNaN, kBatchNaN);
+                }
+                *reinterpret_cast<float4*>(dst + p) = ok ? u : make_float4(kBatchNaN, kBatchNaN, kBatchNaN, kBatchNaN);
+            }
+            continue;
+        }
+        for (uint32_t c = threadIdx.x; c < n; c += kPaThreads) {
             const uint32_t in = c % s.dk - a.turn_at;
             float v = src[c];
             if (in < a.rot) {
                 const bool second = a.halves ? in >= half : in & 1;
                 const float other = src[(int)c + (a.halves ? (second ? -(int)half : (int)half) : second ? -1 : 1)];
-                const double2 t = turn[a.halves ? (second ? in - half : in) : in >> 1];
-                v = (float)(second ? (double)v * t.x + (double)other * t.y : (double)v * t.x - (double)other * t.y);
+                const float2 z = pa_turned(second ? other : v, second ? v : other, t[a.halves ? (second ? in - half : in) : in >> 1]);
+                v = second ? z.y : z.x;
             }
             dst[c] = ok ? v : kBatchNaN;
         }
-        return;
     }
-    if (!ok || w.length == 0) return;
-    // the rows that join this page
+}
+
+// Row r's page and key head g, where r is the first of the step's rows that join that page: it finds the others in the table (the last of several at one place counts), and no
+// other CTA touches the page's part of its head, so no order of CTAs changes anything.
+__device__ void pa_keys(const PaArgs& a, const BatchHead& head, uint32_t r, uint32_t g, float* tile) {
+    __shared__ int32_t joined[64];                                   // row that brings token t of the page, or -1
+    __shared__ uint32_t list[64], at[64];                            // tokens that come, in order, and a token's place among them
+    __shared__ uint32_t most[2], count;
+    const uint32_t tid = threadIdx.x;
+    const PageShape& s = a.s;
+    const BatchRow w = batch_row(a.table, r), prior = batch_row(a.table, r ? r - 1 : 0);
+    if (w.slot < 0 || !page_row_ok(a.pool, s, w) || head.prefix < 0 || w.length == 0) return;
+    const uint32_t place = (uint32_t)w.length - 1;
+    if (r && prior.slot == w.slot && prior.length > 0 && (uint32_t)(prior.length - 1) >> s.shift == place >> s.shift) return;      // (as most rows of a prompt do)
+    const int32_t id = page_id(a.pool, w.slot, place >> s.shift);
+    if (id < 0) return;
+    __syncthreads();
     if (tid < 64) joined[tid] = -1;
     if (tid < 2) most[tid] = 0;
     __syncthreads();
     bool earlier = false;
+#pragma unroll 4
     for (uint32_t i = tid; i < head.rows; i += kPaThreads) {
         const BatchRow z = batch_row(a.table, i);
         if (z.slot != w.slot || z.length <= 0 || (uint32_t)(z.length - 1) >> s.shift != place >> s.shift) continue;
@@ -84,56 +119,53 @@ __global__ void __launch_bounds__(kPaThreads) k_page_append(const __grid_constan
         uint32_t n = 0;
         for (uint32_t t = 0; t < s.page; t += 32) {
             const bool here = t + tid < s.page && joined[t + tid] >= 0;
-            const uint32_t all = __ballot_sync(0xffffffffu, here);
-            if (here) list[n + __popc(all & ((1u << tid) - 1))] = t + tid;
+            const uint32_t all = __ballot_sync(0xffffffffu, here), mine = n + __popc(all & ((1u << tid) - 1));
+            if (here) { list[mine] = t + tid; at[t + tid] = mine; }
             n += __popc(all);
         }
-        if (tid == 0) most[0] = n;
+        if (tid == 0) count = n;
     }
     __syncthreads();
-    const uint32_t n = most[0], g = blockIdx.y, width = s.dk + s.dv, half = a.rot / 2;
-    __syncthreads();
-    if (tid == 0) most[0] = 0;
-    __syncthreads();
-    float* const tile = reinterpret_cast<float*>(pa_mem);             // [tokens that come][keys | values]
+    const uint32_t n = count, width = s.dk + s.dv, half = a.rot / 2;
+    uint8_t* const part = a.pages + (size_t)id * page_bytes(s) + (size_t)g * s.head;
+    const bool fresh = joined[0] >= 0;
+    float2 before = *reinterpret_cast<const float2*>(part), after;
     uint32_t top[2] = {0, 0};
-    // turned pairs, the other keys, and values
-    for (uint32_t x = tid; x < n * half; x += kPaThreads) {
-        const uint32_t m = x / half, i = x - m * half, t = list[m], p = a.turn_at + (a.halves ? i : 2 * i), q = p + (a.halves ? half : 1);
-        const float* src = a.src + (size_t)joined[t] * a.src_rs + a.k_col + g * s.dk;
-        double sin_, cos_;
-        pa_turn(a, (double)head.prefix + ((place & ~(s.page - 1)) + t), i, &sin_, &cos_);
-        const double u = src[p], v = src[q];
-        const float y0 = (float)(u * cos_ - v * sin_), y1 = (float)(u * sin_ + v * cos_);
-        tile[m * width + p] = y0; tile[m * width + q] = y1;
-        top[0] = max(top[0], max(__float_as_uint(fabsf(y0)), __float_as_uint(fabsf(y1))));
-    }
+    // values and the keys that are not turned, then turned pairs: into [tokens that come][keys | values]
+#pragma unroll 4
     for (uint32_t x = tid; x < n * width; x += kPaThreads) {
         const uint32_t m = x / width, c = x - m * width;
         if (c < s.dk && c - a.turn_at < a.rot) continue;
         const float v = a.src[(size_t)joined[list[m]] * a.src_rs + (c < s.dk ? a.k_col + g * s.dk + c : a.v_col + g * s.dv + c - s.dk)];
         tile[x] = v;
-        top[c >= s.dk] = max(top[c >= s.dk], __float_as_uint(fabsf(v)));
+        if (c < s.dk) top[0] = max(top[0], __float_as_uint(fabsf(v))); else top[1] = max(top[1], __float_as_uint(fabsf(v)));
     }
+#pragma unroll 2
+    for (uint32_t x = tid; x < n * half; x += kPaThreads) {
+        const uint32_t m = x / half, i = x - m * half, t = list[m], p = a.turn_at + (a.halves ? i : 2 * i), q = p + (a.halves ? half : 1);
+        const float* src = a.src + (size_t)joined[t] * a.src_rs + a.k_col + g * s.dk;
+        const float2 y = pa_turned(src[p], src[q], pa_turn(a, (double)head.prefix + ((place & ~(s.page - 1)) + t), i));
+        tile[m * width + p] = y.x; tile[m * width + q] = y.y;
+        top[0] = max(top[0], max(__float_as_uint(fabsf(y.x)), __float_as_uint(fabsf(y.y))));
+    }
+#pragma unroll
     for (int i = 0; i < 2; i++) {
         top[i] = __reduce_max_sync(0xffffffffu, top[i]);
         if ((tid & 31) == 0) atomicMax(&most[i], top[i]);
     }
     __syncthreads();
-    uint8_t* const part = a.pages + (size_t)id * page_bytes(s) + (size_t)g * s.head;
-    const bool fresh = joined[0] >= 0;
-    float inv[2];
-    float2 before = *reinterpret_cast<const float2*>(part), after;
     if (fresh) before = make_float2(0.0f, 0.0f);
     after.x = pa_scale(most[0]); after.y = pa_scale(most[1]);
     after.x = before.x != before.x ? before.x : after.x < before.x ? before.x : after.x;      // (a scale that is not a number stays until the page begins anew)
     after.y = before.y != before.y ? before.y : after.y < before.y ? before.y : after.y;
-    inv[0] = 1.0f / after.x; inv[1] = 1.0f / after.y;
+    const float inv[2] = {1.0f / after.x, 1.0f / after.y};
     // codes that the page has, in multiples of a larger scale
+#pragma unroll
     for (int i = 0; i < 2; i++) {
         const float ratio = (i ? before.y : before.x) * inv[i];
         if (fresh || !(ratio < 1.0f)) continue;
         uint32_t* codes = reinterpret_cast<uint32_t*>(part + kPageHead + (i ? s.page * s.kp : 0));
+#pragma unroll 4
         for (uint32_t x = tid; x < s.page * (i ? s.vp : s.kp) / 4; x += kPaThreads) {
             const uint32_t c = codes[x];
             uint32_t o = 0;
@@ -144,49 +176,104 @@ __global__ void __launch_bounds__(kPaThreads) k_page_append(const __grid_constan
     }
     __syncthreads();
     if (tid == 0) *reinterpret_cast<float2*>(part) = after;
-    if (after.x == after.x)
-        for (uint32_t x = tid; x < n * s.dk; x += kPaThreads) {
-            const uint32_t m = x / s.dk, c = x - m * s.dk;
-            part[key_byte(s, list[m], c)] = (uint8_t)pa_code(tile[m * width + c], inv[0]);
+    if (after.x == after.x) {                                        // four values of a key at a time
+        const uint32_t words = (s.dk + 3) / 4;
+        for (uint32_t x = tid; x < n * words; x += kPaThreads) {
+            const uint32_t m = x / words, c = 4 * (x - m * words);
+            const float* from = tile + m * width + c;
+            uint8_t* to = part + key_byte(s, list[m], c);
+            if (c + 4 <= s.dk) *reinterpret_cast<uint32_t*>(to) = pa_code(from[0], inv[0]) | pa_code(from[1], inv[0]) << 8 | pa_code(from[2], inv[0]) << 16 | pa_code(from[3], inv[0]) << 24;
+            else for (uint32_t k = 0; c + k < s.dk; k++) to[k] = (uint8_t)pa_code(from[k], inv[0]);
         }
-    if (after.y == after.y)
-        for (uint32_t x = tid; x < n * s.dv; x += kPaThreads) {
-            const uint32_t m = x / s.dv, c = x - m * s.dv;
-            part[value_byte(s, list[m], c)] = (uint8_t)pa_code(tile[m * width + s.dk + c], inv[1]);
+    }
+    if (after.y == after.y)                                          // one value of tokens t, t + 1, t + 8, t + 9 where all of them come, else byte by byte
+        for (uint32_t x = tid; x < s.page / 4 * s.vp; x += kPaThreads) {
+            const uint32_t unit = x / (4 * s.vp), y = x - unit * 4 * s.vp, c = 16 * (y / 64) + 8 * (y & 1) + (y % 64) / 8, t = 16 * unit + 2 * ((y / 2) & 3);
+            if (c >= s.dv) continue;
+            const int32_t r0 = joined[t], r1 = joined[t + 1], r8 = joined[t + 8], r9 = joined[t + 9];
+            uint8_t* to = part + value_byte(s, t, c);
+            auto code = [&](uint32_t token) { return pa_code(tile[at[token] * width + s.dk + c], inv[1]); };
+            if ((r0 | r1 | r8 | r9) >= 0) *reinterpret_cast<uint32_t*>(to) = code(t) | code(t + 1) << 8 | code(t + 8) << 16 | code(t + 9) << 24;
+            else {
+                if (r0 >= 0) to[0] = (uint8_t)code(t);
+                if (r1 >= 0) to[1] = (uint8_t)code(t + 1);
+                if (r8 >= 0) to[2] = (uint8_t)code(t + 8);
+                if (r9 >= 0) to[3] = (uint8_t)code(t + 9);
+            }
         }
+}
+// CTA (some rows; key head | part of the query heads)
+__global__ void __launch_bounds__(kPaThreads) k_page_append(const __grid_constant__ PaArgs a) {
+    pdl_enter();
+    extern __shared__ float4 pa_mem[];
+    const BatchHead head = batch_head(a.table, a.B);
+    const uint32_t r0 = blockIdx.x * a.rows;
+    if (r0 >= head.rows) return;
+    if (blockIdx.y >= a.s.G) return pa_queries(a, head, r0, (blockIdx.y - a.s.G) * a.part, reinterpret_cast<double2*>(pa_mem));
+    for (uint32_t r = r0; r < min(r0 + a.rows, head.rows); r++) pa_keys(a, head, r, blockIdx.y, reinterpret_cast<float*>(pa_mem));
 }
 
 // ── PAGE_READ ────────────────────────────────────────────────────────────────────────────────────────────────────────
 struct PrArgs {
     PagePool pool; PageShape s;
     const float* table; float* dst;
-    uint32_t B, dst_rs, k_col, v_col;
+    uint32_t B, dst_rs, k_col, v_col, vec;
 };
 constexpr uint32_t kPrThreads = 256, kPrRows = 16;
-// CTA (16 rows, key head)
+// CTA (16 rows, key head): bound by its writes.  The rows' pages are found once, then four codes at a time become numbers; a page's values lie 32 bytes apart from one to the next, and
+// what is fetched with them belongs to the rows beside this one, as a rule.
 __global__ void __launch_bounds__(kPrThreads) k_page_read(const PrArgs a) {
     pdl_enter();
+    __shared__ const uint8_t* parts[kPrRows];                        // null: zeros, or nothing (tokens: -1), or no numbers (-2)
+    __shared__ int32_t tokens[kPrRows];
+    __shared__ float2 scales[kPrRows];
     const PageShape& s = a.s;
-    const BatchHead head = batch_head(a.table, a.B);
-    const uint32_t first = blockIdx.x * kPrRows, g = blockIdx.y, width = s.dk + s.dv;
-    for (uint32_t x = threadIdx.x; x < kPrRows * width; x += kPrThreads) {
-        const uint32_t m = x / width, c = x - m * width, r = first + m;
-        if (r >= head.rows) return;
-        const BatchRow w = batch_row(a.table, r);
-        if (w.slot < 0) continue;
-        float v = kBatchNaN;
-        if (page_row_ok(a.pool, s, w)) {
-            v = 0.0f;
-            if (w.length > 0) {
-                const uint32_t place = w.length - 1, t = place & (s.page - 1);
-                const int32_t id = page_id(a.pool, w.slot, place >> s.shift);
-                const uint8_t* part = a.pool.pages + (size_t)max(id, 0) * page_bytes(s) + (size_t)g * s.head;
-                const float2 scale = *reinterpret_cast<const float2*>(part);
-                const uint8_t code = part[c < s.dk ? key_byte(s, t, c) : value_byte(s, t, c - s.dk)];
-                v = id < 0 ? kBatchNaN : ((float)code - 128.0f) * (c < s.dk ? scale.x : scale.y);
+    const uint32_t first = blockIdx.x * kPrRows, g = blockIdx.y, words = (s.dk + 3) / 4, each = words + (s.dv + 3) / 4;
+    if (threadIdx.x < kPrRows) {
+        const BatchHead head = batch_head(a.table, a.B);
+        const uint32_t r = first + threadIdx.x;
+        const BatchRow w = batch_row(a.table, min(r, a.B - 1));
+        const uint8_t* part = nullptr;
+        int32_t token = 0;
+        if (r >= head.rows || w.slot < 0) token = -1;
+        else if (!page_row_ok(a.pool, s, w)) token = -2;
+        else if (w.length > 0) {
+            const int32_t id = page_id(a.pool, w.slot, (uint32_t)(w.length - 1) >> s.shift);
+            token = id < 0 ? -2 : (w.length - 1) & (int)(s.page - 1);
+            if (id >= 0) {
+                part = a.pool.pages + (size_t)id * page_bytes(s) + (size_t)g * s.head;
+                scales[threadIdx.x] = *reinterpret_cast<const float2*>(part);
             }
         }
-        a.dst[(size_t)r * a.dst_rs + (c < s.dk ? a.k_col + g * s.dk + c : a.v_col + g * s.dv + c - s.dk)] = v;
+        parts[threadIdx.x] = part; tokens[threadIdx.x] = token;
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (uint32_t x = threadIdx.x; x < kPrRows * each; x += kPrThreads) {
+        const uint32_t m = x / each, k = x - m * each;
+        const bool value = k >= words;
+        const uint32_t d = 4 * (value ? k - words : k), n = min(4u, (value ? s.dv : s.dk) - d);
+        const uint8_t* part = parts[m];
+        const int32_t t = tokens[m];
+        if (t == -1) continue;
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (part) {
+            uint32_t c[4];
+            if (!value) {
+                const uint32_t word = *reinterpret_cast<const uint32_t*>(part + key_byte(s, t, d));
+                c[0] = word & 255; c[1] = word >> 8 & 255; c[2] = word >> 16 & 255; c[3] = word >> 24;
+            } else {
+                const uint8_t* from = part + value_byte(s, t, d);
+#pragma unroll
+                for (uint32_t i = 0; i < 4; i++) c[i] = from[32 * i];      // (d is a multiple of 4: the four lie in one half of a tile)
+            }
+            const float scale = value ? scales[m].y : scales[m].x;
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++) v[i] = ((float)c[i] - 128.0f) * scale;
+        } else if (t == -2) v[0] = v[1] = v[2] = v[3] = kBatchNaN;
+        float* to = a.dst + (size_t)(first + m) * a.dst_rs + (value ? a.v_col + g * s.dv : a.k_col + g * s.dk) + d;
+        if (a.vec) *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);
+        else for (uint32_t i = 0; i < n; i++) to[i] = v[i];
     }
 }
 
@@ -263,9 +350,14 @@ bool zg_launch_page_op(const ZgOp& op, float* const* bufs, const size_t* elems, 
             a.turned = a.q_heads ? bufs[s.buf[5]] + s.off[3] : nullptr;
             a.freqs = a.rot && s.buf[4] != ZG_NO_BUF ? bufs[s.buf[4]] + s.off[4] : nullptr;
             if (!a.freqs) for (uint32_t i = 0; i < a.rot / 2; i++) a.freq[i] = std::pow((double)s.f[0], -2.0 * i / a.rot);
-            const size_t smem = sizeof(float) * std::min(a.s.page, a.B) * (a.s.dk + a.s.dv);
+            // More rows a CTA where there are many, of which a prompt's mostly join the page of the row before them.
+            a.rows = std::min(kPaRows, (a.B + 511) / 512);
+            const uint32_t heads = std::max(1u, a.B <= 64 ? 1024 / a.s.dk : 4096 / a.s.dk), parts = (a.q_heads + heads - 1) / heads;
+            a.part = heads * a.s.dk;
+            a.vec = a.q_heads && a.s.dk % 4 == 0 && a.turn_at % 4 == 0 && a.rot % 8 == 0 && a.src_rs % 4 == 0 && a.q_col % 4 == 0 && a.dst_rs % 4 == 0 && s.off[3] % 4 == 0;
+            const size_t smem = std::max(sizeof(float) * std::min(a.s.page, a.B) * (a.s.dk + a.s.dv), sizeof(double2) * a.rows * (a.rot / 2));
             if (!zg_smem_limit<k_page_append>(sizeof(float) * 64 * 512)) return false;
-            launch_pdl(k_page_append, dim3(a.B, a.s.G + (a.q_heads * a.s.dk + kPaQueries - 1) / kPaQueries), dim3(kPaThreads), smem, st, a);
+            launch_pdl(k_page_append, dim3((a.B + a.rows - 1) / a.rows, a.s.G + parts), dim3(kPaThreads), smem, st, a);
             ZG_SEQ_CHECK();
             return true;
         }
@@ -274,6 +366,7 @@ bool zg_launch_page_op(const ZgOp& op, float* const* bufs, const size_t* elems, 
             a.s = page_shape(s.n[1], s.n[2], s.n[3], s.n[5]);
             a.pool = pool(1, 2, a.s);
             a.table = bufs[s.buf[3]]; a.dst = bufs[s.buf[0]]; a.B = s.n[0]; a.dst_rs = s.n[4]; a.k_col = s.off[0]; a.v_col = s.off[1];
+            a.vec = a.s.dk % 4 == 0 && a.s.dv % 4 == 0 && a.dst_rs % 4 == 0 && a.k_col % 4 == 0 && a.v_col % 4 == 0;
             launch_pdl(k_page_read, dim3((a.B + kPrRows - 1) / kPrRows, a.s.G), dim3(kPrThreads), 0, st, a);
             ZG_SEQ_CHECK();
             return true;

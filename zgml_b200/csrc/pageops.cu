@@ -7,7 +7,7 @@
 namespace {
 
 // ── PAGE_APPEND ──────────────────────────────────────────────────────────────────────────────────────────────────────
-constexpr uint32_t kPaThreads = 256, kPaPairs = 128, kPaRows = 16;   // pairs of a head; rows a CTA at most
+constexpr uint32_t kPaThreads = 256, kPaPairs = 128, kPaRows = 16, kPaTurns = 4;      // pairs of a head; rows a CTA at most; tokens of a page that are few
 struct PaArgs {
     PagePool pool; PageShape s;
     uint8_t* pages; const float* src; const float* table; float* turned; const float* freqs;
@@ -88,29 +88,172 @@ __device__ void pa_queries(const PaArgs& a, const BatchHead& head, uint32_t r0, 
     }
 }
 
-// Row r's page and key head g, where r is the first of the step's rows that join that page: it finds the others in the table (the last of several at one place counts), and no
-// other CTA touches the page's part of its head, so no order of CTAs changes anything.
-__device__ void pa_keys(const PaArgs& a, const BatchHead& head, uint32_t r, uint32_t g, float* tile) {
+// what the scales of a part become when values up to `most` (their bits) join it
+__device__ __forceinline__ float2 pa_after(float2 before, uint32_t keys, uint32_t values) {
+    const float x = pa_scale(keys), y = pa_scale(values);            // (a scale that is not a number stays until the page begins anew)
+    return make_float2(before.x != before.x ? before.x : x < before.x ? before.x : x, before.y != before.y ? before.y : y < before.y ? before.y : y);
+}
+// a part's codes in multiples of larger scales
+__device__ __forceinline__ void pa_rescale(const PageShape& s, uint8_t* part, float2 before, float2 after, uint32_t first, uint32_t step) {
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const float ratio = i ? before.y / after.y : before.x / after.x;
+        if (!(ratio < 1.0f)) continue;
+        uint32_t* codes = reinterpret_cast<uint32_t*>(part + kPageHead + (i ? s.page * s.kp : 0));
+#pragma unroll 4
+        for (uint32_t x = first; x < s.page * (i ? s.vp : s.kp) / 4; x += step) {
+            const uint32_t c = codes[x];
+            uint32_t o = 0;
+#pragma unroll
+            for (int b = 0; b < 32; b += 8) o |= pa_code((float)(c >> b & 255) - 128.0f, ratio) << b;
+            codes[x] = o;
+        }
+    }
+}
+// The tokens of one page that a step brings, for all heads: a warp a head, which reads them twice (for the scales, for the codes); turns are made once.
+__device__ void pa_few(const PaArgs& a, const BatchHead& head, uint8_t* page, const int32_t* joined, const uint32_t* list, uint32_t n, uint32_t begin, double2* turn) {
+    const PageShape& s = a.s;
+    const uint32_t lane = threadIdx.x & 31, half = a.rot / 2, turns = min(n, kPaTurns);
+    for (uint32_t x = threadIdx.x; x < turns * half; x += kPaThreads) turn[x] = pa_turn(a, (double)head.prefix + (begin + list[x / half]), x % half);
+    __syncthreads();
+    for (uint32_t g = threadIdx.x >> 5; g < s.G; g += kPaThreads / 32) {
+        uint8_t* const part = page + (size_t)g * s.head;
+        float2 before = *reinterpret_cast<const float2*>(part), after;
+        uint32_t most_k = 0, most_v = 0;
+        float inv_k = 0.0f, inv_v = 0.0f;
+        auto pass = [&](bool codes) {
+            for (uint32_t m = 0; m < n; m++) {
+                const uint32_t t = list[m];
+                const float* const row = a.src + (size_t)joined[t] * a.src_rs;
+                const float* const keys = row + a.k_col + g * s.dk;
+                const float* const values = row + a.v_col + g * s.dv;
+#pragma unroll 4
+                for (uint32_t c = lane; c < s.dv; c += 32) {
+                    const float v = values[c];
+                    if (!codes) most_v = max(most_v, __float_as_uint(fabsf(v)));
+                    else if (inv_v == inv_v) part[value_byte(s, t, c)] = (uint8_t)pa_code(v, inv_v);
+                }
+#pragma unroll 2
+                for (uint32_t i = lane; i < half; i += 32) {
+                    const uint32_t p = a.turn_at + (a.halves ? i : 2 * i), q = p + (a.halves ? half : 1);
+                    const float2 y = pa_turned(keys[p], keys[q], m < turns ? turn[m * half + i] : pa_turn(a, (double)head.prefix + (begin + t), i));
+                    if (!codes) most_k = max(most_k, max(__float_as_uint(fabsf(y.x)), __float_as_uint(fabsf(y.y))));
+                    else if (inv_k == inv_k) { part[key_byte(s, t, p)] = (uint8_t)pa_code(y.x, inv_k); part[key_byte(s, t, q)] = (uint8_t)pa_code(y.y, inv_k); }
+                }
+                for (uint32_t c = lane; c < s.dk - a.rot; c += 32) {
+                    const uint32_t d = c < a.turn_at ? c : c + a.rot;
+                    const float v = keys[d];
+                    if (!codes) most_k = max(most_k, __float_as_uint(fabsf(v)));
+                    else if (inv_k == inv_k) part[key_byte(s, t, d)] = (uint8_t)pa_code(v, inv_k);
+                }
+            }
+        };
+        pass(false);
+        if (joined[0] >= 0) before = make_float2(0.0f, 0.0f);
+        after = pa_after(before, __reduce_max_sync(0xffffffffu, most_k), __reduce_max_sync(0xffffffffu, most_v));
+        if (joined[0] < 0) pa_rescale(s, part, before, after, lane, 32);
+        __syncwarp();
+        if (lane == 0) *reinterpret_cast<float2*>(part) = after;
+        inv_k = 1.0f / after.x; inv_v = 1.0f / after.y;
+        pass(true);
+    }
+}
+// The same of many, for one head and a whole CTA.  Keys go to shared memory as they are turned; values are read again when their scale is known (with both in shared memory fewer CTAs
+// are resident: 85 us instead of 56 for 2048 tokens of 8 heads of 128).
+__device__ void pa_many(const PaArgs& a, const BatchHead& head, uint8_t* part, uint32_t g, const int32_t* joined, const uint32_t* list, uint32_t n, uint32_t begin, float* tile) {
+    __shared__ uint32_t most[2];
+    const PageShape& s = a.s;
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, half = a.rot / 2;
+    if (tid < 2) most[tid] = 0;
+    float2 before = *reinterpret_cast<const float2*>(part);
+    uint32_t top[2] = {0, 0};
+    for (uint32_t m = warp; m < n; m += kPaThreads / 32) {
+        const uint32_t t = list[m];
+        const float* const row = a.src + (size_t)joined[t] * a.src_rs;
+        const double position = (double)head.prefix + (begin + t);
+#pragma unroll 4
+        for (uint32_t c = lane; c < s.dv; c += 32) top[1] = max(top[1], __float_as_uint(fabsf(row[a.v_col + g * s.dv + c])));
+        const float* const keys = row + a.k_col + g * s.dk;
+#pragma unroll 2
+        for (uint32_t i = lane; i < half; i += 32) {
+            const uint32_t p = a.turn_at + (a.halves ? i : 2 * i), q = p + (a.halves ? half : 1);
+            const float2 y = pa_turned(keys[p], keys[q], pa_turn(a, position, i));
+            tile[m * s.dk + p] = y.x; tile[m * s.dk + q] = y.y;
+            top[0] = max(top[0], max(__float_as_uint(fabsf(y.x)), __float_as_uint(fabsf(y.y))));
+        }
+        for (uint32_t c = lane; c < s.dk - a.rot; c += 32) {
+            const uint32_t d = c < a.turn_at ? c : c + a.rot;
+            const float v = keys[d];
+            tile[m * s.dk + d] = v;
+            top[0] = max(top[0], __float_as_uint(fabsf(v)));
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        top[i] = __reduce_max_sync(0xffffffffu, top[i]);
+        if (lane == 0) atomicMax(&most[i], top[i]);
+    }
+    __syncthreads();
+    if (joined[0] >= 0) before = make_float2(0.0f, 0.0f);
+    const float2 after = pa_after(before, most[0], most[1]);
+    if (joined[0] < 0) pa_rescale(s, part, before, after, tid, kPaThreads);
+    __syncthreads();
+    if (tid == 0) *reinterpret_cast<float2*>(part) = after;
+    const float inv_k = 1.0f / after.x, inv_v = 1.0f / after.y;
+    if (after.x == after.x)                                          // four values of a key at a time
+        for (uint32_t m = warp; m < n; m += kPaThreads / 32)
+            for (uint32_t c = 4 * lane; c < s.dk; c += 128) {
+                const float* from = tile + m * s.dk + c;
+                uint8_t* to = part + key_byte(s, list[m], c);
+                if (c + 4 <= s.dk) *reinterpret_cast<uint32_t*>(to) = pa_code(from[0], inv_k) | pa_code(from[1], inv_k) << 8 | pa_code(from[2], inv_k) << 16 | pa_code(from[3], inv_k) << 24;
+                else for (uint32_t k = 0; c + k < s.dk; k++) to[k] = (uint8_t)pa_code(from[k], inv_k);
+            }
+    if (after.y == after.y)                                          // one value of tokens t, t + 1, t + 8, t + 9 where all of them come, else byte by byte
+        for (uint32_t unit = 0; unit < s.page / 16; unit++)
+#pragma unroll 2
+            for (uint32_t y = tid; y < 4 * s.vp; y += kPaThreads) {
+                const uint32_t c = 16 * (y / 64) + 8 * (y & 1) + (y % 64) / 8, t = 16 * unit + 2 * ((y / 2) & 3);
+                const int32_t r0 = joined[t], r1 = joined[t + 1], r8 = joined[t + 8], r9 = joined[t + 9];
+                if (c >= s.dv || (r0 & r1 & r8 & r9) < 0) continue;      // (none of them)
+                uint8_t* to = part + value_byte(s, t, c);
+                auto code = [&](int32_t r) { return pa_code(a.src[(size_t)r * a.src_rs + a.v_col + g * s.dv + c], inv_v); };
+                if ((r0 | r1 | r8 | r9) >= 0) *reinterpret_cast<uint32_t*>(to) = code(r0) | code(r1) << 8 | code(r8) << 16 | code(r9) << 24;
+                else {
+                    if (r0 >= 0) to[0] = (uint8_t)code(r0);
+                    if (r1 >= 0) to[1] = (uint8_t)code(r1);
+                    if (r8 >= 0) to[2] = (uint8_t)code(r8);
+                    if (r9 >= 0) to[3] = (uint8_t)code(r9);
+                }
+            }
+}
+// Row r's page, where r is the first of the step's rows that join it: it finds the others in the table (the last of several at one place counts), and no other CTA touches the
+// page's part of a head, so no order of CTAs changes anything.  Where the rows behind r join it too, as a prompt's do, each head has a CTA (y); else the first CTA takes them all.
+__device__ void pa_keys(const PaArgs& a, const BatchHead& head, uint32_t r, uint32_t y, float* mem) {
     __shared__ int32_t joined[64];                                   // row that brings token t of the page, or -1
-    __shared__ uint32_t list[64], at[64];                            // tokens that come, in order, and a token's place among them
-    __shared__ uint32_t most[2], count;
+    __shared__ uint32_t list[64];                                    // tokens that come, in order
+    __shared__ uint32_t count;
     const uint32_t tid = threadIdx.x;
     const PageShape& s = a.s;
-    const BatchRow w = batch_row(a.table, r), prior = batch_row(a.table, r ? r - 1 : 0);
-    if (w.slot < 0 || !page_row_ok(a.pool, s, w) || head.prefix < 0 || w.length == 0) return;
+    const BatchRow w = batch_row(a.table, r);
     const uint32_t place = (uint32_t)w.length - 1;
-    if (r && prior.slot == w.slot && prior.length > 0 && (uint32_t)(prior.length - 1) >> s.shift == place >> s.shift) return;      // (as most rows of a prompt do)
+    auto joins = [&](const BatchRow& z) { return z.slot == w.slot && z.length > 0 && (uint32_t)(z.length - 1) >> s.shift == place >> s.shift; };
+    // (lane 0: the row before r, which as most rows of a prompt joins the same page; lanes 1 to kPaTurns: those behind it)
+    const uint32_t lane = tid & 31, near_row = lane == 0 ? r - 1 : r + lane;
+    const uint32_t near = __ballot_sync(0xffffffffu, (lane || r) && lane <= kPaTurns && near_row < head.rows && joins(batch_row(a.table, near_row)));
+    if (w.slot < 0 || !page_row_ok(a.pool, s, w) || head.prefix < 0 || w.length == 0 || (near & 1)) return;
+    const bool many = near >> 1 == (1u << kPaTurns) - 1;
+    if (y && !many) return;
     const int32_t id = page_id(a.pool, w.slot, place >> s.shift);
     if (id < 0) return;
     __syncthreads();
     if (tid < 64) joined[tid] = -1;
-    if (tid < 2) most[tid] = 0;
     __syncthreads();
     bool earlier = false;
 #pragma unroll 4
     for (uint32_t i = tid; i < head.rows; i += kPaThreads) {
         const BatchRow z = batch_row(a.table, i);
-        if (z.slot != w.slot || z.length <= 0 || (uint32_t)(z.length - 1) >> s.shift != place >> s.shift) continue;
+        if (!joins(z)) continue;
         if (i < r) earlier = true;
         else atomicMax(&joined[(z.length - 1) & (s.page - 1)], (int)i);
     }
@@ -120,87 +263,15 @@ __device__ void pa_keys(const PaArgs& a, const BatchHead& head, uint32_t r, uint
         for (uint32_t t = 0; t < s.page; t += 32) {
             const bool here = t + tid < s.page && joined[t + tid] >= 0;
             const uint32_t all = __ballot_sync(0xffffffffu, here), mine = n + __popc(all & ((1u << tid) - 1));
-            if (here) { list[mine] = t + tid; at[t + tid] = mine; }
+            if (here) list[mine] = t + tid;
             n += __popc(all);
         }
         if (tid == 0) count = n;
     }
     __syncthreads();
-    const uint32_t n = count, width = s.dk + s.dv, half = a.rot / 2;
-    uint8_t* const part = a.pages + (size_t)id * page_bytes(s) + (size_t)g * s.head;
-    const bool fresh = joined[0] >= 0;
-    float2 before = *reinterpret_cast<const float2*>(part), after;
-    uint32_t top[2] = {0, 0};
-    // values and the keys that are not turned, then turned pairs: into [tokens that come][keys | values]
-#pragma unroll 4
-    for (uint32_t x = tid; x < n * width; x += kPaThreads) {
-        const uint32_t m = x / width, c = x - m * width;
-        if (c < s.dk && c - a.turn_at < a.rot) continue;
-        const float v = a.src[(size_t)joined[list[m]] * a.src_rs + (c < s.dk ? a.k_col + g * s.dk + c : a.v_col + g * s.dv + c - s.dk)];
-        tile[x] = v;
-        if (c < s.dk) top[0] = max(top[0], __float_as_uint(fabsf(v))); else top[1] = max(top[1], __float_as_uint(fabsf(v)));
-    }
-#pragma unroll 2
-    for (uint32_t x = tid; x < n * half; x += kPaThreads) {
-        const uint32_t m = x / half, i = x - m * half, t = list[m], p = a.turn_at + (a.halves ? i : 2 * i), q = p + (a.halves ? half : 1);
-        const float* src = a.src + (size_t)joined[t] * a.src_rs + a.k_col + g * s.dk;
-        const float2 y = pa_turned(src[p], src[q], pa_turn(a, (double)head.prefix + ((place & ~(s.page - 1)) + t), i));
-        tile[m * width + p] = y.x; tile[m * width + q] = y.y;
-        top[0] = max(top[0], max(__float_as_uint(fabsf(y.x)), __float_as_uint(fabsf(y.y))));
-    }
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-        top[i] = __reduce_max_sync(0xffffffffu, top[i]);
-        if ((tid & 31) == 0) atomicMax(&most[i], top[i]);
-    }
-    __syncthreads();
-    if (fresh) before = make_float2(0.0f, 0.0f);
-    after.x = pa_scale(most[0]); after.y = pa_scale(most[1]);
-    after.x = before.x != before.x ? before.x : after.x < before.x ? before.x : after.x;      // (a scale that is not a number stays until the page begins anew)
-    after.y = before.y != before.y ? before.y : after.y < before.y ? before.y : after.y;
-    const float inv[2] = {1.0f / after.x, 1.0f / after.y};
-    // codes that the page has, in multiples of a larger scale
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const float ratio = (i ? before.y : before.x) * inv[i];
-        if (fresh || !(ratio < 1.0f)) continue;
-        uint32_t* codes = reinterpret_cast<uint32_t*>(part + kPageHead + (i ? s.page * s.kp : 0));
-#pragma unroll 4
-        for (uint32_t x = tid; x < s.page * (i ? s.vp : s.kp) / 4; x += kPaThreads) {
-            const uint32_t c = codes[x];
-            uint32_t o = 0;
-#pragma unroll
-            for (int b = 0; b < 32; b += 8) o |= pa_code((float)(c >> b & 255) - 128.0f, ratio) << b;
-            codes[x] = o;
-        }
-    }
-    __syncthreads();
-    if (tid == 0) *reinterpret_cast<float2*>(part) = after;
-    if (after.x == after.x) {                                        // four values of a key at a time
-        const uint32_t words = (s.dk + 3) / 4;
-        for (uint32_t x = tid; x < n * words; x += kPaThreads) {
-            const uint32_t m = x / words, c = 4 * (x - m * words);
-            const float* from = tile + m * width + c;
-            uint8_t* to = part + key_byte(s, list[m], c);
-            if (c + 4 <= s.dk) *reinterpret_cast<uint32_t*>(to) = pa_code(from[0], inv[0]) | pa_code(from[1], inv[0]) << 8 | pa_code(from[2], inv[0]) << 16 | pa_code(from[3], inv[0]) << 24;
-            else for (uint32_t k = 0; c + k < s.dk; k++) to[k] = (uint8_t)pa_code(from[k], inv[0]);
-        }
-    }
-    if (after.y == after.y)                                          // one value of tokens t, t + 1, t + 8, t + 9 where all of them come, else byte by byte
-        for (uint32_t x = tid; x < s.page / 4 * s.vp; x += kPaThreads) {
-            const uint32_t unit = x / (4 * s.vp), y = x - unit * 4 * s.vp, c = 16 * (y / 64) + 8 * (y & 1) + (y % 64) / 8, t = 16 * unit + 2 * ((y / 2) & 3);
-            if (c >= s.dv) continue;
-            const int32_t r0 = joined[t], r1 = joined[t + 1], r8 = joined[t + 8], r9 = joined[t + 9];
-            uint8_t* to = part + value_byte(s, t, c);
-            auto code = [&](uint32_t token) { return pa_code(tile[at[token] * width + s.dk + c], inv[1]); };
-            if ((r0 | r1 | r8 | r9) >= 0) *reinterpret_cast<uint32_t*>(to) = code(t) | code(t + 1) << 8 | code(t + 8) << 16 | code(t + 9) << 24;
-            else {
-                if (r0 >= 0) to[0] = (uint8_t)code(t);
-                if (r1 >= 0) to[1] = (uint8_t)code(t + 1);
-                if (r8 >= 0) to[2] = (uint8_t)code(t + 8);
-                if (r9 >= 0) to[3] = (uint8_t)code(t + 9);
-            }
-        }
+    uint8_t* const page = a.pages + (size_t)id * page_bytes(s);
+    if (!many) pa_few(a, head, page, joined, list, count, place & ~(s.page - 1), reinterpret_cast<double2*>(mem));
+    else pa_many(a, head, page + (size_t)y * s.head, y, joined, list, count, place & ~(s.page - 1), mem);
 }
 // CTA (some rows; key head | part of the query heads)
 __global__ void __launch_bounds__(kPaThreads) k_page_append(const __grid_constant__ PaArgs a) {
@@ -355,8 +426,8 @@ bool zg_launch_page_op(const ZgOp& op, float* const* bufs, const size_t* elems, 
             const uint32_t heads = std::max(1u, a.B <= 64 ? 1024 / a.s.dk : 4096 / a.s.dk), parts = (a.q_heads + heads - 1) / heads;
             a.part = heads * a.s.dk;
             a.vec = a.q_heads && a.s.dk % 4 == 0 && a.turn_at % 4 == 0 && a.rot % 8 == 0 && a.src_rs % 4 == 0 && a.q_col % 4 == 0 && a.dst_rs % 4 == 0 && s.off[3] % 4 == 0;
-            const size_t smem = std::max(sizeof(float) * std::min(a.s.page, a.B) * (a.s.dk + a.s.dv), sizeof(double2) * a.rows * (a.rot / 2));
-            if (!zg_smem_limit<k_page_append>(sizeof(float) * 64 * 512)) return false;
+            const size_t smem = std::max<size_t>({sizeof(float) * std::min(a.s.page, a.B) * a.s.dk, sizeof(double2) * std::max(a.rows, std::min(kPaTurns, a.B)) * (a.rot / 2)});
+            if (!zg_smem_limit<k_page_append>(sizeof(float) * 64 * 256)) return false;
             launch_pdl(k_page_append, dim3((a.B + a.rows - 1) / a.rows, a.s.G + parts), dim3(kPaThreads), smem, st, a);
             ZG_SEQ_CHECK();
             return true;

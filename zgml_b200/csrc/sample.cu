@@ -18,7 +18,7 @@ typedef unsigned long long u64;
 struct SmShared {
     alignas(16) uint32_t mass_low[kSmBins], mass_high[kSmBins], count[kSmBins];      // (sums of 64 bits by words: additions of 64 bits to shared memory are loops)
     ulonglong2 list[kSmList], all_list[kSmList];                     // {order, weight} of candidates, own and of the cluster
-    double table[32];                                                // 2^(i / 32)
+    double table[32];                                                // 2^(43 + i / 32)
     u64 best, total, warp_mass[32], found_mass, threshold, found_target;
     uint32_t n_list[2], n_all, found_count, found_bin, warp_count[32];
 };
@@ -47,21 +47,23 @@ __device__ __forceinline__ u64 warp_sum64(u64 v) {
     return v;
 }
 
-// round(2^43 e^x), x <= 0: 2^(k / 32) of a table times the exponential's series up to f^5, |f| <= ln 2 / 64, whose next term is below 2^-48 (reduction by a table: P. Tang,
-// ACM Transactions on Mathematical Software 15, 1989).
-// Whole numbers are taken from the mantissa of sums with 2^52: conversions of 64 bits are slow (a draw from 64 rows of 128256 tokens took 58 us with them).
-__device__ __forceinline__ u64 sm_weight(double x, const double* table) {
-    if (!(x > -32.0)) return 0;
-    const double shifted = fma(x, 46.166241308446828384, 6755399441055744.0), k = shifted - 6755399441055744.0;      // 32 / ln 2; 1.5 * 2^52
-    const double f = fma(k, -0.021660849392498290, x);               // ln 2 / 32
+// Weights round(2^43 e^x) of exponents x <= 0: 2^(k / 32) of a table times the exponential's series up to r^5, |r| <= ln 2 / 64, whose next term is below 2^-48 (reduction by a table:
+// P. Tang, ACM Transactions on Mathematical Software 15, 1989).  Whole numbers are taken from the mantissa of sums with 2^52 and 1.5 * 2^52: conversions of 64 bits are slow.
+constexpr double kSmShift = 6755399441055744.0, kSmSteps = 46.166241308446828384;      // 1.5 * 2^52; 32 / ln 2
+// t: the exponent in 32nds of a power of two, -3000 at least; *k: t rounded.  table: 2^(43 + i / 32)
+__device__ __forceinline__ u64 sm_weight(double t, const double* table, int* k) {
+    const double shifted = t + kSmShift, r = t - (shifted - kSmShift);
     const int n = __double2loint(shifted);
-    const double p = fma(f, fma(f, fma(f, fma(f, 1.0 / 120.0, 1.0 / 24.0), 1.0 / 6.0), 0.5), 1.0), t = table[n & 31];
-    const double w = fma(fma(p * f, t, t), __hiloint2double((1023 + 43 + (n >> 5)) << 20, 0), 4503599627370496.0);
+    *k = n;
+    constexpr double l = 0.021660849392498290;                       // ln 2 / 32
+    const double p = fma(fma(fma(fma(fma(l * l * l * l * l / 120.0, r, l * l * l * l / 24.0), r, l * l * l / 6.0), r, l * l / 2.0), r, l), r, 1.0);
+    const double power = table[n & 31];
+    const double w = fma(p, __hiloint2double(__double2hiint(power) + ((n & ~31) << 15), __double2loint(power)), 4503599627370496.0);
     return (u64)__double_as_longlong(w) & 0xfffffffffffffull;
 }
 
 // A cluster per row, its CTAs each a slice of the vocabulary: kept in shared memory (KEEP), or read again, from L2, where the rows fill the GPU more than once (with 64 rows of 128256 tokens
-// all logits would take all of its shared memory).  Tokens are counted by bins of logits below the largest, 1 / 64 of an exponent wide; what top_k or top_p cuts off begins in the bin in which
+// all logits would take all of its shared memory).  Tokens are counted by bins of logits below the largest, 1 / 32 of a power of two wide; what top_k or top_p cuts off begins in the bin in which
 // the counts (sums of weights) reach their target.  Where at most kSmList tokens lie in the bins up to there, one CTA gets them all and ranks them one against the other; otherwise
 // the bin is looked at more closely until at most kSmList candidates are left in it, of which each CTA ranks its own.  Weights are whole multiples of 2^-43 of the largest, their sums exact in 64 bits, so that
 // no order of additions changes a choice.
@@ -90,23 +92,28 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 2 : 4) k_sample(const
         x.x += 0.0f; x.y += 0.0f; x.z += 0.0f; x.w += 0.0f;          // (-0 becomes 0)
         return x;
     };
-    // f(logit, place in the slice) for every token of places [from, to), four at a time, the next ones asked for before.  (What f does is long: loops that are not unrolled stay in the
-    // instruction cache.)
-    auto each = [&](uint32_t from, uint32_t to, uint32_t first, uint32_t step, auto&& f) {
+    // f(four logits, place of the first in the slice, how many of them count) for all tokens of places [from, to), the next ones asked for before.  Work on the four goes side by side where f
+    // has no branches between them: an exponential is a dozen operations of 64 bits, each of which waits for the one before it.
+    auto fours = [&](uint32_t from, uint32_t to, uint32_t first, uint32_t step, auto&& f) {
         uint32_t i = from + 4 * first;
         float4 x = four(i, true), y = four(i + 4 * step, true);
 #pragma unroll 1
         for (; i < to; i += 4 * step) {
             const float4 next = four(i + 8 * step, true);
-            f(x.x, i);
-            if (i + 1 < to) f(x.y, i + 1);
-            if (i + 2 < to) f(x.z, i + 2);
-            if (i + 3 < to) f(x.w, i + 3);
+            const float v[4] = {x.x, x.y, x.z, x.w};
+            f(v, i, min(4u, to - i));
             x = y; y = next;
         }
     };
+    // f(logit, place) one after the other
+    auto each = [&](uint32_t from, uint32_t to, uint32_t first, uint32_t step, auto&& f) {
+        fours(from, to, first, step, [&](const float (&v)[4], uint32_t i, uint32_t count) {
+#pragma unroll
+            for (uint32_t k = 0; k < 4; k++) if (k < count) f(v[k], i + k);
+        });
+    };
     auto cluster_sync = [&] { if (C > 1) { sm_cluster_arrive(); sm_cluster_wait(); } else __syncthreads(); };
-    if (tid < 32) sh.table[tid] = exp2(tid / 32.0);
+    if (tid < 32) sh.table[tid] = exp2(43.0 + tid / 32.0);
     if (tid == 0) { sh.best = 0; sh.n_all = 0; sh.n_list[0] = sh.n_list[1] = 0; }
     for (uint32_t i = tid; i < kSmBins; i += T_) sh.count[i] = sh.mass_low[i] = sh.mass_high[i] = 0;
     __syncthreads();
@@ -143,35 +150,69 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 2 : 4) k_sample(const
         cluster_sync();                                              // no CTA leaves while it is read
         return;
     }
-    const double inv_t = 1.0 / (double)T, least = log((double)min_p);      // (min_p is compared as an exponent: those of tokens just below the largest logit round to 1)
-    const float bins_at = 64.0f / T;                                 // (the last bin: all below e^-16 of the largest)
+    // Exponents: (x - M) / T, in 32nds of a power of two as one product with x where that loses nothing (near), what is far below the largest as if it were at 45.
+    const double inv_t = 1.0 / (double)T, steps = inv_t * kSmSteps, top_steps = -(double)M * steps;
+    const bool near = fabs(top_steps) < 65536.0 && T < 1e30f;
+    const float lowest = near ? M - 45.0f * T : 0.0f;
     auto exponent = [&](float x) { return x == M ? 0.0 : ((double)x - (double)M) * inv_t; };
-    auto share = [&](float x) { return exp(exponent(x)); };
-    auto weight = [&](float x) { return sm_weight(exponent(x), sh.table); };
-    auto bin_of = [&](float x) { const float d = (M - x) * bins_at; return d < (float)kSmBins ? (uint32_t)d : x == M ? 0u : kSmBins - 1; };
+    auto in_steps = [&](float x) { return near ? fma((double)fmaxf(x, lowest), steps, top_steps) : fmax(exponent(x) * kSmSteps, -2100.0); };
+    auto weight = [&](float x) { int k; return sm_weight(in_steps(x), sh.table, &k); };
+    // bins of a 32nd of a power of two below the largest logit (the last one: all below 2^-32 of it), as the weight's rounding has them
+    auto bin_of = [&](float x) { return min((uint32_t)-__double2loint(in_steps(x) + kSmShift), kSmBins - 1); };
+    // the smallest logit that min_p lets through (compared as exponents: powers of what is just below the largest logit round to 1)
+    float least_x = -INFINITY;
+    if (min_p > 0.0f) {
+        const double least = log((double)min_p);
+        uint32_t key = sm_key((float)((double)M + least * (double)T));
+        const uint32_t most = (uint32_t)(best >> kSmIndexBits);
+        key = min(key, most);
+        while (key < most && !(exponent(sm_value(key)) >= least)) key++;
+        while (key > 0x00800000u && exponent(sm_value(key - 1)) >= least) key--;
+        least_x = sm_value(key);
+    }
     auto draw = [&](float x, uint32_t index, u64 all) {
         a.dst[r] = (int32_t)index;
-        if (a.probability) a.probability[r] = (float)(share(x) * kSmOne / (double)all);
+        if (a.probability) a.probability[r] = (float)(exp(exponent(x)) * kSmOne / (double)all);
     };
     const bool by_k = top_k != 0 && (uint32_t)top_k < a.V, by_p = top_p < 1.0f;
     u64 threshold = 0;
     // counts (and sums of weights) of the tokens in [lo, hi] by their bins: of equal width below the largest logit, or of the order's numbers
     auto count_bins = [&](u64 lo, u64 hi, bool linear, uint32_t shift, bool masses) {
-        each(0, n, tid, T_, [&](float x, uint32_t i) {
-            uint32_t b;
-            if (lo == 0 && linear) b = bin_of(x);                    // (all of them)
-            else {
+        if (masses && lo == 0 && linear)                             // (of all tokens: those with weights go four at a time)
+            fours(0, n, tid, T_, [&](const float (&x)[4], uint32_t, uint32_t valid) {
+                int k[4];
+                u64 w[4];
+#pragma unroll
+                for (uint32_t e = 0; e < 4; e++) w[e] = sm_weight(in_steps(x[e]), sh.table, &k[e]);
+#pragma unroll
+                for (uint32_t e = 0; e < 4; e++) {
+                    if (e >= valid) break;
+                    const uint32_t b = min((uint32_t)-k[e], kSmBins - 1), low = (uint32_t)w[e], old = atomicAdd(&sh.mass_low[b], low), high = (uint32_t)(w[e] >> 32) + (old + low < old);
+                    if (high) atomicAdd(&sh.mass_high[b], high);
+                    atomicAdd(&sh.count[b], 1u);
+                }
+            });
+        else if (lo == 0 && linear)
+            fours(0, n, tid, T_, [&](const float (&x)[4], uint32_t, uint32_t valid) {
+                uint32_t b[4];
+#pragma unroll
+                for (uint32_t e = 0; e < 4; e++) b[e] = bin_of(x[e]);
+#pragma unroll
+                for (uint32_t e = 0; e < 4; e++) if (e < valid) atomicAdd(&sh.count[b[e]], 1u);
+            });
+        else
+            each(0, n, tid, T_, [&](float x, uint32_t i) {
                 const u64 o = sm_order(x, v0 + i);
                 if (o < lo || o > hi) return;
-                b = linear ? bin_of(x) : (uint32_t)((hi - o) >> shift);
-            }
-            atomicAdd(&sh.count[b], 1u);
-            if (masses) {
-                const u64 w = weight(x);
-                const uint32_t low = (uint32_t)w, old = atomicAdd(&sh.mass_low[b], low), high = (uint32_t)(w >> 32) + (old + low < old);
-                if (high) atomicAdd(&sh.mass_high[b], high);
-            }
-        });
+                int k = 0;
+                const u64 w = masses ? sm_weight(in_steps(x), sh.table, &k) : 0;
+                const uint32_t b = linear ? bin_of(x) : (uint32_t)((hi - o) >> shift), low = (uint32_t)w;
+                if (masses) {
+                    const uint32_t old = atomicAdd(&sh.mass_low[b], low), high = (uint32_t)(w >> 32) + (old + low < old);
+                    if (high) atomicAdd(&sh.mass_high[b], high);
+                }
+                atomicAdd(&sh.count[b], 1u);
+            });
         __syncthreads();
         cluster_sync();
     };
@@ -236,11 +277,17 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 2 : 4) k_sample(const
         const uint32_t first_bin = sh.found_bin;
         if (upto <= kSmList) {
             // few: they go to the first CTA
-            each(0, n, tid, T_, [&](float x, uint32_t i) {
-                if (bin_of(x) > first_bin) return;
+            auto give = [&](float x, uint32_t i) {
                 uint32_t at;
                 asm volatile("atom.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(sm_at(&sh.n_all, 0)) : "memory");
                 asm volatile("st.shared::cluster.v2.u64 [%0], {%1, %2};" ::"r"(sm_at(&sh.all_list[at], 0)), "l"(sm_order(x, v0 + i)), "l"(weight(x)) : "memory");
+            };
+            fours(0, n, tid, T_, [&](const float (&x)[4], uint32_t i, uint32_t valid) {
+                uint32_t b[4];
+#pragma unroll
+                for (uint32_t e = 0; e < 4; e++) b[e] = bin_of(x[e]);
+#pragma unroll
+                for (uint32_t e = 0; e < 4; e++) if (e < valid && b[e] <= first_bin) give(x[e], i + e);
             });
             __syncthreads();
             cluster_sync();                                          // (before that no CTA leaves: its bins are read)
@@ -302,7 +349,7 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 2 : 4) k_sample(const
             for (uint32_t t = tid; t < size; t += T_) {
                 const ulonglong2 x = sh.all_list[t];
                 const float v = sm_value((uint32_t)(x.x >> kSmIndexBits));
-                const bool on = t < count && x.y && exponent(v) >= least;
+                const bool on = t < count && x.y && v >= least_x;
                 sh.all_list[t] = make_ulonglong2(t < count ? (x.x & kSmIndexMask) << 32 | __float_as_uint(v) : 0, on ? x.y : 0);
             }
             sort();
@@ -358,8 +405,9 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 2 : 4) k_sample(const
                 }
                 uint32_t* const n_list = &sh.n_list[1];
                 each(0, n, tid, T_, [&](float x, uint32_t i) {
+                    if (linear && bin_of(x) != bin) return;
                     const u64 o = sm_order(x, v0 + i);
-                    if (o < lo || o > hi || (linear ? bin_of(x) : (uint32_t)((hi - o) >> shift)) != bin) return;
+                    if (o < lo || o > hi || (!linear && (uint32_t)((hi - o) >> shift) != bin)) return;
                     sh.list[atomicAdd(n_list, 1u)] = make_ulonglong2(o, by_mass ? weight(x) : 1);
                 });
                 __syncthreads();
@@ -393,15 +441,20 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 2 : 4) k_sample(const
     }
     // the draw: sums of what stays by warps' parts, then the part in which u of all is passed
     const uint32_t part = ((n + kWarps - 1) / kWarps + 127) / 128 * 128, from = min(warp * part, n), to = min(from + part, n);
-    const float last = threshold ? sm_value((uint32_t)(threshold >> kSmIndexBits)) : -INFINITY;      // what stays: larger logits, and this one up to an index
-    const uint32_t last_index = threshold ? kSmIndexMask - (uint32_t)(threshold & kSmIndexMask) : 0xffffffffu;
-    auto stays = [&](float x, uint32_t i) {
-        if (x < last || (x == last && v0 + i > last_index)) return (u64)0;
-        const double e = exponent(x);
-        return e >= least ? sm_weight(e, sh.table) : (u64)0;
+    const float cut = threshold ? sm_value((uint32_t)(threshold >> kSmIndexBits)) : -INFINITY, last = fmaxf(cut, least_x);      // what stays: larger logits, and this one up to an index
+    const uint32_t last_index = threshold && cut >= least_x ? kSmIndexMask - (uint32_t)(threshold & kSmIndexMask) : 0xffffffffu;
+    auto stays = [&](const float (&x)[4], uint32_t i, uint32_t valid, u64 (&w)[4]) {
+#pragma unroll
+        for (uint32_t e = 0; e < 4; e++) w[e] = weight(x[e]);
+#pragma unroll
+        for (uint32_t e = 0; e < 4; e++) if (!(e < valid && (x[e] > last || (x[e] == last && v0 + i + e <= last_index)))) w[e] = 0;
     };
     u64 sum = 0;
-    each(from, to, lane, 32, [&](float x, uint32_t i) { sum += stays(x, i); });
+    fours(from, to, lane, 32, [&](const float (&x)[4], uint32_t i, uint32_t valid) {
+        u64 w[4];
+        stays(x, i, valid, w);
+        sum += (w[0] + w[1]) + (w[2] + w[3]);
+    });
     sum = warp_sum64(sum);
     __syncthreads();
     if (lane == 0) sh.warp_mass[warp] = sum;
@@ -416,15 +469,12 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 2 : 4) k_sample(const
     for (uint32_t i = 0; i < warp; i++) base += sh.warp_mass[i];
     if (!((double)base > drawn) && (double)(base + sum) > drawn) {
         for (uint32_t i = from; i < to; i += 128) {                  // a lane's four neighbours at a time
-            float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            u64 w[4] = {0, 0, 0, 0}, mine = 0;
-            each(i, min(i + 128, to), lane, 32, [&](float v, uint32_t at) {
-                const uint32_t k = at & 3;
-                const u64 y = stays(v, at);
-#pragma unroll
-                for (uint32_t q = 0; q < 4; q++) if (q == k) { x[q] = v; w[q] = y; }
-                mine += y;
-            });
+            const uint32_t place = i + 4 * lane;
+            const float4 y = four(place, true);
+            const float x[4] = {y.x, y.y, y.z, y.w};
+            u64 w[4];
+            stays(x, place, place < to ? to - place : 0, w);
+            const u64 mine = (w[0] + w[1]) + (w[2] + w[3]);
             u64 upto = mine;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) { const u64 t = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= (uint32_t)o) upto += t; }

@@ -277,11 +277,8 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 2 : 4) k_sample(const
         const uint32_t first_bin = sh.found_bin;
         if (upto <= kSmList) {
             // few: they go to the first CTA
-            auto give = [&](float x, uint32_t i) {
-                uint32_t at;
-                asm volatile("atom.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(sm_at(&sh.n_all, 0)) : "memory");
-                asm volatile("st.shared::cluster.v2.u64 [%0], {%1, %2};" ::"r"(sm_at(&sh.all_list[at], 0)), "l"(sm_order(x, v0 + i)), "l"(weight(x)) : "memory");
-            };
+            uint32_t* const n_list = &sh.n_list[1];
+            auto give = [&](float x, uint32_t i) { sh.list[atomicAdd(n_list, 1u)] = make_ulonglong2(sm_order(x, v0 + i), weight(x)); };
             fours(0, n, tid, T_, [&](const float (&x)[4], uint32_t i, uint32_t valid) {
                 uint32_t b[4];
 #pragma unroll
@@ -290,26 +287,48 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 2 : 4) k_sample(const
                 for (uint32_t e = 0; e < 4; e++) if (e < valid && b[e] <= first_bin) give(x[e], i + e);
             });
             __syncthreads();
+            // (one addition to the first CTA's number for a CTA's candidates: a thousand of them one by one took 20 us)
+            if (tid == 0) {
+                uint32_t begin;
+                asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(begin) : "r"(sm_at(&sh.n_all, 0)), "r"(*n_list) : "memory");
+                sh.n_list[0] = begin;
+            }
+            __syncthreads();
+            for (uint32_t t = tid; t < *n_list; t += T_) {
+                const ulonglong2 x = sh.list[t];
+                asm volatile("st.shared::cluster.v2.u64 [%0], {%1, %2};" ::"r"(sm_at(&sh.all_list[sh.n_list[0] + t], 0)), "l"(x.x), "l"(x.y) : "memory");
+            }
             cluster_sync();                                          // (before that no CTA leaves: its bins are read)
             if (rank != 0) return;
             const uint32_t count = sh.n_all;
-            uint32_t size = 32;
-            while (size < count) size *= 2;
-            // in falling order of x (the order of the logits; then that of falling numbers, in which indices rise), what is behind the last one 0
-            // (by one warp where they are few, which waits for itself alone)
-            const uint32_t sorters = size <= 256 ? 32 : T_;
-            auto sort = [&] {
+            // In falling order of x (the order of the logits; then that of falling numbers, in which indices rise): placed by buckets, which rise as x falls, then ranked in their bucket.
+            auto sort = [&](auto&& bucket) {
+                for (uint32_t i = tid; i < kSmBins; i += T_) sh.count[i] = 0;
                 __syncthreads();
-                for (uint32_t k = 2; k <= size; k *= 2)
-                    for (uint32_t d = k / 2; d > 0; d /= 2) {
-                        if (tid < sorters)
-                            for (uint32_t t = tid; t < size / 2; t += sorters) {
-                                const uint32_t i = 2 * t - (t & (d - 1)), j = i + d;
-                                const ulonglong2 x = sh.all_list[i], y = sh.all_list[j];
-                                if (x.x < y.x == !(i & k)) { sh.all_list[i] = y; sh.all_list[j] = x; }
-                            }
-                        if (sorters == 32) __syncwarp(); else __syncthreads();
-                    }
+                for (uint32_t t = tid; t < count; t += T_) atomicAdd(&sh.count[bucket(sh.all_list[t])], 1u);
+                __syncthreads();
+                uint32_t begin[kBinsEach], sum = 0;
+#pragma unroll
+                for (uint32_t k = 0; k < kBinsEach; k++) { begin[k] = sum; sum += sh.count[kBinsEach * tid + k]; }
+                uint32_t before = sum;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) { const uint32_t t = __shfl_up_sync(0xffffffffu, before, o); if (lane >= (uint32_t)o) before += t; }
+                if (lane == 31) sh.warp_count[warp] = before;
+                __syncthreads();
+#pragma unroll
+                for (uint32_t i = 0; i < kWarps; i++) if (i < warp) before += sh.warp_count[i];
+#pragma unroll
+                for (uint32_t k = 0; k < kBinsEach; k++) sh.count[kBinsEach * tid + k] = sh.mass_low[kBinsEach * tid + k] = before - sum + begin[k];
+                __syncthreads();
+                for (uint32_t t = tid; t < count; t += T_) { const ulonglong2 x = sh.all_list[t]; sh.list[atomicAdd(&sh.count[bucket(x)], 1u)] = x; }
+                __syncthreads();
+                for (uint32_t t = tid; t < count; t += T_) {
+                    const ulonglong2 x = sh.list[t];
+                    const uint32_t b = bucket(x), first = sh.mass_low[b], end = sh.count[b];
+                    uint32_t at = first;
+                    for (uint32_t i = first; i < end; i++) at += sh.list[i].x > x.x;
+                    sh.all_list[at] = x;
+                }
                 __syncthreads();
             };
             // sums of y up to each place; the sum of all
@@ -318,7 +337,7 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 2 : 4) k_sample(const
             auto scan = [&] {
                 u64 sum = 0;
 #pragma unroll
-                for (uint32_t k = 0; k < kEach; k++) { const uint32_t t = kEach * tid + k; sum += t < size ? sh.all_list[t].y : 0; upto_[k] = sum; }
+                for (uint32_t k = 0; k < kEach; k++) { const uint32_t t = kEach * tid + k; sum += t < count ? sh.all_list[t].y : 0; upto_[k] = sum; }
                 u64 before = sum;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) { const u64 t = __shfl_up_sync(0xffffffffu, before, o); if (lane >= (uint32_t)o) before += t; }
@@ -332,33 +351,33 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 2 : 4) k_sample(const
                 for (uint32_t k = 0; k < kEach; k++) upto_[k] += before - sum;
                 return all;
             };
-            for (uint32_t t = count + tid; t < size; t += T_) sh.all_list[t] = make_ulonglong2(0, 0);
-            sort();
+            sort([&](const ulonglong2& x) { return bin_of(sm_value((uint32_t)(x.x >> kSmIndexBits))); });
             if (by_k) {
-                for (uint32_t t = top_k + tid; t < size; t += T_) sh.all_list[t].y = 0;
+                for (uint32_t t = top_k + tid; t < count; t += T_) sh.all_list[t].y = 0;
                 __syncthreads();
             }
             if (by_p) {
                 const u64 sum = scan();
                 if (by_k) target = max((u64)1, (u64)ceil((double)top_p * (double)sum));
 #pragma unroll
-                for (uint32_t k = 0; k < kEach; k++) { const uint32_t t = kEach * tid + k; if (t < size && upto_[k] - sh.all_list[t].y >= target) sh.all_list[t].y = 0; }
+                for (uint32_t k = 0; k < kEach; k++) { const uint32_t t = kEach * tid + k; if (t < count && upto_[k] - sh.all_list[t].y >= target) sh.all_list[t].y = 0; }
+                __syncthreads();
             }
-            __syncthreads();
             // in order of their indices
-            for (uint32_t t = tid; t < size; t += T_) {
+            for (uint32_t t = tid; t < count; t += T_) {
                 const ulonglong2 x = sh.all_list[t];
                 const float v = sm_value((uint32_t)(x.x >> kSmIndexBits));
-                const bool on = t < count && x.y && v >= least_x;
-                sh.all_list[t] = make_ulonglong2(t < count ? (x.x & kSmIndexMask) << 32 | __float_as_uint(v) : 0, on ? x.y : 0);
+                const bool on = x.y && v >= least_x;
+                sh.all_list[t] = make_ulonglong2((x.x & kSmIndexMask) << 32 | __float_as_uint(v), on ? x.y : 0);
             }
-            sort();
+            const uint32_t width = (a.V + kSmBins - 1) / kSmBins;
+            sort([&](const ulonglong2& x) { return (kSmIndexMask - (uint32_t)(x.x >> 32)) / width; });
             const u64 all = scan();
             const double drawn = (double)u * (double)all;
 #pragma unroll
             for (uint32_t k = 0; k < kEach; k++) {
                 const uint32_t t = kEach * tid + k;
-                if (t >= size) break;
+                if (t >= count) break;
                 const ulonglong2 x = sh.all_list[t];
                 if (x.y && !((double)(upto_[k] - x.y) > drawn) && (double)upto_[k] > drawn) draw(__uint_as_float((uint32_t)x.x), kSmIndexMask - (uint32_t)(x.x >> 32), all);
             }

@@ -21,6 +21,7 @@ struct PgArgs {
     float scale, cap;
 };
 constexpr uint32_t kPgTile = 32, kPgShift = 29, kPgFlush = 512;      // (512 tiles of 32 products of two bytes: below 2^31)
+constexpr uint32_t kPgPlan = 8;                                     // words of the plan before the rows' tiles: all tiles (64 bits), warps, -, warps / tiles (64 bits)
 constexpr uint32_t kPgRows = 8, kPgLeast = 2;                                     // tiles a warp at least, where there are few
 constexpr float kPgSlack = 3.0f;                                     // weights reach 2^(29 + 3)
 // Warps (CTAs) of an SM, by their registers: 168, 128 or 255 a thread.
@@ -115,7 +116,7 @@ __global__ void __launch_bounds__(32, pg_warps(KC, VC, NT)) k_paged(const __grid
     PgGroup group;
     if (a.part) {
         // Tiles before each row, of all, and the row in which the warp's share begins.  The rows of a step of at most 32 * kPgRows are read at once and kept.
-        uint64_t* const before = reinterpret_cast<uint64_t*>(a.plan + 4);
+        uint64_t* const before = reinterpret_cast<uint64_t*>(a.plan + kPgPlan);
         auto upto = [&](uint32_t mine) {
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) { const uint32_t t = __shfl_up_sync(0xffffffffu, mine, o); if (lane >= (uint32_t)o) mine += t; }
@@ -150,7 +151,7 @@ __global__ void __launch_bounds__(32, pg_warps(KC, VC, NT)) k_paged(const __grid
         }
         const uint64_t total = all * per_row;
         const uint32_t warps = (uint32_t)min((uint64_t)gridDim.x, max((uint64_t)1, total / kPgLeast));
-        if (blockIdx.x == 0 && lane == 0) { before[live] = all; a.plan[0] = (uint32_t)total; a.plan[1] = (uint32_t)(total >> 32); a.plan[2] = warps; }
+        if (blockIdx.x == 0 && lane == 0) { before[live] = all; a.plan[0] = (uint32_t)total; a.plan[1] = (uint32_t)(total >> 32); a.plan[2] = warps; *reinterpret_cast<double*>(a.plan + 4) = total ? (double)warps / (double)total : 0.0; }
         const bool idle = blockIdx.x >= warps || !total;
         for (uint32_t row = gridDim.x - 1 - blockIdx.x; row < live; row += gridDim.x) settle(row);      // (from the last warp on, which may have nothing else to do)
         if (idle) return;
@@ -501,49 +502,92 @@ __global__ void __launch_bounds__(32, pg_warps(KC, VC, NT)) k_paged(const __grid
     if (gave_up && lane == 0) count_timeout();
 }
 
-// CTA (query of a group of rows, row that begins it): the records of a sequence that several warps took.
+// The records of a sequence that several warps took: a warp a query, or (SHARED) the four of a CTA, a quarter of the records each.  Bound by latency: eight records at a time, statistics
+// and outputs at once.
+template <bool SHARED>
 __global__ void __launch_bounds__(128) k_paged_join(const __grid_constant__ PgArgs a, const uint32_t queries) {
     pdl_enter();
-    __shared__ float parts[4][256];
     const PageShape& s = a.s;
-    const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, r = blockIdx.y, item = blockIdx.x / queries, i = blockIdx.x % queries, per_row = s.G * a.chunks;
+    const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, r = blockIdx.y, query = SHARED ? blockIdx.x : 4 * blockIdx.x + warp, item = query / queries, i = query % queries, per_row = s.G * a.chunks;
     const uint32_t live = batch_head(a.table, a.B).rows;
-    const uint64_t* const before = reinterpret_cast<const uint64_t*>(a.plan + 4);
+    const uint64_t* const before = reinterpret_cast<const uint64_t*>(a.plan + kPgPlan);
     const uint4 plan = *reinterpret_cast<const uint4*>(a.plan);      // (asked for at once: what belongs to rows that are not live is not looked at)
+    const double inv = *reinterpret_cast<const double*>(a.plan + 4);
     const uint64_t b0 = before[r], b1 = before[r + 1];
     const BatchRow begins = batch_row(a.table, r);
-    if (r >= live || b1 == b0) return;
+    if (r >= live || b1 == b0 || item >= per_row) return;
     const uint64_t all = plan.x | (uint64_t)plan.y << 32, tiles = b1 - b0, first = b0 * per_row + item * tiles;
     const uint32_t warps = plan.z;
-    const uint32_t w0 = (uint32_t)(((first + 1) * warps - 1) / all), w1 = (uint32_t)(((first + tiles) * warps - 1) / all), count = w1 - w0 + 1;
+    auto taker = [&](uint64_t tile) {                                // the last warp whose share begins at or before the tile
+        const uint64_t n = (tile + 1) * warps - 1;
+        uint32_t w = min((uint32_t)((double)tile * inv), warps - 1);
+        while (w + 1 < warps && all * (w + 1) <= n) w++;
+        while (w && all * w > n) w--;
+        return w;
+    };
+    const uint32_t w0 = taker(first), w1 = taker(first + tiles - 1), count = w1 - w0 + 1;
     const uint32_t heads = min(a.rep, queries), token = i / heads, g = item / a.chunks, h = item % a.chunks * heads + i % heads;
     if (w0 == w1 || h >= a.rep || (token && token >= pg_group(a, live, r, begins.slot).rows)) return;
     const BatchRow z = token ? batch_row(a.table, r + token) : begins;
     if (!page_row_ok(a.pool, s, z) || z.length == 0) return;
     const uint32_t pitch = s.vp + 4;
-    auto record = [&](uint32_t k) { return a.part + ((size_t)(2 * (w0 + k) + (k ? 0 : 1)) * queries + i) * pitch; };
-    float top_m = -INFINITY, top_n = -INFINITY, sum = 0.0f, v[8] = {};
-    for (uint32_t k = lane; k < count; k += 32) { const float2 x = *reinterpret_cast<const float2*>(record(k)); top_m = fmaxf(top_m, x.x); top_n = fmaxf(top_n, x.y); }
-    top_m = warp_max(top_m); top_n = warp_max(top_n);
-    for (uint32_t k = lane; k < count; k += 32) { const float4 x = *reinterpret_cast<const float4*>(record(k)); sum = fmaf(x.z, pg_frame(x.x, top_m), sum); }
-    sum = warp_sum(sum);
-#pragma unroll 4
-    for (uint32_t k = warp; k < count; k += 4) {
-        const float* x = record(k);
-        const float f = pg_frame(x[1], top_n);
+    constexpr uint32_t kAtOnce = 8, kStep = SHARED ? 4 : 1;
+    float m = -INFINITY, n = -INFINITY, sum = 0.0f;
+    float4 v[2] = {make_float4(0.0f, 0.0f, 0.0f, 0.0f), make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
+    auto add = [](float4& to, float f, const float4& x) { to.x = fmaf(f, x.x, to.x); to.y = fmaf(f, x.y, to.y); to.z = fmaf(f, x.z, to.z); to.w = fmaf(f, x.w, to.w); };
+    for (uint32_t k0 = SHARED ? warp : 0; k0 < count; k0 += kAtOnce * kStep) {
+        float4 st[kAtOnce], x[kAtOnce][2];
 #pragma unroll
-        for (uint32_t e = 0; e < 8; e++) if (lane + 32 * e < s.dv) v[e] = fmaf(x[4 + lane + 32 * e], f, v[e]);
+        for (uint32_t e = 0; e < kAtOnce; e++) {
+            const uint32_t k = k0 + e * kStep;
+            st[e] = make_float4(-INFINITY, -INFINITY, 0.0f, 0.0f); x[e][0] = x[e][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (k >= count) continue;
+            const float* const from = a.part + ((size_t)(2 * (w0 + k) + (k ? 0 : 1)) * queries + i) * pitch;
+            st[e] = *reinterpret_cast<const float4*>(from);
+            if (4 * lane < s.vp) x[e][0] = *reinterpret_cast<const float4*>(from + 4 + 4 * lane);
+            if (128 + 4 * lane < s.vp) x[e][1] = *reinterpret_cast<const float4*>(from + 132 + 4 * lane);
+        }
+        float new_m = m, new_n = n;
+#pragma unroll
+        for (uint32_t e = 0; e < kAtOnce; e++) { new_m = fmaxf(new_m, st[e].x); new_n = fmaxf(new_n, st[e].y); }
+        const float f = pg_frame(n, new_n);
+        sum *= pg_frame(m, new_m);
+        v[0].x *= f; v[0].y *= f; v[0].z *= f; v[0].w *= f; v[1].x *= f; v[1].y *= f; v[1].z *= f; v[1].w *= f;
+        m = new_m; n = new_n;
+#pragma unroll
+        for (uint32_t e = 0; e < kAtOnce; e++) {
+            sum = fmaf(st[e].z, pg_frame(st[e].x, m), sum);
+            const float w = pg_frame(st[e].y, n);
+            add(v[0], w, x[e][0]); add(v[1], w, x[e][1]);
+        }
     }
+    if constexpr (SHARED) {
+        __shared__ float stats[4][3];
+        __shared__ float4 parts[4][64];
+        if (lane == 0) { stats[warp][0] = m; stats[warp][1] = n; stats[warp][2] = sum; }
+        parts[warp][lane] = v[0]; parts[warp][32 + lane] = v[1];
+        __syncthreads();
+        if (warp) return;
+        m = n = -INFINITY; sum = 0.0f;
+        for (uint32_t k = 0; k < 4; k++) { m = fmaxf(m, stats[k][0]); n = fmaxf(n, stats[k][1]); }
+        v[0] = v[1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (uint32_t k = 0; k < 4; k++) {
+            sum = fmaf(stats[k][2], pg_frame(stats[k][0], m), sum);
+            const float w = pg_frame(stats[k][1], n);
+            add(v[0], w, parts[k][lane]); add(v[1], w, parts[k][32 + lane]);
+        }
+    }
+    const float2 f = pg_finish(a, g * a.rep + h, m, n, sum);
+    float* const to = a.dst + (size_t)(r + token) * a.dst_rs + (g * a.rep + h) * s.dv;
 #pragma unroll
-    for (uint32_t e = 0; e < 8; e++) parts[warp][lane + 32 * e] = v[e];
-    __syncthreads();
-    const float2 f = pg_finish(a, g * a.rep + h, top_m, top_n, sum);
-    for (uint32_t d = threadIdx.x; d < s.dv; d += 128)
-        a.dst[(size_t)(r + token) * a.dst_rs + (g * a.rep + h) * s.dv + d] = pg_scaled((parts[0][d] + parts[1][d] + parts[2][d] + parts[3][d]) / f.y, f.x);
+    for (uint32_t e = 0; e < 8; e++) {
+        const uint32_t d = 128 * (e / 4) + 4 * lane + e % 4;
+        if (d < s.dv) to[d] = pg_scaled(reinterpret_cast<const float*>(&v[e / 4])[e % 4] / f.y, f.x);
+    }
 }
 
 // floats before the records: the plan
-size_t pg_plan_elems(uint32_t B) { return (4 + 2 * ((size_t)B + 1) + 3) / 4 * 4; }
+size_t pg_plan_elems(uint32_t B) { return (kPgPlan + 2 * ((size_t)B + 1) + 3) / 4 * 4; }
 template <int KC, int VC, int NT, bool FULL>
 bool pg_launch_as(const PgArgs& a, cudaStream_t st) {
     const size_t smem = kPgTile * (a.s.kp + a.s.vp) + 32 + sizeof(float) * 4 * NT * (a.s.vp + 4);
@@ -557,15 +601,19 @@ template <int KC, int VC, int NT>
 bool pg_launch(const PgArgs& a, cudaStream_t st) {
     return a.s.kp == 32 * KC && a.s.vp == 16 * VC ? pg_launch_as<KC, VC, NT, true>(a, st) : pg_launch_as<KC, VC, NT, false>(a, st);
 }
-// Queries that a warp takes together: of one row, or, where the step has more rows than the page table slots, of the rows that a slot has then.
-struct PgForm { bool narrow, wide; uint32_t queries; };
+// Queries that a warp takes together: four, of one row, or, where the step has more rows than the page table slots, of a slot's rows that follow one another; eight where a key head
+// has more than four and the caches are large, whose pages then come through L2 once for them (32 / 8 heads of 128 doubled, us, with four and with eight: 16 rows of up to 65536 tokens
+// 390 / 269, 64 rows of up to 4096 101 / 100; 64 rows of 32 / 2 heads of up to 4096 51 / 61, 9 x 7 rows of up to 2111 42 / 51).
+struct PgForm { bool narrow, wide; uint32_t queries, tokens; };
+constexpr uint64_t kPgLarge = 1u << 21;
 PgForm pg_form(const ZgSeqOp& op, uint32_t slots) {
     PgForm f;
     const PageShape s = page_shape(op.n[2], op.n[3], op.n[4], op.n[7]);
+    const uint32_t rep = op.n[1] / op.n[2];
     f.narrow = s.kp <= 64 && s.vp <= 64;
     f.wide = s.kp > 128 || s.vp > 128;
-    const uint64_t rep = op.n[1] / op.n[2], together = rep * std::max<uint32_t>(1, op.n[0] / std::max(1u, slots));
-    f.queries = together <= 4 || f.wide ? 4 : 8;
+    f.queries = rep > 4 && !f.wide && (uint64_t)op.n[0] * op.n[2] * ((uint64_t)op.n[8] << s.shift) >= kPgLarge ? 8 : 4;
+    f.tokens = op.n[0] > slots ? std::max(1u, f.queries / rep) : 1;
     return f;
 }
 
@@ -600,7 +648,7 @@ bool zg_launch_paged_attention(const ZgOp& op, float* const* bufs, const size_t*
     a.scale = s.f[0]; a.cap = s.f[1];
     const PgForm f = pg_form(s, a.pool.slots);
     a.chunks = (a.rep + f.queries - 1) / f.queries;
-    a.tokens = std::max(1u, f.queries / a.rep);
+    a.tokens = f.tokens;
     a.plan = reinterpret_cast<uint32_t*>(scratch);
     a.part = scratch ? scratch + pg_plan_elems(a.B) : nullptr;
     bool ok;
@@ -610,7 +658,10 @@ bool zg_launch_paged_attention(const ZgOp& op, float* const* bufs, const size_t*
     if (!ok) return false;
     ZG_SEQ_CHECK();
     if (a.part) {
-        launch_pdl(k_paged_join, dim3(a.s.G * a.chunks * f.queries, a.B), dim3(128), 0, st, a, f.queries);
+        // Four warps a query where few sequences and heads are shared out over all warps, so that each has a dozen records or more.
+        const uint32_t products = a.s.G * a.chunks * f.queries;
+        if ((uint64_t)a.B * a.s.G * a.chunks <= zg_sm_count()) launch_pdl(k_paged_join<true>, dim3(products, a.B), dim3(128), 0, st, a, f.queries);
+        else launch_pdl(k_paged_join<false>, dim3((products + 3) / 4, a.B), dim3(128), 0, st, a, f.queries);
         ZG_SEQ_CHECK();
     }
     return true;

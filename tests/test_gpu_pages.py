@@ -178,12 +178,15 @@ def test_page_copy(cuda_backend, words):
 
 
 # ── PAGED_ATTENTION ──────────────────────────────────────────────────────────────────────────────────────────────────
-def attend_case(be, B, H, G, dk, dv, page, most, entries, *, window=0, cap=0.0, sink=None, bf16=False, pad=0, slots=3, pages=None, live=None, seed=0, loud=1.0, lo=-7, hi=-4, scale=None, change=None, graph=True):
+def attend_case(be, B, H, G, dk, dv, page, most, entries, *, window=0, cap=0.0, sink=None, bf16=False, pad=0, slots=3, pages=None, live=None, seed=0, loud=1.0, lo=-7, hi=-4, scale=None, change=None, graph=True, spare=0):
+    """spare: columns of the page table behind those that any row uses."""
     from zgml_b200 import DeviceOp, abi
     r = np.random.default_rng(seed)
     pages = slots * most + 1 if pages is None else pages
     keys, values, scales = pool(r, pages, G, dk, dv, page, lo, hi)
-    page_table = r.permutation(pages)[:slots * most].reshape(slots, most).astype(np.int32)
+    page_table = np.full((slots, most + spare), -1, np.int32)
+    page_table[:, :most] = r.permutation(pages)[:slots * most].reshape(slots, most)
+    most += spare
     qrs, drs, scale = H * dk + 2 * pad, H * dv + pad, dk ** -0.5 if scale is None else scale
     q, dst = (loud * r.standard_normal((B, qrs))).astype(np.float32), r.standard_normal((B, drs)).astype(np.float32)
     s = None if sink is None else np.full(H, sink, np.float32) if np.ndim(sink) == 0 else np.asarray(sink, np.float32)
@@ -308,8 +311,76 @@ def test_queries_with_outliers(cuda_backend):
     attend_case(cuda_backend, 3, 4, 2, 64, 64, 16, 12, [(0, 190, 0), (1, 100, 0), (2, 3, 0)], change=change)
 
 
+@pytest.mark.parametrize("H,G,dk,dv", [(16, 2, 128, 128), (10, 2, 80, 96), (16, 2, 64, 64), (12, 2, 33, 48), (11, 1, 128, 64), (20, 2, 192, 256), (9, 3, 64, 64)])
+@pytest.mark.parametrize("page", [16, 64])
+def test_tables_of_long_sequences(cuda_backend, H, G, dk, dv, page):
+    """Page tables that could hold far more than they do: sizes go by them, answers by the rows."""
+    entries = [(i % 3, n, 0) for i, n in enumerate(LENGTHS)]
+    for window in (0, 40):
+        attend_case(cuda_backend, len(entries) + 1, H, G, dk, dv, page, 192 // page, entries, spare=(1 << 19) // page, window=window, pad=2)
+    attend_case(cuda_backend, 40, H, G, dk, dv, page, 192 // page, [(i // 15, 180 - 40 + i, 0) for i in range(40)], spare=(1 << 19) // page)      # runs of one slot
+
+
+def test_many_rows(cuda_backend):
+    """More rows than a warp reads at once, most of them short, runs of one slot across its blocks of 32, rows that are idle among them."""
+    r = np.random.default_rng(0)
+    for H, G in ((4, 4), (4, 1)):
+        attend_case(cuda_backend, 700, H, G, 32, 32, 16, 12, [(int(r.integers(-1, 3)), int(r.integers(0, 60)), 0) for _ in range(690)])
+        attend_case(cuda_backend, 400, H, G, 32, 32, 16, 12, [(i // 37 % 3, 1 + i % 192, 0) for i in range(400)], slots=3)
+        attend_case(cuda_backend, 300, H, G, 32, 32, 16, 4, [(i, 1 + i % 64, 0) for i in range(300)], slots=300)
+
+
+@pytest.mark.parametrize("H,G,dk,dv", [(8, 2, 128, 128), (9, 3, 64, 64), (6, 1, 80, 48), (4, 1, 256, 192), (5, 5, 33, 17)])
+def test_without_a_workspace(cuda_backend, monkeypatch, H, G, dk, dv):
+    """No room for records: a CTA takes whole sequences, of thousands of tiles as well."""
+    monkeypatch.setenv("ZG_CUDA_SCRATCH_MB", "0")
+    entries = [(i % 3, n, 0) for i, n in enumerate(LENGTHS)] + [(-1, 1, 0), (0, 0, 0), (3, 1, 0), (0, 193, 0)]
+    for window in (0, 50):
+        attend_case(cuda_backend, len(entries) + 1, H, G, dk, dv, 16, 12, entries, window=window, sink=0.5, spare=4000)
+    attend_case(cuda_backend, 30, H, G, dk, dv, 32, 8, [(0, 100 + i, 0) for i in range(15)] + [(1, 90 + i, 0) for i in range(15)], spare=4000)
+    if dk != 256:
+        attend_case(cuda_backend, 1, G, G, dk, dv, 64, 2400, [(0, 150011, 0)], slots=1, loud=0.1)
+
+
 def test_outside_a_graph(cuda_backend):
     attend_case(cuda_backend, 5, 8, 2, 128, 128, 16, 40, [(i % 3, 640 - 100 * i, 0) for i in range(5)], graph=False)
+
+
+# ── beyond 2^32 ──────────────────────────────────────────────────────────────────────────────────────────────────────
+def test_pages_beyond_4_gb(cuda_backend):
+    """Append, read, attend and copy where pages lie more than 4 GB into their pool."""
+    from zgml_b200 import DeviceBuffer, DeviceOp, DeviceProgram, ExternBuffer, ProgramIO
+    r = np.random.default_rng(4)
+    G, H, dk, dv, page, most, B = 8, 16, 128, 128, 64, 2, 3
+    words = page_words(G, dk, dv, page)
+    count = (9 << 30) // (4 * words)
+    memory = DeviceBuffer(cuda_backend, 4 * words * count, zero=False)
+    used = [count - 1, count // 2 + 7, count - 5, 3, count - 2, count - 9]
+    state = pool(r, 6, G, dk, dv, page)
+    for i, p in enumerate(used):
+        memory.upload(pack_pages(*(x[i:i + 1] for x in state)), 4 * words * p)
+    near = np.array([[0, 1], [2, 3], [4, 5]], np.int32)
+    far = np.array(used, np.int32)[near]
+    entries = [(0, 100, 0), (1, 64, 0), (2, 3, 0)]
+    src, q = r.standard_normal((B, G * (dk + dv))).astype(np.float32), r.standard_normal((B, H * dk)).astype(np.float32)
+    sizes = [memory.elems, src.size, far.size, 8 + 4 * B, q.size, B * H * dv, B * G * (dk + dv), move_words(2)]
+    ops = [DeviceOp.page_append(0, 1, 2, 3, 0, G * dk, B, G, dk, dv, G * (dk + dv), page, most), DeviceOp.paged_attention(5, 4, 0, 2, 3, B, H, G, dk, dv, H * dk, page, most, dk ** -0.5),
+           DeviceOp.page_read(6, 0, 2, 3, B, G, dk, dv, page, most), DeviceOp.page_copy(0, 7, 2, words)]
+    h = cuda_backend.compile_program(DeviceProgram(ops, sizes, externs=[ExternBuffer(0, memory)]))
+    out, back = np.zeros((B, H, dv), np.float32), np.zeros((B, G * (dk + dv)), np.float32)
+    moves = [(used[0], count - 20), (used[3], count - 21)]
+    f = lambda a: np.ascontiguousarray(a).view(np.float32).ravel()
+    cuda_backend.execute_program(h, [ProgramIO(1, f(src)), ProgramIO(2, f(far)), ProgramIO(3, f(table(entries, B))), ProgramIO(4, f(q)), ProgramIO(7, f(page_moves(moves, 2, count)))], [ProgramIO(5, out), ProgramIO(6, back)])
+    k, v, s, _ = ref.append(*state, src, near, entries, B, 0, (0, G * dk, 0), B, G, dk, dv, page)
+    want, tol = ref.attend(np.zeros((B, H, dv)), q.reshape(B, H, dk), k, v, s, near, entries, B, B, dk ** -0.5)
+    close(out, want, tol)
+    assert np.array_equal(back, ref.read(k, v, s, near, entries, B, B, np.zeros((B, G * (dk + dv)))).astype(np.float32))
+    for source, to in moves:
+        a, b = (memory.download(np.int32, 4 * words * p, words) for p in (source, to))
+        assert np.array_equal(a, b)
+    assert np.array_equal(memory.download(np.int32, 4 * words * used[0], words)[:4].view(np.float32)[:2], s[0, 0].astype(np.float32))
+    cuda_backend.free_program(h)
+    memory.free()
 
 
 # ── together ─────────────────────────────────────────────────────────────────────────────────────────────────────────

@@ -16,7 +16,7 @@ namespace {
 struct PgArgs {
     PagePool pool; PageShape s;
     float* dst; const float* q; const float* table; const void* sink;
-    uint32_t* plan; float* part;     // what k_paged leaves for k_paged_join (null: a warp takes whole sequences)
+    uint32_t* plan; float* part;     // what k_paged leaves for k_paged_join
     uint32_t B, H, rep, q_rs, dst_rs, window, sink_bf16, tokens, chunks;      // tokens of a sequence a warp takes together, chunks of a key head's query heads
     float scale, cap;
 };
@@ -90,19 +90,19 @@ __device__ __forceinline__ uint64_t pg_share(uint64_t all, uint32_t w, uint32_t 
 
 // A warp of its own CTA takes a share of all tiles of the step - one group of rows after the other, one key head (and chunk of its query heads) after the other - so that
 // warps have equal work whatever the sequences' lengths are, and none waits for another.  What it takes of a sequence begins or ends with it, or leaves a record for
-// k_paged_join: (m, n, sum, outputs) of each query.  A tile's next keys come while its weights and outputs are computed, its next values while the scores are.
-// 4 NT queries at a time, query 4 t + lane % 4 a lane.
-template <int KC, int VC, int NT, bool FULL>
-__global__ void __launch_bounds__(32, pg_warps(KC, VC, NT)) k_paged(const __grid_constant__ PgArgs a) {
+// k_paged_join: (m, n, sum, outputs) of each query.  (W = 8: a CTA of eight warps for each group and key head, whose records are joined in shared memory: one launch, for few short sequences
+// and where there is no workspace.)  A tile's next keys come while its weights and outputs are computed, its next values while the scores are.  4 NT queries at a time, query 4 t + lane % 4 a lane.
+template <int KC, int VC, int NT, bool FULL, int W>
+__global__ void __launch_bounds__(32 * W, W == 1 ? pg_warps(KC, VC, NT) : 1) k_paged(const __grid_constant__ PgArgs a) {
     pdl_enter();
     extern __shared__ float4 pg_mem[];
-    __shared__ uint64_t bars[2];                                     // of keys and values
+    __shared__ uint64_t bars[W][2];                                  // of a warp's keys and values
     const PageShape& s = a.s;
-    const uint32_t lane = threadIdx.x, row8 = lane / 4, j = lane % 4;
+    const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, row8 = lane / 4, j = lane % 4;
     const uint32_t heads = min(a.rep, 4u * NT), per_row = s.G * a.chunks;      // query heads of a chunk; products of a group of rows
     const uint32_t live = batch_head(a.table, a.B).rows;
     const uint32_t kp = FULL ? 32 * KC : s.kp, vp = FULL ? 16 * VC : s.vp, kc = kp / 32, vc = vp / 16, k_bytes = kPgTile * kp, pitch = vp + 4;
-    uint8_t* const buffer = reinterpret_cast<uint8_t*>(pg_mem);
+    uint8_t* const buffer = reinterpret_cast<uint8_t*>(pg_mem) + warp * (k_bytes + kPgTile * vp + 32 + 16 * NT * pitch);
     float* const rec = reinterpret_cast<float*>(buffer + k_bytes + kPgTile * vp + 32);      // [4 NT][pitch]
     // rows that see nothing, or whose words are out of range
     auto settle = [&](uint32_t row) {
@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(32, pg_warps(KC, VC, NT)) k_paged(const __grid
     uint32_t r, item, off;
     uint64_t left;                                                   // tiles that the warp takes
     PgGroup group;
-    if (a.part) {
+    if constexpr (W == 1) {
         // Tiles before each row, of all, and the row in which the warp's share begins.  The rows of a step of at most 32 * kPgRows are read at once and kept.
         uint64_t* const before = reinterpret_cast<uint64_t*>(a.plan + kPgPlan);
         auto upto = [&](uint32_t mine) {
@@ -178,18 +178,19 @@ __global__ void __launch_bounds__(32, pg_warps(KC, VC, NT)) k_paged(const __grid
         } else for (uint32_t row = 0; row < live && !look(row, pg_tiles(a, live, row, run)); row += 32) {}
         group = pg_group(a, live, r, batch_row(a.table, r).slot);
     } else {
-        r = blockIdx.x / per_row; item = blockIdx.x % per_row; off = 0;
+        r = blockIdx.x / per_row; item = blockIdx.x % per_row;
         if (r >= live) return;
-        if (item == 0) settle(r);
+        if (item == 0 && warp == 0) settle(r);
         const int32_t slot = batch_row(a.table, r).slot;
         uint32_t back = 0;                                           // rows of the same slot directly before r
-        while (back < r && batch_row(a.table, r - 1 - back).slot == slot) back++;
+        while (a.tokens > 1 && back < r && batch_row(a.table, r - 1 - back).slot == slot) back++;
         if (slot < 0 || back % a.tokens) return;
         group = pg_group(a, live, r, slot);
-        left = group.tiles;
-        if (!left) return;
+        if (!group.tiles) return;
+        off = (uint32_t)pg_share(group.tiles, warp, W);
+        left = (uint32_t)pg_share(group.tiles, warp + 1, W) - off;
     }
-    const uint32_t k_bar = smem_u32(&bars[0]), v_bar = k_bar + 8, at = smem_u32(buffer), heads_at = at + k_bytes + kPgTile * vp;
+    const uint32_t k_bar = smem_u32(&bars[warp][0]), v_bar = k_bar + 8, at = smem_u32(buffer), heads_at = at + k_bytes + kPgTile * vp;
     if (lane == 0) {
         mbar_init(k_bar, 2);
         mbar_init(v_bar, 2);
@@ -227,7 +228,7 @@ __global__ void __launch_bounds__(32, pg_warps(KC, VC, NT)) k_paged(const __grid
             }
         };
         int32_t id = find(t0);
-        if (!gave_up) { fetch(t0, id, false); fetch(t0, id, true); }
+        if (!gave_up && (W == 1 || take)) { fetch(t0, id, false); fetch(t0, id, true); }
         __syncwarp();
         id = find(t0 + 1);
         // what the lane's queries see, and its column of the first product: three of the six digits of a query, and 128 times their sums
@@ -451,8 +452,8 @@ __global__ void __launch_bounds__(32, pg_warps(KC, VC, NT)) k_paged(const __grid
 #pragma unroll
             for (int t = 0; t < NT; t++) sum[t] = kBatchNaN;
         }
-        const bool whole = take == group.tiles;
-        float* const record = whole ? nullptr : a.part + (size_t)(2 * blockIdx.x + (off ? 0 : 1)) * 4 * NT * pitch;
+        const bool whole = W == 1 && take == group.tiles;
+        float* const record = whole ? nullptr : W > 1 ? rec : a.part + (size_t)(2 * blockIdx.x + (off ? 0 : 1)) * 4 * NT * pitch;      // (a lane's own places of rec again)
 #pragma unroll
         for (int t = 0; t < NT; t++) {
             float top = m[t];
@@ -471,8 +472,8 @@ __global__ void __launch_bounds__(32, pg_warps(KC, VC, NT)) k_paged(const __grid
                 f = pg_finish(a, g * a.rep + h, top, n[t], sum[t]);
                 to = a.dst + (size_t)(r + token) * a.dst_rs + (g * a.rep + h) * s.dv;
             } else {
-                to = record + i * pitch + 4;
-                if (row8 == 0) *reinterpret_cast<float4*>(record + i * pitch) = make_float4(top, n[t], sum[t], 0.0f);
+                to = record + i * pitch + (W > 1 ? 0 : 4);
+                if (row8 == 0) *reinterpret_cast<float4*>(record + i * pitch + (W > 1 ? vp : 0)) = make_float4(top, n[t], sum[t], 0.0f);
             }
 #pragma unroll
             for (int c = 0; c < VC; c++) {
@@ -488,7 +489,7 @@ __global__ void __launch_bounds__(32, pg_warps(KC, VC, NT)) k_paged(const __grid
         }
         __syncwarp();
         left -= take;
-        if (!left) break;
+        if (W > 1 || !left) break;
         off = 0;
         if (++item == per_row) {
             item = 0;
@@ -500,6 +501,33 @@ __global__ void __launch_bounds__(32, pg_warps(KC, VC, NT)) k_paged(const __grid
         }
     }
     if (gave_up && lane == 0) count_timeout();
+    if constexpr (W > 1) {
+        __syncthreads();
+        const uint32_t g = item / a.chunks, chunk = item % a.chunks;
+        for (uint32_t i = warp; i < group.rows * heads; i += W) {
+            const uint32_t h = chunk * heads + i % heads, row = r + i / heads;
+            const BatchRow z = batch_row(a.table, row);
+            if (h >= a.rep || !page_row_ok(a.pool, s, z) || z.length == 0) continue;
+            const float* const records = reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(pg_mem) + k_bytes + kPgTile * vp + 32) + i * pitch;
+            const size_t each = (k_bytes + kPgTile * vp + 32) / 4 + 4 * NT * pitch;
+            float m = -INFINITY, n = -INFINITY, sum = 0.0f, w[W];
+#pragma unroll
+            for (uint32_t k = 0; k < W; k++) { m = fmaxf(m, records[k * each + vp]); n = fmaxf(n, records[k * each + vp + 1]); }
+#pragma unroll
+            for (uint32_t k = 0; k < W; k++) {
+                sum = fmaf(records[k * each + vp + 2], pg_frame(records[k * each + vp], m), sum);
+                w[k] = pg_frame(records[k * each + vp + 1], n);
+            }
+            const float2 f = pg_finish(a, g * a.rep + h, m, n, sum);
+            float* const to = a.dst + (size_t)row * a.dst_rs + (g * a.rep + h) * s.dv;
+            for (uint32_t d = lane; d < s.dv; d += 32) {
+                float v = 0.0f;
+#pragma unroll
+                for (uint32_t k = 0; k < W; k++) v = fmaf(w[k], records[k * each + d], v);
+                to[d] = pg_scaled(v / f.y, f.x);
+            }
+        }
+    }
 }
 
 // The records of a sequence that several warps took: a warp a query, or (SHARED) the four of a CTA, a quarter of the records each.  Bound by latency: eight records at a time, statistics
@@ -588,31 +616,36 @@ __global__ void __launch_bounds__(128) k_paged_join(const __grid_constant__ PgAr
 
 // floats before the records: the plan
 size_t pg_plan_elems(uint32_t B) { return (kPgPlan + 2 * ((size_t)B + 1) + 3) / 4 * 4; }
-template <int KC, int VC, int NT, bool FULL>
+template <int KC, int VC, int NT, bool FULL, int W>
 bool pg_launch_as(const PgArgs& a, cudaStream_t st) {
-    const size_t smem = kPgTile * (a.s.kp + a.s.vp) + 32 + sizeof(float) * 4 * NT * (a.s.vp + 4);
-    constexpr size_t most = kPgTile * (32 * KC + 16 * VC) + 32 + sizeof(float) * 4 * NT * (16 * VC + 4);
-    if (!zg_smem_limit<k_paged<KC, VC, NT, FULL>>(most)) return false;
-    launch_pdl(k_paged<KC, VC, NT, FULL>, dim3(a.part ? pg_warps(KC, VC, NT) * zg_sm_count() : a.B * a.s.G * a.chunks), dim3(32), smem, st, a);
+    const size_t smem = W * (kPgTile * (a.s.kp + a.s.vp) + 32 + sizeof(float) * 4 * NT * (a.s.vp + 4));
+    constexpr size_t most = W * (kPgTile * (32 * KC + 16 * VC) + 32 + sizeof(float) * 4 * NT * (16 * VC + 4));
+    if (!zg_smem_limit<k_paged<KC, VC, NT, FULL, W>>(most)) return false;
+    launch_pdl(k_paged<KC, VC, NT, FULL, W>, dim3(W == 1 ? pg_warps(KC, VC, NT) * zg_sm_count() : a.B * a.s.G * a.chunks), dim3(32 * W), smem, st, a);
     return true;
 }
 // FULL: sizes that fill the kernel's, whose loops and addresses are then known when it is compiled
-template <int KC, int VC, int NT>
+template <int KC, int VC, int NT, int W>
 bool pg_launch(const PgArgs& a, cudaStream_t st) {
-    return a.s.kp == 32 * KC && a.s.vp == 16 * VC ? pg_launch_as<KC, VC, NT, true>(a, st) : pg_launch_as<KC, VC, NT, false>(a, st);
+    return a.s.kp == 32 * KC && a.s.vp == 16 * VC ? pg_launch_as<KC, VC, NT, true, W>(a, st) : pg_launch_as<KC, VC, NT, false, W>(a, st);
 }
 // Queries that a warp takes together: four, of one row, or, where the step has more rows than the page table slots, of a slot's rows that follow one another; eight where a key head
 // has more than four and the caches are large, whose pages then come through L2 once for them (32 / 8 heads of 128 doubled, us, with four and with eight: 16 rows of up to 65536 tokens
 // 390 / 269, 64 rows of up to 4096 101 / 100; 64 rows of 32 / 2 heads of up to 4096 51 / 61, 9 x 7 rows of up to 2111 42 / 51).
-struct PgForm { bool narrow, wide; uint32_t queries, tokens; };
+struct PgForm { bool narrow, wide, one; uint32_t queries, tokens; };      // one: one launch
 constexpr uint64_t kPgLarge = 1u << 21;
-PgForm pg_form(const ZgSeqOp& op, uint32_t slots) {
+// One launch, a CTA of eight warps for each sequence and key head, where the longest sequence has up to 1024 tokens and the CTAs make two waves at most (an SM holds one: its registers); else equal shares
+// and a second launch that joins them. One launch / two, us: 3 products of 64-dim heads, 64 tokens 6.2 / 10.3, 576 10.3 / 12.3, 2048 14.4 / 12.3; 128 dims, 32 products, 1024 tokens 12.3 / 16.4, 2048
+// 18.5 / 18.5; 128 products, 64 tokens 8.2 / 16.4, 4096 28.7 / 26.7; 256 products, 64 tokens 14.4 / 16.4, 1024 22.6 / 22.6, 2048 30.8 / 27.0; 512 products (four waves), 64 tokens 26.7 / 16.4.
+bool pg_one(uint64_t products, uint64_t capacity) { return products <= 2ull * zg_sm_count() && capacity <= 1024; }
+PgForm pg_form(const ZgSeqOp& op, uint32_t slots, bool scratch) {
     PgForm f;
     const PageShape s = page_shape(op.n[2], op.n[3], op.n[4], op.n[7]);
     const uint32_t rep = op.n[1] / op.n[2];
     f.narrow = s.kp <= 64 && s.vp <= 64;
     f.wide = s.kp > 128 || s.vp > 128;
-    f.queries = rep > 4 && !f.wide && (uint64_t)op.n[0] * op.n[2] * ((uint64_t)op.n[8] << s.shift) >= kPgLarge ? 8 : 4;
+    f.queries = scratch && rep > 4 && !f.wide && (uint64_t)op.n[0] * op.n[2] * ((uint64_t)op.n[8] << s.shift) >= kPgLarge ? 8 : 4;
+    f.one = !scratch || pg_one(op.n[0] * op.n[2] * ((rep + 3) / 4), (uint64_t)op.n[8] << s.shift);
     f.tokens = op.n[0] > slots ? std::max(1u, f.queries / rep) : 1;
     return f;
 }
@@ -646,18 +679,19 @@ bool zg_launch_paged_attention(const ZgOp& op, float* const* bufs, const size_t*
     a.dst = bufs[s.buf[0]] + s.off[1]; a.q = bufs[s.buf[1]] + s.off[0]; a.table = bufs[s.buf[4]];
     a.sink = s.buf[5] == ZG_NO_BUF ? nullptr : a.sink_bf16 ? (const void*)wptr<bf16>(bufs, s.buf[5], s.off[2]) : (const void*)wptr<float>(bufs, s.buf[5], s.off[2]);
     a.scale = s.f[0]; a.cap = s.f[1];
-    const PgForm f = pg_form(s, a.pool.slots);
+    const PgForm f = pg_form(s, a.pool.slots, scratch != nullptr);
     a.chunks = (a.rep + f.queries - 1) / f.queries;
     a.tokens = f.tokens;
     a.plan = reinterpret_cast<uint32_t*>(scratch);
-    a.part = scratch ? scratch + pg_plan_elems(a.B) : nullptr;
+    a.part = f.one ? nullptr : scratch + pg_plan_elems(a.B);
     bool ok;
-    if (f.narrow) ok = f.queries == 4 ? pg_launch<2, 4, 1>(a, st) : pg_launch<2, 4, 2>(a, st);
-    else if (!f.wide) ok = f.queries == 4 ? pg_launch<4, 8, 1>(a, st) : pg_launch<4, 8, 2>(a, st);
-    else ok = pg_launch<8, 16, 1>(a, st);
+    if (f.one) ok = f.narrow ? pg_launch<2, 4, 1, 8>(a, st) : f.wide ? pg_launch<8, 16, 1, 8>(a, st) : pg_launch<4, 8, 1, 8>(a, st);
+    else if (f.narrow) ok = f.queries == 4 ? pg_launch<2, 4, 1, 1>(a, st) : pg_launch<2, 4, 2, 1>(a, st);
+    else if (!f.wide) ok = f.queries == 4 ? pg_launch<4, 8, 1, 1>(a, st) : pg_launch<4, 8, 2, 1>(a, st);
+    else ok = pg_launch<8, 16, 1, 1>(a, st);
     if (!ok) return false;
     ZG_SEQ_CHECK();
-    if (a.part) {
+    if (!f.one) {
         // Four warps a query where few sequences and heads are shared out over all warps, so that each has a dozen records or more.
         const uint32_t products = a.s.G * a.chunks * f.queries;
         if ((uint64_t)a.B * a.s.G * a.chunks <= zg_sm_count()) launch_pdl(k_paged_join<true>, dim3(products, a.B), dim3(128), 0, st, a, f.queries);

@@ -104,6 +104,37 @@ def test_logits_far_apart_and_near(cuda_backend, kind):
     p.close()
 
 
+@pytest.mark.parametrize("B,V", [(3, 6000), (3, 9000), (40, 9000), (200, 6000), (300, 2500), (70, 40000), (160, 66000), (130, 70001)])
+def test_rows_that_fill_the_gpu(cuda_backend, B, V):
+    """Rows by fewer CTAs each, and rows that are read again."""
+    r = np.random.default_rng(B + V)
+    p = program(cuda_backend, B, V)
+    choices = [CHOICES[i % len(CHOICES)] for i in range(B)]
+    check(p, ((1 + 2 * (np.arange(B)[:, None] % 2)) * r.standard_normal((B, V))).astype(np.float32), choices, r.random(B))
+    p.close()
+
+
+@pytest.mark.parametrize("V", [300, 9000])
+def test_least_share_of_logits_near_zero(cuda_backend, V):
+    """The largest logit over the temperature is all but -ln(min_p): what is let through ends within a range of tiny numbers of either sign, most of which are one exponent in 64 bits."""
+    T = np.arange(1 << 22, 1 << 23, dtype=np.float64)
+    M = np.round(T * np.log(2.0))
+    gap = M / T - np.log(2.0)
+    r = np.random.default_rng(V)
+    p = program(cuda_backend, 8, V)
+    logits, choices = np.empty((8, V), np.float32), []
+    for i in range(8):
+        near = np.where((np.abs(gap) > 1e-13 * (1 + i)) & ((gap > 0) == (i % 2 == 0)), np.abs(gap), 1)
+        at = near.argmin()
+        end = gap[at] * T[at]                          # what is let through ends here
+        logits[i] = end * (1 + r.uniform(0.05, 3, V) * r.choice([-1, 1], V)) * 10.0 ** r.choice([0, 0, -20, -38], V)
+        logits[i] = np.where(np.abs(logits[i] - end) < 0.04 * abs(end), 0, logits[i])
+        logits[i, V // 2] = M[at]
+        choices.append((T[at], 0, 1.0, 0.5))
+    check(p, logits, choices, r.random(8))
+    p.close()
+
+
 def test_many_draws(cuda_backend):
     """One distribution, 2000 random numbers: the shares of the tokens are their probabilities."""
     r = np.random.default_rng(9)

@@ -10,7 +10,7 @@ struct SmArgs {
     int32_t* dst; const float* logits; const float* table; float* probability;
     uint32_t B, V, rs, slice, vec;
 };
-constexpr uint32_t kSmBins = 1024, kSmList = 1024, kSmCluster = 8, kSmSlice = 40960;
+constexpr uint32_t kSmBins = 1024, kSmList = 1024, kSmCluster = 8, kSmSlice = 40960, kSmHalf = 16384;      // tokens of a slice at most; those that leave room for another CTA
 constexpr uint32_t kSmIndexBits = 20, kSmIndexMask = (1u << kSmIndexBits) - 1;
 constexpr double kSmOne = 8796093022208.0;                           // 2^43: the largest weight
 typedef unsigned long long u64;
@@ -48,7 +48,7 @@ __device__ __forceinline__ u64 warp_sum64(u64 v) {
 }
 
 // Weights round(2^43 e^x) of exponents x <= 0: 2^(k / 32) of a table times the exponential's series up to r^5, |r| <= ln 2 / 64, whose next term is below 2^-48 (reduction by a table:
-// P. Tang, ACM Transactions on Mathematical Software 15, 1989).  Whole numbers are taken from the mantissa of sums with 2^52 and 1.5 * 2^52: conversions of 64 bits are slow.
+// P. Tang, ACM Transactions on Mathematical Software 15, 1989).  Whole numbers are taken from the mantissa of sums with 2^52 and 1.5 * 2^52.
 constexpr double kSmShift = 6755399441055744.0, kSmSteps = 46.166241308446828384;      // 1.5 * 2^52; 32 / ln 2
 // t: the exponent in 32nds of a power of two, -3000 at least; *k: t rounded.  table: 2^(43 + i / 32)
 __device__ __forceinline__ u64 sm_weight(double t, const double* table, int* k) {
@@ -62,8 +62,8 @@ __device__ __forceinline__ u64 sm_weight(double t, const double* table, int* k) 
     return (u64)__double_as_longlong(w) & 0xfffffffffffffull;
 }
 
-// A cluster per row, its CTAs each a slice of the vocabulary: kept in shared memory (KEEP), or read again, from L2, where the rows fill the GPU more than once (with 64 rows of 128256 tokens
-// all logits would take all of its shared memory).  Tokens are counted by bins of logits below the largest, 1 / 32 of a power of two wide; what top_k or top_p cuts off begins in the bin in which
+// A cluster of C CTAs per row, each a slice of the vocabulary: kept in shared memory (KEEP), or, where the rows fill the GPU several times, read again from L2 by smaller CTAs of which more are
+// resident.  Tokens are counted by bins of logits below the largest, 1 / 32 of a power of two wide; what top_k or top_p cuts off begins in the bin in which
 // the counts (sums of weights) reach their target.  Where at most kSmList tokens lie in the bins up to there, one CTA gets them all and ranks them one against the other; otherwise
 // the bin is looked at more closely until at most kSmList candidates are left in it, of which each CTA ranks its own.  Weights are whole multiples of 2^-43 of the largest, their sums exact in 64 bits, so that
 // no order of additions changes a choice.
@@ -165,10 +165,20 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 2 : 4) k_sample(const
         const double least = log((double)min_p);
         uint32_t key = sm_key((float)((double)M + least * (double)T));
         const uint32_t most = (uint32_t)(best >> kSmIndexBits);
-        key = min(key, most);
-        while (key < most && !(exponent(sm_value(key)) >= least)) key++;
-        while (key > 0x00800000u && exponent(sm_value(key - 1)) >= least) key--;
-        least_x = sm_value(key);
+        // from there in growing steps to one on the other side, then by halves between them
+        auto through = [&](uint32_t k) { return exponent(sm_value(k)) >= least; };
+        uint32_t in = most, out = 0x007fffffu;                       // the largest logit is let through, -inf is not
+        key = min(max(key, out + 1), most);
+        const bool down = through(key);
+        (down ? in : out) = key;
+        for (uint32_t step = 1; in - out > step; step *= 2) {
+            const uint32_t k = down ? in - step : out + step;
+            const bool t = through(k);
+            (t ? in : out) = k;
+            if (t != down) break;
+        }
+        while (in - out > 1) { const uint32_t k = out + (in - out) / 2; if (through(k)) in = k; else out = k; }
+        least_x = sm_value(in);
     }
     auto draw = [&](float x, uint32_t index, u64 all) {
         a.dst[r] = (int32_t)index;
@@ -287,7 +297,7 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 2 : 4) k_sample(const
                 for (uint32_t e = 0; e < 4; e++) if (e < valid && b[e] <= first_bin) give(x[e], i + e);
             });
             __syncthreads();
-            // (one addition to the first CTA's number for a CTA's candidates: a thousand of them one by one took 20 us)
+            // one addition to the first CTA's number for a CTA's candidates
             if (tid == 0) {
                 uint32_t begin;
                 asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(begin) : "r"(sm_at(&sh.n_all, 0)), "r"(*n_list) : "memory");
@@ -301,7 +311,8 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 2 : 4) k_sample(const
             cluster_sync();                                          // (before that no CTA leaves: its bins are read)
             if (rank != 0) return;
             const uint32_t count = sh.n_all;
-            // In falling order of x (the order of the logits; then that of falling numbers, in which indices rise): placed by buckets, which rise as x falls, then ranked in their bucket.
+            // In falling order of x (the order of the logits; then that of falling numbers, in which indices rise): placed by buckets, which rise as x falls, then ranked in their bucket (64 rows
+            // with a thousand candidates: 54 us, each ranked among all of them 129).
             auto sort = [&](auto&& bucket) {
                 for (uint32_t i = tid; i < kSmBins; i += T_) sh.count[i] = 0;
                 __syncthreads();
@@ -550,10 +561,17 @@ bool zg_launch_sample(const ZgOp& op, float* const* bufs, cudaStream_t st) {
     a.probability = s.buf[3] == ZG_NO_BUF ? nullptr : bufs[s.buf[3]] + s.off[2];
     a.B = s.n[0]; a.V = s.n[1]; a.rs = s.n[2];
     a.vec = a.rs % 4 == 0 && (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0;
-    const uint32_t C = a.V <= 1024 ? 1 : kSmCluster;
-    a.slice = ((a.V + C - 1) / C + 3) / 4 * 4;
-    const bool keep = C == 1 || a.B * C <= 2 * zg_sm_count();
-    if (!(C == 1 ? sm_launch<1, true>(a, st) : keep ? sm_launch<kSmCluster, true>(a, st) : sm_launch<kSmCluster, false>(a, st))) return false;
+    // CTAs of a row: eight, fewer where a slice would be small (one row of 4096 tokens, us, by 1 / 8 CTAs: 10.3 / 12.3), or where the rows fill the SMs, two CTAs each, without, and their slices
+    // leave room for two (256 rows of 32000 tokens by 2 / 4 / 8 CTAs: 53.0 / 66.7 / 106.6; 64 rows: 30.8 / 26.7 / 36.9; 64 rows of 65536: 49.2 / 35.3 / 45.7).
+    const uint32_t sms = zg_sm_count();
+    auto slice = [&](uint32_t C) { return ((a.V + C - 1) / C + 3) / 4 * 4; };
+    uint32_t C = kSmCluster;
+    while (C > 1 && (slice(C) <= 2048 || ((uint64_t)a.B * C > 2 * sms && slice(C / 2) <= kSmHalf))) C /= 2;
+    a.slice = slice(C);
+    // Slices are kept up to three waves of CTAs (128256 tokens, us, kept / read again: 1 row 20.5 / 29.7, 32 rows 49.2 / 81.9, 64 63.9 / 87.1, 96 85.1 / 99.2, 128 107 / 103, 512 405 / 339;
+    // 200000 tokens: 32 rows 65.6 / 86.1, 64 112 / 102).
+    const bool keep = C < kSmCluster || (uint64_t)a.B * C <= 3 * sms * (a.slice <= kSmHalf ? 2 : 1);
+    if (!(C == 1 ? sm_launch<1, true>(a, st) : C == 2 ? sm_launch<2, true>(a, st) : C == 4 ? sm_launch<4, true>(a, st) : keep ? sm_launch<kSmCluster, true>(a, st) : sm_launch<kSmCluster, false>(a, st))) return false;
     ZG_SEQ_CHECK();
     return true;
 }

@@ -7,7 +7,7 @@
 namespace {
 
 // ── PAGE_APPEND ──────────────────────────────────────────────────────────────────────────────────────────────────────
-constexpr uint32_t kPaThreads = 256, kPaPairs = 128, kPaRows = 16, kPaTurns = 4;      // pairs of a head; rows a CTA at most; tokens of a page that are few
+constexpr uint32_t kPaThreads = 256, kPaPairs = 128, kPaRows = 16, kPaTurns = 4;      // pairs of a head; rows a CTA at most; tokens of a page whose turns are kept, and behind a page's first one that make it many
 struct PaArgs {
     PagePool pool; PageShape s;
     uint8_t* pages; const float* src; const float* table; float* turned; const float* freqs;
@@ -159,7 +159,7 @@ __device__ void pa_few(const PaArgs& a, const BatchHead& head, uint8_t* page, co
     }
 }
 // The same of many, for one head and a whole CTA.  Keys go to shared memory as they are turned; values are read again when their scale is known (with both in shared memory fewer CTAs
-// are resident: 85 us instead of 56 for 2048 tokens of 8 heads of 128).
+// are resident: 1.5 times the time for 2048 tokens of 8 heads of 128).
 __device__ void pa_many(const PaArgs& a, const BatchHead& head, uint8_t* part, uint32_t g, const int32_t* joined, const uint32_t* list, uint32_t n, uint32_t begin, float* tile) {
     __shared__ uint32_t most[2];
     const PageShape& s = a.s;
@@ -228,7 +228,8 @@ __device__ void pa_many(const PaArgs& a, const BatchHead& head, uint8_t* part, u
             }
 }
 // Row r's page, where r is the first of the step's rows that join it: it finds the others in the table (the last of several at one place counts), and no other CTA touches the
-// page's part of a head, so no order of CTAs changes anything.  Where the rows behind r join it too, as a prompt's do, each head has a CTA (y); else the first CTA takes them all.
+// page's part of a head, so no order of CTAs changes anything.  Where the four rows behind r join it too, as a prompt's do, each head has a CTA (y); else the first CTA takes them
+// all, a warp a head, and makes each turn once (8 heads of 128, us, a CTA a head / one: 64 sequences of 8 tokens 24.6 / 35.9, 4 of 512 44.8 / 53.7; of one token 17.2 / 14.4; 128 of 2 27.3 / 22.1).
 __device__ void pa_keys(const PaArgs& a, const BatchHead& head, uint32_t r, uint32_t y, float* mem) {
     __shared__ int32_t joined[64];                                   // row that brings token t of the page, or -1
     __shared__ uint32_t list[64];                                    // tokens that come, in order
@@ -297,7 +298,7 @@ struct PrArgs {
 };
 constexpr uint32_t kPrThreads = 256, kPrRows = 16;
 // CTA (16 rows, key head): bound by its writes.  The rows' pages are found once.  Keys are read four codes at a time; values, of which a tile holds sixteen tokens side by side, a tile at a
-// time for all rows whose tokens it holds (byte by byte for each row 11.5 us instead of 7 for 2186 rows of 8 heads of 128: every byte came from a line of its own).
+// time for all rows whose tokens it holds (byte by byte for each row 11.5 us instead of 10 for 2186 rows of 8 heads of 128: every byte came from a line of its own).
 __global__ void __launch_bounds__(kPrThreads) k_page_read(const PrArgs a) {
     pdl_enter();
     __shared__ const uint8_t* parts[kPrRows];                        // null: zeros, or nothing (tokens: -1), or no numbers (-2)
@@ -377,7 +378,8 @@ __global__ void __launch_bounds__(kPrThreads) k_page_read(const PrArgs a) {
 
 // ── PAGE_COPY ────────────────────────────────────────────────────────────────────────────────────────────────────────
 constexpr uint32_t kPcThreads = 256, kPcVectors = 4;                 // vectors of 16 bytes a thread
-// CTA (move, share of the page): bound by the reads and writes.  VEC: pages of whole vectors
+// CTA (move, share of the page): bound by the reads and writes, 6.5 TB/s of them where 4079 pages of 33 KB are moved (with one vector a thread 53.3 us, with four 47.1, with eight 49.2).  V: vectors of 16
+// bytes, or words where a page is no whole number of vectors.
 template <typename V>
 __global__ void __launch_bounds__(kPcThreads) k_page_copy(V* pages, const float* table, uint32_t B, uint32_t count, uint32_t vectors) {
     pdl_enter();
@@ -448,9 +450,11 @@ bool zg_launch_page_op(const ZgOp& op, float* const* bufs, const size_t* elems, 
             a.turned = a.q_heads ? bufs[s.buf[5]] + s.off[3] : nullptr;
             a.freqs = a.rot && s.buf[4] != ZG_NO_BUF ? bufs[s.buf[4]] + s.off[4] : nullptr;
             if (!a.freqs) for (uint32_t i = 0; i < a.rot / 2; i++) a.freq[i] = std::pow((double)s.f[0], -2.0 * i / a.rot);
-            // More rows a CTA where there are many, of which a prompt's mostly join the page of the row before them.
+            // More rows a CTA where there are many, of which a prompt's mostly join the page of the row before them (2048 rows, 32 / 8 heads of 128, us, with one row a CTA and with four: 59.4 / 44.8;
+            // 8192 rows, with one and with sixteen: 219 / 146).  Query heads in smaller parts where there are few rows (with 1024 / 4096 values: 64 rows 14.4 / 16.4, 128 17.1 / 18.3, 256 of pairs
+            // 20.7 / 22.1; 512 26.7 / 24.6, 2048 51.0 / 44.7).
             a.rows = std::min(kPaRows, (a.B + 511) / 512);
-            const uint32_t heads = std::max(1u, a.B <= 64 ? 1024 / a.s.dk : 4096 / a.s.dk), parts = (a.q_heads + heads - 1) / heads;
+            const uint32_t heads = std::max(1u, a.B <= 256 ? 1024 / a.s.dk : 4096 / a.s.dk), parts = (a.q_heads + heads - 1) / heads;
             a.part = heads * a.s.dk;
             a.vec = a.q_heads && a.s.dk % 4 == 0 && a.turn_at % 4 == 0 && a.rot % 8 == 0 && a.src_rs % 4 == 0 && a.q_col % 4 == 0 && a.dst_rs % 4 == 0 && s.off[3] % 4 == 0;
             const size_t smem = std::max<size_t>({sizeof(float) * std::min(a.s.page, a.B) * a.s.dk, sizeof(double2) * std::max(a.rows, std::min(kPaTurns, a.B)) * (a.rot / 2)});

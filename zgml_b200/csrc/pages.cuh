@@ -1,7 +1,7 @@
 // Pages of a cache in 8 bits (PAGE_APPEND, PAGED_ATTENTION, PAGE_READ, PAGE_COPY; layout in include/zgml_cuda.h) as the kernels address them.
 // A page holds `page` tokens (16, 32 or 64) of every key head, a head after the other: two scales and two words beside them, then keys, then values.  A value is a code, a whole
-// number of -127 to 127, times its scale, a power of two; stored is code + 128, which as the low bits of a half-precision 1024 + x needs no sign extension.  Keys lie in tiles of 8 tokens by 32
-// values and values in tiles of 16 tokens by 16 values, so that the 8 bytes at 8 * lane of a tile are what lane `lane` of a warp holds of two matrix-product operands
+// number of -127 to 127, times its scale, a power of two; stored is code + 128.  Keys lie in tiles of 8 tokens by 32
+// values and values in tiles of 16 tokens by 16 values, so that the 8 bytes at 8 * lane of a tile are what lane `lane` of a warp holds of a matrix product's operand
 // (of keys: token lane / 4, eight values from 8 (lane % 4) on; of values: tokens t, t + 1, t + 8, t + 9 with t = 2 (lane % 4) of values lane / 4 and lane / 4 + 8).
 #pragma once
 #include "batch_table.cuh"

@@ -19,8 +19,8 @@ struct SmShared {
     alignas(16) uint32_t mass_low[kSmBins], mass_high[kSmBins], count[kSmBins];      // (sums of 64 bits by words: additions of 64 bits to shared memory are loops)
     ulonglong2 list[kSmList], all_list[kSmList];                     // {order, weight} of candidates, own and of the cluster
     double table[32];                                                // 2^(43 + i / 32)
-    u64 best, total, warp_mass[32], found_mass, threshold, found_target;
-    uint32_t n_list[2], n_all, found_count, found_bin, warp_count[32];
+    u64 best, total, warp_mass[32], group_mass[32], found_mass, threshold, found_target;
+    uint32_t n_list[2], n_all, n_picked, span[2], found_count, found_bin, found_upto, warp_count[32], group_count[32];      // groups of 32 bins
 };
 __device__ __forceinline__ uint32_t sm_at(const void* p, uint32_t rank) {
     uint32_t at;
@@ -187,6 +187,28 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 2 : 4) k_sample(const
     const bool by_k = top_k != 0 && (uint32_t)top_k < a.V, by_p = top_p < 1.0f;
     u64 threshold = 0;
     // counts (and sums of weights) of the tokens in [lo, hi] by their bins: of equal width below the largest logit, or of the order's numbers
+    auto add_mass = [&](uint32_t b, u64 w) {
+        const uint32_t low = (uint32_t)w;
+        if (w) {
+            const uint32_t old = atomicAdd(&sh.mass_low[b], low), high = (uint32_t)(w >> 32) + (old + low < old);
+            if (high) atomicAdd(&sh.mass_high[b], high);
+        }
+        atomicAdd(&sh.count[b], 1u);
+    };
+    // sums of groups of 32 bins, the masses' by 16 bits and 32
+    auto group_sums = [&](bool masses) {
+#pragma unroll
+        for (uint32_t g = warp; g < kSmBins / 32; g += kWarps) {
+            const uint32_t tokens = __reduce_add_sync(0xffffffffu, sh.count[32 * g + lane]);
+            u64 mass = 0;
+            if (masses) {
+                const uint32_t low = sh.mass_low[32 * g + lane];
+                mass = ((u64)__reduce_add_sync(0xffffffffu, sh.mass_high[32 * g + lane]) << 32) + ((u64)__reduce_add_sync(0xffffffffu, low >> 16) << 16) + __reduce_add_sync(0xffffffffu, low & 0xffffu);
+            }
+            if (lane == 0) { sh.group_count[g] = tokens; sh.group_mass[g] = mass; }
+        }
+    };
+    auto within = [&](float x, u64 lo, u64 hi) { return x >= sm_value(max((uint32_t)(lo >> kSmIndexBits), 0x007fffffu)) && x <= sm_value((uint32_t)(hi >> kSmIndexBits)); };
     auto count_bins = [&](u64 lo, u64 hi, bool linear, uint32_t shift, bool masses) {
         if (masses && lo == 0 && linear)                             // (of all tokens: those with weights go four at a time)
             fours(0, n, tid, T_, [&](const float (&x)[4], uint32_t, uint32_t valid) {
@@ -197,9 +219,7 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 2 : 4) k_sample(const
 #pragma unroll
                 for (uint32_t e = 0; e < 4; e++) {
                     if (e >= valid) break;
-                    const uint32_t b = min((uint32_t)-k[e], kSmBins - 1), low = (uint32_t)w[e], old = atomicAdd(&sh.mass_low[b], low), high = (uint32_t)(w[e] >> 32) + (old + low < old);
-                    if (high) atomicAdd(&sh.mass_high[b], high);
-                    atomicAdd(&sh.count[b], 1u);
+                    add_mass(min((uint32_t)-k[e], kSmBins - 1), w[e]);
                 }
             });
         else if (lo == 0 && linear)
@@ -212,80 +232,69 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 2 : 4) k_sample(const
             });
         else
             each(0, n, tid, T_, [&](float x, uint32_t i) {
+                if (!within(x, lo, hi)) return;
                 const u64 o = sm_order(x, v0 + i);
                 if (o < lo || o > hi) return;
                 int k = 0;
                 const u64 w = masses ? sm_weight(in_steps(x), sh.table, &k) : 0;
-                const uint32_t b = linear ? bin_of(x) : (uint32_t)((hi - o) >> shift), low = (uint32_t)w;
-                if (masses) {
-                    const uint32_t old = atomicAdd(&sh.mass_low[b], low), high = (uint32_t)(w >> 32) + (old + low < old);
-                    if (high) atomicAdd(&sh.mass_high[b], high);
-                }
-                atomicAdd(&sh.count[b], 1u);
+                add_mass(linear ? bin_of(x) : (uint32_t)((hi - o) >> shift), w);
             });
         __syncthreads();
+        group_sums(masses);
         cluster_sync();
     };
-    // Of the cluster's bins: the one in which `target` is reached (with `share_of` >= 0: target = share_of of the sum), how many tokens it has, what comes before it and the tokens up to its end.
-    auto find_bin = [&](bool masses, u64 target, double share_of, u64 above, uint32_t* upto) {
-        typedef typename std::conditional<kBinsEach == 4, uint4, uint2>::type Bins;
-        u64 mine[kBinsEach] = {};
-        uint32_t here[kBinsEach] = {}, tokens = 0;
-        u64 sum = 0;
-        auto add = [&](const uint32_t* bins, auto&& take) {
-            Bins x[C];
+    // Of the bins of N CTAs: the one in which `target` is reached (with `share_of` >= 0: target = share_of of the sum), how many tokens it has, what comes before it and the tokens up to its end.  One
+    // warp looks for the group, then in the group (with all bins of eight CTAs read by all threads 4 us instead of 1.5).
+    auto find_bin = [&](auto ctas, bool masses, u64 target, double share_of, u64 above) {
+        constexpr uint32_t N = decltype(ctas)::value;
+        if (warp == 0) {
+            auto peer = [&](const auto* p, uint32_t c) { return N == 1 ? p : sm_peer(p, c); };
+            uint32_t tokens[2] = {0, 0}, tokens_before = 0;
+            u64 mass[2] = {0, 0}, before = above;
+            uint32_t at = lane;                                      // group, then bin
 #pragma unroll
-            for (uint32_t c = 0; c < C; c++) x[c] = *reinterpret_cast<const Bins*>(sm_peer(bins, c) + kBinsEach * tid);
+            for (int level = 0; level < 2; level++) {
+                uint32_t t[N], low[N], high[N];
 #pragma unroll
-            for (uint32_t c = 0; c < C; c++)
+                for (uint32_t c = 0; c < N; c++) {
+                    t[c] = *(level ? peer(&sh.count[at], c) : peer(&sh.group_count[at], c));
+                    if (!masses) low[c] = high[c] = 0;
+                    else if (level) { low[c] = *peer(&sh.mass_low[at], c); high[c] = *peer(&sh.mass_high[at], c); }
+                    else { const u64 m = *peer(&sh.group_mass[at], c); low[c] = (uint32_t)m; high[c] = (uint32_t)(m >> 32); }
+                }
 #pragma unroll
-                for (uint32_t k = 0; k < kBinsEach; k++) take(k, reinterpret_cast<const uint32_t*>(&x[c])[k]);
-        };
-        add(sh.count, [&](uint32_t k, uint32_t v) { here[k] += v; });
-        if (masses) {
-            add(sh.mass_low, [&](uint32_t k, uint32_t v) { mine[k] += v; });
-            add(sh.mass_high, [&](uint32_t k, uint32_t v) { mine[k] += (u64)v << 32; });
-        }
+                for (uint32_t c = 0; c < N; c++) { tokens[level] += t[c]; mass[level] += masses ? (u64)high[c] << 32 | low[c] : t[c]; }
+                uint32_t upto = tokens[level];
+                u64 sum = mass[level];
 #pragma unroll
-        for (uint32_t k = 0; k < kBinsEach; k++) {
-            if (!masses) mine[k] = here[k];
-            tokens += here[k]; sum += mine[k];
-        }
-        u64 before = sum;
-        uint32_t tokens_before = tokens;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const u64 t = __shfl_up_sync(0xffffffffu, before, o);
-            const uint32_t q = __shfl_up_sync(0xffffffffu, tokens_before, o);
-            if (lane >= (uint32_t)o) { before += t; tokens_before += q; }
-        }
-        if (lane == 31) { sh.warp_mass[warp] = before; sh.warp_count[warp] = tokens_before; }
-        __syncthreads();
-        u64 all = 0;
-#pragma unroll
-        for (uint32_t i = 0; i < kWarps; i++) {
-            if (i < warp) { before += sh.warp_mass[i]; tokens_before += sh.warp_count[i]; }
-            all += sh.warp_mass[i];
-        }
-        if (share_of >= 0.0) target = max((u64)1, (u64)ceil(share_of * (double)all));
-        before += above - sum;
-        tokens_before -= tokens;
-#pragma unroll
-        for (uint32_t k = 0; k < kBinsEach; k++) {
-            tokens_before += here[k];
-            if (before < target && before + mine[k] >= target) { sh.found_bin = kBinsEach * tid + k; sh.found_count = here[k]; sh.found_mass = before; sh.n_list[0] = tokens_before; sh.found_target = target; }
-            before += mine[k];
+                for (int o = 1; o < 32; o <<= 1) {
+                    const u64 m = __shfl_up_sync(0xffffffffu, sum, o);
+                    const uint32_t q = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= (uint32_t)o) { sum += m; upto += q; }
+                }
+                if (level == 0 && share_of >= 0.0) target = max((u64)1, (u64)ceil(share_of * (double)__shfl_sync(0xffffffffu, sum, 31)));
+                before += sum - mass[level];
+                tokens_before += upto - tokens[level];
+                const bool here = before < target && before + mass[level] >= target;
+                if (level) {
+                    if (here) { sh.found_bin = at; sh.found_count = tokens[1]; sh.found_mass = before; sh.found_upto = tokens_before + tokens[1]; sh.found_target = target; }
+                } else {
+                    const int group = max(__ffs(__ballot_sync(0xffffffffu, here)) - 1, 0);
+                    before = __shfl_sync(0xffffffffu, before, group);
+                    tokens_before = __shfl_sync(0xffffffffu, tokens_before, group);
+                    at = 32 * group + lane;
+                }
+            }
         }
         __syncthreads();
-        *upto = sh.n_list[0];
         return sh.found_target;
     };
+    const std::integral_constant<uint32_t, C> cluster;
     if (by_k || by_p) {
-        uint32_t upto;
         count_bins(0, best, true, 0, !by_k);
-        u64 target = find_bin(!by_k, top_k, by_k ? -1.0 : (double)top_p, 0, &upto);
+        u64 target = find_bin(cluster, !by_k, top_k, by_k ? -1.0 : (double)top_p, 0);
         const uint32_t first_bin = sh.found_bin;
-        if (upto <= kSmList) {
+        if (sh.found_upto <= kSmList) {
             // few: they go to the first CTA
             uint32_t* const n_list = &sh.n_list[1];
             auto give = [&](float x, uint32_t i) { sh.list[atomicAdd(n_list, 1u)] = make_ulonglong2(sm_order(x, v0 + i), weight(x)); };
@@ -404,7 +413,7 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 2 : 4) k_sample(const
                     for (uint32_t i = tid; i < kSmBins; i += T_) sh.count[i] = sh.mass_low[i] = sh.mass_high[i] = 0;
                     __syncthreads();
                     count_bins(lo, hi, linear, shift, by_mass);
-                    target = find_bin(by_mass, by_mass ? target : (u64)top_k, by_mass && linear ? (double)top_p : -1.0, above, &upto);
+                    target = find_bin(cluster, by_mass, by_mass ? target : (u64)top_k, by_mass && linear ? (double)top_p : -1.0, above);
                 }
                 counted = false;
                 const uint32_t bin = sh.found_bin, count = sh.found_count;
@@ -434,37 +443,62 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 2 : 4) k_sample(const
                     continue;
                 }
                 uint32_t* const n_list = &sh.n_list[1];
-                each(0, n, tid, T_, [&](float x, uint32_t i) {
-                    if (linear && bin_of(x) != bin) return;
-                    const u64 o = sm_order(x, v0 + i);
-                    if (o < lo || o > hi || (!linear && (uint32_t)((hi - o) >> shift) != bin)) return;
-                    sh.list[atomicAdd(n_list, 1u)] = make_ulonglong2(o, by_mass ? weight(x) : 1);
+                if (tid == 0) *n_list = 0;
+                __syncthreads();
+                fours(0, n, tid, T_, [&](const float (&x)[4], uint32_t i, uint32_t valid) {
+                    bool in[4];
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; e++) in[e] = e < valid && within(x[e], lo, hi) && (!linear || bin_of(x[e]) == bin);
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; e++) {
+                        const u64 o = sm_order(x[e], v0 + i + e);
+                        if (in[e] && o >= lo && o <= hi && (linear || (uint32_t)((hi - o) >> shift) == bin)) sh.list[atomicAdd(n_list, 1u)] = make_ulonglong2(o, by_mass ? weight(x[e]) : 1);
+                    }
                 });
                 __syncthreads();
-                cluster_sync();
+                cluster_sync();                                      // (and peers have read the bins)
                 uint32_t ends[C];
 #pragma unroll
                 for (uint32_t c = 0; c < C; c++) ends[c] = *sm_peer(n_list, c);
 #pragma unroll
                 for (uint32_t c = 1; c < C; c++) ends[c] += ends[c - 1];
+                // Every CTA gets them all, and looks for the one in which the target is reached by bins of their own range, then among the few of one bin.
+                uint32_t top = 0, least = 0xffffffffu;
+                if (tid == 0) { sh.n_picked = 0; sh.span[0] = 0; sh.span[1] = 0xffffffffu; }
+                for (uint32_t i = tid; i < kSmBins; i += T_) sh.count[i] = sh.mass_low[i] = sh.mass_high[i] = 0;
                 for (uint32_t t = tid; t < count; t += T_) {
                     uint32_t c = 0, begin = 0;
 #pragma unroll
                     for (uint32_t k = 0; k + 1 < C; k++) if (t >= ends[k]) { c = k + 1; begin = ends[k]; }
-                    sh.all_list[t] = *sm_peer(&sh.list[t - begin], c);
+                    const ulonglong2 x = *sm_peer(&sh.list[t - begin], c);
+                    sh.all_list[t] = x;
+                    top = max(top, (uint32_t)(x.x >> kSmIndexBits)); least = min(least, (uint32_t)(x.x >> kSmIndexBits));
                 }
                 __syncthreads();
-                for (uint32_t t = warp; t < *n_list; t += kWarps) {
-                    const ulonglong2 me = sh.list[t];
+                top = __reduce_max_sync(0xffffffffu, top); least = __reduce_min_sync(0xffffffffu, least);
+                if (lane == 0) { atomicMax(&sh.span[0], top); atomicMin(&sh.span[1], least); }
+                __syncthreads();
+                const u64 last = (u64)sh.span[0] << kSmIndexBits | kSmIndexMask, first = (u64)sh.span[1] << kSmIndexBits;
+                uint32_t apart = 0;
+                while ((last - first) >> apart >= kSmBins) apart++;
+                for (uint32_t t = tid; t < count; t += T_) { const ulonglong2 x = sh.all_list[t]; add_mass((uint32_t)((last - x.x) >> apart), x.y); }
+                __syncthreads();
+                group_sums(true);
+                __syncthreads();
+                find_bin(std::integral_constant<uint32_t, 1>(), true, target, -1.0, above);
+                const uint32_t inner = sh.found_bin;
+                const u64 ahead_of = sh.found_mass;
+                for (uint32_t t = tid; t < count; t += T_) if ((uint32_t)((last - sh.all_list[t].x) >> apart) == inner) sh.count[atomicAdd(&sh.n_picked, 1u)] = t;
+                __syncthreads();
+                for (uint32_t t = warp; t < sh.n_picked; t += kWarps) {
+                    const ulonglong2 me = sh.all_list[sh.count[t]];
                     u64 ahead = 0;
-                    for (uint32_t i = lane; i < count; i += 32) { const ulonglong2 x = sh.all_list[i]; if (x.x > me.x) ahead += x.y; }
-                    ahead = above + warp_sum64(ahead);
-                    if (ahead < target && ahead + me.y >= target && lane < C) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(sm_at(&sh.threshold, lane)), "l"(me.x) : "memory");
+                    for (uint32_t i = lane; i < sh.n_picked; i += 32) { const ulonglong2 x = sh.all_list[sh.count[i]]; if (x.x > me.x) ahead += x.y; }
+                    ahead = ahead_of + warp_sum64(ahead);
+                    if (ahead < target && ahead + me.y >= target && lane == 0) sh.threshold = me.x;
                 }
                 __syncthreads();
-                cluster_sync();                                      // (and peers have read the list)
                 threshold = sh.threshold;
-                if (tid == 0) *n_list = 0;
                 break;
             }
         }

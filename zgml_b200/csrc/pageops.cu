@@ -7,11 +7,11 @@
 namespace {
 
 // ── PAGE_APPEND ──────────────────────────────────────────────────────────────────────────────────────────────────────
-constexpr uint32_t kPaThreads = 256, kPaPairs = 128, kPaRows = 16, kPaTurns = 4;      // pairs of a head; rows a CTA at most; tokens of a page whose turns are kept, and behind a page's first one that make it many
+constexpr uint32_t kPaThreads = 256, kPaPairs = 128, kPaRows = 16, kPaTurns = 4;      // pairs of a head; rows a CTA at most; tokens of a page whose turns are kept, and rows behind its first that make it many
 struct PaArgs {
     PagePool pool; PageShape s;
     uint8_t* pages; const float* src; const float* table; float* turned; const float* freqs;
-    uint32_t B, src_rs, k_col, v_col, q_col, q_heads, dst_rs, turn_at, rot, halves, rows, part, vec;      // rows a CTA, query values of one
+    uint32_t B, src_rs, k_col, v_col, q_col, q_heads, dst_rs, turn_at, rot, halves, rows, part, vec, key_rows, key_ctas, shares;      // rows of a CTA of queries, values of a row in it; rows of keys' CTAs, CTAs of those rows
     double freq[kPaPairs];                                           // base^(-2i / rot), where no table of frequencies is given
 };
 // Cosine and sine of a position's turn.  Everything up to the turned value is in 64 bits, and that is rounded once: a code is a turned value over its scale, rounded, and an
@@ -34,80 +34,84 @@ __device__ __forceinline__ float pa_scale(uint32_t bits) {
 }
 __device__ __forceinline__ uint32_t pa_code(float x, float inv) { return (uint32_t)(int)(rintf(x * inv) + 128.0f); }
 
-// Query heads of the CTA's rows: a part of their values.  Bound by reading and writing them.
+// Query heads of the CTA's rows: a part of their values.  Bound by reading and writing them; what is asked for of the rows comes for all at once.
 __device__ void pa_queries(const PaArgs& a, const BatchHead& head, uint32_t r0, uint32_t first, double2* turn) {
+    __shared__ int8_t states[kPaRows];                               // of a row: -1 idle, 0 out of range
     const PageShape& s = a.s;
     const uint32_t rows = min(a.rows, head.rows - r0), n = min(a.part, a.q_heads * s.dk - first), half = a.rot / 2;
+    if (threadIdx.x < rows) {
+        const BatchRow w = batch_row(a.table, r0 + threadIdx.x);
+        bool ok = page_row_ok(a.pool, s, w) && head.prefix >= 0;
+        ok = ok && (w.length == 0 || page_id(a.pool, w.slot, (w.length - 1) >> s.shift) >= 0);
+        states[threadIdx.x] = w.slot < 0 ? -1 : ok;
+    }
     for (uint32_t x = threadIdx.x; x < rows * half; x += kPaThreads) {
         const uint32_t m = x / half;
         const BatchRow w = batch_row(a.table, r0 + m);
         if (w.slot >= 0 && w.length >= 0 && head.prefix >= 0) turn[x] = pa_turn(a, (double)head.prefix + w.length - 1, x - m * half);
     }
     __syncthreads();
-    for (uint32_t m = 0; m < rows; m++) {
-        const BatchRow w = batch_row(a.table, r0 + m);
-        if (w.slot < 0) continue;
-        bool ok = page_row_ok(a.pool, s, w) && head.prefix >= 0;
-        ok = ok && (w.length == 0 || page_id(a.pool, w.slot, (w.length - 1) >> s.shift) >= 0);
+    const float4 lost = make_float4(kBatchNaN, kBatchNaN, kBatchNaN, kBatchNaN);
+    if (a.vec) {                                                     // four pairs, or four values that stay
+        const uint32_t quads = a.rot / 8, each = quads + (s.dk - a.rot) / 4, items = n / s.dk * each;
+#pragma unroll 2
+        for (uint32_t i = threadIdx.x; i < rows * items; i += kPaThreads) {
+            const uint32_t m = i / items, x = i - m * items, h = x / each, k = x - h * each;
+            const int state = states[m];
+            if (state < 0) continue;
+            const float* src = a.src + (size_t)(r0 + m) * a.src_rs + a.q_col + first;
+            float* dst = a.turned + (size_t)(r0 + m) * a.dst_rs + first;
+            uint32_t p = h * s.dk, q = p;
+            if (k < quads) { p += a.turn_at + (a.halves ? 4 * k : 8 * k); q = p + (a.halves ? half : 4); }
+            else { const uint32_t d = 4 * (k - quads); p += d < a.turn_at ? d : d + a.rot; }
+            float4 u = *reinterpret_cast<const float4*>(src + p);
+            if (k < quads) {
+                float4 v = *reinterpret_cast<const float4*>(src + q);
+                const double2* y = turn + m * half + 4 * k;
+                float2 z[4];
+                if (a.halves) { z[0] = pa_turned(u.x, v.x, y[0]); z[1] = pa_turned(u.y, v.y, y[1]); z[2] = pa_turned(u.z, v.z, y[2]); z[3] = pa_turned(u.w, v.w, y[3]); }
+                else { z[0] = pa_turned(u.x, u.y, y[0]); z[1] = pa_turned(u.z, u.w, y[1]); z[2] = pa_turned(v.x, v.y, y[2]); z[3] = pa_turned(v.z, v.w, y[3]); }
+                if (a.halves) { u = make_float4(z[0].x, z[1].x, z[2].x, z[3].x); v = make_float4(z[0].y, z[1].y, z[2].y, z[3].y); }
+                else { u = make_float4(z[0].x, z[0].y, z[1].x, z[1].y); v = make_float4(z[2].x, z[2].y, z[3].x, z[3].y); }
+                *reinterpret_cast<float4*>(dst + q) = state ? v : lost;
+            }
+            *reinterpret_cast<float4*>(dst + p) = state ? u : lost;
+        }
+        return;
+    }
+    for (uint32_t i = threadIdx.x; i < rows * n; i += kPaThreads) {
+        const uint32_t m = i / n, c = i - m * n, in = c % s.dk - a.turn_at;
+        const int state = states[m];
+        if (state < 0) continue;
         const float* src = a.src + (size_t)(r0 + m) * a.src_rs + a.q_col + first;
-        float* dst = a.turned + (size_t)(r0 + m) * a.dst_rs + first;
-        const double2* t = turn + m * half;
-        if (a.vec) {                                                 // four pairs, or four values that stay
-            const uint32_t quads = a.rot / 8, each = quads + (s.dk - a.rot) / 4;
-            for (uint32_t x = threadIdx.x; x < n / s.dk * each; x += kPaThreads) {
-                const uint32_t h = x / each, k = x - h * each;
-                uint32_t p = h * s.dk, q = p;
-                if (k < quads) { p += a.turn_at + (a.halves ? 4 * k : 8 * k); q = p + (a.halves ? half : 4); }
-                else { const uint32_t d = 4 * (k - quads); p += d < a.turn_at ? d : d + a.rot; }
-                float4 u = *reinterpret_cast<const float4*>(src + p);
-                if (k < quads) {
-                    float4 v = *reinterpret_cast<const float4*>(src + q);
-                    const double2* y = t + 4 * k;
-                    float2 z[4];
-                    if (a.halves) { z[0] = pa_turned(u.x, v.x, y[0]); z[1] = pa_turned(u.y, v.y, y[1]); z[2] = pa_turned(u.z, v.z, y[2]); z[3] = pa_turned(u.w, v.w, y[3]); }
-                    else { z[0] = pa_turned(u.x, u.y, y[0]); z[1] = pa_turned(u.z, u.w, y[1]); z[2] = pa_turned(v.x, v.y, y[2]); z[3] = pa_turned(v.z, v.w, y[3]); }
-                    if (a.halves) { u = make_float4(z[0].x, z[1].x, z[2].x, z[3].x); v = make_float4(z[0].y, z[1].y, z[2].y, z[3].y); }
-                    else { u = make_float4(z[0].x, z[0].y, z[1].x, z[1].y); v = make_float4(z[2].x, z[2].y, z[3].x, z[3].y); }
-                    *reinterpret_cast<float4*>(dst + q) = ok ? v : make_float4(kBatchNaN, kBatchNaN, kBatchNaN, kBatchNaN);
-                }
-                *reinterpret_cast<float4*>(dst + p) = ok ? u : make_float4(kBatchNaN, kBatchNaN, kBatchNaN, kBatchNaN);
-            }
-            continue;
+        float v = src[c];
+        if (in < a.rot) {
+            const bool second = a.halves ? in >= half : in & 1;
+            const float other = src[(int)c + (a.halves ? (second ? -(int)half : (int)half) : second ? -1 : 1)];
+            const float2 z = pa_turned(second ? other : v, second ? v : other, turn[m * half + (a.halves ? (second ? in - half : in) : in >> 1)]);
+            v = second ? z.y : z.x;
         }
-        for (uint32_t c = threadIdx.x; c < n; c += kPaThreads) {
-            const uint32_t in = c % s.dk - a.turn_at;
-            float v = src[c];
-            if (in < a.rot) {
-                const bool second = a.halves ? in >= half : in & 1;
-                const float other = src[(int)c + (a.halves ? (second ? -(int)half : (int)half) : second ? -1 : 1)];
-                const float2 z = pa_turned(second ? other : v, second ? v : other, t[a.halves ? (second ? in - half : in) : in >> 1]);
-                v = second ? z.y : z.x;
-            }
-            dst[c] = ok ? v : kBatchNaN;
-        }
+        a.turned[(size_t)(r0 + m) * a.dst_rs + first + c] = state ? v : kBatchNaN;
     }
 }
 
-// what the scales of a part become when values up to `most` (their bits) join it
-__device__ __forceinline__ float2 pa_after(float2 before, uint32_t keys, uint32_t values) {
-    const float x = pa_scale(keys), y = pa_scale(values);            // (a scale that is not a number stays until the page begins anew)
-    return make_float2(before.x != before.x ? before.x : x < before.x ? before.x : x, before.y != before.y ? before.y : y < before.y ? before.y : y);
+// what a scale becomes when values up to `most` (their bits) join it (one that is not a number stays until the page begins anew)
+__device__ __forceinline__ float pa_after(float before, uint32_t most) {
+    const float x = pa_scale(most);
+    return before != before || x < before ? before : x;
 }
-// a part's codes in multiples of larger scales
-__device__ __forceinline__ void pa_rescale(const PageShape& s, uint8_t* part, float2 before, float2 after, uint32_t first, uint32_t step) {
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const float ratio = i ? before.y / after.y : before.x / after.x;
-        if (!(ratio < 1.0f)) continue;
-        uint32_t* codes = reinterpret_cast<uint32_t*>(part + kPageHead + (i ? s.page * s.kp : 0));
+// codes of a part's keys or values in multiples of a larger scale
+__device__ __forceinline__ void pa_rescale(const PageShape& s, uint8_t* part, bool values, float before, float after, uint32_t first, uint32_t step) {
+    const float ratio = before / after;
+    if (!(ratio < 1.0f)) return;
+    uint32_t* codes = reinterpret_cast<uint32_t*>(part + kPageHead + (values ? s.page * s.kp : 0));
 #pragma unroll 4
-        for (uint32_t x = first; x < s.page * (i ? s.vp : s.kp) / 4; x += step) {
-            const uint32_t c = codes[x];
-            uint32_t o = 0;
+    for (uint32_t x = first; x < s.page * (values ? s.vp : s.kp) / 4; x += step) {
+        const uint32_t c = codes[x];
+        uint32_t o = 0;
 #pragma unroll
-            for (int b = 0; b < 32; b += 8) o |= pa_code((float)(c >> b & 255) - 128.0f, ratio) << b;
-            codes[x] = o;
-        }
+        for (int b = 0; b < 32; b += 8) o |= pa_code((float)(c >> b & 255) - 128.0f, ratio) << b;
+        codes[x] = o;
     }
 }
 // The tokens of one page that a step brings, for all heads: a warp a head, which reads them twice (for the scales, for the codes); turns are made once.
@@ -118,7 +122,7 @@ __device__ void pa_few(const PaArgs& a, const BatchHead& head, uint8_t* page, co
     __syncthreads();
     for (uint32_t g = threadIdx.x >> 5; g < s.G; g += kPaThreads / 32) {
         uint8_t* const part = page + (size_t)g * s.head;
-        float2 before = *reinterpret_cast<const float2*>(part), after;
+        float2 before = *reinterpret_cast<const float2*>(part);
         uint32_t most_k = 0, most_v = 0;
         float inv_k = 0.0f, inv_v = 0.0f;
         auto pass = [&](bool codes) {
@@ -150,87 +154,90 @@ __device__ void pa_few(const PaArgs& a, const BatchHead& head, uint8_t* page, co
         };
         pass(false);
         if (joined[0] >= 0) before = make_float2(0.0f, 0.0f);
-        after = pa_after(before, __reduce_max_sync(0xffffffffu, most_k), __reduce_max_sync(0xffffffffu, most_v));
-        if (joined[0] < 0) pa_rescale(s, part, before, after, lane, 32);
+        const float2 after = make_float2(pa_after(before.x, __reduce_max_sync(0xffffffffu, most_k)), pa_after(before.y, __reduce_max_sync(0xffffffffu, most_v)));
+        if (joined[0] < 0) { pa_rescale(s, part, false, before.x, after.x, lane, 32); pa_rescale(s, part, true, before.y, after.y, lane, 32); }
         __syncwarp();
         if (lane == 0) *reinterpret_cast<float2*>(part) = after;
         inv_k = 1.0f / after.x; inv_v = 1.0f / after.y;
         pass(true);
     }
 }
-// The same of many, for one head and a whole CTA.  Keys go to shared memory as they are turned; values are read again when their scale is known (with both in shared memory fewer CTAs
-// are resident: 1.5 times the time for 2048 tokens of 8 heads of 128).
-__device__ void pa_many(const PaArgs& a, const BatchHead& head, uint8_t* part, uint32_t g, const int32_t* joined, const uint32_t* list, uint32_t n, uint32_t begin, float* tile) {
-    __shared__ uint32_t most[2];
+// The same of many, for a head's keys or its values and a whole CTA.  Keys go to shared memory as they are turned; values are read again when their scale is known (with both in shared memory
+// fewer CTAs are resident: 1.5 times the time for 2048 tokens of 8 heads of 128).
+__device__ void pa_many(const PaArgs& a, const BatchHead& head, uint8_t* part, uint32_t g, bool values, const int32_t* joined, const uint32_t* list, uint32_t n, uint32_t begin, float* tile) {
+    __shared__ uint32_t most;
     const PageShape& s = a.s;
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, half = a.rot / 2;
-    if (tid < 2) most[tid] = 0;
-    float2 before = *reinterpret_cast<const float2*>(part);
-    uint32_t top[2] = {0, 0};
+    float* const scale = reinterpret_cast<float*>(part) + values;
+    float before = *scale;
+    uint32_t top = 0;
+    __syncthreads();                                                 // (another head's, or its keys, are done)
+    if (tid == 0) most = 0;
     for (uint32_t m = warp; m < n; m += kPaThreads / 32) {
         const uint32_t t = list[m];
         const float* const row = a.src + (size_t)joined[t] * a.src_rs;
-        const double position = (double)head.prefix + (begin + t);
+        if (values) {
 #pragma unroll 4
-        for (uint32_t c = lane; c < s.dv; c += 32) top[1] = max(top[1], __float_as_uint(fabsf(row[a.v_col + g * s.dv + c])));
+            for (uint32_t c = lane; c < s.dv; c += 32) top = max(top, __float_as_uint(fabsf(row[a.v_col + g * s.dv + c])));
+            continue;
+        }
+        const double position = (double)head.prefix + (begin + t);
         const float* const keys = row + a.k_col + g * s.dk;
 #pragma unroll 2
         for (uint32_t i = lane; i < half; i += 32) {
             const uint32_t p = a.turn_at + (a.halves ? i : 2 * i), q = p + (a.halves ? half : 1);
             const float2 y = pa_turned(keys[p], keys[q], pa_turn(a, position, i));
             tile[m * s.dk + p] = y.x; tile[m * s.dk + q] = y.y;
-            top[0] = max(top[0], max(__float_as_uint(fabsf(y.x)), __float_as_uint(fabsf(y.y))));
+            top = max(top, max(__float_as_uint(fabsf(y.x)), __float_as_uint(fabsf(y.y))));
         }
         for (uint32_t c = lane; c < s.dk - a.rot; c += 32) {
             const uint32_t d = c < a.turn_at ? c : c + a.rot;
             const float v = keys[d];
             tile[m * s.dk + d] = v;
-            top[0] = max(top[0], __float_as_uint(fabsf(v)));
+            top = max(top, __float_as_uint(fabsf(v)));
         }
     }
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-        top[i] = __reduce_max_sync(0xffffffffu, top[i]);
-        if (lane == 0) atomicMax(&most[i], top[i]);
-    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0) atomicMax(&most, top);
     __syncthreads();
-    if (joined[0] >= 0) before = make_float2(0.0f, 0.0f);
-    const float2 after = pa_after(before, most[0], most[1]);
-    if (joined[0] < 0) pa_rescale(s, part, before, after, tid, kPaThreads);
+    if (joined[0] >= 0) before = 0.0f;
+    const float after = pa_after(before, most), inv = 1.0f / after;
+    if (joined[0] < 0) pa_rescale(s, part, values, before, after, tid, kPaThreads);
     __syncthreads();
-    if (tid == 0) *reinterpret_cast<float2*>(part) = after;
-    const float inv_k = 1.0f / after.x, inv_v = 1.0f / after.y;
-    if (after.x == after.x)                                          // four values of a key at a time
+    if (tid == 0) *scale = after;
+    if (after != after) return;
+    if (!values) {                                                   // four values of a key at a time
         for (uint32_t m = warp; m < n; m += kPaThreads / 32)
             for (uint32_t c = 4 * lane; c < s.dk; c += 128) {
                 const float* from = tile + m * s.dk + c;
                 uint8_t* to = part + key_byte(s, list[m], c);
-                if (c + 4 <= s.dk) *reinterpret_cast<uint32_t*>(to) = pa_code(from[0], inv_k) | pa_code(from[1], inv_k) << 8 | pa_code(from[2], inv_k) << 16 | pa_code(from[3], inv_k) << 24;
-                else for (uint32_t k = 0; c + k < s.dk; k++) to[k] = (uint8_t)pa_code(from[k], inv_k);
+                if (c + 4 <= s.dk) *reinterpret_cast<uint32_t*>(to) = pa_code(from[0], inv) | pa_code(from[1], inv) << 8 | pa_code(from[2], inv) << 16 | pa_code(from[3], inv) << 24;
+                else for (uint32_t k = 0; c + k < s.dk; k++) to[k] = (uint8_t)pa_code(from[k], inv);
             }
-    if (after.y == after.y)                                          // one value of tokens t, t + 1, t + 8, t + 9 where all of them come, else byte by byte
-        for (uint32_t unit = 0; unit < s.page / 16; unit++)
+        return;
+    }
+    // one value of tokens t, t + 1, t + 8, t + 9 where all of them come, else byte by byte
+    for (uint32_t unit = 0; unit < s.page / 16; unit++)
 #pragma unroll 2
-            for (uint32_t y = tid; y < 4 * s.vp; y += kPaThreads) {
-                const uint32_t c = 16 * (y / 64) + 8 * (y & 1) + (y % 64) / 8, t = 16 * unit + 2 * ((y / 2) & 3);
-                const int32_t r0 = joined[t], r1 = joined[t + 1], r8 = joined[t + 8], r9 = joined[t + 9];
-                if (c >= s.dv || (r0 & r1 & r8 & r9) < 0) continue;      // (none of them)
-                uint8_t* to = part + value_byte(s, t, c);
-                auto code = [&](int32_t r) { return pa_code(a.src[(size_t)r * a.src_rs + a.v_col + g * s.dv + c], inv_v); };
-                if ((r0 | r1 | r8 | r9) >= 0) *reinterpret_cast<uint32_t*>(to) = code(r0) | code(r1) << 8 | code(r8) << 16 | code(r9) << 24;
-                else {
-                    if (r0 >= 0) to[0] = (uint8_t)code(r0);
-                    if (r1 >= 0) to[1] = (uint8_t)code(r1);
-                    if (r8 >= 0) to[2] = (uint8_t)code(r8);
-                    if (r9 >= 0) to[3] = (uint8_t)code(r9);
-                }
+        for (uint32_t y = tid; y < 4 * s.vp; y += kPaThreads) {
+            const uint32_t c = 16 * (y / 64) + 8 * (y & 1) + (y % 64) / 8, t = 16 * unit + 2 * ((y / 2) & 3);
+            const int32_t r0 = joined[t], r1 = joined[t + 1], r8 = joined[t + 8], r9 = joined[t + 9];
+            if (c >= s.dv || (r0 & r1 & r8 & r9) < 0) continue;      // (none of them)
+            uint8_t* to = part + value_byte(s, t, c);
+            auto code = [&](int32_t r) { return pa_code(a.src[(size_t)r * a.src_rs + a.v_col + g * s.dv + c], inv); };
+            if ((r0 | r1 | r8 | r9) >= 0) *reinterpret_cast<uint32_t*>(to) = code(r0) | code(r1) << 8 | code(r8) << 16 | code(r9) << 24;
+            else {
+                if (r0 >= 0) to[0] = (uint8_t)code(r0);
+                if (r1 >= 0) to[1] = (uint8_t)code(r1);
+                if (r8 >= 0) to[2] = (uint8_t)code(r8);
+                if (r9 >= 0) to[3] = (uint8_t)code(r9);
             }
+        }
 }
 // Row r's page, where r is the first of the step's rows that join it: it finds the others in the table (the last of several at one place counts), and no other CTA touches the
-// page's part of a head, so no order of CTAs changes anything.  Where the four rows behind r join it too, as a prompt's do, each head has a CTA (y); else the first CTA takes them
-// all, a warp a head, and makes each turn once (8 heads of 128, us, a CTA a head / one: 64 sequences of 8 tokens 24.6 / 35.9, 4 of 512 44.8 / 53.7; of one token 17.2 / 14.4; 128 of 2 27.3 / 22.1).
-__device__ void pa_keys(const PaArgs& a, const BatchHead& head, uint32_t r, uint32_t y, float* mem) {
+// page's part of a head, so no order of CTAs changes anything.
+__device__ void pa_keys(const PaArgs& a, const BatchHead& head, uint32_t r, bool many, uint32_t y, float* mem) {
     __shared__ int32_t joined[64];                                   // row that brings token t of the page, or -1
     __shared__ uint32_t list[64];                                    // tokens that come, in order
     __shared__ uint32_t count;
@@ -238,20 +245,16 @@ __device__ void pa_keys(const PaArgs& a, const BatchHead& head, uint32_t r, uint
     const PageShape& s = a.s;
     const BatchRow w = batch_row(a.table, r);
     const uint32_t place = (uint32_t)w.length - 1;
-    auto joins = [&](const BatchRow& z) { return z.slot == w.slot && z.length > 0 && (uint32_t)(z.length - 1) >> s.shift == place >> s.shift; };
-    const uint32_t behind = r + 1 + (tid & 31);
-    const bool many = __popc(__ballot_sync(0xffffffffu, behind <= r + kPaTurns && behind < head.rows && joins(batch_row(a.table, behind)))) == kPaTurns;
-    if (y && !many) return;
     const int32_t id = page_id(a.pool, w.slot, place >> s.shift);
     if (id < 0) return;
     __syncthreads();
     if (tid < 64) joined[tid] = -1;
     __syncthreads();
     bool earlier = false;
-#pragma unroll 4
+#pragma unroll 8
     for (uint32_t i = tid; i < head.rows; i += kPaThreads) {
         const BatchRow z = batch_row(a.table, i);
-        if (!joins(z)) continue;
+        if (z.slot != w.slot || z.length <= 0 || (uint32_t)(z.length - 1) >> s.shift != place >> s.shift) continue;
         if (i < r) earlier = true;
         else atomicMax(&joined[(z.length - 1) & (s.page - 1)], (int)i);
     }
@@ -269,25 +272,43 @@ __device__ void pa_keys(const PaArgs& a, const BatchHead& head, uint32_t r, uint
     __syncthreads();
     uint8_t* const page = a.pages + (size_t)id * page_bytes(s);
     if (!many) pa_few(a, head, page, joined, list, count, place & ~(s.page - 1), reinterpret_cast<double2*>(mem));
-    else pa_many(a, head, page + (size_t)y * s.head, y, joined, list, count, place & ~(s.page - 1), mem);
+    else for (uint32_t u = y; u < 2 * s.G; u += a.shares) pa_many(a, head, page + (size_t)(u % s.G) * s.head, u % s.G, u >= s.G, joined, list, count, place & ~(s.page - 1), mem);
 }
-// CTA (some rows; key head | part of the query heads)
+// CTAs (rows; share of their work), then (rows; part of the query heads).  Where the four rows behind the one that begins a page join it too, as a prompt's do, its heads' keys and values are shared out;
+// else one CTA, another for each of the rows' pages, takes all heads, a warp each, and makes each turn once (8 heads of 128, us, shared out from two tokens on / from five / from sixteen: 128 sequences of 2
+// tokens 35.5 / 20.5 / 20.7, 64 of 8 28.3 / 28.5 / 34.9, 4 of 512 50.0 / 43.1 / 67.6).
 __global__ void __launch_bounds__(kPaThreads) k_page_append(const __grid_constant__ PaArgs a) {
     pdl_enter();
     extern __shared__ float4 pa_mem[];
+    const PageShape& s = a.s;
+    const uint32_t lane = threadIdx.x & 31;
     const BatchHead head = batch_head(a.table, a.B);
-    const uint32_t r0 = blockIdx.x * a.rows;
-    if (r0 >= head.rows) return;
-    if (blockIdx.y >= a.s.G) return pa_queries(a, head, r0, (blockIdx.y - a.s.G) * a.part, reinterpret_cast<double2*>(pa_mem));
-    // rows that append something, and not to the page that the row before them appends to (as most rows of a prompt do)
-    const uint32_t r = r0 + (threadIdx.x & 31);
-    bool begins = false;
-    if ((threadIdx.x & 31) < a.rows && r < head.rows) {
-        const BatchRow w = batch_row(a.table, r), z = batch_row(a.table, r ? r - 1 : 0);
-        begins = w.slot >= 0 && page_row_ok(a.pool, a.s, w) && head.prefix >= 0 && w.length > 0 &&
-                 !(r && z.slot == w.slot && z.length > 0 && (uint32_t)(z.length - 1) >> a.s.shift == (uint32_t)(w.length - 1) >> a.s.shift);
+    if (blockIdx.x >= a.key_ctas) {
+        const uint32_t b = blockIdx.x - a.key_ctas, blocks = (a.B + a.rows - 1) / a.rows, r0 = b % blocks * a.rows;
+        if (r0 < head.rows) pa_queries(a, head, r0, b / blocks * a.part, reinterpret_cast<double2*>(pa_mem));
+        return;
     }
-    for (uint32_t todo = __ballot_sync(0xffffffffu, begins); todo; todo &= todo - 1) pa_keys(a, head, r0 + __ffs(todo) - 1, blockIdx.y, reinterpret_cast<float*>(pa_mem));
+    const uint32_t y = blockIdx.x % a.shares, r0 = blockIdx.x / a.shares * a.key_rows, r = min(r0 + lane, a.B - 1);
+    const BatchRow w = batch_row(a.table, r), z = batch_row(a.table, r ? r - 1 : 0);
+    if (r0 >= head.rows) return;
+    // rows that append something, and not to the page that the row before them appends to (as most rows of a prompt do); those whose page the next four join
+    const bool live = r0 + lane < head.rows && w.length > 0;
+    const uint32_t nth = (uint32_t)(w.length - 1) >> s.shift;
+    const bool begins = live && lane < a.key_rows && w.slot >= 0 && page_row_ok(a.pool, s, w) && head.prefix >= 0 &&
+                        !(r && z.slot == w.slot && z.length > 0 && (uint32_t)(z.length - 1) >> s.shift == nth);
+    bool many = true;
+#pragma unroll
+    for (uint32_t d = 1; d <= kPaTurns; d++) {
+        const int32_t slot = __shfl_down_sync(0xffffffffu, w.slot, d);
+        const uint32_t page = __shfl_down_sync(0xffffffffu, nth, d);
+        const int follows = __shfl_down_sync(0xffffffffu, (int)live, d);      // (every lane takes part in all three)
+        many &= follows && slot == w.slot && page == nth;
+    }
+    const uint32_t few = __ballot_sync(0xffffffffu, begins && !many);
+    for (uint32_t todo = __ballot_sync(0xffffffffu, begins && (many || __popc(few & ((1u << lane) - 1)) % a.shares == y)); todo; todo &= todo - 1) {
+        const uint32_t first = __ffs(todo) - 1;
+        pa_keys(a, head, r0 + first, !(few >> first & 1), y, reinterpret_cast<float*>(pa_mem));
+    }
 }
 
 // ── PAGE_READ ────────────────────────────────────────────────────────────────────────────────────────────────────────
@@ -450,16 +471,19 @@ bool zg_launch_page_op(const ZgOp& op, float* const* bufs, const size_t* elems, 
             a.turned = a.q_heads ? bufs[s.buf[5]] + s.off[3] : nullptr;
             a.freqs = a.rot && s.buf[4] != ZG_NO_BUF ? bufs[s.buf[4]] + s.off[4] : nullptr;
             if (!a.freqs) for (uint32_t i = 0; i < a.rot / 2; i++) a.freq[i] = std::pow((double)s.f[0], -2.0 * i / a.rot);
-            // More rows a CTA where there are many, of which a prompt's mostly join the page of the row before them (2048 rows, 32 / 8 heads of 128, us, with one row a CTA and with four: 59.4 / 44.8;
-            // 8192 rows, with one and with sixteen: 219 / 146).  Query heads in smaller parts where there are few rows (with 1024 / 4096 values: 64 rows 14.4 / 16.4, 128 17.1 / 18.3, 256 of pairs
-            // 20.7 / 22.1; 512 26.7 / 24.6, 2048 51.0 / 44.7).
+            // Keys and values of each head in a CTA of their own (one prompt of 512 tokens, us, together / apart: 28.9 / 22.6, four 48.4 / 43.7), fewer where there are many rows, which each of a page's
+            // CTAs looks through (8192 rows with 16 CTAs / with four: 173 / 143).  As many rows as such CTAs, so that each row's page may have one.  More rows of queries where there are many; query heads in smaller parts where there are few rows
+            // (with 1024 / 4096 values, us: 64 rows of 32 / 8 heads of 128 14.4 / 16.4, 128 17.1 / 18.3, 256 of pairs 20.7 / 22.1; 512 26.7 / 24.6, 2048 51.0 / 44.7).
             a.rows = std::min(kPaRows, (a.B + 511) / 512);
+            a.shares = std::min(2 * a.s.G, std::max(1u, 32768 / a.B));
+            a.key_rows = std::min(kPaRows, 2 * a.s.G);
+            a.key_ctas = (a.B + a.key_rows - 1) / a.key_rows * a.shares;
             const uint32_t heads = std::max(1u, a.B <= 256 ? 1024 / a.s.dk : 4096 / a.s.dk), parts = (a.q_heads + heads - 1) / heads;
             a.part = heads * a.s.dk;
             a.vec = a.q_heads && a.s.dk % 4 == 0 && a.turn_at % 4 == 0 && a.rot % 8 == 0 && a.src_rs % 4 == 0 && a.q_col % 4 == 0 && a.dst_rs % 4 == 0 && s.off[3] % 4 == 0;
             const size_t smem = std::max<size_t>({sizeof(float) * std::min(a.s.page, a.B) * a.s.dk, sizeof(double2) * std::max(a.rows, std::min(kPaTurns, a.B)) * (a.rot / 2)});
             if (!zg_smem_limit<k_page_append>(sizeof(float) * 64 * 256)) return false;
-            launch_pdl(k_page_append, dim3((a.B + a.rows - 1) / a.rows, a.s.G + parts), dim3(kPaThreads), smem, st, a);
+            launch_pdl(k_page_append, dim3(a.key_ctas + (a.B + a.rows - 1) / a.rows * parts), dim3(kPaThreads), smem, st, a);
             ZG_SEQ_CHECK();
             return true;
         }

@@ -86,8 +86,9 @@ def read(keys, values, scales, page_table, entries, live, B, dst):
 
 
 def attend(dst, q, keys, values, scales, page_table, entries, live, B, scale, window=0, cap=0.0, sink=None):
-    """(dst [B, H, dv], how far a kernel may be off).  Scores are sums of dk products whose factors are exact or pairs of halves (2^-22 of a query each), on tensor cores that
-    cut (2^-23 of the sum of magnitudes a step of 16); weights come from exponentials of base 2 (2^-22, and their argument's rounding), outputs from sums over 32 keys at a time that are then rounded."""
+    """(dst [B, H, dv], how far a kernel may be off).  A score is a sum of dk products of exact codes and queries of 45 bits of their largest element, exact but for the rounding of the parts that are joined:
+    2^-21 of the sum of magnitudes, and 2^-23 of it for 16 products, are above both (as they are for operands of 22 bits).  Weights come from exponentials of base 2 (2^-22, and their argument's rounding) and are
+    32 bits of the largest contribution, outputs exact sums that are rounded and joined after 512 tiles and between warps (a rounding for 32 keys is above that)."""
     dst, tol = dst.astype(np.float64), np.zeros(dst.shape)
     page, (slots, most), H = keys.shape[2], page_table.shape, q.shape[1]
     G, dk = keys.shape[1], keys.shape[3]

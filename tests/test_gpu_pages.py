@@ -83,6 +83,24 @@ def test_a_sequences_tokens_at_once(cuda_backend, page, first, tokens):
     a.close()
 
 
+@pytest.mark.parametrize("B,G", [(5000, 8), (2100, 8), (300, 1), (90, 20)])
+def test_prompts_and_single_tokens_at_once(cuda_backend, B, G):
+    """Long runs of rows in one page beside short ones and single rows, in order and shuffled by blocks and row by row."""
+    a = Append(cuda_backend, B, G, 8, 4, 16, H=1, rot=8, slots=100, most=40, pages=4000, seed=B)
+    r, rows = a.r, []
+    for slot in r.permutation(100):
+        if len(rows) < B:
+            first, tokens = int(r.integers(0, 30)), int(r.choice([1, 1, 2, 4, 5, 6, 40, 600]))
+            rows += [(int(slot), first + 1 + i, 0) for i in range(tokens)]
+    rows = rows[:B]
+    rows += [(-1, 1, 0)] * (B - len(rows))
+    a.check(rows)
+    blocks = [rows[i:i + 7] for i in range(0, B, 7)]
+    a.check([x for i in r.permutation(len(blocks)) for x in blocks[i]])
+    a.check([rows[i] for i in r.permutation(B)])
+    a.close()
+
+
 def test_scales_grow_and_stay(cuda_backend):
     """Token after token in one page, ever larger and then small again: each code is what the definition makes of the last state."""
     a = Append(cuda_backend, 1, 1, 8, 8, 16, slots=1, most=1, pages=2)
@@ -380,6 +398,36 @@ def test_pages_beyond_4_gb(cuda_backend):
         assert np.array_equal(a, b)
     assert np.array_equal(memory.download(np.int32, 4 * words * used[0], words)[:4].view(np.float32)[:2], s[0, 0].astype(np.float32))
     cuda_backend.free_program(h)
+    memory.free()
+
+
+# ── two at once ──────────────────────────────────────────────────────────────────────────────────────────────────────
+def test_two_programs_over_one_pool(cuda_backend):
+    """Programs of their own workspaces over one pool, run by turns: what one leaves in its workspace is not the other's."""
+    from zgml_b200 import DeviceBuffer, DeviceOp, DeviceProgram, ExternBuffer, ProgramIO
+    r = np.random.default_rng(8)
+    G, H, d, page, most = 2, 8, 64, 16, 200
+    state = pool(r, 2 * most, G, d, d, page)
+    words = np.ascontiguousarray(pack_pages(*state))
+    memory = DeviceBuffer(cuda_backend, words.nbytes, zero=False)
+    memory.upload(words, 0)
+    page_table = r.permutation(2 * most).reshape(2, most).astype(np.int32)
+    f = lambda x: np.ascontiguousarray(x).view(np.float32).ravel()
+    programs = []
+    for B in (1, 3, 40):
+        entries = [(i % 2, 1 + (997 * (i + B)) % (most * page), 0) for i in range(B)]
+        q = r.standard_normal((B, H, d)).astype(np.float32)
+        h = cuda_backend.compile_program(DeviceProgram([DeviceOp.paged_attention(4, 1, 0, 2, 3, B, H, G, d, d, H * d, page, most, d ** -0.5)], [memory.elems, q.size, page_table.size, 8 + 4 * B, q.size], externs=[ExternBuffer(0, memory)]))
+        programs.append((h, entries, q, *ref.attend(np.zeros((B, H, d)), q, *state, page_table, entries, B, B, d ** -0.5)))
+    first = {}
+    for turn in range(3):
+        for i, (h, entries, q, want, tol) in enumerate(programs):
+            out = np.zeros(q.shape, np.float32)
+            cuda_backend.execute_program(h, [ProgramIO(1, f(q)), ProgramIO(2, f(page_table)), ProgramIO(3, f(table(entries, len(entries))))], [ProgramIO(4, out)])
+            close(out, want, tol)
+            assert np.array_equal(out, first.setdefault(i, out))
+    for h, *_ in programs:
+        cuda_backend.free_program(h)
     memory.free()
 
 

@@ -431,6 +431,20 @@ def test_two_programs_over_one_pool(cuda_backend):
     memory.free()
 
 
+def test_on_another_stream():
+    import torch
+    from zgml_b200 import CudaBackend
+    be = CudaBackend(0)
+    stream = torch.cuda.Stream()
+    be.set_stream(stream.cuda_stream)
+    a = Append(be, 90, 2, 32, 16, 16, H=3, rot=32, slots=6, most=3, pages=20)
+    a.check([(i % 6, 1 + i // 6 * 2 + i % 2, 0) for i in range(90)])
+    a.close()
+    for spare in (0, 4000):
+        attend_case(be, 20, 8, 2, 64, 64, 16, 12, [(i % 3, LENGTHS[i % len(LENGTHS)], 0) for i in range(20)], spare=spare)
+    be.close()
+
+
 # ── together ─────────────────────────────────────────────────────────────────────────────────────────────────────────
 def test_a_decode_loop(cuda_backend):
     """Requests come with prompts, decode, fork, drop drafts, end, and their pages are compacted: one program of copies, appends, attention and reads, replayed with other tables, over one pool that the

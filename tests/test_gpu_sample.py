@@ -190,3 +190,16 @@ def test_rules_then_a_choice(cuda_backend):
         assert got.view(np.int32)[1] % 7 == 0
         p.close()
     cuda_backend.set_graph_mode(True)
+
+
+def test_on_another_stream():
+    import torch
+    from zgml_b200 import CudaBackend
+    be = CudaBackend(0)
+    stream = torch.cuda.Stream()
+    be.set_stream(stream.cuda_stream)
+    r = np.random.default_rng(5)
+    p = program(be, len(CHOICES), 20000)
+    check(p, (3 * r.standard_normal((len(CHOICES), 20000))).astype(np.float32), CHOICES, r.random(len(CHOICES)))
+    p.close()
+    be.close()

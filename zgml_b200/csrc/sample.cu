@@ -446,13 +446,20 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 2 : 4) k_sample(const
                 if (tid == 0) *n_list = 0;
                 __syncthreads();
                 fours(0, n, tid, T_, [&](const float (&x)[4], uint32_t i, uint32_t valid) {
-                    bool in[4];
+                    uint32_t in = 0;
+                    if (linear) {
 #pragma unroll
-                    for (uint32_t e = 0; e < 4; e++) in[e] = e < valid && within(x[e], lo, hi) && (!linear || bin_of(x[e]) == bin);
+                        for (uint32_t e = 0; e < 4; e++) in |= (bin_of(x[e]) == bin) << e;
+                    } else {
+#pragma unroll
+                        for (uint32_t e = 0; e < 4; e++) in |= within(x[e], lo, hi) << e;
+                    }
+                    if (!in) return;
 #pragma unroll
                     for (uint32_t e = 0; e < 4; e++) {
+                        if (e >= valid || !(in >> e & 1)) continue;
                         const u64 o = sm_order(x[e], v0 + i + e);
-                        if (in[e] && o >= lo && o <= hi && (linear || (uint32_t)((hi - o) >> shift) == bin)) sh.list[atomicAdd(n_list, 1u)] = make_ulonglong2(o, by_mass ? weight(x[e]) : 1);
+                        if (o >= lo && o <= hi && (linear || (uint32_t)((hi - o) >> shift) == bin)) sh.list[atomicAdd(n_list, 1u)] = make_ulonglong2(o, by_mass ? weight(x[e]) : 1);
                     }
                 });
                 __syncthreads();

@@ -297,13 +297,12 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 2 : 4) k_sample(const
         if (sh.found_upto <= kSmList) {
             // few: they go to the first CTA
             uint32_t* const n_list = &sh.n_list[1];
-            auto give = [&](float x, uint32_t i) { sh.list[atomicAdd(n_list, 1u)] = make_ulonglong2(sm_order(x, v0 + i), weight(x)); };
             fours(0, n, tid, T_, [&](const float (&x)[4], uint32_t i, uint32_t valid) {
                 uint32_t b[4];
 #pragma unroll
                 for (uint32_t e = 0; e < 4; e++) b[e] = bin_of(x[e]);
 #pragma unroll
-                for (uint32_t e = 0; e < 4; e++) if (e < valid && b[e] <= first_bin) give(x[e], i + e);
+                for (uint32_t e = 0; e < 4; e++) if (e < valid && b[e] <= first_bin) sh.list[atomicAdd(n_list, 1u)].x = sm_order(x[e], v0 + i + e);
             });
             __syncthreads();
             // one addition to the first CTA's number for a CTA's candidates
@@ -314,8 +313,8 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 2 : 4) k_sample(const
             }
             __syncthreads();
             for (uint32_t t = tid; t < *n_list; t += T_) {
-                const ulonglong2 x = sh.list[t];
-                asm volatile("st.shared::cluster.v2.u64 [%0], {%1, %2};" ::"r"(sm_at(&sh.all_list[sh.n_list[0] + t], 0)), "l"(x.x), "l"(x.y) : "memory");
+                const u64 x = sh.list[t].x;
+                asm volatile("st.shared::cluster.v2.u64 [%0], {%1, %2};" ::"r"(sm_at(&sh.all_list[sh.n_list[0] + t], 0)), "l"(x), "l"(weight(sm_value((uint32_t)(x >> kSmIndexBits)))) : "memory");
             }
             cluster_sync();                                          // (before that no CTA leaves: its bins are read)
             if (rank != 0) return;
@@ -459,9 +458,11 @@ __global__ void __launch_bounds__(KEEP ? 512 : 256, KEEP ? 2 : 4) k_sample(const
                     for (uint32_t e = 0; e < 4; e++) {
                         if (e >= valid || !(in >> e & 1)) continue;
                         const u64 o = sm_order(x[e], v0 + i + e);
-                        if (o >= lo && o <= hi && (linear || (uint32_t)((hi - o) >> shift) == bin)) sh.list[atomicAdd(n_list, 1u)] = make_ulonglong2(o, by_mass ? weight(x[e]) : 1);
+                        if (o >= lo && o <= hi && (linear || (uint32_t)((hi - o) >> shift) == bin)) sh.list[atomicAdd(n_list, 1u)].x = o;
                     }
                 });
+                __syncthreads();
+                for (uint32_t t = tid; t < *n_list; t += T_) sh.list[t].y = by_mass ? weight(sm_value((uint32_t)(sh.list[t].x >> kSmIndexBits))) : 1;      // (side by side: few lanes of a warp find one)
                 __syncthreads();
                 cluster_sync();                                      // (and peers have read the bins)
                 uint32_t ends[C];

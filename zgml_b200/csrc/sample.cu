@@ -604,14 +604,14 @@ bool zg_launch_sample(const ZgOp& op, float* const* bufs, cudaStream_t st) {
     a.B = s.n[0]; a.V = s.n[1]; a.rs = s.n[2];
     a.vec = a.rs % 4 == 0 && (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0;
     // CTAs of a row: eight, fewer where a slice would be small (one row of 4096 tokens, us, by 1 / 8 CTAs: 10.3 / 12.3), or where the rows fill the SMs, two CTAs each, without, and their slices
-    // leave room for two (256 rows of 32000 tokens by 2 / 4 / 8 CTAs: 53.0 / 66.7 / 106.6; 64 rows: 30.8 / 26.7 / 36.9; 64 rows of 65536: 49.2 / 35.3 / 45.7).
+    // leave room for two (256 rows of 32000 tokens by 2 / 4 / 8 CTAs: 51.5 / 61.4 / 86.1; 64 rows: 30.8 / 24.6 / 30.8; 64 rows of 65536: 47.1 / 34.9 / 39.5).
     const uint32_t sms = zg_sm_count();
     auto slice = [&](uint32_t C) { return ((a.V + C - 1) / C + 3) / 4 * 4; };
     uint32_t C = kSmCluster;
     while (C > 1 && (slice(C) <= 2048 || ((uint64_t)a.B * C > 2 * sms && slice(C / 2) <= kSmHalf))) C /= 2;
     a.slice = slice(C);
-    // Slices are kept up to three waves of CTAs (128256 tokens, us, kept / read again: 1 row 20.5 / 29.7, 32 rows 49.2 / 81.9, 64 63.9 / 87.1, 96 85.1 / 99.2, 128 107 / 103, 512 405 / 339;
-    // 200000 tokens: 32 rows 65.6 / 86.1, 64 112 / 102).
+    // Slices are kept up to three waves of CTAs (128256 tokens, us, kept / read again: 1 row 18.5 / 28.7, 32 rows 43.7 / 75.8, 64 58.8 / 79.9, 96 76.5 / 92.3, 128 95.8 / 99.5,
+    // 192 149 / 145, 512 364 / 340; 200000 tokens: 32 rows 63.5 / 77.8, 64 104 / 98).
     const bool keep = C < kSmCluster || (uint64_t)a.B * C <= 3 * sms * (a.slice <= kSmHalf ? 2 : 1);
     if (!(C == 1 ? sm_launch<1, true>(a, st) : C == 2 ? sm_launch<2, true>(a, st) : C == 4 ? sm_launch<4, true>(a, st) : keep ? sm_launch<kSmCluster, true>(a, st) : sm_launch<kSmCluster, false>(a, st))) return false;
     ZG_SEQ_CHECK();

@@ -334,7 +334,7 @@ def test_queries_with_outliers(cuda_backend):
 def test_tables_of_long_sequences(cuda_backend, H, G, dk, dv, page):
     """Page tables that could hold far more than they do: sizes go by them, answers by the rows."""
     entries = [(i % 3, n, 0) for i, n in enumerate(LENGTHS)]
-    for window in (0, 40):
+    for window in (0, 40, 1 << 18):
         attend_case(cuda_backend, len(entries) + 1, H, G, dk, dv, page, 192 // page, entries, spare=(1 << 19) // page, window=window, pad=2)
     attend_case(cuda_backend, 40, H, G, dk, dv, page, 192 // page, [(i // 15, 180 - 40 + i, 0) for i in range(40)], spare=(1 << 19) // page)      # runs of one slot
 
@@ -343,7 +343,8 @@ def test_many_rows(cuda_backend):
     """More rows than a warp reads at once, most of them short, runs of one slot across its blocks of 32, rows that are idle among them."""
     r = np.random.default_rng(0)
     for H, G in ((4, 4), (4, 1)):
-        attend_case(cuda_backend, 700, H, G, 32, 32, 16, 12, [(int(r.integers(-1, 3)), int(r.integers(0, 60)), 0) for _ in range(690)])
+        for window in (0, 20):
+            attend_case(cuda_backend, 700, H, G, 32, 32, 16, 12, [(int(r.integers(-1, 3)), int(r.integers(0, 60)), 0) for _ in range(690)], window=window, spare=3000)
         attend_case(cuda_backend, 400, H, G, 32, 32, 16, 12, [(i // 37 % 3, 1 + i % 192, 0) for i in range(400)], slots=3)
         attend_case(cuda_backend, 300, H, G, 32, 32, 16, 4, [(i, 1 + i % 64, 0) for i in range(300)], slots=300)
 

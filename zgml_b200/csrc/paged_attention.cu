@@ -634,18 +634,19 @@ bool pg_launch(const PgArgs& a, cudaStream_t st) {
 // 390 / 269, 64 rows of up to 4096 101 / 100; 64 rows of 32 / 2 heads of up to 4096 51 / 61, 9 x 7 rows of up to 2111 42 / 51).
 struct PgForm { bool narrow, wide, one; uint32_t queries, tokens; };      // one: one launch
 constexpr uint64_t kPgLarge = 1u << 21;
-// One launch, a CTA of eight warps for each sequence and key head, where the longest sequence has up to 1024 tokens and the CTAs make two waves at most (an SM holds one: its registers); else equal shares
+// One launch, a CTA of eight warps for each sequence and key head, where the longest sequence has, or its window shows, up to 1024 tokens and the CTAs make two waves at most (an SM holds one: its registers); else equal shares
 // and a second launch that joins them. One launch / two, us: 3 products of 64-dim heads, 64 tokens 6.2 / 10.3, 576 10.3 / 12.3, 2048 14.4 / 12.3; 128 dims, 32 products, 1024 tokens 12.3 / 16.4, 2048
 // 18.5 / 18.5; 128 products, 64 tokens 8.2 / 16.4, 4096 28.7 / 26.7; 256 products, 64 tokens 14.4 / 16.4, 1024 22.6 / 22.6, 2048 30.8 / 27.0; 512 products (four waves), 64 tokens 26.7 / 16.4.
-bool pg_one(uint64_t products, uint64_t capacity) { return products <= 2ull * zg_sm_count() && capacity <= 1024; }
+bool pg_one(uint64_t products, uint64_t seen) { return products <= 2ull * zg_sm_count() && seen <= 1024; }
 PgForm pg_form(const ZgSeqOp& op, uint32_t slots, bool scratch) {
     PgForm f;
     const PageShape s = page_shape(op.n[2], op.n[3], op.n[4], op.n[7]);
     const uint32_t rep = op.n[1] / op.n[2];
     f.narrow = s.kp <= 64 && s.vp <= 64;
     f.wide = s.kp > 128 || s.vp > 128;
-    f.queries = scratch && rep > 4 && !f.wide && (uint64_t)op.n[0] * op.n[2] * ((uint64_t)op.n[8] << s.shift) >= kPgLarge ? 8 : 4;
-    f.one = !scratch || pg_one(op.n[0] * op.n[2] * ((rep + 3) / 4), (uint64_t)op.n[8] << s.shift);
+    const uint64_t capacity = (uint64_t)op.n[8] << s.shift, seen = op.n[9] ? std::min(capacity, (uint64_t)op.n[9] + kPgTile) : capacity;      // positions of a row at most
+    f.queries = scratch && rep > 4 && !f.wide && (uint64_t)op.n[0] * op.n[2] * seen >= kPgLarge ? 8 : 4;
+    f.one = !scratch || pg_one(op.n[0] * op.n[2] * ((rep + 3) / 4), seen);
     f.tokens = op.n[0] > slots ? std::max(1u, f.queries / rep) : 1;
     return f;
 }

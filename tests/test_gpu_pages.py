@@ -347,6 +347,9 @@ def test_many_rows(cuda_backend):
             attend_case(cuda_backend, 700, H, G, 32, 32, 16, 12, [(int(r.integers(-1, 3)), int(r.integers(0, 60)), 0) for _ in range(690)], window=window, spare=3000)
         attend_case(cuda_backend, 400, H, G, 32, 32, 16, 12, [(i // 37 % 3, 1 + i % 192, 0) for i in range(400)], slots=3)
         attend_case(cuda_backend, 300, H, G, 32, 32, 16, 4, [(i, 1 + i % 64, 0) for i in range(300)], slots=300)
+    for first in (0, 1, 33):                             # a chunk of one sequence's prompt, one launch and two
+        for spare in (0, 3000):
+            attend_case(cuda_backend, 140, 2, 1, 32, 32, 16, 13, [(1, 5, 0)] * first + [(0, 1 + i, 0) for i in range(139 - first)], slots=2, spare=spare)
 
 
 @pytest.mark.parametrize("H,G,dk,dv", [(8, 2, 128, 128), (9, 3, 64, 64), (6, 1, 80, 48), (4, 1, 256, 192), (5, 5, 33, 17)])

@@ -182,9 +182,15 @@ __global__ void __launch_bounds__(32 * W, W == 1 ? pg_warps(KC, VC, NT) : 1) k_p
         if (r >= live) return;
         if (item == 0 && warp == 0) settle(r);
         const int32_t slot = batch_row(a.table, r).slot;
-        uint32_t back = 0;                                           // rows of the same slot directly before r
-        while (a.tokens > 1 && back < r && batch_row(a.table, r - 1 - back).slot == slot) back++;
-        if (slot < 0 || back % a.tokens) return;
+        if (slot < 0) return;
+        if (a.tokens > 1) {
+            uint32_t back = 0, same;                                 // rows of the same slot directly before r
+            do {
+                same = __ballot_sync(0xffffffffu, back + lane < r && batch_row(a.table, r - 1 - back - lane).slot == slot);
+                back += same == 0xffffffffu ? 32 : __ffs(~same) - 1;
+            } while (same == 0xffffffffu);
+            if (back % a.tokens) return;
+        }
         group = pg_group(a, live, r, slot);
         if (!group.tiles) return;
         off = (uint32_t)pg_share(group.tiles, warp, W);

@@ -276,7 +276,7 @@ __device__ void pa_keys(const PaArgs& a, const BatchHead& head, uint32_t r, bool
 }
 // CTAs (rows; share of their work), then (rows; part of the query heads).  Where the four rows behind the one that begins a page join it too, as a prompt's do, its heads' keys and values are shared out;
 // else one CTA, another for each of the rows' pages, takes all heads, a warp each, and makes each turn once (8 heads of 128, us, shared out from two tokens on / from five / from sixteen: 128 sequences of 2
-// tokens 35.5 / 20.5 / 20.7, 64 of 8 28.3 / 28.5 / 34.9, 4 of 512 50.0 / 43.1 / 67.6).
+// tokens 35.5 / 20.5 / 20.7, 64 of 8 28.3 / 28.5 / 34.9, 4 of 512 50.0 / 43.1 / 67.6).  Bound by latency: 256 single rows 11 us, 2048 rows of four prompts 36 us, 2.4 TB/s.
 __global__ void __launch_bounds__(kPaThreads) k_page_append(const __grid_constant__ PaArgs a) {
     pdl_enter();
     extern __shared__ float4 pa_mem[];

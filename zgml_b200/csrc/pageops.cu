@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(kPrThreads) k_page_read(const PrArgs a) {
     pdl_enter();
     __shared__ const uint8_t* parts[kPrRows];                        // null: zeros, or nothing (tokens: -1), or no numbers (-2)
     __shared__ int32_t tokens[kPrRows];
-    __shared__ int8_t rows[kPrRows][16];                             // of a tile that row m reads for all: the row of each of its tokens, or -1
+    __shared__ alignas(16) int8_t rows[kPrRows][16];                 // of a tile that row m reads for all: the row of each of its tokens, or -1
     __shared__ uint32_t leaders;
     const PageShape& s = a.s;
     const uint32_t first = blockIdx.x * kPrRows, g = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;

@@ -373,7 +373,9 @@ typedef enum ZgOpTag {
  *                   buf 0 pool 1 src 2 page table 3 table 4 frequency table 5 turned query heads | off 0 key column 1 value column 2 query column 3 column in buf 5 4 frequency offset
  *                   n 0 B 1 G 2 dk 3 dv 4 src row stride 5 page 6 most 7 first turned value 8 turned values 9 layout 10 query heads 11 row stride of buf 5 | f 0 base
  * PAGED_ATTENTION   softmax attention of each row over the first `length` positions of its slot, with a window n9 > 0 over the last n9 of them.  Query head h reads key head
- *                   h / (H / G).  Score cap f1 and sinks as CACHED_ATTENTION has them.  A row that sees no key gets zeros.
+ *                   h / (H / G).  Score cap f1 and sinks as CACHED_ATTENTION has them.  A row that sees no key gets zeros.  Weights w of the values are whole multiples of 2^-29 of the largest near them: that
+ *                   and roundings put an output off by at most 24 * 2^-23 of sum w (127 * scale) / sum w, scale being its value's page's, however many keys there are; exponentials (2^-20, and 2^-23 for each nat below the
+ *                   largest score) and scores (2^-21) of each weight by themselves.
  *                   buf 0 dst [B, H * dv] 1 q 2 pool 3 page table 4 table 5 sinks | off 0 q column 1 dst column 2 sinks
  *                   n 0 B 1 H 2 G 3 dk 4 dv 5 q row stride 6 dst row stride 7 page 8 most 9 window 10 wdt of the sinks | f 0 score scale 1 score cap
  * PAGE_READ         dst[row] = the cache row at each row's position (keys at column off 0, values at off 1), code * scale; a row of length 0 gets zeros.

@@ -3,8 +3,9 @@
 // Both products run on the tensor cores in whole numbers, whose sums are exact: codes of 8 bits, which need no conversion, times digits of 8 bits.  A query is six digits of base 256 (45 bits
 // of its largest element), a weight four (32 bits of the largest contribution); the digits of four queries are 24 and 16 columns of the instructions, codes their rows.  Stored codes are offset
 // by 128: sum (c + 128) d - 128 sum d is exact too, and a bit of each code of a value is turned over.  Scales are powers of two: a key's joins its scores, a value's its weights.  A weight is 2^(s + e - n), with the score s in powers of
-// two, e the exponent of its value's scale and n a whole number that no s + e so far passes by more than 3, so that the largest contributions keep their bits whatever the pages' scales
-// are; the sum of the softmax has a frame m of its own, and the quotient is put right by 2^(n - m).
+// two, e the exponent of its value's scale and n a whole number that no s + e passes by more than 3, so that the largest contributions keep their bits whatever the pages' scales
+// are; the sum of the softmax has a frame m of its own, and the quotient is put right by the difference of the frames.  n falls again where weights have become small, before what they lose could add up to 2^-20 of
+// sum w (127 scale) / sum w.  When n changes, products join those before in a frame of their own, in two parts, and so does the softmax's sum every four tiles: nothing grows with a sequence's length.
 #include "pages.cuh"
 #include "exp2.cuh"
 #include "split_tc.cuh"
@@ -20,7 +21,8 @@ struct PgArgs {
     uint32_t B, H, rep, q_rs, dst_rs, window, sink_bf16, tokens, chunks;      // tokens of a sequence a warp takes together, chunks of a key head's query heads
     float scale, cap;
 };
-constexpr uint32_t kPgTile = 32, kPgShift = 29, kPgFlush = 512;      // (512 tiles of 32 products of two bytes: below 2^31)
+constexpr uint32_t kPgTile = 32, kPgShift = 29, kPgFlush = 512;      // tiles (512 of 32 products of two bytes: below 2^31)
+constexpr float kPgCredit = 176.0f, kPgGrant = 3.0f;
 constexpr uint32_t kPgPlan = 8;                                     // words of the plan before the rows' tiles: all tiles (64 bits), warps, -, warps / tiles (64 bits)
 constexpr uint32_t kPgRows = 8, kPgLeast = 2;      // blocks of 32 rows that are read at once; tiles a warp at least where there are few (one sequence of 4096 tokens, us, with 1 / 2 / 4: 18.5 / 15.1 / 16.4)
 constexpr float kPgSlack = 3.0f;                                     // weights reach 2^(29 + 3)
@@ -50,6 +52,17 @@ __device__ __forceinline__ float pg_frame(float from, float to) { return from ==
 __device__ __forceinline__ float pg_scaled(float x, float back) {
     const float half = truncf(back * 0.5f);
     return x * exp2f(half) * exp2f(back - half);
+}
+// floats of a warp behind its tile: outputs in two parts, four of a lane for each four queries, statistics of queries (W = 8)
+__host__ __device__ constexpr uint32_t pg_aside(uint32_t NT, uint32_t vp) { return NT * (8 * vp + 128 + 16); }
+// What x brings joins f times a sum, f a power of two, kept as (sum, what its roundings added too much): W. Kahan, Communications of the ACM 8, 1965.  However many parts, two roundings of the sum of their magnitudes.
+__device__ __forceinline__ float2 pg_add(float2 sum, float f, float x) {
+    const float y = fmaf(-sum.y, f, x), t = fmaf(sum.x, f, y);
+    return make_float2(t, fmaf(-sum.x, f, t) - y);
+}
+// sum of w x, by pairs
+__device__ __forceinline__ float pg_tree(const float (&w)[8], const float (&x)[8]) {
+    return (fmaf(w[0], x[0], w[1] * x[1]) + fmaf(w[2], x[2], w[3] * x[3])) + (fmaf(w[4], x[4], w[5] * x[5]) + fmaf(w[6], x[6], w[7] * x[7]));
 }
 // What a query's outputs are multiplied by as a power of two, and divided by, in the frames m of the sum and n of the outputs.
 __device__ __forceinline__ float2 pg_finish(const PgArgs& a, uint32_t h, float m, float n, float sum) {
@@ -102,9 +115,10 @@ __global__ void __launch_bounds__(32 * W, W == 1 ? pg_warps(KC, VC, NT) : 1) k_p
     const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, row8 = lane / 4, j = lane % 4;
     const uint32_t heads = min(a.rep, 4u * NT), per_row = s.G * a.chunks;      // query heads of a chunk; products of a group of rows
     const uint32_t live = batch_head(a.table, a.B).rows;
-    const uint32_t kp = FULL ? 32 * KC : s.kp, vp = FULL ? 16 * VC : s.vp, kc = kp / 32, vc = vp / 16, k_bytes = kPgTile * kp, pitch = vp + 4;
-    uint8_t* const buffer = reinterpret_cast<uint8_t*>(pg_mem) + warp * (k_bytes + kPgTile * vp + 32 + 16 * NT * pitch);
-    float* const rec = reinterpret_cast<float*>(buffer + k_bytes + kPgTile * vp + 32);      // [4 NT][pitch]
+    const uint32_t kp = FULL ? 32 * KC : s.kp, vp = FULL ? 16 * VC : s.vp, kc = kp / 32, vc = vp / 16, k_bytes = kPgTile * kp, buffer_bytes = k_bytes + kPgTile * vp + 32 + 4 * pg_aside(NT, vp);
+    uint8_t* const buffer = reinterpret_cast<uint8_t*>(pg_mem) + warp * buffer_bytes;
+    float2* const rec = reinterpret_cast<float2*>(buffer + k_bytes + kPgTile * vp + 32) + lane;      // a lane's outputs in two parts, 32 apart
+    float2* const aside = rec + 4 * NT * vp;                         // what a lane seldom needs
     // rows that see nothing, or whose words are out of range
     auto settle = [&](uint32_t row) {
         const BatchRow z = batch_row(a.table, row);
@@ -306,24 +320,33 @@ __global__ void __launch_bounds__(32 * W, W == 1 ? pg_warps(KC, VC, NT) : 1) k_p
         }
         all_in = __reduce_min_sync(0xffffffffu, all_in);
         least = __reduce_max_sync(0xffffffffu, least);
-        // Frames: m of the lane's sum of weights, n of the products' weights.  They stay while no score passes them by much, which one vote of the warp tells.
-        float m[NT], n[NT], sum[NT];
+        // Frames: m of the lane's sum of weights, n of the products' weights.  They stay while no score passes them by much, which one vote of the warp tells.  But weights far below n are rounded the
+        // same way by the thousand (in one frame for a sequence, outputs of 1.3e-4 came out as 2.4e-4 behind 65536 keys some 2^29 below the first).  So lanes pay for n: for each tile, in which a lane's four weights may
+        // lose 2^-28 of 2^n together, 2^n is taken from its credit, and kPgCredit times what they weigh is added.  Where nothing is left, n becomes what the present tile asks for, and lanes in debt get
+        // kPgGrant times the new 2^n: eight lanes at most 48 times the largest contribution of this tile.  Their debts, of at most 2^n each, are 16 times that of the tile that set n, or less.  So all that is
+        // taken is at most 176 + 48 + 16 times what all weights are, and what is lost 240 * 2^-28 of that, however many they are.  (64 rows of 64 / 8 heads of 128, up to 8192, scores of 0.7 to 2.6 powers of two: 163 us, with one frame
+        // and plain sums 152; 32 / 8 heads up to 4096 65.7 and 65.5; putting products away every 8 tiles 170.)
+        float m[NT], n[NT], credit[NT], sum[NT];                     // credit in units of 2^n; sum: of four tiles, which then joins those before
+        auto sums = [&](int t) { return aside + 64 * t; };
+        auto kept = [&](int t) { return &aside[64 * t + 32].x; };    // the frame of the products that were put away
         int o[NT][VC][2][4];                                         // even and odd digits: two of each
-        uint32_t since = 0;                                          // tiles since the sums were put away
+        uint32_t since = 0;                                          // tiles since the products were put away
         bool stored = false;
 #pragma unroll
         for (int t = 0; t < NT; t++) {
-            m[t] = n[t] = -INFINITY; sum[t] = 0.0f;
+            m[t] = n[t] = *kept(t) = -INFINITY;
+            credit[t] = sum[t] = 0.0f;
+            *sums(t) = make_float2(0.0f, 0.0f);
 #pragma unroll
             for (int c = 0; c < VC; c++)
 #pragma unroll
                 for (int k = 0; k < 8; k++) o[t][c][k / 4][k % 4] = 0;
         }
-        auto output = [&](int t, int c, int k) {
+        auto output = [&](int t, int c, int k) {                     // in the frame n
             const int (&x)[2][4] = o[t][c];
-            const float v = fmaf(fmaf(fmaf((float)x[1][2 * k + 1], 256.0f, (float)x[0][2 * k + 1]), 256.0f, (float)x[1][2 * k]), 256.0f, (float)x[0][2 * k]);
-            return stored ? v + rec[(4 * t + j) * pitch + 16 * c + 8 * k + row8] : v;
+            return fmaf(fmaf(fmaf((float)x[1][2 * k + 1], 256.0f, (float)x[0][2 * k + 1]), 256.0f, (float)x[1][2 * k]), 256.0f, (float)x[0][2 * k]);
         };
+        auto place = [&](int t, int c, int k) { return 32 * (2 * (t * vc + c) + k); };
         for (uint32_t tile = t0; tile < t1 && !gave_up; tile++) {
             const bool more = tile + 1 < t1;
             if (!__all_sync(0xffffffffu, mbar_wait(k_bar, k_phase))) {
@@ -383,50 +406,65 @@ __global__ void __launch_bounds__(32 * W, W == 1 ? pg_warps(KC, VC, NT) : 1) k_p
             // weights
             const float e[2] = {scales.y == scales.y ? (float)((int)(__float_as_uint(scales.y) >> 23) - 127) : kBatchNaN, scales.w == scales.w ? (float)((int)(__float_as_uint(scales.w) >> 23) - 127) : kBatchNaN};
             bool over = false;
+            float top[NT];                                           // the lane's largest contribution
 #pragma unroll
             for (int t = 0; t < NT; t++) {
                 const float top0 = fmaxf(sc[t][0][0], sc[t][0][1]), top1 = fmaxf(sc[t][1][0], sc[t][1][1]);
-                over = over || fmaxf(top0 + e[0], top1 + e[1]) > n[t] + kPgSlack || fmaxf(top0, top1) > m[t] + 64.0f;
+                top[t] = fmaxf(top0 + e[0], top1 + e[1]);
+                over = over || top[t] > n[t] + kPgSlack || fmaxf(top0, top1) > m[t] + 64.0f || (credit[t] < 0.0f && n[t] > -INFINITY);
             }
             if (__any_sync(0xffffffffu, over) || since == kPgFlush) {
-                float alpha[NT];
+                if (since) {                                         // the products so far go to shared memory, in a frame of theirs
 #pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    const float top0 = fmaxf(sc[t][0][0], sc[t][0][1]), top1 = fmaxf(sc[t][1][0], sc[t][1][1]), new_m = fmaxf(m[t], ceilf(fmaxf(top0, top1)));
-                    float new_n = fmaxf(n[t], ceilf(fmaxf(top0 + e[0], top1 + e[1])));
-#pragma unroll
-                    for (int k = 4; k < 32; k *= 2) new_n = fmaxf(new_n, __shfl_xor_sync(0xffffffffu, new_n, k));
-                    alpha[t] = new_n == n[t] ? 1.0f : pg_pow2(n[t] - new_n);
-                    sum[t] *= new_m == m[t] ? 1.0f : pg_pow2(m[t] - new_m);
-                    m[t] = new_m; n[t] = new_n;
-                }
-                if (stored || since) {                               // the sums so far, in the new frame, go to shared memory, where a lane has places of its own
-#pragma unroll
-                    for (int t = 0; t < NT; t++)
+                    for (int t = 0; t < NT; t++) {
+                        const float from = *kept(t), to = fmaxf(from, n[t]), before = pg_frame(from, to), now = pg_frame(n[t], to);
+                        *kept(t) = to;
 #pragma unroll
                         for (int c = 0; c < VC; c++) {
                             if (!FULL && c >= vc) break;
 #pragma unroll
-                            for (int k = 0; k < 2; k++) rec[(4 * t + j) * pitch + 16 * c + 8 * k + row8] = output(t, c, k) * alpha[t];
+                            for (int k = 0; k < 2; k++) {
+                                const uint32_t at = place(t, c, k);
+                                rec[at] = pg_add(stored ? rec[at] : make_float2(0.0f, 0.0f), before, output(t, c, k) * now);
+                            }
 #pragma unroll
                             for (int k = 0; k < 8; k++) o[t][c][k / 4][k % 4] = 0;
                         }
+                    }
                     stored = true;
                     since = 0;
                 }
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    const float new_m = fmaxf(m[t], ceilf(fmaxf(fmaxf(sc[t][0][0], sc[t][0][1]), fmaxf(sc[t][1][0], sc[t][1][1])))), f = new_m == m[t] ? 1.0f : pg_pow2(m[t] - new_m);
+                    float most = top[t], least_left = credit[t];
+#pragma unroll
+                    for (int k = 4; k < 32; k *= 2) { most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, k)); least_left = fminf(least_left, __shfl_xor_sync(0xffffffffu, least_left, k)); }
+                    const float new_n = least_left < 0.0f ? ceilf(most) : fmaxf(n[t], ceilf(most));
+                    credit[t] = credit[t] >= 0.0f && n[t] > -INFINITY ? fminf(credit[t] * exp2f(fminf(n[t] - new_n, 60.0f)), 0x1p60f) : kPgGrant;
+                    sum[t] *= f; sums(t)->x *= f; sums(t)->y *= f;
+                    m[t] = new_m; n[t] = new_n;
+                }
             }
             since++;
+            if ((tile - t0) % 4 == 3) {
+#pragma unroll
+                for (int t = 0; t < NT; t++) { *sums(t) = pg_add(*sums(t), 1.0f, sum[t]); sum[t] = 0.0f; }
+            }
             uint32_t low_digits[NT][2], high_digits[NT][2];              // of each half's weights: digits 0 and 2, and 1 and 3, of four positions
 #pragma unroll
             for (int t = 0; t < NT; t++) {
                 const float fm = m[t] == -INFINITY ? 0.0f : m[t], fn = (float)kPgShift - (n[t] == -INFINITY ? 0.0f : n[t]);
+                float weights[2], mass = 0.0f;
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
                     uint32_t turned[2];
+                    weights[u] = 0.0f;
 #pragma unroll
                     for (int k = 0; k < 2; k++) {
                         const float x = sc[t][u][k], y = x == -INFINITY ? 0.0f : sa_ex2(x + (fn + e[u]));
-                        sum[t] += sa_ex2(x - fm) + (y - y);              // (a scale that is not a number is one of the sum's too)
+                        mass += y;
+                        weights[u] += sa_ex2(x - fm);
                         const uint32_t w = __float2uint_rn(y);
                         // a lane's weight is two columns of 16 bits, a position a row; turned around they are rows of positions
                         asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(turned[k]) : "r"(w));
@@ -434,6 +472,8 @@ __global__ void __launch_bounds__(32 * W, W == 1 ? pg_warps(KC, VC, NT) : 1) k_p
                     low_digits[t][u] = __byte_perm(turned[0], turned[1], 0x6420);
                     high_digits[t][u] = __byte_perm(turned[0], turned[1], 0x7531);
                 }
+                sum[t] += (weights[0] + weights[1]) + (mass - mass);      // (a scale that is not a number is one of the sum's too)
+                credit[t] = fmaf(mass, kPgCredit / (float)(1u << kPgShift), credit[t] - 1.0f);
             }
             __syncwarp();
             if (!__all_sync(0xffffffffu, mbar_wait(v_bar, v_phase))) {
@@ -459,8 +499,10 @@ __global__ void __launch_bounds__(32 * W, W == 1 ? pg_warps(KC, VC, NT) : 1) k_p
 #pragma unroll
             for (int t = 0; t < NT; t++) sum[t] = kBatchNaN;
         }
+#pragma unroll
+        for (int t = 0; t < NT; t++) sum[t] = pg_add(*sums(t), 1.0f, sum[t]).x;
         const bool whole = W == 1 && take == group.tiles;
-        float* const record = whole ? nullptr : W > 1 ? rec : a.part + (size_t)(2 * blockIdx.x + (off ? 0 : 1)) * 4 * NT * pitch;      // (a lane's own places of rec again)
+        float* const record = whole || W > 1 ? nullptr : a.part + (size_t)(2 * blockIdx.x + (off ? 0 : 1)) * 4 * NT * (vp + 4);
 #pragma unroll
         for (int t = 0; t < NT; t++) {
             float top = m[t];
@@ -471,16 +513,18 @@ __global__ void __launch_bounds__(32 * W, W == 1 ? pg_warps(KC, VC, NT) : 1) k_p
             for (int k = 4; k < 32; k *= 2) sum[t] += __shfl_xor_sync(0xffffffffu, sum[t], k);
             const uint32_t i = 4 * t + j, token = i / heads, h = chunk * heads + i % heads;
             const bool on = token < group.rows && h < a.rep;
+            const float frame = fmaxf(*kept(t), n[t]), before = pg_frame(*kept(t), frame), now = pg_frame(n[t], frame);
             float* to;
             float2 f = make_float2(0.0f, 1.0f);
             if (whole) {
                 const BatchRow z = batch_row(a.table, r + (on ? token : 0));
                 if (!on || !page_row_ok(a.pool, s, z) || z.length == 0) continue;      // (the latter two: settle)
-                f = pg_finish(a, g * a.rep + h, top, n[t], sum[t]);
+                f = pg_finish(a, g * a.rep + h, top, frame, sum[t]);
                 to = a.dst + (size_t)(r + token) * a.dst_rs + (g * a.rep + h) * s.dv;
             } else {
-                to = record + i * pitch + (W > 1 ? 0 : 4);
-                if (row8 == 0) *reinterpret_cast<float4*>(record + i * pitch + (W > 1 ? vp : 0)) = make_float4(top, n[t], sum[t], 0.0f);
+                float* const stats = W > 1 ? &aside[64 * NT + 2 * i].x - 2 * lane : record + i * (vp + 4);
+                to = stats + 4;
+                if (row8 == 0) *reinterpret_cast<float4*>(stats) = make_float4(top, frame, sum[t], 0.0f);
             }
 #pragma unroll
             for (int c = 0; c < VC; c++) {
@@ -488,8 +532,11 @@ __global__ void __launch_bounds__(32 * W, W == 1 ? pg_warps(KC, VC, NT) : 1) k_p
 #pragma unroll
                 for (int k = 0; k < 2; k++) {
                     const uint32_t d = 16 * c + 8 * k + row8;
-                    const float v = output(t, c, k);
-                    if (!whole) to[d] = v;
+                    float v = output(t, c, k) * now;
+                    const uint32_t at = place(t, c, k);
+                    if (stored) v = pg_add(rec[at], before, v).x;
+                    if (W > 1) rec[at].x = v;
+                    else if (!whole) to[d] = v;
                     else if (d < s.dv) to[d] = pg_scaled(v / f.y, f.x);
                 }
             }
@@ -515,23 +562,22 @@ __global__ void __launch_bounds__(32 * W, W == 1 ? pg_warps(KC, VC, NT) : 1) k_p
             const uint32_t h = chunk * heads + i % heads, row = r + i / heads;
             const BatchRow z = batch_row(a.table, row);
             if (h >= a.rep || !page_row_ok(a.pool, s, z) || z.length == 0) continue;
-            const float* const records = reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(pg_mem) + k_bytes + kPgTile * vp + 32) + i * pitch;
-            const size_t each = (k_bytes + kPgTile * vp + 32) / 4 + 4 * NT * pitch;
-            float m = -INFINITY, n = -INFINITY, sum = 0.0f, w[W];
+            const uint32_t each = buffer_bytes / 4;
+            const float* const records = reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(pg_mem) + k_bytes + kPgTile * vp + 32);
+            const float* const stats = records + NT * (8 * vp + 128) + 4 * i;
+            float m = -INFINITY, n = -INFINITY, w[W], x[W];
 #pragma unroll
-            for (uint32_t k = 0; k < W; k++) { m = fmaxf(m, records[k * each + vp]); n = fmaxf(n, records[k * each + vp + 1]); }
+            for (uint32_t k = 0; k < W; k++) { m = fmaxf(m, stats[k * each]); n = fmaxf(n, stats[k * each + 1]); }
 #pragma unroll
-            for (uint32_t k = 0; k < W; k++) {
-                sum = fmaf(records[k * each + vp + 2], pg_frame(records[k * each + vp], m), sum);
-                w[k] = pg_frame(records[k * each + vp + 1], n);
-            }
-            const float2 f = pg_finish(a, g * a.rep + h, m, n, sum);
+            for (uint32_t k = 0; k < W; k++) { x[k] = stats[k * each + 2]; w[k] = pg_frame(stats[k * each], m); }
+            const float2 f = pg_finish(a, g * a.rep + h, m, n, pg_tree(w, x));
+#pragma unroll
+            for (uint32_t k = 0; k < W; k++) w[k] = pg_frame(stats[k * each + 1], n);
             float* const to = a.dst + (size_t)row * a.dst_rs + (g * a.rep + h) * s.dv;
             for (uint32_t d = lane; d < s.dv; d += 32) {
-                float v = 0.0f;
 #pragma unroll
-                for (uint32_t k = 0; k < W; k++) v = fmaf(w[k], records[k * each + d], v);
-                to[d] = pg_scaled(v / f.y, f.x);
+                for (uint32_t k = 0; k < W; k++) x[k] = records[k * each + 2 * (32 * (2 * (i / 4 * vc + d / 16) + d / 8 % 2) + 4 * (d % 8) + i % 4)];
+                to[d] = pg_scaled(pg_tree(w, x) / f.y, f.x);
             }
         }
     }
@@ -540,7 +586,7 @@ __global__ void __launch_bounds__(32 * W, W == 1 ? pg_warps(KC, VC, NT) : 1) k_p
 // The records of a sequence that several warps took: a warp a query, or (SHARED) the four of a CTA, a quarter of the records each.  Bound by latency: eight records at a time, statistics
 // and outputs at once.
 template <bool SHARED>
-__global__ void __launch_bounds__(128) k_paged_join(const __grid_constant__ PgArgs a, const uint32_t queries) {
+__global__ void __launch_bounds__(128, 4) k_paged_join(const __grid_constant__ PgArgs a, const uint32_t queries) {
     pdl_enter();
     const PageShape& s = a.s;
     const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, r = blockIdx.y, query = SHARED ? blockIdx.x : 4 * blockIdx.x + warp, item = query / queries, i = query % queries, per_row = s.G * a.chunks;
@@ -567,9 +613,10 @@ __global__ void __launch_bounds__(128) k_paged_join(const __grid_constant__ PgAr
     if (!page_row_ok(a.pool, s, z) || z.length == 0) return;
     const uint32_t pitch = s.vp + 4;
     constexpr uint32_t kAtOnce = 8, kStep = SHARED ? 4 : 1;
-    float m = -INFINITY, n = -INFINITY, sum = 0.0f;
-    float4 v[2] = {make_float4(0.0f, 0.0f, 0.0f, 0.0f), make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
-    auto add = [](float4& to, float f, const float4& x) { to.x = fmaf(f, x.x, to.x); to.y = fmaf(f, x.y, to.y); to.z = fmaf(f, x.z, to.z); to.w = fmaf(f, x.w, to.w); };
+    float m = -INFINITY, n = -INFINITY;
+    float2 sum = make_float2(0.0f, 0.0f), v[8];                      // dims 128 (d / 4) + 4 lane + d % 4
+#pragma unroll
+    for (uint32_t d = 0; d < 8; d++) v[d] = make_float2(0.0f, 0.0f);
     for (uint32_t k0 = SHARED ? warp : 0; k0 < count; k0 += kAtOnce * kStep) {
         float4 st[kAtOnce], x[kAtOnce][2];
 #pragma unroll
@@ -582,42 +629,52 @@ __global__ void __launch_bounds__(128) k_paged_join(const __grid_constant__ PgAr
             if (4 * lane < s.vp) x[e][0] = *reinterpret_cast<const float4*>(from + 4 + 4 * lane);
             if (128 + 4 * lane < s.vp) x[e][1] = *reinterpret_cast<const float4*>(from + 132 + 4 * lane);
         }
-        float new_m = m, new_n = n;
+        float new_m = m, new_n = n, w[kAtOnce], parts[kAtOnce];
 #pragma unroll
         for (uint32_t e = 0; e < kAtOnce; e++) { new_m = fmaxf(new_m, st[e].x); new_n = fmaxf(new_n, st[e].y); }
+#pragma unroll
+        for (uint32_t e = 0; e < kAtOnce; e++) { w[e] = pg_frame(st[e].x, new_m); parts[e] = st[e].z; }
+        sum = pg_add(sum, pg_frame(m, new_m), pg_tree(w, parts));
         const float f = pg_frame(n, new_n);
-        sum *= pg_frame(m, new_m);
-        v[0].x *= f; v[0].y *= f; v[0].z *= f; v[0].w *= f; v[1].x *= f; v[1].y *= f; v[1].z *= f; v[1].w *= f;
         m = new_m; n = new_n;
 #pragma unroll
-        for (uint32_t e = 0; e < kAtOnce; e++) {
-            sum = fmaf(st[e].z, pg_frame(st[e].x, m), sum);
-            const float w = pg_frame(st[e].y, n);
-            add(v[0], w, x[e][0]); add(v[1], w, x[e][1]);
+        for (uint32_t e = 0; e < kAtOnce; e++) w[e] = pg_frame(st[e].y, n);
+#pragma unroll
+        for (uint32_t d = 0; d < 8; d++) {
+            if (d >= 4 && s.vp <= 128) break;
+#pragma unroll
+            for (uint32_t e = 0; e < kAtOnce; e++) { const float4 y = x[e][d / 4]; parts[e] = d % 4 == 0 ? y.x : d % 4 == 1 ? y.y : d % 4 == 2 ? y.z : y.w; }
+            v[d] = pg_add(v[d], f, pg_tree(w, parts));
         }
     }
     if constexpr (SHARED) {
         __shared__ float stats[4][3];
         __shared__ float4 parts[4][64];
-        if (lane == 0) { stats[warp][0] = m; stats[warp][1] = n; stats[warp][2] = sum; }
-        parts[warp][lane] = v[0]; parts[warp][32 + lane] = v[1];
+        if (lane == 0) { stats[warp][0] = m; stats[warp][1] = n; stats[warp][2] = sum.x; }
+        parts[warp][lane] = make_float4(v[0].x, v[1].x, v[2].x, v[3].x); parts[warp][32 + lane] = make_float4(v[4].x, v[5].x, v[6].x, v[7].x);
         __syncthreads();
         if (warp) return;
-        m = n = -INFINITY; sum = 0.0f;
-        for (uint32_t k = 0; k < 4; k++) { m = fmaxf(m, stats[k][0]); n = fmaxf(n, stats[k][1]); }
-        v[0] = v[1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (uint32_t k = 0; k < 4; k++) {
-            sum = fmaf(stats[k][2], pg_frame(stats[k][0], m), sum);
-            const float w = pg_frame(stats[k][1], n);
-            add(v[0], w, parts[k][lane]); add(v[1], w, parts[k][32 + lane]);
+        m = fmaxf(fmaxf(stats[0][0], stats[1][0]), fmaxf(stats[2][0], stats[3][0])); n = fmaxf(fmaxf(stats[0][1], stats[1][1]), fmaxf(stats[2][1], stats[3][1]));
+        float w[4] = {1.0f, 1.0f, 1.0f, 1.0f};
+        auto four = [&](float x0, float x1, float x2, float x3) { return fmaf(w[0], x0, w[1] * x1) + fmaf(w[2], x2, w[3] * x3); };
+#pragma unroll
+        for (uint32_t k = 0; k < 4; k++) w[k] = pg_frame(stats[k][0], m);
+        sum.x = four(stats[0][2], stats[1][2], stats[2][2], stats[3][2]);
+#pragma unroll
+        for (uint32_t k = 0; k < 4; k++) w[k] = pg_frame(stats[k][1], n);
+#pragma unroll
+        for (uint32_t q = 0; q < 2; q++) {
+            const float4 x0 = parts[0][32 * q + lane], x1 = parts[1][32 * q + lane], x2 = parts[2][32 * q + lane], x3 = parts[3][32 * q + lane];
+            v[4 * q].x = four(x0.x, x1.x, x2.x, x3.x); v[4 * q + 1].x = four(x0.y, x1.y, x2.y, x3.y);
+            v[4 * q + 2].x = four(x0.z, x1.z, x2.z, x3.z); v[4 * q + 3].x = four(x0.w, x1.w, x2.w, x3.w);
         }
     }
-    const float2 f = pg_finish(a, g * a.rep + h, m, n, sum);
+    const float2 f = pg_finish(a, g * a.rep + h, m, n, sum.x);
     float* const to = a.dst + (size_t)(r + token) * a.dst_rs + (g * a.rep + h) * s.dv;
 #pragma unroll
     for (uint32_t e = 0; e < 8; e++) {
         const uint32_t d = 128 * (e / 4) + 4 * lane + e % 4;
-        if (d < s.dv) to[d] = pg_scaled(reinterpret_cast<const float*>(&v[e / 4])[e % 4] / f.y, f.x);
+        if (d < s.dv) to[d] = pg_scaled(v[e].x / f.y, f.x);
     }
 }
 
@@ -625,8 +682,8 @@ __global__ void __launch_bounds__(128) k_paged_join(const __grid_constant__ PgAr
 size_t pg_plan_elems(uint32_t B) { return (kPgPlan + 2 * ((size_t)B + 1) + 3) / 4 * 4; }
 template <int KC, int VC, int NT, bool FULL, int W>
 bool pg_launch_as(const PgArgs& a, cudaStream_t st) {
-    const size_t smem = W * (kPgTile * (a.s.kp + a.s.vp) + 32 + sizeof(float) * 4 * NT * (a.s.vp + 4));
-    constexpr size_t most = W * (kPgTile * (32 * KC + 16 * VC) + 32 + sizeof(float) * 4 * NT * (16 * VC + 4));
+    const size_t smem = W * (kPgTile * (a.s.kp + a.s.vp) + 32 + sizeof(float) * pg_aside(NT, a.s.vp));
+    constexpr size_t most = W * (kPgTile * (32 * KC + 16 * VC) + 32 + sizeof(float) * pg_aside(NT, 16 * VC));
     if (!zg_smem_limit<k_paged<KC, VC, NT, FULL, W>>(most)) return false;
     launch_pdl(k_paged<KC, VC, NT, FULL, W>, dim3(W == 1 ? pg_warps(KC, VC, NT) * zg_sm_count() : a.B * a.s.G * a.chunks), dim3(32 * W), smem, st, a);
     return true;

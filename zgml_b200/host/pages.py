@@ -73,7 +73,8 @@ def page_moves(moves: Sequence[Tuple[int, int]], most: int, pages: int) -> np.nd
 
 class PagePool:
     """Which pages of a pool the slots' sequences have.  Sequences may share pages (fork); a page that several have is copied before one of them writes to it: `extend` and
-    `compact` return the copies as (source, destination) pairs, which have to run (PAGE_COPY, once per pool that the pages stand for) before the step that uses `table`."""
+    `compact` return the copies as (source, destination) pairs, which have to run (PAGE_COPY, once per pool that the pages stand for) before the step that uses `table`.  Lists of several calls
+    run one after the other, or together, in one PAGE_COPY, if each call was given the copies of those before it that had not run (`pending`): `moves += pool.extend(slot, 1, moves)`."""
 
     def __init__(self, pages: int, page_tokens: int, slots: int, most: int):
         if page_tokens not in PAGE_TOKENS or pages < 1 or slots < 1 or most < 1:
@@ -103,8 +104,9 @@ class PagePool:
             self._free.append(page)
             self._free.sort(reverse=True)
 
-    def extend(self, slot: int, tokens: int) -> List[Tuple[int, int]]:
-        """Room for `tokens` more positions of the slot's sequence; returns the copies to make first.  Where the pool has no room, RuntimeError, and nothing has changed."""
+    def extend(self, slot: int, tokens: int, pending: Sequence[Tuple[int, int]] = ()) -> List[Tuple[int, int]]:
+        """Room for `tokens` more positions of the slot's sequence; returns the copies to make first.  Where the pool has no room, or no page for a copy that those in `pending` leave alone (when they
+        have run there may be one), RuntimeError, and nothing has changed."""
         if tokens < 0:
             raise ValueError(f"{tokens} more positions")
         held, start, end = self._held[slot], self.lengths[slot], self.lengths[slot] + tokens
@@ -117,11 +119,18 @@ class PagePool:
         new = max(0, -(-end // self.page_tokens) - len(held))
         if len(shared) + new > len(self._free):
             raise RuntimeError(f"no free page for slot {slot}: {len(shared) + new} wanted, {len(self._free)} free")
+        touched, origin = {p for m in pending for p in m}, {d: s for s, d in pending}
+        copied = [n for n in shared if n * self.page_tokens < start]      # (only the page that holds positions already needs its bytes)
+        if copied and touched.issuperset(self._free):
+            raise RuntimeError(f"no free page for slot {slot} that the copies before do not touch")
         moves = []
-        for n in shared:                                             # (only the page that holds positions already needs its bytes)
-            page = self._free.pop()
-            if n * self.page_tokens < start:
-                moves.append((held[n], page))
+        for n in shared:
+            if n in copied:
+                page = next(p for p in reversed(self._free) if p not in touched)
+                self._free.remove(page)
+                moves.append((origin.get(held[n], held[n]), page))
+            else:
+                page = self._free.pop()
             self._users[held[n]] -= 1
             self._users[page], held[n] = 1, page
         for _ in range(new):
@@ -133,7 +142,7 @@ class PagePool:
         return moves
 
     def fork(self, slot: int, to: int, length: int = None):
-        """The free slot `to` begins as the first `length` positions (all) of slot's sequence, in the same pages."""
+        """The free slot `to` begins as the first `length` positions (all) of slot's sequence, in the same pages: positions that steps have written, since a copy runs before its step."""
         length = self.lengths[slot] if length is None else length
         if slot == to or self._held[to] or not 0 <= length <= self.lengths[slot]:
             raise ValueError(f"{length} positions of slot {slot}, which has {self.lengths[slot]}, to slot {to}")
@@ -157,16 +166,16 @@ class PagePool:
     def release(self, slot: int):
         self.shrink(slot, 0)
 
-    def compact(self) -> List[Tuple[int, int]]:
-        """Moves the pages in use to the lowest numbers; returns the copies to make before the next step."""
+    def compact(self, pending: Sequence[Tuple[int, int]] = ()) -> List[Tuple[int, int]]:
+        """Moves the pages in use to the lowest numbers, those aside that copies in `pending` touch; returns the copies to make before the next step."""
+        touched, origin = {p for m in pending for p in m}, {d: s for s, d in pending}
         live = [p for p in range(self.pages) if self._users[p]]
-        holes = [p for p in range(len(live)) if not self._users[p]]
-        moves = list(zip([p for p in live if p >= len(live)], holes))
-        to: Dict[int, int] = dict(moves)
-        for source, dst in moves:
+        holes = [p for p in range(len(live)) if not self._users[p] and p not in touched]
+        to: Dict[int, int] = dict(zip([p for p in live if p >= len(live)], holes))
+        for source, dst in to.items():
             self._users[dst], self._users[source] = self._users[source], 0
         for slot, held in enumerate(self._held):
             self._held[slot] = [to.get(p, p) for p in held]
             self._set(slot)
-        self._free = list(range(self.pages - 1, len(live) - 1, -1))
-        return moves
+        self._free = [p for p in range(self.pages - 1, -1, -1) if not self._users[p]]
+        return [(origin.get(source, source), dst) for source, dst in to.items()]

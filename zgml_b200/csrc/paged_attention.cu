@@ -24,9 +24,9 @@ struct PgArgs {
 constexpr uint32_t kPgTile = 32, kPgShift = 29, kPgFlush = 512;      // tiles (512 of 32 products of two bytes: below 2^31)
 constexpr float kPgCredit = 176.0f, kPgGrant = 3.0f;
 constexpr uint32_t kPgPlan = 8;                                     // words of the plan before the rows' tiles: all tiles (64 bits), warps, -, warps / tiles (64 bits)
-constexpr uint32_t kPgRows = 8, kPgLeast = 2;      // blocks of 32 rows that are read at once; tiles a warp at least where there are few (one sequence of 4096 tokens, us, with 1 / 2 / 4: 18.5 / 15.1 / 16.4)
+constexpr uint32_t kPgRows = 8, kPgLeast = 2;      // blocks of 32 rows that are read at once; tiles a warp at least where there are few (one sequence of 4096 tokens, us, with 1 / 2 / 4: 20.6 / 16.5 / 16.5)
 constexpr float kPgSlack = 3.0f;                                     // weights reach 2^(29 + 3)
-// Warps (CTAs) of an SM, by their registers: 168, 128 or 255 a thread.
+// Warps (CTAs) of an SM, by their registers: 16 of 128 a thread, 12 of 168, 8 of 255.
 constexpr uint32_t pg_warps(int KC, int VC, int NT) { return NT == 1 && KC <= 2 && VC <= 4 ? 16 : NT == 1 && KC <= 4 && VC <= 8 ? 12 : 8; }
 __device__ __forceinline__ float pg_sink(const PgArgs& a, uint32_t h) { return a.sink_bf16 ? __bfloat162float(reinterpret_cast<const bf16*>(a.sink)[h]) : reinterpret_cast<const float*>(a.sink)[h]; }
 // 2^d of a whole number d, 0 below 2^-126
@@ -105,7 +105,8 @@ __device__ __forceinline__ uint64_t pg_share(uint64_t all, uint32_t w, uint32_t 
 // warps have equal work whatever the sequences' lengths are, and none waits for another.  What it takes of a sequence begins or ends with it, or leaves a record for
 // k_paged_join: (m, n, sum, outputs) of each query.  (W = 8: a CTA of eight warps for each group and key head, whose records are joined in shared memory: one launch, for few short sequences
 // and where there is no workspace.)  A tile's next keys come while its weights and outputs are computed, its next values while the scores are.  4 NT queries at a time, query 4 t + lane % 4 a lane.
-// Bound by HBM in long caches (32 / 8 heads of 128, 16 rows of up to 65536 tokens: 201 us, 0.97 of the copy bandwidth; 64 of up to 4096: 61 us, 0.76, where the first and last tiles of a share count).
+// Bound by HBM in long caches (32 / 8 heads of 128, 16 rows of up to 65536 tokens, 1307 MB: 206 us for the launch by itself, 0.97 of the measured copy bandwidth).  64 rows of up to 4096, 305 MB, take 62 us, 0.75: those two
+// lie on a line of 7.0 TB/s (reads alone) and 18 us, which a warp's way to its first tile takes (table, page, copy, query, digits one after the other) and its changes of sequence and key head, with no copies under way.
 template <int KC, int VC, int NT, bool FULL, int W>
 __global__ void __launch_bounds__(32 * W, W == 1 ? pg_warps(KC, VC, NT) : 1) k_paged(const __grid_constant__ PgArgs a) {
     pdl_enter();
@@ -324,8 +325,8 @@ __global__ void __launch_bounds__(32 * W, W == 1 ? pg_warps(KC, VC, NT) : 1) k_p
         // same way by the thousand (in one frame for a sequence, outputs of 1.3e-4 came out as 2.4e-4 behind 65536 keys some 2^29 below the first).  So lanes pay for n: for each tile, in which a lane's four weights may
         // lose 2^-28 of 2^n together, 2^n is taken from its credit, and kPgCredit times what they weigh is added.  Where nothing is left, n becomes what the present tile asks for, and lanes in debt get
         // kPgGrant times the new 2^n: eight lanes at most 48 times the largest contribution of this tile.  Their debts, of at most 2^n each, are 16 times that of the tile that set n, or less.  So all that is
-        // taken is at most 176 + 48 + 16 times what all weights are, and what is lost 240 * 2^-28 of that, however many they are.  (64 rows of 64 / 8 heads of 128, up to 8192, scores of 0.7 to 2.6 powers of two: 163 us, with one frame
-        // and plain sums 152; 32 / 8 heads up to 4096 65.7 and 65.5; putting products away every 8 tiles 170.)
+        // taken is at most 176 + 48 + 16 times what all weights are, and what is lost 240 * 2^-28 of that, however many they are.  (64 rows of 64 / 8 heads of 128, up to 8192, us: 163, with one frame and plain
+        // sums 153, with products put away every 8 tiles 170; 32 / 8 heads up to 4096 66.1, 65.7 and 66.6.)
         float m[NT], n[NT], credit[NT], sum[NT];                     // credit in units of 2^n; sum: of four tiles, which then joins those before
         auto sums = [&](int t) { return aside + 64 * t; };
         auto kept = [&](int t) { return &aside[64 * t + 32].x; };    // the frame of the products that were put away
@@ -441,7 +442,7 @@ __global__ void __launch_bounds__(32 * W, W == 1 ? pg_warps(KC, VC, NT) : 1) k_p
 #pragma unroll
                     for (int k = 4; k < 32; k *= 2) { most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, k)); least_left = fminf(least_left, __shfl_xor_sync(0xffffffffu, least_left, k)); }
                     const float new_n = least_left < 0.0f ? ceilf(most) : fmaxf(n[t], ceilf(most));
-                    credit[t] = credit[t] >= 0.0f && n[t] > -INFINITY ? fminf(credit[t] * exp2f(fminf(n[t] - new_n, 60.0f)), 0x1p60f) : kPgGrant;
+                    credit[t] = credit[t] >= 0.0f && n[t] > -INFINITY ? fminf(credit[t] * pg_pow2(fminf(n[t] - new_n, 60.0f)), 0x1p60f) : kPgGrant;
                     sum[t] *= f; sums(t)->x *= f; sums(t)->y *= f;
                     m[t] = new_m; n[t] = new_n;
                 }
@@ -556,29 +557,31 @@ __global__ void __launch_bounds__(32 * W, W == 1 ? pg_warps(KC, VC, NT) : 1) k_p
     }
     if (gave_up && lane == 0) count_timeout();
     if constexpr (W > 1) {
+        static_assert(NT == 1 && W == 8);
         __syncthreads();
-        const uint32_t g = item / a.chunks, chunk = item % a.chunks;
-        for (uint32_t i = warp; i < group.rows * heads; i += W) {
-            const uint32_t h = chunk * heads + i % heads, row = r + i / heads;
-            const BatchRow z = batch_row(a.table, row);
-            if (h >= a.rep || !page_row_ok(a.pool, s, z) || z.length == 0) continue;
-            const uint32_t each = buffer_bytes / 4;
-            const float* const records = reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(pg_mem) + k_bytes + kPgTile * vp + 32);
-            const float* const stats = records + NT * (8 * vp + 128) + 4 * i;
-            float m = -INFINITY, n = -INFINITY, w[W], x[W];
+        const uint32_t g = item / a.chunks, h = item % a.chunks * heads + j % heads, row = r + j / heads;      // a lane's query and places are those that it had
+        if (j / heads >= group.rows || h >= a.rep) return;
+        const BatchRow z = batch_row(a.table, row);
+        if (!page_row_ok(a.pool, s, z) || z.length == 0) return;
+        const uint8_t* const records = reinterpret_cast<const uint8_t*>(pg_mem) + k_bytes + kPgTile * vp + 32;
+        float4 st[W];
+        float m = -INFINITY, n = -INFINITY, w[W], x[W];
 #pragma unroll
-            for (uint32_t k = 0; k < W; k++) { m = fmaxf(m, stats[k * each]); n = fmaxf(n, stats[k * each + 1]); }
+        for (uint32_t k = 0; k < W; k++) {
+            st[k] = reinterpret_cast<const float4*>(records + k * buffer_bytes)[2 * vp + 32 + j];
+            m = fmaxf(m, st[k].x); n = fmaxf(n, st[k].y);
+        }
 #pragma unroll
-            for (uint32_t k = 0; k < W; k++) { x[k] = stats[k * each + 2]; w[k] = pg_frame(stats[k * each], m); }
-            const float2 f = pg_finish(a, g * a.rep + h, m, n, pg_tree(w, x));
+        for (uint32_t k = 0; k < W; k++) { x[k] = st[k].z; w[k] = pg_frame(st[k].x, m); }
+        const float2 f = pg_finish(a, g * a.rep + h, m, n, pg_tree(w, x));
 #pragma unroll
-            for (uint32_t k = 0; k < W; k++) w[k] = pg_frame(stats[k * each + 1], n);
-            float* const to = a.dst + (size_t)row * a.dst_rs + (g * a.rep + h) * s.dv;
-            for (uint32_t d = lane; d < s.dv; d += 32) {
+        for (uint32_t k = 0; k < W; k++) w[k] = pg_frame(st[k].y, n);
+        float* const to = a.dst + (size_t)row * a.dst_rs + (g * a.rep + h) * s.dv;
+        for (uint32_t p = warp; p < 2 * vc; p += W) {
+            const uint32_t d = 8 * p + row8;
 #pragma unroll
-                for (uint32_t k = 0; k < W; k++) x[k] = records[k * each + 2 * (32 * (2 * (i / 4 * vc + d / 16) + d / 8 % 2) + 4 * (d % 8) + i % 4)];
-                to[d] = pg_scaled(pg_tree(w, x) / f.y, f.x);
-            }
+            for (uint32_t k = 0; k < W; k++) x[k] = reinterpret_cast<const float2*>(records + k * buffer_bytes)[32 * p + lane].x;
+            if (d < s.dv) to[d] = pg_scaled(pg_tree(w, x) / f.y, f.x);
         }
     }
 }
@@ -694,13 +697,13 @@ bool pg_launch(const PgArgs& a, cudaStream_t st) {
     return a.s.kp == 32 * KC && a.s.vp == 16 * VC ? pg_launch_as<KC, VC, NT, true, W>(a, st) : pg_launch_as<KC, VC, NT, false, W>(a, st);
 }
 // Queries that a warp takes together: four, of one row, or, where the step has more rows than the page table slots, of a slot's rows that follow one another; eight where a key head
-// has more than four and the caches are large, whose pages then come through L2 once for them (32 / 8 heads of 128 doubled, us, with four and with eight: 16 rows of up to 65536 tokens
-// 390 / 269, 64 rows of up to 4096 101 / 100; 64 rows of 32 / 2 heads of up to 4096 51 / 61, 9 x 7 rows of up to 2111 42 / 51).
+// has more than four and the caches are large, whose pages then come through L2 once for them (64 / 8 heads of 128, us, with four and with eight: 16 rows of up to 65536 tokens
+// 397 / 293, 32 of up to 16384 193 / 160, 64 of up to 8192 192 / 163, 64 of up to 4096 102 / 111; 64 rows of 32 / 2 heads of up to 4096 51 / 68, 9 x 7 rows of 16 / 2 heads of up to 2111 29 / 45).
 struct PgForm { bool narrow, wide, one; uint32_t queries, tokens; };      // one: one launch
-constexpr uint64_t kPgLarge = 1u << 21;
+constexpr uint64_t kPgLarge = 1u << 22;
 // One launch, a CTA of eight warps for each sequence and key head, where the longest sequence has, or its window shows, up to 1024 tokens and the CTAs make two waves at most (an SM holds one: its registers); else equal shares
-// and a second launch that joins them. One launch / two, us: 3 products of 64-dim heads, 64 tokens 6.2 / 10.3, 576 10.3 / 12.3, 2048 14.4 / 12.3; 128 dims, 32 products, 1024 tokens 12.3 / 16.4, 2048
-// 18.5 / 18.5; 128 products, 64 tokens 8.2 / 16.4, 4096 28.7 / 26.7; 256 products, 64 tokens 14.4 / 16.4, 1024 22.6 / 22.6, 2048 30.8 / 27.0; 512 products (four waves), 64 tokens 26.7 / 16.4.
+// and a second launch that joins them. One launch / two, us: 3 products of 64-dim heads, 64 tokens 8.3 / 10.3, 576 10.3 / 12.4, 2048 16.5 / 13.3; 128 dims, 32 products, 1024 tokens 14.4 / 16.9, 2048
+// 18.6 / 18.5; 128 products, 64 tokens 8.3 / 16.5, 4096 30.8 / 28.0; 256 products, 64 tokens 14.4 / 16.5, 1024 23.0 / 23.9, 2048 32.8 / 28.8; 512 products (four waves), 64 tokens 26.7 / 16.5.
 bool pg_one(uint64_t products, uint64_t seen) { return products <= 2ull * zg_sm_count() && seen <= 1024; }
 PgForm pg_form(const ZgSeqOp& op, uint32_t slots, bool scratch) {
     PgForm f;
@@ -758,7 +761,7 @@ bool zg_launch_paged_attention(const ZgOp& op, float* const* bufs, const size_t*
     ZG_SEQ_CHECK();
     if (!f.one) {
         // Four warps a query where few sequences and heads are shared out over all warps, so that each has a dozen records or more (32 / 8 heads of 128, us, four / one: one sequence of 4096
-        // tokens 15.1 / 26.7, of 65536 45.0 / 91.2, 16 of 4096 26.6 / 28.8; 64 of 4096 74.0 / 65.4, 256 of 1500 128 / 104).
+        // tokens 16.5 / 24.7, of 65536 48.9 / 79.3, 16 of 4096 28.5 / 30.8; 64 of 4096 74.9 / 65.4, 256 of 1500 128 / 103).
         const uint32_t products = a.s.G * a.chunks * f.queries;
         if ((uint64_t)a.B * a.s.G * a.chunks <= zg_sm_count()) launch_pdl(k_paged_join<true>, dim3(products, a.B), dim3(128), 0, st, a, f.queries);
         else launch_pdl(k_paged_join<false>, dim3((products + 3) / 4, a.B), dim3(128), 0, st, a, f.queries);

@@ -3,7 +3,7 @@ number of keys.
 
 The bound, in units of 2^-23 of the sum of weight * 127 * scale of the values over the sum of weights (the largest that a page of such scales can give): 8 for weights rounded to whole numbers (less than 2^-20 of what all
 weigh is lost), and roundings of half a unit each: of the outputs 4 where digits are joined, 3 where products are put away, 7 where warps' records are joined (by eights, these one after the other, four warps) and 1 of
-the quotient; of the softmax's sum 2 of a tile's four, 3 of four tiles, 2 of all, 3 of a warp's lanes, 7 of records.  Beside it the exponentials (2^-22 and the rounding of their argument: 0.7 * 2^-20 up to 32, where the
+the quotient; of the softmax's sum 2 of a tile's four, 2 of all tiles, 3 of a warp's lanes, 7 of records: 22.5, taken as 24.  Beside it the exponentials (2^-22 and the rounding of their argument: 0.7 * 2^-20 up to 32, where the
 largest weights are whole numbers, and more below them) and the scores' own roundings, weight by weight."""
 import numpy as np
 import pytest

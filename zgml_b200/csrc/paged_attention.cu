@@ -5,7 +5,7 @@
 // by 128: sum (c + 128) d - 128 sum d is exact too, and a bit of each code of a value is turned over.  Scales are powers of two: a key's joins its scores, a value's its weights.  A weight is 2^(s + e - n), with the score s in powers of
 // two, e the exponent of its value's scale and n a whole number that no s + e passes by more than 3, so that the largest contributions keep their bits whatever the pages' scales
 // are; the sum of the softmax has a frame m of its own, and the quotient is put right by the difference of the frames.  n falls again where weights have become small, before what they lose could add up to 2^-20 of
-// sum w (127 scale) / sum w.  When n changes, products join those before in a frame of their own, in two parts, and so does the softmax's sum every four tiles: nothing grows with a sequence's length.
+// sum w (127 scale) / sum w.  When n changes, products join those before in a frame of their own, in two parts, and the softmax's sum is kept in two: nothing grows with a sequence's length.
 #include "pages.cuh"
 #include "exp2.cuh"
 #include "split_tc.cuh"
@@ -53,8 +53,8 @@ __device__ __forceinline__ float pg_scaled(float x, float back) {
     const float half = truncf(back * 0.5f);
     return x * exp2f(half) * exp2f(back - half);
 }
-// floats of a warp behind its tile: outputs in two parts, four of a lane for each four queries, statistics of queries (W = 8)
-__host__ __device__ constexpr uint32_t pg_aside(uint32_t NT, uint32_t vp) { return NT * (8 * vp + 128 + 16); }
+// floats of a warp behind its tile: outputs in two parts, one of a lane for each four queries, statistics of queries (W = 8)
+__host__ __device__ constexpr uint32_t pg_aside(uint32_t NT, uint32_t vp) { return NT * (8 * vp + 32 + 16); }
 // What x brings joins f times a sum, f a power of two, kept as (sum, what its roundings added too much): W. Kahan, Communications of the ACM 8, 1965.  However many parts, two roundings of the sum of their magnitudes.
 __device__ __forceinline__ float2 pg_add(float2 sum, float f, float x) {
     const float y = fmaf(-sum.y, f, x), t = fmaf(sum.x, f, y);
@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(32 * W, W == 1 ? pg_warps(KC, VC, NT) : 1) k_p
     const uint32_t kp = FULL ? 32 * KC : s.kp, vp = FULL ? 16 * VC : s.vp, kc = kp / 32, vc = vp / 16, k_bytes = kPgTile * kp, buffer_bytes = k_bytes + kPgTile * vp + 32 + 4 * pg_aside(NT, vp);
     uint8_t* const buffer = reinterpret_cast<uint8_t*>(pg_mem) + warp * buffer_bytes;
     float2* const rec = reinterpret_cast<float2*>(buffer + k_bytes + kPgTile * vp + 32) + lane;      // a lane's outputs in two parts, 32 apart
-    float2* const aside = rec + 4 * NT * vp;                         // what a lane seldom needs
+    float* const aside = &rec[4 * NT * vp].x - lane;                 // what a lane seldom needs
     // rows that see nothing, or whose words are out of range
     auto settle = [&](uint32_t row) {
         const BatchRow z = batch_row(a.table, row);
@@ -326,18 +326,18 @@ __global__ void __launch_bounds__(32 * W, W == 1 ? pg_warps(KC, VC, NT) : 1) k_p
         // lose 2^-28 of 2^n together, 2^n is taken from its credit, and kPgCredit times what they weigh is added.  Where nothing is left, n becomes what the present tile asks for, and lanes in debt get
         // kPgGrant times the new 2^n: eight lanes at most 48 times the largest contribution of this tile.  Their debts, of at most 2^n each, are 16 times that of the tile that set n, or less.  So all that is
         // taken is at most 176 + 48 + 16 times what all weights are, and what is lost 240 * 2^-28 of that, however many they are.  (64 rows of 64 / 8 heads of 128, up to 8192, us: 163, with one frame and plain
-        // sums 153, with products put away every 8 tiles 170; 32 / 8 heads up to 4096 66.1, 65.7 and 66.6.)
-        float m[NT], n[NT], credit[NT], sum[NT];                     // credit in units of 2^n; sum: of four tiles, which then joins those before
-        auto sums = [&](int t) { return aside + 64 * t; };
-        auto kept = [&](int t) { return &aside[64 * t + 32].x; };    // the frame of the products that were put away
+        // sums 153, with products put away every 8 tiles 170; of 32 / 8 heads, up to 4096, 64.3 with either.)
+        float m[NT], n[NT], credit[NT];                              // credit in units of 2^n
+        float2 sum[NT];
+        auto kept = [&](int t) { return aside + 32 * t; };           // the frame of the products that were put away
         int o[NT][VC][2][4];                                         // even and odd digits: two of each
         uint32_t since = 0;                                          // tiles since the products were put away
         bool stored = false;
 #pragma unroll
         for (int t = 0; t < NT; t++) {
             m[t] = n[t] = *kept(t) = -INFINITY;
-            credit[t] = sum[t] = 0.0f;
-            *sums(t) = make_float2(0.0f, 0.0f);
+            credit[t] = 0.0f;
+            sum[t] = make_float2(0.0f, 0.0f);
 #pragma unroll
             for (int c = 0; c < VC; c++)
 #pragma unroll
@@ -443,15 +443,11 @@ __global__ void __launch_bounds__(32 * W, W == 1 ? pg_warps(KC, VC, NT) : 1) k_p
                     for (int k = 4; k < 32; k *= 2) { most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, k)); least_left = fminf(least_left, __shfl_xor_sync(0xffffffffu, least_left, k)); }
                     const float new_n = least_left < 0.0f ? ceilf(most) : fmaxf(n[t], ceilf(most));
                     credit[t] = credit[t] >= 0.0f && n[t] > -INFINITY ? fminf(credit[t] * pg_pow2(fminf(n[t] - new_n, 60.0f)), 0x1p60f) : kPgGrant;
-                    sum[t] *= f; sums(t)->x *= f; sums(t)->y *= f;
+                    sum[t].x *= f; sum[t].y *= f;
                     m[t] = new_m; n[t] = new_n;
                 }
             }
             since++;
-            if ((tile - t0) % 4 == 3) {
-#pragma unroll
-                for (int t = 0; t < NT; t++) { *sums(t) = pg_add(*sums(t), 1.0f, sum[t]); sum[t] = 0.0f; }
-            }
             uint32_t low_digits[NT][2], high_digits[NT][2];              // of each half's weights: digits 0 and 2, and 1 and 3, of four positions
 #pragma unroll
             for (int t = 0; t < NT; t++) {
@@ -473,7 +469,7 @@ __global__ void __launch_bounds__(32 * W, W == 1 ? pg_warps(KC, VC, NT) : 1) k_p
                     low_digits[t][u] = __byte_perm(turned[0], turned[1], 0x6420);
                     high_digits[t][u] = __byte_perm(turned[0], turned[1], 0x7531);
                 }
-                sum[t] += (weights[0] + weights[1]) + (mass - mass);      // (a scale that is not a number is one of the sum's too)
+                sum[t] = pg_add(sum[t], 1.0f, (weights[0] + weights[1]) + (mass - mass));      // (a scale that is not a number is one of the sum's too)
                 credit[t] = fmaf(mass, kPgCredit / (float)(1u << kPgShift), credit[t] - 1.0f);
             }
             __syncwarp();
@@ -498,10 +494,8 @@ __global__ void __launch_bounds__(32 * W, W == 1 ? pg_warps(KC, VC, NT) : 1) k_p
         }
         if (gave_up) {
 #pragma unroll
-            for (int t = 0; t < NT; t++) sum[t] = kBatchNaN;
+            for (int t = 0; t < NT; t++) sum[t].x = kBatchNaN;
         }
-#pragma unroll
-        for (int t = 0; t < NT; t++) sum[t] = pg_add(*sums(t), 1.0f, sum[t]).x;
         const bool whole = W == 1 && take == group.tiles;
         float* const record = whole || W > 1 ? nullptr : a.part + (size_t)(2 * blockIdx.x + (off ? 0 : 1)) * 4 * NT * (vp + 4);
 #pragma unroll
@@ -509,9 +503,9 @@ __global__ void __launch_bounds__(32 * W, W == 1 ? pg_warps(KC, VC, NT) : 1) k_p
             float top = m[t];
 #pragma unroll
             for (int k = 4; k < 32; k *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
-            sum[t] *= pg_frame(m[t], top);
+            float total = sum[t].x * pg_frame(m[t], top);
 #pragma unroll
-            for (int k = 4; k < 32; k *= 2) sum[t] += __shfl_xor_sync(0xffffffffu, sum[t], k);
+            for (int k = 4; k < 32; k *= 2) total += __shfl_xor_sync(0xffffffffu, total, k);
             const uint32_t i = 4 * t + j, token = i / heads, h = chunk * heads + i % heads;
             const bool on = token < group.rows && h < a.rep;
             const float frame = fmaxf(*kept(t), n[t]), before = pg_frame(*kept(t), frame), now = pg_frame(n[t], frame);
@@ -520,12 +514,12 @@ __global__ void __launch_bounds__(32 * W, W == 1 ? pg_warps(KC, VC, NT) : 1) k_p
             if (whole) {
                 const BatchRow z = batch_row(a.table, r + (on ? token : 0));
                 if (!on || !page_row_ok(a.pool, s, z) || z.length == 0) continue;      // (the latter two: settle)
-                f = pg_finish(a, g * a.rep + h, top, frame, sum[t]);
+                f = pg_finish(a, g * a.rep + h, top, frame, total);
                 to = a.dst + (size_t)(r + token) * a.dst_rs + (g * a.rep + h) * s.dv;
             } else {
-                float* const stats = W > 1 ? &aside[64 * NT + 2 * i].x - 2 * lane : record + i * (vp + 4);
+                float* const stats = W > 1 ? aside - lane + 32 * NT + 4 * i : record + i * (vp + 4);
                 to = stats + 4;
-                if (row8 == 0) *reinterpret_cast<float4*>(stats) = make_float4(top, frame, sum[t], 0.0f);
+                if (row8 == 0) *reinterpret_cast<float4*>(stats) = make_float4(top, frame, total, 0.0f);
             }
 #pragma unroll
             for (int c = 0; c < VC; c++) {
@@ -568,7 +562,7 @@ __global__ void __launch_bounds__(32 * W, W == 1 ? pg_warps(KC, VC, NT) : 1) k_p
         float m = -INFINITY, n = -INFINITY, w[W], x[W];
 #pragma unroll
         for (uint32_t k = 0; k < W; k++) {
-            st[k] = reinterpret_cast<const float4*>(records + k * buffer_bytes)[2 * vp + 32 + j];
+            st[k] = reinterpret_cast<const float4*>(records + k * buffer_bytes)[2 * vp + 8 + j];
             m = fmaxf(m, st[k].x); n = fmaxf(n, st[k].y);
         }
 #pragma unroll

@@ -105,8 +105,8 @@ __device__ __forceinline__ uint64_t pg_share(uint64_t all, uint32_t w, uint32_t 
 // warps have equal work whatever the sequences' lengths are, and none waits for another.  What it takes of a sequence begins or ends with it, or leaves a record for
 // k_paged_join: (m, n, sum, outputs) of each query.  (W = 8: a CTA of eight warps for each group and key head, whose records are joined in shared memory: one launch, for few short sequences
 // and where there is no workspace.)  A tile's next keys come while its weights and outputs are computed, its next values while the scores are.  4 NT queries at a time, query 4 t + lane % 4 a lane.
-// Bound by HBM in long caches (32 / 8 heads of 128, 16 rows of up to 65536 tokens, 1307 MB: 206 us for the launch by itself, 0.97 of the measured copy bandwidth).  64 rows of up to 4096, 305 MB, take 62 us, 0.75: those two
-// lie on a line of 7.0 TB/s (reads alone) and 18 us, which a warp's way to its first tile takes (table, page, copy, query, digits one after the other) and its changes of sequence and key head, with no copies under way.
+// Bound by HBM in long caches (32 / 8 heads of 128, 16 rows of up to 65536 tokens, 1307 MB: 202 us for the launch by itself, 6.5 TB/s).  64 rows of up to 4096, 305 MB, take 63 us, 4.9 TB/s: some 20 us of either are
+// a warp's way to its first tile (table, page, copy, query, digits one after the other) and its changes of sequence and key head, with no copies under way.
 template <int KC, int VC, int NT, bool FULL, int W>
 __global__ void __launch_bounds__(32 * W, W == 1 ? pg_warps(KC, VC, NT) : 1) k_paged(const __grid_constant__ PgArgs a) {
     pdl_enter();

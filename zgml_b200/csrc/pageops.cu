@@ -318,8 +318,9 @@ struct PrArgs {
     uint32_t B, dst_rs, k_col, v_col, vec;
 };
 constexpr uint32_t kPrThreads = 256, kPrRows = 16;
-// CTA (16 rows, key head): bound by its writes.  The rows' pages are found once.  Keys are read four codes at a time; values, of which a tile holds sixteen tokens side by side, a tile at a
-// time for all rows whose tokens it holds (byte by byte for each row 11.5 us instead of 10 for 2186 rows of 8 heads of 128: every byte came from a line of its own).
+// CTA (16 rows, key head): bound by latency, of the table, the page's id, its scale and its codes, one after the other for 16 KB of writes (2186 rows of 8 heads of 128: 12 us for the launch by itself, of which its
+// 18 MB of writes need 2.7).  The rows' pages are found once.  Keys are read four codes at a time; values, of which a tile holds sixteen tokens side by side, a tile at a
+// time for all rows whose tokens it holds (byte by byte for each row a step of append and read took 1.5 us more: every byte came from a line of its own).
 __global__ void __launch_bounds__(kPrThreads) k_page_read(const PrArgs a) {
     pdl_enter();
     __shared__ const uint8_t* parts[kPrRows];                        // null: zeros, or nothing (tokens: -1), or no numbers (-2)
@@ -399,7 +400,7 @@ __global__ void __launch_bounds__(kPrThreads) k_page_read(const PrArgs a) {
 
 // ── PAGE_COPY ────────────────────────────────────────────────────────────────────────────────────────────────────────
 constexpr uint32_t kPcThreads = 256, kPcVectors = 4;                 // vectors of 16 bytes a thread
-// CTA (move, share of the page): bound by the reads and writes, 6.5 TB/s of them where 4079 pages of 33 KB are moved (with one vector a thread 53.3 us, with four 47.1, with eight 49.2).  V: vectors of 16
+// CTA (move, share of the page): bound by the reads and writes: 268 MB, 4079 pages of 33 KB, in 40 us for the launch by itself, 6.7 TB/s (replays, us: one vector a thread 53.3, four 47.1, eight 49.2).  V: vectors of 16
 // bytes, or words where a page is no whole number of vectors.
 template <typename V>
 __global__ void __launch_bounds__(kPcThreads) k_page_copy(V* pages, const float* table, uint32_t B, uint32_t count, uint32_t vectors) {
